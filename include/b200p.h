@@ -621,6 +621,58 @@ int b200p_canon_conv(const float* n, const float* conv_w, const float* conv_stat
 int b200p_tanh_norm(const float* h, const float* alpha, const float* w, const float* b, void* x_out, int64_t M, int64_t W,
                     int dtype, void* stream);
 
+/* ---- paged key-value cache ----------------------------------------------------------------------------------------------
+ * Keys and values lie in pages, kpages / vpages `dtype` [P, G, page, D]: the slots of one page and key head are neighbours.  Slot s of
+ * row r is in page table[r, s / page] (table int32 [rows, width]) at s % page.  `page` is a multiple of 16, at most 4096; D a multiple of
+ * 8, at most 256; a row has at most 2^30 slots.  Pages are 16-byte aligned and contiguous.  The pages of one call may stand in the table in
+ * any order, rows may share pages (a common beginning), and the table may be wider than a row needs: entries behind a row's last page
+ * are not read.
+ * Tokens of a call come with three numbers each: t_row (their row; negative: an idle token, for which nothing is read or written but the
+ * re-zeroing of qkv_f32), t_slot (where they lie in the row) and, for the rotation, t_pos (their position in the text, which differs from the slot
+ * once tokens before them were evicted).
+ * An id outside [0, P) (and a row or slot outside the table) names no place: nothing is written there, keys there count as masked, and
+ * b200p_paged_fault_count counts the meeting.
+ * mass fp32 [P, G, page] (optional) is the attention weight that every cached token has received from later queries. */
+
+/* Step 1: qkv [M, >= (H + 2 G) D] = [q | k | v] (row stride ldq elements) in `dtype`, or (qkv_f32 = 1, 16-bit dtypes) the projection's fp32
+ * accumulation buffer: rounded to `dtype` on read and re-zeroed behind the read, as in b200p_rope_kv_append.  q and k are rms-normed per
+ * head with q_norm_w / k_norm_w (`dtype` [D], NULL: not normed), their pairs (i, i + n_rot) (pairs = 0) or (2i, 2i + 1) (pairs = 1), i < n_rot, turn
+ * by the angle t_pos * rates[i] (rates fp32 [n_rot]; the angle is formed in double precision) and they are rounded once.  q_out `dtype`
+ * [M, H D]; k and v go to their slots, whose mass becomes 0.  The tokens of one call lie at slots of their own. */
+int b200p_paged_append(void* qkv, int64_t ldq, void* q_out, void* kpages, void* vpages, float* mass, const int32_t* table,
+                       const int32_t* t_row, const int32_t* t_slot, const int32_t* t_pos, const void* q_norm_w, const void* k_norm_w,
+                       const float* rates, int n_rot, int pairs, float eps, int64_t M, int H, int G, int D, int64_t P, int page, int rows,
+                       int width, int dtype, int qkv_f32, void* stream);
+/* Step 2: attention of M tokens, each over its own row: token t at slot s sees the slots j < n = s + 1 with j < first or j >= n - window
+ * (window 0: every j < n); fp32 softmax of q . k_j * scale; query head h reads key head h / (H / G).  q `dtype` [M, H D]; out `dtype` [M, H D]
+ * (flags = B200P_OUT_PERM8: PERM8 order).  A token that sees nothing gets zeros.  mass (NULL: none): every visible slot's mass grows by
+ * the weights that the query heads of its key head gave it; slots that several tokens of one call see receive their sums in no fixed order.
+ * Hidden keys and values are not read.  workspace: b200p_paged_attn_workspace_bytes(M, H, D, keys), keys = width * page with a mass,
+ * 0 without; it needs no initial state and serves one stream at a time. */
+int b200p_paged_attn(const void* q, const void* kpages, const void* vpages, float* mass, const int32_t* table, const int32_t* t_row,
+                     const int32_t* t_slot, void* out, int64_t M, int H, int G, int D, int64_t P, int page, int rows, int width, float scale,
+                     int64_t first, int64_t window, int dtype, int flags, void* workspace, size_t workspace_bytes, void* stream);
+size_t b200p_paged_attn_workspace_bytes(int64_t M, int H, int D, int64_t keys);
+/* Eviction, step 1: kept int32 [rows, G, keep] = the slots that row r's key head g keeps, ascending.  A row with lengths[r] > keep keeps its
+ * `first` first and `recent` last slots and of those between the keep - first - recent with the largest mass (ties: the lowest slots; NaN and slots
+ * without a page count as less than every number); other rows keep all, -1 behind their last. */
+int b200p_paged_select(const float* mass, const int32_t* table, const int32_t* lengths, int32_t* kept, int64_t P, int G, int page, int rows,
+                       int width, int keep, int first, int recent, void* stream);
+/* step 2: slot i of row r and key head g takes what slot kept[r, g, i] holds (keys, values and, unless NULL, mass), for ascending kept slots,
+ * in place; a row then has min(lengths[r], keep) tokens, which the caller notes, and its pages behind those are free.  Rows that are cut share no
+ * pages that change. */
+int b200p_paged_compact(void* kpages, void* vpages, float* mass, const int32_t* table, const int32_t* lengths, const int32_t* kept, int64_t P,
+                        int G, int D, int page, int rows, int width, int keep, int dtype, void* stream);
+/* Dense view: slots j < min(lengths[r] + extra, Tcap) of row r = row_of[i] go to kcache / vcache `dtype` [count, G, Tcap, D] at [i, :, j]
+ * (row_of[i] < 0: nothing); what lies behind stays as it was.  Prompt attention (b200p_attn) then reads them: append the portion, gather
+ * with extra = its tokens. */
+int b200p_paged_gather(const void* kpages, const void* vpages, const int32_t* table, const int32_t* row_of, const int32_t* lengths,
+                       void* kcache, void* vcache, int extra, int64_t count, int G, int D, int64_t P, int page, int rows, int width,
+                       int64_t Tcap, int dtype, void* stream);
+/* *count = how often a call on the current device met a row, slot or page id that names no place since the last reset; reset != 0 clears it.
+ * Synchronises `stream`; not capturable. */
+int b200p_paged_fault_count(unsigned int* count, int reset, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -138,6 +138,16 @@ SIGNATURES = {
                               _i32, _vp, _sz, _vp]),
     "b200p_mix_attn_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "b200p_mix_attn_tiles_supported": (_i32, [_i32, _i32, _i32, _i32, _i32]),
+    # paged key-value cache
+    "b200p_paged_append": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _i64, _i32, _i32, _i32,
+                                  _i64, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "b200p_paged_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _i64, _i64, _i32,
+                                _i32, _vp, _sz, _vp]),
+    "b200p_paged_attn_workspace_bytes": (_sz, [_i64, _i32, _i32, _i64]),
+    "b200p_paged_select": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "b200p_paged_compact": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "b200p_paged_gather": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _i32, _i64, _i32, _vp]),
+    "b200p_paged_fault_count": (_i32, [C.POINTER(C.c_uint), _i32, _vp]),
 }
 
 # Translation units a model family needs (csrc/*.cu): the library can be linked from a subset, so that a fresh checkout

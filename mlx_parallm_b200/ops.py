@@ -767,3 +767,141 @@ def mix_attn(q, kcache, vcache, t_row, t_pos, talk, sink, out, H, G, dk, dv, win
         int(window), _p(out), out.stride(0), M, H, G, dk, dv, dtype_code(kcache.dtype), _p(workspace),
         0 if workspace is None else workspace.numel() * 4, _stream()))
     return out
+
+
+# ---- paged key-value cache ---------------------------------------------------------------------------------------------
+# Tensors of every call: kpages / vpages [P, G, page, D] in the model's storage type, table int32 [rows, width] of page ids, mass fp32
+# [P, G, page] or None, and per token int32 t_row (negative: idle), t_slot, t_pos (include/b200p.h).
+def _refuse(what: str):
+    raise ValueError(what)
+
+
+def _here(*ts):
+    for t in ts:
+        if t is not None and not (t.is_cuda and t.is_contiguous() and (_device_index is None or t.get_device() == _device_index())):
+            _dev(t)
+            _refuse("tensors of a paged cache are contiguous and lie on the current device")
+
+
+def _paged(kpages, vpages, table, mass, *others):
+    """Checks of the tensors every call shares -> (P, G, page, D, rows, width)."""
+    _here(kpages, vpages, table, mass, *others)
+    if kpages.dim() != 4 or vpages.shape != kpages.shape or vpages.dtype != kpages.dtype:
+        _refuse(f"pages are [P, key heads, page, D] and alike for keys and values: got {tuple(kpages.shape)} and {tuple(vpages.shape)}")
+    if table.dtype != torch.int32 or table.dim() != 2:
+        _refuse("the page table is int32 [rows, width]")
+    if mass is not None and (mass.dtype != torch.float32 or mass.shape != kpages.shape[:3]):
+        _refuse(f"mass is float32 [P, key heads, page]: got {mass.dtype} {tuple(mass.shape)}")
+    return (*kpages.shape, *table.shape)
+
+
+def _kept(kept, lengths, rows: int, G: int):
+    if lengths.dtype != torch.int32 or lengths.numel() != rows or kept.dtype != torch.int32 or kept.dim() != 3 or kept.shape[:2] != (rows, G):
+        _refuse(f"lengths int32 [{rows}], kept int32 [{rows}, {G}, keep]: got {tuple(lengths.shape)} and {tuple(kept.shape)}")
+
+
+def _tokens(M: int, *ts):
+    for t in ts:
+        if t.dtype != torch.int32 or t.numel() != M:
+            _refuse(f"rows, slots and positions are int32, one for each of the {M} tokens")
+
+
+def paged_append(qkv, q_out, kpages, vpages, table, t_row, t_slot, t_pos, H: int, rates=None, pairs: int = 0, q_norm_w=None, k_norm_w=None,
+                 eps: float = 1e-6, mass=None):
+    """Norms of queries and keys per head, rotation by ``t_pos * rates`` (fp32 [n_rot]; pairs (i, i + n_rot), or (2i, 2i + 1) with ``pairs`` 1),
+    queries to ``q_out`` [M, H D], keys and values to the slots ``t_slot`` of rows ``t_row``, whose mass becomes 0 (b200p_paged_append).
+    ``qkv`` [M, >= (H + 2 G) D] (a column slice is fine) in the pages' dtype, or float32 for 16-bit pages: an accumulation buffer, re-zeroed."""
+    P, G, page, D, rows, width = _paged(kpages, vpages, table, mass, q_out, t_row, t_slot, t_pos, rates, q_norm_w, k_norm_w)
+    M = qkv.shape[0]
+    dt = kpages.dtype
+    if not qkv.is_cuda or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < (H + 2 * G) * D or (qkv.dtype != dt and qkv.dtype != torch.float32) \
+            or (M > 1 and qkv.stride(0) < qkv.shape[1]) or (_device_index is not None and qkv.get_device() != _device_index()):
+        _dev(qkv)
+        _refuse(f"qkv is [M, >= {(H + 2 * G) * D}] in the pages' dtype or float32: got {tuple(qkv.shape)} {qkv.dtype}")
+    if q_out.dtype != dt or q_out.numel() != M * H * D:
+        _refuse(f"q_out is [M, {H * D}] in the pages' dtype")
+    _tokens(M, t_row, t_slot, t_pos)
+    if rates is not None and (rates.dtype != torch.float32 or 2 * rates.numel() > D):
+        _refuse("rates are float32, one per rotated pair")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.dtype != dt or w.numel() != D):
+            _refuse(f"norm weights are [{D}] in the pages' dtype")
+    _call("b200p_paged_append", lambda: lib().b200p_paged_append(
+        qkv.data_ptr(), qkv.stride(0) if M > 1 else qkv.shape[1], q_out.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _p(mass), table.data_ptr(),
+        t_row.data_ptr(), t_slot.data_ptr(), t_pos.data_ptr(), _p(q_norm_w), _p(k_norm_w), _p(rates), 0 if rates is None else rates.numel(), int(pairs),
+        float(eps), M, int(H), G, D, P, page, rows, width, dtype_code(dt), 1 if qkv.dtype != dt else 0, _stream()))
+    return q_out
+
+
+def paged_attn_workspace_bytes(M: int, H: int, D: int, keys: int = 0) -> int:
+    """``keys``: the table's width * page where a mass is added up, else 0."""
+    return int(lib().b200p_paged_attn_workspace_bytes(int(M), int(H), int(D), int(keys)))
+
+
+def paged_attn(q, kpages, vpages, table, t_row, t_slot, out, scale: float, first: int = 0, window: int = 0, mass=None, workspace=None,
+               out_perm: bool = False):
+    """Attention of single tokens, each over the slots up to its own of its row; with ``window`` only the last ``window`` of them and the ``first``
+    first; ``mass`` grows by the weights every slot receives (b200p_paged_attn).  ``q``, ``out`` [M, H D] in the pages' dtype."""
+    P, G, page, D, rows, width = _paged(kpages, vpages, table, mass, q, out, t_row, t_slot, workspace)
+    M = t_row.numel()
+    H = q.numel() // (M * D) if M else G
+    if q.dtype != kpages.dtype or out.dtype != kpages.dtype or q.numel() != M * H * D or out.numel() != M * H * D:
+        _refuse(f"q and out are [{M}, heads * {D}] in the pages' dtype: got {tuple(q.shape)} and {tuple(out.shape)}")
+    _tokens(M, t_row, t_slot)
+    ws_ptr, ws_bytes = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _call("b200p_paged_attn", lambda: lib().b200p_paged_attn(
+        q.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _p(mass), table.data_ptr(), t_row.data_ptr(), t_slot.data_ptr(), out.data_ptr(), M, H, G, D, P,
+        page, rows, width, float(scale), int(first), int(window), dtype_code(q.dtype), _lib.OUT_PERM8 if out_perm else 0, ws_ptr, ws_bytes, _stream()))
+    return out
+
+
+def paged_select(mass, table, lengths, kept, first: int = 0, recent: int = 0):
+    """``kept`` int32 [rows, G, keep]: which slots every row's key heads keep when the row is cut to ``keep`` tokens (b200p_paged_select)."""
+    _here(mass, table, lengths, kept)
+    if mass.dim() != 3 or mass.dtype != torch.float32 or table.dtype != torch.int32 or table.dim() != 2:
+        _refuse("mass is float32 [P, key heads, page], the page table int32 [rows, width]")
+    (P, G, page), (rows, width) = mass.shape, table.shape
+    _kept(kept, lengths, rows, G)
+    _call("b200p_paged_select", lambda: lib().b200p_paged_select(
+        mass.data_ptr(), table.data_ptr(), lengths.data_ptr(), kept.data_ptr(), P, G, page, rows, width, kept.shape[2], int(first), int(recent), _stream()))
+    return kept
+
+
+def paged_compact(kpages, vpages, table, lengths, kept, mass=None):
+    """Close the ``kept`` slots (ascending, -1 behind the last) of every row and key head up to its first ones, in place (b200p_paged_compact)."""
+    P, G, page, D, rows, width = _paged(kpages, vpages, table, mass, lengths, kept)
+    _kept(kept, lengths, rows, G)
+    _call("b200p_paged_compact", lambda: lib().b200p_paged_compact(
+        kpages.data_ptr(), vpages.data_ptr(), _p(mass), table.data_ptr(), lengths.data_ptr(), kept.data_ptr(), P, G, D, page, rows, width, kept.shape[2],
+        dtype_code(kpages.dtype), _stream()))
+
+
+def paged_evict(kpages, vpages, mass, table, lengths, kept, first: int = 0, recent: int = 0):
+    """Cut every row that holds more than ``keep = kept.shape[2]`` tokens to its ``first`` first, its ``recent`` last and the most attended ones
+    between, closed up in place; afterwards a row holds min(lengths, keep) tokens (``lengths`` is the caller's to change)."""
+    paged_select(mass, table, lengths, kept, first, recent)
+    paged_compact(kpages, vpages, table, lengths, kept, mass)
+    return kept
+
+
+def paged_gather(kpages, vpages, table, rows, lengths, kcache, vcache, extra: int = 0):
+    """Dense caches [n, G, Tcap, D] of the rows ``rows`` (int32 [n]): slots below lengths + ``extra``, what lies behind untouched."""
+    P, G, page, D, R, width = _paged(kpages, vpages, table, None, rows, lengths, kcache, vcache)
+    n = rows.numel()
+    if rows.dtype != torch.int32 or lengths.dtype != torch.int32 or lengths.numel() != R:
+        _refuse(f"rows int32 [n], lengths int32 [{R}]")
+    if kcache.dim() != 4 or kcache.shape[0] != n or kcache.shape[1] != G or kcache.shape[3] != D or vcache.shape != kcache.shape \
+            or kcache.dtype != kpages.dtype or vcache.dtype != kpages.dtype:
+        _refuse(f"dense caches are [{n}, {G}, Tcap, {D}] in the pages' dtype: got {tuple(kcache.shape)} and {tuple(vcache.shape)}")
+    _call("b200p_paged_gather", lambda: lib().b200p_paged_gather(
+        kpages.data_ptr(), vpages.data_ptr(), table.data_ptr(), rows.data_ptr(), lengths.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), int(extra), n, G, D,
+        P, page, R, width, kcache.shape[2], dtype_code(kpages.dtype), _stream()))
+
+
+def paged_fault_count(reset: bool = False) -> int:
+    """How often a paged call on the current device met a row, slot or page id that names no place since the last reset.  Synchronises the
+    current stream: call it at generation boundaries, never under graph capture."""
+    import ctypes as C
+    n = C.c_uint(0)
+    _lib.check(lib().b200p_paged_fault_count(C.byref(n), 1 if reset else 0, _stream()), "b200p_paged_fault_count")
+    return int(n.value)

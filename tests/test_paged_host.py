@@ -1,0 +1,143 @@
+"""Argument checks of the paged-cache entry points (no device: every refusal comes before a launch), the tile arithmetic of the window, and the
+oracle of the GPU tests against itself."""
+import math
+
+import pytest
+import torch
+
+import paged_oracle as po
+from mlx_parallm_b200 import _lib
+
+OK = 1 << 20           # an aligned address that a refused call never touches
+ARG, ALIGN = -1, -2
+
+
+def L():
+    return _lib.lib()
+
+
+def append(**kw):
+    a = dict(qkv=OK, ldq=12 * 64, q=OK, k=OK, v=OK, mass=0, table=OK, row=OK, slot=OK, pos=OK, qw=0, kw=0, rates=OK, n=32, pairs=0, eps=1e-6, M=2, H=8,
+             G=2, D=64, P=9, page=16, rows=2, width=4, dtype=_lib.BF16, f32=0)
+    a.update(kw)
+    return L().b200p_paged_append(a["qkv"], a["ldq"], a["q"], a["k"], a["v"], a["mass"], a["table"], a["row"], a["slot"], a["pos"], a["qw"], a["kw"],
+                                  a["rates"], a["n"], a["pairs"], a["eps"], a["M"], a["H"], a["G"], a["D"], a["P"], a["page"], a["rows"], a["width"],
+                                  a["dtype"], a["f32"], 0)
+
+
+def attn(**kw):
+    a = dict(q=OK, k=OK, v=OK, mass=0, table=OK, row=OK, slot=OK, out=OK, M=2, H=8, G=2, D=64, P=9, page=16, rows=2, width=4, scale=1.0, first=0, window=0,
+             dtype=_lib.BF16, flags=0, ws=OK, bytes=1 << 30)
+    a.update(kw)
+    return L().b200p_paged_attn(a["q"], a["k"], a["v"], a["mass"], a["table"], a["row"], a["slot"], a["out"], a["M"], a["H"], a["G"], a["D"], a["P"],
+                                a["page"], a["rows"], a["width"], a["scale"], a["first"], a["window"], a["dtype"], a["flags"], a["ws"], a["bytes"], 0)
+
+
+def select(**kw):
+    a = dict(mass=OK, table=OK, lengths=OK, kept=OK, P=9, G=2, page=16, rows=2, width=4, keep=20, first=4, recent=8)
+    a.update(kw)
+    return L().b200p_paged_select(*[a[x] for x in ("mass", "table", "lengths", "kept", "P", "G", "page", "rows", "width", "keep", "first", "recent")], 0)
+
+
+def compact(**kw):
+    a = dict(k=OK, v=OK, mass=0, table=OK, lengths=OK, kept=OK, P=9, G=2, D=64, page=16, rows=2, width=4, keep=20, dtype=_lib.F16)
+    a.update(kw)
+    return L().b200p_paged_compact(*[a[x] for x in ("k", "v", "mass", "table", "lengths", "kept", "P", "G", "D", "page", "rows", "width", "keep", "dtype")], 0)
+
+
+def gather(**kw):
+    a = dict(k=OK, v=OK, table=OK, row_of=OK, lengths=OK, kc=OK, vc=OK, extra=0, count=2, G=2, D=64, P=9, page=16, rows=2, width=4, cap=64, dtype=_lib.F32)
+    a.update(kw)
+    return L().b200p_paged_gather(*[a[x] for x in ("k", "v", "table", "row_of", "lengths", "kc", "vc", "extra", "count", "G", "D", "P", "page", "rows", "width",
+                                                   "cap", "dtype")], 0)
+
+
+PAGES = [dict(page=8), dict(page=24), dict(page=0), dict(page=8192), dict(P=0), dict(P=1 << 31), dict(rows=0), dict(width=0), dict(width=1 << 27), dict(G=0),
+         dict(table=0)]
+
+
+@pytest.mark.parametrize("call", [append, attn, select, compact, gather])
+@pytest.mark.parametrize("bad", PAGES, ids=str)
+def test_pages_that_are_refused(call, bad):
+    assert call(**bad) == ARG and _lib.last_error()
+
+
+@pytest.mark.parametrize("call,bad,rc", [
+    (append, dict(D=60), ARG), (append, dict(D=264), ARG), (append, dict(dtype=3), ARG), (append, dict(H=7), ARG), (append, dict(qkv=0), ARG),
+    (append, dict(q=0), ARG), (append, dict(row=0), ARG), (append, dict(slot=0), ARG), (append, dict(pos=0), ARG), (append, dict(rates=0), ARG),
+    (append, dict(n=33), ARG), (append, dict(n=-1), ARG), (append, dict(pairs=2), ARG), (append, dict(ldq=12 * 64 - 1), ARG), (append, dict(M=-1), ARG),
+    (append, dict(f32=1, dtype=_lib.F32), ARG), (append, dict(k=OK + 8), ALIGN), (append, dict(v=OK + 2), ALIGN),
+    (attn, dict(D=60), ARG), (attn, dict(D=0), ARG), (attn, dict(D=512), ARG), (attn, dict(dtype=-1), ARG), (attn, dict(H=9), ARG), (attn, dict(H=0), ARG),
+    (attn, dict(q=0), ARG), (attn, dict(out=0), ARG), (attn, dict(k=0), ARG), (attn, dict(row=0), ARG), (attn, dict(slot=0), ARG), (attn, dict(M=-1), ARG),
+    (attn, dict(M=65536), ARG), (attn, dict(first=-1), ARG), (attn, dict(window=-1), ARG), (attn, dict(flags=2), ARG), (attn, dict(q=OK + 2), ALIGN),
+    (attn, dict(out=OK + 2), ALIGN), (attn, dict(k=OK + 2), ALIGN), (attn, dict(mass=OK, ws=0), ARG), (attn, dict(mass=OK, bytes=100), ARG),
+    (select, dict(mass=0), ARG), (select, dict(lengths=0), ARG), (select, dict(kept=0), ARG), (select, dict(keep=0), ARG), (select, dict(first=-1), ARG),
+    (select, dict(recent=-1), ARG), (select, dict(first=13), ARG), (select, dict(first=(1 << 31) - 1, recent=(1 << 31) - 1), ARG), (select, dict(rows=65536), ARG),
+    (compact, dict(k=0), ARG), (compact, dict(kept=0), ARG), (compact, dict(keep=0), ARG), (compact, dict(dtype=7), ARG), (compact, dict(v=OK + 8), ALIGN),
+    (gather, dict(row_of=0), ARG), (gather, dict(kc=0), ARG), (gather, dict(cap=0), ARG), (gather, dict(count=-1), ARG), (gather, dict(vc=OK + 4), ALIGN),
+], ids=lambda x: getattr(x, "__name__", str(x)))
+def test_arguments_that_are_refused(call, bad, rc):
+    assert call(**bad) == rc and _lib.last_error()
+
+
+def test_nothing_to_do_needs_no_device():
+    assert append(M=0) == 0 and attn(M=0) == 0 and gather(count=0) == 0
+
+
+def test_workspace_grows_with_the_weights_only():
+    f = L().b200p_paged_attn_workspace_bytes
+    assert f(0, 8, 64, 0) == 0 and f(2, 8, 64, 1000) >= 4 * 2 * 8 * 1000 + f(2, 8, 64, 0)
+
+
+def test_ops_refuse_cpu_tensors():
+    from mlx_parallm_b200 import ops
+    k = torch.zeros((2, 1, 16, 8))
+    i = torch.zeros(1, dtype=torch.int32)
+    t = torch.zeros((1, 1), dtype=torch.int32)
+    with pytest.raises(_lib.B200PError):
+        ops.paged_attn(torch.zeros((1, 8)), k, k, t, i, i, torch.zeros((1, 8)), 1.0)
+    with pytest.raises(_lib.B200PError):
+        ops.paged_append(torch.zeros((1, 24)), torch.zeros((1, 8)), k, k, t, i, i, i, 1)
+    with pytest.raises(_lib.B200PError):
+        ops.paged_evict(k, k, torch.zeros((2, 1, 16)), t, i, torch.zeros((1, 1, 4), dtype=torch.int32))
+    with pytest.raises(_lib.B200PError):
+        ops.paged_gather(k, k, t, i, i, k, k)
+
+
+# ---------------------------------------------------------------- the oracle
+def test_oracle_of_the_attention_is_a_softmax_over_the_visible_slots():
+    g = torch.Generator().manual_seed(1)
+    k, v = torch.randn((3, 1, 16, 8), generator=g), torch.randn((3, 1, 16, 8), generator=g)
+    mass = torch.zeros((3, 1, 16))
+    table = torch.tensor([[2, 0]], dtype=torch.int32)
+    q = torch.randn((1, 16), generator=g)
+    out, tol, new, off = po.attn(q, k, v, mass, table, torch.tensor([0]), torch.tensor([19]), 2, 0.5, 2, 5, 0.0)
+    keys, values = torch.cat([k[2], k[0]], 1)[0].double(), torch.cat([v[2], v[0]], 1)[0].double()
+    seen = [0, 1, 15, 16, 17, 18, 19]
+    assert po.visible(20, 2, 5) == seen
+    for h in range(2):
+        s = q[0, 8 * h:8 * h + 8].double() @ keys[seen].T * 0.5
+        assert torch.allclose(out[0, h], torch.softmax(s, -1) @ values[seen], atol=1e-12)
+    assert abs(float(new.sum()) - 2) < 1e-12 and float(new[1].abs().max()) == 0.0
+    assert float(new[2, 0, 2:15].abs().max()) == 0.0 and float(new[0, 0, 4:].abs().max()) == 0.0
+
+
+def test_oracle_of_the_eviction():
+    mass = torch.tensor([[[5.0, 1, 1, math.nan, 0, 3, 1, 1, 0, 9, 9, 9, 9, 9, 9, 9]]])
+    kept = po.select(mass, torch.zeros((1, 1), dtype=torch.int32), torch.tensor([10]), 5, 1, 1)
+    assert kept[0, 0].tolist() == [0, 1, 2, 5, 9]
+    k = torch.arange(16.0).reshape(1, 1, 16, 1)
+    new, _, m = po.compact(k, k, mass, torch.zeros((1, 1), dtype=torch.int32), torch.tensor([10]), kept)
+    assert new.flatten()[:6].tolist() == [0, 1, 2, 5, 9, 5] and m.flatten()[:5].tolist() == [5, 1, 1, 3, 9]
+
+
+def test_oracle_of_the_append_turns_pairs():
+    k = torch.zeros((1, 1, 16, 8))
+    qkv = torch.zeros((1, 24))
+    qkv[0, 0], qkv[0, 8 + 1] = 1.0, 1.0
+    i = torch.tensor([0])
+    rates = torch.tensor([1.0, 0.5])
+    for pairs in (0, 1):
+        q, kk, _, _, _ = po.append(qkv, k, k, None, torch.zeros((1, 1), dtype=torch.int32), i, i + 3, i + 2, 1, rates, pairs, None, None, 0.0)
+        assert abs(float(q[0, 0, 0]) - math.cos(2.0)) < 1e-12 and abs(float(q[0, 0, 2 if pairs == 0 else 1]) - math.sin(2.0)) < 1e-12
+        assert abs(float(kk[0, 0, 3, 1]) - math.cos(1.0 if pairs == 0 else 2.0)) < 1e-12
