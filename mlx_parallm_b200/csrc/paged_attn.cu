@@ -7,6 +7,8 @@
 // Scores, their maximum and sum, the outputs and the weights are fp32 throughout; the output is rounded once.
 #include <stdlib.h>
 
+#include <atomic>
+
 #include "mma_util.cuh"
 #include "paged.cuh"
 
@@ -48,175 +50,595 @@ struct Span {
 struct PagedAttn {
   const void *q, *k, *v;
   void* out;
-  float *mass, *ws;
+  float* mass;
   PageTable pt;
   const int32_t *t_row, *t_slot;
-  int H, G, D, first, window, cap, out_perm;      // cap: visible slots a token can have, in whole tiles
+  int M, H, G, D, first, window, out_perm;
   float scale_log2e;
+  // workspace
+  int64_t* base;       // [M + 1] units before every token; all units
+  float* stat;         // [M, H, 2] maximum and sum of the heads that one CTA took whole (with a mass)
+  float* rec;          // [CTAs, 2, rows of a block, D + 4] parts: maximum, sum, -, -, outputs
+  float* scores;       // [M, H, cap] log2-scaled scores (with a mass)
+  int cap;             // visible slots a token can have, in whole tiles
 };
 
-// ------------------------------------------------------------------------------------------------ any type and size
-// One CTA per (block of 8 query heads of a key head, token); its warps take the tiles in turn.  A warp stages a tile of keys and values in
-// shared memory (rows padded to an odd number of 16-byte pieces); two lanes share a key for the scores, for the outputs a lane owns 4 (D
-// > 128: 8) dimensions of every head.
-constexpr int PG_WARPS = 4, PG_ROWS = 8;
-
-template <typename T, int NG>
-__global__ void __launch_bounds__(PG_WARPS * 32)
-paged_attn_any_kernel(const PagedAttn a) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = a.H / a.G, blocks = (per + PG_ROWS - 1) / PG_ROWS;
-  const int g = blockIdx.x / blocks, r0 = (blockIdx.x % blocks) * PG_ROWS, t = blockIdx.y;
-  const int rows = min(PG_ROWS, per - r0), D = a.D;
-  const int row = a.t_row[t];
-  if (row < 0 || row >= a.pt.rows) return;
-  const Span span(slots_seen(a.pt, a.t_slot[t]), a.first, a.window);
-  const int chunks = D * (int)sizeof(T) / 16, stride = (chunks | 1) * 16;
-  float* qs = reinterpret_cast<float*>(smem);                       // [PG_ROWS][D]
-  float* ps = qs + PG_ROWS * D + warp * PG_ROWS * PA_TILE;          // [PG_WARPS][PG_ROWS][16]
-  float* ms = qs + PG_ROWS * D + PG_WARPS * PG_ROWS * PA_TILE;      // [PG_WARPS][PG_ROWS][2 + D]
-  uint8_t* ks = reinterpret_cast<uint8_t*>(ms + PG_WARPS * PG_ROWS * (2 + D)) + warp * 2 * PA_TILE * stride;
-  uint8_t* vs = ks + PA_TILE * stride;
-  const T* q = reinterpret_cast<const T*>(a.q) + ((int64_t)t * a.H + (int64_t)g * per + r0) * D;
-  for (int i = threadIdx.x; i < rows * D; i += blockDim.x) qs[i] = Tr<T>::to_f(q[i]) * a.scale_log2e;
-  __syncthreads();
-  float o[PG_ROWS][NG][4], m[PG_ROWS], l[PG_ROWS];
-#pragma unroll
-  for (int r = 0; r < PG_ROWS; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-#pragma unroll
-    for (int x = 0; x < NG; ++x) o[r][x][0] = o[r][x][1] = o[r][x][2] = o[r][x][3] = 0.f;
-  }
-  float* scores = a.ws + ((int64_t)t * a.H + (int64_t)g * per + r0) * a.cap;
-  for (int v = warp; v < span.tiles; v += PG_WARPS) {
-    const int j0 = span.key0(v);
-    const int64_t id = page_id(a.pt, row, j0 / a.pt.page);
-    const int64_t base = ((id < 0 ? 0 : id) * a.G + g) * a.pt.page + j0 % a.pt.page;
-    if (id < 0 && lane == 0) atomicAdd(&g_paged_attn_fault, 1u);
-    const uint8_t* kg = reinterpret_cast<const uint8_t*>(a.k) + base * D * (int)sizeof(T);
-    const uint8_t* vg = reinterpret_cast<const uint8_t*>(a.v) + base * D * (int)sizeof(T);
-    for (int x = lane; x < PA_TILE * chunks; x += 32) {
-      const int key = x / chunks, c = x - key * chunks;
-      const bool ok = id >= 0 && span.visible(j0 + key);
-      cp_async16((uint32_t)__cvta_generic_to_shared(ks + key * stride + c * 16), kg + (ok ? x : 0) * 16, ok);
-      cp_async16((uint32_t)__cvta_generic_to_shared(vs + key * stride + c * 16), vg + (ok ? x : 0) * 16, ok);
+// The work is cut evenly however unequal the rows are: every token's visible tiles are counted in units of one tile per warp, the units of all
+// (token, key head, block of query heads) items are laid end to end, and each of C CTAs takes the same number of them.  An item that lies in one
+// CTA's share is finished there; of one that is cut every CTA leaves a part, and paged_attn_join_kernel joins them.  (One CTA per item left the
+// GPU idle behind the longest rows: 64 rows of 130 to 500 tokens took 108 us, of 8192 tokens 940.)
+struct Token {
+  int row, units;
+  Span span;
+  __device__ Token(const PagedAttn& a, int t, int warps) : row(a.t_row[t]), units(0), span(0, 0, 0) {
+    if (row >= 0 && row < a.pt.rows) {
+      span = Span(slots_seen(a.pt, a.t_slot[t]), a.first, a.window);
+      units = span.tiles > warps ? (span.tiles + warps - 1) / warps : 1;      // a token that sees nothing: one, for its zeros
     }
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncwarp();
-    const int key = lane & 15, half = lane >> 4;
-    float s[PG_ROWS];
+  }
+};
+// CTAs that share U units
+__device__ __forceinline__ int64_t shares(int64_t U, int most) { return U < most ? U : most; }
+__device__ __forceinline__ int64_t share_begin(int64_t U, int64_t C, int64_t c) { return U * c / C; }
+
+// A position in a CTA's share: the token, and of its units the run [a, b) of one item.
+struct Cursor {
+  int64_t u, end, base;
+  int t, item, a, b;
+  Token tok;
+  __device__ Cursor(const PagedAttn& p, int64_t u_, int64_t end_, int t_, int64_t base_, int warps)
+      : u(u_), end(end_), base(base_), t(t_), item(0), a(0), b(0), tok(p, t_, warps) {}
+  __device__ bool next(const PagedAttn& p, int items, int warps) {
+    if (u >= end) return false;
+    while (u >= base + (int64_t)tok.units * items) {
+      base += (int64_t)tok.units * items;
+      tok = Token(p, ++t, warps);
+    }
+    const unsigned at = (unsigned)(u - base);
+    item = at / (unsigned)tok.units;
+    a = at - item * tok.units;
+    b = (int)min((int64_t)tok.units, a + (end - u));
+    u += b - a;
+    return true;
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ engines
+// What a warp does with a staged tile of 16 keys.  ROWS query heads of one key head share it, so keys and values are read once.
+
+// 16-bit types, D a multiple of 16: mma.sync m16n8k16, query heads as the 16 rows (of which 4 to 8 are in use: the kernel waits for its bytes, the
+// tensor cores idle either way).  The weights multiply the values as two 16-bit numbers each (the rounded weight and what it lost), so that
+// the output carries its own rounding only.
+template <typename T_, int D_>
+struct TcEngine {
+  using T = T_;
+  static constexpr int D = D_, ROWS = 16, WARPS = 4, STAGES = D_ > 128 ? 2 : 3;
+  static constexpr int CHUNKS = D / 8, PIECES = CHUNKS % 8 ? (CHUNKS | 1) : CHUNKS;    // 16-byte pieces of a staged line
+  static constexpr int Q_STRIDE = D * 2 + 16, Q_BYTES = ROWS * Q_STRIDE;
+  static constexpr int NQ = (ROWS * CHUNKS + WARPS * 32 - 1) / (WARPS * 32);
+  // f16: the largest weight of a tile is 2^14 and not 1 (m is the maximum less 14), so that small weights keep their bits
+  static constexpr float SHIFT = std::is_same<T_, __half>::value ? 14.f : 0.f;
+  float o[D / 8][4], m[2], l[2];
+  uint32_t qf[D > 128 ? 1 : D / 16][4];
+
+  static __device__ __forceinline__ int dim(const PagedAttn&) { return D; }
+  static __host__ __device__ __forceinline__ int tile_bytes(int) { return 2 * PA_TILE * PIECES * 16; }
+  static __device__ __forceinline__ uint32_t at(int key, int c) {
+    return (uint32_t)(key * PIECES * 16 + ((CHUNKS % 8 ? c : c ^ (key & 7)) << 4));
+  }
+  static __device__ __forceinline__ void q_frag(uint32_t qs, int ks, uint32_t (&f)[4]) {
+    const int lane = threadIdx.x & 31, mat = lane >> 3, r = lane & 7;
+    ldsm_x4(qs + (r + 8 * (mat & 1)) * Q_STRIDE + (2 * ks + (mat >> 1)) * 16, f);
+  }
+  static __device__ __forceinline__ void put_q(uint8_t* qs, int r, int c, const uint4& x, int) {
+    *reinterpret_cast<uint4*>(qs + r * Q_STRIDE + c * 16) = x;
+  }
+  __device__ __forceinline__ void begin(uint32_t qs) {
 #pragma unroll
-    for (int r = 0; r < PG_ROWS; ++r) s[r] = 0.f;
-    constexpr int E = 16 / sizeof(T);
+    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+    if constexpr (D <= 128) {
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) q_frag(qs, ks, qf[ks]);
+    }
+  }
+  __device__ __forceinline__ void tile(const PagedAttn& a, uint32_t qs, uint32_t ks, int j0, const Span& sp, bool all, bool page, float* sc, int rows,
+                                       uint8_t*) {
+    const int lane = threadIdx.x & 31, qr = lane >> 2, qc = lane & 3, mat = lane >> 3, r8 = lane & 7;
+    const uint32_t vs = ks + PA_TILE * PIECES * 16;
+    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t bf[4], qt[4];
+      ldsm_x4(ks + at(r8 + 8 * (mat >> 1), 2 * k + (mat & 1)), bf);
+      if constexpr (D <= 128) {
+        mma16816<T>(s0, qf[k], bf[0], bf[1]);
+        mma16816<T>(s1, qf[k], bf[2], bf[3]);
+      } else {
+        q_frag(qs, k, qt);
+        mma16816<T>(s0, qt, bf[0], bf[1]);
+        mma16816<T>(s1, qt, bf[2], bf[3]);
+      }
+    }
+    // two rows (query heads qr and qr + 8) of four keys: 2 qc, 2 qc + 1 and the same + 8
+    float x[2][4] = {{s0[0], s0[1], s1[0], s1[1]}, {s0[2], s0[3], s1[2], s1[3]}};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool seen = all || (page && sp.visible(j0 + 2 * qc + (i & 1) + 8 * (i >> 1)));
+      x[0][i] = seen ? x[0][i] * a.scale_log2e : -INFINITY;
+      x[1][i] = seen ? x[1][i] * a.scale_log2e : -INFINITY;
+    }
+    if (sc) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (qr + 8 * h < rows) {
+          float* p = sc + (int64_t)(qr + 8 * h) * a.cap + 2 * qc;
+          *reinterpret_cast<float2*>(p) = make_float2(x[h][0], x[h][1]);
+          *reinterpret_cast<float2*>(p + 8) = make_float2(x[h][2], x[h][3]);
+        }
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float t = fmaxf(fmaxf(x[h][0], x[h][1]), fmaxf(x[h][2], x[h][3]));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      t = fmaxf(t - SHIFT, m[h]);
+      const float ref = t == -INFINITY ? 0.f : t;                // nothing seen yet
+      const float f = exp2f(m[h] - ref);
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = exp2f(x[h][i] - ref);
+      m[h] = t;
+      l[h] = l[h] * f + (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) { o[j][2 * h] *= f; o[j][2 * h + 1] *= f; }
+      float q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = p[i] - Tr<T>::to_f(Tr<T>::from_f(p[i]));
+      hi[h] = pack2<T>(p[0], p[1]);
+      hi[h + 2] = pack2<T>(p[2], p[3]);
+      lo[h] = pack2<T>(q[0], q[1]);
+      lo[h + 2] = pack2<T>(q[2], q[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      uint32_t bf[4];
+      ldsm_x4_trans(vs + at(r8 + 8 * (mat & 1), 2 * j + (mat >> 1)), bf);
+      mma16816<T>(o[2 * j], hi, bf[0], bf[1]);
+      mma16816<T>(o[2 * j + 1], hi, bf[2], bf[3]);
+      mma16816<T>(o[2 * j], lo, bf[0], bf[1]);
+      mma16816<T>(o[2 * j + 1], lo, bf[2], bf[3]);
+    }
+  }
+  // rows [8 pass, 8 pass + 8) of this warp's part to p [8][D + 4]
+  __device__ __forceinline__ void publish(float* p, int pass, int) {
+    const int lane = threadIdx.x & 31, qr = lane >> 2, qc = lane & 3;
+    float* row = p + qr * (D + 4);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (h == pass) {
+        float sum = l[h];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (qc == 0) { row[0] = m[h]; row[1] = sum; }
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(row + 4 + 8 * j + 2 * qc) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+      }
+  }
+};
+
+// Every type and size, in fp32 FMAs: two lanes share a key for the scores, for the outputs a lane owns 4 (NG 2: 8) dimensions of 8 query heads.
+template <typename T_, int NG>
+struct FmaEngine {
+  using T = T_;
+  static constexpr int ROWS = 8, WARPS = sizeof(T_) == 4 && NG == 2 ? 2 : 4, STAGES = 2;
+  static constexpr int E = 16 / (int)sizeof(T_);
+  static constexpr int Q_BYTES = (ROWS * NG * 128 + WARPS * ROWS * PA_TILE) * 4;     // queries and every warp's weights, fp32
+  static constexpr int NQ = (ROWS * NG * 128 / E + WARPS * 32 - 1) / (WARPS * 32);
+  float o[ROWS][NG][4], m[ROWS], l[ROWS];
+
+  static __device__ __forceinline__ int dim(const PagedAttn& a) { return a.D; }
+  static __host__ __device__ __forceinline__ int line(int D) { return (D / E | 1) * 16; }
+  static __host__ __device__ __forceinline__ int tile_bytes(int D) { return 2 * PA_TILE * line(D); }
+  static __device__ __forceinline__ void put_q(uint8_t* qs, int r, int c, const uint4& x, int D) {
+    const T* v = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) reinterpret_cast<float*>(qs)[r * D + c * E + e] = Tr<T>::to_f(v[e]);
+  }
+  __device__ __forceinline__ void begin(uint32_t) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+#pragma unroll
+      for (int x = 0; x < NG; ++x) o[r][x][0] = o[r][x][1] = o[r][x][2] = o[r][x][3] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void tile(const PagedAttn& a, uint32_t qs_, uint32_t, int j0, const Span& sp, bool all, bool page, float* sc, int rows,
+                                       uint8_t* ks) {
+    const int lane = threadIdx.x & 31, key = lane & 15, half = lane >> 4, D = a.D, chunks = D / E, stride = line(D);
+    const uint8_t* vs = ks + PA_TILE * stride;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const float* qs = reinterpret_cast<const float*>(smem);
+    float* ps = reinterpret_cast<float*>(smem) + ROWS * NG * 128 + (threadIdx.x >> 5) * ROWS * PA_TILE;
+    float s[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) s[r] = 0.f;
     for (int c = half; c < chunks; c += 2) {
       T kv[E];
       *reinterpret_cast<uint4*>(kv) = *reinterpret_cast<const uint4*>(ks + key * stride + c * 16);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float x = Tr<T>::to_f(kv[e]);
+      for (int e = 0; e < E; e += 4) {
 #pragma unroll
-        for (int r = 0; r < PG_ROWS; ++r)
-          if (r < rows) s[r] = fmaf(x, qs[r * D + c * E + e], s[r]);
+        for (int r = 0; r < ROWS; ++r)
+          if (r < rows) {
+            const float4 q = *reinterpret_cast<const float4*>(qs + r * D + c * E + e);
+            s[r] = fmaf(Tr<T>::to_f(kv[e]), q.x, s[r]);
+            s[r] = fmaf(Tr<T>::to_f(kv[e + 1]), q.y, s[r]);
+            s[r] = fmaf(Tr<T>::to_f(kv[e + 2]), q.z, s[r]);
+            s[r] = fmaf(Tr<T>::to_f(kv[e + 3]), q.w, s[r]);
+          }
       }
     }
-    const bool seen = id >= 0 && span.visible(j0 + key);
+    const bool seen = all || (page && sp.visible(j0 + key));
 #pragma unroll
-    for (int r = 0; r < PG_ROWS; ++r) {
+    for (int r = 0; r < ROWS; ++r) {
       if (r >= rows) break;
-      float x = s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16);
+      float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * a.scale_log2e;
       x = seen ? x : -INFINITY;
-      if (a.mass && half == 0) scores[(int64_t)r * a.cap + v * PA_TILE + key] = x;
-      const float mx = fmaxf(m[r], warp_max(x));
-      const float ref = mx == -INFINITY ? 0.f : mx;              // nothing seen yet
+      if (sc && half == 0) sc[(int64_t)r * a.cap + key] = x;
+      const float t = fmaxf(m[r], warp_max(x));
+      const float ref = t == -INFINITY ? 0.f : t;
       const float f = exp2f(m[r] - ref), p = exp2f(x - ref);
-      m[r] = mx;
+      m[r] = t;
       l[r] = l[r] * f + warp_sum(half == 0 ? p : 0.f);
       if (half == 0) ps[r * PA_TILE + key] = p;
 #pragma unroll
-      for (int x2 = 0; x2 < NG; ++x2)
+      for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[r][x2][e] *= f;
+        for (int e = 0; e < 4; ++e) o[r][g][e] *= f;
     }
     __syncwarp();
     for (int k = 0; k < PA_TILE; ++k)
 #pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        const int d = (lane + 32 * x) * 4;
+      for (int g = 0; g < NG; ++g) {
+        const int d = (lane + 32 * g) * 4;
         if (d >= D) break;
         T vv[4];
         if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(vv) = *reinterpret_cast<const uint4*>(vs + k * stride + d * 4);
         else *reinterpret_cast<uint2*>(vv) = *reinterpret_cast<const uint2*>(vs + k * stride + d * 2);
 #pragma unroll
-        for (int r = 0; r < PG_ROWS; ++r)
+        for (int r = 0; r < ROWS; ++r)
           if (r < rows)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[r][x][e] = fmaf(ps[r * PA_TILE + k], Tr<T>::to_f(vv[e]), o[r][x][e]);
+            for (int e = 0; e < 4; ++e) o[r][g][e] = fmaf(ps[r * PA_TILE + k], Tr<T>::to_f(vv[e]), o[r][g][e]);
       }
-    __syncwarp();
   }
+  static __device__ __forceinline__ uint32_t at(int key, int c, int D) { return (uint32_t)(key * line(D) + c * 16); }
+  __device__ __forceinline__ void publish(float* p, int, int D) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int r = 0; r < PG_ROWS; ++r) {
-    float* p = ms + (warp * PG_ROWS + r) * (2 + D);
-    if (lane == 0) { p[0] = m[r]; p[1] = l[r]; }
+    for (int r = 0; r < ROWS; ++r) {
+      float* row = p + r * (D + 4);
+      if (lane == 0) { row[0] = m[r]; row[1] = l[r]; }
 #pragma unroll
-    for (int x = 0; x < NG; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if ((lane + 32 * x) * 4 < D) p[2 + (lane + 32 * x) * 4 + e] = o[r][x][e];
-  }
-  __syncthreads();
-  T* out = reinterpret_cast<T*>(a.out) + ((int64_t)t * a.H + (int64_t)g * per + r0) * D;
-  for (int i = threadIdx.x; i < rows * D; i += blockDim.x) {
-    const int r = i / D, d = i - r * D;
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int w = 0; w < PG_WARPS; ++w) M = fmaxf(M, ms[(w * PG_ROWS + r) * (2 + D)]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    for (int w = 0; w < PG_WARPS; ++w) {
-      const float* p = ms + (w * PG_ROWS + r) * (2 + D);
-      const float f = exp2f(p[0] - ref);
-      L += p[1] * f;
-      acc += p[2 + d] * f;
+      for (int g = 0; g < NG; ++g)
+        if ((lane + 32 * g) * 4 < D) *reinterpret_cast<float4*>(row + 4 + (lane + 32 * g) * 4) = make_float4(o[r][g][0], o[r][g][1], o[r][g][2], o[r][g][3]);
     }
-    out[(int64_t)r * D + (a.out_perm ? perm8_pos(d) : d)] = Tr<T>::from_f(L == 0.f ? 0.f : acc / L);
   }
-  if (!a.mass) return;
-  __syncthreads();
-  if (threadIdx.x < rows) {                                        // maximum and 1 / sum of every head, into the first warp's record
-    const int r = threadIdx.x;
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < PG_WARPS; ++w) M = fmaxf(M, ms[(w * PG_ROWS + r) * (2 + D)]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    for (int w = 0; w < PG_WARPS; ++w) L += ms[(w * PG_ROWS + r) * (2 + D) + 1] * exp2f(ms[(w * PG_ROWS + r) * (2 + D)] - ref);
-    qs[2 * r] = ref;
-    qs[2 * r + 1] = L == 0.f ? 0.f : 1.f / L;
-  }
-  __syncthreads();
-  for (int x = threadIdx.x; x < span.tiles * PA_TILE; x += blockDim.x) {
-    const int j = span.key0(x / PA_TILE) + x % PA_TILE;
-    if (!span.visible(j)) continue;
-    const int64_t id = page_id(a.pt, row, j / a.pt.page);
-    if (id < 0) continue;
-    float w = 0.f;
-    for (int r = 0; r < rows; ++r) w += exp2f(scores[(int64_t)r * a.cap + x] - qs[2 * r]) * qs[2 * r + 1];
-    atomicAdd(&a.mass[(id * a.G + g) * a.pt.page + j % a.pt.page], w);
+};
+
+template <typename E> struct IsTc { static constexpr bool value = false; };
+template <typename T, int D> struct IsTc<TcEngine<T, D>> { static constexpr bool value = true; };
+
+template <typename T>
+__device__ __forceinline__ void store_row4(T* out, int d, float4 v, int perm) {
+  if (perm) {
+    out[perm8_pos(d)] = Tr<T>::from_f(v.x);
+    out[perm8_pos(d + 1)] = Tr<T>::from_f(v.y);
+    out[perm8_pos(d + 2)] = Tr<T>::from_f(v.z);
+    out[perm8_pos(d + 3)] = Tr<T>::from_f(v.w);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(out + d) = v;
+  } else {
+    *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
   }
 }
 
-template <typename T, int NG>
-static int launch_any(const PagedAttn& a, int64_t M, cudaStream_t st) {
-  const int chunks = a.D * (int)sizeof(T) / 16, stride = (chunks | 1) * 16;
-  const size_t smem = 4 * (size_t)(PG_ROWS * a.D + PG_WARPS * PG_ROWS * PA_TILE + PG_WARPS * PG_ROWS * (2 + a.D)) + (size_t)PG_WARPS * 2 * PA_TILE * stride;
-  auto kern = paged_attn_any_kernel<T, NG>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_attn_any_kernel)");
-  const int per = a.H / a.G, blocks = (per + PG_ROWS - 1) / PG_ROWS;
-  kern<<<dim3((unsigned)(blocks * a.G), (unsigned)M), PG_WARPS * 32, smem, st>>>(a);
-  B200P_LAUNCH_CHECK("paged_attn_any_kernel");
-  return B200P_OK;
+// ------------------------------------------------------------------------------------------------ the kernel
+template <typename E>
+__global__ void __launch_bounds__(E::WARPS * 32, 2)
+paged_attn_kernel(const PagedAttn a) {
+  using T = typename E::T;
+  constexpr int W = E::WARPS, THREADS = W * 32;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int64_t s_sum[W], s_base;
+  __shared__ int s_t, s_part[W];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int D = E::dim(a), chunks = D * (int)sizeof(T) / 16;
+  const int per = a.H / a.G, blocks = (per + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
+  uint8_t* ring = smem + E::Q_BYTES + warp * E::STAGES * E::tile_bytes(D);
+  const uint32_t qs = (uint32_t)__cvta_generic_to_shared(smem), ring32 = (uint32_t)__cvta_generic_to_shared(ring);
+  pdl_wait();
+
+  // ---- the plan: units of all tokens, this CTA's share, the token in which it begins -------------------------------------
+  const int chunk = (a.M + THREADS - 1) / THREADS;
+  const int t0 = min(a.M, (int)threadIdx.x * chunk), t1 = min(a.M, t0 + chunk);
+  int64_t mine = 0;
+  for (int t = t0; t < t1; ++t) mine += (int64_t)Token(a, t, W).units * items;
+  int64_t before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  if (lane == 31) s_sum[warp] = before;
+  __syncthreads();
+  before -= mine;
+  int64_t U = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w < warp) before += s_sum[w];
+    U += s_sum[w];
+  }
+  if (blockIdx.x == 0) {
+    int64_t x = before;
+    for (int t = t0; t < t1; ++t) {
+      a.base[t] = x;
+      x += (int64_t)Token(a, t, W).units * items;
+    }
+    if (threadIdx.x == 0) a.base[a.M] = U;
+  }
+  const int64_t C = shares(U, (int)gridDim.x);
+  if ((int64_t)blockIdx.x >= C) return;
+  const int64_t ub = share_begin(U, C, blockIdx.x), ue = share_begin(U, C, blockIdx.x + 1);
+  if (ub >= before && ub < before + mine) {
+    int64_t x = before;
+    for (int t = t0; t < t1; ++t) {
+      const int64_t n = (int64_t)Token(a, t, W).units * items;
+      if (ub < x + n) {
+        s_t = t;
+        s_base = x;
+        break;
+      }
+      x += n;
+    }
+  }
+  __syncthreads();
+
+  // ---- loads run ahead of the products, across items --------------------------------------------------------------------
+  Cursor ld(a, ub, ue, s_t, s_base, W), cu = ld;
+  bool more = ld.next(a, items, W);
+  int tile = ld.a * W + warp, tile_end = min(ld.b * W, ld.tok.span.tiles);
+  unsigned paged = 0;                                             // stages whose keys have a page
+  auto issue = [&](int stage) {
+    while (more && tile >= tile_end) {
+      more = ld.next(a, items, W);
+      tile = ld.a * W + warp;
+      tile_end = min(ld.b * W, ld.tok.span.tiles);
+    }
+    if (more) {
+      const Span& sp = ld.tok.span;
+      const int j0 = sp.key0(tile), g = ld.item / blocks;
+      const int64_t id = page_id(a.pt, ld.tok.row, j0 / a.pt.page);
+      const int64_t line = ((id < 0 ? 0 : id) * a.G + g) * a.pt.page + j0 % a.pt.page;
+      const uint4* kg = reinterpret_cast<const uint4*>(a.k) + line * chunks;
+      const uint4* vg = reinterpret_cast<const uint4*>(a.v) + line * chunks;
+      const uint32_t ks = ring32 + stage * E::tile_bytes(D), vs = ks + E::tile_bytes(D) / 2;
+      if (id < 0 && lane == 0) atomicAdd(&g_paged_attn_fault, 1u);
+      paged = (paged & ~(1u << stage)) | ((id >= 0 ? 1u : 0u) << stage);
+      if constexpr (IsTc<E>::value) {
+#pragma unroll
+        for (int i = 0; i < (PA_TILE * E::CHUNKS + 31) / 32; ++i) {
+          const int x = i * 32 + lane, key = x / E::CHUNKS, c = x % E::CHUNKS;
+          if (PA_TILE * E::CHUNKS % 32 && key >= PA_TILE) break;
+          const bool ok = id >= 0 && sp.visible(j0 + key);
+          cp_async16(ks + E::at(key, c), kg + (ok ? x : 0), ok);
+          cp_async16(vs + E::at(key, c), vg + (ok ? x : 0), ok);
+        }
+      } else {
+        for (int x = lane; x < PA_TILE * chunks; x += 32) {
+          const int key = x / chunks, c = x - key * chunks;
+          const bool ok = id >= 0 && sp.visible(j0 + key);
+          cp_async16(ks + E::at(key, c, D), kg + (ok ? x : 0), ok);
+          cp_async16(vs + E::at(key, c, D), vg + (ok ? x : 0), ok);
+        }
+      }
+      tile += W;
+    }
+    cp_async_commit();
+  };
+  // the queries of an item, a few 16-byte pieces per thread: those of the next one are fetched while this one's keys pass
+  uint4 qn[E::NQ];
+  auto fetch_q = [&](const Cursor& c) {
+    const int g = c.item / blocks, r0 = (c.item - g * blocks) * E::ROWS, rows = min(E::ROWS, per - r0);
+    const uint4* q = reinterpret_cast<const uint4*>(a.q) + ((int64_t)c.t * a.H + (int64_t)g * per + r0) * chunks;
+#pragma unroll
+    for (int i = 0; i < E::NQ; ++i) {
+      const int x = i * THREADS + (int)threadIdx.x;
+      qn[i] = x < rows * chunks ? q[x] : make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto put_q = [&]() {
+#pragma unroll
+    for (int i = 0; i < E::NQ; ++i) {
+      const int x = i * THREADS + (int)threadIdx.x;
+      if (x < E::ROWS * chunks) E::put_q(smem, x / chunks, x % chunks, qn[i], D);
+    }
+  };
+  bool work = cu.next(a, items, W);
+  fetch_q(cu);
+#pragma unroll
+  for (int s = 0; s < E::STAGES - 1; ++s) issue(s);
+  put_q();
+  __syncthreads();
+
+  E e;
+  int stage = 0;                                                  // of the next tile
+  while (work) {
+    const Cursor me = cu;
+    work = cu.next(a, items, W);
+    if (work) fetch_q(cu);
+    const int g = me.item / blocks, r0 = (me.item - g * blocks) * E::ROWS, rows = min(E::ROWS, per - r0);
+    const int64_t head = (int64_t)me.t * a.H + (int64_t)g * per + r0;
+    const Span sp = me.tok.span;
+    e.begin(qs);
+    const int end = min(me.b * W, sp.tiles);
+    for (int v = me.a * W + warp; v < end; v += W) {
+      issue(stage == 0 ? E::STAGES - 1 : stage - 1);
+      cp_async_wait<E::STAGES - 1>();
+      __syncwarp();
+      const int j0 = sp.key0(v);
+      const bool page = (paged >> stage) & 1u;
+      const bool all = page && j0 + PA_TILE <= sp.n && (j0 >= sp.lo || j0 + PA_TILE <= sp.first);
+      e.tile(a, qs, ring32 + stage * E::tile_bytes(D), j0, sp, all, page, a.mass ? a.scores + head * a.cap + v * PA_TILE : nullptr, rows,
+             ring + stage * E::tile_bytes(D));
+      __syncwarp();                                               // the stage is refilled by the next issue
+      stage = stage + 1 == E::STAGES ? 0 : stage + 1;
+    }
+    // ---- the warps' parts become one: each in the one stage of its ring that waits for nothing ------------------------------
+    const int part = (warp * E::STAGES + (stage == 0 ? E::STAGES - 1 : stage - 1)) * E::tile_bytes(D);
+    if (lane == 0) s_part[warp] = part;
+    const bool whole = me.a == 0 && me.b == me.tok.units;
+    float* rec = a.rec + (((int64_t)blockIdx.x * 2 + (me.a == 0 ? 1 : 0)) * E::ROWS) * (D + 4);
+    for (int pass = 0; pass * 8 < rows; ++pass) {
+      e.publish(reinterpret_cast<float*>(smem + E::Q_BYTES + part), pass, D);
+      __syncthreads();
+      if (pass == 0 && work) put_q();
+      const int here = min(8, rows - pass * 8), quads = D / 4;
+      for (int x = threadIdx.x; x < here * quads; x += THREADS) {
+        const int r = x / quads, d = (x - r * quads) * 4;
+        float M = -INFINITY, L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, reinterpret_cast<const float*>(smem + E::Q_BYTES + s_part[w])[r * (D + 4)]);
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float* p = reinterpret_cast<const float*>(smem + E::Q_BYTES + s_part[w]) + r * (D + 4);
+          const float f = exp2f(p[0] - ref);
+          const float4 y = *reinterpret_cast<const float4*>(p + 4 + d);
+          L += p[1] * f;
+          acc.x += y.x * f; acc.y += y.y * f; acc.z += y.z * f; acc.w += y.w * f;
+        }
+        const int row = pass * 8 + r;
+        if (whole) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          store_row4<T>(reinterpret_cast<T*>(a.out) + (head + row) * D, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv), a.out_perm);
+          if (a.mass && d == 0) *reinterpret_cast<float2*>(a.stat + (head + row) * 2) = make_float2(ref, inv);
+        } else {
+          float* p = rec + row * (D + 4);
+          *reinterpret_cast<float4*>(p + 4 + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(p) = make_float2(M, L);
+        }
+      }
+      __syncthreads();
+    }
+  }
+  cp_async_wait<0>();
 }
+
+// One CTA per item (x) that was cut: a warp joins the parts of a query head, several warps share a head's parts where the heads are few.  With
+// a mass (y: slices of the visible slots) every CTA forms the heads' maxima and sums anew and adds its slice's weights up.
+constexpr int PJ_WARPS = 8, PJ_SLICE = 1024;
+
+template <typename E>
+__global__ void __launch_bounds__(PJ_WARPS * 32)
+paged_attn_join_kernel(const PagedAttn a, int most) {
+  using T = typename E::T;
+  extern __shared__ __align__(16) float sm[];                     // [PJ_WARPS][D + 4], then [ROWS][2]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = E::dim(a);
+  float* stat = sm + PJ_WARPS * (D + 4);
+  const int per = a.H / a.G, blocks = (per + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
+  const int t = blockIdx.x / items, item = blockIdx.x - t * items;
+  const int g = item / blocks, r0 = (item - g * blocks) * E::ROWS, rows = min(E::ROWS, per - r0);
+  pdl_wait();
+  const Token tok(a, t, E::WARPS);
+  if (tok.units == 0) return;
+  if (blockIdx.y > 0 && (int)blockIdx.y * PJ_SLICE >= tok.span.tiles * PA_TILE) return;
+  const bool outputs = blockIdx.y == 0;
+  const int64_t U = a.base[a.M], C = shares(U, most), u0 = a.base[t] + (int64_t)item * tok.units, u1 = u0 + tok.units;
+  int64_t c0 = u0 * C / U, c1 = (u1 - 1) * C / U;
+  while (share_begin(U, C, c0 + 1) <= u0) ++c0;
+  while (share_begin(U, C, c1 + 1) <= u1 - 1) ++c1;
+  const int64_t head = (int64_t)t * a.H + (int64_t)g * per + r0;
+  const bool cut = c0 != c1;
+  if (!cut && !a.mass) return;
+  if (cut) {
+    const int parts = (int)(c1 - c0 + 1), quads = D / 4;
+    const int ways = rows >= PJ_WARPS ? 1 : PJ_WARPS / rows;      // warps per head
+    for (int rb = 0; rb < rows; rb += PJ_WARPS / ways) {
+      const int r = rb + warp / ways, way = warp - warp / ways * ways;
+      const bool mine = warp < PJ_WARPS / ways * ways && r < rows;
+      float M = -INFINITY, L = 0.f;
+      float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+      if (mine) {
+        auto part = [&](int i) { return a.rec + (((c0 + i) * 2 + (i == 0 ? 1 : 0)) * E::ROWS + r) * (D + 4); };
+        for (int i = way; i < parts; i += ways) M = fmaxf(M, part(i)[0]);
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll 4
+        for (int i = way; i < parts; i += ways) {
+          const float* p = part(i);
+          const float f = exp2f(p[0] - ref);
+          L += p[1] * f;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (outputs && lane + 32 * x < quads) {
+              const float4 y = *reinterpret_cast<const float4*>(p + 4 + (lane + 32 * x) * 4);
+              acc[x].x += y.x * f; acc[x].y += y.y * f; acc[x].z += y.z * f; acc[x].w += y.w * f;
+            }
+        }
+        float* p = sm + warp * (D + 4);
+        if (lane == 0) { p[0] = M; p[1] = L; }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (outputs && lane + 32 * x < quads) *reinterpret_cast<float4*>(p + 4 + (lane + 32 * x) * 4) = acc[x];
+      }
+      __syncthreads();
+      if (mine && way == 0) {
+        M = -INFINITY, L = 0.f;
+        for (int w = 0; w < ways; ++w) M = fmaxf(M, sm[(warp + w) * (D + 4)]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        for (int w = 0; w < ways; ++w) L += sm[(warp + w) * (D + 4) + 1] * exp2f(sm[(warp + w) * (D + 4)] - ref);
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        if (lane == 0) { stat[2 * r] = ref; stat[2 * r + 1] = inv; }
+        if (outputs)
+          for (int x = lane; x < quads; x += 32) {
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = 0; w < ways; ++w) {
+              const float* p = sm + (warp + w) * (D + 4);
+              const float f = exp2f(p[0] - ref) * inv;
+              const float4 y = *reinterpret_cast<const float4*>(p + 4 + x * 4);
+              s.x += y.x * f; s.y += y.y * f; s.z += y.z * f; s.w += y.w * f;
+            }
+            store_row4<T>(reinterpret_cast<T*>(a.out) + (head + r) * D, x * 4, s, a.out_perm);
+          }
+      }
+      __syncthreads();
+    }
+  } else {
+    if ((int)threadIdx.x < 2 * rows) stat[threadIdx.x] = a.stat[head * 2 + threadIdx.x];
+    __syncthreads();
+  }
+  if (!a.mass) return;
+  const float* sc = a.scores + head * a.cap;
+  const int seen = tok.span.tiles * PA_TILE;
+  for (int v0 = blockIdx.y * PJ_SLICE; v0 < seen; v0 += gridDim.y * PJ_SLICE)
+    for (int x = v0 + threadIdx.x; x < min(seen, v0 + PJ_SLICE); x += PJ_WARPS * 32) {
+      const int j = tok.span.key0(x / PA_TILE) + x % PA_TILE;
+      if (!tok.span.visible(j)) continue;
+      const int64_t id = page_id(a.pt, tok.row, j / a.pt.page);
+      if (id < 0) continue;
+      float w = 0.f;
+      for (int r = 0; r < rows; ++r) w += exp2f(sc[(int64_t)r * a.cap + x] - stat[2 * r]) * stat[2 * r + 1];
+      atomicAdd(&a.mass[(id * a.G + g) * a.pt.page + j % a.pt.page], w);    // slots that several tokens see
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+constexpr int PA_CTAS = 2;            // per SM: one's join beside the other's stream
 
 // visible slots a token can have, in whole tiles
 static int64_t visible_cap(int64_t slots, int64_t first, int64_t window) {
@@ -224,13 +646,62 @@ static int64_t visible_cap(int64_t slots, int64_t first, int64_t window) {
   return ((seen < slots ? seen : slots) + PA_TILE - 1) / PA_TILE * PA_TILE;
 }
 
+static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+static size_t base_bytes(int64_t M) { return round256((size_t)(M + 1) * 8); }
+static size_t rec_bytes(int D) { return round256((size_t)sm_count() * PA_CTAS * 2 * 16 * (D + 4) * 4); }
+static size_t stat_bytes(int64_t M, int H) { return round256((size_t)M * H * 8); }
+
+template <typename E>
+static int launch_paged(PagedAttn a, cudaStream_t st) {
+  const int smem = E::Q_BYTES + E::WARPS * E::STAGES * E::tile_bytes(a.D);
+  const int blocks = (a.H / a.G + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
+  B200P_REQUIRE((int64_t)items * (a.cap / PA_TILE / E::WARPS + 1) < (1ll << 31) && (int64_t)a.M * items < (1ll << 31), B200P_ERR_ARG,
+                "%d tokens of %d key heads over %d slots: too many for one call", a.M, a.G, a.cap);
+  auto kern = paged_attn_kernel<E>;
+  static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_attn_kernel)");
+  const int ctas = sm_count() * (2 * (smem + 1024 + 256) <= 228 * 1024 ? 2 : 1);
+  const int64_t most = (int64_t)a.M * items * ((a.cap / PA_TILE + E::WARPS - 1) / E::WARPS);
+  const int grid = (int)(most < ctas ? most : ctas);
+  launch_pdl(kern, (unsigned)grid, E::WARPS * 32, smem, st, a);
+  B200P_LAUNCH_CHECK("paged_attn_kernel");
+  // slices of a mass: as many as there are, but no more CTAs than fill the GPU
+  const int64_t slices = a.mass ? (a.cap + PJ_SLICE - 1) / PJ_SLICE : 1, fill = 8ll * sm_count() / ((int64_t)a.M * items) + 1;
+  launch_pdl(paged_attn_join_kernel<E>, dim3((unsigned)(a.M * items), (unsigned)(slices < fill ? slices : fill)), PJ_WARPS * 32, (PJ_WARPS * (a.D + 4) + 2 * E::ROWS) * 4, st, a,
+             grid);
+  B200P_LAUNCH_CHECK("paged_attn_join_kernel");
+  return B200P_OK;
+}
+
+template <typename T>
+static int launch_paged_type(const PagedAttn& a, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    switch (a.D) {
+      case 64: return launch_paged<TcEngine<T, 64>>(a, st);
+      case 80: return launch_paged<TcEngine<T, 80>>(a, st);
+      case 96: return launch_paged<TcEngine<T, 96>>(a, st);
+      case 128: return launch_paged<TcEngine<T, 128>>(a, st);
+      case 256: return launch_paged<TcEngine<T, 256>>(a, st);
+    }
+  }
+  return a.D <= 128 ? launch_paged<FmaEngine<T, 1>>(a, st) : launch_paged<FmaEngine<T, 2>>(a, st);
+}
+
 }  // namespace b200p
 
 using namespace b200p;
 
 extern "C" size_t b200p_paged_attn_workspace_bytes(int64_t M, int H, int D, int64_t keys) {
-  (void)D;
-  return M > 0 && H > 0 && keys > 0 ? (size_t)M * H * ((keys + PA_TILE - 1) / PA_TILE * PA_TILE) * sizeof(float) : 0;
+  if (M <= 0 || H <= 0 || D <= 0) return 0;
+  size_t n = base_bytes(M) + rec_bytes(D);
+  if (keys > 0) n += stat_bytes(M, H) + (size_t)M * H * ((keys + PA_TILE - 1) / PA_TILE * PA_TILE) * 4;
+  return n;
 }
 
 extern "C" int b200p_paged_attn(const void* q, const void* kpages, const void* vpages, float* mass, const int32_t* table, const int32_t* t_row,
@@ -247,12 +718,21 @@ extern "C" int b200p_paged_attn(const void* q, const void* kpages, const void* v
   B200P_REQUIRE((flags & ~B200P_OUT_PERM8) == 0, B200P_ERR_ARG, "unknown flags 0x%x", flags);
   B200P_REQUIRE(aligned(q, 16) && aligned(out, 16), B200P_ERR_ALIGN, "q and out must be 16-byte aligned");
   if (M == 0) return B200P_OK;
-  const int64_t slots = (int64_t)width * page, cap = visible_cap(slots, first, window);
-  B200P_REQUIRE(!mass || (workspace && workspace_bytes >= b200p_paged_attn_workspace_bytes(M, H, D, cap) && aligned(workspace, 16)), B200P_ERR_ARG,
-                "paged attention workspace too small");
-  const PagedAttn a{q,     kpages, vpages, out, mass, (float*)workspace, pt, t_row, t_slot, H, G, D, (int)(first < slots ? first : slots),
-                    (int)(window < slots ? window : slots), (int)cap, (flags & B200P_OUT_PERM8) ? 1 : 0, scale * 1.4426950408889634f};
-  if (D <= 128) B200P_DISPATCH_DTYPE(dtype, T, return (launch_any<T, 1>(a, M, (cudaStream_t)stream)));
-  B200P_DISPATCH_DTYPE(dtype, T, return (launch_any<T, 2>(a, M, (cudaStream_t)stream)));
+  const int64_t slots = (int64_t)width * page;
+  first = first < slots ? first : slots;
+  window = window < slots ? window : slots;
+  const int64_t cap = visible_cap(slots, first, window);
+  B200P_REQUIRE(workspace && workspace_bytes >= b200p_paged_attn_workspace_bytes(M, H, D, mass ? cap : 0) && aligned(workspace, 256), B200P_ERR_ARG,
+                "paged attention workspace too small or not aligned to 256 bytes");
+  PagedAttn a{};
+  a.q = q, a.k = kpages, a.v = vpages, a.out = out, a.mass = mass, a.pt = pt, a.t_row = t_row, a.t_slot = t_slot;
+  a.M = (int)M, a.H = H, a.G = G, a.D = D, a.first = (int)first, a.window = (int)window, a.out_perm = (flags & B200P_OUT_PERM8) ? 1 : 0;
+  a.scale_log2e = scale * 1.4426950408889634f, a.cap = (int)cap;
+  uint8_t* ws = (uint8_t*)workspace;
+  a.base = (int64_t*)ws;
+  a.rec = (float*)(ws += base_bytes(M));
+  a.stat = (float*)(ws += rec_bytes(D));
+  a.scores = (float*)(ws + stat_bytes(M, H));
+  B200P_DISPATCH_DTYPE(dtype, T, return (launch_paged_type<T>(a, (cudaStream_t)stream)));
   return B200P_OK;
 }

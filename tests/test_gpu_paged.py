@@ -207,7 +207,7 @@ def _check_attn(ops, c, q, row, slot, H, first, window, mass, scale, perm=False)
     ws = torch.full((max(16, n),), 0xa5, dtype=torch.uint8, device="cuda")
     ops.paged_attn(q.cuda(), k, v, table, row.cuda(), slot.cuda(), out, scale, first=first, window=window, mass=ms, workspace=ws, out_perm=perm)
     exp, tol, em, off = po.attn(q, c.k, c.v, c.mass if mass else None, c.table, row, slot, H, scale, first, window,
-                                0.0 if dt is torch.float32 else po.half_step(dt))
+                                0.0 if dt is torch.float32 else po.half_step(dt) ** 2)
     got = out.cpu().double().view(M, H, D)
     if perm:
         got = got.view(M, H, D // 8, 8)[..., [0, 2, 4, 6, 1, 3, 5, 7]].reshape(M, H, D)
@@ -490,7 +490,7 @@ def _decode(ops, dtype, steps, graph):
         at = [po.place(c.table, c.P, page, r, int(lengths[r])) for r in range(3)]
         for p, o in at:                                     # what the device stored is checked by the append's tests
             ok[p, :, o], ov[p, :, o], om[p, :, o] = k.cpu()[p, :, o], v.cpu()[p, :, o], 0.0
-        exp, tol, em, off = po.attn(q, ok, ov, om, c.table, rows, lengths, H, 0.25, 0, 0, 0.0 if dt is torch.float32 else po.half_step(dt))
+        exp, tol, em, off = po.attn(q, ok, ov, om, c.table, rows, lengths, H, 0.25, 0, 0, 0.0 if dt is torch.float32 else po.half_step(dt) ** 2)
         err = (d["out"].cpu().double().view(3, H, D) - exp).abs()
         assert bool((err <= tol + po.half_step(dt) * exp.abs() * 1.001 + 2.0 ** -25).all()), i
         assert bool(((ms.cpu().double() - em).abs() <= off).all()), i
