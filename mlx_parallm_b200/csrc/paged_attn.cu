@@ -45,6 +45,7 @@ struct Span {
   }
   __device__ int key0(int v) const { return (v < t0 ? v : v - t0 + skip) * PA_TILE; }
   __device__ bool visible(int j) const { return j < n && (j < first || j >= lo); }
+  __device__ bool whole(int j0) const { return j0 + PA_TILE <= n && (j0 >= lo || j0 + PA_TILE <= first); }
 };
 
 struct PagedAttn {
@@ -56,20 +57,22 @@ struct PagedAttn {
   int M, H, G, D, first, window, out_perm;
   float scale_log2e;
   // workspace
-  int64_t* base;       // [M + 1] units before every token; all units
-  float* stat;         // [M, H, 2] maximum and sum of the heads that one CTA took whole (with a mass)
+  unsigned* arrived;   // [CTAs] parts that are in, of the item that is cut first in this CTA: zero between calls
   float* rec;          // [CTAs, 2, rows of a block, D + 4] parts: maximum, sum, -, -, outputs
-  float* scores;       // [M, H, cap] log2-scaled scores (with a mass)
-  int cap;             // visible slots a token can have, in whole tiles
+  float* stat;         // [M, H, 2] maximum and 1 / sum of every head (with a mass)
+  float* scores;       // [M, items, cap, pitch] log2-scaled scores (with a mass)
+  int cap, pitch;      // visible slots a token can have, in whole tiles; heads of a line of scores, a power of two
 };
 
 // The work is cut evenly however unequal the rows are: every token's visible tiles are counted in units of one tile per warp, the units of all
 // (token, key head, block of query heads) items are laid end to end, and each of C CTAs takes the same number of them.  An item that lies in one
-// CTA's share is finished there; of one that is cut every CTA leaves a part, and paged_attn_join_kernel joins them.  (One CTA per item left the
-// GPU idle behind the longest rows: 64 rows of 130 to 500 tokens took 108 us, of 8192 tokens 940.)
+// CTA's share is finished there; of one that is cut every CTA leaves a part, and the CTA that comes last joins them, in their order (it reads
+// what the others left: nobody waits).  (One CTA per item left the GPU idle behind the longest rows: 64 rows of 130 to 500 tokens took 108 us,
+// 16 of 8192 940.  Joining in a second launch: one row of 1000 tokens 11.6 us.)
 struct Token {
   int row, units;
   Span span;
+  __device__ Token() : row(-1), units(0), span(0, 0, 0) {}
   __device__ Token(const PagedAttn& a, int t, int warps) : row(a.t_row[t]), units(0), span(0, 0, 0) {
     if (row >= 0 && row < a.pt.rows) {
       span = Span(slots_seen(a.pt, a.t_slot[t]), a.first, a.window);
@@ -77,9 +80,14 @@ struct Token {
     }
   }
 };
-// CTAs that share U units
-__device__ __forceinline__ int64_t shares(int64_t U, int most) { return U < most ? U : most; }
+// CTAs that share U units of n items; a join reads a part per CTA, one after the other, so that 64 of them are enough for an item
+__device__ __forceinline__ int64_t shares(int64_t U, int64_t n, int most) { return min(min(U, 64 * n), (int64_t)most); }
 __device__ __forceinline__ int64_t share_begin(int64_t U, int64_t C, int64_t c) { return U * c / C; }
+__device__ __forceinline__ int64_t share_of(int64_t U, int64_t C, int64_t u) {
+  int64_t c = u * C / U;
+  while (share_begin(U, C, c + 1) <= u) ++c;
+  return c;
+}
 
 // A position in a CTA's share: the token, and of its units the run [a, b) of one item.
 struct Cursor {
@@ -106,125 +114,139 @@ struct Cursor {
 // ------------------------------------------------------------------------------------------------ engines
 // What a warp does with a staged tile of 16 keys.  ROWS query heads of one key head share it, so keys and values are read once.
 
-// 16-bit types, D a multiple of 16: mma.sync m16n8k16, query heads as the 16 rows (of which 4 to 8 are in use: the kernel waits for its bytes, the
-// tensor cores idle either way).  The weights multiply the values as two 16-bit numbers each (the rounded weight and what it lost), so that
-// the output carries its own rounding only.
-template <typename T_, int D_>
+// 16-bit types, D a multiple of 16: mma.sync m16n8k16 with the 16 keys as its rows and the query heads as its columns, 8 (or, NB 2, 16) of them, so
+// that hardly a product is wasted on absent heads: S^T = K Q^T, O^T = V^T P^T.  (With the heads as the 16 rows the products and the registers
+// were twice as many.)  The weights multiply the values as two 16-bit numbers each (the rounded weight and what it lost), so that the output carries
+// its own rounding only.
+template <typename T_, int D_, int NB>
 struct TcEngine {
   using T = T_;
-  static constexpr int D = D_, ROWS = 16, WARPS = 4, STAGES = D_ > 128 ? 2 : 3;
+  static constexpr int D = D_, ROWS = 8 * NB, WARPS = 4, STAGES = D_ > 128 ? 2 : 3, CTAS = D_ > 128 ? 1 : 2;
   static constexpr int CHUNKS = D / 8, PIECES = CHUNKS % 8 ? (CHUNKS | 1) : CHUNKS;    // 16-byte pieces of a staged line
   static constexpr int Q_STRIDE = D * 2 + 16, Q_BYTES = ROWS * Q_STRIDE;
   static constexpr int NQ = (ROWS * CHUNKS + WARPS * 32 - 1) / (WARPS * 32);
   // f16: the largest weight of a tile is 2^14 and not 1 (m is the maximum less 14), so that small weights keep their bits
   static constexpr float SHIFT = std::is_same<T_, __half>::value ? 14.f : 0.f;
-  float o[D / 8][4], m[2], l[2];
-  uint32_t qf[D > 128 ? 1 : D / 16][4];
+  float o[NB][D / 16][4], m[NB][2], l[NB][2];                    // of the heads 8 nb + 2 qc and the next
+  uint32_t qf[NB][D / 16][2];
 
   static __device__ __forceinline__ int dim(const PagedAttn&) { return D; }
   static __host__ __device__ __forceinline__ int tile_bytes(int) { return 2 * PA_TILE * PIECES * 16; }
   static __device__ __forceinline__ uint32_t at(int key, int c) {
     return (uint32_t)(key * PIECES * 16 + ((CHUNKS % 8 ? c : c ^ (key & 7)) << 4));
   }
-  static __device__ __forceinline__ void q_frag(uint32_t qs, int ks, uint32_t (&f)[4]) {
-    const int lane = threadIdx.x & 31, mat = lane >> 3, r = lane & 7;
-    ldsm_x4(qs + (r + 8 * (mat & 1)) * Q_STRIDE + (2 * ks + (mat >> 1)) * 16, f);
-  }
   static __device__ __forceinline__ void put_q(uint8_t* qs, int r, int c, const uint4& x, int) {
     *reinterpret_cast<uint4*>(qs + r * Q_STRIDE + c * 16) = x;
   }
   __device__ __forceinline__ void begin(uint32_t qs) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
-    if constexpr (D <= 128) {
+    for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) q_frag(qs, ks, qf[ks]);
+      for (int j = 0; j < D / 16; ++j) o[nb][j][0] = o[nb][j][1] = o[nb][j][2] = o[nb][j][3] = 0.f;
+      m[nb][0] = m[nb][1] = -INFINITY;
+      l[nb][0] = l[nb][1] = 0.f;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t p = qs + (8 * nb + (lane >> 2)) * Q_STRIDE + k * 32 + (lane & 3) * 4;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(qf[nb][k][0]) : "r"(p));
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(qf[nb][k][1]) : "r"(p + 16));
+      }
     }
   }
-  __device__ __forceinline__ void tile(const PagedAttn& a, uint32_t qs, uint32_t ks, int j0, const Span& sp, bool all, bool page, float* sc, int rows,
+  __device__ __forceinline__ void tile(const PagedAttn& a, uint32_t, uint32_t ks, int j0, const Span& sp, bool all, bool page, float* sc, int rows,
                                        uint8_t*) {
     const int lane = threadIdx.x & 31, qr = lane >> 2, qc = lane & 3, mat = lane >> 3, r8 = lane & 7;
     const uint32_t vs = ks + PA_TILE * PIECES * 16;
-    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+    float s[NB][4];                                              // keys qr and qr + 8 of two heads
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      uint32_t bf[4], qt[4];
-      ldsm_x4(ks + at(r8 + 8 * (mat >> 1), 2 * k + (mat & 1)), bf);
-      if constexpr (D <= 128) {
-        mma16816<T>(s0, qf[k], bf[0], bf[1]);
-        mma16816<T>(s1, qf[k], bf[2], bf[3]);
-      } else {
-        q_frag(qs, k, qt);
-        mma16816<T>(s0, qt, bf[0], bf[1]);
-        mma16816<T>(s1, qt, bf[2], bf[3]);
+      uint32_t kf[4];
+      ldsm_x4(ks + at(r8 + 8 * (mat & 1), 2 * k + (mat >> 1)), kf);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) mma16816<T>(s[nb], kf, qf[nb][k][0], qf[nb][k][1]);
+    }
+    const bool seen0 = all || (page && sp.visible(j0 + qr)), seen1 = all || (page && sp.visible(j0 + qr + 8));
+    uint32_t hi[NB][2], lo[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float f[2], p[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x = seen0 ? s[nb][h] * a.scale_log2e : -INFINITY, y = seen1 ? s[nb][2 + h] * a.scale_log2e : -INFINITY;
+        s[nb][h] = x;
+        s[nb][2 + h] = y;
+        float t = fmaxf(x, y);
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+        t = fmaxf(t - SHIFT, m[nb][h]);
+        const float ref = t == -INFINITY ? 0.f : t;              // nothing seen yet
+        f[h] = exp2f(m[nb][h] - ref);
+        p[h] = exp2f(x - ref);
+        p[2 + h] = exp2f(y - ref);
+        m[nb][h] = t;
+        l[nb][h] = l[nb][h] * f[h] + (p[h] + p[2 + h]);
       }
-    }
-    // two rows (query heads qr and qr + 8) of four keys: 2 qc, 2 qc + 1 and the same + 8
-    float x[2][4] = {{s0[0], s0[1], s1[0], s1[1]}, {s0[2], s0[3], s1[2], s1[3]}};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool seen = all || (page && sp.visible(j0 + 2 * qc + (i & 1) + 8 * (i >> 1)));
-      x[0][i] = seen ? x[0][i] * a.scale_log2e : -INFINITY;
-      x[1][i] = seen ? x[1][i] * a.scale_log2e : -INFINITY;
-    }
-    if (sc) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (qr + 8 * h < rows) {
-          float* p = sc + (int64_t)(qr + 8 * h) * a.cap + 2 * qc;
-          *reinterpret_cast<float2*>(p) = make_float2(x[h][0], x[h][1]);
-          *reinterpret_cast<float2*>(p + 8) = make_float2(x[h][2], x[h][3]);
+      if (sc) {                                                  // lines of a.pitch heads, one per key
+        const int head = 8 * nb + 2 * qc;
+        if (head + 1 < a.pitch) {
+          *reinterpret_cast<float2*>(sc + qr * a.pitch + head) = make_float2(s[nb][0], s[nb][1]);
+          *reinterpret_cast<float2*>(sc + (qr + 8) * a.pitch + head) = make_float2(s[nb][2], s[nb][3]);
+        } else if (head < a.pitch) {
+          sc[qr * a.pitch] = s[nb][0];
+          sc[(qr + 8) * a.pitch] = s[nb][2];
         }
-    }
-    uint32_t hi[4], lo[4];
+      }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float t = fmaxf(fmaxf(x[h][0], x[h][1]), fmaxf(x[h][2], x[h][3]));
-      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-      t = fmaxf(t - SHIFT, m[h]);
-      const float ref = t == -INFINITY ? 0.f : t;                // nothing seen yet
-      const float f = exp2f(m[h] - ref);
-      float p[4];
+      for (int j = 0; j < D / 16; ++j) {
+        o[nb][j][0] *= f[0]; o[nb][j][1] *= f[1]; o[nb][j][2] *= f[0]; o[nb][j][3] *= f[1];
+      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = exp2f(x[h][i] - ref);
-      m[h] = t;
-      l[h] = l[h] * f + (p[0] + p[1]) + (p[2] + p[3]);
-#pragma unroll
-      for (int j = 0; j < D / 8; ++j) { o[j][2 * h] *= f; o[j][2 * h + 1] *= f; }
-      float q[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = p[i] - Tr<T>::to_f(Tr<T>::from_f(p[i]));
-      hi[h] = pack2<T>(p[0], p[1]);
-      hi[h + 2] = pack2<T>(p[2], p[3]);
-      lo[h] = pack2<T>(q[0], q[1]);
-      lo[h + 2] = pack2<T>(q[2], q[3]);
+      for (int i = 0; i < 2; ++i) {                              // 8 keys x 8 heads, turned to the operand's order
+        const float a0 = p[2 * i], a1 = p[2 * i + 1];
+        hi[nb][i] = transpose8(pack2<T>(a0, a1));
+        lo[nb][i] = transpose8(pack2<T>(a0 - Tr<T>::to_f(Tr<T>::from_f(a0)), a1 - Tr<T>::to_f(Tr<T>::from_f(a1))));
+      }
     }
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
-      uint32_t bf[4];
-      ldsm_x4_trans(vs + at(r8 + 8 * (mat & 1), 2 * j + (mat >> 1)), bf);
-      mma16816<T>(o[2 * j], hi, bf[0], bf[1]);
-      mma16816<T>(o[2 * j + 1], hi, bf[2], bf[3]);
-      mma16816<T>(o[2 * j], lo, bf[0], bf[1]);
-      mma16816<T>(o[2 * j + 1], lo, bf[2], bf[3]);
+      uint32_t vf[4];
+      ldsm_x4_trans(vs + at(r8 + 8 * (mat >> 1), 2 * j + (mat & 1)), vf);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        mma16816<T>(o[nb][j], vf, hi[nb][0], hi[nb][1]);
+        mma16816<T>(o[nb][j], vf, lo[nb][0], lo[nb][1]);
+      }
     }
   }
-  // rows [8 pass, 8 pass + 8) of this warp's part to p [8][D + 4]
+  static __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+  }
+  // heads [8 pass, 8 pass + 8) of this warp's part to p [8][D + 4]
   __device__ __forceinline__ void publish(float* p, int pass, int) {
     const int lane = threadIdx.x & 31, qr = lane >> 2, qc = lane & 3;
-    float* row = p + qr * (D + 4);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (h == pass) {
-        float sum = l[h];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (qc == 0) { row[0] = m[h]; row[1] = sum; }
+    for (int nb = 0; nb < NB; ++nb)
+      if (nb == pass) {
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(row + 4 + 8 * j + 2 * qc) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+        for (int h = 0; h < 2; ++h) {
+          float* row = p + (2 * qc + h) * (D + 4);
+          float sum = l[nb][h];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          if (qr == 0) { row[0] = m[nb][h]; row[1] = sum; }
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            row[4 + 16 * j + qr] = o[nb][j][h];
+            row[4 + 16 * j + 8 + qr] = o[nb][j][2 + h];
+          }
+        }
       }
   }
 };
@@ -233,7 +255,7 @@ struct TcEngine {
 template <typename T_, int NG>
 struct FmaEngine {
   using T = T_;
-  static constexpr int ROWS = 8, WARPS = sizeof(T_) == 4 && NG == 2 ? 2 : 4, STAGES = 2;
+  static constexpr int ROWS = 8, WARPS = sizeof(T_) == 4 && NG == 2 ? 2 : 4, STAGES = 2, CTAS = 1;
   static constexpr int E = 16 / (int)sizeof(T_);
   static constexpr int Q_BYTES = (ROWS * NG * 128 + WARPS * ROWS * PA_TILE) * 4;     // queries and every warp's weights, fp32
   static constexpr int NQ = (ROWS * NG * 128 / E + WARPS * 32 - 1) / (WARPS * 32);
@@ -288,7 +310,7 @@ struct FmaEngine {
       if (r >= rows) break;
       float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * a.scale_log2e;
       x = seen ? x : -INFINITY;
-      if (sc && half == 0) sc[(int64_t)r * a.cap + key] = x;
+      if (sc && half == 0) sc[key * a.pitch + r] = x;
       const float t = fmaxf(m[r], warp_max(x));
       const float ref = t == -INFINITY ? 0.f : t;
       const float f = exp2f(m[r] - ref), p = exp2f(x - ref);
@@ -331,7 +353,7 @@ struct FmaEngine {
 };
 
 template <typename E> struct IsTc { static constexpr bool value = false; };
-template <typename T, int D> struct IsTc<TcEngine<T, D>> { static constexpr bool value = true; };
+template <typename T, int D, int NB> struct IsTc<TcEngine<T, D, NB>> { static constexpr bool value = true; };
 
 template <typename T>
 __device__ __forceinline__ void store_row4(T* out, int d, float4 v, int perm) {
@@ -349,13 +371,14 @@ __device__ __forceinline__ void store_row4(T* out, int d, float4 v, int perm) {
 
 // ------------------------------------------------------------------------------------------------ the kernel
 template <typename E>
-__global__ void __launch_bounds__(E::WARPS * 32, 2)
+__global__ void __launch_bounds__(E::WARPS * 32, E::CTAS)
 paged_attn_kernel(const PagedAttn a) {
   using T = typename E::T;
   constexpr int W = E::WARPS, THREADS = W * 32;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t s_sum[W], s_base;
-  __shared__ int s_t, s_part[W];
+  __shared__ int s_t, s_part[W], s_live[W];
+  __shared__ bool s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = E::dim(a), chunks = D * (int)sizeof(T) / 16;
   const int per = a.H / a.G, blocks = (per + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
@@ -367,31 +390,33 @@ paged_attn_kernel(const PagedAttn a) {
   const int chunk = (a.M + THREADS - 1) / THREADS;
   const int t0 = min(a.M, (int)threadIdx.x * chunk), t1 = min(a.M, t0 + chunk);
   int64_t mine = 0;
-  for (int t = t0; t < t1; ++t) mine += (int64_t)Token(a, t, W).units * items;
+  int live = 0;
+  for (int t = t0; t < t1; ++t) {
+    const int n = Token(a, t, W).units;
+    mine += (int64_t)n * items;
+    live += n > 0;
+  }
   int64_t before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
     if (lane >= o) before += x;
   }
-  if (lane == 31) s_sum[warp] = before;
+  live = __reduce_add_sync(0xffffffffu, live);
+  if (lane == 31) {
+    s_sum[warp] = before;
+    s_live[warp] = live;
+  }
   __syncthreads();
   before -= mine;
-  int64_t U = 0;
+  int64_t U = 0, n_items = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
     if (w < warp) before += s_sum[w];
     U += s_sum[w];
+    n_items += (int64_t)s_live[w] * items;
   }
-  if (blockIdx.x == 0) {
-    int64_t x = before;
-    for (int t = t0; t < t1; ++t) {
-      a.base[t] = x;
-      x += (int64_t)Token(a, t, W).units * items;
-    }
-    if (threadIdx.x == 0) a.base[a.M] = U;
-  }
-  const int64_t C = shares(U, (int)gridDim.x);
+  const int64_t C = shares(U, n_items, (int)gridDim.x);
   if ((int64_t)blockIdx.x >= C) return;
   const int64_t ub = share_begin(U, C, blockIdx.x), ue = share_begin(U, C, blockIdx.x + 1);
   if (ub >= before && ub < before + mine) {
@@ -413,40 +438,46 @@ paged_attn_kernel(const PagedAttn a) {
   bool more = ld.next(a, items, W);
   int tile = ld.a * W + warp, tile_end = min(ld.b * W, ld.tok.span.tiles);
   unsigned paged = 0;                                             // stages whose keys have a page
-  auto issue = [&](int stage) {
+  int64_t id = -1;                                                // of the next tile: looked up a tile ahead
+  auto seek = [&]() {                                             // the next tile this warp loads
     while (more && tile >= tile_end) {
       more = ld.next(a, items, W);
       tile = ld.a * W + warp;
       tile_end = min(ld.b * W, ld.tok.span.tiles);
     }
+    if (more) id = page_id(a.pt, ld.tok.row, ld.tok.span.key0(tile) / a.pt.page);
+  };
+  auto issue = [&](int stage) {
     if (more) {
       const Span& sp = ld.tok.span;
       const int j0 = sp.key0(tile), g = ld.item / blocks;
-      const int64_t id = page_id(a.pt, ld.tok.row, j0 / a.pt.page);
       const int64_t line = ((id < 0 ? 0 : id) * a.G + g) * a.pt.page + j0 % a.pt.page;
       const uint4* kg = reinterpret_cast<const uint4*>(a.k) + line * chunks;
       const uint4* vg = reinterpret_cast<const uint4*>(a.v) + line * chunks;
       const uint32_t ks = ring32 + stage * E::tile_bytes(D), vs = ks + E::tile_bytes(D) / 2;
-      if (id < 0 && lane == 0) atomicAdd(&g_paged_attn_fault, 1u);
-      paged = (paged & ~(1u << stage)) | ((id >= 0 ? 1u : 0u) << stage);
+      const bool page = id >= 0, all = page && sp.whole(j0);
+      if (!page && lane == 0) atomicAdd(&g_paged_attn_fault, 1u);
+      paged = (paged & ~(1u << stage)) | ((page ? 1u : 0u) << stage);
       if constexpr (IsTc<E>::value) {
+        constexpr int N = PA_TILE * E::CHUNKS;
 #pragma unroll
-        for (int i = 0; i < (PA_TILE * E::CHUNKS + 31) / 32; ++i) {
+        for (int i = 0; i < (N + 31) / 32; ++i) {
           const int x = i * 32 + lane, key = x / E::CHUNKS, c = x % E::CHUNKS;
-          if (PA_TILE * E::CHUNKS % 32 && key >= PA_TILE) break;
-          const bool ok = id >= 0 && sp.visible(j0 + key);
+          if (N % 32 && x >= N) break;
+          const bool ok = all || (page && sp.visible(j0 + key));
           cp_async16(ks + E::at(key, c), kg + (ok ? x : 0), ok);
           cp_async16(vs + E::at(key, c), vg + (ok ? x : 0), ok);
         }
       } else {
         for (int x = lane; x < PA_TILE * chunks; x += 32) {
           const int key = x / chunks, c = x - key * chunks;
-          const bool ok = id >= 0 && sp.visible(j0 + key);
+          const bool ok = all || (page && sp.visible(j0 + key));
           cp_async16(ks + E::at(key, c, D), kg + (ok ? x : 0), ok);
           cp_async16(vs + E::at(key, c, D), vg + (ok ? x : 0), ok);
         }
       }
       tile += W;
+      seek();
     }
     cp_async_commit();
   };
@@ -470,6 +501,7 @@ paged_attn_kernel(const PagedAttn a) {
   };
   bool work = cu.next(a, items, W);
   fetch_q(cu);
+  seek();
 #pragma unroll
   for (int s = 0; s < E::STAGES - 1; ++s) issue(s);
   put_q();
@@ -484,6 +516,7 @@ paged_attn_kernel(const PagedAttn a) {
     const int g = me.item / blocks, r0 = (me.item - g * blocks) * E::ROWS, rows = min(E::ROWS, per - r0);
     const int64_t head = (int64_t)me.t * a.H + (int64_t)g * per + r0;
     const Span sp = me.tok.span;
+    float* scores = a.scores + ((int64_t)me.t * items + me.item) * a.cap * a.pitch;
     e.begin(qs);
     const int end = min(me.b * W, sp.tiles);
     for (int v = me.a * W + warp; v < end; v += W) {
@@ -492,8 +525,8 @@ paged_attn_kernel(const PagedAttn a) {
       __syncwarp();
       const int j0 = sp.key0(v);
       const bool page = (paged >> stage) & 1u;
-      const bool all = page && j0 + PA_TILE <= sp.n && (j0 >= sp.lo || j0 + PA_TILE <= sp.first);
-      e.tile(a, qs, ring32 + stage * E::tile_bytes(D), j0, sp, all, page, a.mass ? a.scores + head * a.cap + v * PA_TILE : nullptr, rows,
+      const bool all = page && sp.whole(j0);
+      e.tile(a, qs, ring32 + stage * E::tile_bytes(D), j0, sp, all, page, a.mass ? scores + (int64_t)v * PA_TILE * a.pitch : nullptr, rows,
              ring + stage * E::tile_bytes(D));
       __syncwarp();                                               // the stage is refilled by the next issue
       stage = stage + 1 == E::STAGES ? 0 : stage + 1;
@@ -502,7 +535,8 @@ paged_attn_kernel(const PagedAttn a) {
     const int part = (warp * E::STAGES + (stage == 0 ? E::STAGES - 1 : stage - 1)) * E::tile_bytes(D);
     if (lane == 0) s_part[warp] = part;
     const bool whole = me.a == 0 && me.b == me.tok.units;
-    float* rec = a.rec + (((int64_t)blockIdx.x * 2 + (me.a == 0 ? 1 : 0)) * E::ROWS) * (D + 4);
+    const int64_t part_size = (int64_t)E::ROWS * (D + 4);
+    float* rec = a.rec + ((int64_t)blockIdx.x * 2 + (me.a == 0 ? 1 : 0)) * part_size;
     for (int pass = 0; pass * 8 < rows; ++pass) {
       e.publish(reinterpret_cast<float*>(smem + E::Q_BYTES + part), pass, D);
       __syncthreads();
@@ -536,105 +570,90 @@ paged_attn_kernel(const PagedAttn a) {
       }
       __syncthreads();
     }
+    if (whole) continue;
+    // ---- an item that is cut: the last of its CTAs joins the parts ----------------------------------------------------------
+    const int64_t u0 = me.base + (int64_t)me.item * me.tok.units, c0 = share_of(U, C, u0), c1 = share_of(U, C, u0 + me.tok.units - 1);
+    const int parts = (int)(c1 - c0) + 1;
+    if (threadIdx.x == 0) {
+      __threadfence();                                            // (the barrier before: every thread's part of the record)
+      const bool last = atomicAdd(a.arrived + c0, 1u) == (unsigned)(parts - 1);
+      if (last) {
+        a.arrived[c0] = 0;                                        // as it was found
+        __threadfence();
+      }
+      s_last = last;
+    }
+    __syncthreads();
+    if (!s_last) continue;
+    const float* first = a.rec + (c0 * 2 + 1) * part_size;
+    const float* other = a.rec + (c0 + 1) * 2 * part_size;       // of part i > 0: + (i - 1) * 2 * part_size
+    const int quads = D / 4;
+    for (int x = threadIdx.x; x < rows * quads; x += THREADS) {
+      const int r = x / quads, d = (x - r * quads) * 4;
+      float M = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      constexpr int AHEAD = 8;
+      for (int i0 = 0; i0 < parts; i0 += AHEAD) {
+        float2 ml[AHEAD];
+        float4 y[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const float* p = (i0 + i == 0 ? first : other + (int64_t)(i0 + i - 1) * 2 * part_size) + r * (D + 4);
+          ml[i] = i0 + i < parts ? __ldcg(reinterpret_cast<const float2*>(p)) : make_float2(-INFINITY, 0.f);
+          y[i] = i0 + i < parts ? __ldcg(reinterpret_cast<const float4*>(p + 4 + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
+        const float ref = top == -INFINITY ? 0.f : top, f = exp2f(M - ref);
+        M = top;
+        L *= f;
+        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const float w = exp2f(ml[i].x - ref);
+          L += ml[i].y * w;
+          acc.x += y[i].x * w; acc.y += y[i].y * w; acc.z += y[i].z * w; acc.w += y[i].w * w;
+        }
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      store_row4<T>(reinterpret_cast<T*>(a.out) + (head + r) * D, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv), a.out_perm);
+      if (a.mass && d == 0) *reinterpret_cast<float2*>(a.stat + (head + r) * 2) = make_float2(M == -INFINITY ? 0.f : M, inv);
+    }
   }
   cp_async_wait<0>();
 }
 
-// One CTA per item (x) that was cut: a warp joins the parts of a query head, several warps share a head's parts where the heads are few.  With
-// a mass (y: slices of the visible slots) every CTA forms the heads' maxima and sums anew and adds its slice's weights up.
-constexpr int PJ_WARPS = 8, PJ_SLICE = 1024;
+// The weights that every visible slot received: a CTA per item (x) and slice of its visible slots (y), a thread per slot.
+constexpr int PM_THREADS = 256;
 
-template <typename E>
-__global__ void __launch_bounds__(PJ_WARPS * 32)
-paged_attn_join_kernel(const PagedAttn a, int most) {
-  using T = typename E::T;
-  extern __shared__ __align__(16) float sm[];                     // [PJ_WARPS][D + 4], then [ROWS][2]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = E::dim(a);
-  float* stat = sm + PJ_WARPS * (D + 4);
-  const int per = a.H / a.G, blocks = (per + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
+template <int ROWS>
+__global__ void __launch_bounds__(PM_THREADS)
+paged_attn_mass_kernel(const PagedAttn a, int warps) {
+  const int per = a.H / a.G, blocks = (per + ROWS - 1) / ROWS, items = a.G * blocks;
   const int t = blockIdx.x / items, item = blockIdx.x - t * items;
-  const int g = item / blocks, r0 = (item - g * blocks) * E::ROWS, rows = min(E::ROWS, per - r0);
+  const int g = item / blocks, r0 = (item - g * blocks) * ROWS, rows = min(ROWS, per - r0);
   pdl_wait();
-  const Token tok(a, t, E::WARPS);
-  if (tok.units == 0) return;
-  if (blockIdx.y > 0 && (int)blockIdx.y * PJ_SLICE >= tok.span.tiles * PA_TILE) return;
-  const bool outputs = blockIdx.y == 0;
-  const int64_t U = a.base[a.M], C = shares(U, most), u0 = a.base[t] + (int64_t)item * tok.units, u1 = u0 + tok.units;
-  int64_t c0 = u0 * C / U, c1 = (u1 - 1) * C / U;
-  while (share_begin(U, C, c0 + 1) <= u0) ++c0;
-  while (share_begin(U, C, c1 + 1) <= u1 - 1) ++c1;
-  const int64_t head = (int64_t)t * a.H + (int64_t)g * per + r0;
-  const bool cut = c0 != c1;
-  if (!cut && !a.mass) return;
-  if (cut) {
-    const int parts = (int)(c1 - c0 + 1), quads = D / 4;
-    const int ways = rows >= PJ_WARPS ? 1 : PJ_WARPS / rows;      // warps per head
-    for (int rb = 0; rb < rows; rb += PJ_WARPS / ways) {
-      const int r = rb + warp / ways, way = warp - warp / ways * ways;
-      const bool mine = warp < PJ_WARPS / ways * ways && r < rows;
-      float M = -INFINITY, L = 0.f;
-      float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-      if (mine) {
-        auto part = [&](int i) { return a.rec + (((c0 + i) * 2 + (i == 0 ? 1 : 0)) * E::ROWS + r) * (D + 4); };
-        for (int i = way; i < parts; i += ways) M = fmaxf(M, part(i)[0]);
-        const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
-        for (int i = way; i < parts; i += ways) {
-          const float* p = part(i);
-          const float f = exp2f(p[0] - ref);
-          L += p[1] * f;
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            if (outputs && lane + 32 * x < quads) {
-              const float4 y = *reinterpret_cast<const float4*>(p + 4 + (lane + 32 * x) * 4);
-              acc[x].x += y.x * f; acc[x].y += y.y * f; acc[x].z += y.z * f; acc[x].w += y.w * f;
-            }
-        }
-        float* p = sm + warp * (D + 4);
-        if (lane == 0) { p[0] = M; p[1] = L; }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (outputs && lane + 32 * x < quads) *reinterpret_cast<float4*>(p + 4 + (lane + 32 * x) * 4) = acc[x];
-      }
-      __syncthreads();
-      if (mine && way == 0) {
-        M = -INFINITY, L = 0.f;
-        for (int w = 0; w < ways; ++w) M = fmaxf(M, sm[(warp + w) * (D + 4)]);
-        const float ref = M == -INFINITY ? 0.f : M;
-        for (int w = 0; w < ways; ++w) L += sm[(warp + w) * (D + 4) + 1] * exp2f(sm[(warp + w) * (D + 4)] - ref);
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        if (lane == 0) { stat[2 * r] = ref; stat[2 * r + 1] = inv; }
-        if (outputs)
-          for (int x = lane; x < quads; x += 32) {
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = 0; w < ways; ++w) {
-              const float* p = sm + (warp + w) * (D + 4);
-              const float f = exp2f(p[0] - ref) * inv;
-              const float4 y = *reinterpret_cast<const float4*>(p + 4 + x * 4);
-              s.x += y.x * f; s.y += y.y * f; s.z += y.z * f; s.w += y.w * f;
-            }
-            store_row4<T>(reinterpret_cast<T*>(a.out) + (head + r) * D, x * 4, s, a.out_perm);
-          }
-      }
-      __syncthreads();
-    }
-  } else {
-    if ((int)threadIdx.x < 2 * rows) stat[threadIdx.x] = a.stat[head * 2 + threadIdx.x];
-    __syncthreads();
-  }
-  if (!a.mass) return;
-  const float* sc = a.scores + head * a.cap;
+  const Token tok(a, t, warps);
   const int seen = tok.span.tiles * PA_TILE;
-  for (int v0 = blockIdx.y * PJ_SLICE; v0 < seen; v0 += gridDim.y * PJ_SLICE)
-    for (int x = v0 + threadIdx.x; x < min(seen, v0 + PJ_SLICE); x += PJ_WARPS * 32) {
-      const int j = tok.span.key0(x / PA_TILE) + x % PA_TILE;
-      if (!tok.span.visible(j)) continue;
-      const int64_t id = page_id(a.pt, tok.row, j / a.pt.page);
-      if (id < 0) continue;
-      float w = 0.f;
-      for (int r = 0; r < rows; ++r) w += exp2f(sc[(int64_t)r * a.cap + x] - stat[2 * r]) * stat[2 * r + 1];
-      atomicAdd(&a.mass[(id * a.G + g) * a.pt.page + j % a.pt.page], w);    // slots that several tokens see
-    }
+  if ((int)blockIdx.y * PM_THREADS >= seen) return;
+  const float2* stat = reinterpret_cast<const float2*>(a.stat) + (int64_t)t * a.H + (int64_t)g * per + r0;
+  const float* sc = a.scores + (int64_t)blockIdx.x * a.cap * a.pitch;
+  float2 st[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) st[r] = r < rows ? stat[r] : make_float2(0.f, 0.f);
+  for (int x = blockIdx.y * PM_THREADS + threadIdx.x; x < seen; x += gridDim.y * PM_THREADS) {
+    const int j = tok.span.key0(x / PA_TILE) + x % PA_TILE;
+    if (!tok.span.visible(j)) continue;
+    const int64_t id = page_id(a.pt, tok.row, j / a.pt.page);
+    if (id < 0) continue;
+    const float* s = sc + (int64_t)x * a.pitch;
+    float w = 0.f;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (r < rows) w += exp2f(s[r] - st[r].x) * st[r].y;
+    atomicAdd(&a.mass[(id * a.G + g) * a.pt.page + j % a.pt.page], w);    // slots that several tokens see
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -647,7 +666,7 @@ static int64_t visible_cap(int64_t slots, int64_t first, int64_t window) {
 }
 
 static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-static size_t base_bytes(int64_t M) { return round256((size_t)(M + 1) * 8); }
+constexpr size_t PA_ARRIVED = 4096;                               // bytes
 static size_t rec_bytes(int D) { return round256((size_t)sm_count() * PA_CTAS * 2 * 16 * (D + 4) * 4); }
 static size_t stat_bytes(int64_t M, int H) { return round256((size_t)M * H * 8); }
 
@@ -669,25 +688,29 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   const int ctas = sm_count() * (2 * (smem + 1024 + 256) <= 228 * 1024 ? 2 : 1);
   const int64_t most = (int64_t)a.M * items * ((a.cap / PA_TILE + E::WARPS - 1) / E::WARPS);
   const int grid = (int)(most < ctas ? most : ctas);
+  B200P_REQUIRE(grid <= (int)(PA_ARRIVED / 4), B200P_ERR_ARCH, "%d SMs", sm_count());
+  a.pitch = 1;
+  while (a.pitch < E::ROWS && a.pitch < a.H / a.G) a.pitch *= 2;
   launch_pdl(kern, (unsigned)grid, E::WARPS * 32, smem, st, a);
   B200P_LAUNCH_CHECK("paged_attn_kernel");
-  // slices of a mass: as many as there are, but no more CTAs than fill the GPU
-  const int64_t slices = a.mass ? (a.cap + PJ_SLICE - 1) / PJ_SLICE : 1, fill = 8ll * sm_count() / ((int64_t)a.M * items) + 1;
-  launch_pdl(paged_attn_join_kernel<E>, dim3((unsigned)(a.M * items), (unsigned)(slices < fill ? slices : fill)), PJ_WARPS * 32, (PJ_WARPS * (a.D + 4) + 2 * E::ROWS) * 4, st, a,
-             grid);
-  B200P_LAUNCH_CHECK("paged_attn_join_kernel");
+  if (!a.mass) return B200P_OK;
+  // slices: as many as there are, but no more CTAs than fill the GPU
+  const int64_t slices = (a.cap + PM_THREADS - 1) / PM_THREADS, fill = 8ll * sm_count() / ((int64_t)a.M * items) + 1;
+  launch_pdl(paged_attn_mass_kernel<E::ROWS>, dim3((unsigned)(a.M * items), (unsigned)(slices < fill ? slices : fill)), PM_THREADS, 0, st, a, (int)E::WARPS);
+  B200P_LAUNCH_CHECK("paged_attn_mass_kernel");
   return B200P_OK;
 }
 
 template <typename T>
 static int launch_paged_type(const PagedAttn& a, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
+    const bool few = a.H / a.G <= 8;
     switch (a.D) {
-      case 64: return launch_paged<TcEngine<T, 64>>(a, st);
-      case 80: return launch_paged<TcEngine<T, 80>>(a, st);
-      case 96: return launch_paged<TcEngine<T, 96>>(a, st);
-      case 128: return launch_paged<TcEngine<T, 128>>(a, st);
-      case 256: return launch_paged<TcEngine<T, 256>>(a, st);
+      case 64: return few ? launch_paged<TcEngine<T, 64, 1>>(a, st) : launch_paged<TcEngine<T, 64, 2>>(a, st);
+      case 80: return few ? launch_paged<TcEngine<T, 80, 1>>(a, st) : launch_paged<TcEngine<T, 80, 2>>(a, st);
+      case 96: return few ? launch_paged<TcEngine<T, 96, 1>>(a, st) : launch_paged<TcEngine<T, 96, 2>>(a, st);
+      case 128: return few ? launch_paged<TcEngine<T, 128, 1>>(a, st) : launch_paged<TcEngine<T, 128, 2>>(a, st);
+      case 256: return launch_paged<TcEngine<T, 256, 1>>(a, st);     // (16 heads do not fit the registers)
     }
   }
   return a.D <= 128 ? launch_paged<FmaEngine<T, 1>>(a, st) : launch_paged<FmaEngine<T, 2>>(a, st);
@@ -699,8 +722,8 @@ using namespace b200p;
 
 extern "C" size_t b200p_paged_attn_workspace_bytes(int64_t M, int H, int D, int64_t keys) {
   if (M <= 0 || H <= 0 || D <= 0) return 0;
-  size_t n = base_bytes(M) + rec_bytes(D);
-  if (keys > 0) n += stat_bytes(M, H) + (size_t)M * H * ((keys + PA_TILE - 1) / PA_TILE * PA_TILE) * 4;
+  size_t n = PA_ARRIVED + rec_bytes(D);
+  if (keys > 0) n += stat_bytes(M, H) + (size_t)M * H * 2 * ((keys + PA_TILE - 1) / PA_TILE * PA_TILE) * 4;     // (pitch < 2 x heads)
   return n;
 }
 
@@ -729,8 +752,8 @@ extern "C" int b200p_paged_attn(const void* q, const void* kpages, const void* v
   a.M = (int)M, a.H = H, a.G = G, a.D = D, a.first = (int)first, a.window = (int)window, a.out_perm = (flags & B200P_OUT_PERM8) ? 1 : 0;
   a.scale_log2e = scale * 1.4426950408889634f, a.cap = (int)cap;
   uint8_t* ws = (uint8_t*)workspace;
-  a.base = (int64_t*)ws;
-  a.rec = (float*)(ws += base_bytes(M));
+  a.arrived = (unsigned*)ws;
+  a.rec = (float*)(ws += PA_ARRIVED);
   a.stat = (float*)(ws += rec_bytes(D));
   a.scores = (float*)(ws + stat_bytes(M, H));
   B200P_DISPATCH_DTYPE(dtype, T, return (launch_paged_type<T>(a, (cudaStream_t)stream)));
