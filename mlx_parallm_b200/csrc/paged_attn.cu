@@ -32,6 +32,15 @@ int paged_attn_faults(unsigned int* count, int reset, cudaStream_t st) {
 
 constexpr int PA_TILE = 16;      // keys of a tile: never across a page
 
+__device__ __forceinline__ float raise2(float x) {                // 2^x, to 2 steps of fp32; results below 2^-126 become 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // The tiles a token reads: those that hold first slots, then those from the window's beginning on.
 struct Span {
   int n, lo, first;              // slots; the window's beginning (0: everything is visible)
@@ -43,7 +52,8 @@ struct Span {
     skip = lo / PA_TILE > t0 ? lo / PA_TILE : t0;
     tiles = n > 0 ? t0 + (n + PA_TILE - 1) / PA_TILE - skip : 0;
   }
-  __device__ int key0(int v) const { return (v < t0 ? v : v - t0 + skip) * PA_TILE; }
+  __device__ int key_tile(int v) const { return v < t0 ? v : v - t0 + skip; }
+  __device__ int key0(int v) const { return key_tile(v) * PA_TILE; }
   __device__ bool visible(int j) const { return j < n && (j < first || j >= lo); }
   __device__ bool whole(int j0) const { return j0 + PA_TILE <= n && (j0 >= lo || j0 + PA_TILE <= first); }
 };
@@ -61,6 +71,8 @@ struct PagedAttn {
   float* rec;          // [CTAs, 2, rows of a block, D + 4] parts: maximum, sum, -, -, outputs
   float* stat;         // [M, H, 2] maximum and 1 / sum of every head (with a mass)
   float* scores;       // [M, items, cap, pitch] log2-scaled scores (with a mass)
+  uint64_t inv_tpp;    // 2^40 / (tiles of a page), rounded up: tile * inv_tpp >> 40 is the page's index for any tile below 2^26
+  int tpp;
   int cap, pitch;      // visible slots a token can have, in whole tiles; heads of a line of scores, a power of two
 };
 
@@ -184,9 +196,9 @@ struct TcEngine {
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
         t = fmaxf(t - SHIFT, m[nb][h]);
         const float ref = t == -INFINITY ? 0.f : t;              // nothing seen yet
-        f[h] = exp2f(m[nb][h] - ref);
-        p[h] = exp2f(x - ref);
-        p[2 + h] = exp2f(y - ref);
+        f[h] = raise2(m[nb][h] - ref);
+        p[h] = raise2(x - ref);
+        p[2 + h] = raise2(y - ref);
         m[nb][h] = t;
         l[nb][h] = l[nb][h] * f[h] + (p[h] + p[2 + h]);
       }
@@ -200,9 +212,11 @@ struct TcEngine {
           sc[(qr + 8) * a.pitch] = s[nb][2];
         }
       }
+      if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {  // a maximum grew (or is not a number)
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        o[nb][j][0] *= f[0]; o[nb][j][1] *= f[1]; o[nb][j][2] *= f[0]; o[nb][j][3] *= f[1];
+        for (int j = 0; j < D / 16; ++j) {
+          o[nb][j][0] *= f[0]; o[nb][j][1] *= f[1]; o[nb][j][2] *= f[0]; o[nb][j][3] *= f[1];
+        }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {                              // 8 keys x 8 heads, turned to the operand's order
@@ -313,7 +327,7 @@ struct FmaEngine {
       if (sc && half == 0) sc[key * a.pitch + r] = x;
       const float t = fmaxf(m[r], warp_max(x));
       const float ref = t == -INFINITY ? 0.f : t;
-      const float f = exp2f(m[r] - ref), p = exp2f(x - ref);
+      const float f = raise2(m[r] - ref), p = raise2(x - ref);
       m[r] = t;
       l[r] = l[r] * f + warp_sum(half == 0 ? p : 0.f);
       if (half == 0) ps[r * PA_TILE + key] = p;
@@ -438,42 +452,55 @@ paged_attn_kernel(const PagedAttn a) {
   bool more = ld.next(a, items, W);
   int tile = ld.a * W + warp, tile_end = min(ld.b * W, ld.tok.span.tiles);
   unsigned paged = 0;                                             // stages whose keys have a page
-  int64_t id = -1;                                                // of the next tile: looked up a tile ahead
+  int id = -1, off = 0;                                           // the next tile's page, looked up a tile ahead, and its tile in it
   auto seek = [&]() {                                             // the next tile this warp loads
     while (more && tile >= tile_end) {
       more = ld.next(a, items, W);
       tile = ld.a * W + warp;
       tile_end = min(ld.b * W, ld.tok.span.tiles);
     }
-    if (more) id = page_id(a.pt, ld.tok.row, ld.tok.span.key0(tile) / a.pt.page);
+    if (more) {
+      const int kt = ld.tok.span.key_tile(tile), index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 40);
+      off = kt - index * a.tpp;
+      id = __ldg(a.pt.table + (int64_t)ld.tok.row * a.pt.width + index);
+    }
   };
   auto issue = [&](int stage) {
     if (more) {
       const Span& sp = ld.tok.span;
-      const int j0 = sp.key0(tile), g = ld.item / blocks;
-      const int64_t line = ((id < 0 ? 0 : id) * a.G + g) * a.pt.page + j0 % a.pt.page;
-      const uint4* kg = reinterpret_cast<const uint4*>(a.k) + line * chunks;
-      const uint4* vg = reinterpret_cast<const uint4*>(a.v) + line * chunks;
+      const int j0 = sp.key0(tile);
+      const bool page = (unsigned)id < (unsigned)a.pt.P, all = page && sp.whole(j0);
+      const int64_t line = (((int64_t)(page ? id : 0) * a.G + ld.item / blocks) * a.tpp + off) * PA_TILE;
+      const uint4* kg = reinterpret_cast<const uint4*>(a.k) + line * chunks + lane;
+      const uint4* vg = reinterpret_cast<const uint4*>(a.v) + line * chunks + lane;
       const uint32_t ks = ring32 + stage * E::tile_bytes(D), vs = ks + E::tile_bytes(D) / 2;
-      const bool page = id >= 0, all = page && sp.whole(j0);
-      if (!page && lane == 0) atomicAdd(&g_paged_attn_fault, 1u);
       paged = (paged & ~(1u << stage)) | ((page ? 1u : 0u) << stage);
+      if (!page && lane == 0) atomicAdd(&g_paged_attn_fault, 1u);
       if constexpr (IsTc<E>::value) {
         constexpr int N = PA_TILE * E::CHUNKS;
+        if (all) {
 #pragma unroll
-        for (int i = 0; i < (N + 31) / 32; ++i) {
-          const int x = i * 32 + lane, key = x / E::CHUNKS, c = x % E::CHUNKS;
-          if (N % 32 && x >= N) break;
-          const bool ok = all || (page && sp.visible(j0 + key));
-          cp_async16(ks + E::at(key, c), kg + (ok ? x : 0), ok);
-          cp_async16(vs + E::at(key, c), vg + (ok ? x : 0), ok);
+          for (int i = 0; i < N / 32; ++i) {
+            const uint32_t at = E::at((i * 32 + lane) / E::CHUNKS, (i * 32 + lane) % E::CHUNKS);
+            copy16(ks + at, kg + i * 32);
+            copy16(vs + at, vg + i * 32);
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < N / 32; ++i) {
+            const int key = (i * 32 + lane) / E::CHUNKS;
+            const uint32_t at = E::at(key, (i * 32 + lane) % E::CHUNKS);
+            const bool ok = page && sp.visible(j0 + key);
+            cp_async16(ks + at, ok ? kg + i * 32 : kg, ok);
+            cp_async16(vs + at, ok ? vg + i * 32 : vg, ok);
+          }
         }
       } else {
         for (int x = lane; x < PA_TILE * chunks; x += 32) {
           const int key = x / chunks, c = x - key * chunks;
           const bool ok = all || (page && sp.visible(j0 + key));
-          cp_async16(ks + E::at(key, c, D), kg + (ok ? x : 0), ok);
-          cp_async16(vs + E::at(key, c, D), vg + (ok ? x : 0), ok);
+          cp_async16(ks + E::at(key, c, D), kg + (ok ? x - lane : 0), ok);
+          cp_async16(vs + E::at(key, c, D), vg + (ok ? x - lane : 0), ok);
         }
       }
       tile += W;
@@ -552,7 +579,7 @@ paged_attn_kernel(const PagedAttn a) {
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           const float* p = reinterpret_cast<const float*>(smem + E::Q_BYTES + s_part[w]) + r * (D + 4);
-          const float f = exp2f(p[0] - ref);
+          const float f = raise2(p[0] - ref);
           const float4 y = *reinterpret_cast<const float4*>(p + 4 + d);
           L += p[1] * f;
           acc.x += y.x * f; acc.y += y.y * f; acc.z += y.z * f; acc.w += y.w * f;
@@ -605,13 +632,13 @@ paged_attn_kernel(const PagedAttn a) {
         float top = M;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
-        const float ref = top == -INFINITY ? 0.f : top, f = exp2f(M - ref);
+        const float ref = top == -INFINITY ? 0.f : top, f = raise2(M - ref);
         M = top;
         L *= f;
         acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-          const float w = exp2f(ml[i].x - ref);
+          const float w = raise2(ml[i].x - ref);
           L += ml[i].y * w;
           acc.x += y[i].x * w; acc.y += y[i].y * w; acc.z += y[i].z * w; acc.w += y[i].w * w;
         }
@@ -651,7 +678,7 @@ paged_attn_mass_kernel(const PagedAttn a, int warps) {
     float w = 0.f;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
-      if (r < rows) w += exp2f(s[r] - st[r].x) * st[r].y;
+      if (r < rows) w += raise2(s[r] - st[r].x) * st[r].y;
     atomicAdd(&a.mass[(id * a.G + g) * a.pt.page + j % a.pt.page], w);    // slots that several tokens see
   }
 }
@@ -689,6 +716,8 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   const int64_t most = (int64_t)a.M * items * ((a.cap / PA_TILE + E::WARPS - 1) / E::WARPS);
   const int grid = (int)(most < ctas ? most : ctas);
   B200P_REQUIRE(grid <= (int)(PA_ARRIVED / 4), B200P_ERR_ARCH, "%d SMs", sm_count());
+  a.tpp = a.pt.page / PA_TILE;
+  a.inv_tpp = ((1ull << 40) + a.tpp - 1) / a.tpp;
   a.pitch = 1;
   while (a.pitch < E::ROWS && a.pitch < a.H / a.G) a.pitch *= 2;
   launch_pdl(kern, (unsigned)grid, E::WARPS * 32, smem, st, a);
