@@ -648,8 +648,7 @@ int b200p_paged_append(void* qkv, int64_t ldq, void* q_out, void* kpages, void* 
  * (flags = B200P_OUT_PERM8: PERM8 order).  A token that sees nothing gets zeros.  mass (NULL: none): every visible slot's mass grows by
  * the weights that the query heads of its key head gave it; slots that several tokens of one call see receive their sums in no fixed order.
  * Hidden keys and values are not read.  workspace: b200p_paged_attn_workspace_bytes(M, H, D, keys), keys = width * page with a mass,
- * 0 without, aligned to 256 bytes.  Its first 4096 bytes are counters that have to be zero when it is first used; every call leaves them zero, the
- * rest needs no initial state.  One workspace serves one stream at a time, and calls of any sizes in turn. */
+ * 0 without, aligned to 256 bytes; it needs no initial state and serves one stream at a time. */
 int b200p_paged_attn(const void* q, const void* kpages, const void* vpages, float* mass, const int32_t* table, const int32_t* t_row,
                      const int32_t* t_slot, void* out, int64_t M, int H, int G, int D, int64_t P, int page, int rows, int width, float scale,
                      int64_t first, int64_t window, int dtype, int flags, void* workspace, size_t workspace_bytes, void* stream);

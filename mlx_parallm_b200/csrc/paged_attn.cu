@@ -37,6 +37,7 @@ __device__ __forceinline__ float raise2(float x) {                // 2^x, to 2 s
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -45,6 +46,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
 struct Span {
   int n, lo, first;              // slots; the window's beginning (0: everything is visible)
   int t0, skip, tiles;           // tiles before the gap, the tile behind it, tiles in all
+  Span() = default;
   __host__ __device__ Span(int n_, int first_, int window) : n(n_), first(first_) {
     lo = window > 0 && n > window ? n - window : 0;
     const int f = first < lo ? first : lo;
@@ -67,9 +69,9 @@ struct PagedAttn {
   int M, H, G, D, first, window, out_perm;
   float scale_log2e;
   // workspace
-  unsigned* arrived;   // [CTAs] parts that are in, of the item that is cut first in this CTA: zero between calls
-  float* rec;          // [CTAs, 2, rows of a block, D + 4] parts: maximum, sum, -, -, outputs
-  float* stat;         // [M, H, 2] maximum and 1 / sum of every head (with a mass)
+  unsigned* base;      // [M + 2] units before every token; all units; items
+  float* rec;          // [shares, 2, rows of a block, D + 4] parts: maximum, sum, -, -, outputs
+  float* stat;         // [M, H, 2] maximum and 1 / sum of the heads that lie in one share (with a mass)
   float* scores;       // [M, items, cap, pitch] log2-scaled scores (with a mass)
   uint64_t inv_tpp;    // 2^40 / (tiles of a page), rounded up: tile * inv_tpp >> 40 is the page's index for any tile below 2^26
   int tpp;
@@ -77,50 +79,76 @@ struct PagedAttn {
 };
 
 // The work is cut evenly however unequal the rows are: every token's visible tiles are counted in units of one tile per warp, the units of all
-// (token, key head, block of query heads) items are laid end to end, and each of C CTAs takes the same number of them.  An item that lies in one
-// CTA's share is finished there; of one that is cut every CTA leaves a part, and the CTA that comes last joins them, in their order (it reads
-// what the others left: nobody waits).  (One CTA per item left the GPU idle behind the longest rows: 64 rows of 130 to 500 tokens took 108 us,
-// 16 of 8192 940.  Joining in a second launch: one row of 1000 tokens 11.6 us.)
+// (token, key head, block of query heads) items are laid end to end, and each CTA takes an equal share of that line.  An item that lies in one share is
+// finished there; of one that is cut every share leaves a part, and a second launch joins them.  (One CTA per item left the GPU idle behind the longest
+// rows: 64 rows of 130 to 500 tokens took 108 us, 16 of 8192 940.  Joining in the CTA whose part comes last, by counters, cost a row of 1000 tokens 3.7 us
+// of fences and atomics in a row; the second launch costs it less.  Small shares for whoever comes first, since SMs differ by a quarter in what they get of
+// the memory's bandwidth, cost more in parts than they evened out.)
 struct Token {
   int row, units;
   Span span;
   __device__ Token() : row(-1), units(0), span(0, 0, 0) {}
-  __device__ Token(const PagedAttn& a, int t, int warps) : row(a.t_row[t]), units(0), span(0, 0, 0) {
-    if (row >= 0 && row < a.pt.rows) {
-      span = Span(slots_seen(a.pt, a.t_slot[t]), a.first, a.window);
+  __device__ Token(const PagedAttn& a, int row_, int slots, int warps) : row(row_), units(0), span(0, 0, 0) {
+    if (row >= 0) {
+      span = Span(slots, a.first, a.window);
       units = span.tiles > warps ? (span.tiles + warps - 1) / warps : 1;      // a token that sees nothing: one, for its zeros
     }
   }
+  __device__ Token(const PagedAttn& a, int t, int warps) : Token() {
+    const int r = a.t_row[t];
+    if (r >= 0 && r < a.pt.rows) *this = Token(a, r, slots_seen(a.pt, a.t_slot[t]), warps);
+  }
 };
-// CTAs that share U units of n items; a join reads a part per CTA, one after the other, so that 64 of them are enough for an item
-__device__ __forceinline__ int64_t shares(int64_t U, int64_t n, int most) { return min(min(U, 64 * n), (int64_t)most); }
-__device__ __forceinline__ int64_t share_begin(int64_t U, int64_t C, int64_t c) { return U * c / C; }
-__device__ __forceinline__ int64_t share_of(int64_t U, int64_t C, int64_t u) {
-  int64_t c = u * C / U;
-  while (share_begin(U, C, c + 1) <= u) ++c;
-  return c;
-}
 
-// A position in a CTA's share: the token, and of its units the run [a, b) of one item.
+constexpr int PA_TOKENS = 512;         // up to so many tokens a CTA keeps all of them in shared memory
+
+struct Shares {
+  unsigned n, q, r;                    // how many; the first r have q + 1 units, the others q
+  // of U units that belong to so many items: a join reads the parts one after the other, 64 are enough
+  __device__ Shares(unsigned U, unsigned items, unsigned ctas) : n(min(min(U, ctas), items < 65536 ? 64 * items : ctas)) {
+    q = n ? U / n : 1;
+    r = U - q * n;
+  }
+  __device__ unsigned begin(unsigned c) const { return c * q + min(c, r); }
+  __device__ unsigned of(unsigned u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
+};
+
+// The tokens of a call of up to PA_TOKENS: their rows and where their slots end.  (Under a full stream of keys a look at global memory
+// takes 2 to 3 us, L2 hit or not.)
+struct Tokens {
+  int row[PA_TOKENS], slots[PA_TOKENS];
+};
+
+// A position in a share: the token, and of its units the run [a, b) of one item.
 struct Cursor {
-  int64_t u, end, base;
+  unsigned u, end, base;
   int t, item, a, b;
   Token tok;
-  __device__ Cursor(const PagedAttn& p, int64_t u_, int64_t end_, int t_, int64_t base_, int warps)
-      : u(u_), end(end_), base(base_), t(t_), item(0), a(0), b(0), tok(p, t_, warps) {}
-  __device__ bool next(const PagedAttn& p, int items, int warps) {
+  __device__ void load(const PagedAttn& p, const Tokens& ts, int warps) {
+    tok = p.M <= PA_TOKENS ? Token(p, ts.row[t], ts.slots[t], warps) : Token(p, t, warps);
+  }
+  __device__ bool next(const PagedAttn& p, const Tokens& ts, int items, int warps) {
     if (u >= end) return false;
-    while (u >= base + (int64_t)tok.units * items) {
-      base += (int64_t)tok.units * items;
-      tok = Token(p, ++t, warps);
+    while (u - base >= (unsigned)(tok.units * items)) {
+      base += tok.units * items;
+      ++t;
+      load(p, ts, warps);
     }
-    const unsigned at = (unsigned)(u - base);
+    const unsigned at = u - base;
     item = at / (unsigned)tok.units;
     a = at - item * tok.units;
-    b = (int)min((int64_t)tok.units, a + (end - u));
+    b = min(tok.units, (int)(a + (end - u)));
     u += b - a;
     return true;
   }
+};
+
+// What the streaming warps need to know of a run of one item's tiles.
+struct Run {
+  int tile, tile_end;                  // of the item's visible tiles; tile < 0: there is no run any more
+  Span span;
+  int row, g, head, rows, line;        // table row, key head, first query head of all, heads, item of all
+  int part;                            // where it goes; -1: it is the whole item
 };
 
 // ------------------------------------------------------------------------------------------------ engines
@@ -133,7 +161,12 @@ struct Cursor {
 template <typename T_, int D_, int NB>
 struct TcEngine {
   using T = T_;
-  static constexpr int D = D_, ROWS = 8 * NB, WARPS = 4, STAGES = D_ > 128 ? 2 : 3, CTAS = D_ > 128 ? 1 : 2;
+#ifndef PAV_W
+#define PAV_W 5
+#define PAV_S 2
+#define PAV_C 2
+#endif
+  static constexpr int D = D_, MAX_D = D_, ROWS = 8 * NB, WARPS = PAV_W, STAGES = D_ > 80 ? PAV_S : D_ > 64 ? 3 : 4, CTAS = D_ > 128 ? 1 : PAV_C;
   static constexpr int CHUNKS = D / 8, PIECES = CHUNKS % 8 ? (CHUNKS | 1) : CHUNKS;    // 16-byte pieces of a staged line
   static constexpr int Q_STRIDE = D * 2 + 16, Q_BYTES = ROWS * Q_STRIDE;
   static constexpr int NQ = (ROWS * CHUNKS + WARPS * 32 - 1) / (WARPS * 32);
@@ -269,7 +302,7 @@ struct TcEngine {
 template <typename T_, int NG>
 struct FmaEngine {
   using T = T_;
-  static constexpr int ROWS = 8, WARPS = sizeof(T_) == 4 && NG == 2 ? 2 : 4, STAGES = 2, CTAS = 1;
+  static constexpr int MAX_D = 128 * NG, ROWS = 8, WARPS = sizeof(T_) == 4 && NG == 2 ? 2 : 4, STAGES = 2, CTAS = 1;
   static constexpr int E = 16 / (int)sizeof(T_);
   static constexpr int Q_BYTES = (ROWS * NG * 128 + WARPS * ROWS * PA_TILE) * 4;     // queries and every warp's weights, fp32
   static constexpr int NQ = (ROWS * NG * 128 / E + WARPS * 32 - 1) / (WARPS * 32);
@@ -302,6 +335,7 @@ struct FmaEngine {
     float s[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) s[r] = 0.f;
+#pragma unroll 1
     for (int c = half; c < chunks; c += 2) {
       T kv[E];
       *reinterpret_cast<uint4*>(kv) = *reinterpret_cast<const uint4*>(ks + key * stride + c * 16);
@@ -337,6 +371,7 @@ struct FmaEngine {
         for (int e = 0; e < 4; ++e) o[r][g][e] *= f;
     }
     __syncwarp();
+#pragma unroll 2
     for (int k = 0; k < PA_TILE; ++k)
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -384,139 +419,132 @@ __device__ __forceinline__ void store_row4(T* out, int d, float4 v, int perm) {
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
+template <int W>
+struct Plan {
+  unsigned sum[W], live[W], base;
+  int t, part[W];
+  Tokens tok;
+  Run run[4];
+};
+
+template <int THREADS>
+__device__ __forceinline__ void meet(int barrier) { asm volatile("barrier.cta.sync %0, %1;" ::"r"(barrier), "n"(THREADS) : "memory"); }
+
+// W warps that stream and multiply, and one that works out what they do next.  They meet at the end of every run.
+// The code has to stay small: it is fetched through the memory that streams the keys, and when it had 90 KB every seldom taken path took microseconds.
 template <typename E>
-__global__ void __launch_bounds__(E::WARPS * 32, E::CTAS)
-paged_attn_kernel(const PagedAttn a) {
+__global__ void __launch_bounds__(E::WARPS * 32 + 32, E::CTAS)
+paged_attn_kernel(const __grid_constant__ PagedAttn a) {
   using T = typename E::T;
   constexpr int W = E::WARPS, THREADS = W * 32;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t s_sum[W], s_base;
-  __shared__ int s_t, s_part[W], s_live[W];
-  __shared__ bool s_last;
+  __shared__ Plan<W> s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = E::dim(a), chunks = D * (int)sizeof(T) / 16;
   const int per = a.H / a.G, blocks = (per + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
-  uint8_t* ring = smem + E::Q_BYTES + warp * E::STAGES * E::tile_bytes(D);
-  const uint32_t qs = (uint32_t)__cvta_generic_to_shared(smem), ring32 = (uint32_t)__cvta_generic_to_shared(ring);
+  {                                                               // the first look at them is a wait for DRAM: all of it at once, beside the plan
+    const int64_t line = (int64_t)blockIdx.x * (THREADS + 32) + threadIdx.x, tables = ((int64_t)a.pt.rows * a.pt.width * 4 + 127) / 128,
+                  queries = ((int64_t)a.M * a.H * D * (int)sizeof(T) + 127) / 128;
+    if (line < tables) prefetch_l2(reinterpret_cast<const uint8_t*>(a.pt.table) + line * 128);
+    else if (line - tables < queries) prefetch_l2(reinterpret_cast<const uint8_t*>(a.q) + (line - tables) * 128);
+  }
   pdl_wait();
 
-  // ---- the plan: units of all tokens, this CTA's share, the token in which it begins -------------------------------------
+  // ---- the plan: units of all tokens, the shares, the token in which this CTA's begins -------------------------------------
   const int chunk = (a.M + THREADS - 1) / THREADS;
-  const int t0 = min(a.M, (int)threadIdx.x * chunk), t1 = min(a.M, t0 + chunk);
-  int64_t mine = 0;
-  int live = 0;
+  const int t0 = min(a.M, (int)threadIdx.x * chunk), t1 = min(a.M, t0 + chunk);        // (none for the last warp)
+  unsigned mine = 0, live = 0;
+#pragma unroll 1
   for (int t = t0; t < t1; ++t) {
-    const int n = Token(a, t, W).units;
-    mine += (int64_t)n * items;
-    live += n > 0;
+    const Token tok(a, t, W);
+    mine += tok.units * items;
+    live += tok.units > 0;
+    if (a.M <= PA_TOKENS) {
+      s.tok.row[t] = tok.row;
+      s.tok.slots[t] = tok.span.n;
+    }
   }
-  int64_t before = mine;
+  unsigned before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+    const unsigned x = __shfl_up_sync(0xffffffffu, before, o);
     if (lane >= o) before += x;
   }
   live = __reduce_add_sync(0xffffffffu, live);
-  if (lane == 31) {
-    s_sum[warp] = before;
-    s_live[warp] = live;
+  if (lane == 31 && warp < W) {
+    s.sum[warp] = before;
+    s.live[warp] = live;
   }
   __syncthreads();
   before -= mine;
-  int64_t U = 0, n_items = 0;
+  unsigned U = 0, n_items = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    if (w < warp) before += s_sum[w];
-    U += s_sum[w];
-    n_items += (int64_t)s_live[w] * items;
+    if (w < warp) before += s.sum[w];
+    U += s.sum[w];
+    n_items += s.live[w] * items;
   }
-  const int64_t C = shares(U, n_items, (int)gridDim.x);
-  if ((int64_t)blockIdx.x >= C) return;
-  const int64_t ub = share_begin(U, C, blockIdx.x), ue = share_begin(U, C, blockIdx.x + 1);
-  if (ub >= before && ub < before + mine) {
-    int64_t x = before;
-    for (int t = t0; t < t1; ++t) {
-      const int64_t n = (int64_t)Token(a, t, W).units * items;
-      if (ub < x + n) {
-        s_t = t;
-        s_base = x;
-        break;
-      }
-      x += n;
+  pdl_launch_dependents();                                        // (the join waits for this launch's end; until then it has no room anyway)
+  const Shares sh(U, n_items, gridDim.x);
+  if (blockIdx.x >= max(sh.n, 1u)) return;                        // (the first one writes down the plan, work or no work)
+  const unsigned ub = sh.begin(blockIdx.x);
+#pragma unroll 1
+  for (int t = t0; t < t1; ++t) {
+    const unsigned n = (a.M <= PA_TOKENS ? Token(a, s.tok.row[t], s.tok.slots[t], W) : Token(a, t, W)).units * items;
+    if (ub - before < n) {
+      s.t = t;
+      s.base = before;
     }
+    if (blockIdx.x == 0) a.base[t] = before;
+    before += n;
   }
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.base[a.M] = U, a.base[a.M + 1] = n_items;
+  if (sh.n == 0) return;
   __syncthreads();
 
-  // ---- loads run ahead of the products, across items --------------------------------------------------------------------
-  Cursor ld(a, ub, ue, s_t, s_base, W), cu = ld;
-  bool more = ld.next(a, items, W);
-  int tile = ld.a * W + warp, tile_end = min(ld.b * W, ld.tok.span.tiles);
-  unsigned paged = 0;                                             // stages whose keys have a page
-  int id = -1, off = 0;                                           // the next tile's page, looked up a tile ahead, and its tile in it
-  auto seek = [&]() {                                             // the next tile this warp loads
-    while (more && tile >= tile_end) {
-      more = ld.next(a, items, W);
-      tile = ld.a * W + warp;
-      tile_end = min(ld.b * W, ld.tok.span.tiles);
-    }
-    if (more) {
-      const int kt = ld.tok.span.key_tile(tile), index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 40);
-      off = kt - index * a.tpp;
-      id = __ldg(a.pt.table + (int64_t)ld.tok.row * a.pt.width + index);
-    }
-  };
-  auto issue = [&](int stage) {
-    if (more) {
-      const Span& sp = ld.tok.span;
-      const int j0 = sp.key0(tile);
-      const bool page = (unsigned)id < (unsigned)a.pt.P, all = page && sp.whole(j0);
-      const int64_t line = (((int64_t)(page ? id : 0) * a.G + ld.item / blocks) * a.tpp + off) * PA_TILE;
-      const uint4* kg = reinterpret_cast<const uint4*>(a.k) + line * chunks + lane;
-      const uint4* vg = reinterpret_cast<const uint4*>(a.v) + line * chunks + lane;
-      const uint32_t ks = ring32 + stage * E::tile_bytes(D), vs = ks + E::tile_bytes(D) / 2;
-      paged = (paged & ~(1u << stage)) | ((page ? 1u : 0u) << stage);
-      if (!page && lane == 0) atomicAdd(&g_paged_attn_fault, 1u);
-      if constexpr (IsTc<E>::value) {
-        constexpr int N = PA_TILE * E::CHUNKS;
-        if (all) {
-#pragma unroll
-          for (int i = 0; i < N / 32; ++i) {
-            const uint32_t at = E::at((i * 32 + lane) / E::CHUNKS, (i * 32 + lane) % E::CHUNKS);
-            copy16(ks + at, kg + i * 32);
-            copy16(vs + at, vg + i * 32);
-          }
-        } else {
+  // ---- the warp for the runs and the parts ----------------------------------------------------------------------------------
+  if (warp == W) {
+    Cursor c;
+    c.u = ub, c.end = sh.begin(blockIdx.x + 1), c.base = s.base, c.t = s.t;
+    c.load(a, s.tok, W);
+    // runs 0 to 2 before the others start, then run n + 3 when run n has ended
 #pragma unroll 1
-          for (int i = 0; i < N / 32; ++i) {
-            const int key = (i * 32 + lane) / E::CHUNKS;
-            const uint32_t at = E::at(key, (i * 32 + lane) % E::CHUNKS);
-            const bool ok = page && sp.visible(j0 + key);
-            cp_async16(ks + at, ok ? kg + i * 32 : kg, ok);
-            cp_async16(vs + at, ok ? vg + i * 32 : vg, ok);
-          }
-        }
-      } else {
-        for (int x = lane; x < PA_TILE * chunks; x += 32) {
-          const int key = x / chunks, c = x - key * chunks;
-          const bool ok = all || (page && sp.visible(j0 + key));
-          cp_async16(ks + E::at(key, c, D), kg + (ok ? x - lane : 0), ok);
-          cp_async16(vs + E::at(key, c, D), vg + (ok ? x - lane : 0), ok);
-        }
+    for (int n = 0;; ++n) {
+      Run r;
+      r.tile = -1;
+      if (c.next(a, s.tok, items, W)) {
+        r.g = c.item / blocks;
+        const int r0 = (c.item - r.g * blocks) * E::ROWS;
+        r.tile = c.a * W, r.tile_end = min(c.b * W, c.tok.span.tiles);
+        r.span = c.tok.span;
+        r.row = c.tok.row, r.head = c.t * a.H + r.g * per + r0, r.rows = min(E::ROWS, per - r0), r.line = c.t * items + c.item;
+        r.part = c.b - c.a < c.tok.units ? (int)blockIdx.x * 2 + (c.a == 0 ? 1 : 0) : -1;
       }
-      tile += W;
-      seek();
+      if (lane == 0) s.run[n & 3] = r;
+      if (n < 2) continue;
+      if (n == 2) __syncthreads();
+      meet<THREADS + 32>(2);                                      // the end of run n - 2
+      if (s.run[(n - 1) & 3].tile < 0) return;
     }
-    cp_async_commit();
-  };
-  // the queries of an item, a few 16-byte pieces per thread: those of the next one are fetched while this one's keys pass
+  }
+
+  // ---- loads run ahead of the products, across runs -------------------------------------------------------------------------
+  uint8_t* ring = smem + E::Q_BYTES + warp * E::STAGES * E::tile_bytes(D);
+  const uint32_t qs = (uint32_t)__cvta_generic_to_shared(smem), ring32 = (uint32_t)__cvta_generic_to_shared(ring);
+  int tile = 0, tile_end = 0, ld_run = -1, id = -1, off = 0;      // the next tile to load: its run, its page, its place in it
+  int inflight = 0, ld_stage = 0, stage = 0;                      // tiles on their way or here; where the next one goes; where the next one lies
+  unsigned paged = 0;                                             // stages whose keys have a page
+  Span ls(0, 0, 0);
+  const int32_t* table = nullptr;
+  int64_t kv_head = 0;
   uint4 qn[E::NQ];
-  auto fetch_q = [&](const Cursor& c) {
-    const int g = c.item / blocks, r0 = (c.item - g * blocks) * E::ROWS, rows = min(E::ROWS, per - r0);
-    const uint4* q = reinterpret_cast<const uint4*>(a.q) + ((int64_t)c.t * a.H + (int64_t)g * per + r0) * chunks;
+  auto fetch_q = [&](const Run& r) {
+    const uint4* q = reinterpret_cast<const uint4*>(a.q) + (int64_t)r.head * chunks;
+    const int n = r.rows * chunks;
 #pragma unroll
     for (int i = 0; i < E::NQ; ++i) {
       const int x = i * THREADS + (int)threadIdx.x;
-      qn[i] = x < rows * chunks ? q[x] : make_uint4(0, 0, 0, 0);
+      qn[i] = x < n ? q[x] : make_uint4(0, 0, 0, 0);
     }
   };
   auto put_q = [&]() {
@@ -526,166 +554,249 @@ paged_attn_kernel(const PagedAttn a) {
       if (x < E::ROWS * chunks) E::put_q(smem, x / chunks, x % chunks, qn[i], D);
     }
   };
-  bool work = cu.next(a, items, W);
-  fetch_q(cu);
-  seek();
-#pragma unroll
-  for (int s = 0; s < E::STAGES - 1; ++s) issue(s);
-  put_q();
   __syncthreads();
+  fetch_q(s.run[0]);
 
   E e;
-  int stage = 0;                                                  // of the next tile
-  while (work) {
-    const Cursor me = cu;
-    work = cu.next(a, items, W);
-    if (work) fetch_q(cu);
-    const int g = me.item / blocks, r0 = (me.item - g * blocks) * E::ROWS, rows = min(E::ROWS, per - r0);
-    const int64_t head = (int64_t)me.t * a.H + (int64_t)g * per + r0;
-    const Span sp = me.tok.span;
-    float* scores = a.scores + ((int64_t)me.t * items + me.item) * a.cap * a.pitch;
-    e.begin(qs);
-    const int end = min(me.b * W, sp.tiles);
-    for (int v = me.a * W + warp; v < end; v += W) {
-      issue(stage == 0 ? E::STAGES - 1 : stage - 1);
-      cp_async_wait<E::STAGES - 1>();
+#pragma unroll 1
+  for (int n = 0;; ++n) {
+    const Run& r = s.run[n & 3];
+    const bool more = s.run[(n + 1) & 3].tile >= 0;
+    const int rows = r.rows, end = r.tile_end;
+    const Span sp = r.span;
+    float* scores = a.mass ? a.scores + (int64_t)r.line * a.cap * a.pitch : nullptr;
+    bool begun = false;
+#pragma unroll 1
+    for (int v = r.tile + warp;; v += W) {
+      // as many loads as there are stages (but one stage stays free at a run's end)
+#pragma unroll 1
+      while (inflight < (v < end ? E::STAGES : E::STAGES - 1)) {
+        bool turned = false;
+#pragma unroll 1
+        while (tile >= tile_end && ld_run <= n) {                 // (no further than the run behind this one)
+          const Run& l = s.run[(ld_run + 1) & 3];
+          if (l.tile < 0) break;
+          ++ld_run;
+          tile = l.tile + warp, tile_end = l.tile_end;
+          ls = l.span;
+          table = a.pt.table + (int64_t)l.row * a.pt.width;
+          kv_head = l.g;
+          turned = true;
+        }
+        if (tile >= tile_end) break;
+        auto seek = [&]() {
+          const int kt = ls.key_tile(tile), index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 40);
+          off = kt - index * a.tpp;
+          id = __ldg(table + index);
+        };
+        if (turned) seek();
+        const int j0 = ls.key0(tile);
+        const bool page = (unsigned)id < (unsigned)a.pt.P, all = page && ls.whole(j0);
+        const int64_t line = (((int64_t)(page ? id : 0) * a.G + kv_head) * a.tpp + off) * PA_TILE;
+        const uint4* kg = reinterpret_cast<const uint4*>(a.k) + line * chunks + lane;
+        const uint4* vg = reinterpret_cast<const uint4*>(a.v) + line * chunks + lane;
+        const uint32_t ks = ring32 + ld_stage * E::tile_bytes(D), vs = ks + E::tile_bytes(D) / 2;
+        paged = (paged & ~(1u << ld_stage)) | ((page ? 1u : 0u) << ld_stage);
+        if (!page && lane == 0) atomicAdd(&g_paged_attn_fault, 1u);
+        if constexpr (IsTc<E>::value) {
+          constexpr int N = PA_TILE * E::CHUNKS;
+          if (all) {
+#pragma unroll
+            for (int i = 0; i < N / 32; ++i) {
+              const uint32_t at = E::at((i * 32 + lane) / E::CHUNKS, (i * 32 + lane) % E::CHUNKS);
+              copy16(ks + at, kg + i * 32);
+              copy16(vs + at, vg + i * 32);
+            }
+          } else {
+#pragma unroll 1
+            for (int i = 0; i < N / 32; ++i) {
+              const int key = (i * 32 + lane) / E::CHUNKS;
+              const uint32_t at = E::at(key, (i * 32 + lane) % E::CHUNKS);
+              const bool ok = page && ls.visible(j0 + key);
+              cp_async16(ks + at, ok ? kg + i * 32 : kg, ok);
+              cp_async16(vs + at, ok ? vg + i * 32 : vg, ok);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int x = lane; x < PA_TILE * chunks; x += 32) {
+            const int key = x / chunks, c = x - key * chunks;
+            const bool ok = all || (page && ls.visible(j0 + key));
+            cp_async16(ks + E::at(key, c, D), kg + (ok ? x - lane : 0), ok);
+            cp_async16(vs + E::at(key, c, D), vg + (ok ? x - lane : 0), ok);
+          }
+        }
+        cp_async_commit();
+        ld_stage = ld_stage + 1 == E::STAGES ? 0 : ld_stage + 1;
+        ++inflight;
+        tile += W;
+        if (tile < tile_end) seek();                              // a tile ahead
+      }
+      if (!begun) {
+        begun = true;
+        if (n == 0) {
+          put_q();
+          meet<THREADS>(1);
+        }
+        e.begin(qs);
+        if (more) fetch_q(s.run[(n + 1) & 3]);                    // for the end of this run
+      }
+      if (v >= end) break;
+      if (inflight >= 4) cp_async_wait<3>();
+      else if (inflight == 3) cp_async_wait<2>();
+      else if (inflight == 2) cp_async_wait<1>();
+      else cp_async_wait<0>();
       __syncwarp();
       const int j0 = sp.key0(v);
       const bool page = (paged >> stage) & 1u;
       const bool all = page && sp.whole(j0);
-      e.tile(a, qs, ring32 + stage * E::tile_bytes(D), j0, sp, all, page, a.mass ? scores + (int64_t)v * PA_TILE * a.pitch : nullptr, rows,
+      e.tile(a, qs, ring32 + stage * E::tile_bytes(D), j0, sp, all, page, scores ? scores + (int64_t)v * PA_TILE * a.pitch : nullptr, rows,
              ring + stage * E::tile_bytes(D));
-      __syncwarp();                                               // the stage is refilled by the next issue
+      __syncwarp();                                               // the stage is refilled by the next load
       stage = stage + 1 == E::STAGES ? 0 : stage + 1;
+      --inflight;
     }
-    // ---- the warps' parts become one: each in the one stage of its ring that waits for nothing ------------------------------
-    const int part = (warp * E::STAGES + (stage == 0 ? E::STAGES - 1 : stage - 1)) * E::tile_bytes(D);
-    if (lane == 0) s_part[warp] = part;
-    const bool whole = me.a == 0 && me.b == me.tok.units;
-    const int64_t part_size = (int64_t)E::ROWS * (D + 4);
-    float* rec = a.rec + ((int64_t)blockIdx.x * 2 + (me.a == 0 ? 1 : 0)) * part_size;
+    // ---- the warps' parts become one: each in the one stage of its ring that waits for nothing; a warp per head -------------
+    const int part = (warp * E::STAGES + ld_stage) * E::tile_bytes(D);
+    if (lane == 0) s.part[warp] = part;
+    const int head = r.head;
+    const bool cut = r.part >= 0;
+    float* rec = a.rec + (int64_t)r.part * E::ROWS * (D + 4);
+#pragma unroll 1
     for (int pass = 0; pass * 8 < rows; ++pass) {
       e.publish(reinterpret_cast<float*>(smem + E::Q_BYTES + part), pass, D);
-      __syncthreads();
-      if (pass == 0 && work) put_q();
-      const int here = min(8, rows - pass * 8), quads = D / 4;
-      for (int x = threadIdx.x; x < here * quads; x += THREADS) {
-        const int r = x / quads, d = (x - r * quads) * 4;
-        float M = -INFINITY, L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      meet<THREADS>(1);
+      if (pass == 0 && more) put_q();
+#pragma unroll 1
+      for (int row = warp; row < rows; row += W) {
+        if (row >> 3 != pass) continue;
+        float M = -INFINITY, L = 0.f, f[W];
+        const float* p[W];
 #pragma unroll
-        for (int w = 0; w < W; ++w) M = fmaxf(M, reinterpret_cast<const float*>(smem + E::Q_BYTES + s_part[w])[r * (D + 4)]);
+        for (int w = 0; w < W; ++w) {
+          p[w] = reinterpret_cast<const float*>(smem + E::Q_BYTES + s.part[w]) + (row & 7) * (D + 4);
+          f[w] = p[w][0];
+          M = fmaxf(M, f[w]);
+        }
         const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const float* p = reinterpret_cast<const float*>(smem + E::Q_BYTES + s_part[w]) + r * (D + 4);
-          const float f = raise2(p[0] - ref);
-          const float4 y = *reinterpret_cast<const float4*>(p + 4 + d);
-          L += p[1] * f;
-          acc.x += y.x * f; acc.y += y.y * f; acc.z += y.z * f; acc.w += y.w * f;
+          f[w] = raise2(f[w] - ref);
+          L += p[w][1] * f[w];
         }
-        const int row = pass * 8 + r;
-        if (whole) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          store_row4<T>(reinterpret_cast<T*>(a.out) + (head + row) * D, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv), a.out_perm);
-          if (a.mass && d == 0) *reinterpret_cast<float2*>(a.stat + (head + row) * 2) = make_float2(ref, inv);
-        } else {
-          float* p = rec + row * (D + 4);
-          *reinterpret_cast<float4*>(p + 4 + d) = acc;
-          if (d == 0) *reinterpret_cast<float2*>(p) = make_float2(M, L);
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll 1
+        for (int d = 4 * lane; d < D; d += 128) {
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(p[w] + 4 + d);
+            acc.x += y.x * f[w]; acc.y += y.y * f[w]; acc.z += y.z * f[w]; acc.w += y.w * f[w];
+          }
+          if (!cut)
+            store_row4<T>(reinterpret_cast<T*>(a.out) + ((int64_t)head + row) * D, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv), a.out_perm);
+          else
+            *reinterpret_cast<float4*>(rec + row * (D + 4) + 4 + d) = acc;
+        }
+        if (lane == 0) {
+          if (cut) *reinterpret_cast<float2*>(rec + row * (D + 4)) = make_float2(M, L);
+          else if (a.mass) *reinterpret_cast<float2*>(a.stat + ((int64_t)head + row) * 2) = make_float2(ref, inv);
         }
       }
-      __syncthreads();
+      if (pass * 8 + 8 < rows) meet<THREADS>(1);
     }
-    if (whole) continue;
-    // ---- an item that is cut: the last of its CTAs joins the parts ----------------------------------------------------------
-    const int64_t u0 = me.base + (int64_t)me.item * me.tok.units, c0 = share_of(U, C, u0), c1 = share_of(U, C, u0 + me.tok.units - 1);
-    const int parts = (int)(c1 - c0) + 1;
-    if (threadIdx.x == 0) {
-      __threadfence();                                            // (the barrier before: every thread's part of the record)
-      const bool last = atomicAdd(a.arrived + c0, 1u) == (unsigned)(parts - 1);
-      if (last) {
-        a.arrived[c0] = 0;                                        // as it was found
-        __threadfence();
-      }
-      s_last = last;
-    }
-    __syncthreads();
-    if (!s_last) continue;
-    const float* first = a.rec + (c0 * 2 + 1) * part_size;
-    const float* other = a.rec + (c0 + 1) * 2 * part_size;       // of part i > 0: + (i - 1) * 2 * part_size
-    const int quads = D / 4;
-    for (int x = threadIdx.x; x < rows * quads; x += THREADS) {
-      const int r = x / quads, d = (x - r * quads) * 4;
-      float M = -INFINITY, L = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      constexpr int AHEAD = 8;
-      for (int i0 = 0; i0 < parts; i0 += AHEAD) {
-        float2 ml[AHEAD];
-        float4 y[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const float* p = (i0 + i == 0 ? first : other + (int64_t)(i0 + i - 1) * 2 * part_size) + r * (D + 4);
-          ml[i] = i0 + i < parts ? __ldcg(reinterpret_cast<const float2*>(p)) : make_float2(-INFINITY, 0.f);
-          y[i] = i0 + i < parts ? __ldcg(reinterpret_cast<const float4*>(p + 4 + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        float top = M;
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
-        const float ref = top == -INFINITY ? 0.f : top, f = raise2(M - ref);
-        M = top;
-        L *= f;
-        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const float w = raise2(ml[i].x - ref);
-          L += ml[i].y * w;
-          acc.x += y[i].x * w; acc.y += y[i].y * w; acc.z += y[i].z * w; acc.w += y[i].w * w;
-        }
-      }
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      store_row4<T>(reinterpret_cast<T*>(a.out) + (head + r) * D, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv), a.out_perm);
-      if (a.mass && d == 0) *reinterpret_cast<float2*>(a.stat + (head + r) * 2) = make_float2(M == -INFINITY ? 0.f : M, inv);
-    }
+    meet<THREADS + 32>(2);
+    if (!more) return;
   }
-  cp_async_wait<0>();
 }
 
-// The weights that every visible slot received: a CTA per item (x) and slice of its visible slots (y), a thread per slot.
-constexpr int PM_THREADS = 256;
-
-template <int ROWS>
-__global__ void __launch_bounds__(PM_THREADS)
-paged_attn_mass_kernel(const PagedAttn a, int warps) {
+// What is left of an item (x): a warp per query head joins its parts where it was cut, with all their loads under way at once.  With a mass, CTAs
+// share the item's visible slots (y) and form the heads' maxima and sums anew, then a thread per slot adds up what the heads gave it.
+template <typename E>
+__global__ void __launch_bounds__(E::ROWS * 32)
+paged_attn_join_kernel(const __grid_constant__ PagedAttn a, unsigned ctas) {
+  constexpr int ROWS = E::ROWS, NQ4 = E::MAX_D > 128 ? 2 : 1, AHEAD = 16 / NQ4;
+  __shared__ float2 s_stat[ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = E::dim(a);
   const int per = a.H / a.G, blocks = (per + ROWS - 1) / ROWS, items = a.G * blocks;
   const int t = blockIdx.x / items, item = blockIdx.x - t * items;
   const int g = item / blocks, r0 = (item - g * blocks) * ROWS, rows = min(ROWS, per - r0);
+  const int64_t head = (int64_t)t * a.H + (int64_t)g * per + r0;
   pdl_wait();
-  const Token tok(a, t, warps);
-  const int seen = tok.span.tiles * PA_TILE;
-  if ((int)blockIdx.y * PM_THREADS >= seen) return;
-  const float2* stat = reinterpret_cast<const float2*>(a.stat) + (int64_t)t * a.H + (int64_t)g * per + r0;
-  const float* sc = a.scores + (int64_t)blockIdx.x * a.cap * a.pitch;
-  float2 st[ROWS];
+  const unsigned base = a.base[t], units = (a.base[t + 1] - base) / items, U = a.base[a.M];
+  if (units == 0) return;                                         // an idle token
+  const Shares sh(U, a.base[a.M + 1], ctas);
+  const unsigned u0 = base + item * units, c0 = sh.of(u0), c1 = sh.of(u0 + units - 1);
+  if (c0 == c1 && !a.mass) return;
+  if (c0 != c1 && warp < rows) {
+    const int parts = (int)(c1 - c0) + 1;
+    const int64_t size = (int64_t)ROWS * (D + 4);
+    const float* first = a.rec + ((int64_t)c0 * 2 + 1) * size + warp * (D + 4);
+    float M = -INFINITY, L = 0.f;
+    float4 acc[NQ4];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) st[r] = r < rows ? stat[r] : make_float2(0.f, 0.f);
-  for (int x = blockIdx.y * PM_THREADS + threadIdx.x; x < seen; x += gridDim.y * PM_THREADS) {
+    for (int x = 0; x < NQ4; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int i0 = 0; i0 < parts; i0 += AHEAD) {
+      float2 ml[AHEAD];
+      float4 y[AHEAD][NQ4];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {                           // part i > 0 is the first of its share's two
+        const int at = i0 + i;
+        const float* p = first + (at == 0 ? 0 : (2 * (int64_t)at - 1) * size);
+        ml[i] = at < parts ? *reinterpret_cast<const float2*>(p) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int x = 0; x < NQ4; ++x)
+          y[i][x] = at < parts && 4 * lane + 128 * x < D ? *reinterpret_cast<const float4*>(p + 4 + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
+      const float ref = top == -INFINITY ? 0.f : top, f = raise2(M - ref);
+      M = top;
+      L *= f;
+#pragma unroll
+      for (int x = 0; x < NQ4; ++x) acc[x].x *= f, acc[x].y *= f, acc[x].z *= f, acc[x].w *= f;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const float w = raise2(ml[i].x - ref);
+        L += ml[i].y * w;
+#pragma unroll
+        for (int x = 0; x < NQ4; ++x) acc[x].x += y[i][x].x * w, acc[x].y += y[i][x].y * w, acc[x].z += y[i][x].z * w, acc[x].w += y[i][x].w * w;
+      }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    if (blockIdx.y == 0) {
+#pragma unroll
+      for (int x = 0; x < NQ4; ++x)
+        if (4 * lane + 128 * x < D)
+          store_row4<typename E::T>(reinterpret_cast<typename E::T*>(a.out) + (head + warp) * D, 4 * lane + 128 * x,
+                                    make_float4(acc[x].x * inv, acc[x].y * inv, acc[x].z * inv, acc[x].w * inv), a.out_perm);
+    }
+    if (lane == 0) s_stat[warp] = make_float2(M == -INFINITY ? 0.f : M, inv);
+  }
+  if (!a.mass) return;
+  if (c0 == c1 && (int)threadIdx.x < rows) s_stat[threadIdx.x] = reinterpret_cast<const float2*>(a.stat)[head + threadIdx.x];
+  __syncthreads();
+  const Token tok(a, t, E::WARPS);
+  const int seen = tok.span.tiles * PA_TILE;
+  const float* sc = a.scores + (int64_t)blockIdx.x * a.cap * a.pitch;
+#pragma unroll 1
+  for (int x = blockIdx.y * ROWS * 32 + threadIdx.x; x < seen; x += gridDim.y * ROWS * 32) {
     const int j = tok.span.key0(x / PA_TILE) + x % PA_TILE;
     if (!tok.span.visible(j)) continue;
     const int64_t id = page_id(a.pt, tok.row, j / a.pt.page);
     if (id < 0) continue;
-    const float* s = sc + (int64_t)x * a.pitch;
+    const float* p = sc + (int64_t)x * a.pitch;
     float w = 0.f;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
-      if (r < rows) w += raise2(s[r] - st[r].x) * st[r].y;
+      if (r < rows) w += raise2(p[r] - s_stat[r].x) * s_stat[r].y;
     atomicAdd(&a.mass[(id * a.G + g) * a.pt.page + j % a.pt.page], w);    // slots that several tokens see
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host
-constexpr int PA_CTAS = 2;            // per SM: one's join beside the other's stream
-
 // visible slots a token can have, in whole tiles
 static int64_t visible_cap(int64_t slots, int64_t first, int64_t window) {
   const int64_t seen = window > 0 ? first + window + 2 * PA_TILE : slots;
@@ -693,40 +804,38 @@ static int64_t visible_cap(int64_t slots, int64_t first, int64_t window) {
 }
 
 static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-constexpr size_t PA_ARRIVED = 4096;                               // bytes
-static size_t rec_bytes(int D) { return round256((size_t)sm_count() * PA_CTAS * 2 * 16 * (D + 4) * 4); }
+static size_t base_bytes(int64_t M) { return round256((size_t)(M + 2) * 4); }
+static size_t rec_bytes(int D) { return round256((size_t)sm_count() * 2 * 2 * 16 * (D + 4) * 4); }      // (two CTAs per SM at most)
 static size_t stat_bytes(int64_t M, int H) { return round256((size_t)M * H * 8); }
 
 template <typename E>
 static int launch_paged(PagedAttn a, cudaStream_t st) {
   const int smem = E::Q_BYTES + E::WARPS * E::STAGES * E::tile_bytes(a.D);
   const int blocks = (a.H / a.G + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
-  B200P_REQUIRE((int64_t)items * (a.cap / PA_TILE / E::WARPS + 1) < (1ll << 31) && (int64_t)a.M * items < (1ll << 31), B200P_ERR_ARG,
+  B200P_REQUIRE((int64_t)a.M * items * (a.cap / PA_TILE / E::WARPS + 1) < (1ll << 31), B200P_ERR_ARG,
                 "%d tokens of %d key heads over %d slots: too many for one call", a.M, a.G, a.cap);
   auto kern = paged_attn_kernel<E>;
   static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024);
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_attn_kernel)");
-  const int ctas = sm_count() * (2 * (smem + 1024 + 256) <= 228 * 1024 ? 2 : 1);
+  const int ctas = sm_count() * E::CTAS;
   const int64_t most = (int64_t)a.M * items * ((a.cap / PA_TILE + E::WARPS - 1) / E::WARPS);
   const int grid = (int)(most < ctas ? most : ctas);
-  B200P_REQUIRE(grid <= (int)(PA_ARRIVED / 4), B200P_ERR_ARCH, "%d SMs", sm_count());
   a.tpp = a.pt.page / PA_TILE;
   a.inv_tpp = ((1ull << 40) + a.tpp - 1) / a.tpp;
   a.pitch = 1;
   while (a.pitch < E::ROWS && a.pitch < a.H / a.G) a.pitch *= 2;
-  launch_pdl(kern, (unsigned)grid, E::WARPS * 32, smem, st, a);
+  launch_pdl(kern, (unsigned)grid, E::WARPS * 32 + 32, smem, st, a);
   B200P_LAUNCH_CHECK("paged_attn_kernel");
-  if (!a.mass) return B200P_OK;
-  // slices: as many as there are, but no more CTAs than fill the GPU
-  const int64_t slices = (a.cap + PM_THREADS - 1) / PM_THREADS, fill = 8ll * sm_count() / ((int64_t)a.M * items) + 1;
-  launch_pdl(paged_attn_mass_kernel<E::ROWS>, dim3((unsigned)(a.M * items), (unsigned)(slices < fill ? slices : fill)), PM_THREADS, 0, st, a, (int)E::WARPS);
-  B200P_LAUNCH_CHECK("paged_attn_mass_kernel");
+  // slices of a mass: as many as there are, but no more CTAs than fill the GPU
+  const int64_t slices = a.mass ? (a.cap + E::ROWS * 32 - 1) / (E::ROWS * 32) : 1, fill = 8ll * sm_count() / ((int64_t)a.M * items) + 1;
+  launch_pdl(paged_attn_join_kernel<E>, dim3((unsigned)(a.M * items), (unsigned)(slices < fill ? slices : fill)), E::ROWS * 32, 0, st, a, (unsigned)grid);
+  B200P_LAUNCH_CHECK("paged_attn_join_kernel");
   return B200P_OK;
 }
 
@@ -751,7 +860,7 @@ using namespace b200p;
 
 extern "C" size_t b200p_paged_attn_workspace_bytes(int64_t M, int H, int D, int64_t keys) {
   if (M <= 0 || H <= 0 || D <= 0) return 0;
-  size_t n = PA_ARRIVED + rec_bytes(D);
+  size_t n = base_bytes(M) + rec_bytes(D);
   if (keys > 0) n += stat_bytes(M, H) + (size_t)M * H * 2 * ((keys + PA_TILE - 1) / PA_TILE * PA_TILE) * 4;     // (pitch < 2 x heads)
   return n;
 }
@@ -781,8 +890,8 @@ extern "C" int b200p_paged_attn(const void* q, const void* kpages, const void* v
   a.M = (int)M, a.H = H, a.G = G, a.D = D, a.first = (int)first, a.window = (int)window, a.out_perm = (flags & B200P_OUT_PERM8) ? 1 : 0;
   a.scale_log2e = scale * 1.4426950408889634f, a.cap = (int)cap;
   uint8_t* ws = (uint8_t*)workspace;
-  a.arrived = (unsigned*)ws;
-  a.rec = (float*)(ws += PA_ARRIVED);
+  a.base = (unsigned*)ws;
+  a.rec = (float*)(ws += base_bytes(M));
   a.stat = (float*)(ws += rec_bytes(D));
   a.scores = (float*)(ws + stat_bytes(M, H));
   B200P_DISPATCH_DTYPE(dtype, T, return (launch_paged_type<T>(a, (cudaStream_t)stream)));

@@ -834,7 +834,7 @@ def paged_append(qkv, q_out, kpages, vpages, table, t_row, t_slot, t_pos, H: int
 
 
 def paged_attn_workspace_bytes(M: int, H: int, D: int, keys: int = 0) -> int:
-    """Bytes of a workspace (zeroed before its first use, one stream at a time); ``keys``: the table's width * page where a mass is added up, else 0."""
+    """Bytes of a workspace (256-byte aligned, one stream at a time); ``keys``: the table's width * page where a mass is added up, else 0."""
     return int(lib().b200p_paged_attn_workspace_bytes(int(M), int(H), int(D), int(keys)))
 
 

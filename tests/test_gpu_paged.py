@@ -205,9 +205,7 @@ def _check_attn(ops, c, q, row, slot, H, first, window, mass, scale, perm=False)
     keys = c.table.shape[1] * c.page if mass else 0
     n = ops.paged_attn_workspace_bytes(M, H, D, keys)
     ws = torch.full((n,), 0xa5, dtype=torch.uint8, device="cuda")
-    ws[:4096] = 0
     ops.paged_attn(q.cuda(), k, v, table, row.cuda(), slot.cuda(), out, scale, first=first, window=window, mass=ms, workspace=ws, out_perm=perm)
-    assert bool((ws[:4096] == 0).all()), "the counters are left as they were found"
     exp, tol, em, off = po.attn(q, c.k, c.v, c.mass if mass else None, c.table, row, slot, H, scale, first, window,
                                 0.0 if dt is torch.float32 else po.half_step(dt) ** 2)
     got = out.cpu().double().view(M, H, D)
@@ -305,7 +303,7 @@ def test_attention_over_more_than_two_giga_elements(ops):
     q = c.normal(2, H * D).to(c.dtype)
     table = torch.where(c.table >= 0, c.table + (P - c.P), c.table)
     out = torch.empty((2, H * D), dtype=torch.bfloat16, device="cuda")
-    ws = torch.zeros((ops.paged_attn_workspace_bytes(2, H, D, table.shape[1] * page),), dtype=torch.uint8, device="cuda")
+    ws = torch.empty((ops.paged_attn_workspace_bytes(2, H, D, table.shape[1] * page),), dtype=torch.uint8, device="cuda")
     ops.paged_attn(q.cuda(), k, v, table.cuda(), row.cuda(), slot.cuda(), out, 0.1, mass=mass, workspace=ws)
     near, nearest = _check_attn(ops, c, q, row, slot, H, 0, 0, True, 0.1)
     assert same(out, near)
@@ -462,7 +460,7 @@ def _decode(ops, dtype, steps, graph):
     d = dict(x=torch.empty((3, (H + 2 * G) * D), dtype=dt, device="cuda"), q=torch.empty((3, H * D), dtype=dt, device="cuda"),
              out=torch.empty((3, H * D), dtype=dt, device="cuda"), slot=torch.zeros(3, dtype=torch.int32, device="cuda"),
              pos=torch.zeros(3, dtype=torch.int32, device="cuda"), row=rows.cuda(), rates=rates.cuda(),
-             ws=torch.zeros((ops.paged_attn_workspace_bytes(3, H, D, table.shape[1] * page),), dtype=torch.uint8, device="cuda"))
+             ws=torch.empty((ops.paged_attn_workspace_bytes(3, H, D, table.shape[1] * page),), dtype=torch.uint8, device="cuda"))
 
     def step():
         ops.paged_append(d["x"], d["q"], k, v, table, d["row"], d["slot"], d["pos"], H, rates=d["rates"], mass=ms)
@@ -523,7 +521,6 @@ def test_two_graphs_share_a_workspace(ops):
     H = 8
     n = ops.paged_attn_workspace_bytes(3, H, 128, table.shape[1] * 16)
     ws = torch.full((n,), 0x7f, dtype=torch.uint8, device="cuda")
-    ws[:4096] = 0
     q = c.normal(3, H * 128).to(c.dtype).cuda()
     calls = [(i32([0, 1, 2]), i32([2999, 499, 63])), (i32([1]), i32([300])), (i32([2, 0]), i32([10, 1500]))]
     calls = [(a.cuda(), b.cuda(), torch.empty((a.numel(), H * 128), dtype=c.dtype, device="cuda")) for a, b in calls]
@@ -557,7 +554,7 @@ def test_on_a_stream_of_its_own(ops):
     q = c.normal(2, 8 * 128).to(c.dtype).cuda()
     row, slot = i32([0, 1]).cuda(), i32([2999, 499]).cuda()
     outs = [torch.zeros((2, 8 * 128), dtype=c.dtype, device="cuda") for _ in range(3)]
-    ws = [torch.zeros((max(16, ops.paged_attn_workspace_bytes(2, 8, 128, 0)),), dtype=torch.uint8, device="cuda") for _ in range(3)]
+    ws = [torch.empty((max(16, ops.paged_attn_workspace_bytes(2, 8, 128, 0)),), dtype=torch.uint8, device="cuda") for _ in range(3)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
     ops.paged_attn(q, k, v, table, row, slot, outs[2], 0.1, workspace=ws[2])
@@ -590,7 +587,7 @@ def test_prompt_through_the_dense_view(ops):
         a, b = torch.empty_like(q), torch.empty_like(q)
         ws = torch.empty((max(16, ops.attn_workspace_bytes(1, L, H, D)),), dtype=torch.uint8, device="cuda")
         ops.attn(q, dk, dv, before, a, 1, L, H, G, D, D ** -0.5, workspace=ws)
-        ws2 = torch.zeros((max(16, ops.paged_attn_workspace_bytes(L, H, D, 0)),), dtype=torch.uint8, device="cuda")
+        ws2 = torch.empty((max(16, ops.paged_attn_workspace_bytes(L, H, D, 0)),), dtype=torch.uint8, device="cuda")
         ops.paged_attn(q, k, v, table, row, slot, b, D ** -0.5, workspace=ws2)
         # weights and results rounded to f16 on either side: 2 x (2^-11 + 2^-11) of sums of at most sum p |v|
         bound = 4 * 2.0 ** -11 * float(v[~torch.isnan(v)].abs().max()) 
@@ -604,7 +601,7 @@ def test_refusals(ops):
     k, v, table, ms = c.cuda()
     q = torch.zeros((2, 8 * 64), dtype=torch.bfloat16, device="cuda")
     out, row, slot = torch.zeros_like(q), i32([0, 1]).cuda(), i32([99, 49]).cuda()
-    ws = torch.zeros((ops.paged_attn_workspace_bytes(2, 8, 64, 0) + 16,), dtype=torch.uint8, device="cuda")
+    ws = torch.empty((ops.paged_attn_workspace_bytes(2, 8, 64, 0) + 16,), dtype=torch.uint8, device="cuda")
     x = torch.zeros((2, 12 * 64), dtype=torch.bfloat16, device="cuda")
     ln, kept = i32([100, 50]).cuda(), torch.zeros((2, 2, 20), dtype=torch.int32, device="cuda")
     dk = torch.zeros((2, 2, 128, 64), dtype=torch.bfloat16, device="cuda")
