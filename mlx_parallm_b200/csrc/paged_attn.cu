@@ -82,8 +82,9 @@ struct PagedAttn {
 // (token, key head, block of query heads) items are laid end to end, and each CTA takes an equal share of that line.  An item that lies in one share is
 // finished there; of one that is cut every share leaves a part, and a second launch joins them.  (One CTA per item left the GPU idle behind the longest
 // rows: 64 rows of 130 to 500 tokens took 108 us, 16 of 8192 940.  Joining in the CTA whose part comes last, by counters, cost a row of 1000 tokens 3.7 us
-// of fences and atomics in a row; the second launch costs it less.  Small shares for whoever comes first, since SMs differ by a quarter in what they get of
-// the memory's bandwidth, cost more in parts than they evened out.)
+// of fences and atomics in a row; the second launch costs it less.  SMs differ by a quarter in what they get of the memory's bandwidth, so that of 16 rows of
+// 8192 tokens the first CTAs are done after 63 us and the last after 90; small shares for whoever comes first evened that out but cost more in parts and
+// in the count of those taken: 106 us in all against 95.)
 struct Token {
   int row, units;
   Span span;
@@ -161,12 +162,7 @@ struct Run {
 template <typename T_, int D_, int NB>
 struct TcEngine {
   using T = T_;
-#ifndef PAV_W
-#define PAV_W 5
-#define PAV_S 2
-#define PAV_C 2
-#endif
-  static constexpr int D = D_, MAX_D = D_, ROWS = 8 * NB, WARPS = PAV_W, STAGES = D_ > 80 ? PAV_S : D_ > 64 ? 3 : 4, CTAS = D_ > 128 ? 1 : PAV_C;
+  static constexpr int D = D_, MAX_D = D_, ROWS = 8 * NB, WARPS = 4, STAGES = D_ > 128 ? 2 : D_ > 64 ? 3 : 4, CTAS = D_ > 128 ? 1 : 2;
   static constexpr int CHUNKS = D / 8, PIECES = CHUNKS % 8 ? (CHUNKS | 1) : CHUNKS;    // 16-byte pieces of a staged line
   static constexpr int Q_STRIDE = D * 2 + 16, Q_BYTES = ROWS * Q_STRIDE;
   static constexpr int NQ = (ROWS * CHUNKS + WARPS * 32 - 1) / (WARPS * 32);
@@ -723,11 +719,42 @@ paged_attn_join_kernel(const __grid_constant__ PagedAttn a, unsigned ctas) {
   const int g = item / blocks, r0 = (item - g * blocks) * ROWS, rows = min(ROWS, per - r0);
   const int64_t head = (int64_t)t * a.H + (int64_t)g * per + r0;
   pdl_wait();
+  // with a mass: this thread's first slot and what its heads scored, on their way beside the parts
+  const bool weighs = a.mass != nullptr;
+  Token tok;
+  int seen = 0;
+  float w8[ROWS];
+  int64_t place = -1;
+  auto look = [&](int x) {
+    place = -1;
+    if (x >= seen) return;
+    const int j = tok.span.key0(x / PA_TILE) + x % PA_TILE;
+    if (!tok.span.visible(j)) return;
+    const int64_t id = page_id(a.pt, tok.row, j / a.pt.page);
+    if (id < 0) return;
+    place = (id * a.G + g) * a.pt.page + j % a.pt.page;
+    const float* p = a.scores + ((int64_t)blockIdx.x * a.cap + x) * a.pitch;
+    if (a.pitch >= 4) {
+#pragma unroll
+      for (int r = 0; r < ROWS; r += 4)
+        if (r < a.pitch) *reinterpret_cast<float4*>(w8 + r) = *reinterpret_cast<const float4*>(p + r);
+    } else {
+      w8[0] = p[0];
+      if (a.pitch > 1) w8[1] = p[1];
+    }
+  };
+  const int x0 = blockIdx.y * ROWS * 32 + threadIdx.x;
+  if (weighs) {
+    tok = Token(a, t, E::WARPS);
+    seen = tok.span.tiles * PA_TILE;
+    if (blockIdx.y > 0 && (int)(blockIdx.y * ROWS * 32) >= seen) return;
+    look(x0);
+  }
   const unsigned base = a.base[t], units = (a.base[t + 1] - base) / items, U = a.base[a.M];
   if (units == 0) return;                                         // an idle token
   const Shares sh(U, a.base[a.M + 1], ctas);
   const unsigned u0 = base + item * units, c0 = sh.of(u0), c1 = sh.of(u0 + units - 1);
-  if (c0 == c1 && !a.mass) return;
+  if (c0 == c1 && !weighs) return;
   if (c0 != c1 && warp < rows) {
     const int parts = (int)(c1 - c0) + 1;
     const int64_t size = (int64_t)ROWS * (D + 4);
@@ -747,7 +774,7 @@ paged_attn_join_kernel(const __grid_constant__ PagedAttn a, unsigned ctas) {
         ml[i] = at < parts ? *reinterpret_cast<const float2*>(p) : make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int x = 0; x < NQ4; ++x)
-          y[i][x] = at < parts && 4 * lane + 128 * x < D ? *reinterpret_cast<const float4*>(p + 4 + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+          y[i][x] = at < parts && blockIdx.y == 0 && 4 * lane + 128 * x < D ? *reinterpret_cast<const float4*>(p + 4 + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       float top = M;
 #pragma unroll
@@ -775,24 +802,18 @@ paged_attn_join_kernel(const __grid_constant__ PagedAttn a, unsigned ctas) {
     }
     if (lane == 0) s_stat[warp] = make_float2(M == -INFINITY ? 0.f : M, inv);
   }
-  if (!a.mass) return;
+  if (!weighs) return;
   if (c0 == c1 && (int)threadIdx.x < rows) s_stat[threadIdx.x] = reinterpret_cast<const float2*>(a.stat)[head + threadIdx.x];
   __syncthreads();
-  const Token tok(a, t, E::WARPS);
-  const int seen = tok.span.tiles * PA_TILE;
-  const float* sc = a.scores + (int64_t)blockIdx.x * a.cap * a.pitch;
 #pragma unroll 1
-  for (int x = blockIdx.y * ROWS * 32 + threadIdx.x; x < seen; x += gridDim.y * ROWS * 32) {
-    const int j = tok.span.key0(x / PA_TILE) + x % PA_TILE;
-    if (!tok.span.visible(j)) continue;
-    const int64_t id = page_id(a.pt, tok.row, j / a.pt.page);
-    if (id < 0) continue;
-    const float* p = sc + (int64_t)x * a.pitch;
+  for (int x = x0; x < seen; x += gridDim.y * ROWS * 32) {
+    if (x != x0) look(x);
+    if (place < 0) continue;
     float w = 0.f;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
-      if (r < rows) w += raise2(p[r] - s_stat[r].x) * s_stat[r].y;
-    atomicAdd(&a.mass[(id * a.G + g) * a.pt.page + j % a.pt.page], w);    // slots that several tokens see
+      if (r < rows) w += raise2(w8[r] - s_stat[r].x) * s_stat[r].y;
+    atomicAdd(a.mass + place, w);                                 // slots that several tokens see
   }
 }
 
@@ -833,7 +854,7 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   launch_pdl(kern, (unsigned)grid, E::WARPS * 32 + 32, smem, st, a);
   B200P_LAUNCH_CHECK("paged_attn_kernel");
   // slices of a mass: as many as there are, but no more CTAs than fill the GPU
-  const int64_t slices = a.mass ? (a.cap + E::ROWS * 32 - 1) / (E::ROWS * 32) : 1, fill = 8ll * sm_count() / ((int64_t)a.M * items) + 1;
+  const int64_t slices = a.mass ? (a.cap + E::ROWS * 32 - 1) / (E::ROWS * 32) : 1, fill = ((E::ROWS == 8 ? 6ll : 3ll) * sm_count() + a.M * items - 1) / ((int64_t)a.M * items);
   launch_pdl(paged_attn_join_kernel<E>, dim3((unsigned)(a.M * items), (unsigned)(slices < fill ? slices : fill)), E::ROWS * 32, 0, st, a, (unsigned)grid);
   B200P_LAUNCH_CHECK("paged_attn_join_kernel");
   return B200P_OK;
