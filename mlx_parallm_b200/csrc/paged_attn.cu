@@ -69,7 +69,7 @@ struct PagedAttn {
   int M, H, G, D, first, window, out_perm;
   float scale_log2e;
   // workspace
-  unsigned* base;      // [M + 2] units before every token; all units; items
+  uint2* parts;        // [M, items] the first of the shares an item lies in and their number (idle tokens': not written)
   float* rec;          // [shares, 2, rows of a block, D + 4] parts: maximum, sum, -, -, outputs
   float* stat;         // [M, H, 2] maximum and 1 / sum of the heads that lie in one share (with a mass)
   float* scores;       // [M, items, cap, pitch] log2-scaled scores (with a mass)
@@ -482,7 +482,7 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
   }
   pdl_launch_dependents();                                        // (the join waits for this launch's end; until then it has no room anyway)
   const Shares sh(U, n_items, gridDim.x);
-  if (blockIdx.x >= max(sh.n, 1u)) return;                        // (the first one writes down the plan, work or no work)
+  if (blockIdx.x >= sh.n) return;
   const unsigned ub = sh.begin(blockIdx.x);
 #pragma unroll 1
   for (int t = t0; t < t1; ++t) {
@@ -491,11 +491,8 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
       s.t = t;
       s.base = before;
     }
-    if (blockIdx.x == 0) a.base[t] = before;
     before += n;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.base[a.M] = U, a.base[a.M + 1] = n_items;
-  if (sh.n == 0) return;
   __syncthreads();
 
   // ---- the warp for the runs and the parts ----------------------------------------------------------------------------------
@@ -514,7 +511,10 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
         r.tile = c.a * W, r.tile_end = min(c.b * W, c.tok.span.tiles);
         r.span = c.tok.span;
         r.row = c.tok.row, r.head = c.t * a.H + r.g * per + r0, r.rows = min(E::ROWS, per - r0), r.line = c.t * items + c.item;
-        r.part = c.b - c.a < c.tok.units ? (int)blockIdx.x * 2 + (c.a == 0 ? 1 : 0) : -1;
+        const bool cut = c.b - c.a < c.tok.units;
+        r.part = cut ? (int)blockIdx.x * 2 + (c.a == 0 ? 1 : 0) : -1;
+        if (c.a == 0 && lane == 0)                                // for the join
+          a.parts[r.line] = make_uint2(blockIdx.x, cut ? sh.of(c.base + (c.item + 1) * c.tok.units - 1) - blockIdx.x + 1 : 1u);
       }
       if (lane == 0) s.run[n & 3] = r;
       if (n < 2) continue;
@@ -706,34 +706,92 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
   }
 }
 
-// What is left of an item (x): a warp per query head joins its parts where it was cut, with all their loads under way at once.  With a mass, CTAs
-// share the item's visible slots (y) and form the heads' maxima and sums anew, then a thread per slot adds up what the heads gave it.
-template <typename E>
-__global__ void __launch_bounds__(E::ROWS * 32)
-paged_attn_join_kernel(const __grid_constant__ PagedAttn a, unsigned ctas) {
-  constexpr int ROWS = E::ROWS, NQ4 = E::MAX_D > 128 ? 2 : 1, AHEAD = 16 / NQ4;
-  __shared__ float2 s_stat[ROWS];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = E::dim(a);
-  const int per = a.H / a.G, blocks = (per + ROWS - 1) / ROWS, items = a.G * blocks;
-  const int t = blockIdx.x / items, item = blockIdx.x - t * items;
-  const int g = item / blocks, r0 = (item - g * blocks) * ROWS, rows = min(ROWS, per - r0);
-  const int64_t head = (int64_t)t * a.H + (int64_t)g * per + r0;
+// Part i of an item that lies in the shares from c0 on: the first is its share's second, the others are their shares' first.
+__device__ __forceinline__ const float* part_at(const PagedAttn& a, unsigned c0, unsigned i, int rows, int row) {
+  return a.rec + (((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * rows + row) * (a.D + 4);
+}
+
+// A CTA per token and query head joins the parts where the item was cut: four warps take them in turn, then become one.  Few instructions: a launch
+// this short waits for its code more than for its data.
+constexpr int PJ_WARPS = 4;
+
+template <typename T, int NQ>            // 128 dimensions of a warp's lanes, NQ times
+__global__ void __launch_bounds__(PJ_WARPS * 32)
+paged_attn_join_kernel(const __grid_constant__ PagedAttn a, int rows_log2) {
+  __shared__ float2 s_ml[PJ_WARPS];
+  __shared__ float4 s_o[PJ_WARPS][32 * NQ];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.x, g = blockIdx.y, t = blockIdx.z, block_rows = 1 << rows_log2, blk = r >> rows_log2, row = r & (block_rows - 1);
+  const int blocks = (gridDim.x + block_rows - 1) >> rows_log2;
   pdl_wait();
-  // with a mass: this thread's first slot and what its heads scored, on their way beside the parts
-  const bool weighs = a.mass != nullptr;
-  Token tok;
-  int seen = 0;
+  const int token_row = a.t_row[t];
+  const uint2 parts = a.parts[((int64_t)t * a.G + g) * blocks + blk];
+  if (token_row < 0 || token_row >= a.pt.rows || parts.y < 2) return;
+  float M = -INFINITY, L = 0.f;
+  float4 acc[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (unsigned i = warp; i < parts.y; i += PJ_WARPS) {
+    const float* p = part_at(a, parts.x, i, block_rows, row);
+    const float2 ml = *reinterpret_cast<const float2*>(p);
+    const float top = fmaxf(M, ml.x), ref = top == -INFINITY ? 0.f : top, f = raise2(M - ref), w = raise2(ml.x - ref);
+    M = top;
+    L = L * f + ml.y * w;
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      const float4 y = 4 * lane + 128 * x < a.D ? *reinterpret_cast<const float4*>(p + 4 + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+      acc[x].x = acc[x].x * f + y.x * w, acc[x].y = acc[x].y * f + y.y * w, acc[x].z = acc[x].z * f + y.z * w, acc[x].w = acc[x].w * f + y.w * w;
+    }
+  }
+  if (lane == 0) s_ml[warp] = make_float2(M, L);
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) s_o[warp][lane + 32 * x] = acc[x];
+  __syncthreads();
+  const int d = 4 * threadIdx.x;
+  if (d >= a.D) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < PJ_WARPS; ++w) top = fmaxf(top, s_ml[w].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < PJ_WARPS; ++w) {
+    const float f = raise2(s_ml[w].x - ref);
+    const float4 y = s_o[w][threadIdx.x];
+    sum += s_ml[w].y * f;
+    o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  store_row4<T>(reinterpret_cast<T*>(a.out) + ((int64_t)t * a.H + g * gridDim.x + r) * a.D, d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), a.out_perm);
+}
+
+// The weights that every visible slot received: a CTA per item (x) and slice of its visible slots (y), a thread per slot.  The heads' maxima and sums
+// come from the parts again (a warp per head, a lane per part), which needs no word from the join.
+template <int ROWS>
+__global__ void __launch_bounds__(256)
+paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks, int warps) {
+  __shared__ float2 s_stat[ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, items = a.G * blocks;
+  const int t = blockIdx.z, item = blockIdx.y, g = blocks == 1 ? item : item / blocks, r0 = (item - g * blocks) * ROWS, rows = min(ROWS, per - r0);
+  const int64_t head = (int64_t)t * a.H + (int64_t)g * per + r0, line = (int64_t)t * items + item;
+  pdl_wait();
+  const Token tok(a, t, warps);
+  const uint2 parts = a.parts[line];
+  const int seen = tok.span.tiles * PA_TILE;
+  if ((int)blockIdx.x * 256 >= seen) return;
   float w8[ROWS];
   int64_t place = -1;
-  auto look = [&](int x) {
+  auto look = [&](int x) {                                        // a slot's place and what its heads scored
     place = -1;
     if (x >= seen) return;
-    const int j = tok.span.key0(x / PA_TILE) + x % PA_TILE;
+    const int kt = tok.span.key_tile(x / PA_TILE), j = kt * PA_TILE + x % PA_TILE, index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 40);
     if (!tok.span.visible(j)) return;
-    const int64_t id = page_id(a.pt, tok.row, j / a.pt.page);
+    const int64_t id = page_id(a.pt, tok.row, index);
     if (id < 0) return;
-    place = (id * a.G + g) * a.pt.page + j % a.pt.page;
-    const float* p = a.scores + ((int64_t)blockIdx.x * a.cap + x) * a.pitch;
+    place = (id * a.G + g) * a.pt.page + (kt - index * a.tpp) * PA_TILE + x % PA_TILE;
+    const float* p = a.scores + (line * a.cap + x) * a.pitch;
     if (a.pitch >= 4) {
 #pragma unroll
       for (int r = 0; r < ROWS; r += 4)
@@ -743,70 +801,30 @@ paged_attn_join_kernel(const __grid_constant__ PagedAttn a, unsigned ctas) {
       if (a.pitch > 1) w8[1] = p[1];
     }
   };
-  const int x0 = blockIdx.y * ROWS * 32 + threadIdx.x;
-  if (weighs) {
-    tok = Token(a, t, E::WARPS);
-    seen = tok.span.tiles * PA_TILE;
-    if (blockIdx.y > 0 && (int)(blockIdx.y * ROWS * 32) >= seen) return;
-    look(x0);
-  }
-  const unsigned base = a.base[t], units = (a.base[t + 1] - base) / items, U = a.base[a.M];
-  if (units == 0) return;                                         // an idle token
-  const Shares sh(U, a.base[a.M + 1], ctas);
-  const unsigned u0 = base + item * units, c0 = sh.of(u0), c1 = sh.of(u0 + units - 1);
-  if (c0 == c1 && !weighs) return;
-  if (c0 != c1 && warp < rows) {
-    const int parts = (int)(c1 - c0) + 1;
-    const int64_t size = (int64_t)ROWS * (D + 4);
-    const float* first = a.rec + ((int64_t)c0 * 2 + 1) * size + warp * (D + 4);
-    float M = -INFINITY, L = 0.f;
-    float4 acc[NQ4];
-#pragma unroll
-    for (int x = 0; x < NQ4; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int x0 = blockIdx.x * 256 + threadIdx.x;
+  look(x0);                                                       // on its way beside the parts
 #pragma unroll 1
-    for (int i0 = 0; i0 < parts; i0 += AHEAD) {
-      float2 ml[AHEAD];
-      float4 y[AHEAD][NQ4];
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {                           // part i > 0 is the first of its share's two
-        const int at = i0 + i;
-        const float* p = first + (at == 0 ? 0 : (2 * (int64_t)at - 1) * size);
-        ml[i] = at < parts ? *reinterpret_cast<const float2*>(p) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int x = 0; x < NQ4; ++x)
-          y[i][x] = at < parts && blockIdx.y == 0 && 4 * lane + 128 * x < D ? *reinterpret_cast<const float4*>(p + 4 + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r = warp; r < rows; r += 8) {
+    float2 st;
+    if (parts.y < 2) {
+      st = reinterpret_cast<const float2*>(a.stat)[head + r];
+    } else {
+      float M = -INFINITY, L = 0.f;
+#pragma unroll 1
+      for (unsigned i = lane; i < parts.y; i += 32) {
+        const float2 ml = *reinterpret_cast<const float2*>(part_at(a, parts.x, i, ROWS, r));
+        const float top = fmaxf(M, ml.x), ref = top == -INFINITY ? 0.f : top;
+        L = L * raise2(M - ref) + ml.y * raise2(ml.x - ref);
+        M = top;
       }
-      float top = M;
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
-      const float ref = top == -INFINITY ? 0.f : top, f = raise2(M - ref);
-      M = top;
-      L *= f;
-#pragma unroll
-      for (int x = 0; x < NQ4; ++x) acc[x].x *= f, acc[x].y *= f, acc[x].z *= f, acc[x].w *= f;
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const float w = raise2(ml[i].x - ref);
-        L += ml[i].y * w;
-#pragma unroll
-        for (int x = 0; x < NQ4; ++x) acc[x].x += y[i][x].x * w, acc[x].y += y[i][x].y * w, acc[x].z += y[i][x].z * w, acc[x].w += y[i][x].w * w;
-      }
+      const float top = warp_max(M), ref = top == -INFINITY ? 0.f : top, sum = warp_sum(L * raise2(M - ref));
+      st = make_float2(ref, sum == 0.f ? 0.f : 1.f / sum);
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    if (blockIdx.y == 0) {
-#pragma unroll
-      for (int x = 0; x < NQ4; ++x)
-        if (4 * lane + 128 * x < D)
-          store_row4<typename E::T>(reinterpret_cast<typename E::T*>(a.out) + (head + warp) * D, 4 * lane + 128 * x,
-                                    make_float4(acc[x].x * inv, acc[x].y * inv, acc[x].z * inv, acc[x].w * inv), a.out_perm);
-    }
-    if (lane == 0) s_stat[warp] = make_float2(M == -INFINITY ? 0.f : M, inv);
+    if (lane == 0) s_stat[r] = st;
   }
-  if (!weighs) return;
-  if (c0 == c1 && (int)threadIdx.x < rows) s_stat[threadIdx.x] = reinterpret_cast<const float2*>(a.stat)[head + threadIdx.x];
   __syncthreads();
 #pragma unroll 1
-  for (int x = x0; x < seen; x += gridDim.y * ROWS * 32) {
+  for (int x = x0; x < seen; x += gridDim.x * 256) {
     if (x != x0) look(x);
     if (place < 0) continue;
     float w = 0.f;
@@ -825,7 +843,7 @@ static int64_t visible_cap(int64_t slots, int64_t first, int64_t window) {
 }
 
 static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-static size_t base_bytes(int64_t M) { return round256((size_t)(M + 2) * 4); }
+static size_t parts_bytes(int64_t M, int H) { return round256((size_t)M * H * 8); }      // (no more items than heads)
 static size_t rec_bytes(int D) { return round256((size_t)sm_count() * 2 * 2 * 16 * (D + 4) * 4); }      // (two CTAs per SM at most)
 static size_t stat_bytes(int64_t M, int H) { return round256((size_t)M * H * 8); }
 
@@ -833,7 +851,7 @@ template <typename E>
 static int launch_paged(PagedAttn a, cudaStream_t st) {
   const int smem = E::Q_BYTES + E::WARPS * E::STAGES * E::tile_bytes(a.D);
   const int blocks = (a.H / a.G + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
-  B200P_REQUIRE((int64_t)a.M * items * (a.cap / PA_TILE / E::WARPS + 1) < (1ll << 31), B200P_ERR_ARG,
+  B200P_REQUIRE((int64_t)a.M * items * (a.cap / PA_TILE / E::WARPS + 1) < (1ll << 31) && items < 65536, B200P_ERR_ARG,
                 "%d tokens of %d key heads over %d slots: too many for one call", a.M, a.G, a.cap);
   auto kern = paged_attn_kernel<E>;
   static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
@@ -853,10 +871,20 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   while (a.pitch < E::ROWS && a.pitch < a.H / a.G) a.pitch *= 2;
   launch_pdl(kern, (unsigned)grid, E::WARPS * 32 + 32, smem, st, a);
   B200P_LAUNCH_CHECK("paged_attn_kernel");
-  // slices of a mass: as many as there are, but no more CTAs than fill the GPU
-  const int64_t slices = a.mass ? (a.cap + E::ROWS * 32 - 1) / (E::ROWS * 32) : 1, fill = ((E::ROWS == 8 ? 6ll : 3ll) * sm_count() + a.M * items - 1) / ((int64_t)a.M * items);
-  launch_pdl(paged_attn_join_kernel<E>, dim3((unsigned)(a.M * items), (unsigned)(slices < fill ? slices : fill)), E::ROWS * 32, 0, st, a, (unsigned)grid);
+  using T = typename E::T;
+  const int per = a.H / a.G, rows_log2 = E::ROWS == 8 ? 3 : 4;
+  const dim3 heads((unsigned)per, (unsigned)a.G, (unsigned)a.M);
+  if (a.D <= 128)
+    launch_pdl(paged_attn_join_kernel<T, 1>, heads, PJ_WARPS * 32, 0, st, a, rows_log2);
+  else
+    launch_pdl(paged_attn_join_kernel<T, 2>, heads, PJ_WARPS * 32, 0, st, a, rows_log2);
   B200P_LAUNCH_CHECK("paged_attn_join_kernel");
+  if (!a.mass) return B200P_OK;
+  // slices of the visible slots: as many as there are, but no more CTAs than fill the GPU
+  const int64_t slices = (a.cap + 255) / 256, fill = (6ll * sm_count() + (int64_t)a.M * items - 1) / ((int64_t)a.M * items);
+  launch_pdl(paged_attn_mass_kernel<E::ROWS>, dim3((unsigned)(slices < fill ? slices : fill), (unsigned)items, (unsigned)a.M), 256, 0, st, a, per, blocks,
+             (int)E::WARPS);
+  B200P_LAUNCH_CHECK("paged_attn_mass_kernel");
   return B200P_OK;
 }
 
@@ -881,7 +909,7 @@ using namespace b200p;
 
 extern "C" size_t b200p_paged_attn_workspace_bytes(int64_t M, int H, int D, int64_t keys) {
   if (M <= 0 || H <= 0 || D <= 0) return 0;
-  size_t n = base_bytes(M) + rec_bytes(D);
+  size_t n = parts_bytes(M, H) + rec_bytes(D);
   if (keys > 0) n += stat_bytes(M, H) + (size_t)M * H * 2 * ((keys + PA_TILE - 1) / PA_TILE * PA_TILE) * 4;     // (pitch < 2 x heads)
   return n;
 }
@@ -911,8 +939,8 @@ extern "C" int b200p_paged_attn(const void* q, const void* kpages, const void* v
   a.M = (int)M, a.H = H, a.G = G, a.D = D, a.first = (int)first, a.window = (int)window, a.out_perm = (flags & B200P_OUT_PERM8) ? 1 : 0;
   a.scale_log2e = scale * 1.4426950408889634f, a.cap = (int)cap;
   uint8_t* ws = (uint8_t*)workspace;
-  a.base = (unsigned*)ws;
-  a.rec = (float*)(ws += base_bytes(M));
+  a.parts = (uint2*)ws;
+  a.rec = (float*)(ws += parts_bytes(M, H));
   a.stat = (float*)(ws += rec_bytes(D));
   a.scores = (float*)(ws + stat_bytes(M, H));
   B200P_DISPATCH_DTYPE(dtype, T, return (launch_paged_type<T>(a, (cudaStream_t)stream)));
