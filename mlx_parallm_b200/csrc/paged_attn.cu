@@ -294,15 +294,17 @@ struct TcEngine {
   }
 };
 
-// Every type and size, in fp32 FMAs: two lanes share a key for the scores, for the outputs a lane owns 4 (NG 2: 8) dimensions of 8 query heads.
-template <typename T_, int NG>
+// Every type and size, in fp32 FMAs, R query heads at a time: four lanes share two keys for the scores, for the outputs a lane owns 4 (NG 2: 8)
+// dimensions of every head, so that a 16-byte piece of queries or weights read from shared memory serves 8 or 16 products.
+template <typename T_, int NG, int R>
 struct FmaEngine {
   using T = T_;
-  static constexpr int MAX_D = 128 * NG, ROWS = 8, WARPS = sizeof(T_) == 4 && NG == 2 ? 2 : 4, STAGES = 2, CTAS = 1;
+  static constexpr int MAX_D = 128 * NG, ROWS = R, STAGES = 2, CTAS = 1;
+  static constexpr int WARPS = sizeof(T_) * NG == 8 ? 3 : 6;
   static constexpr int E = 16 / (int)sizeof(T_);
   static constexpr int Q_BYTES = (ROWS * NG * 128 + WARPS * ROWS * PA_TILE) * 4;     // queries and every warp's weights, fp32
   static constexpr int NQ = (ROWS * NG * 128 / E + WARPS * 32 - 1) / (WARPS * 32);
-  float o[ROWS][NG][4], m[ROWS], l[ROWS];
+  float o[ROWS][NG][4], m[ROWS], l[ROWS];                         // l: this lane's two keys' share
 
   static __device__ __forceinline__ int dim(const PagedAttn& a) { return a.D; }
   static __host__ __device__ __forceinline__ int line(int D) { return (D / E | 1) * 16; }
@@ -321,67 +323,92 @@ struct FmaEngine {
       for (int x = 0; x < NG; ++x) o[r][x][0] = o[r][x][1] = o[r][x][2] = o[r][x][3] = 0.f;
     }
   }
-  __device__ __forceinline__ void tile(const PagedAttn& a, uint32_t qs_, uint32_t, int j0, const Span& sp, bool all, bool page, float* sc, int rows,
+  __device__ __forceinline__ void tile(const PagedAttn& a, uint32_t, uint32_t, int j0, const Span& sp, bool all, bool page, float* sc, int rows,
                                        uint8_t* ks) {
-    const int lane = threadIdx.x & 31, key = lane & 15, half = lane >> 4, D = a.D, chunks = D / E, stride = line(D);
+    const int lane = threadIdx.x & 31, key = lane & 7, quarter = lane >> 3, D = a.D, chunks = D / E, stride = line(D);
     const uint8_t* vs = ks + PA_TILE * stride;
     extern __shared__ __align__(16) uint8_t smem[];
     const float* qs = reinterpret_cast<const float*>(smem);
     float* ps = reinterpret_cast<float*>(smem) + ROWS * NG * 128 + (threadIdx.x >> 5) * ROWS * PA_TILE;
-    float s[ROWS];
+    float s[ROWS][2];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) s[r] = 0.f;
+    for (int r = 0; r < ROWS; ++r) s[r][0] = s[r][1] = 0.f;
 #pragma unroll 1
-    for (int c = half; c < chunks; c += 2) {
-      T kv[E];
-      *reinterpret_cast<uint4*>(kv) = *reinterpret_cast<const uint4*>(ks + key * stride + c * 16);
+    for (int c = quarter; c < chunks; c += 4) {
+      T k0[E], k1[E];
+      *reinterpret_cast<uint4*>(k0) = *reinterpret_cast<const uint4*>(ks + key * stride + c * 16);
+      *reinterpret_cast<uint4*>(k1) = *reinterpret_cast<const uint4*>(ks + (key + 8) * stride + c * 16);
 #pragma unroll
-      for (int e = 0; e < E; e += 4) {
+      for (int e = 0; e < E; e += 4)
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-          if (r < rows) {
-            const float4 q = *reinterpret_cast<const float4*>(qs + r * D + c * E + e);
-            s[r] = fmaf(Tr<T>::to_f(kv[e]), q.x, s[r]);
-            s[r] = fmaf(Tr<T>::to_f(kv[e + 1]), q.y, s[r]);
-            s[r] = fmaf(Tr<T>::to_f(kv[e + 2]), q.z, s[r]);
-            s[r] = fmaf(Tr<T>::to_f(kv[e + 3]), q.w, s[r]);
-          }
-      }
+        for (int r = 0; r < ROWS; ++r) {                          // (queries of absent heads are zeros)
+          const float4 q = *reinterpret_cast<const float4*>(qs + r * D + c * E + e);
+          s[r][0] = fmaf(Tr<T>::to_f(k0[e]), q.x, s[r][0]);
+          s[r][1] = fmaf(Tr<T>::to_f(k1[e]), q.x, s[r][1]);
+          s[r][0] = fmaf(Tr<T>::to_f(k0[e + 1]), q.y, s[r][0]);
+          s[r][1] = fmaf(Tr<T>::to_f(k1[e + 1]), q.y, s[r][1]);
+          s[r][0] = fmaf(Tr<T>::to_f(k0[e + 2]), q.z, s[r][0]);
+          s[r][1] = fmaf(Tr<T>::to_f(k1[e + 2]), q.z, s[r][1]);
+          s[r][0] = fmaf(Tr<T>::to_f(k0[e + 3]), q.w, s[r][0]);
+          s[r][1] = fmaf(Tr<T>::to_f(k1[e + 3]), q.w, s[r][1]);
+        }
     }
-    const bool seen = all || (page && sp.visible(j0 + key));
+    const bool seen0 = all || (page && sp.visible(j0 + key)), seen1 = all || (page && sp.visible(j0 + key + 8));
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      if (r >= rows) break;
-      float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * a.scale_log2e;
-      x = seen ? x : -INFINITY;
-      if (sc && half == 0) sc[key * a.pitch + r] = x;
-      const float t = fmaxf(m[r], warp_max(x));
+      float x = s[r][0], y = s[r][1];
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      y += __shfl_xor_sync(0xffffffffu, y, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      y += __shfl_xor_sync(0xffffffffu, y, 16);
+      x = seen0 ? x * a.scale_log2e : -INFINITY;
+      y = seen1 ? y * a.scale_log2e : -INFINITY;
+      if (sc && quarter == 0 && r < rows) {
+        sc[key * a.pitch + r] = x;
+        sc[(key + 8) * a.pitch + r] = y;
+      }
+      float t = fmaxf(x, y);
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+      t = fmaxf(t, m[r]);
       const float ref = t == -INFINITY ? 0.f : t;
-      const float f = raise2(m[r] - ref), p = raise2(x - ref);
+      const float f = raise2(m[r] - ref), p0 = raise2(x - ref), p1 = raise2(y - ref);
       m[r] = t;
-      l[r] = l[r] * f + warp_sum(half == 0 ? p : 0.f);
-      if (half == 0) ps[r * PA_TILE + key] = p;
+      l[r] = l[r] * f + (p0 + p1);
+      if (quarter == 0) {
+        ps[r * PA_TILE + key] = p0;
+        ps[r * PA_TILE + key + 8] = p1;
+      }
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[r][g][e] *= f;
     }
     __syncwarp();
-#pragma unroll 2
-    for (int k = 0; k < PA_TILE; ++k)
+#pragma unroll 1
+    for (int k = 0; k < PA_TILE; k += 4) {
+      float4 w[ROWS];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) w[r] = *reinterpret_cast<const float4*>(ps + r * PA_TILE + k);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const int d = (lane + 32 * g) * 4;
         if (d >= D) break;
-        T vv[4];
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(vv) = *reinterpret_cast<const uint4*>(vs + k * stride + d * 4);
-        else *reinterpret_cast<uint2*>(vv) = *reinterpret_cast<const uint2*>(vs + k * stride + d * 2);
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-          if (r < rows)
+        for (int i = 0; i < 4; ++i) {
+          T vv[4];
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(vv) = *reinterpret_cast<const uint4*>(vs + (k + i) * stride + d * 4);
+          else *reinterpret_cast<uint2*>(vv) = *reinterpret_cast<const uint2*>(vs + (k + i) * stride + d * 2);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[r][g][e] = fmaf(ps[r * PA_TILE + k], Tr<T>::to_f(vv[e]), o[r][g][e]);
+          for (int r = 0; r < ROWS; ++r) {
+            const float p = i == 0 ? w[r].x : i == 1 ? w[r].y : i == 2 ? w[r].z : w[r].w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[r][g][e] = fmaf(p, Tr<T>::to_f(vv[e]), o[r][g][e]);
+          }
+        }
       }
+    }
   }
   static __device__ __forceinline__ uint32_t at(int key, int c, int D) { return (uint32_t)(key * line(D) + c * 16); }
   __device__ __forceinline__ void publish(float* p, int, int D) {
@@ -389,7 +416,11 @@ struct FmaEngine {
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       float* row = p + r * (D + 4);
-      if (lane == 0) { row[0] = m[r]; row[1] = l[r]; }
+      float sum = l[r];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      if (lane == 0) { row[0] = m[r]; row[1] = sum; }
 #pragma unroll
       for (int g = 0; g < NG; ++g)
         if ((lane + 32 * g) * 4 < D) *reinterpret_cast<float4*>(row + 4 + (lane + 32 * g) * 4) = make_float4(o[r][g][0], o[r][g][1], o[r][g][2], o[r][g][3]);
@@ -872,7 +903,7 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   launch_pdl(kern, (unsigned)grid, E::WARPS * 32 + 32, smem, st, a);
   B200P_LAUNCH_CHECK("paged_attn_kernel");
   using T = typename E::T;
-  const int per = a.H / a.G, rows_log2 = E::ROWS == 8 ? 3 : 4;
+  const int per = a.H / a.G, rows_log2 = E::ROWS == 4 ? 2 : E::ROWS == 8 ? 3 : 4;
   const dim3 heads((unsigned)per, (unsigned)a.G, (unsigned)a.M);
   if (a.D <= 128)
     launch_pdl(paged_attn_join_kernel<T, 1>, heads, PJ_WARPS * 32, 0, st, a, rows_log2);
@@ -900,7 +931,9 @@ static int launch_paged_type(const PagedAttn& a, cudaStream_t st) {
       case 256: return launch_paged<TcEngine<T, 256, 1>>(a, st);     // (16 heads do not fit the registers)
     }
   }
-  return a.D <= 128 ? launch_paged<FmaEngine<T, 1>>(a, st) : launch_paged<FmaEngine<T, 2>>(a, st);
+  const bool four = a.H / a.G <= 4;
+  if (a.D <= 128) return four ? launch_paged<FmaEngine<T, 1, 4>>(a, st) : launch_paged<FmaEngine<T, 1, 8>>(a, st);
+  return four ? launch_paged<FmaEngine<T, 2, 4>>(a, st) : launch_paged<FmaEngine<T, 2, 8>>(a, st);
 }
 
 }  // namespace b200p
