@@ -13,9 +13,141 @@ __device__ unsigned int g_paged_fault = 0;
 int paged_attn_faults(unsigned int* count, int reset, cudaStream_t st);
 
 // ------------------------------------------------------------------------------------------------ append
-// One CTA per token.  Angles: position * rate in double precision, reduced to a turn there (positions of 10^6 times a rate of one leave fp32
-// with an error of 0.06 rad); sine and cosine once per pair, shared by all heads.  A warp per head: mean square, weights and rotation in
-// fp32, one rounding at the end.
+// Sine and cosine of position * rate: the product in double precision, reduced to a turn there (positions of 10^6 times a rate of one leave fp32 with
+// an error of 0.06 rad).
+__device__ __forceinline__ float2 turn(int pos, float rate) {
+  const double turns = (double)pos * (double)rate * 0.15915494309189535;
+  float2 sc;
+  sincospif((float)((turns - rint(turns)) * 2.0), &sc.x, &sc.y);
+  return sc;
+}
+
+// Every head is split over 2^width_log2 lanes (the power of two that holds D / 8), 8 neighbouring values a lane: one to two 16-byte loads and stores, the
+// mean square by shuffles, a rotation partner from the lane that has it (pairs of halves) or from this one (neighbours).  A lane keeps its 8 angles and
+// walks over heads, two asked for at a time; a CTA holds 2^tpc_log2 tokens, each with (256 >> width_log2) >> tpc_log2 walkers, and where the tokens are few
+// gridDim.y CTAs share a token's heads.  fp32 from the read to the one rounding.  Bound by HBM from some hundred tokens on.  (A CTA per token, a warp per
+// head and an element per lane took 114 us for 6004 tokens of 64 + 16 heads.)
+template <typename T, typename TIN>
+__global__ void __launch_bounds__(256)
+paged_append_rows_kernel(TIN* qkv, int64_t ldq, T* q_out, T* kp, T* vp, float* mass, PageTable pt, const int32_t* t_row, const int32_t* t_slot,
+                         const int32_t* t_pos, const T* qw, const T* kw, const float* rates, int n_rot, int pairs, float eps, int M, int H, int G, int D,
+                         int width_log2, int tpc_log2) {
+  constexpr bool ACC_IN = !std::is_same<TIN, T>::value;
+  constexpr int AHEAD = 2, IN = sizeof(TIN) * 8 / 16, OUT = sizeof(T) * 8 / 16;      // 16-byte pieces of 8 values
+  __shared__ float2 s_turn[8][128];
+  const int tpc = 1 << tpc_log2, width = 1 << width_log2, token0 = blockIdx.x << tpc_log2;
+  pdl_wait();
+  for (int i = threadIdx.x; i < n_rot << tpc_log2; i += 256) {
+    const int k = i & (tpc - 1), pair = i >> tpc_log2;
+    if (token0 + k < M) s_turn[k][pair] = turn(t_pos[token0 + k], rates[pair]);
+  }
+  const int c = threadIdx.x & (width - 1), slot = threadIdx.x >> width_log2;
+  const int k = slot & (tpc - 1), t = min(token0 + k, M - 1), step = (256 >> width_log2) >> tpc_log2;
+  const bool mine = token0 + k < M && c < D / 8;
+  const int row = t_row[t], place = t_slot[t], heads = H + 2 * G;
+  const bool live = row >= 0 && row < pt.rows;
+  int64_t id = -1;
+  if (live && place >= 0 && place < table_slots(pt)) id = page_id(pt, row, place / pt.page);
+  if (mine && c == 0 && slot < tpc && blockIdx.y == 0 && (row >= pt.rows || (live && id < 0))) atomicAdd(&g_paged_fault, 1u);
+  const int off = id < 0 ? 0 : place % pt.page;
+  __syncthreads();
+  // out = x * cs + partner * sn
+  float cs[8], sn[8];
+  int partner = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int e = 8 * c + j;
+    cs[j] = 1.f;
+    sn[j] = 0.f;
+    if (e < 2 * n_rot) {
+      const float2 sc = s_turn[k][pairs ? e >> 1 : (e < n_rot ? e : e - n_rot)];
+      cs[j] = sc.y;
+      sn[j] = (pairs ? (e & 1) : e >= n_rot) ? sc.x : -sc.x;
+    }
+  }
+  if (!pairs && 8 * c < 2 * n_rot) partner += 8 * c < n_rot ? n_rot / 8 : -(n_rot / 8);
+  TIN* src = qkv + (int64_t)t * ldq + 8 * c;
+  const int first = (int)blockIdx.y * step + (slot >> tpc_log2), stride = step * gridDim.y;
+  uint4 in[AHEAD][IN];
+  auto fetch = [&](int head0) {
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+      if (mine && (live || ACC_IN) && head0 + a * stride < heads) {
+        uint4* p = reinterpret_cast<uint4*>(src + (int64_t)(head0 + a * stride) * D);
+#pragma unroll
+        for (int i = 0; i < IN; ++i) {
+          in[a][i] = p[i];
+          if (ACC_IN) p[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
+  };
+  fetch(first);
+#pragma unroll 1
+  for (int base = 0; base < heads; base += AHEAD * stride) {      // the same number of turns for every lane of a warp
+    uint4 now[AHEAD][IN];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+      for (int i = 0; i < IN; ++i) now[a][i] = in[a][i];
+    fetch(base + first + AHEAD * stride);
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int head = base + first + a * stride;
+      const bool ok = mine && live && head < heads;
+      float x[8];
+      const TIN* v = reinterpret_cast<const TIN*>(now[a]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = ok ? Tr<TIN>::to_f(v[j]) : 0.f;
+        if (ACC_IN) x[j] = Tr<T>::to_f(Tr<T>::from_f(x[j]));
+      }
+      if (qw || kw) {
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+        for (int o = 1; o < width; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const T* w = head < H ? qw : head < H + G ? kw : nullptr;
+        if (w && ok) {
+          const float inv = 1.f / sqrtf(ss / (float)D + eps);
+          uint4 wv[OUT];
+#pragma unroll
+          for (int i = 0; i < OUT; ++i) wv[i] = reinterpret_cast<const uint4*>(w + 8 * c)[i];
+          const T* wf = reinterpret_cast<const T*>(wv);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] *= inv * Tr<T>::to_f(wf[j]);
+        }
+      }
+      if (n_rot) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = pairs ? x[j ^ 1] : __shfl_sync(0xffffffffu, x[j], partner);
+        if (head < H + G)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = x[j] * cs[j] + y[j] * sn[j];
+      }
+      if (!ok) continue;
+      T* dst;
+      if (head < H) {
+        dst = q_out + ((int64_t)t * H + head) * D;
+      } else {
+        if (id < 0) continue;
+        const int g = head < H + G ? head - H : head - H - G;
+        const int64_t at = (id * G + g) * pt.page + off;
+        dst = (head < H + G ? kp : vp) + at * D;
+        if (mass && head < H + G && c == 0) mass[at] = 0.f;
+      }
+      uint4 out[OUT];
+      T* f = reinterpret_cast<T*>(out);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = Tr<T>::from_f(x[j]);
+#pragma unroll
+      for (int i = 0; i < OUT; ++i) reinterpret_cast<uint4*>(dst + 8 * c)[i] = out[i];
+    }
+  }
+}
+
+// The same for what the lanes above do not hold (halves that are no multiple of 8 values apart, rows that are not 16-byte aligned): one CTA per token, a
+// warp per head.
 template <typename T, typename TIN>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(TIN* qkv, int64_t ldq, T* q_out, T* kp, T* vp, float* mass, PageTable pt, const int32_t* t_row, const int32_t* t_slot,
@@ -31,8 +163,9 @@ paged_append_kernel(TIN* qkv, int64_t ldq, T* q_out, T* kp, T* vp, float* mass, 
   if (live) {
     if (slot >= 0 && slot < table_slots(pt)) id = page_id(pt, row, slot / pt.page);
     for (int i = threadIdx.x; i < n_rot; i += blockDim.x) {
-      const double turns = (double)t_pos[t] * (double)rates[i] * 0.15915494309189535;
-      sincospif((float)((turns - rint(turns)) * 2.0), &sn[i], &cs[i]);
+      const float2 sc = turn(t_pos[t], rates[i]);
+      sn[i] = sc.x;
+      cs[i] = sc.y;
     }
   }
   if (threadIdx.x == 0 && (row >= pt.rows || (live && id < 0))) atomicAdd(&g_paged_fault, 1u);
@@ -220,32 +353,56 @@ paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int3
 }
 
 // ------------------------------------------------------------------------------------------------ dense view
-// A page of a head is one run in the pages and one run of the dense cache: CTAs copy runs.
-__global__ void __launch_bounds__(256)
+// A CTA copies GATHER_BYTES' worth of slots of one key head's keys and values, whatever the pages: a thread asks for four pieces of either before it
+// stores the first.  (A CTA per page and one piece at a time: 18.4 us for 7777 tokens of 8 heads, 64 MB moved.)
+constexpr int GATHER_THREADS = 256, GATHER_AHEAD = 4;
+
+__global__ void __launch_bounds__(GATHER_THREADS)
 paged_gather_kernel(const uint4* kp, const uint4* vp, PageTable pt, const int32_t* rows, const int32_t* lengths, uint4* kc, uint4* vc, int extra, int G,
-                    int chunks, int64_t Tcap) {
-  const int g = blockIdx.y, i = blockIdx.z, r = rows[i];
+                    int chunks, unsigned inv_chunks, int slots, int64_t Tcap) {
+  const int g = blockIdx.y, i = blockIdx.z;
+  pdl_wait();
+  const int r = rows[i];
   if (r < 0) return;
   if (r >= pt.rows) {
-    if (threadIdx.x == 0) atomicAdd(&g_paged_fault, 1u);
+    if (threadIdx.x == 0 && blockIdx.x == 0 && g == 0) atomicAdd(&g_paged_fault, 1u);
     return;
   }
   int64_t n = (int64_t)lengths[r] + extra;
   if (n > table_slots(pt)) n = table_slots(pt);
   if (n > Tcap) n = Tcap;
-  const int64_t j0 = (int64_t)blockIdx.x * pt.page;
+  const int j0 = blockIdx.x * slots;
   if (j0 >= n) return;
-  const int64_t id = page_id(pt, r, blockIdx.x);
-  if (id < 0) {
-    if (threadIdx.x == 0) atomicAdd(&g_paged_fault, 1u);
-    return;
+  const int count = (int)(n - j0 < slots ? n - j0 : slots) * chunks;
+  const int64_t dst = (((int64_t)i * G + g) * Tcap + j0) * chunks;
+  bool missing = false;
+  for (int x0 = threadIdx.x; x0 < count; x0 += GATHER_AHEAD * GATHER_THREADS) {
+    uint4 a[GATHER_AHEAD], b[GATHER_AHEAD];
+    bool here[GATHER_AHEAD];
+#pragma unroll
+    for (int u = 0; u < GATHER_AHEAD; ++u) {
+      const int x = x0 + u * GATHER_THREADS;
+      here[u] = false;
+      if (x < count) {
+        const int line = chunks == 1 ? x : (int)__umulhi((unsigned)x, inv_chunks), j = j0 + line, index = j / pt.page;      // (x / chunks: x is at most 1024)
+        const int64_t id = page_id(pt, r, index);
+        here[u] = id >= 0;
+        missing |= id < 0;
+        const int64_t src = ((id < 0 ? 0 : id * G + g) * pt.page + (j - index * pt.page)) * chunks + (x - line * chunks);
+        if (id >= 0) {
+          a[u] = ldg_stream(kp + src);
+          b[u] = ldg_stream(vp + src);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < GATHER_AHEAD; ++u)
+      if (here[u]) {
+        kc[dst + x0 + u * GATHER_THREADS] = a[u];
+        vc[dst + x0 + u * GATHER_THREADS] = b[u];
+      }
   }
-  const int64_t left = n - j0, count = (left < pt.page ? left : pt.page) * chunks;
-  const int64_t src = (id * G + g) * pt.page * chunks, dst = (((int64_t)i * G + g) * Tcap + j0) * chunks;
-  for (int64_t x = threadIdx.x; x < count; x += blockDim.x) {
-    kc[dst + x] = kp[src + x];
-    vc[dst + x] = vp[src + x];
-  }
+  if (missing) atomicAdd(&g_paged_fault, 1u);
 }
 
 }  // namespace b200p
@@ -269,6 +426,28 @@ extern "C" int b200p_paged_append(void* qkv, int64_t ldq, void* q_out, void* kpa
                 (long long)ldq);
   if (M == 0) return B200P_OK;
   const cudaStream_t st = (cudaStream_t)stream;
+  const size_t in = qkv_f32 || dtype == B200P_F32 ? 4 : 2;
+  if ((pairs || n_rot % 8 == 0) && aligned(qkv, 16) && ldq * in % 16 == 0 && aligned(q_out, 16) && aligned(q_norm_w, 16) && aligned(k_norm_w, 16)) {
+    int width_log2 = 0, lg = 3;
+    while ((8 << width_log2) < D) ++width_log2;
+    const int walkers = 256 >> width_log2, sms = sm_count();
+    while (lg > 0 && ((M >> lg) < 4 * sms || (1 << lg) > walkers)) --lg;
+    // two CTAs per SM at least, by sharing a token's heads
+    int64_t split = 2 * sms / M, most = (H + 2 * G + walkers - 1) / walkers;
+    if (split < 1 || lg > 0) split = 1;
+    const dim3 grid((unsigned)((M + (1 << lg) - 1) >> lg), (unsigned)(split < most ? split : most));
+    if (qkv_f32) {
+      B200P_DISPATCH_DTYPE(dtype, T, (launch_pdl(paged_append_rows_kernel<T, float>, grid, 256, 0, st, (float*)qkv, ldq, (T*)q_out, (T*)kpages, (T*)vpages,
+                                          mass, pt, t_row, t_slot, t_pos, (const T*)q_norm_w, (const T*)k_norm_w, rates, n_rot, pairs, eps, (int)M, H, G, D,
+                                          width_log2, lg)));
+    } else {
+      B200P_DISPATCH_DTYPE(dtype, T, (launch_pdl(paged_append_rows_kernel<T, T>, grid, 256, 0, st, (T*)qkv, ldq, (T*)q_out, (T*)kpages, (T*)vpages, mass,
+                                          pt, t_row, t_slot, t_pos, (const T*)q_norm_w, (const T*)k_norm_w, rates, n_rot, pairs, eps, (int)M, H, G, D,
+                                          width_log2, lg)));
+    }
+    B200P_LAUNCH_CHECK("paged_append_rows_kernel");
+    return B200P_OK;
+  }
   if (qkv_f32) {
     B200P_DISPATCH_DTYPE(dtype, T, (paged_append_kernel<T, float><<<(unsigned)M, 256, 0, st>>>((float*)qkv, ldq, (T*)q_out, (T*)kpages, (T*)vpages, mass, pt,
                                        t_row, t_slot, t_pos, (const T*)q_norm_w, (const T*)k_norm_w, rates, n_rot, pairs, eps, H, G, D)));
@@ -319,9 +498,14 @@ extern "C" int b200p_paged_gather(const void* kpages, const void* vpages, const 
   B200P_REQUIRE(aligned(kcache, 16) && aligned(vcache, 16), B200P_ERR_ALIGN, "caches must be 16-byte aligned");
   if (count == 0) return B200P_OK;
   const int chunks = D * (dtype == B200P_F32 ? 4 : 2) / 16;
-  const int64_t most = (Tcap + page - 1) / page;
-  paged_gather_kernel<<<dim3((unsigned)(most < width ? most : width), (unsigned)G, (unsigned)count), 256, 0, (cudaStream_t)stream>>>(
-      (const uint4*)kpages, (const uint4*)vpages, pt, row_of, lengths, (uint4*)kcache, (uint4*)vcache, extra, G, chunks, Tcap);
+  const int64_t longest = Tcap < (int64_t)width * page ? Tcap : (int64_t)width * page;
+  // 16 KB of keys and of values per CTA, 4 where that leaves SMs without one
+  int slots = 16384 / (16 * chunks);
+  while (slots > 64 / chunks + 1 && (longest + slots - 1) / slots * G * count < 2 * sm_count()) slots = (slots + 1) / 2;
+  const unsigned inv = (unsigned)(((1ull << 32) + chunks - 1) / chunks);
+  PdlClass pdl_cls(32);
+  launch_pdl(paged_gather_kernel, dim3((unsigned)((longest + slots - 1) / slots), (unsigned)G, (unsigned)count), GATHER_THREADS, 0, (cudaStream_t)stream,
+             (const uint4*)kpages, (const uint4*)vpages, pt, row_of, lengths, (uint4*)kcache, (uint4*)vcache, extra, G, chunks, inv, slots, Tcap);
   B200P_LAUNCH_CHECK("paged_gather_kernel");
   return B200P_OK;
 }
