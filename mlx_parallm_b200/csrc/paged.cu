@@ -1,10 +1,15 @@
 // Paged key-value cache: append (norms, rotation, write), eviction by received attention weight (selection, closing up), dense view.
+#include <cooperative_groups.h>
 #include <stdlib.h>
 
+#include <atomic>
+
+#include "mma_util.cuh"
 #include "paged.cuh"
 
 namespace b200p {
 
+namespace cg = cooperative_groups;
 int sm_count();
 
 // Calls of the append and the eviction that met an id that names no page where they needed one (b200p_paged_fault_count).
@@ -223,133 +228,283 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One CTA per row and key head: the need-th largest key of the candidates [first, n - recent) by four passes over 8 bits each, then the
-// kept slots in order (of the keys equal to it the lowest slots).
-constexpr int SEL_THREADS = 1024;
+// A cluster of CTAs per row and key head, each with a run of the row's slots whose keys it keeps in shared memory (rows too long for that: it reads the
+// weights anew in every pass).  The need-th largest key of the candidates [first, n - recent) in three passes over 11, 11 and 10 bits: every CTA counts
+// its keys' digits, then adds up all CTAs' counts of its share of the digits through distributed shared memory and hands the sums to the others' copies;
+// the digit in which the need-th lies is found from the sums.  Then each warp counts what it keeps of its slots, and with the counts before it (of the keys
+// equal to the last one the lowest slots are kept) it writes them in order.  Bound by its few barriers: the weights are 4 bytes a slot.
+// (One CTA, 8 bits at a time from global memory: 40001 slots of 8 heads took 230 us.)
+constexpr int SEL_THREADS = 1024, SEL_WARPS = 32, SEL_MAX_CLUSTER = 8, SEL_BINS = 2048;
+
+struct SelShared {
+  unsigned hist[SEL_BINS], sums[SEL_BINS];
+  unsigned warp_sum[SEL_WARPS];
+  unsigned digit, left;
+  unsigned take[SEL_WARPS], eq[SEL_WARPS];
+  unsigned all_above, all_eq;          // this CTA's, for the others
+};
+
 __global__ void __launch_bounds__(SEL_THREADS)
-paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int32_t* kept, int G, int keep, int first, int recent) {
-  __shared__ unsigned hist[256];
-  __shared__ unsigned s_prefix, s_need;
-  __shared__ unsigned w_take[32], w_eq[32];
-  const int g = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int32_t* kept, int G, int keep, int first, int recent, int room) {
+  extern __shared__ uint32_t keys[];
+  __shared__ SelShared s;
+  cg::cluster_group cluster = cg::this_cluster();
+  const unsigned S = cluster.num_blocks(), rank = cluster.block_rank();
+  const int g = blockIdx.y, r = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
   int n = lengths[r];
   n = n < 0 ? 0 : (n > table_slots(pt) ? table_slots(pt) : n);
   int32_t* out = kept + ((int64_t)r * G + g) * keep;
-  if (n <= keep) {
-    for (int i = tid; i < keep; i += SEL_THREADS) out[i] = i < n ? i : -1;
+  if (n <= keep) {                                                // the same for the whole cluster
+    for (int i = rank * SEL_THREADS + tid; i < keep; i += S * SEL_THREADS) out[i] = i < n ? i : -1;
     return;
   }
+  // this CTA's slots [j0, j1): whole tiles, and in each warp a run of 32 at a time
+  const int per = ((n + (int)S - 1) / (int)S + 31) / 32 * 32, j0 = min(n, (int)rank * per), j1 = min(n, j0 + per);
   const int lo = first, hi = n - recent;
-  auto key_at = [&](int j) -> uint32_t {
+  const bool held = per <= room;
+  auto look = [&](int j) -> uint32_t {
     const int64_t id = page_id(pt, r, j / pt.page);
     return id < 0 ? 0u : weight_key(mass[(id * G + g) * pt.page + j % pt.page]);
   };
+  for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s.hist[i] = 0;
+  __syncthreads();
   unsigned need = (unsigned)(keep - first - recent), prefix = 0, mask = 0;
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += SEL_THREADS) hist[i] = 0;
-      __syncthreads();
-      for (int j = lo + tid; j < hi; j += SEL_THREADS) {
-        const uint32_t u = key_at(j);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1u);
+  const bool picks = need > 0;
+  constexpr int BITS[3] = {11, 11, 10};
+  int shift = 32;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    if (!picks && pass > 0) break;
+    const int bits = BITS[pass], bins = 1 << bits;
+    shift -= bits;
+    for (int b = j0 + warp * 32; b < j1; b += SEL_THREADS) {
+      const int j = b + lane;
+      uint32_t u = 0;
+      if (j < j1) {
+        if (!held) {
+          u = look(j);
+        } else if (pass == 0) {
+          u = look(j);
+          keys[j - j0] = u;
+        } else {
+          u = keys[j - j0];
+        }
       }
-      __syncthreads();
-      if (tid == 0) {
-        unsigned left = need;
-        int b = 255;
-        while (b > 0 && hist[b] < left) left -= hist[b--];
-        s_prefix = prefix | ((unsigned)b << shift);
-        s_need = left;
+      // tokens that nobody looked at have equal weights: one count for a warp whose keys share a digit
+      const bool counts = picks && j < j1 && j >= lo && j < hi && (u & mask) == prefix;
+      const unsigned d = (u >> shift) & (bins - 1), who = __ballot_sync(0xffffffffu, counts);
+      if (!who) continue;
+      const int leader = __ffs(who) - 1;
+      const unsigned common = __shfl_sync(0xffffffffu, d, leader);
+      if (__all_sync(0xffffffffu, !counts || d == common)) {
+        if (lane == leader) atomicAdd(&s.hist[d], (unsigned)__popc(who));
+      } else if (counts) {
+        atomicAdd(&s.hist[d], 1u);
       }
-      __syncthreads();
-      prefix = s_prefix;
-      need = s_need;
-      mask |= 255u << shift;
-      __syncthreads();
     }
+    if (!picks) break;
+    cluster.sync();
+    // all CTAs' counts of this CTA's share of the digits, into every CTA
+    const int part = bins / (int)S;
+    for (int i = tid; i < part; i += SEL_THREADS) {
+      const int d = rank * part + i;
+      unsigned sum = 0;
+      for (unsigned c = 0; c < S; ++c) sum += cluster.map_shared_rank(s.hist, c)[d];
+      for (unsigned c = 0; c < S; ++c) cluster.map_shared_rank(s.sums, c)[d] = sum;
+    }
+    cluster.sync();
+    // the digit: the largest with at least `need` keys from it up.  Thread i holds the digits [i w, (i + 1) w) counted from the top
+    const int w = bins / SEL_THREADS;
+    unsigned mine = 0;
+    for (int k = 0; k < w; ++k) mine += s.sums[bins - 1 - (tid * w + k)];
+    unsigned before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned x = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += x;
+    }
+    if (lane == 31) s.warp_sum[warp] = before;
+    __syncthreads();
+    unsigned add = 0;
+    for (int k = 0; k < warp; ++k) add += s.warp_sum[k];
+    before += add - mine;
+    if (before < need && before + mine >= need) {
+      int k = 0;
+      while (before + s.sums[bins - 1 - (tid * w + k)] < need) before += s.sums[bins - 1 - (tid * w + k++)];
+      s.digit = bins - 1 - (tid * w + k);
+      s.left = need - before;
+    }
+    for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s.hist[i] = 0;
+    __syncthreads();
+    prefix |= s.digit << shift;
+    need = s.left;
+    mask |= (unsigned)(bins - 1) << shift;
   }
-  int base = 0;
-  unsigned eq_base = 0;
-  for (int j0 = 0; j0 < n; j0 += SEL_THREADS) {
-    const int j = j0 + tid;
-    const bool always = j < n && (j < lo || j >= hi);
-    const uint32_t u = j < n && !always ? key_at(j) : 0u;
-    const bool cand = j < n && !always && keep > first + recent;
+  __syncthreads();
+  // ---- counts of what is kept for certain and of the keys equal to the last one, by warp and by CTA ------------------------
+  const int run = (per / 32 + SEL_WARPS - 1) / SEL_WARPS * 32, w0 = min(j1, j0 + warp * run), w1 = min(j1, w0 + run);
+  auto key_at = [&](int j) -> uint32_t { return held ? keys[j - j0] : look(j); };
+  unsigned above = 0, equal = 0;
+  for (int b = w0; b < w1; b += 32) {
+    const int j = b + lane;
+    const bool always = j < w1 && (j < lo || j >= hi), cand = picks && j < w1 && !always;
+    const uint32_t u = cand ? key_at(j) : 0u;
+    above += __popc(__ballot_sync(0xffffffffu, always || (cand && u > prefix)));
+    equal += __popc(__ballot_sync(0xffffffffu, cand && u == prefix));
+  }
+  if (lane == 0) {
+    s.take[warp] = above;
+    s.eq[warp] = equal;
+  }
+  __syncthreads();
+  unsigned a = s.take[lane], e = s.eq[lane], sum_a = a, sum_e = e;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned x = __shfl_up_sync(0xffffffffu, sum_a, o), y = __shfl_up_sync(0xffffffffu, sum_e, o);
+    if (lane >= o) sum_a += x, sum_e += y;
+  }
+  if (tid == 31) {
+    s.all_above = sum_a;
+    s.all_eq = sum_e;
+  }
+  unsigned at = __shfl_sync(0xffffffffu, sum_a - a, warp), rank_e = __shfl_sync(0xffffffffu, sum_e - e, warp);      // before this warp
+  cluster.sync();
+  for (unsigned c = 0; c < rank; ++c) {
+    at += *cluster.map_shared_rank(&s.all_above, c);
+    rank_e += *cluster.map_shared_rank(&s.all_eq, c);
+  }
+  at += min(rank_e, need);
+  for (int b = w0; b < w1; b += 32) {
+    const int j = b + lane;
+    const bool always = j < w1 && (j < lo || j >= hi), cand = picks && j < w1 && !always;
+    const uint32_t u = cand ? key_at(j) : 0u;
     const bool eq = cand && u == prefix;
-    const unsigned be = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) w_eq[warp] = __popc(be);
-    __syncthreads();
-    unsigned rank = eq_base + __popc(be & ((1u << lane) - 1)), all_eq = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) rank += w_eq[w];
-      all_eq += w_eq[w];
-    }
-    const bool take = always || (cand && u > prefix) || (eq && rank < need);
+    const unsigned be = __ballot_sync(0xffffffffu, eq), below = (1u << lane) - 1;
+    const bool take = always || (cand && u > prefix) || (eq && rank_e + __popc(be & below) < need);
     const unsigned bt = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) w_take[warp] = __popc(bt);
-    __syncthreads();
-    int at = base + __popc(bt & ((1u << lane) - 1)), all = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) at += w_take[w];
-      all += w_take[w];
+    if (take) out[at + __popc(bt & below)] = j;
+    at += __popc(bt);
+    rank_e += __popc(be);
+  }
+  cluster.sync();                                                 // a CTA's shared memory lives until the others have read it
+}
+
+// A CTA or a cluster of them per row, key head and kind (keys or values; the weights go with the keys) closes the kept slots up in rounds: a round's lines
+// go to shared memory, four rounds under way at once, then (everybody has read that round) to their places.  A slot never moves up and the kept ones
+// ascend, so no later round reads a place that an earlier one wrote.  Where lines come from and go to is looked up for MOVE_LINES of them at once: a look
+// at the list, then the table, then the line, round by round, made every round wait 5 us (16 rows of 8 heads cut from 4096 to 2048 tokens: 160 us).
+// Bound by HBM where rows and heads are many.
+constexpr int MOVE_THREADS = 256, MOVE_UNITS = 4, MOVE_STAGES = 4, MOVE_LINES = 2048, MOVE_MAX_CLUSTER = 8;
+constexpr int MOVE_SMEM = MOVE_STAGES * MOVE_UNITS * MOVE_THREADS * 16 + MOVE_LINES * 16;
+
+__global__ void __launch_bounds__(MOVE_THREADS)
+paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int32_t* lengths, const int32_t* kept, int G, int chunks, unsigned inv_chunks,
+                     int keep) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint4* ring = reinterpret_cast<uint4*>(smem);
+  int64_t* from = reinterpret_cast<int64_t*>(smem + MOVE_STAGES * MOVE_UNITS * MOVE_THREADS * 16);
+  int64_t* to = from + MOVE_LINES;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x;
+  const int g = blockIdx.y >> 1, r = blockIdx.z;
+  const bool values = blockIdx.y & 1;
+  uint4* pages = values ? vp : kp;
+  pdl_wait();
+  int n = lengths[r];
+  n = n > table_slots(pt) ? table_slots(pt) : n;
+  const int32_t* list = kept + ((int64_t)r * G + g) * keep;
+  if (n <= 1) return;                                             // nothing can move: the same for the whole cluster
+  auto meet = [&]() {
+    if (S > 1) cluster.sync();
+    else __syncthreads();
+  };
+  auto place = [&](int j) -> int64_t {
+    const int index = j / pt.page;
+    const int64_t id = page_id(pt, r, index);
+    return id < 0 ? -1 : (id * G + g) * pt.page + (j - index * pt.page);
+  };
+  // in round m this CTA takes the kept slots from (m S + rank) lines on
+  const int lines = min(MOVE_THREADS * MOVE_UNITS / chunks, MOVE_LINES), rounds = (keep + S * lines - 1) / (S * lines), ahead = MOVE_LINES / lines;
+  for (int m0 = 0; m0 < rounds; m0 += ahead) {
+    const int m1 = min(rounds, m0 + ahead);
+    constexpr int EACH = MOVE_LINES / MOVE_THREADS;
+    float weight[EACH];
+    int64_t weight_to[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const int q = k * MOVE_THREADS + tid, m = m0 + q / lines, i = (m * S + rank) * lines + q % lines;
+      int64_t src = -1, dst = -1;
+      if (m < m1 && i < keep) {
+        const int j = list[i];
+        if (j > i && j < n) {
+          src = place(j), dst = place(i);
+          if ((src < 0 || dst < 0) && !values) atomicAdd(&g_paged_fault, 1u);
+        }
+      }
+      if (src < 0 || dst < 0) src = dst = -1;
+      from[q] = src;
+      to[q] = dst;
+      weight_to[k] = mass && !values ? dst : -1;
+      weight[k] = weight_to[k] >= 0 ? mass[src] : 0.f;
     }
-    if (take && at < keep) out[at] = j;
-    base += all;
-    eq_base += all_eq;
-    __syncthreads();
+    meet();                                                       // everybody has read its weights
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if (weight_to[k] >= 0) mass[weight_to[k]] = weight[k];
+    // a thread's units of a round: x = u MOVE_THREADS + tid of lines * chunks
+    auto read = [&](int m) {
+      if (m < m1) {
+        uint4* at = ring + (m % MOVE_STAGES) * MOVE_UNITS * MOVE_THREADS;
+#pragma unroll
+        for (int u = 0; u < MOVE_UNITS; ++u) {
+          const int x = u * MOVE_THREADS + tid, line = chunks == 1 ? x : (int)__umulhi((unsigned)x, inv_chunks);
+          if (line >= lines) continue;
+          const int64_t src = from[(m - m0) * lines + line];
+          if (src >= 0) cp_async16((uint32_t)__cvta_generic_to_shared(at + x), pages + src * chunks + (x - line * chunks), true);
+        }
+      }
+      cp_async_commit();
+    };
+    for (int m = m0; m < m0 + MOVE_STAGES - 1; ++m) read(m);
+    for (int m = m0; m < m1; ++m) {
+      read(m + MOVE_STAGES - 1);
+      cp_async_wait<MOVE_STAGES - 1>();
+      meet();                                                     // everybody has read round m
+      const uint4* at = ring + (m % MOVE_STAGES) * MOVE_UNITS * MOVE_THREADS;
+#pragma unroll
+      for (int u = 0; u < MOVE_UNITS; ++u) {
+        const int x = u * MOVE_THREADS + tid, line = chunks == 1 ? x : (int)__umulhi((unsigned)x, inv_chunks);
+        if (line >= lines) continue;
+        const int64_t dst = to[(m - m0) * lines + line];
+        if (dst >= 0) pages[dst * chunks + (x - line * chunks)] = at[x];
+      }
+    }
+    meet();                                                       // the lists are written anew
   }
 }
 
-// One CTA per row and key head closes the kept slots up in rounds: a round's lines go to registers, then (all of them read) to their places.
-// A slot never moves up and the kept ones ascend, so no later round reads a place that an earlier one wrote.
-constexpr int MOVE_THREADS = 512, MOVE_UNITS = 4;
-__global__ void __launch_bounds__(MOVE_THREADS)
-paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int32_t* lengths, const int32_t* kept, int G, int chunks, int keep) {
-  const int g = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
-  int n = lengths[r];
-  n = n > table_slots(pt) ? table_slots(pt) : n;
-  const int32_t* from = kept + ((int64_t)r * G + g) * keep;
-  auto place = [&](int j) -> int64_t {
-    const int64_t id = page_id(pt, r, j / pt.page);
-    return id < 0 ? -1 : (id * G + g) * pt.page + j % pt.page;
-  };
-  const int lines = min(MOVE_THREADS * MOVE_UNITS / chunks, MOVE_THREADS);     // per round; one weight per thread
-  for (int i0 = 0; i0 < keep; i0 += lines) {
-    uint4 a[MOVE_UNITS], b[MOVE_UNITS];
-    float m = 0.f;
-    int64_t to[MOVE_UNITS], to_m = -1;
-#pragma unroll
-    for (int u = 0; u < MOVE_UNITS; ++u) {
-      const int x = u * MOVE_THREADS + tid, line = x / chunks, c = x - line * chunks, i = i0 + line;
-      to[u] = -1;
-      if (line < lines && i < keep) {
-        const int j = from[i];
-        if (j > i && j < n) {
-          const int64_t src = place(j), dst = place(i);
-          if (src >= 0 && dst >= 0) {
-            a[u] = kp[src * chunks + c];
-            b[u] = vp[src * chunks + c];
-            to[u] = dst * chunks + c;
-          } else if (c == 0) {
-            atomicAdd(&g_paged_fault, 1u);
-          }
-        }
-      }
-    }
-    if (mass && tid < lines && i0 + tid < keep) {
-      const int i = i0 + tid, j = from[i];
-      if (j > i && j < n) {
-        const int64_t src = place(j), dst = place(i);
-        if (src >= 0 && dst >= 0) { m = mass[src]; to_m = dst; }
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < MOVE_UNITS; ++u)
-      if (to[u] >= 0) { kp[to[u]] = a[u]; vp[to[u]] = b[u]; }
-    if (to_m >= 0) mass[to_m] = m;
-    __syncthreads();
-  }
+// grid (cluster, y, z) of clusters along x
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_clusters(void (*kern)(KArgs...), int S, int y, int z, int threads, size_t smem, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)S, (unsigned)y, (unsigned)z);
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)S;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+// CTAs of a cluster: as many as still find an SM each, at most `most`
+static int cluster_of(int64_t clusters, int most, int per_sm) {
+  int S = 1;
+  while (S < most && clusters * S * 2 <= (int64_t)sm_count() * per_sm) S *= 2;
+  return S;
 }
 
 // ------------------------------------------------------------------------------------------------ dense view
@@ -468,7 +623,25 @@ extern "C" int b200p_paged_select(const float* mass, const int32_t* table, const
   B200P_REQUIRE(keep > 0 && first >= 0 && recent >= 0 && (int64_t)first + recent <= keep, B200P_ERR_ARG, "%d first and %d recent of %d kept tokens", first,
                 recent, keep);
   B200P_REQUIRE(rows < 65536, B200P_ERR_ARG, "too many rows");
-  paged_select_kernel<<<dim3((unsigned)G, (unsigned)rows), SEL_THREADS, 0, (cudaStream_t)stream>>>(mass, pt, lengths, kept, G, keep, first, recent);
+  B200P_REQUIRE(G < 32768, B200P_ERR_ARG, "too many key heads");
+  constexpr int SEL_ROOM = 48 * 1024;                             // keys: 192 KB
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
+    e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_ROOM * 4);
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_select_kernel)");
+  const int64_t slots = (int64_t)width * page;
+  // more CTAs for a row where SMs are free and a CTA's passes are long (4096 slots: 4 per thread)
+  int S = cluster_of((int64_t)G * rows, SEL_MAX_CLUSTER, 1);
+  while (S > 1 && slots / S < 2048) S /= 2;
+  int64_t room = ((slots + S - 1) / S + 31) / 32 * 32;
+  if (room > SEL_ROOM) room = 0;                                  // (a shorter row of such a table is read three times all the same)
+  e = launch_clusters(paged_select_kernel, S, G, rows, SEL_THREADS, (size_t)room * 4, (cudaStream_t)stream, mass, pt, lengths, kept, G, keep, first, recent,
+                      (int)room);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_select_kernel");
   B200P_LAUNCH_CHECK("paged_select_kernel");
   return B200P_OK;
 }
@@ -481,8 +654,22 @@ extern "C" int b200p_paged_compact(void* kpages, void* vpages, float* mass, cons
   B200P_REQUIRE(lengths && kept && keep > 0, B200P_ERR_ARG, "null pointer or nothing to keep");
   B200P_REQUIRE(rows < 65536, B200P_ERR_ARG, "too many rows");
   const int chunks = D * (dtype == B200P_F32 ? 4 : 2) / 16;
-  paged_compact_kernel<<<dim3((unsigned)G, (unsigned)rows), MOVE_THREADS, 0, (cudaStream_t)stream>>>((uint4*)kpages, (uint4*)vpages, mass, pt, lengths, kept,
-                                                                                                     G, chunks, keep);
+  B200P_REQUIRE(G < 32768, B200P_ERR_ARG, "too many key heads");
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
+    e = cudaFuncSetAttribute(paged_compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOVE_SMEM);
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_compact_kernel)");
+  const int lines = MOVE_THREADS * MOVE_UNITS / chunks;
+  int S = cluster_of((int64_t)2 * G * rows, MOVE_MAX_CLUSTER, 2);
+  while (S > 1 && keep <= S / 2 * lines) S /= 2;                   // (CTAs without a line)
+  const unsigned inv = (unsigned)(((1ull << 32) + chunks - 1) / chunks);
+  e = launch_clusters(paged_compact_kernel, S, 2 * G, rows, MOVE_THREADS, MOVE_SMEM, (cudaStream_t)stream, (uint4*)kpages, (uint4*)vpages, mass, pt, lengths,
+                      kept, G, chunks, inv, keep);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_compact_kernel");
   B200P_LAUNCH_CHECK("paged_compact_kernel");
   return B200P_OK;
 }
