@@ -240,6 +240,7 @@ struct SelShared {
   unsigned hist[SEL_BINS], sums[SEL_BINS];
   unsigned warp_sum[SEL_WARPS];
   unsigned digit, left;
+  bool all;
   unsigned take[SEL_WARPS], eq[SEL_WARPS];
   unsigned all_above, all_eq;          // this CTA's, for the others
 };
@@ -304,20 +305,24 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
       }
     }
     if (!picks) break;
-    cluster.sync();
-    // all CTAs' counts of this CTA's share of the digits, into every CTA
-    const int part = bins / (int)S;
-    for (int i = tid; i < part; i += SEL_THREADS) {
-      const int d = rank * part + i;
-      unsigned sum = 0;
-      for (unsigned c = 0; c < S; ++c) sum += cluster.map_shared_rank(s.hist, c)[d];
-      for (unsigned c = 0; c < S; ++c) cluster.map_shared_rank(s.sums, c)[d] = sum;
+    const unsigned* sums = s.hist;
+    if (S == 1) {
+      __syncthreads();
+    } else {                                                      // all CTAs' counts of this CTA's share of the digits, into every CTA
+      sums = s.sums;
+      cluster.sync();
+      const int part = bins / (int)S;
+      for (int i = tid; i < part; i += SEL_THREADS) {
+        const int d = rank * part + i;
+        unsigned sum = 0;
+        for (unsigned c = 0; c < S; ++c) sum += cluster.map_shared_rank(s.hist, c)[d];
+        for (unsigned c = 0; c < S; ++c) cluster.map_shared_rank(s.sums, c)[d] = sum;
+      }
+      cluster.sync();
     }
-    cluster.sync();
     // the digit: the largest with at least `need` keys from it up.  Thread i holds the digits [i w, (i + 1) w) counted from the top
-    const int w = bins / SEL_THREADS;
-    unsigned mine = 0;
-    for (int k = 0; k < w; ++k) mine += s.sums[bins - 1 - (tid * w + k)];
+    const int w = bins / SEL_THREADS, top = bins - 1 - tid * w;
+    const unsigned c0 = sums[top], c1 = w > 1 ? sums[top - 1] : 0, mine = c0 + c1;
     unsigned before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -326,20 +331,25 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
     }
     if (lane == 31) s.warp_sum[warp] = before;
     __syncthreads();
-    unsigned add = 0;
-    for (int k = 0; k < warp; ++k) add += s.warp_sum[k];
-    before += add - mine;
-    if (before < need && before + mine >= need) {
-      int k = 0;
-      while (before + s.sums[bins - 1 - (tid * w + k)] < need) before += s.sums[bins - 1 - (tid * w + k++)];
-      s.digit = bins - 1 - (tid * w + k);
-      s.left = need - before;
-    }
     for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s.hist[i] = 0;
+    unsigned others = lane < warp ? s.warp_sum[lane] : 0;
+    others = __reduce_add_sync(0xffffffffu, others);
+    before += others - mine;
+    if (before < need && before + mine >= need) {
+      const bool second = before + c0 < need;
+      s.digit = top - second;
+      s.left = need - before - (second ? c0 : 0);
+      s.all = (second ? c1 : c0) == s.left;
+    }
     __syncthreads();
     prefix |= s.digit << shift;
     need = s.left;
     mask |= (unsigned)(bins - 1) << shift;
+    if (s.all && prefix) {                                        // every key of this digit is kept: no need to look at the others' bits
+      --prefix;
+      need = 0;
+      break;
+    }
   }
   __syncthreads();
   // ---- counts of what is kept for certain and of the keys equal to the last one, by warp and by CTA ------------------------

@@ -377,6 +377,29 @@ def test_evict_long_rows(ops):
             assert torch.equal(kept[r, g].cpu().long(), exp)
 
 
+def test_evict_rows_longer_than_shared_memory(ops):
+    """So many rows that each has one CTA, one of them with more weights than it holds: they are read anew in every pass."""
+    G, keep, first, recent, rows, width = 2, 5000, 3, 500, 80, 15
+    P = 3 * width
+    g = torch.Generator().manual_seed(25)
+    table = torch.full((rows, width), -1, dtype=torch.int32)
+    for r, at in ((0, 0), (41, width), (79, 2 * width)):
+        table[r] = torch.randperm(width, generator=g).to(torch.int32) + at
+    lengths = torch.zeros(rows, dtype=torch.int32)
+    lengths[0], lengths[41], lengths[79] = 61000, 5000, 50001
+    mass = torch.rand((P, G, 4096), generator=g)
+    mass[2 * width:] = (mass[2 * width:] * 7).floor()
+    kept = torch.empty((rows, G, keep), dtype=torch.int32, device="cuda")
+    ops.paged_select(mass.cuda(), table.cuda(), lengths.cuda(), kept, first, recent)
+    for r in (0, 79):
+        n = int(lengths[r])
+        line = mass[table[r].long()].transpose(0, 1).reshape(G, -1)[:, :n]
+        for h in range(G):
+            order = torch.sort(line[h, first:n - recent], descending=True, stable=True).indices[:keep - first - recent] + first
+            assert torch.equal(kept[r, h].cpu().long(), torch.cat([torch.arange(first), order.sort().values, torch.arange(n - recent, n)]))
+    assert torch.equal(kept[41].cpu(), torch.arange(5000, dtype=torch.int32).expand(2, -1)) and bool((kept[1] == -1).all())
+
+
 def test_evict_pages_that_do_not_exist(ops):
     c = Cache([200, 100], 16, 2, 64, torch.bfloat16, 23)
     c.table[0, 3], c.table[1, 0] = -1, c.P
