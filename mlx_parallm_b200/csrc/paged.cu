@@ -401,19 +401,23 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
 }
 
 // A CTA or a cluster of them per row, key head and kind (keys or values; the weights go with the keys) closes the kept slots up in rounds: a round's lines
-// go to shared memory, four rounds under way at once, then (everybody has read that round) to their places.  A slot never moves up and the kept ones
+// go to shared memory, then (everybody has read that round) to their places.  One CTA keeps four rounds of 16 KB under way; a cluster, whose barriers cost 2
+// us, takes rounds of 80 KB (one row of 8 heads cut from 40001 to 5000 tokens, selection and all, in rounds of 16 KB 43 us, 80 KB 38, 160 KB and half the
+// CTAs per SM 46).  A slot never moves up and the kept ones
 // ascend, so no later round reads a place that an earlier one wrote.  Where lines come from and go to is looked up for MOVE_LINES of them at once: a look
 // at the list, then the table, then the line, round by round, made every round wait 5 us (16 rows of 8 heads cut from 4096 to 2048 tokens: 160 us).
 // Bound by HBM where rows and heads are many.
-constexpr int MOVE_THREADS = 256, MOVE_UNITS = 4, MOVE_STAGES = 4, MOVE_LINES = 2048, MOVE_MAX_CLUSTER = 8;
-constexpr int MOVE_SMEM = MOVE_STAGES * MOVE_UNITS * MOVE_THREADS * 16 + MOVE_LINES * 16;
+constexpr int MOVE_THREADS = 256, MOVE_STAGES = 4, MOVE_LINES = 2048, MOVE_MAX_CLUSTER = 8;
+constexpr int MOVE_UNITS_ONE = 4, MOVE_UNITS_CLUSTER = 20;        // 16-byte pieces of a thread in a round
+static constexpr int move_smem(int stages, int units) { return stages * units * MOVE_THREADS * 16 + MOVE_LINES * 16; }
 
+template <int STAGES, int UNITS>
 __global__ void __launch_bounds__(MOVE_THREADS)
 paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int32_t* lengths, const int32_t* kept, int G, int chunks, unsigned inv_chunks,
                      int keep) {
   extern __shared__ __align__(16) uint8_t smem[];
   uint4* ring = reinterpret_cast<uint4*>(smem);
-  int64_t* from = reinterpret_cast<int64_t*>(smem + MOVE_STAGES * MOVE_UNITS * MOVE_THREADS * 16);
+  int64_t* from = reinterpret_cast<int64_t*>(smem + STAGES * UNITS * MOVE_THREADS * 16);
   int64_t* to = from + MOVE_LINES;
   cg::cluster_group cluster = cg::this_cluster();
   const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x;
@@ -435,7 +439,7 @@ paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int3
     return id < 0 ? -1 : (id * G + g) * pt.page + (j - index * pt.page);
   };
   // in round m this CTA takes the kept slots from (m S + rank) lines on
-  const int lines = min(MOVE_THREADS * MOVE_UNITS / chunks, MOVE_LINES), rounds = (keep + S * lines - 1) / (S * lines), ahead = MOVE_LINES / lines;
+  const int lines = min(MOVE_THREADS * UNITS / chunks, MOVE_LINES), rounds = (keep + S * lines - 1) / (S * lines), ahead = MOVE_LINES / lines;
   for (int m0 = 0; m0 < rounds; m0 += ahead) {
     const int m1 = min(rounds, m0 + ahead);
     constexpr int EACH = MOVE_LINES / MOVE_THREADS;
@@ -465,27 +469,27 @@ paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int3
     // a thread's units of a round: x = u MOVE_THREADS + tid of lines * chunks
     auto read = [&](int m) {
       if (m < m1) {
-        uint4* at = ring + (m % MOVE_STAGES) * MOVE_UNITS * MOVE_THREADS;
-#pragma unroll
-        for (int u = 0; u < MOVE_UNITS; ++u) {
+        uint4* at = ring + (m % STAGES) * UNITS * MOVE_THREADS;
+#pragma unroll 4
+        for (int u = 0; u < UNITS; ++u) {
           const int x = u * MOVE_THREADS + tid, line = chunks == 1 ? x : (int)__umulhi((unsigned)x, inv_chunks);
-          if (line >= lines) continue;
+          if (line >= lines) break;
           const int64_t src = from[(m - m0) * lines + line];
           if (src >= 0) cp_async16((uint32_t)__cvta_generic_to_shared(at + x), pages + src * chunks + (x - line * chunks), true);
         }
       }
       cp_async_commit();
     };
-    for (int m = m0; m < m0 + MOVE_STAGES - 1; ++m) read(m);
+    for (int m = m0; m < m0 + STAGES - 1; ++m) read(m);
     for (int m = m0; m < m1; ++m) {
-      read(m + MOVE_STAGES - 1);
-      cp_async_wait<MOVE_STAGES - 1>();
+      read(m + STAGES - 1);
+      cp_async_wait<STAGES - 1>();
       meet();                                                     // everybody has read round m
-      const uint4* at = ring + (m % MOVE_STAGES) * MOVE_UNITS * MOVE_THREADS;
-#pragma unroll
-      for (int u = 0; u < MOVE_UNITS; ++u) {
+      const uint4* at = ring + (m % STAGES) * UNITS * MOVE_THREADS;
+#pragma unroll 4
+      for (int u = 0; u < UNITS; ++u) {
         const int x = u * MOVE_THREADS + tid, line = chunks == 1 ? x : (int)__umulhi((unsigned)x, inv_chunks);
-        if (line >= lines) continue;
+        if (line >= lines) break;
         const int64_t dst = to[(m - m0) * lines + line];
         if (dst >= 0) pages[dst * chunks + (x - line * chunks)] = at[x];
       }
@@ -665,20 +669,23 @@ extern "C" int b200p_paged_compact(void* kpages, void* vpages, float* mass, cons
   B200P_REQUIRE(rows < 65536, B200P_ERR_ARG, "too many rows");
   const int chunks = D * (dtype == B200P_F32 ? 4 : 2) / 16;
   B200P_REQUIRE(G < 32768, B200P_ERR_ARG, "too many key heads");
+  constexpr int ONE = move_smem(MOVE_STAGES, MOVE_UNITS_ONE), CLUSTER = move_smem(1, MOVE_UNITS_CLUSTER);
+  auto one = paged_compact_kernel<MOVE_STAGES, MOVE_UNITS_ONE>;
+  auto many = paged_compact_kernel<1, MOVE_UNITS_CLUSTER>;
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
-    e = cudaFuncSetAttribute(paged_compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOVE_SMEM);
+    e = cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize, ONE);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize, CLUSTER);
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_compact_kernel)");
-  const int lines = MOVE_THREADS * MOVE_UNITS / chunks;
   int S = cluster_of((int64_t)2 * G * rows, MOVE_MAX_CLUSTER, 2);
-  while (S > 1 && keep <= S / 2 * lines) S /= 2;                   // (CTAs without a line)
+  while (S > 1 && keep * chunks <= S * 1024) S /= 2;               // (at least 16 KB of lines each)
   const unsigned inv = (unsigned)(((1ull << 32) + chunks - 1) / chunks);
-  e = launch_clusters(paged_compact_kernel, S, 2 * G, rows, MOVE_THREADS, MOVE_SMEM, (cudaStream_t)stream, (uint4*)kpages, (uint4*)vpages, mass, pt, lengths,
-                      kept, G, chunks, inv, keep);
+  e = launch_clusters(S > 1 ? many : one, S, 2 * G, rows, MOVE_THREADS, S > 1 ? CLUSTER : ONE, (cudaStream_t)stream, (uint4*)kpages, (uint4*)vpages, mass, pt,
+                      lengths, kept, G, chunks, inv, keep);
   if (e != cudaSuccess) return cuda_fail(e, "paged_compact_kernel");
   B200P_LAUNCH_CHECK("paged_compact_kernel");
   return B200P_OK;
