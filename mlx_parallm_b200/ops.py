@@ -771,14 +771,22 @@ def mix_attn(q, kcache, vcache, t_row, t_pos, talk, sink, out, H, G, dk, dv, win
 
 # ---- paged key-value cache ---------------------------------------------------------------------------------------------
 # Tensors of every call: kpages / vpages [P, G, page, D] in the model's storage type, table int32 [rows, width] of page ids, mass fp32
-# [P, G, page] or None, and per token int32 t_row (negative: idle), t_slot, t_pos (include/b200p.h).
+# [P, G, page] or None, and per token int32 t_row (negative: idle), t_slot, t_pos (include/b200p.h).  Each call is checked in a few microseconds and
+# refused with ValueError (or the library's B200PError).
+_I32 = torch.int32
+
+
 def _refuse(what: str):
     raise ValueError(what)
 
 
 def _here(*ts):
+    """Contiguous, on the current device."""
+    if not ts[0].is_cuda:
+        _dev(*ts)
+    dev = ts[0].get_device() if _device_index is None else _device_index()
     for t in ts:
-        if t is not None and not (t.is_cuda and t.is_contiguous() and (_device_index is None or t.get_device() == _device_index())):
+        if t is not None and (t.get_device() != dev or not t.is_contiguous()):
             _dev(t)
             _refuse("tensors of a paged cache are contiguous and lie on the current device")
 
@@ -786,24 +794,25 @@ def _here(*ts):
 def _paged(kpages, vpages, table, mass, *others):
     """Checks of the tensors every call shares -> (P, G, page, D, rows, width)."""
     _here(kpages, vpages, table, mass, *others)
-    if kpages.dim() != 4 or vpages.shape != kpages.shape or vpages.dtype != kpages.dtype:
-        _refuse(f"pages are [P, key heads, page, D] and alike for keys and values: got {tuple(kpages.shape)} and {tuple(vpages.shape)}")
-    if table.dtype != torch.int32 or table.dim() != 2:
+    shape, tshape = kpages.shape, table.shape
+    if len(shape) != 4 or vpages.shape != shape or vpages.dtype is not kpages.dtype:
+        _refuse(f"pages are [P, key heads, page, D] and alike for keys and values: got {tuple(shape)} and {tuple(vpages.shape)}")
+    if table.dtype is not _I32 or len(tshape) != 2:
         _refuse("the page table is int32 [rows, width]")
-    if mass is not None and (mass.dtype != torch.float32 or mass.shape != kpages.shape[:3]):
+    if mass is not None and (mass.dtype is not torch.float32 or mass.shape != shape[:3]):
         _refuse(f"mass is float32 [P, key heads, page]: got {mass.dtype} {tuple(mass.shape)}")
-    return (*kpages.shape, *table.shape)
-
-
-def _kept(kept, lengths, rows: int, G: int):
-    if lengths.dtype != torch.int32 or lengths.numel() != rows or kept.dtype != torch.int32 or kept.dim() != 3 or kept.shape[:2] != (rows, G):
-        _refuse(f"lengths int32 [{rows}], kept int32 [{rows}, {G}, keep]: got {tuple(lengths.shape)} and {tuple(kept.shape)}")
+    return (*shape, *tshape)
 
 
 def _tokens(M: int, *ts):
     for t in ts:
-        if t.dtype != torch.int32 or t.numel() != M:
+        if t.dtype is not _I32 or t.numel() != M:
             _refuse(f"rows, slots and positions are int32, one for each of the {M} tokens")
+
+
+def _kept(kept, lengths, rows: int, G: int):
+    if lengths.dtype is not _I32 or lengths.numel() != rows or kept.dtype is not _I32 or kept.dim() != 3 or kept.shape[:2] != (rows, G):
+        _refuse(f"lengths int32 [{rows}], kept int32 [{rows}, {G}, keep]: got {tuple(lengths.shape)} and {tuple(kept.shape)}")
 
 
 def paged_append(qkv, q_out, kpages, vpages, table, t_row, t_slot, t_pos, H: int, rates=None, pairs: int = 0, q_norm_w=None, k_norm_w=None,
@@ -812,24 +821,29 @@ def paged_append(qkv, q_out, kpages, vpages, table, t_row, t_slot, t_pos, H: int
     queries to ``q_out`` [M, H D], keys and values to the slots ``t_slot`` of rows ``t_row``, whose mass becomes 0 (b200p_paged_append).
     ``qkv`` [M, >= (H + 2 G) D] (a column slice is fine) in the pages' dtype, or float32 for 16-bit pages: an accumulation buffer, re-zeroed."""
     P, G, page, D, rows, width = _paged(kpages, vpages, table, mass, q_out, t_row, t_slot, t_pos, rates, q_norm_w, k_norm_w)
-    M = qkv.shape[0]
-    dt = kpages.dtype
-    if not qkv.is_cuda or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < (H + 2 * G) * D or (qkv.dtype != dt and qkv.dtype != torch.float32) \
-            or (M > 1 and qkv.stride(0) < qkv.shape[1]) or (_device_index is not None and qkv.get_device() != _device_index()):
+    M, columns = qkv.shape
+    ld, inner = qkv.stride()
+    dt, qdt = kpages.dtype, qkv.dtype
+    if qkv.get_device() != kpages.get_device():
         _dev(qkv)
-        _refuse(f"qkv is [M, >= {(H + 2 * G) * D}] in the pages' dtype or float32: got {tuple(qkv.shape)} {qkv.dtype}")
-    if q_out.dtype != dt or q_out.numel() != M * H * D:
+        _refuse("qkv lies on the pages' device")
+    if inner != 1 or columns < (H + 2 * G) * D or (qdt is not dt and qdt is not torch.float32) or (M > 1 and ld < columns):
+        _refuse(f"qkv is [M, >= {(H + 2 * G) * D}] in the pages' dtype or float32: got {tuple(qkv.shape)} {qdt}")
+    if q_out.dtype is not dt or q_out.numel() != M * H * D:
         _refuse(f"q_out is [M, {H * D}] in the pages' dtype")
     _tokens(M, t_row, t_slot, t_pos)
-    if rates is not None and (rates.dtype != torch.float32 or 2 * rates.numel() > D):
-        _refuse("rates are float32, one per rotated pair")
+    n_rot = 0
+    if rates is not None:
+        n_rot = rates.numel()
+        if rates.dtype is not torch.float32 or 2 * n_rot > D:
+            _refuse("rates are float32, one per rotated pair")
     for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.dtype != dt or w.numel() != D):
+        if w is not None and (w.dtype is not dt or w.numel() != D):
             _refuse(f"norm weights are [{D}] in the pages' dtype")
     _call("b200p_paged_append", lambda: lib().b200p_paged_append(
-        qkv.data_ptr(), qkv.stride(0) if M > 1 else qkv.shape[1], q_out.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _p(mass), table.data_ptr(),
-        t_row.data_ptr(), t_slot.data_ptr(), t_pos.data_ptr(), _p(q_norm_w), _p(k_norm_w), _p(rates), 0 if rates is None else rates.numel(), int(pairs),
-        float(eps), M, int(H), G, D, P, page, rows, width, dtype_code(dt), 1 if qkv.dtype != dt else 0, _stream()))
+        qkv.data_ptr(), ld if M > 1 else columns, q_out.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _p(mass), table.data_ptr(), t_row.data_ptr(),
+        t_slot.data_ptr(), t_pos.data_ptr(), _p(q_norm_w), _p(k_norm_w), _p(rates), n_rot, int(pairs), float(eps), M, int(H), G, D, P, page, rows, width,
+        dtype_code(dt), 0 if qdt is dt else 1, _stream()))
     return q_out
 
 
@@ -843,22 +857,22 @@ def paged_attn(q, kpages, vpages, table, t_row, t_slot, out, scale: float, first
     """Attention of single tokens, each over the slots up to its own of its row; with ``window`` only the last ``window`` of them and the ``first``
     first; ``mass`` grows by the weights every slot receives (b200p_paged_attn).  ``q``, ``out`` [M, H D] in the pages' dtype."""
     P, G, page, D, rows, width = _paged(kpages, vpages, table, mass, q, out, t_row, t_slot, workspace)
-    M = t_row.numel()
-    H = q.numel() // (M * D) if M else G
-    if q.dtype != kpages.dtype or out.dtype != kpages.dtype or q.numel() != M * H * D or out.numel() != M * H * D:
+    M, n, dt = t_row.numel(), q.numel(), kpages.dtype
+    H = n // (M * D) if M else G
+    if q.dtype is not dt or out.dtype is not dt or n != M * H * D or out.numel() != n:
         _refuse(f"q and out are [{M}, heads * {D}] in the pages' dtype: got {tuple(q.shape)} and {tuple(out.shape)}")
     _tokens(M, t_row, t_slot)
-    ws_ptr, ws_bytes = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
     _call("b200p_paged_attn", lambda: lib().b200p_paged_attn(
         q.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _p(mass), table.data_ptr(), t_row.data_ptr(), t_slot.data_ptr(), out.data_ptr(), M, H, G, D, P,
-        page, rows, width, float(scale), int(first), int(window), dtype_code(q.dtype), _lib.OUT_PERM8 if out_perm else 0, ws_ptr, ws_bytes, _stream()))
+        page, rows, width, float(scale), int(first), int(window), dtype_code(dt), _lib.OUT_PERM8 if out_perm else 0, _p(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream()))
     return out
 
 
 def paged_select(mass, table, lengths, kept, first: int = 0, recent: int = 0):
     """``kept`` int32 [rows, G, keep]: which slots every row's key heads keep when the row is cut to ``keep`` tokens (b200p_paged_select)."""
     _here(mass, table, lengths, kept)
-    if mass.dim() != 3 or mass.dtype != torch.float32 or table.dtype != torch.int32 or table.dim() != 2:
+    if mass.dim() != 3 or mass.dtype is not torch.float32 or table.dtype is not _I32 or table.dim() != 2:
         _refuse("mass is float32 [P, key heads, page], the page table int32 [rows, width]")
     (P, G, page), (rows, width) = mass.shape, table.shape
     _kept(kept, lengths, rows, G)
@@ -879,6 +893,7 @@ def paged_compact(kpages, vpages, table, lengths, kept, mass=None):
 def paged_evict(kpages, vpages, mass, table, lengths, kept, first: int = 0, recent: int = 0):
     """Cut every row that holds more than ``keep = kept.shape[2]`` tokens to its ``first`` first, its ``recent`` last and the most attended ones
     between, closed up in place; afterwards a row holds min(lengths, keep) tokens (``lengths`` is the caller's to change)."""
+    _paged(kpages, vpages, table, mass, lengths, kept)              # both calls' tensors before the first writes anything
     paged_select(mass, table, lengths, kept, first, recent)
     paged_compact(kpages, vpages, table, lengths, kept, mass)
     return kept
@@ -887,15 +902,14 @@ def paged_evict(kpages, vpages, mass, table, lengths, kept, first: int = 0, rece
 def paged_gather(kpages, vpages, table, rows, lengths, kcache, vcache, extra: int = 0):
     """Dense caches [n, G, Tcap, D] of the rows ``rows`` (int32 [n]): slots below lengths + ``extra``, what lies behind untouched."""
     P, G, page, D, R, width = _paged(kpages, vpages, table, None, rows, lengths, kcache, vcache)
-    n = rows.numel()
-    if rows.dtype != torch.int32 or lengths.dtype != torch.int32 or lengths.numel() != R:
+    n, shape, dt = rows.numel(), kcache.shape, kpages.dtype
+    if rows.dtype is not _I32 or lengths.dtype is not _I32 or lengths.numel() != R:
         _refuse(f"rows int32 [n], lengths int32 [{R}]")
-    if kcache.dim() != 4 or kcache.shape[0] != n or kcache.shape[1] != G or kcache.shape[3] != D or vcache.shape != kcache.shape \
-            or kcache.dtype != kpages.dtype or vcache.dtype != kpages.dtype:
-        _refuse(f"dense caches are [{n}, {G}, Tcap, {D}] in the pages' dtype: got {tuple(kcache.shape)} and {tuple(vcache.shape)}")
+    if len(shape) != 4 or shape[0] != n or shape[1] != G or shape[3] != D or vcache.shape != shape or kcache.dtype is not dt or vcache.dtype is not dt:
+        _refuse(f"dense caches are [{n}, {G}, Tcap, {D}] in the pages' dtype: got {tuple(shape)} and {tuple(vcache.shape)}")
     _call("b200p_paged_gather", lambda: lib().b200p_paged_gather(
         kpages.data_ptr(), vpages.data_ptr(), table.data_ptr(), rows.data_ptr(), lengths.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), int(extra), n, G, D,
-        P, page, R, width, kcache.shape[2], dtype_code(kpages.dtype), _stream()))
+        P, page, R, width, shape[2], dtype_code(dt), _stream()))
 
 
 def paged_fault_count(reset: bool = False) -> int:
