@@ -30,6 +30,7 @@ import torch
 from .. import ops
 from .._lib import EPI_ADD_RESIDUAL, EPI_SILU_MUL, EPI_STORE, EPI_STORE_F32
 from .base import BatchedKVCache, PagedKVCache
+from .paged import PageBook, PagedLayer
 
 MAX_TOKENS_PER_FORWARD = 8192     # chunk size (B*L) of one prefill pass through the layers
 # Up to this many rows the fused q|k|v projection accumulates in an fp32 buffer through the stream-K kernel (csrc/qmm_sk.cu:
@@ -174,6 +175,7 @@ class DecoderModel:
             self.lm_head = QuantizedLinear(args.hidden_size, args.vocab_size, args._group_size, args._bits)
         self.dtype: Optional[torch.dtype] = None
         self.device: Optional[torch.device] = None
+        self._rope_rates: Optional[torch.Tensor] = None
         self._arenas: Dict[int, dict] = {}
         # One forward at a time per model instance: the scratch arenas, the self-cleaning qmm
         # workspace and the fp32 accumulators are shared by every caller of this model, and the reference server runs
@@ -245,6 +247,7 @@ class DecoderModel:
             raise TypeError(f"scales must share one dtype, got {dts}")
         self.dtype = dts.pop()
         self.device = device
+        self._rope_rates = None
         a0 = self.args
         self._fast16 = self.dtype in (torch.float16, torch.bfloat16)
         # PERM8 needs every GEMM input row to be made of aligned groups of 8 (hidden, heads*head_dim, intermediate)
@@ -350,11 +353,7 @@ class DecoderModel:
 
     def _advance_device(self, cache, a: dict, B: int, ids_i32=None):
         """End of a decode step on the device: every row took one token."""
-        seen = set()
-        for c in cache:
-            if c._lengths.data_ptr() not in seen:
-                seen.add(c._lengths.data_ptr())
-                ops.advance_lengths(c._lengths, 1)
+        advance_counters(cache, 1)
 
     # -- caches ----------------------------------------------------------------------------------
     def make_cache(self, batch_size: int, step: Optional[int] = None, paged: bool = True) -> List[BatchedKVCache]:
@@ -362,6 +361,25 @@ class DecoderModel:
         caches = [klass(self.head_dim, l.self_attn.n_kv_heads, batch_size) for l in self.model.layers]
         bind_cache_group(caches, self.device, step)
         return caches
+
+    def make_paged_cache(self, batch_size: int, max_tokens: int, page: int = 64, pages: Optional[int] = None, window: int = 0, first: int = 0,
+                         keep: int = 0, recent: Optional[int] = None, observe: int = 32) -> List[PagedLayer]:
+        """A cache in pages (models/paged.py) for ``batch_size`` rows of up to ``max_tokens`` tokens, drawn from ``pages`` pages of ``page`` tokens
+        (None: as many as all rows need).  ``window`` > 0: a token sees the last ``window`` tokens and the ``first`` first ones.  ``keep`` > 0: a row
+        that is full is cut to ``keep`` tokens, the ``first`` first, the ``recent`` newest (None: half of the others) and the most attended
+        ones; the weights of decode steps and of a prompt's last ``observe`` tokens count."""
+        if self.device is None:
+            raise RuntimeError("load the model's weights first")
+        book = PageBook(batch_size, max_tokens, self.device, page, pages, window, first, keep, recent, observe)
+        self.rope_rates()                                               # (not inside a capture)
+        return [PagedLayer(book, l.self_attn.n_heads, l.self_attn.n_kv_heads, self.head_dim) for l in self.model.layers]
+
+    def rope_rates(self) -> torch.Tensor:
+        """fp32 [head_dim / 2]: the angle of pair i at position p is p * rates[i]."""
+        if self._rope_rates is None:
+            i = torch.arange(self.head_dim // 2, dtype=torch.float64)
+            self._rope_rates = (self.rope_scale * float(self.args.rope_theta) ** (-2.0 * i / self.head_dim)).float().to(self.device)
+        return self._rope_rates
 
     # -- scratch ---------------------------------------------------------------------------------
     def _arena(self, M: int, B: int) -> dict:
@@ -421,6 +439,7 @@ class DecoderModel:
         M = a["h"].shape[0]
         rows_mode = fx is not None and fx.mode == "rows"
         a["x_final"] = False
+        paged = cache[0].book.tokens(B, L) if isinstance(cache[0], PagedLayer) else None
         for li, (layer, c) in enumerate(zip(layers, cache)):
             at, mlp = layer.self_attn, layer.mlp
             lengths = c.lengths(self.device)
@@ -433,12 +452,17 @@ class DecoderModel:
                 for name, (At, Bt, scale) in at.lora.items():
                     col0 = 0 if name == "q_proj" else (at.n_heads + at.n_kv_heads) * at.head_dim
                     ops.lora_add(a["x"], At, Bt, qkv_buf, col0, scale)
-            ops.rope_kv_append(qkv_buf, a["q"], c.keys, c.values, lengths, B, L, at.n_heads,
-                               at.n_kv_heads, at.head_dim, args.rope_theta, self.rope_scale,
-                               at.q_norm.weight if at.q_norm else None, at.k_norm.weight if at.k_norm else None,
-                               args.rms_norm_eps)
-            ops.attn(a["q"], c.keys, c.values, lengths, a["att"], B, L, at.n_heads, at.n_kv_heads, at.head_dim,
-                     at.scale, workspace=a["ws_attn"], out_perm=pm)
+            if paged is not None:
+                c.append_and_attend(qkv_buf, a["q"], a["att"], paged, B, L, at.n_heads, self.rope_rates(), at.scale,
+                                    at.q_norm.weight if at.q_norm else None, at.k_norm.weight if at.k_norm else None,
+                                    args.rms_norm_eps, a["ws_attn"], pm)
+            else:
+                ops.rope_kv_append(qkv_buf, a["q"], c.keys, c.values, lengths, B, L, at.n_heads,
+                                   at.n_kv_heads, at.head_dim, args.rope_theta, self.rope_scale,
+                                   at.q_norm.weight if at.q_norm else None, at.k_norm.weight if at.k_norm else None,
+                                   args.rms_norm_eps)
+                ops.attn(a["q"], c.keys, c.values, lengths, a["att"], B, L, at.n_heads, at.n_kv_heads, at.head_dim,
+                         at.scale, workspace=a["ws_attn"], out_perm=pm)
             if fx is not None:
                 # row-parallel partial sums accumulate into the peer-mapped buffer; ONE kernel then does the
                 # all-reduce over NVLink + residual add + post-attention RMSNorm (and re-zeroes the other buffer)
@@ -579,12 +603,18 @@ def release_rows(caches, rows: List[int]):
             c._sync_lengths()
 
 
-def advance_cache(caches: List[BatchedKVCache], L: int):
-    """lengths += L once per distinct device tensor; host mirrors on every layer."""
+def advance_counters(caches, L: int):
+    """Every distinct device counter of the caches (lengths; a paged cache's positions too) += L."""
     seen = set()
     for c in caches:
-        t = c._lengths
-        if t.data_ptr() not in seen:
-            seen.add(t.data_ptr())
-            ops.advance_lengths(t, L)
+        for t in c.counters():
+            if t.data_ptr() not in seen:
+                seen.add(t.data_ptr())
+                ops.advance_lengths(t, L)
+
+
+def advance_cache(caches: List[BatchedKVCache], L: int):
+    """lengths += L once per distinct device tensor; host mirrors on every layer."""
+    advance_counters(caches, L)
+    for c in caches:
         c.advance_host(L)

@@ -88,6 +88,10 @@ class RowState:
         self._lengths = t
         self._lengths_shared = True
 
+    def counters(self) -> tuple:
+        """Device counters a step adds its tokens to."""
+        return (self._lengths,)
+
     def _sync_lengths(self):
         if self._lengths is not None:
             self._lengths.copy_(torch.tensor(self._offsets, dtype=torch.int32), non_blocking=False)

@@ -34,6 +34,7 @@ import torch
 from . import ops, sample_utils
 from .models._transformer import DecoderModel, advance_cache, advance_rows, bind_cache_group, prepare_cache, prepare_rows
 from .models.base import BatchedKVCache, PagedKVCache
+from .models.paged import PagedLayer
 from .sample_utils import top_p_sampling
 from .tokenizer_utils import TokenizerWrapper, load_tokenizer
 
@@ -381,6 +382,8 @@ def generate_step(
         if dropped:
             raise RuntimeError(f"KV cache overflow: {dropped} (token, head) appends were dropped by b200p_rope_kv_append; "
                                "results of this generation are invalid")
+        if isinstance(cache[0], PagedLayer) and ops.paged_fault_count(reset=True):
+            raise RuntimeError("a paged cache's table named pages that do not exist; results of this generation are invalid")
 
     # prefill (eager, chunked) + first sample
     if prompt_lengths is not None:

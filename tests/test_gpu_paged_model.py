@@ -1,0 +1,124 @@
+"""Models over a cache in pages (DecoderModel.make_paged_cache) against the oracle and against the same model over dense caches."""
+import numpy as np
+import pytest
+import torch
+
+from helpers import greedy_report, make_pair, prompts_for, rel_err
+from oracle.model import generate_step as oracle_generate_step
+
+pytestmark = pytest.mark.gpu
+
+LOGIT_TOL = 1e-2          # per-step logits within 1e-2 relative, as for dense caches
+MODELS = [("tiny-llama", "float16"), ("tiny-llama", "float32"), ("tiny-qwen3", "bfloat16"), ("small-llama", "float16"), ("small-phi3", "bfloat16")]
+
+
+def tokens_of(gm, prompts, steps, cache):
+    from mlx_parallm_b200.utils import generate_step
+    return np.stack([y[:, 0].cpu().numpy() for _, (y, _) in zip(range(steps), generate_step(torch.from_numpy(prompts), gm, cache=cache))], 1)
+
+
+@pytest.mark.parametrize("keep", [0, 30], ids=["plain", "weighed"])
+@pytest.mark.parametrize("name,dtype", MODELS)
+def test_logits_of_prompt_and_steps(name, dtype, keep):
+    """A prompt, a portion behind it and single tokens: every position's logits against the oracle's whole forward."""
+    cfg, om, gm = make_pair(name, dtype=dtype)
+    ids = prompts_for(cfg, 3, 29)
+    exp = om.forward(ids, om.make_cache(3))
+    cache = gm.make_paged_cache(3, 40, page=16, keep=keep)
+    t = torch.from_numpy(ids)
+    got = [gm(t[:, :13], cache=cache), gm(t[:, 13:25], cache=cache)] + [gm(t[:, i:i + 1], cache=cache) for i in range(25, 29)]
+    err = rel_err(torch.cat(got, 1).cpu().numpy(), exp)
+    print(f"{name} {dtype}: logits rel err {err:.2e}")
+    assert err < LOGIT_TOL
+    assert cache[0].offsets == [29] * 3 and cache[0].book.lengths.tolist() == [29] * 3 == cache[0].book.positions.tolist()
+
+
+@pytest.mark.parametrize("name,dtype", MODELS)
+def test_greedy_generation(name, dtype):
+    """generate_step over pages (captured decode step) keeps to the oracle's transcript but for near-ties."""
+    cfg, om, gm = make_pair(name, dtype=dtype)
+    ids = prompts_for(cfg, 4, 20, seed=3)
+    got = tokens_of(gm, ids, 40, gm.make_paged_cache(4, 64, page=16))
+    steps = [(y[:, 0], lg) for _, (y, lg) in zip(range(40), oracle_generate_step(ids, om))]
+    frac, near, real = greedy_report(got, np.stack([y for y, _ in steps], 1), [lg for _, lg in steps], LOGIT_TOL)
+    assert not real, real
+
+
+def test_prompt_in_portions(monkeypatch):
+    from mlx_parallm_b200.models import _transformer
+    cfg, om, gm = make_pair("small-llama", dtype="float16")
+    ids = prompts_for(cfg, 2, 150)
+    whole = gm(torch.from_numpy(ids), cache=gm.make_paged_cache(2, 160, page=48), last_only=True)
+    monkeypatch.setattr(_transformer, "MAX_TOKENS_PER_FORWARD", 100)
+    parts = gm(torch.from_numpy(ids), cache=gm.make_paged_cache(2, 160, page=48), last_only=True)
+    exp = om.forward(ids, om.make_cache(2), last_only=True)
+    assert rel_err(whole.cpu().numpy(), exp) < LOGIT_TOL and rel_err(parts.cpu().numpy(), exp) < LOGIT_TOL
+
+
+def test_window_that_hides_nothing_and_one_that_does():
+    cfg, om, gm = make_pair("small-llama", dtype="float16")
+    ids = prompts_for(cfg, 2, 60)
+    exp = om.forward(ids, om.make_cache(2), last_only=True)
+    wide = gm(torch.from_numpy(ids), cache=gm.make_paged_cache(2, 64, page=16, window=64, first=3), last_only=True).cpu().numpy()
+    assert rel_err(wide, exp) < LOGIT_TOL
+    cache = gm.make_paged_cache(2, 64, page=16, window=16, first=2)
+    narrow = gm(torch.from_numpy(ids), cache=cache, last_only=True).cpu().numpy()
+    assert np.isfinite(narrow).all() and rel_err(narrow, exp) > 10 * LOGIT_TOL
+
+
+@pytest.mark.parametrize("keep", [0, 24])
+def test_captured_and_eager_steps_agree(keep):
+    """The same tokens from a replayed and from a launched decode step, through growth of the rows and (keep) three cuts."""
+    from mlx_parallm_b200.utils import DecodeSession
+    cfg, _, gm = make_pair("small-llama", dtype="float16")
+    ids = torch.from_numpy(prompts_for(cfg, 3, 20, seed=5))
+    out = []
+    for graph in (False, True):
+        cache = gm.make_paged_cache(3, 48 if keep else 128, page=16, keep=keep, first=2, recent=8)
+        first = gm(ids, cache=cache, last_only=True)[:, -1].argmax(-1).to(torch.int32)
+        session = DecodeSession(gm, cache, 3, True, use_graph=graph)
+        session.tok.copy_(first)
+        toks = []
+        for _ in range(90):
+            session.run()
+            toks.append(session.tok.clone())
+            assert bool(torch.isfinite(session.logits).all())
+        out.append(torch.stack(toks, 1).cpu())
+        book = cache[0].book
+        assert book.positions.tolist() == [110] * 3 and book.lengths.tolist() == cache[0].offsets
+        assert [n + e for n, e in zip(cache[0].offsets, book.evicted)] == [110] * 3
+        if keep:
+            assert max(cache[0].offsets) <= 48 and sum(len(o) for o in book.owned) + len(book.free) == book.pages
+    assert torch.equal(out[0], out[1])
+
+
+def test_long_generation_with_cuts_through_generate_step():
+    cfg, _, gm = make_pair("tiny-qwen3", dtype="bfloat16")
+    got = tokens_of(gm, prompts_for(cfg, 2, 30), 200, gm.make_paged_cache(2, 64, page=16, keep=40, first=4))
+    assert got.shape == (2, 200) and (0 <= got).all() and (got < cfg["vocab_size"]).all()
+
+
+def test_rows_are_given_back_and_taken_again():
+    cfg, om, gm = make_pair("small-llama", dtype="float16")
+    cache = gm.make_paged_cache(2, 64, page=16, pages=4)
+    book = cache[0].book
+    ids = prompts_for(cfg, 2, 30)
+    gm(torch.from_numpy(ids), cache=cache)
+    assert len(book.free) == 0
+    with pytest.raises(RuntimeError, match="exhausted"):
+        gm(torch.from_numpy(ids[:, :9]), cache=cache)
+    for c in cache:
+        c.reset(2)
+    assert len(book.free) == 4 and int(book.table.max()) == -1
+    again = prompts_for(cfg, 2, 20, seed=9)
+    got = gm(torch.from_numpy(again), cache=cache, last_only=True).cpu().numpy()
+    assert rel_err(got, om.forward(again, om.make_cache(2), last_only=True)) < LOGIT_TOL
+
+
+def test_a_prompt_that_does_not_fit_is_refused():
+    cfg, _, gm = make_pair("tiny-llama", dtype="float16")
+    ids = torch.from_numpy(prompts_for(cfg, 1, 65))
+    with pytest.raises(RuntimeError, match="does not fit"):
+        gm(ids, cache=gm.make_paged_cache(1, 64, page=16))
+    with pytest.raises(RuntimeError, match="do not fit"):
+        gm(ids, cache=gm.make_paged_cache(1, 64, page=16, keep=32, first=2))

@@ -141,3 +141,60 @@ def test_oracle_of_the_append_turns_pairs():
         q, kk, _, _, _ = po.append(qkv, k, k, None, torch.zeros((1, 1), dtype=torch.int32), i, i + 3, i + 2, 1, rates, pairs, None, None, 0.0)
         assert abs(float(q[0, 0, 0]) - math.cos(2.0)) < 1e-12 and abs(float(q[0, 0, 2 if pairs == 0 else 1]) - math.sin(2.0)) < 1e-12
         assert abs(float(kk[0, 0, 3, 1]) - math.cos(1.0 if pairs == 0 else 2.0)) < 1e-12
+
+
+# ---------------------------------------------------------------- the book of pages
+def book(**kw):
+    from mlx_parallm_b200.models.paged import PageBook
+    return PageBook(**{**dict(rows=3, max_tokens=100, device="cpu", page=16), **kw})
+
+
+def test_book_gives_and_takes_pages():
+    b = book(pages=9)
+    assert b.width == 7 and b.max_tokens == 112
+    b.room_for([17, 0, 16])
+    assert [len(o) for o in b.owned] == [2, 0, 1] and len(b.free) == 6
+    assert b.table[0, :2].tolist() == b.owned[0] and int(b.table[0, 2]) == -1 and int(b.table[1].max()) == -1
+    b.room_for([17, 1, 32])                     # nothing new for row 0, a page each for the others
+    assert [len(o) for o in b.owned] == [2, 1, 2]
+    ids = [p for o in b.owned for p in o] + b.free
+    assert sorted(ids) == list(range(9))
+    before = [list(o) for o in b.owned]
+    with pytest.raises(RuntimeError, match="exhausted"):
+        b.room_for([100, 1, 32])
+    assert b.owned == before, "all or nothing"
+    with pytest.raises(RuntimeError, match="does not fit"):
+        b.room_for([113, 0, 0])
+    b.shrink([16, 0, 17])
+    assert [len(o) for o in b.owned] == [1, 0, 2] and int(b.table[1].max()) == -1 and int(b.table[0, 1]) == -1
+    assert sorted([p for o in b.owned for p in o] + b.free) == list(range(9))
+
+
+@pytest.mark.parametrize("bad", [dict(page=8), dict(page=40), dict(rows=0), dict(max_tokens=0), dict(pages=0), dict(window=-1), dict(first=-1),
+                                 dict(keep=112), dict(keep=10, first=8, recent=3), dict(keep=10, recent=-1)], ids=str)
+def test_book_refuses(bad):
+    with pytest.raises(ValueError):
+        book(**bad)
+
+
+def test_layers_share_the_book_and_keep_positions_of_the_text():
+    from mlx_parallm_b200.models.paged import PagedLayer
+    b = book()
+    layers = [PagedLayer(b, 4, 2, 64) for _ in range(2)]
+    assert layers[0].counters()[0] is b.lengths and layers[0].capacity == 112 and layers[1]._lengths is b.lengths
+    for c in layers:
+        c._offsets = [5, 20, 0]
+    b.evicted = [0, 7, 0]
+    b.room_for([5, 20, 0])
+    layers[0]._sync_lengths()
+    assert b.lengths.tolist() == [5, 20, 0] and b.positions.tolist() == [5, 27, 0]
+    layers[0].release_rows_host([1])
+    layers[0]._sync_lengths()
+    assert b.positions.tolist() == [5, 0, 0] and b.owned[1] == []
+    with pytest.raises(ValueError):
+        layers[0].reset(4)
+    for c in layers:
+        c.reset(3)
+    assert len(b.free) == b.pages and b.lengths.tolist() == [0, 0, 0] == b.positions.tolist() and layers[1].offsets == [0, 0, 0]
+    with pytest.raises(RuntimeError, match="adds up"):
+        b.cut(10, 0, 0)
