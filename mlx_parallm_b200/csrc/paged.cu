@@ -29,16 +29,16 @@ __device__ __forceinline__ float2 turn(int pos, float rate) {
 
 // Every head is split over 2^width_log2 lanes (the power of two that holds D / 8), 8 neighbouring values a lane: one to two 16-byte loads and stores, the
 // mean square by shuffles, a rotation partner from the lane that has it (pairs of halves) or from this one (neighbours).  A lane keeps its 8 angles and
-// walks over heads, two asked for at a time; a CTA holds 2^tpc_log2 tokens, each with (256 >> width_log2) >> tpc_log2 walkers, and where the tokens are few
+// walks over heads, four asked for ahead (two where a token's heads are shared out); a CTA holds 2^tpc_log2 tokens, each with (256 >> width_log2) >> tpc_log2 walkers, and where the tokens are few
 // gridDim.y CTAs share a token's heads.  fp32 from the read to the one rounding.  Bound by HBM from some hundred tokens on.  (A CTA per token, a warp per
 // head and an element per lane took 114 us for 6004 tokens of 64 + 16 heads.)
-template <typename T, typename TIN>
-__global__ void __launch_bounds__(256)
+template <typename T, typename TIN, int AHEAD>
+__global__ void __launch_bounds__(256, 3)
 paged_append_rows_kernel(TIN* qkv, int64_t ldq, T* q_out, T* kp, T* vp, float* mass, PageTable pt, const int32_t* t_row, const int32_t* t_slot,
                          const int32_t* t_pos, const T* qw, const T* kw, const float* rates, int n_rot, int pairs, float eps, int M, int H, int G, int D,
                          int width_log2, int tpc_log2) {
   constexpr bool ACC_IN = !std::is_same<TIN, T>::value;
-  constexpr int AHEAD = 2, IN = sizeof(TIN) * 8 / 16, OUT = sizeof(T) * 8 / 16;      // 16-byte pieces of 8 values
+  constexpr int IN = sizeof(TIN) * 8 / 16, OUT = sizeof(T) * 8 / 16;      // 16-byte pieces of 8 values
   __shared__ float2 s_turn[8][128];
   const int tpc = 1 << tpc_log2, width = 1 << width_log2, token0 = blockIdx.x << tpc_log2;
   pdl_wait();
@@ -74,38 +74,32 @@ paged_append_rows_kernel(TIN* qkv, int64_t ldq, T* q_out, T* kp, T* vp, float* m
   TIN* src = qkv + (int64_t)t * ldq + 8 * c;
   const int first = (int)blockIdx.y * step + (slot >> tpc_log2), stride = step * gridDim.y;
   uint4 in[AHEAD][IN];
-  auto fetch = [&](int head0) {
+  auto fetch = [&](uint4 (&into)[IN], int head) {
+    if (mine && (live || ACC_IN) && head < heads) {
+      uint4* p = reinterpret_cast<uint4*>(src + (int64_t)head * D);
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a)
-      if (mine && (live || ACC_IN) && head0 + a * stride < heads) {
-        uint4* p = reinterpret_cast<uint4*>(src + (int64_t)(head0 + a * stride) * D);
-#pragma unroll
-        for (int i = 0; i < IN; ++i) {
-          in[a][i] = p[i];
-          if (ACC_IN) p[i] = make_uint4(0, 0, 0, 0);
-        }
+      for (int i = 0; i < IN; ++i) {
+        into[i] = p[i];
+        if (ACC_IN) p[i] = make_uint4(0, 0, 0, 0);
       }
+    }
   };
-  fetch(first);
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a) fetch(in[a], first + a * stride);
 #pragma unroll 1
   for (int base = 0; base < heads; base += AHEAD * stride) {      // the same number of turns for every lane of a warp
-    uint4 now[AHEAD][IN];
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a)
-#pragma unroll
-      for (int i = 0; i < IN; ++i) now[a][i] = in[a][i];
-    fetch(base + first + AHEAD * stride);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
       const int head = base + first + a * stride;
       const bool ok = mine && live && head < heads;
       float x[8];
-      const TIN* v = reinterpret_cast<const TIN*>(now[a]);
+      const TIN* v = reinterpret_cast<const TIN*>(in[a]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[j] = ok ? Tr<TIN>::to_f(v[j]) : 0.f;
         if (ACC_IN) x[j] = Tr<T>::to_f(Tr<T>::from_f(x[j]));
       }
+      fetch(in[a], head + AHEAD * stride);
       if (qw || kw) {
         float ss = 0.f;
 #pragma unroll
@@ -269,6 +263,10 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
     return id < 0 ? 0u : weight_key(mass[(id * G + g) * pt.page + j % pt.page]);
   };
   for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s.hist[i] = 0;
+  if (held) {
+#pragma unroll 4
+    for (int j = j0 + tid; j < j1; j += SEL_THREADS) keys[j - j0] = look(j);      // (a thread looks at its own slots again below)
+  }
   __syncthreads();
   unsigned need = (unsigned)(keep - first - recent), prefix = 0, mask = 0;
   const bool picks = need > 0;
@@ -282,16 +280,7 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
     for (int b = j0 + warp * 32; b < j1; b += SEL_THREADS) {
       const int j = b + lane;
       uint32_t u = 0;
-      if (j < j1) {
-        if (!held) {
-          u = look(j);
-        } else if (pass == 0) {
-          u = look(j);
-          keys[j - j0] = u;
-        } else {
-          u = keys[j - j0];
-        }
-      }
+      if (j < j1) u = held ? keys[j - j0] : look(j);
       // tokens that nobody looked at have equal weights: one count for a warp whose keys share a digit
       const bool counts = picks && j < j1 && j >= lo && j < hi && (u & mask) == prefix;
       const unsigned d = (u >> shift) & (bins - 1), who = __ballot_sync(0xffffffffu, counts);
@@ -605,14 +594,16 @@ extern "C" int b200p_paged_append(void* qkv, int64_t ldq, void* q_out, void* kpa
     int64_t split = 2 * sms / M, most = (H + 2 * G + walkers - 1) / walkers;
     if (split < 1 || lg > 0) split = 1;
     const dim3 grid((unsigned)((M + (1 << lg) - 1) >> lg), (unsigned)(split < most ? split : most));
+    auto go = [&](auto t, auto in) {
+      using T = decltype(t);
+      using TIN = decltype(in);
+      launch_pdl(lg > 0 ? paged_append_rows_kernel<T, TIN, 4> : paged_append_rows_kernel<T, TIN, 2>, grid, 256, 0, st, (TIN*)qkv, ldq, (T*)q_out, (T*)kpages,
+                 (T*)vpages, mass, pt, t_row, t_slot, t_pos, (const T*)q_norm_w, (const T*)k_norm_w, rates, n_rot, pairs, eps, (int)M, H, G, D, width_log2, lg);
+    };
     if (qkv_f32) {
-      B200P_DISPATCH_DTYPE(dtype, T, (launch_pdl(paged_append_rows_kernel<T, float>, grid, 256, 0, st, (float*)qkv, ldq, (T*)q_out, (T*)kpages, (T*)vpages,
-                                          mass, pt, t_row, t_slot, t_pos, (const T*)q_norm_w, (const T*)k_norm_w, rates, n_rot, pairs, eps, (int)M, H, G, D,
-                                          width_log2, lg)));
+      B200P_DISPATCH_DTYPE(dtype, T, (go(T(), float())));
     } else {
-      B200P_DISPATCH_DTYPE(dtype, T, (launch_pdl(paged_append_rows_kernel<T, T>, grid, 256, 0, st, (T*)qkv, ldq, (T*)q_out, (T*)kpages, (T*)vpages, mass,
-                                          pt, t_row, t_slot, t_pos, (const T*)q_norm_w, (const T*)k_norm_w, rates, n_rot, pairs, eps, (int)M, H, G, D,
-                                          width_log2, lg)));
+      B200P_DISPATCH_DTYPE(dtype, T, (go(T(), T())));
     }
     B200P_LAUNCH_CHECK("paged_append_rows_kernel");
     return B200P_OK;
