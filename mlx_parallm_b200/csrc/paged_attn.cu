@@ -105,8 +105,8 @@ constexpr int PA_TOKENS = 512;         // up to so many tokens a CTA keeps all o
 
 struct Shares {
   unsigned n, q, r;                    // how many; the first r have q + 1 units, the others q
-  // of U units that belong to so many items: a join reads the parts one after the other, 64 are enough
-  __device__ Shares(unsigned U, unsigned items, unsigned ctas) : n(min(min(U, ctas), items < 65536 ? 64 * items : ctas)) {
+  // of U units that belong to so many items: a warp of the join reads its parts one after the other, 128 of an item are enough
+  __device__ Shares(unsigned U, unsigned items, unsigned ctas) : n(min(min(U, ctas), items < 65536 ? 128 * items : ctas)) {
     q = n ? U / n : 1;
     r = U - q * n;
   }
@@ -742,11 +742,10 @@ __device__ __forceinline__ const float* part_at(const PagedAttn& a, unsigned c0,
   return a.rec + (((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * rows + row) * (a.D + 4);
 }
 
-// A CTA per token and query head joins the parts where the item was cut: four warps take them in turn, then become one.  Few instructions: a launch
-// this short waits for its code more than for its data.
-constexpr int PJ_WARPS = 4;
-
-template <typename T, int NQ>            // 128 dimensions of a warp's lanes, NQ times
+// A CTA per token and query head joins the parts where the item was cut: its warps take them in turn, then become one.  Few instructions: a launch
+// this short waits for its code more than for its data.  Eight warps where the CTAs are few (one row of 1000 tokens of 32 heads, both launches, us, four /
+// eight warps: 7.8 / 7.4, one key head over 60000 tokens 24.1 / 19.9), four where they are many (64 rows of 40 heads 25.2 / 26.4).
+template <typename T, int NQ, int PJ_WARPS>            // 128 dimensions of a warp's lanes, NQ times
 __global__ void __launch_bounds__(PJ_WARPS * 32)
 paged_attn_join_kernel(const __grid_constant__ PagedAttn a, int rows_log2) {
   __shared__ float2 s_ml[PJ_WARPS];
@@ -905,10 +904,10 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   using T = typename E::T;
   const int per = a.H / a.G, rows_log2 = E::ROWS == 4 ? 2 : E::ROWS == 8 ? 3 : 4;
   const dim3 heads((unsigned)per, (unsigned)a.G, (unsigned)a.M);
-  if (a.D <= 128)
-    launch_pdl(paged_attn_join_kernel<T, 1>, heads, PJ_WARPS * 32, 0, st, a, rows_log2);
+  if ((int64_t)a.M * a.H <= 4 * sm_count())
+    launch_pdl(a.D <= 128 ? paged_attn_join_kernel<T, 1, 8> : paged_attn_join_kernel<T, 2, 8>, heads, 8 * 32, 0, st, a, rows_log2);
   else
-    launch_pdl(paged_attn_join_kernel<T, 2>, heads, PJ_WARPS * 32, 0, st, a, rows_log2);
+    launch_pdl(a.D <= 128 ? paged_attn_join_kernel<T, 1, 4> : paged_attn_join_kernel<T, 2, 4>, heads, 4 * 32, 0, st, a, rows_log2);
   B200P_LAUNCH_CHECK("paged_attn_join_kernel");
   if (!a.mass) return B200P_OK;
   // slices of the visible slots: as many as there are, but no more CTAs than fill the GPU
