@@ -73,7 +73,7 @@ struct PagedAttn {
   float* rec;          // [shares, 2, rows of a block, D + 4] parts: maximum, sum, -, -, outputs
   float* stat;         // [M, H, 2] maximum and 1 / sum of the heads that lie in one share (with a mass)
   float* scores;       // [M, items, cap, pitch] log2-scaled scores (with a mass)
-  uint64_t inv_tpp;    // 2^40 / (tiles of a page), rounded up: tile * inv_tpp >> 40 is the page's index for any tile below 2^26
+  uint64_t inv_tpp;    // 2^36 / (tiles of a page, 256 at most), rounded up: tile * inv_tpp >> 36 is the page's index for any tile below 2^26
   int tpp;
   int cap, pitch;      // visible slots a token can have, in whole tiles; heads of a line of scores, a power of two
 };
@@ -612,9 +612,9 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
         }
         if (tile >= tile_end) break;
         auto seek = [&]() {
-          const int kt = ls.key_tile(tile), index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 40);
+          const int kt = ls.key_tile(tile), index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 36);
           off = kt - index * a.tpp;
-          id = __ldg(table + index);
+          id = table[index];
         };
         if (turned) seek();
         const int j0 = ls.key0(tile);
@@ -816,7 +816,7 @@ paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks,
   auto look = [&](int x) {                                        // a slot's place and what its heads scored
     place = -1;
     if (x >= seen) return;
-    const int kt = tok.span.key_tile(x / PA_TILE), j = kt * PA_TILE + x % PA_TILE, index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 40);
+    const int kt = tok.span.key_tile(x / PA_TILE), j = kt * PA_TILE + x % PA_TILE, index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 36);
     if (!tok.span.visible(j)) return;
     const int64_t id = page_id(a.pt, tok.row, index);
     if (id < 0) return;
@@ -881,7 +881,7 @@ template <typename E>
 static int launch_paged(PagedAttn a, cudaStream_t st) {
   const int smem = E::Q_BYTES + E::WARPS * E::STAGES * E::tile_bytes(a.D);
   const int blocks = (a.H / a.G + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
-  B200P_REQUIRE((int64_t)a.M * items * (a.cap / PA_TILE / E::WARPS + 1) < (1ll << 31) && items < 65536, B200P_ERR_ARG,
+  B200P_REQUIRE((int64_t)a.M * items * (a.cap / PA_TILE / E::WARPS + 1) < (1ll << 31) && (int64_t)a.M * a.H < (1ll << 31) && items < 65536, B200P_ERR_ARG,
                 "%d tokens of %d key heads over %d slots: too many for one call", a.M, a.G, a.cap);
   auto kern = paged_attn_kernel<E>;
   static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
@@ -896,7 +896,7 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   const int64_t most = (int64_t)a.M * items * ((a.cap / PA_TILE + E::WARPS - 1) / E::WARPS);
   const int grid = (int)(most < ctas ? most : ctas);
   a.tpp = a.pt.page / PA_TILE;
-  a.inv_tpp = ((1ull << 40) + a.tpp - 1) / a.tpp;
+  a.inv_tpp = ((1ull << 36) + a.tpp - 1) / a.tpp;
   a.pitch = 1;
   while (a.pitch < E::ROWS && a.pitch < a.H / a.G) a.pitch *= 2;
   launch_pdl(kern, (unsigned)grid, E::WARPS * 32 + 32, smem, st, a);

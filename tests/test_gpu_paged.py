@@ -272,6 +272,43 @@ def test_attention_rows_share_pages(ops):
     _check_attn(ops, c, q, i32([0, 1, 2, 0]), i32([199, 89, 63, 150]), 8, 0, 0, True, 0.1)
 
 
+def test_attention_of_more_tokens_than_a_cta_keeps(ops):
+    """A portion of several rows as single tokens, more of them than a CTA holds in shared memory, idle ones among them."""
+    c = Cache([500, 150], 16, 2, 64, torch.bfloat16, 18)
+    row = i32([0] * 500 + [-1] * 7 + [1] * 150)
+    slot = i32(list(range(500)) + [3] * 7 + list(range(150)))
+    q = c.normal(row.numel(), 8 * 64).to(c.dtype)
+    for first, window, mass in ((0, 0, True), (5, 40, False)):
+        _check_attn(ops, c, q, row, slot, 8, first, window, mass, 0.125)
+
+
+def test_attention_of_many_key_heads(ops):
+    c = Cache([70, 33, 1], 32, 130, 8, torch.float16, 19)
+    q = c.normal(3, 260 * 8).to(c.dtype)
+    _check_attn(ops, c, q, i32([0, 1, 2]), i32([69, 32, 0]), 260, 0, 0, True, 0.3)
+
+
+def test_attention_in_very_wide_tables(ops):
+    """Tables of 2^30 tokens and a row at their end: tiles, pages and offsets beyond 16 million; only what is visible is looked up."""
+    G, D, H, page = 1, 64, 4, 16
+    width = (1 << 30) // page - 1
+    c = Cache([64, 64], page, G, D, torch.bfloat16, 20)
+    table = torch.full((1, width), -7, dtype=torch.int32, device="cuda")
+    table[0, :4] = c.table[0].cuda()
+    table[0, width - 4:] = c.table[1].cuda()
+    n = width * page
+    k, v = c.k.cuda(), c.v.cuda()
+    q = c.normal(1, H * D).to(c.dtype)
+    out = torch.empty((1, H * D), dtype=c.dtype, device="cuda")
+    ws = torch.empty((ops.paged_attn_workspace_bytes(1, H, D, 0),), dtype=torch.uint8, device="cuda")
+    ops.paged_attn(q.cuda(), k, v, table, i32([0]).cuda(), i32([n - 1]).cuda(), out, 0.125, first=30, window=50, workspace=ws)
+    # the same 30 first and 50 last tokens as a short row's: 30 of the first 64, then the last 50 of the other 64
+    near = torch.cat([c.table[0], c.table[1]])[None]
+    exp, tol, _, _ = po.attn(q, c.k, c.v, None, near, i32([0]), i32([127]), H, 0.125, 30, 50, po.half_step(c.dtype) ** 2)
+    err = (out.cpu().double().view(1, H, D) - exp).abs() - tol - po.half_step(c.dtype) * exp.abs() * 1.001
+    assert bool((err <= 0).all()) and ops.paged_fault_count(reset=True) == 0
+
+
 def test_attention_perm8_output(ops):
     c = Cache([200, 90], 16, 2, 128, torch.float16, 15)
     q = c.normal(2, 8 * 128).to(c.dtype)
