@@ -228,19 +228,21 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
 // the digit in which the need-th lies is found from the sums.  Then each warp counts what it keeps of its slots, and with the counts before it (of the keys
 // equal to the last one the lowest slots are kept) it writes them in order.  Bound by its few barriers: the weights are 4 bytes a slot.
 // (One CTA, 8 bits at a time from global memory: 40001 slots of 8 heads took 230 us.)
-constexpr int SEL_THREADS = 1024, SEL_WARPS = 32, SEL_MAX_CLUSTER = 8, SEL_BINS = 2048;
+constexpr int SEL_MAX_CLUSTER = 8, SEL_BINS = 2048;
 
 struct SelShared {
   unsigned hist[SEL_BINS], sums[SEL_BINS];
-  unsigned warp_sum[SEL_WARPS];
+  unsigned warp_sum[32];
   unsigned digit, left;
   bool all;
-  unsigned take[SEL_WARPS], eq[SEL_WARPS];
+  unsigned take[32], eq[32];
   unsigned all_above, all_eq;          // this CTA's, for the others
 };
 
+template <int SEL_THREADS>
 __global__ void __launch_bounds__(SEL_THREADS)
 paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int32_t* kept, int G, int keep, int first, int recent, int room) {
+  constexpr int SEL_WARPS = SEL_THREADS / 32, EACH = SEL_BINS / SEL_THREADS;
   extern __shared__ uint32_t keys[];
   __shared__ SelShared s;
   cg::cluster_group cluster = cg::this_cluster();
@@ -311,7 +313,12 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
     }
     // the digit: the largest with at least `need` keys from it up.  Thread i holds the digits [i w, (i + 1) w) counted from the top
     const int w = bins / SEL_THREADS, top = bins - 1 - tid * w;
-    const unsigned c0 = sums[top], c1 = w > 1 ? sums[top - 1] : 0, mine = c0 + c1;
+    unsigned c[EACH], mine = 0;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      c[k] = k < w ? sums[top - k] : 0;
+      mine += c[k];
+    }
     unsigned before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -321,14 +328,19 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
     if (lane == 31) s.warp_sum[warp] = before;
     __syncthreads();
     for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s.hist[i] = 0;
-    unsigned others = lane < warp ? s.warp_sum[lane] : 0;
+    unsigned others = lane < warp ? s.warp_sum[lane] : 0;      // (warp: below 32)
     others = __reduce_add_sync(0xffffffffu, others);
     before += others - mine;
     if (before < need && before + mine >= need) {
-      const bool second = before + c0 < need;
-      s.digit = top - second;
-      s.left = need - before - (second ? c0 : 0);
-      s.all = (second ? c1 : c0) == s.left;
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        if (before < need && before + c[k] >= need) {
+          s.digit = top - k;
+          s.left = need - before;
+          s.all = c[k] == need - before;
+        }
+        before += c[k];
+      }
     }
     __syncthreads();
     prefix |= s.digit << shift;
@@ -357,7 +369,7 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
     s.eq[warp] = equal;
   }
   __syncthreads();
-  unsigned a = s.take[lane], e = s.eq[lane], sum_a = a, sum_e = e;
+  unsigned a = lane < SEL_WARPS ? s.take[lane] : 0, e = lane < SEL_WARPS ? s.eq[lane] : 0, sum_a = a, sum_e = e;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned x = __shfl_up_sync(0xffffffffu, sum_a, o), y = __shfl_up_sync(0xffffffffu, sum_e, o);
@@ -398,7 +410,9 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
 // Bound by HBM where rows and heads are many.
 constexpr int MOVE_THREADS = 256, MOVE_STAGES = 4, MOVE_LINES = 2048, MOVE_MAX_CLUSTER = 8;
 constexpr int MOVE_UNITS_ONE = 4, MOVE_UNITS_CLUSTER = 20;        // 16-byte pieces of a thread in a round
-static constexpr int move_smem(int stages, int units) { return stages * units * MOVE_THREADS * 16 + MOVE_LINES * 16; }
+// shared memory of a CTA's share: the ring's stages that its rounds use, and the lists of its lines
+__host__ __device__ inline int move_ring(int stages, int units, int rounds) { return min(stages, rounds) * units * MOVE_THREADS * 16; }
+__host__ __device__ inline int move_lists(int rounds, int lines) { return min(MOVE_LINES, rounds * lines); }
 
 template <int STAGES, int UNITS>
 __global__ void __launch_bounds__(MOVE_THREADS)
@@ -406,8 +420,6 @@ paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int3
                      int keep) {
   extern __shared__ __align__(16) uint8_t smem[];
   uint4* ring = reinterpret_cast<uint4*>(smem);
-  int64_t* from = reinterpret_cast<int64_t*>(smem + STAGES * UNITS * MOVE_THREADS * 16);
-  int64_t* to = from + MOVE_LINES;
   cg::cluster_group cluster = cg::this_cluster();
   const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x;
   const int g = blockIdx.y >> 1, r = blockIdx.z;
@@ -429,6 +441,9 @@ paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int3
   };
   // in round m this CTA takes the kept slots from (m S + rank) lines on
   const int lines = min(MOVE_THREADS * UNITS / chunks, MOVE_LINES), rounds = (keep + S * lines - 1) / (S * lines), ahead = MOVE_LINES / lines;
+  const int listed = move_lists(rounds, lines);
+  int64_t* from = reinterpret_cast<int64_t*>(smem + move_ring(STAGES, UNITS, rounds));
+  int64_t* to = from + listed;
   for (int m0 = 0; m0 < rounds; m0 += ahead) {
     const int m1 = min(rounds, m0 + ahead);
     constexpr int EACH = MOVE_LINES / MOVE_THREADS;
@@ -446,8 +461,10 @@ paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int3
         }
       }
       if (src < 0 || dst < 0) src = dst = -1;
-      from[q] = src;
-      to[q] = dst;
+      if (q < listed) {
+        from[q] = src;
+        to[q] = dst;
+      }
       weight_to[k] = mass && !values ? dst : -1;
       weight[k] = weight_to[k] >= 0 ? mass[src] : 0.f;
     }
@@ -630,11 +647,13 @@ extern "C" int b200p_paged_select(const float* mass, const int32_t* table, const
   B200P_REQUIRE(rows < 65536, B200P_ERR_ARG, "too many rows");
   B200P_REQUIRE(G < 32768, B200P_ERR_ARG, "too many key heads");
   constexpr int SEL_ROOM = 48 * 1024;                             // keys: 192 KB
+  auto large = paged_select_kernel<1024>;
+  auto small = paged_select_kernel<256>;
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
-    e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_ROOM * 4);
+    e = cudaFuncSetAttribute(large, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_ROOM * 4);
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_select_kernel)");
@@ -644,8 +663,10 @@ extern "C" int b200p_paged_select(const float* mass, const int32_t* table, const
   while (S > 1 && slots / S < 2048) S /= 2;
   int64_t room = ((slots + S - 1) / S + 31) / 32 * 32;
   if (room > SEL_ROOM) room = 0;                                  // (a shorter row of such a table is read three times all the same)
-  e = launch_clusters(paged_select_kernel, S, G, rows, SEL_THREADS, (size_t)room * 4, (cudaStream_t)stream, mass, pt, lengths, kept, G, keep, first, recent,
-                      (int)room);
+  // short rows in numbers: a CTA of 256 threads has less to set up, and more of them fit an SM
+  const bool many = slots <= 4096 && (int64_t)G * rows > 2 * sm_count();
+  e = launch_clusters(many ? small : large, S, G, rows, many ? 256 : 1024, (size_t)room * 4, (cudaStream_t)stream, mass, pt, lengths, kept, G, keep, first,
+                      recent, (int)room);
   if (e != cudaSuccess) return cuda_fail(e, "paged_select_kernel");
   B200P_LAUNCH_CHECK("paged_select_kernel");
   return B200P_OK;
@@ -660,22 +681,25 @@ extern "C" int b200p_paged_compact(void* kpages, void* vpages, float* mass, cons
   B200P_REQUIRE(rows < 65536, B200P_ERR_ARG, "too many rows");
   const int chunks = D * (dtype == B200P_F32 ? 4 : 2) / 16;
   B200P_REQUIRE(G < 32768, B200P_ERR_ARG, "too many key heads");
-  constexpr int ONE = move_smem(MOVE_STAGES, MOVE_UNITS_ONE), CLUSTER = move_smem(1, MOVE_UNITS_CLUSTER);
   auto one = paged_compact_kernel<MOVE_STAGES, MOVE_UNITS_ONE>;
   auto many = paged_compact_kernel<1, MOVE_UNITS_CLUSTER>;
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
-    e = cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize, ONE);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize, CLUSTER);
+    e = cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             move_ring(MOVE_STAGES, MOVE_UNITS_ONE, MOVE_STAGES) + MOVE_LINES * 16);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       move_ring(1, MOVE_UNITS_CLUSTER, 1) + MOVE_LINES * 16);
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_compact_kernel)");
   int S = cluster_of((int64_t)2 * G * rows, MOVE_MAX_CLUSTER, 2);
   while (S > 1 && keep * chunks <= S * 1024) S /= 2;               // (at least 16 KB of lines each)
   const unsigned inv = (unsigned)(((1ull << 32) + chunks - 1) / chunks);
-  e = launch_clusters(S > 1 ? many : one, S, 2 * G, rows, MOVE_THREADS, S > 1 ? CLUSTER : ONE, (cudaStream_t)stream, (uint4*)kpages, (uint4*)vpages, mass, pt,
+  const int stages = S > 1 ? 1 : MOVE_STAGES, units = S > 1 ? MOVE_UNITS_CLUSTER : MOVE_UNITS_ONE, lines = min(MOVE_THREADS * units / chunks, MOVE_LINES);
+  const int rounds = (int)(((int64_t)keep + S * lines - 1) / (S * lines)), smem = move_ring(stages, units, rounds) + move_lists(rounds, lines) * 16;
+  e = launch_clusters(S > 1 ? many : one, S, 2 * G, rows, MOVE_THREADS, smem, (cudaStream_t)stream, (uint4*)kpages, (uint4*)vpages, mass, pt,
                       lengths, kept, G, chunks, inv, keep);
   if (e != cudaSuccess) return cuda_fail(e, "paged_compact_kernel");
   B200P_LAUNCH_CHECK("paged_compact_kernel");

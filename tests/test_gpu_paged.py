@@ -368,6 +368,7 @@ EVICT = [
     ("bf16", 1, 8, 16, [33, 17], 1, 0, 0),
     ("f16", 1, 128, 16, [9000, 3], 4500, 1, 1000),
     ("f32", 2, 96, 128, [700, 300], 77, 0, 77),
+    ("bf16", 8, 16, 16, [100, 60, 61, 99, 0] * 8, 60, 3, 20),          # more rows and heads than two for every SM
 ]
 
 
