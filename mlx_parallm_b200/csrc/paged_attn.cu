@@ -744,34 +744,49 @@ __device__ __forceinline__ const float* part_at(const PagedAttn& a, unsigned c0,
 
 // A CTA per token and query head joins the parts where the item was cut: its warps take them in turn, then become one.  Few instructions: a launch
 // this short waits for its code more than for its data.  Eight warps where the CTAs are few (one row of 1000 tokens of 32 heads, both launches, us, four /
-// eight warps: 7.8 / 7.4, one key head over 60000 tokens 24.1 / 19.9), four where they are many (64 rows of 40 heads 25.2 / 26.4).
-template <typename T, int NQ, int PJ_WARPS>            // 128 dimensions of a warp's lanes, NQ times
-__global__ void __launch_bounds__(PJ_WARPS * 32)
-paged_attn_join_kernel(const __grid_constant__ PagedAttn a, int rows_log2) {
+// eight warps: 7.8 / 7.4), four where they are many (64 rows of 40 heads 25.2 / 26.4).  PJ_AHEAD parts of a warp on their way at once: four for the few,
+// which have long lists (one key head over 60000 tokens 20.0 with one, 17.9 with three, 17.2 with four, 16.5 with eight, but one row of 1000 then 7.3 ->
+// 7.5), one for the many (64 rows of 40 heads 25.2, with four 26.1).
+template <typename T, int NQ, int PJ_WARPS, int PJ_AHEAD>  // 128 dimensions of a warp's lanes, NQ times
+__device__ __forceinline__ void join_parts(const PagedAttn& a, int t, int64_t line, int row, int64_t head, int block_rows) {
   __shared__ float2 s_ml[PJ_WARPS];
   __shared__ float4 s_o[PJ_WARPS][32 * NQ];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.x, g = blockIdx.y, t = blockIdx.z, block_rows = 1 << rows_log2, blk = r >> rows_log2, row = r & (block_rows - 1);
-  const int blocks = (gridDim.x + block_rows - 1) >> rows_log2;
-  pdl_wait();
   const int token_row = a.t_row[t];
-  const uint2 parts = a.parts[((int64_t)t * a.G + g) * blocks + blk];
+  const uint2 parts = a.parts[line];
   if (token_row < 0 || token_row >= a.pt.rows || parts.y < 2) return;
   float M = -INFINITY, L = 0.f;
   float4 acc[NQ];
 #pragma unroll
   for (int x = 0; x < NQ; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-  for (unsigned i = warp; i < parts.y; i += PJ_WARPS) {
-    const float* p = part_at(a, parts.x, i, block_rows, row);
-    const float2 ml = *reinterpret_cast<const float2*>(p);
-    const float top = fmaxf(M, ml.x), ref = top == -INFINITY ? 0.f : top, f = raise2(M - ref), w = raise2(ml.x - ref);
-    M = top;
-    L = L * f + ml.y * w;
+#pragma unroll 1
+  for (unsigned i0 = warp; i0 < parts.y; i0 += PJ_AHEAD * PJ_WARPS) {
+    float2 ml[PJ_AHEAD];
+    float4 y[PJ_AHEAD][NQ];
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      const float4 y = 4 * lane + 128 * x < a.D ? *reinterpret_cast<const float4*>(p + 4 + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
-      acc[x].x = acc[x].x * f + y.x * w, acc[x].y = acc[x].y * f + y.y * w, acc[x].z = acc[x].z * f + y.z * w, acc[x].w = acc[x].w * f + y.w * w;
+    for (int u = 0; u < PJ_AHEAD; ++u) {
+      const unsigned i = i0 + u * PJ_WARPS;
+      const bool in = i < parts.y;
+      const float* p = part_at(a, parts.x, i, block_rows, row);
+      ml[u] = in ? *reinterpret_cast<const float2*>(p) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+        y[u][x] = in && 4 * lane + 128 * x < a.D ? *reinterpret_cast<const float4*>(p + 4 + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top = M;
+#pragma unroll
+    for (int u = 0; u < PJ_AHEAD; ++u) top = fmaxf(top, ml[u].x);
+    const float ref = top == -INFINITY ? 0.f : top, f = raise2(M - ref);
+    M = top;
+    L *= f;
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) acc[x].x *= f, acc[x].y *= f, acc[x].z *= f, acc[x].w *= f;
+#pragma unroll
+    for (int u = 0; u < PJ_AHEAD; ++u) {
+      const float w = raise2(ml[u].x - ref);
+      L += ml[u].y * w;
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) acc[x].x += y[u][x].x * w, acc[x].y += y[u][x].y * w, acc[x].z += y[u][x].z * w, acc[x].w += y[u][x].w * w;
     }
   }
   if (lane == 0) s_ml[warp] = make_float2(M, L);
@@ -794,12 +809,21 @@ paged_attn_join_kernel(const __grid_constant__ PagedAttn a, int rows_log2) {
     o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  store_row4<T>(reinterpret_cast<T*>(a.out) + ((int64_t)t * a.H + g * gridDim.x + r) * a.D, d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), a.out_perm);
+  store_row4<T>(reinterpret_cast<T*>(a.out) + head * a.D, d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), a.out_perm);
 }
 
-// The weights that every visible slot received: a CTA per item (x) and slice of its visible slots (y), a thread per slot.  The heads' maxima and sums
-// come from the parts again (a warp per head, a lane per part), which needs no word from the join.
-template <int ROWS>
+template <typename T, int NQ, int PJ_WARPS>
+__global__ void __launch_bounds__(PJ_WARPS * 32)
+paged_attn_join_kernel(const __grid_constant__ PagedAttn a, int rows_log2) {
+  const int r = blockIdx.x, g = blockIdx.y, t = blockIdx.z, rows = 1 << rows_log2, blocks = (gridDim.x + rows - 1) >> rows_log2;
+  pdl_wait();
+  join_parts<T, NQ, PJ_WARPS, PJ_WARPS == 8 ? 4 : 1>(a, t, ((int64_t)t * a.G + g) * blocks + (r >> rows_log2), r & (rows - 1), ((int64_t)t * a.G + g) * gridDim.x + r, rows);
+}
+
+// With a mass, one launch for both: the first ROWS CTAs (x) of an item (y) of a token (z) join its heads, the others are slices of its visible slots, a
+// thread per slot, and add up the weights that it received.  The heads' maxima and sums come from the parts again (a warp per head, a lane per part),
+// which needs no word from the join.
+template <typename T, int NQ, int ROWS>
 __global__ void __launch_bounds__(256)
 paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks, int warps) {
   __shared__ float2 s_stat[ROWS];
@@ -807,10 +831,15 @@ paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks,
   const int t = blockIdx.z, item = blockIdx.y, g = blocks == 1 ? item : item / blocks, r0 = (item - g * blocks) * ROWS, rows = min(ROWS, per - r0);
   const int64_t head = (int64_t)t * a.H + (int64_t)g * per + r0, line = (int64_t)t * items + item;
   pdl_wait();
+  if (blockIdx.x < ROWS) {
+    if ((int)blockIdx.x < rows) join_parts<T, NQ, 8, 1>(a, t, line, blockIdx.x, head + blockIdx.x, ROWS);
+    return;
+  }
+  const int slice = blockIdx.x - ROWS, slices = gridDim.x - ROWS;
   const Token tok(a, t, warps);
   const uint2 parts = a.parts[line];
   const int seen = tok.span.tiles * PA_TILE;
-  if ((int)blockIdx.x * 256 >= seen) return;
+  if (slice * 256 >= seen) return;
   float w8[ROWS];
   int64_t place = -1;
   auto look = [&](int x) {                                        // a slot's place and what its heads scored
@@ -831,7 +860,7 @@ paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks,
       if (a.pitch > 1) w8[1] = p[1];
     }
   };
-  const int x0 = blockIdx.x * 256 + threadIdx.x;
+  const int x0 = slice * 256 + threadIdx.x;
   look(x0);                                                       // on its way beside the parts
 #pragma unroll 1
   for (int r = warp; r < rows; r += 8) {
@@ -854,7 +883,7 @@ paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks,
   }
   __syncthreads();
 #pragma unroll 1
-  for (int x = x0; x < seen; x += gridDim.x * 256) {
+  for (int x = x0; x < seen; x += slices * 256) {
     if (x != x0) look(x);
     if (place < 0) continue;
     float w = 0.f;
@@ -904,17 +933,19 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   using T = typename E::T;
   const int per = a.H / a.G, rows_log2 = E::ROWS == 4 ? 2 : E::ROWS == 8 ? 3 : 4;
   const dim3 heads((unsigned)per, (unsigned)a.G, (unsigned)a.M);
+  if (a.mass) {
+    // slices of the visible slots: as many as there are, but no more CTAs than fill the GPU
+    const int64_t slices = (a.cap + 255) / 256, fill = (6ll * sm_count() + (int64_t)a.M * items - 1) / ((int64_t)a.M * items);
+    const dim3 rest((unsigned)(E::ROWS + (slices < fill ? slices : fill)), (unsigned)items, (unsigned)a.M);
+    launch_pdl(a.D <= 128 ? paged_attn_mass_kernel<T, 1, E::ROWS> : paged_attn_mass_kernel<T, 2, E::ROWS>, rest, 256, 0, st, a, per, blocks, (int)E::WARPS);
+    B200P_LAUNCH_CHECK("paged_attn_mass_kernel");
+    return B200P_OK;
+  }
   if ((int64_t)a.M * a.H <= 4 * sm_count())
     launch_pdl(a.D <= 128 ? paged_attn_join_kernel<T, 1, 8> : paged_attn_join_kernel<T, 2, 8>, heads, 8 * 32, 0, st, a, rows_log2);
   else
     launch_pdl(a.D <= 128 ? paged_attn_join_kernel<T, 1, 4> : paged_attn_join_kernel<T, 2, 4>, heads, 4 * 32, 0, st, a, rows_log2);
   B200P_LAUNCH_CHECK("paged_attn_join_kernel");
-  if (!a.mass) return B200P_OK;
-  // slices of the visible slots: as many as there are, but no more CTAs than fill the GPU
-  const int64_t slices = (a.cap + 255) / 256, fill = (6ll * sm_count() + (int64_t)a.M * items - 1) / ((int64_t)a.M * items);
-  launch_pdl(paged_attn_mass_kernel<E::ROWS>, dim3((unsigned)(slices < fill ? slices : fill), (unsigned)items, (unsigned)a.M), 256, 0, st, a, per, blocks,
-             (int)E::WARPS);
-  B200P_LAUNCH_CHECK("paged_attn_mass_kernel");
   return B200P_OK;
 }
 
