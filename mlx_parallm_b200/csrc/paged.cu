@@ -654,7 +654,7 @@ extern "C" int b200p_paged_select(const float* mass, const int32_t* table, const
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
     e = cudaFuncSetAttribute(large, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_ROOM * 4);
-    if (dev < 64) ready.fetch_or(1ull << dev);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_select_kernel)");
   const int64_t slots = (int64_t)width * page;
@@ -691,7 +691,7 @@ extern "C" int b200p_paged_compact(void* kpages, void* vpages, float* mass, cons
                              move_ring(MOVE_STAGES, MOVE_UNITS_ONE, MOVE_STAGES) + MOVE_LINES * 16);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                        move_ring(1, MOVE_UNITS_CLUSTER, 1) + MOVE_LINES * 16);
-    if (dev < 64) ready.fetch_or(1ull << dev);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_compact_kernel)");
   int S = cluster_of((int64_t)2 * G * rows, MOVE_MAX_CLUSTER, 2);

@@ -55,6 +55,7 @@ struct Span {
     tiles = n > 0 ? t0 + (n + PA_TILE - 1) / PA_TILE - skip : 0;
   }
   __device__ int key_tile(int v) const { return v < t0 ? v : v - t0 + skip; }
+  __device__ int tile_of(int kt) const { return kt < t0 ? kt : kt - skip + t0; }
   __device__ int key0(int v) const { return key_tile(v) * PA_TILE; }
   __device__ bool visible(int j) const { return j < n && (j < first || j >= lo); }
   __device__ bool whole(int j0) const { return j0 + PA_TILE <= n && (j0 >= lo || j0 + PA_TILE <= first); }
@@ -820,77 +821,136 @@ paged_attn_join_kernel(const __grid_constant__ PagedAttn a, int rows_log2) {
   join_parts<T, NQ, PJ_WARPS, PJ_WARPS == 8 ? 4 : 1>(a, t, ((int64_t)t * a.G + g) * blocks + (r >> rows_log2), r & (rows - 1), ((int64_t)t * a.G + g) * gridDim.x + r, rows);
 }
 
-// With a mass, one launch for both: the first ROWS CTAs (x) of an item (y) of a token (z) join its heads, the others are slices of its visible slots, a
-// thread per slot, and add up the weights that it received.  The heads' maxima and sums come from the parts again (a warp per head, a lane per part),
-// which needs no word from the join.
+// With a mass, one launch for both: the first ROWS CTAs (x) of an item (y) of a token (z) join its heads, the others are slices of the row's visible
+// slots, a thread per slot, and add up the weights that it received.  The heads' maxima and sums come from the parts again (a warp per head, a lane per
+// part), which needs no word from the join.  The slices of a row's first token in the call do so for all of the row's tokens and all of their
+// heads in turn, the others leave, so that a slot's weights are added by one thread in one order (unless rows share its page).
 template <typename T, int NQ, int ROWS>
 __global__ void __launch_bounds__(256)
 paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks, int warps) {
-  __shared__ float2 s_stat[ROWS];
+  __shared__ float2 s_stat[2][ROWS];
+  __shared__ int s_from[8];
+  __shared__ int2 s_seen[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, items = a.G * blocks;
-  const int t = blockIdx.z, item = blockIdx.y, g = blocks == 1 ? item : item / blocks, r0 = (item - g * blocks) * ROWS, rows = min(ROWS, per - r0);
-  const int64_t head = (int64_t)t * a.H + (int64_t)g * per + r0, line = (int64_t)t * items + item;
-  pdl_wait();
+  const int t = blockIdx.z, item = blockIdx.y, g = blocks == 1 ? item : item / blocks, block = item - g * blocks;
   if (blockIdx.x < ROWS) {
-    if ((int)blockIdx.x < rows) join_parts<T, NQ, 8, 1>(a, t, line, blockIdx.x, head + blockIdx.x, ROWS);
+    const int r0 = block * ROWS;
+    pdl_wait();
+    if (r0 + (int)blockIdx.x < per)
+      join_parts<T, NQ, 8, 1>(a, t, (int64_t)t * items + item, blockIdx.x, (int64_t)t * a.H + (int64_t)g * per + r0 + blockIdx.x, ROWS);
     return;
   }
-  const int slice = blockIdx.x - ROWS, slices = gridDim.x - ROWS;
-  const Token tok(a, t, warps);
-  const uint2 parts = a.parts[line];
-  const int seen = tok.span.tiles * PA_TILE;
-  if (slice * 256 >= seen) return;
-  float w8[ROWS];
-  int64_t place = -1;
-  auto look = [&](int x) {                                        // a slot's place and what its heads scored
-    place = -1;
-    if (x >= seen) return;
-    const int kt = tok.span.key_tile(x / PA_TILE), j = kt * PA_TILE + x % PA_TILE, index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 36);
-    if (!tok.span.visible(j)) return;
-    const int64_t id = page_id(a.pt, tok.row, index);
-    if (id < 0) return;
-    place = (id * a.G + g) * a.pt.page + (kt - index * a.tpp) * PA_TILE + x % PA_TILE;
-    const float* p = a.scores + (line * a.cap + x) * a.pitch;
-    if (a.pitch >= 4) {
-#pragma unroll
-      for (int r = 0; r < ROWS; r += 4)
-        if (r < a.pitch) *reinterpret_cast<float4*>(w8 + r) = *reinterpret_cast<const float4*>(p + r);
-    } else {
-      w8[0] = p[0];
-      if (a.pitch > 1) w8[1] = p[1];
-    }
-  };
-  const int x0 = slice * 256 + threadIdx.x;
-  look(x0);                                                       // on its way beside the parts
+  if (block) return;
+  // The tokens' rows and slots are older than the launch before this one, which let this one begin behind its own wait.
+  const int slice = blockIdx.x - ROWS, slices = gridDim.x - ROWS, row = a.t_row[t];
+  if (row < 0 || row >= a.pt.rows) return;
+  bool before = false;                                            // a token of this row stands before this one: most often close by
+  unsigned first32 = 0;                                           // which of the next tokens, this warp's 32 of 256, are of this row
+  int lo = INT_MAX, hi = 0;                                       // the fewest and the most slots that one of them sees
 #pragma unroll 1
-  for (int r = warp; r < rows; r += 8) {
-    float2 st;
-    if (parts.y < 2) {
-      st = reinterpret_cast<const float2*>(a.stat)[head + r];
-    } else {
-      float M = -INFINITY, L = 0.f;
-#pragma unroll 1
-      for (unsigned i = lane; i < parts.y; i += 32) {
-        const float2 ml = *reinterpret_cast<const float2*>(part_at(a, parts.x, i, ROWS, r));
-        const float top = fmaxf(M, ml.x), ref = top == -INFINITY ? 0.f : top;
-        L = L * raise2(M - ref) + ml.y * raise2(ml.x - ref);
-        M = top;
-      }
-      const float top = warp_max(M), ref = top == -INFINITY ? 0.f : top, sum = warp_sum(L * raise2(M - ref));
-      st = make_float2(ref, sum == 0.f ? 0.f : 1.f / sum);
+  for (int i0 = 0; i0 < a.M; i0 += 256) {
+    const int i = i0 + threadIdx.x;
+    const bool mine = i < a.M - t && a.t_row[t + i] == row;
+    if (i < t) before |= a.t_row[t - 1 - i] == row;
+    if (mine) {
+      const int n = slots_seen(a.pt, a.t_slot[t + i]);
+      lo = min(lo, n), hi = max(hi, n);
     }
-    if (lane == 0) s_stat[r] = st;
+    const unsigned found = __ballot_sync(~0u, mine);
+    if (i0 == 0) {
+      first32 = found;
+      if (a.M > 256 && __syncthreads_or(before)) return;
+    }
   }
+  lo = __reduce_min_sync(~0u, lo), hi = __reduce_max_sync(~0u, hi), before = __any_sync(~0u, before);
+  if (lane == 0) s_from[warp] = (int)first32, s_seen[warp] = make_int2(lo, before ? -1 : hi);
   __syncthreads();
-#pragma unroll 1
-  for (int x = x0; x < seen; x += slices * 256) {
-    if (x != x0) look(x);
-    if (place < 0) continue;
-    float w = 0.f;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-      if (r < rows) w += raise2(w8[r] - s_stat[r].x) * s_stat[r].y;
-    atomicAdd(a.mass + place, w);                                 // slots that several tokens see
+  for (int w = 0; w < 8; ++w) {
+    if (s_seen[w].y < 0) return;
+    lo = min(lo, s_seen[w].x), hi = max(hi, s_seen[w].y);
+  }
+  const Span all(hi, a.first, lo < a.window || !a.window ? 0 : a.window + hi - lo);      // what any of them sees
+  const int seen = all.tiles * PA_TILE;
+  if (slice * 256 >= seen) return;
+  int buffer = 0;
+  bool waited = false;
+#pragma unroll 1
+  for (int base = t; base < a.M; base += 256) {
+    // the row's tokens among the next 256, in their order
+    unsigned found;
+    if (base > t) {
+      found = __ballot_sync(~0u, base + threadIdx.x < a.M && a.t_row[base + threadIdx.x] == row);
+      __syncthreads();
+      if (lane == 0) s_from[warp] = (int)found;
+      __syncthreads();
+    }
+#pragma unroll 1
+    for (int w = 0; w < 8; ++w)
+#pragma unroll 1
+      for (found = (unsigned)s_from[w]; found; found &= found - 1) {
+        const int tt = base + 32 * w + __ffs(found) - 1;
+        const Span span(slots_seen(a.pt, a.t_slot[tt]), a.first, a.window);
+        if (!waited) pdl_wait(), waited = true;
+#pragma unroll 1
+        for (int blk = 0; blk < blocks; ++blk, buffer ^= 1) {
+          const int rows = min(ROWS, per - blk * ROWS);
+          const int64_t line = (int64_t)tt * items + g * blocks + blk, head = (int64_t)tt * a.H + (int64_t)g * per + blk * ROWS;
+          const uint2 parts = a.parts[line];
+          float w8[ROWS];
+          int64_t place = -1;
+          auto look = [&](int x) {                                // a slot's place and what its heads scored
+            place = -1;
+            if (x >= seen) return;
+            const int kt = all.key_tile(x / PA_TILE), j = kt * PA_TILE + x % PA_TILE, index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 36);
+            if (!span.visible(j)) return;
+            const int64_t id = page_id(a.pt, row, index);
+            if (id < 0) return;
+            place = (id * a.G + g) * a.pt.page + (kt - index * a.tpp) * PA_TILE + x % PA_TILE;
+            const float* p = a.scores + (line * a.cap + span.tile_of(kt) * PA_TILE + x % PA_TILE) * a.pitch;
+            if (a.pitch >= 4) {
+#pragma unroll
+              for (int r = 0; r < ROWS; r += 4)
+                if (r < a.pitch) *reinterpret_cast<float4*>(w8 + r) = *reinterpret_cast<const float4*>(p + r);
+            } else {
+              w8[0] = p[0];
+              if (a.pitch > 1) w8[1] = p[1];
+            }
+          };
+          const int x0 = slice * 256 + threadIdx.x;
+          look(x0);                                               // on its way beside the parts
+#pragma unroll 1
+          for (int r = warp; r < rows; r += 8) {
+            float2 st;
+            if (parts.y < 2) {
+              st = reinterpret_cast<const float2*>(a.stat)[head + r];
+            } else {
+              float M = -INFINITY, L = 0.f;
+#pragma unroll 1
+              for (unsigned i = lane; i < parts.y; i += 32) {
+                const float2 ml = *reinterpret_cast<const float2*>(part_at(a, parts.x, i, ROWS, r));
+                const float top = fmaxf(M, ml.x), ref = top == -INFINITY ? 0.f : top;
+                L = L * raise2(M - ref) + ml.y * raise2(ml.x - ref);
+                M = top;
+              }
+              const float top = warp_max(M), ref = top == -INFINITY ? 0.f : top, sum = warp_sum(L * raise2(M - ref));
+              st = make_float2(ref, sum == 0.f ? 0.f : 1.f / sum);
+            }
+            if (lane == 0) s_stat[buffer][r] = st;
+          }
+          __syncthreads();
+#pragma unroll 1
+          for (int x = x0; x < seen; x += slices * 256) {
+            if (x != x0) look(x);
+            if (place < 0) continue;
+            float w = 0.f;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+              if (r < rows) w += raise2(w8[r] - s_stat[buffer][r].x) * s_stat[buffer][r].y;
+            atomicAdd(a.mass + place, w);                         // (rows may share the page)
+          }
+        }
+      }
   }
 }
 
@@ -918,7 +978,7 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024);
-    if (dev < 64) ready.fetch_or(1ull << dev);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_attn_kernel)");
   const int ctas = sm_count() * E::CTAS;

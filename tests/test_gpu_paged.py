@@ -272,6 +272,30 @@ def test_attention_rows_share_pages(ops):
     _check_attn(ops, c, q, i32([0, 1, 2, 0]), i32([199, 89, 63, 150]), 8, 0, 0, True, 0.1)
 
 
+@pytest.mark.parametrize("dtype,H,G,D,first,window", [("bf16", 8, 2, 128, 0, 0), ("f16", 40, 1, 64, 3, 50), ("f32", 9, 1, 24, 0, 33), ("bf16", 16, 2, 256, 30, 20)])
+def test_received_weights_of_many_tokens_have_one_order(ops, dtype, H, G, D, first, window):
+    """Portions of three rows, as runs and woven into one another: every slot's mass is the 64-bit sum, and has the same bits each time."""
+    lengths = [400, 290, 64]
+    rows = [r for r, n in enumerate(lengths) for _ in range(n - 40)] + [i % 3 for i in range(90)] + [-1, 2, 0]
+    at, slots = [0, 0, 0], []
+    for r in rows:
+        slots.append(at[r] if r >= 0 else 5)
+        at[max(r, 0)] += r >= 0
+    row, slot = i32(rows), i32(slots)
+    assert all(a <= n for a, n in zip(at, lengths))
+    c = Cache(lengths, 16, G, D, DT[dtype], 31)
+    q = c.normal(len(rows), H * D).to(c.dtype)
+    _check_attn(ops, c, q, row, slot, H, first, window, True, D ** -0.5)
+    k, v, table, qd = c.k.cuda(), c.v.cuda(), c.table.cuda(), q.cuda()
+    ws = torch.empty((ops.paged_attn_workspace_bytes(len(rows), H, D, c.table.shape[1] * 16),), dtype=torch.uint8, device="cuda")
+    seen = []
+    for _ in range(3):
+        mass, out = c.mass.cuda(), torch.empty_like(qd)
+        ops.paged_attn(qd, k, v, table, row.cuda(), slot.cuda(), out, D ** -0.5, first=first, window=window, mass=mass, workspace=ws)
+        seen.append(mass.cpu())
+    assert torch.equal(seen[0].view(torch.int32), seen[1].view(torch.int32)) and torch.equal(seen[0].view(torch.int32), seen[2].view(torch.int32))
+
+
 def test_attention_of_more_tokens_than_a_cta_keeps(ops):
     """A portion of several rows as single tokens, more of them than a CTA holds in shared memory, idle ones among them."""
     c = Cache([500, 150], 16, 2, 64, torch.bfloat16, 18)
