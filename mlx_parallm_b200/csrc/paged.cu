@@ -29,9 +29,10 @@ __device__ __forceinline__ float2 turn(int pos, float rate) {
 
 // Every head is split over 2^width_log2 lanes (the power of two that holds D / 8), 8 neighbouring values a lane: one to two 16-byte loads and stores, the
 // mean square by shuffles, a rotation partner from the lane that has it (pairs of halves) or from this one (neighbours).  A lane keeps its 8 angles and
-// walks over heads, four asked for ahead (two where a token's heads are shared out); a CTA holds 2^tpc_log2 tokens, each with (256 >> width_log2) >> tpc_log2 walkers, and where the tokens are few
-// gridDim.y CTAs share a token's heads.  fp32 from the read to the one rounding.  Bound by HBM from some hundred tokens on.  (A CTA per token, a warp per
-// head and an element per lane took 114 us for 6004 tokens of 64 + 16 heads.)
+// walks over heads, four asked for ahead (two where a token's heads are shared out: 52.5 us with two for 6004 tokens of 64 + 16 heads, 49.6 with four); a
+// CTA holds 2^tpc_log2 tokens, each with (256 >> width_log2) >> tpc_log2 walkers, and where the tokens are few gridDim.y CTAs share a token's heads.
+// fp32 from the read to the one rounding.  Bound by HBM from some hundred tokens on: 246 MB at 4.96 TB/s.  (A CTA per token, a warp per head and an
+// element per lane took 114 us.)
 template <typename T, typename TIN, int AHEAD>
 __global__ void __launch_bounds__(256, 3)
 paged_append_rows_kernel(TIN* qkv, int64_t ldq, T* q_out, T* kp, T* vp, float* mass, PageTable pt, const int32_t* t_row, const int32_t* t_slot,
@@ -404,10 +405,9 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
 // A CTA or a cluster of them per row, key head and kind (keys or values; the weights go with the keys) closes the kept slots up in rounds: a round's lines
 // go to shared memory, then (everybody has read that round) to their places.  One CTA keeps four rounds of 16 KB under way; a cluster, whose barriers cost 2
 // us, takes rounds of 80 KB (one row of 8 heads cut from 40001 to 5000 tokens, selection and all, in rounds of 16 KB 43 us, 80 KB 38, 160 KB and half the
-// CTAs per SM 46).  A slot never moves up and the kept ones
-// ascend, so no later round reads a place that an earlier one wrote.  Where lines come from and go to is looked up for MOVE_LINES of them at once: a look
-// at the list, then the table, then the line, round by round, made every round wait 5 us (16 rows of 8 heads cut from 4096 to 2048 tokens: 160 us).
-// Bound by HBM where rows and heads are many.
+// CTAs per SM 46).  A slot never moves up and the kept ones ascend, so no later round reads a place that an earlier one wrote.  Where lines come from and
+// go to is looked up for MOVE_LINES of them at once: a look at the list, then the table, then the line, round by round, made every round wait 5 us (16 rows
+// of 8 heads cut from 4096 to 2048 tokens: 160 us, now 69).  Bound by HBM where rows and heads are many.
 constexpr int MOVE_THREADS = 256, MOVE_STAGES = 4, MOVE_LINES = 2048, MOVE_MAX_CLUSTER = 8;
 constexpr int MOVE_UNITS_ONE = 4, MOVE_UNITS_CLUSTER = 20;        // 16-byte pieces of a thread in a round
 // shared memory of a CTA's share: the ring's stages that its rounds use, and the lists of its lines
@@ -529,7 +529,7 @@ static int cluster_of(int64_t clusters, int most, int per_sm) {
 
 // ------------------------------------------------------------------------------------------------ dense view
 // A CTA copies GATHER_BYTES' worth of slots of one key head's keys and values, whatever the pages: a thread asks for four pieces of either before it
-// stores the first.  (A CTA per page and one piece at a time: 18.4 us for 7777 tokens of 8 heads, 64 MB moved.)
+// stores the first: 12.7 us for 7777 tokens of 8 heads, 64 MB moved.  (A CTA per page and one piece at a time: 18.4.)
 constexpr int GATHER_THREADS = 256, GATHER_AHEAD = 4;
 
 __global__ void __launch_bounds__(GATHER_THREADS)
@@ -644,6 +644,7 @@ extern "C" int b200p_paged_select(const float* mass, const int32_t* table, const
   B200P_REQUIRE(lengths && kept, B200P_ERR_ARG, "null pointer");
   B200P_REQUIRE(keep > 0 && first >= 0 && recent >= 0 && (int64_t)first + recent <= keep, B200P_ERR_ARG, "%d first and %d recent of %d kept tokens", first,
                 recent, keep);
+  B200P_REQUIRE(keep <= 1 << 30, B200P_ERR_ARG, "%d kept tokens: a row has at most 2^30", keep);
   B200P_REQUIRE(rows < 65536, B200P_ERR_ARG, "too many rows");
   B200P_REQUIRE(G < 32768, B200P_ERR_ARG, "too many key heads");
   constexpr int SEL_ROOM = 48 * 1024;                             // keys: 192 KB
@@ -678,6 +679,7 @@ extern "C" int b200p_paged_compact(void* kpages, void* vpages, float* mass, cons
   const int rc = check_pages(kpages, vpages, pt, G, D, dtype);
   if (rc) return rc;
   B200P_REQUIRE(lengths && kept && keep > 0, B200P_ERR_ARG, "null pointer or nothing to keep");
+  B200P_REQUIRE(keep <= 1 << 30, B200P_ERR_ARG, "%d kept tokens: a row has at most 2^30", keep);
   B200P_REQUIRE(rows < 65536, B200P_ERR_ARG, "too many rows");
   const int chunks = D * (dtype == B200P_F32 ? 4 : 2) / 16;
   B200P_REQUIRE(G < 32768, B200P_ERR_ARG, "too many key heads");
@@ -695,7 +697,7 @@ extern "C" int b200p_paged_compact(void* kpages, void* vpages, float* mass, cons
   }
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_compact_kernel)");
   int S = cluster_of((int64_t)2 * G * rows, MOVE_MAX_CLUSTER, 2);
-  while (S > 1 && keep * chunks <= S * 1024) S /= 2;               // (at least 16 KB of lines each)
+  while (S > 1 && (int64_t)keep * chunks <= S * 1024) S /= 2;               // (at least 16 KB of lines each)
   const unsigned inv = (unsigned)(((1ull << 32) + chunks - 1) / chunks);
   const int stages = S > 1 ? 1 : MOVE_STAGES, units = S > 1 ? MOVE_UNITS_CLUSTER : MOVE_UNITS_ONE, lines = min(MOVE_THREADS * units / chunks, MOVE_LINES);
   const int rounds = (int)(((int64_t)keep + S * lines - 1) / (S * lines)), smem = move_ring(stages, units, rounds) + move_lists(rounds, lines) * 16;

@@ -825,6 +825,8 @@ paged_attn_join_kernel(const __grid_constant__ PagedAttn a, int rows_log2) {
 // slots, a thread per slot, and add up the weights that it received.  The heads' maxima and sums come from the parts again (a warp per head, a lane per
 // part), which needs no word from the join.  The slices of a row's first token in the call do so for all of the row's tokens and all of their
 // heads in turn, the others leave, so that a slot's weights are added by one thread in one order (unless rows share its page).
+// (Atomics of all tokens at once: 12 rows of 3333 tokens 33.4 us instead of 34.8, the last 32 of 2048 tokens 50 instead of 115; four tokens of a row at a
+// time 88, but 36.9 for the 12 rows.)
 template <typename T, int NQ, int ROWS>
 __global__ void __launch_bounds__(256)
 paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks, int warps) {
@@ -994,8 +996,8 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   const int per = a.H / a.G, rows_log2 = E::ROWS == 4 ? 2 : E::ROWS == 8 ? 3 : 4;
   const dim3 heads((unsigned)per, (unsigned)a.G, (unsigned)a.M);
   if (a.mass) {
-    // slices of the visible slots: as many as there are, but no more CTAs than fill the GPU
-    const int64_t slices = (a.cap + 255) / 256, fill = (6ll * sm_count() + (int64_t)a.M * items - 1) / ((int64_t)a.M * items);
+    // slices of the visible slots: as many as there are, but no more CTAs than fill the GPU (each row's first token has some that stay)
+    const int64_t stay = (int64_t)(a.M < a.pt.rows ? a.M : a.pt.rows) * items, slices = (a.cap + 255) / 256, fill = (6ll * sm_count() + stay - 1) / stay;
     const dim3 rest((unsigned)(E::ROWS + (slices < fill ? slices : fill)), (unsigned)items, (unsigned)a.M);
     launch_pdl(a.D <= 128 ? paged_attn_mass_kernel<T, 1, E::ROWS> : paged_attn_mass_kernel<T, 2, E::ROWS>, rest, 256, 0, st, a, per, blocks, (int)E::WARPS);
     B200P_LAUNCH_CHECK("paged_attn_mass_kernel");

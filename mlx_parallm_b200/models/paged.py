@@ -43,7 +43,7 @@ class PageBook:
             raise ValueError("window and first are counts")
         if self.keep and not (0 <= self.recent and self.first + self.recent <= self.keep < width * page):
             raise ValueError(f"a row of {width * page} tokens cannot be cut to {self.keep}, {self.first} first and {self.recent} recent ones among them")
-        self.observe = int(observe)            # a prompt's last tokens, whose weights count when its row is cut
+        self.observe = int(observe)            # the last tokens of each portion of a prompt, whose weights count when its row is cut
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros((rows,), dtype=torch.int32, device=device)
         self.positions = torch.zeros((rows,), dtype=torch.int32, device=device)

@@ -71,9 +71,9 @@ def test_pages_that_are_refused(call, bad):
     (attn, dict(q=0), ARG), (attn, dict(out=0), ARG), (attn, dict(k=0), ARG), (attn, dict(row=0), ARG), (attn, dict(slot=0), ARG), (attn, dict(M=-1), ARG),
     (attn, dict(M=65536), ARG), (attn, dict(first=-1), ARG), (attn, dict(window=-1), ARG), (attn, dict(flags=2), ARG), (attn, dict(q=OK + 2), ALIGN),
     (attn, dict(out=OK + 2), ALIGN), (attn, dict(k=OK + 2), ALIGN), (attn, dict(mass=OK, ws=0), ARG), (attn, dict(mass=OK, bytes=100), ARG),
-    (select, dict(mass=0), ARG), (select, dict(lengths=0), ARG), (select, dict(kept=0), ARG), (select, dict(keep=0), ARG), (select, dict(first=-1), ARG),
+    (select, dict(mass=0), ARG), (select, dict(lengths=0), ARG), (select, dict(kept=0), ARG), (select, dict(keep=0), ARG), (select, dict(keep=(1 << 30) + 1), ARG), (select, dict(first=-1), ARG),
     (select, dict(recent=-1), ARG), (select, dict(first=13), ARG), (select, dict(first=(1 << 31) - 1, recent=(1 << 31) - 1), ARG), (select, dict(rows=65536), ARG),
-    (compact, dict(k=0), ARG), (compact, dict(kept=0), ARG), (compact, dict(keep=0), ARG), (compact, dict(dtype=7), ARG), (compact, dict(v=OK + 8), ALIGN),
+    (compact, dict(k=0), ARG), (compact, dict(kept=0), ARG), (compact, dict(keep=0), ARG), (compact, dict(keep=(1 << 30) + 1), ARG), (compact, dict(dtype=7), ARG), (compact, dict(v=OK + 8), ALIGN),
     (gather, dict(row_of=0), ARG), (gather, dict(kc=0), ARG), (gather, dict(cap=0), ARG), (gather, dict(count=-1), ARG), (gather, dict(vc=OK + 4), ALIGN),
 ], ids=lambda x: getattr(x, "__name__", str(x)))
 def test_arguments_that_are_refused(call, bad, rc):
