@@ -27,51 +27,30 @@ __device__ __forceinline__ float2 turn(int pos, float rate) {
   return sc;
 }
 
-// Every head is split over 2^width_log2 lanes (the power of two that holds D / 8), 8 neighbouring values a lane: one to two 16-byte loads and stores, the
-// mean square by shuffles, a rotation partner from the lane that has it (pairs of halves) or from this one (neighbours).  A lane keeps its 8 angles and
-// walks over heads, four asked for ahead (two where a token's heads are shared out: 52.5 us with two for 6004 tokens of 64 + 16 heads, 49.6 with four); a
-// CTA holds 2^tpc_log2 tokens, each with (256 >> width_log2) >> tpc_log2 walkers, and where the tokens are few gridDim.y CTAs share a token's heads.
-// fp32 from the read to the one rounding.  Bound by HBM from some hundred tokens on: 246 MB at 4.96 TB/s.  (A CTA per token, a warp per head and an
-// element per lane took 114 us.)
-template <typename T, typename TIN, int AHEAD>
+// Every head is split over 2^width_log2 lanes (the power of two that holds D / 8), 8 neighbouring values a lane: one to two 16-byte loads and stores (8
+// bytes at a time, four values and the four that they turn with, took 102 us), a rotation partner from the lane that has it (pairs of halves) or from
+// this one (neighbours).  A lane keeps its angles and the norms' weights and walks over heads: without norms one after the other, four on their way (two where
+// the tokens are few); with them two at once, their mean squares by shuffles side by side.  A CTA holds 2^tpc_log2 tokens, each with (256 >> width_log2) >>
+// tpc_log2 walkers, and where the tokens are few gridDim.y CTAs share a token's heads.  fp32 from the read to the one rounding.
+// Bound by HBM from some hundred tokens on, with norms by the instructions: 6004 tokens of 64 + 16 heads of 128, 246 MB, 47.5 us (two ahead 52.5), with
+// norms 62.5 (four at once 66, one after the other 84); one token 2.6.  (A CTA per token, a warp per head and an element per lane took 114 us;
+// CTAs that take their tokens one after the other, so that what is read lies closer together, 73.)
+template <typename T, typename TIN, int AHEAD, bool PAIRS, bool NORM>
 __global__ void __launch_bounds__(256, 3)
 paged_append_rows_kernel(TIN* qkv, int64_t ldq, T* q_out, T* kp, T* vp, float* mass, PageTable pt, const int32_t* t_row, const int32_t* t_slot,
-                         const int32_t* t_pos, const T* qw, const T* kw, const float* rates, int n_rot, int pairs, float eps, int M, int H, int G, int D,
+                         const int32_t* t_pos, const T* qw, const T* kw, const float* rates, int n_rot, float eps, int M, int H, int G, int D,
                          int width_log2, int tpc_log2) {
   constexpr bool ACC_IN = !std::is_same<TIN, T>::value;
-  constexpr int IN = sizeof(TIN) * 8 / 16, OUT = sizeof(T) * 8 / 16;      // 16-byte pieces of 8 values
+  constexpr int IN = sizeof(TIN) * 8 / 16, OUT = sizeof(T) * 8 / 16, TURNS = PAIRS ? 4 : 8;      // 16-byte pieces of 8 values; angles
+  constexpr int GROUP = NORM ? AHEAD : 1;                         // heads worked on at once
   __shared__ float2 s_turn[8][128];
   const int tpc = 1 << tpc_log2, width = 1 << width_log2, token0 = blockIdx.x << tpc_log2;
-  pdl_wait();
-  for (int i = threadIdx.x; i < n_rot << tpc_log2; i += 256) {
-    const int k = i & (tpc - 1), pair = i >> tpc_log2;
-    if (token0 + k < M) s_turn[k][pair] = turn(t_pos[token0 + k], rates[pair]);
-  }
   const int c = threadIdx.x & (width - 1), slot = threadIdx.x >> width_log2;
   const int k = slot & (tpc - 1), t = min(token0 + k, M - 1), step = (256 >> width_log2) >> tpc_log2;
   const bool mine = token0 + k < M && c < D / 8;
+  pdl_wait();
   const int row = t_row[t], place = t_slot[t], heads = H + 2 * G;
   const bool live = row >= 0 && row < pt.rows;
-  int64_t id = -1;
-  if (live && place >= 0 && place < table_slots(pt)) id = page_id(pt, row, place / pt.page);
-  if (mine && c == 0 && slot < tpc && blockIdx.y == 0 && (row >= pt.rows || (live && id < 0))) atomicAdd(&g_paged_fault, 1u);
-  const int off = id < 0 ? 0 : place % pt.page;
-  __syncthreads();
-  // out = x * cs + partner * sn
-  float cs[8], sn[8];
-  int partner = threadIdx.x & 31;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int e = 8 * c + j;
-    cs[j] = 1.f;
-    sn[j] = 0.f;
-    if (e < 2 * n_rot) {
-      const float2 sc = s_turn[k][pairs ? e >> 1 : (e < n_rot ? e : e - n_rot)];
-      cs[j] = sc.y;
-      sn[j] = (pairs ? (e & 1) : e >= n_rot) ? sc.x : -sc.x;
-    }
-  }
-  if (!pairs && 8 * c < 2 * n_rot) partner += 8 * c < n_rot ? n_rot / 8 : -(n_rot / 8);
   TIN* src = qkv + (int64_t)t * ldq + 8 * c;
   const int first = (int)blockIdx.y * step + (slot >> tpc_log2), stride = step * gridDim.y;
   uint4 in[AHEAD][IN];
@@ -86,62 +65,119 @@ paged_append_rows_kernel(TIN* qkv, int64_t ldq, T* q_out, T* kp, T* vp, float* m
     }
   };
 #pragma unroll
-  for (int a = 0; a < AHEAD; ++a) fetch(in[a], first + a * stride);
+  for (int a = 0; a < AHEAD; ++a) fetch(in[a], first + a * stride);      // on their way while the angles are worked out
+  for (int i = threadIdx.x; i < n_rot << tpc_log2; i += 256) {
+    const int kk = i & (tpc - 1), pair = i >> tpc_log2;
+    if (token0 + kk < M) s_turn[kk][pair] = turn(t_pos[token0 + kk], rates[pair]);
+  }
+  int64_t id = -1;
+  if (live && place >= 0 && place < table_slots(pt)) id = page_id(pt, row, place / pt.page);
+  if (mine && c == 0 && slot < tpc && blockIdx.y == 0 && (row >= pt.rows || (live && id < 0))) atomicAdd(&g_paged_fault, 1u);
+  const int off = id < 0 ? 0 : place % pt.page;
+  uint4 weight[2][OUT];                                           // of queries and keys
+  if constexpr (NORM)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const T* w = i ? kw : qw;
+#pragma unroll
+      for (int n = 0; n < OUT; ++n)
+        if (w && c < D / 8) weight[i][n] = reinterpret_cast<const uint4*>(w + 8 * c)[n];
+    }
+  __syncthreads();
+  const float inv_D = 1.f / (float)D;
+  float cs[TURNS], sn[TURNS];                                     // halves: out = x * cs + partner * sn
+  const int partner = (threadIdx.x & 31) + (PAIRS || 8 * c >= 2 * n_rot ? 0 : 8 * c < n_rot ? n_rot / 8 : -(n_rot / 8));
+#pragma unroll
+  for (int j = 0; j < TURNS; ++j) {
+    const int e = TURNS * c + j;
+    const bool turns = e < (PAIRS ? n_rot : 2 * n_rot), second = !PAIRS && e >= n_rot;
+    const float2 sc = turns ? s_turn[k][second ? e - n_rot : e] : make_float2(0.f, 1.f);
+    cs[j] = sc.y, sn[j] = PAIRS || second ? sc.x : -sc.x;
+  }
 #pragma unroll 1
-  for (int base = 0; base < heads; base += AHEAD * stride) {      // the same number of turns for every lane of a warp
+  for (int base = first; base - first < heads; base += AHEAD * stride) {      // the same number of turns for every lane of a warp
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      const int head = base + first + a * stride;
-      const bool ok = mine && live && head < heads;
-      float x[8];
-      const TIN* v = reinterpret_cast<const TIN*>(in[a]);
+    for (int a0 = 0; a0 < AHEAD; a0 += GROUP) {
+      float x[GROUP][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = ok ? Tr<TIN>::to_f(v[j]) : 0.f;
-        if (ACC_IN) x[j] = Tr<T>::to_f(Tr<T>::from_f(x[j]));
+      for (int a = 0; a < GROUP; ++a) {
+        const int head = base + (a0 + a) * stride;
+        const bool ok = mine && live && head < heads;
+        const TIN* v = reinterpret_cast<const TIN*>(in[a0 + a]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[a][j] = ok ? Tr<TIN>::to_f(v[j]) : 0.f;
+          if (ACC_IN) x[a][j] = Tr<T>::to_f(Tr<T>::from_f(x[a][j]));
+        }
+        fetch(in[a0 + a], head + AHEAD * stride);
       }
-      fetch(in[a], head + AHEAD * stride);
-      if (qw || kw) {
-        float ss = 0.f;
+      if constexpr (NORM) {
+        float ss[GROUP];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
-        for (int o = 1; o < width; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const T* w = head < H ? qw : head < H + G ? kw : nullptr;
-        if (w && ok) {
-          const float inv = 1.f / sqrtf(ss / (float)D + eps);
-          uint4 wv[OUT];
+        for (int a = 0; a < GROUP; ++a) {
+          ss[a] = 0.f;
 #pragma unroll
-          for (int i = 0; i < OUT; ++i) wv[i] = reinterpret_cast<const uint4*>(w + 8 * c)[i];
-          const T* wf = reinterpret_cast<const T*>(wv);
+          for (int j = 0; j < 8; ++j) ss[a] += x[a][j] * x[a][j];
+        }
+        for (int o = 1; o < width; o <<= 1)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] *= inv * Tr<T>::to_f(wf[j]);
+          for (int a = 0; a < GROUP; ++a) ss[a] += __shfl_xor_sync(0xffffffffu, ss[a], o);
+#pragma unroll
+        for (int a = 0; a < GROUP; ++a) {
+          const int head = base + (a0 + a) * stride;
+          const bool queries = head < H;
+          if (head < H + G && (queries ? qw : kw)) {
+            const float inv = rsqrtf(fmaf(ss[a], inv_D, eps));
+            uint4 w8[OUT];
+#pragma unroll
+            for (int n = 0; n < OUT; ++n) w8[n] = queries ? weight[0][n] : weight[1][n];
+            const T* w = reinterpret_cast<const T*>(w8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[a][j] *= inv * Tr<T>::to_f(w[j]);
+          }
         }
       }
-      if (n_rot) {
-        float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = pairs ? x[j ^ 1] : __shfl_sync(0xffffffffu, x[j], partner);
-        if (head < H + G)
+      for (int a = 0; a < GROUP; ++a) {
+        const int head = base + (a0 + a) * stride;
+        if (n_rot) {
+          const bool turned = head < H + G && 8 * c < 2 * n_rot;
+          if constexpr (PAIRS) {
+            if (turned)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = x[j] * cs[j] + y[j] * sn[j];
+              for (int j = 0; j < 4; ++j)
+                if (4 * c + j < n_rot) {
+                  const float y0 = x[a][2 * j], y1 = x[a][2 * j + 1];
+                  x[a][2 * j] = y0 * cs[j] - y1 * sn[j];
+                  x[a][2 * j + 1] = y0 * sn[j] + y1 * cs[j];
+                }
+          } else {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = __shfl_sync(0xffffffffu, x[a][j], partner);
+            if (turned)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[a][j] = x[a][j] * cs[j] + y[j] * sn[j];
+          }
+        }
+        if (!(mine && live && head < heads)) continue;
+        T* dst;
+        if (head < H) {
+          dst = q_out + ((int64_t)t * H + head) * D;
+        } else {
+          if (id < 0) continue;
+          const int64_t at = (id * G + (head < H + G ? head - H : head - H - G)) * pt.page + off;
+          dst = (head < H + G ? kp : vp) + at * D;
+          if (mass && head < H + G && c == 0) mass[at] = 0.f;
+        }
+        uint4* to = reinterpret_cast<uint4*>(dst + 8 * c);
+        if constexpr (sizeof(T) == 2) {
+          *to = make_uint4(pack2<T>(x[a][0], x[a][1]), pack2<T>(x[a][2], x[a][3]), pack2<T>(x[a][4], x[a][5]), pack2<T>(x[a][6], x[a][7]));
+        } else {
+          *reinterpret_cast<float4*>(to) = make_float4(x[a][0], x[a][1], x[a][2], x[a][3]);
+          *reinterpret_cast<float4*>(to + 1) = make_float4(x[a][4], x[a][5], x[a][6], x[a][7]);
+        }
       }
-      if (!ok) continue;
-      T* dst;
-      if (head < H) {
-        dst = q_out + ((int64_t)t * H + head) * D;
-      } else {
-        if (id < 0) continue;
-        const int g = head < H + G ? head - H : head - H - G;
-        const int64_t at = (id * G + g) * pt.page + off;
-        dst = (head < H + G ? kp : vp) + at * D;
-        if (mass && head < H + G && c == 0) mass[at] = 0.f;
-      }
-      uint4 out[OUT];
-      T* f = reinterpret_cast<T*>(out);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = Tr<T>::from_f(x[j]);
-#pragma unroll
-      for (int i = 0; i < OUT; ++i) reinterpret_cast<uint4*>(dst + 8 * c)[i] = out[i];
     }
   }
 }
@@ -614,8 +650,15 @@ extern "C" int b200p_paged_append(void* qkv, int64_t ldq, void* q_out, void* kpa
     auto go = [&](auto t, auto in) {
       using T = decltype(t);
       using TIN = decltype(in);
-      launch_pdl(lg > 0 ? paged_append_rows_kernel<T, TIN, 4> : paged_append_rows_kernel<T, TIN, 2>, grid, 256, 0, st, (TIN*)qkv, ldq, (T*)q_out, (T*)kpages,
-                 (T*)vpages, mass, pt, t_row, t_slot, t_pos, (const T*)q_norm_w, (const T*)k_norm_w, rates, n_rot, pairs, eps, (int)M, H, G, D, width_log2, lg);
+      auto pick = [&](auto pairs) {
+        constexpr bool PAIRS = decltype(pairs)::value;
+        return q_norm_w || k_norm_w ? paged_append_rows_kernel<T, TIN, 2, PAIRS, true>
+               : lg > 0             ? paged_append_rows_kernel<T, TIN, 4, PAIRS, false>
+                                    : paged_append_rows_kernel<T, TIN, 2, PAIRS, false>;
+      };
+      auto kern = pairs ? pick(std::true_type()) : pick(std::false_type());
+      launch_pdl(kern, grid, 256, 0, st, (TIN*)qkv, ldq, (T*)q_out, (T*)kpages, (T*)vpages, mass, pt, t_row, t_slot, t_pos, (const T*)q_norm_w,
+                 (const T*)k_norm_w, rates, n_rot, eps, (int)M, H, G, D, width_log2, lg);
     };
     if (qkv_f32) {
       B200P_DISPATCH_DTYPE(dtype, T, (go(T(), float())));
