@@ -77,6 +77,11 @@ APPEND = [
     ("f16", 32, 8, 128, 64, 0, 0, "qk", False, [600], [100], 0, False),
     ("bf16", 64, 8, 128, 128, 64, 0, "", False, [700, 1, 333], [0, 12, 128], 0, True),
     ("f32", 3, 1, 8, 16, 4, 1, "qk", False, [20], [0], 0, True),
+    ("bf16", 16, 8, 128, 16, 64, 0, "qk", False, [650, 0, 31], [3, 8, 100], 0, True),      # prompts: norms, neighbours, an accumulation buffer
+    ("f16", 9, 3, 64, 64, 30, 1, "", False, [1203], [60], 5, True),
+    ("bf16", 16, 4, 96, 32, 24, 1, "k", True, [601, 20], [0, 31], 0, True),
+    ("f16", 7, 7, 72, 16, 32, 0, "q", True, [640], [1], 0, False),
+    ("f32", 6, 2, 256, 16, 128, 0, "qk", False, [600], [0], 0, True),
 ]
 
 
