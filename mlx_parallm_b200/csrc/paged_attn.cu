@@ -722,7 +722,8 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
             acc.x += y.x * f[w]; acc.y += y.y * f[w]; acc.z += y.z * f[w]; acc.w += y.w * f[w];
           }
           if (!cut)
-            store_row4<T>(reinterpret_cast<T*>(a.out) + ((int64_t)head + row) * D, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv), a.out_perm);
+            store_row4<T>(reinterpret_cast<T*>(a.out) + ((int64_t)head + row) * D, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv),
+                          a.out_perm);
           else
             *reinterpret_cast<float4*>(rec + row * (D + 4) + 4 + d) = acc;
         }
@@ -743,30 +744,21 @@ __device__ __forceinline__ const float* part_at(const PagedAttn& a, unsigned c0,
   return a.rec + (((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * rows + row) * (a.D + 4);
 }
 
-// A CTA per token and query head joins the parts where the item was cut: its warps take them in turn, then become one.  Few instructions: a launch
-// this short waits for its code more than for its data.  Eight warps where the CTAs are few (one row of 1000 tokens of 32 heads, both launches, us, four /
-// eight warps: 7.8 / 7.4), four where they are many (64 rows of 40 heads 25.2 / 26.4).  PJ_AHEAD parts of a warp on their way at once: four for the few,
-// which have long lists (one key head over 60000 tokens 20.0 with one, 17.9 with three, 17.2 with four, 16.5 with eight, but one row of 1000 then 7.3 ->
-// 7.5), one for the many (64 rows of 40 heads 25.2, with four 26.1).
-template <typename T, int NQ, int PJ_WARPS, int PJ_AHEAD>  // 128 dimensions of a warp's lanes, NQ times
-__device__ __forceinline__ void join_parts(const PagedAttn& a, int t, int64_t line, int row, int64_t head, int block_rows) {
-  __shared__ float2 s_ml[PJ_WARPS];
-  __shared__ float4 s_o[PJ_WARPS][32 * NQ];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int token_row = a.t_row[t];
-  const uint2 parts = a.parts[line];
-  if (token_row < 0 || token_row >= a.pt.rows || parts.y < 2) return;
-  float M = -INFINITY, L = 0.f;
-  float4 acc[NQ];
+// A warp's share of an item's parts, from i_first on: their maximum, sum and outputs, 128 dimensions of its lanes NQ times.
+template <int NQ, int PJ_AHEAD>
+__device__ __forceinline__ void sum_parts(const PagedAttn& a, uint2 parts, int row, int block_rows, unsigned i_first, unsigned i_step, float& M, float& L,
+                                          float4 (&acc)[NQ]) {
+  const int lane = threadIdx.x & 31;
+  M = -INFINITY, L = 0.f;
 #pragma unroll
   for (int x = 0; x < NQ; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-  for (unsigned i0 = warp; i0 < parts.y; i0 += PJ_AHEAD * PJ_WARPS) {
+  for (unsigned i0 = i_first; i0 < parts.y; i0 += PJ_AHEAD * i_step) {
     float2 ml[PJ_AHEAD];
     float4 y[PJ_AHEAD][NQ];
 #pragma unroll
     for (int u = 0; u < PJ_AHEAD; ++u) {
-      const unsigned i = i0 + u * PJ_WARPS;
+      const unsigned i = i0 + u * i_step;
       const bool in = i < parts.y;
       const float* p = part_at(a, parts.x, i, block_rows, row);
       ml[u] = in ? *reinterpret_cast<const float2*>(p) : make_float2(-INFINITY, 0.f);
@@ -790,6 +782,24 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, int t, int64_t li
       for (int x = 0; x < NQ; ++x) acc[x].x += y[u][x].x * w, acc[x].y += y[u][x].y * w, acc[x].z += y[u][x].z * w, acc[x].w += y[u][x].w * w;
     }
   }
+}
+
+// A CTA per token and query head joins the parts where the item was cut: its warps take them in turn, then become one.  Few instructions: a launch
+// this short waits for its code more than for its data.  Eight warps where the CTAs are few (one row of 1000 tokens of 32 heads, both launches, us, four /
+// eight warps: 7.8 / 7.4), four where they are many (64 rows of 40 heads 25.2 / 26.4).  PJ_AHEAD parts of a warp on their way at once: four for the few,
+// which have long lists (one key head over 60000 tokens 20.0 with one, 17.9 with three, 17.2 with four, 16.5 with eight, but one row of 1000 then 7.3 ->
+// 7.5), one for the many (64 rows of 40 heads 25.2, with four 26.1).
+template <typename T, int NQ, int PJ_WARPS, int PJ_AHEAD>
+__device__ __forceinline__ void join_parts(const PagedAttn& a, int t, int64_t line, int row, int64_t head, int block_rows) {
+  __shared__ float2 s_ml[PJ_WARPS];
+  __shared__ float4 s_o[PJ_WARPS][32 * NQ];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int token_row = a.t_row[t];
+  const uint2 parts = a.parts[line];
+  if (token_row < 0 || token_row >= a.pt.rows || parts.y < 2) return;
+  float M, L;
+  float4 acc[NQ];
+  sum_parts<NQ, PJ_AHEAD>(a, parts, row, block_rows, warp, PJ_WARPS, M, L, acc);
   if (lane == 0) s_ml[warp] = make_float2(M, L);
 #pragma unroll
   for (int x = 0; x < NQ; ++x) s_o[warp][lane + 32 * x] = acc[x];
@@ -813,38 +823,62 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, int t, int64_t li
   store_row4<T>(reinterpret_cast<T*>(a.out) + head * a.D, d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), a.out_perm);
 }
 
+// The same by one warp.
+template <typename T, int NQ>
+__device__ __forceinline__ void join_alone(const PagedAttn& a, int t, int64_t line, int row, int64_t head, int block_rows) {
+  const int token_row = a.t_row[t], lane = threadIdx.x & 31;
+  const uint2 parts = a.parts[line];
+  if (token_row < 0 || token_row >= a.pt.rows || parts.y < 2) return;
+  float M, L;
+  float4 acc[NQ];
+  sum_parts<NQ, 4>(a, parts, row, block_rows, 0, 1, M, L, acc);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const int d = 4 * lane + 128 * x;
+    if (d < a.D)
+      store_row4<T>(reinterpret_cast<T*>(a.out) + head * a.D, d, make_float4(acc[x].x * inv, acc[x].y * inv, acc[x].z * inv, acc[x].w * inv), a.out_perm);
+  }
+}
+
 template <typename T, int NQ, int PJ_WARPS>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
 paged_attn_join_kernel(const __grid_constant__ PagedAttn a, int rows_log2) {
   const int r = blockIdx.x, g = blockIdx.y, t = blockIdx.z, rows = 1 << rows_log2, blocks = (gridDim.x + rows - 1) >> rows_log2;
   pdl_wait();
-  join_parts<T, NQ, PJ_WARPS, PJ_WARPS == 8 ? 4 : 1>(a, t, ((int64_t)t * a.G + g) * blocks + (r >> rows_log2), r & (rows - 1), ((int64_t)t * a.G + g) * gridDim.x + r, rows);
+  const int64_t tg = (int64_t)t * a.G + g;
+  join_parts<T, NQ, PJ_WARPS, PJ_WARPS == 8 ? 4 : 1>(a, t, tg * blocks + (r >> rows_log2), r & (rows - 1), tg * gridDim.x + r, rows);
 }
 
-// With a mass, one launch for both: the first ROWS CTAs (x) of an item (y) of a token (z) join its heads, the others are slices of the row's visible
-// slots, a thread per slot, and add up the weights that it received.  The heads' maxima and sums come from the parts again (a warp per head, a lane per
-// part), which needs no word from the join.  The slices of a row's first token in the call do so for all of the row's tokens and all of their
-// heads in turn, the others leave, so that a slot's weights are added by one thread in one order (unless rows share its page).
-// (Atomics of all tokens at once: 12 rows of 3333 tokens 33.4 us instead of 34.8, the last 32 of 2048 tokens 50 instead of 115; four tokens of a row at a
-// time 88, but 36.9 for the 12 rows.)
+// With a mass, one launch for both: the first CTAs (x) of an item (y) of a token (z) join its heads, a CTA each where the items are few, else one with
+// a warp per head; the others are slices of the row's visible slots, a thread per slot, and add up the weights that it received.  The heads' maxima and
+// sums come from the parts again (a warp per head, a lane per part), which needs no word from the join.  The slices of a row's first token in the call do so
+// for all of the row's tokens and all of their heads in turn, the others leave, so that a slot's weights are added by one thread in one order (unless rows
+// share its page).
+// 12 rows of 3333 tokens, 64 heads: 26.1 us for the launch before, 5.8 for this one (9.0 with a CTA for every head).  (Atomics of all tokens at once took 1.4
+// less there, and 50 for the last 32 of 2048 tokens instead of 115; four tokens of a row at a time 88 there, but 2 more for the 12 rows.)
 template <typename T, int NQ, int ROWS>
 __global__ void __launch_bounds__(256)
-paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks, int warps) {
+paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks, int joiners) {
   __shared__ float2 s_stat[2][ROWS];
   __shared__ int s_from[8];
   __shared__ int2 s_seen[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, items = a.G * blocks;
   const int t = blockIdx.z, item = blockIdx.y, g = blocks == 1 ? item : item / blocks, block = item - g * blocks;
-  if (blockIdx.x < ROWS) {
+  if ((int)blockIdx.x < joiners) {
     const int r0 = block * ROWS;
     pdl_wait();
-    if (r0 + (int)blockIdx.x < per)
+    if (joiners == 1) {
+#pragma unroll 1
+      for (int r = warp; r < min(ROWS, per - r0); r += 8)
+        join_alone<T, NQ>(a, t, (int64_t)t * items + item, r, (int64_t)t * a.H + (int64_t)g * per + r0 + r, ROWS);
+    } else if (r0 + (int)blockIdx.x < per)
       join_parts<T, NQ, 8, 1>(a, t, (int64_t)t * items + item, blockIdx.x, (int64_t)t * a.H + (int64_t)g * per + r0 + blockIdx.x, ROWS);
     return;
   }
   if (block) return;
   // The tokens' rows and slots are older than the launch before this one, which let this one begin behind its own wait.
-  const int slice = blockIdx.x - ROWS, slices = gridDim.x - ROWS, row = a.t_row[t];
+  const int slice = blockIdx.x - joiners, slices = gridDim.x - joiners, row = a.t_row[t];
   if (row < 0 || row >= a.pt.rows) return;
   bool before = false;                                            // a token of this row stands before this one: most often close by
   unsigned first32 = 0;                                           // which of the next tokens, this warp's 32 of 256, are of this row
@@ -995,15 +1029,17 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   using T = typename E::T;
   const int per = a.H / a.G, rows_log2 = E::ROWS == 4 ? 2 : E::ROWS == 8 ? 3 : 4;
   const dim3 heads((unsigned)per, (unsigned)a.G, (unsigned)a.M);
+  const bool few = (int64_t)a.M * a.H <= 4 * sm_count();             // CTAs of the join
   if (a.mass) {
     // slices of the visible slots: as many as there are, but no more CTAs than fill the GPU (each row's first token has some that stay)
     const int64_t stay = (int64_t)(a.M < a.pt.rows ? a.M : a.pt.rows) * items, slices = (a.cap + 255) / 256, fill = (6ll * sm_count() + stay - 1) / stay;
-    const dim3 rest((unsigned)(E::ROWS + (slices < fill ? slices : fill)), (unsigned)items, (unsigned)a.M);
-    launch_pdl(a.D <= 128 ? paged_attn_mass_kernel<T, 1, E::ROWS> : paged_attn_mass_kernel<T, 2, E::ROWS>, rest, 256, 0, st, a, per, blocks, (int)E::WARPS);
+    const int joiners = few ? E::ROWS : 1;
+    const dim3 rest((unsigned)(joiners + (slices < fill ? slices : fill)), (unsigned)items, (unsigned)a.M);
+    launch_pdl(a.D <= 128 ? paged_attn_mass_kernel<T, 1, E::ROWS> : paged_attn_mass_kernel<T, 2, E::ROWS>, rest, 256, 0, st, a, per, blocks, joiners);
     B200P_LAUNCH_CHECK("paged_attn_mass_kernel");
     return B200P_OK;
   }
-  if ((int64_t)a.M * a.H <= 4 * sm_count())
+  if (few)
     launch_pdl(a.D <= 128 ? paged_attn_join_kernel<T, 1, 8> : paged_attn_join_kernel<T, 2, 8>, heads, 8 * 32, 0, st, a, rows_log2);
   else
     launch_pdl(a.D <= 128 ? paged_attn_join_kernel<T, 1, 4> : paged_attn_join_kernel<T, 2, 4>, heads, 4 * 32, 0, st, a, rows_log2);
