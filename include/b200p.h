@@ -645,9 +645,9 @@ int b200p_paged_append(void* qkv, int64_t ldq, void* q_out, void* kpages, void* 
                        int width, int dtype, int qkv_f32, void* stream);
 /* Step 2: attention of M tokens, each over its own row: token t at slot s sees the slots j < n = s + 1 with j < first or j >= n - window
  * (window 0: every j < n); fp32 softmax of q . k_j * scale; query head h reads key head h / (H / G).  q `dtype` [M, H D]; out `dtype` [M, H D]
- * (flags = B200P_OUT_PERM8: PERM8 order).  A token that sees nothing, or nothing but scores of minus infinity, gets zeros; an infinite value that it
- * sees makes its outputs infinite or NaN.  mass (NULL: none): every visible slot's mass grows by
- * the weights that the query heads of its key head gave it, token by token in the call's order (tokens of different rows that share a page: in
+ * (flags = B200P_OUT_PERM8: PERM8 order).  Nothing is written for a token whose row is behind the table.  A token that sees nothing, or nothing but
+ * scores of minus infinity, gets zeros; an infinite value that it sees makes its outputs infinite or NaN.  mass (NULL: none): every visible slot's mass
+ * grows by the weights that the query heads of its key head gave it, token by token in the call's order (tokens of different rows that share a page: in
  * no fixed order).
  * Hidden keys and values are not read.  workspace: b200p_paged_attn_workspace_bytes(M, H, D, keys), keys = width * page with a mass,
  * 0 without, aligned to 256 bytes; it needs no initial state and serves one stream at a time. */

@@ -268,6 +268,17 @@ def test_attention_pages_that_do_not_exist(ops, dtype, D):
         assert ops.paged_fault_count(reset=True) > 0
 
 
+def test_attention_rows_behind_the_table(ops):
+    """Their tokens are left as idle ones are, and counted, however many tokens the call has."""
+    c = Cache([50, 20], 16, 2, 64, torch.float16, 32)
+    for n in (3, 700):
+        row, slot = i32([0, 2, 1] + [-1] * (n - 3)), i32([49, 5, 19] + [0] * (n - 3))
+        q = c.normal(n, 8 * 64).to(c.dtype)
+        for mass in (False, True):
+            _check_attn(ops, c, q, row, slot, 8, 0, 0, mass, 0.2)
+            assert ops.paged_fault_count(reset=True) == 1
+
+
 def test_attention_rows_share_pages(ops):
     """A common beginning: two rows and two tokens of one of them add their weights to the same places."""
     c = Cache([200, 90, 64], 16, 2, 128, torch.bfloat16, 14)
