@@ -367,7 +367,7 @@ class DecoderModel:
         """A cache in pages (models/paged.py) for ``batch_size`` rows of up to ``max_tokens`` tokens, drawn from ``pages`` pages of ``page`` tokens
         (None: as many as all rows need).  ``window`` > 0: a token sees the last ``window`` tokens and the ``first`` first ones.  ``keep`` > 0: a row
         that is full is cut to ``keep`` tokens, the ``first`` first, the ``recent`` newest (None: half of the others) and the most attended
-        ones; the weights of decode steps and of the last ``observe`` tokens of each prompt portion count."""
+        ones; the weights of decode steps and of a prompt's last ``observe`` tokens count."""
         if self.device is None:
             raise RuntimeError("load the model's weights first")
         book = PageBook(batch_size, max_tokens, self.device, page, pages, window, first, keep, recent, observe)
@@ -534,12 +534,15 @@ class DecoderModel:
             cache = self.make_cache(B, step=max(L, 1))
         prepare_cache(cache, B, L, self.dtype, self.device)
         Lc = max(1, min(L, MAX_TOKENS_PER_FORWARD // B))
+        book = cache[0].book if isinstance(cache[0], PagedLayer) else None
         outs = []
         for l0 in range(0, L, Lc):
             l1 = min(L, l0 + Lc)
             n = l1 - l0
             a = self._arena(B * n, B)
             chunk = ids[:, l0:l1].contiguous().view(-1)
+            if book is not None:
+                book.behind = L - l1
             self._layers_forward(chunk, B, n, cache, a)
             advance_cache(cache, n)
             src = a["x"] if a.get("x_final") else a["h"]      # row-sharded TP: x already holds final_norm(h) on every rank

@@ -43,7 +43,8 @@ class PageBook:
             raise ValueError("window and first are counts")
         if self.keep and not (0 <= self.recent and self.first + self.recent <= self.keep < width * page):
             raise ValueError(f"a row of {width * page} tokens cannot be cut to {self.keep}, {self.first} first and {self.recent} recent ones among them")
-        self.observe = int(observe)            # the last tokens of each portion of a prompt, whose weights count when its row is cut
+        self.observe = int(observe)            # a prompt's last tokens, whose weights count when its row is cut
+        self.behind = 0                        # tokens of the prompt behind the portion that is being read
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros((rows,), dtype=torch.int32, device=device)
         self.positions = torch.zeros((rows,), dtype=torch.int32, device=device)
@@ -155,6 +156,7 @@ class PagedLayer(RowState):
         if batch_size is not None and batch_size != self.batch_size:
             raise ValueError("a paged cache keeps the batch size it was made with")
         self.book.evicted = [0] * self.batch_size
+        self.book.behind = 0
         super().reset(None)
         self.book.positions.zero_()
         self.book.shrink([0] * self.batch_size)
@@ -200,9 +202,10 @@ class PagedLayer(RowState):
         ops.paged_append(qkv, q, self.kpages, self.vpages, book.table, row, slot, pos, heads, rates=rates, q_norm_w=q_norm, k_norm_w=k_norm, eps=eps,
                          mass=self.mass)
         keys = book.max_tokens if self.mass is not None else 0
+        observed = min(L, max(0, book.observe - book.behind))
         if L == 1:
-            ops.paged_attn(q, self.kpages, self.vpages, book.table, row, slot, out, scale, first=book.first, window=book.window, mass=self.mass,
-                           workspace=book.workspace(B, heads, D, keys), out_perm=out_perm)
+            ops.paged_attn(q, self.kpages, self.vpages, book.table, row, slot, out, scale, first=book.first, window=book.window,
+                           mass=self.mass if observed or not book.behind else None, workspace=book.workspace(B, heads, D, keys), out_perm=out_perm)
             return
         if book.window:
             ops.paged_attn(q, self.kpages, self.vpages, book.table, row, slot, out, scale, first=book.first, window=book.window,
@@ -212,8 +215,8 @@ class PagedLayer(RowState):
             dense = book.scratch("dense", (2, B, self.n_kv_heads, cap, D), self.kpages.dtype)
             ops.paged_gather(self.kpages, self.vpages, book.table, book.row_index, book.lengths, dense[0], dense[1], extra=L)
             ops.attn(q, dense[0], dense[1], book.lengths, out, B, L, heads, self.n_kv_heads, D, scale, workspace=attn_workspace, out_perm=out_perm)
-        if self.mass is not None and book.observe > 0:                  # what the prompt's last tokens look at
-            n = min(L, book.observe)
+        if self.mass is not None and observed > 0:                      # what the prompt's last tokens look at
+            n = observed
             last = lambda t: t.view(B, L, -1)[:, L - n:].reshape(B * n, -1).contiguous()
             ql = last(q)
             ops.paged_attn(ql, self.kpages, self.vpages, book.table, last(row).view(-1), last(slot).view(-1), torch.empty_like(ql), scale, first=book.first,

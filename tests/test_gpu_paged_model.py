@@ -55,6 +55,30 @@ def test_prompt_in_portions(monkeypatch):
     assert rel_err(whole.cpu().numpy(), exp) < LOGIT_TOL and rel_err(parts.cpu().numpy(), exp) < LOGIT_TOL
 
 
+@pytest.mark.parametrize("observe", [0, 7, 60, 1000])
+def test_weights_of_a_prompts_last_tokens(monkeypatch, observe):
+    """The last ``observe`` tokens of a prompt give every head's weight of one each, and no others, in however many portions it is read."""
+    from mlx_parallm_b200.models import _transformer
+    cfg, om, gm = make_pair("small-llama", dtype="float16")
+    ids = torch.from_numpy(prompts_for(cfg, 2, 150))
+    seen = []
+    for at_once in (8192, 100, 46):
+        monkeypatch.setattr(_transformer, "MAX_TOKENS_PER_FORWARD", at_once)
+        cache = gm.make_paged_cache(2, 200, page=48, keep=100, observe=observe)
+        gm(ids, cache=cache, last_only=True)
+        for c in cache:
+            pages = c.book.table.cpu()
+            mass = torch.stack([torch.cat([c.mass[p].cpu() for p in row if p >= 0], 1)[:, :150] for row in pages])
+            # a row of 150 weights sums to 1 to about 150 roundings of 2^-24
+            exp = min(observe, 150) * c.n_heads
+            assert bool(((mass.sum((1, 2)) - exp).abs() <= 1e-4 * exp).all()), (at_once, mass.sum((1, 2)), exp)
+            seen.append(mass)
+        gm(ids[:, :1], cache=cache, last_only=True)             # and a step's token its own
+        left = torch.stack([torch.cat([cache[0].mass[p].cpu() for p in row if p >= 0], 1)[:, :151] for row in cache[0].book.table.cpu()]).sum((1, 2))
+        exp = (min(observe, 150) + 1) * cache[0].n_heads
+        assert bool(((left - exp).abs() <= 1e-4 * exp).all())
+
+
 def test_window_that_hides_nothing_and_one_that_does():
     cfg, om, gm = make_pair("small-llama", dtype="float16")
     ids = prompts_for(cfg, 2, 60)
