@@ -75,17 +75,17 @@ struct PagedAttn {
   float* stat;         // [M, H, 2] maximum and 1 / sum of the heads that lie in one share (with a mass)
   float* scores;       // [M, items, cap, pitch] log2-scaled scores (with a mass)
   uint64_t inv_tpp;    // 2^36 / (tiles of a page, 256 at most), rounded up: tile * inv_tpp >> 36 is the page's index for any tile below 2^26
-  int tpp;
+  int tpp, last;       // tiles of a page; CTAs for small shares at the line's end
   int cap, pitch;      // visible slots a token can have, in whole tiles; heads of a line of scores, a power of two
 };
 
 // The work is cut evenly however unequal the rows are: every token's visible tiles are counted in units of one tile per warp, the units of all
-// (token, key head, block of query heads) items are laid end to end, and each CTA takes an equal share of that line.  An item that lies in one share is
+// (token, key head, block of query heads) items are laid end to end, and each resident CTA takes an equal share of that line.  An item in one share is
 // finished there; of one that is cut every share leaves a part, and a second launch joins them.  (One CTA per item left the GPU idle behind the longest
 // rows: 64 rows of 130 to 500 tokens took 108 us, 16 of 8192 940.  Joining in the CTA whose part comes last, by counters, cost a row of 1000 tokens 3.7 us
 // of fences and atomics in a row; the second launch costs it less.  SMs differ by a quarter in what they get of the memory's bandwidth, so that of 16 rows of
-// 8192 tokens the first CTAs are done after 63 us and the last after 90; small shares for whoever comes first evened that out but cost more in parts and
-// in the count of those taken: 106 us in all against 95.)
+// 8192 tokens the first CTAs are done after 63 us and the last after 90; a counter of small shares for whoever comes first evened that out but cost more than
+// it gave: 106 us in all against 95.)
 struct Token {
   int row, units;
   Span span;
@@ -104,15 +104,33 @@ struct Token {
 
 constexpr int PA_TOKENS = 512;         // up to so many tokens a CTA keeps all of them in shared memory
 
+// Where every CTA's share is long (PA_LAST_UNITS units, some 50 us in all) it gives a part away: PA_LAST_PERCENT of the line, its end, is cut into small
+// shares for 3/4 as many more CTAs, which the hardware starts where the first ones have ended.  (16 rows of 8192 tokens 95.1 -> 90.0 us, 128 of 1000
+// 96.1 -> 90.9, 64 of 1000 52.4 -> 51.8; 64 of 500, below the bound, 31.3, and 33.5 with it.  CTAs that find no share, where the table has room for long rows
+// and the rows are short: 0.3 us at most.)
+constexpr int PA_LAST_UNITS = 24, PA_LAST_PERCENT = 12;
+__host__ __device__ inline int last_ctas(int ctas) { return ctas * 3 / 4; }
+
 struct Shares {
-  unsigned n, q, r;                    // how many; the first r have q + 1 units, the others q
+  unsigned n, n1, u1, q, r, q2, r2;    // how many; the first n1 lie in [0, u1): r of q + 1 units, then of q; the small ones alike behind it
   // of U units that belong to so many items: a warp of the join reads its parts one after the other, 128 of an item are enough
-  __device__ Shares(unsigned U, unsigned items, unsigned ctas) : n(min(min(U, ctas), items < 65536 ? 128 * items : ctas)) {
-    q = n ? U / n : 1;
-    r = U - q * n;
+  __device__ Shares(unsigned U, unsigned items, unsigned ctas, unsigned last)
+      : n(min(min(U, ctas), items < 65536 ? 128 * items : ctas)), n1(n), u1(U), q2(1), r2(0) {
+    if (last && n == ctas && U >= PA_LAST_UNITS * ctas) {
+      u1 = U - U / 100 * PA_LAST_PERCENT;
+      n += last;
+      q2 = (U - u1) / last;
+      r2 = U - u1 - q2 * last;
+    }
+    q = n1 ? u1 / n1 : 1;
+    r = u1 - q * n1;
   }
-  __device__ unsigned begin(unsigned c) const { return c * q + min(c, r); }
-  __device__ unsigned of(unsigned u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
+  __device__ unsigned begin(unsigned c) const { return c <= n1 ? c * q + min(c, r) : u1 + (c - n1) * q2 + min(c - n1, r2); }
+  __device__ unsigned of(unsigned u) const {
+    const bool small = u >= u1;
+    const unsigned v = small ? u - u1 : u, size = small ? q2 : q, more = small ? r2 : r;
+    return (small ? n1 : 0) + (v < more * (size + 1) ? v / (size + 1) : more + (v - more * (size + 1)) / size);
+  }
 };
 
 // The tokens of a call of up to PA_TOKENS: their rows and where their slots end.  (Under a full stream of keys a look at global memory
@@ -524,7 +542,7 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
     n_items += s.live[w] * items;
   }
   pdl_launch_dependents();                                        // (the join waits for this launch's end; until then it has no room anyway)
-  const Shares sh(U, n_items, gridDim.x);
+  const Shares sh(U, n_items, gridDim.x - a.last, a.last);
   if (blockIdx.x >= sh.n) return;
   const unsigned ub = sh.begin(blockIdx.x);
 #pragma unroll 1
@@ -1010,7 +1028,8 @@ static int64_t visible_cap(int64_t slots, int64_t first, int64_t window) {
 
 static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 static size_t parts_bytes(int64_t M, int H) { return round256((size_t)M * H * 8); }      // (no more items than heads)
-static size_t rec_bytes(int D) { return round256((size_t)sm_count() * 2 * 2 * 16 * (D + 4) * 4); }      // (two CTAs per SM at most)
+// two CTAs per SM at most and those for small shares: two parts of 16 heads each
+static size_t rec_bytes(int D) { return round256((size_t)(2 * sm_count() + last_ctas(2 * sm_count())) * 2 * 16 * (D + 4) * 4); }
 static size_t stat_bytes(int64_t M, int H) { return round256((size_t)M * H * 8); }
 
 template <typename E>
@@ -1030,7 +1049,8 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_attn_kernel)");
   const int ctas = sm_count() * E::CTAS;
   const int64_t most = (int64_t)a.M * items * ((a.cap / PA_TILE + E::WARPS - 1) / E::WARPS);
-  const int grid = (int)(most < ctas ? most : ctas);
+  a.last = most >= (int64_t)PA_LAST_UNITS * ctas ? last_ctas(ctas) : 0;
+  const int grid = (int)(most < ctas ? most : ctas) + a.last;
   a.tpp = a.pt.page / PA_TILE;
   a.inv_tpp = ((1ull << 36) + a.tpp - 1) / a.tpp;
   a.pitch = 1;

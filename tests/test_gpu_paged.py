@@ -198,6 +198,9 @@ ATTN = [
     ("f32", 8, 2, 128, 16, [300, 90], 17, 33),
     ("f16", 8, 2, 256, 16, [300, 90], 500, 7),
     ("bf16", 8, 2, 128, 64, [20000, 40, 9000], 0, 0),
+    ("bf16", 32, 32, 64, 64, [15000, 299, 0, 1500], 0, 0),          # work enough for small shares at its end, in each engine
+    ("f16", 64, 32, 80, 48, [3, 8000, 9000], 100, 8500),
+    ("f32", 32, 32, 8, 16, [12000, 77, 5000], 0, 0),
 ]
 
 
