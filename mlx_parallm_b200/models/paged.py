@@ -22,6 +22,10 @@ from .. import ops
 from .base import RowState
 
 
+class PagesExhausted(RuntimeError):
+    """A step found no room for its tokens in a cache in pages: none of them was appended."""
+
+
 class PageBook:
     """Which pages belong to which row, for all layers of a generation: the device ``table`` [rows, width] (-1: none), the rows' ``lengths`` (slots in
     use) and ``positions`` (places in the text: larger than the length once tokens were evicted), and the list of free pages."""
@@ -60,14 +64,14 @@ class PageBook:
         return self.width * self.page
 
     def room_for(self, counts: List[int]) -> None:
-        """Give every row the pages for ``counts[r]`` tokens (a row that has more keeps them).  All or nothing: RuntimeError if the pool is short."""
+        """Give every row the pages for ``counts[r]`` tokens (a row that has more keeps them).  All or nothing: PagesExhausted if the pool is short."""
         if max(counts, default=0) > self.max_tokens:
-            raise RuntimeError(f"a row of {max(counts)} tokens does not fit a paged cache of {self.max_tokens} per row")
+            raise PagesExhausted(f"a row of {max(counts)} tokens does not fit a paged cache of {self.max_tokens} per row")
         need = [max(0, -(-n // self.page) - len(o)) for n, o in zip(counts, self.owned)]
         if sum(need) == 0:
             return
         if sum(need) > len(self.free):
-            raise RuntimeError(f"paged cache exhausted: {sum(need)} pages wanted, {len(self.free)} of {self.pages} free")
+            raise PagesExhausted(f"paged cache exhausted: {sum(need)} pages wanted, {len(self.free)} of {self.pages} free")
         for r, k in enumerate(need):
             if k:
                 new = [self.free.pop() for _ in range(k)]
@@ -187,8 +191,8 @@ class PagedLayer(RowState):
             if self.book.keep and needed > room:
                 left = min(self.book.keep, room - new)
                 if left < max(1, self.book.first + self.book.recent):
-                    raise RuntimeError(f"{new} tokens at once do not fit a paged cache of {room} per row beside the {self.book.first} first and "
-                                       f"{self.book.recent} recent ones it keeps")
+                    raise PagesExhausted(f"{new} tokens at once do not fit a paged cache of {room} per row beside the {self.book.first} first and "
+                                         f"{self.book.recent} recent ones it keeps")
                 self.book.cut(left, self.book.first, self.book.recent)
             self.book.room_for([n + new for n in self._offsets])
         return moved

@@ -34,7 +34,7 @@ import torch
 from . import ops, sample_utils
 from .models._transformer import DecoderModel, advance_cache, advance_rows, bind_cache_group, prepare_cache, prepare_rows
 from .models.base import BatchedKVCache, PagedKVCache
-from .models.paged import PagedLayer
+from .models.paged import PagedLayer, PagesExhausted
 from .sample_utils import top_p_sampling
 from .tokenizer_utils import TokenizerWrapper, load_tokenizer
 
@@ -331,7 +331,8 @@ def generate_step(
 
     Same contract as the reference: prefill on the whole (left-padded) prompt batch, greedy if temp == 0
     else top-p / categorical sampling, repetition_penalty raises NotImplementedError (utils.py:366-367),
-    and the step for token n+1 is already in flight when token n is yielded (utils.py:420-427).
+    and the step for token n+1 is already in flight when token n is yielded (utils.py:420-427).  A cache in
+    pages that has no room for that step says so (PagesExhausted) when token n+1 is asked for: prompt + n places give n + 1 tokens.
     ``probs`` is per row (the reference gathers row 0 only).  ``prompt_lengths`` (models with ``supports_ragged``
     only): row b's last prompt_lengths[b] ids are its prompt, the ids before them are left padding and are not fed at all, so a
     row's tokens do not depend on the other rows of the batch."""
@@ -399,7 +400,11 @@ def generate_step(
         n_steps += 1
         if n_steps % 256 == 0:
             check_exchange()
-        step.run()                                   # launches step n+1 (utils.py:422-423)
+        try:
+            step.run()                               # launches step n+1 (utils.py:422-423)
+        except PagesExhausted:                       # no room for the token that is handed out now: the one behind it is the caller's to miss
+            yield out_y, out_p
+            raise
         if not step.greedy:
             sample(step.logits)
         next_y = step.tok.to(torch.int64).view(B, 1)

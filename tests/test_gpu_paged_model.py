@@ -146,3 +146,38 @@ def test_a_prompt_that_does_not_fit_is_refused():
         gm(ids, cache=gm.make_paged_cache(1, 64, page=16))
     with pytest.raises(RuntimeError, match="do not fit"):
         gm(ids, cache=gm.make_paged_cache(1, 64, page=16, keep=32, first=2))
+
+
+@pytest.mark.parametrize("pages", [None, 6], ids=["all pages", "pages that just suffice"])
+def test_generations_that_just_fit(pages):
+    """prompt + max_tokens places (a whole number of pages), through generate_step and the four text front-ends: all of the tokens, no error; one
+    token more is refused once it is asked for."""
+    from fake_tokenizer import FakeTokenizer
+    from mlx_parallm_b200.models.paged import PagesExhausted
+    from mlx_parallm_b200.tokenizer_utils import TokenizerWrapper
+    from mlx_parallm_b200.utils import batch_generate, batch_stream_generate_text, generate, generate_step, stream_generate
+    cfg, om, gm = make_pair("small-llama", dtype="float16")
+    ids = prompts_for(cfg, 2, 28)
+    width = 48 if pages is None else 64
+    make = lambda rows: gm.make_paged_cache(rows, width, page=16, pages=None if pages is None else pages * rows // 2)
+    steps = [(y[:, 0], lg) for _, (y, lg) in zip(range(21), oracle_generate_step(ids, om))]
+
+    def check(got):
+        got = np.stack(got, 1)
+        n = got.shape[1]
+        assert not greedy_report(got, np.stack([y for y, _ in steps[:n]], 1), [lg for _, lg in steps[:n]], LOGIT_TOL)[2]
+        return n
+
+    assert check([y[:, 0].cpu().numpy() for (y, _), _ in zip(generate_step(torch.from_numpy(ids), gm, cache=make(2)), range(20))]) == 20
+    run = generate_step(torch.from_numpy(ids), gm, cache=make(2))
+    assert check([next(run)[0][:, 0].cpu().numpy() for _ in range(21)]) == 21
+    with pytest.raises(PagesExhausted):
+        next(run)
+    tok = TokenizerWrapper(FakeTokenizer(cfg["vocab_size"], eos_token_id=cfg["vocab_size"] + 1))      # (never said)
+    texts = [" ".join(f"w{i}" for i in row) for row in ids]
+    assert len(generate(gm, tok, texts[0], max_tokens=20, cache=make(1)).split()) == 20
+    assert len("".join(stream_generate(gm, tok, texts[0], max_tokens=20, cache=make(1))).split()) == 20
+    answers = batch_generate(gm, tok, texts, max_tokens=20, format_prompts=False, cache=make(2))
+    assert check([np.array([int(t.split()[i][1:]) for t in answers]) for i in range(20)]) == 20
+    said = list(batch_stream_generate_text(gm, tok, ids, 20, cache=make(2)))
+    assert len(said) == 20 and all(reason == "length" for _, reason in said[-1])

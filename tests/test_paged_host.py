@@ -1,6 +1,7 @@
 """Argument checks of the paged-cache entry points (no device: every refusal comes before a launch), the tile arithmetic of the window, and the
 oracle of the GPU tests against itself."""
 import math
+import threading
 
 import pytest
 import torch
@@ -198,3 +199,65 @@ def test_layers_share_the_book_and_keep_positions_of_the_text():
     assert len(b.free) == b.pages and b.lengths.tolist() == [0, 0, 0] == b.positions.tolist() and layers[1].offsets == [0, 0, 0]
     with pytest.raises(RuntimeError, match="adds up"):
         b.cut(10, 0, 0)
+
+
+# ---------------------------------------------------------------- generation up to the last place
+class _Step:
+    """A decode step that counts up and has room for ``room`` steps."""
+    greedy = True
+
+    def __init__(self, room):
+        self.tok, self.probs, self.room, self.n = torch.zeros(1, dtype=torch.int32), torch.ones(1), room, 0
+
+    def run(self):
+        from mlx_parallm_b200.models.paged import PagesExhausted
+        if self.n == self.room:
+            raise PagesExhausted("full")
+        self.n += 1
+        self.tok += 1
+
+
+class _Model:
+    device, kernel_units, _lock = "cpu", (), threading.Lock()
+
+    def __call__(self, ids, cache, last_only):
+        return torch.zeros((1, 1, 4))
+
+    def greedy_tokens(self, logits, tok, probs):
+        tok.fill_(10)
+
+
+def test_every_token_that_was_made_is_given_before_a_full_cache_raises(monkeypatch):
+    """The step for the next token is launched before a token is handed out: that it finds no room is said when that token is asked for.  Prompt + n
+    places give n + 1 tokens, so zip(generate_step(...), range(n)), which looks for one more, ends with all of its n."""
+    from mlx_parallm_b200 import utils
+    from mlx_parallm_b200.models.paged import PagesExhausted
+    monkeypatch.setattr(utils.ops, "check_waits", lambda: None)
+    cache = [type("C", (), {"_lengths": 1})()]
+    for room in (1, 2, 5):
+        step = _Step(room)
+        monkeypatch.setattr(utils, "_decode_step_for", lambda *a: step)
+        got = [int(y) for (y, _), _ in zip(utils.generate_step([[1, 2]], _Model(), cache=cache), range(room))]
+        assert got == list(range(10, 10 + room))
+        step.n = 0
+        run, got = utils.generate_step([[1, 2]], _Model(), cache=cache), []
+        with pytest.raises(PagesExhausted):
+            for y, _ in run:
+                got.append(int(y))
+        assert got == list(range(10, 11 + room))
+
+
+def test_a_cache_without_room_says_so_in_one_kind_of_error():
+    from mlx_parallm_b200.models.paged import PagedLayer, PagesExhausted
+    b = book(pages=9)
+    with pytest.raises(PagesExhausted, match="does not fit"):
+        b.room_for([113, 0, 0])
+    with pytest.raises(PagesExhausted, match="exhausted"):
+        b.room_for([100, 50, 0])
+    b = book(keep=40, first=4)
+    layer = PagedLayer(b, 4, 2, 64)
+    layer._offsets = [60, 60, 60]
+    layer.kpages = torch.empty(1)
+    with pytest.raises(PagesExhausted, match="do not fit"):
+        layer.ensure_capacity(60 + 110, torch.float32, "cpu")
+    assert issubclass(PagesExhausted, RuntimeError)
