@@ -649,12 +649,14 @@ int b200p_paged_append(void* qkv, int64_t ldq, void* q_out, void* kpages, void* 
  * scores of minus infinity, gets zeros; an infinite value that it sees makes its outputs infinite or NaN.  mass (NULL: none): every visible slot's mass
  * grows by the weights that the query heads of its key head gave it, token by token in the call's order (tokens of different rows that share a page: in
  * no fixed order).
- * Hidden keys and values are not read.  workspace: b200p_paged_attn_workspace_bytes(M, H, D, keys), keys = width * page with a mass,
- * 0 without, aligned to 256 bytes; it needs no initial state and serves one stream at a time. */
+ * Hidden keys and values are not read.  workspace: b200p_paged_attn_workspace_bytes_of(M, H, G, D, keys), or without the number of key heads
+ * (up to twice as many scores) b200p_paged_attn_workspace_bytes(M, H, D, keys); keys = 0 without a mass, with one width * page or, if that is less
+ * and window > 0, first + window + 32.  Aligned to 256 bytes; it needs no initial state and serves one stream at a time. */
 int b200p_paged_attn(const void* q, const void* kpages, const void* vpages, float* mass, const int32_t* table, const int32_t* t_row,
                      const int32_t* t_slot, void* out, int64_t M, int H, int G, int D, int64_t P, int page, int rows, int width, float scale,
                      int64_t first, int64_t window, int dtype, int flags, void* workspace, size_t workspace_bytes, void* stream);
 size_t b200p_paged_attn_workspace_bytes(int64_t M, int H, int D, int64_t keys);
+size_t b200p_paged_attn_workspace_bytes_of(int64_t M, int H, int G, int D, int64_t keys);
 /* Eviction, step 1: kept int32 [rows, G, keep] = the slots that row r's key head g keeps, ascending.  A row with lengths[r] > keep keeps its
  * `first` first and `recent` last slots and of those between the keep - first - recent with the largest mass (ties: the lowest slots; NaN and slots
  * without a page count as less than every number); other rows keep all, -1 behind their last. */

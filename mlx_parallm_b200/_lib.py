@@ -144,6 +144,7 @@ SIGNATURES = {
     "b200p_paged_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _i64, _i64, _i32,
                                 _i32, _vp, _sz, _vp]),
     "b200p_paged_attn_workspace_bytes": (_sz, [_i64, _i32, _i32, _i64]),
+    "b200p_paged_attn_workspace_bytes_of": (_sz, [_i64, _i32, _i32, _i32, _i64]),
     "b200p_paged_select": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "b200p_paged_compact": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "b200p_paged_gather": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _i32, _i64, _i32, _vp]),

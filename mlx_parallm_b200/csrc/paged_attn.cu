@@ -1099,11 +1099,25 @@ static int launch_paged_type(const PagedAttn& a, cudaStream_t st) {
 
 using namespace b200p;
 
-extern "C" size_t b200p_paged_attn_workspace_bytes(int64_t M, int H, int D, int64_t keys) {
+static size_t workspace_bytes(int64_t M, int H, int D, int64_t keys, int64_t lines) {
   if (M <= 0 || H <= 0 || D <= 0) return 0;
   size_t n = parts_bytes(M, H) + rec_bytes(D);
-  if (keys > 0) n += stat_bytes(M, H) + (size_t)M * H * 2 * ((keys + PA_TILE - 1) / PA_TILE * PA_TILE) * 4;     // (pitch < 2 x heads)
+  if (keys > 0) n += stat_bytes(M, H) + (size_t)M * lines * ((keys + PA_TILE - 1) / PA_TILE * PA_TILE) * 4;
   return n;
+}
+
+extern "C" size_t b200p_paged_attn_workspace_bytes(int64_t M, int H, int D, int64_t keys) {
+  return workspace_bytes(M, H, D, keys, 2 * (int64_t)H);          // (a line of scores is less than twice its heads, whatever G)
+}
+
+extern "C" size_t b200p_paged_attn_workspace_bytes_of(int64_t M, int H, int G, int D, int64_t keys) {
+  if (G <= 0 || H < G || H % G) return 0;
+  // a key head's scores of a slot: a power of two up to 16 heads, whole blocks of 16 behind that (blocks of 4 or 8 take no more)
+  const int per = H / G;
+  int64_t line = 1;
+  while (line < 16 && line < per) line *= 2;
+  if (per > 16) line = (per + 15) / 16 * 16;
+  return workspace_bytes(M, H, D, keys, G * line);
 }
 
 extern "C" int b200p_paged_attn(const void* q, const void* kpages, const void* vpages, float* mass, const int32_t* table, const int32_t* t_row,
@@ -1124,7 +1138,7 @@ extern "C" int b200p_paged_attn(const void* q, const void* kpages, const void* v
   first = first < slots ? first : slots;
   window = window < slots ? window : slots;
   const int64_t cap = visible_cap(slots, first, window);
-  B200P_REQUIRE(workspace && workspace_bytes >= b200p_paged_attn_workspace_bytes(M, H, D, mass ? cap : 0) && aligned(workspace, 256), B200P_ERR_ARG,
+  B200P_REQUIRE(workspace && workspace_bytes >= b200p_paged_attn_workspace_bytes_of(M, H, G, D, mass ? cap : 0) && aligned(workspace, 256), B200P_ERR_ARG,
                 "paged attention workspace too small or not aligned to 256 bytes");
   PagedAttn a{};
   a.q = q, a.k = kpages, a.v = vpages, a.out = out, a.mass = mass, a.pt = pt, a.t_row = t_row, a.t_slot = t_slot;

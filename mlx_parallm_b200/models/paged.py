@@ -22,6 +22,9 @@ from .. import ops
 from .base import RowState
 
 
+OBSERVED_BYTES = 256 << 20        # workspace of a call that adds up the weights of a prompt's last tokens (one token per row at least)
+
+
 class PagesExhausted(RuntimeError):
     """A step found no room for its tokens in a cache in pages: none of them was appended."""
 
@@ -113,9 +116,16 @@ class PageBook:
             t = self._scratch[name] = torch.empty(shape, dtype=dtype, device=self.device)
         return t
 
-    def workspace(self, M: int, H: int, D: int, keys: int) -> torch.Tensor:
+    @property
+    def weighed(self) -> int:
+        """Slots of a row that a token can give a weight to (0: nobody adds them up)."""
+        if not self.keep:
+            return 0
+        return min(self.max_tokens, self.first + self.window + 32) if self.window else self.max_tokens
+
+    def workspace(self, M: int, H: int, G: int, D: int, keys: int) -> torch.Tensor:
         """The workspace of calls of M tokens, which are on one stream (the decode step's stays where a captured step knows it)."""
-        need = ops.paged_attn_workspace_bytes(M, H, D, keys)
+        need = ops.paged_attn_workspace_bytes(M, H, D, keys, G)
         key = "step" if M == self.rows else "portion"
         t = self._scratch.get(key)
         if t is None or t.numel() < need:
@@ -184,7 +194,7 @@ class PagedLayer(RowState):
             self.vpages = torch.zeros(shape, dtype=dtype, device=device)
             self.mass = torch.zeros(shape[:3], dtype=torch.float32, device=device) if self.book.keep else None
             if self.kpages.is_cuda:                                     # a decode step's workspace: not inside its capture
-                self.book.workspace(self.batch_size, self.n_heads, self.head_dim, self.book.max_tokens if self.book.keep else 0)
+                self.book.workspace(self.batch_size, self.n_heads, self.n_kv_heads, self.head_dim, self.book.weighed)
             moved = True
         if self is self.book.layers[0]:
             new, room = needed - max(self._offsets), self.book.max_tokens
@@ -201,27 +211,30 @@ class PagedLayer(RowState):
     def append_and_attend(self, qkv, q, out, tokens, B: int, L: int, heads: int, rates, scale: float, q_norm, k_norm, eps: float, attn_workspace,
                           out_perm: bool):
         """Norms, rotation and append of the step's tokens, then their attention: ``out`` [B L, heads D]."""
-        book, D = self.book, self.head_dim
+        book, G, D = self.book, self.n_kv_heads, self.head_dim
         row, slot, pos = tokens
         ops.paged_append(qkv, q, self.kpages, self.vpages, book.table, row, slot, pos, heads, rates=rates, q_norm_w=q_norm, k_norm_w=k_norm, eps=eps,
                          mass=self.mass)
-        keys = book.max_tokens if self.mass is not None else 0
         observed = min(L, max(0, book.observe - book.behind))
         if L == 1:
             ops.paged_attn(q, self.kpages, self.vpages, book.table, row, slot, out, scale, first=book.first, window=book.window,
-                           mass=self.mass if observed or not book.behind else None, workspace=book.workspace(B, heads, D, keys), out_perm=out_perm)
+                           mass=self.mass if observed or not book.behind else None, workspace=book.workspace(B, heads, G, D, book.weighed),
+                           out_perm=out_perm)
             return
         if book.window:
             ops.paged_attn(q, self.kpages, self.vpages, book.table, row, slot, out, scale, first=book.first, window=book.window,
-                           workspace=book.workspace(B * L, heads, D, 0), out_perm=out_perm)
+                           workspace=book.workspace(B * L, heads, G, D, 0), out_perm=out_perm)
         else:
             cap = -(-(max(self._offsets) + L) // 256) * 256
-            dense = book.scratch("dense", (2, B, self.n_kv_heads, cap, D), self.kpages.dtype)
+            dense = book.scratch("dense", (2, B, G, cap, D), self.kpages.dtype)
             ops.paged_gather(self.kpages, self.vpages, book.table, book.row_index, book.lengths, dense[0], dense[1], extra=L)
-            ops.attn(q, dense[0], dense[1], book.lengths, out, B, L, heads, self.n_kv_heads, D, scale, workspace=attn_workspace, out_perm=out_perm)
+            ops.attn(q, dense[0], dense[1], book.lengths, out, B, L, heads, G, D, scale, workspace=attn_workspace, out_perm=out_perm)
         if self.mass is not None and observed > 0:                      # what the prompt's last tokens look at
-            n = observed
-            last = lambda t: t.view(B, L, -1)[:, L - n:].reshape(B * n, -1).contiguous()
-            ql = last(q)
-            ops.paged_attn(ql, self.kpages, self.vpages, book.table, last(row).view(-1), last(slot).view(-1), torch.empty_like(ql), scale, first=book.first,
-                           window=book.window, mass=self.mass, workspace=book.workspace(B * n, heads, D, keys))
+            # as many at once as their scores have room for, every row's in order
+            size = lambda n: ops.paged_attn_workspace_bytes(n * B, heads, D, book.weighed, G)
+            n = max(1, min(observed, OBSERVED_BYTES // (size(2) - size(1)), 65535 // B))
+            for l0 in range(L - observed, L, n):
+                part = lambda t: t.view(B, L, -1)[:, l0:l0 + n].reshape(-1, t.numel() // (B * L)).contiguous()
+                ql = part(q)
+                ops.paged_attn(ql, self.kpages, self.vpages, book.table, part(row).view(-1), part(slot).view(-1), torch.empty_like(ql), scale,
+                               first=book.first, window=book.window, mass=self.mass, workspace=book.workspace(ql.shape[0], heads, G, D, book.weighed))

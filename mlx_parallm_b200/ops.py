@@ -847,8 +847,11 @@ def paged_append(qkv, q_out, kpages, vpages, table, t_row, t_slot, t_pos, H: int
     return q_out
 
 
-def paged_attn_workspace_bytes(M: int, H: int, D: int, keys: int = 0) -> int:
-    """Bytes of a workspace (256-byte aligned, one stream at a time); ``keys``: the table's width * page where a mass is added up, else 0."""
+def paged_attn_workspace_bytes(M: int, H: int, D: int, keys: int = 0, G: Optional[int] = None) -> int:
+    """Bytes of a workspace (256-byte aligned, one stream at a time); ``keys``: 0, or where a mass is added up the table's width * page (behind a
+    window first + window + 32 are enough).  ``G``: the key heads; without them the bytes that suffice for any number."""
+    if G is not None:
+        return int(lib().b200p_paged_attn_workspace_bytes_of(int(M), int(H), int(G), int(D), int(keys)))
     return int(lib().b200p_paged_attn_workspace_bytes(int(M), int(H), int(D), int(keys)))
 
 

@@ -181,3 +181,21 @@ def test_generations_that_just_fit(pages):
     assert check([np.array([int(t.split()[i][1:]) for t in answers]) for i in range(20)]) == 20
     said = list(batch_stream_generate_text(gm, tok, ids, 20, cache=make(2)))
     assert len(said) == 20 and all(reason == "length" for _, reason in said[-1])
+
+
+@pytest.mark.parametrize("window", [0, 70])
+def test_weights_of_a_prompts_last_tokens_in_small_calls(monkeypatch, window):
+    """However many calls the workspace's bound makes of them: the same weights, to the roundings of a sum of 60 (fp32, and scores that came through
+    logits of LOGIT_TOL in the layers before)."""
+    from mlx_parallm_b200.models import paged
+    cfg, om, gm = make_pair("small-llama", dtype="float16")
+    ids = torch.from_numpy(prompts_for(cfg, 3, 90))
+    out = []
+    for size in (1 << 28, 1 << 20, 1):
+        monkeypatch.setattr(paged, "OBSERVED_BYTES", size)
+        cache = gm.make_paged_cache(3, 1000, page=48, keep=100, observe=60, window=window, first=3 if window else 0)
+        gm(ids, cache=cache, last_only=True)
+        out.append([c.mass.clone() for c in cache])
+        assert all(abs(float(m.sum()) - 3 * 60 * c.n_heads) <= 1e-4 * 180 * c.n_heads for m, c in zip(out[-1], cache))
+    for a, b, c in zip(*out):
+        assert float((a - b).abs().max()) <= LOGIT_TOL * float(a.abs().max()) and float((a - c).abs().max()) <= LOGIT_TOL * float(a.abs().max())

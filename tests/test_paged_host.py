@@ -261,3 +261,59 @@ def test_a_cache_without_room_says_so_in_one_kind_of_error():
     with pytest.raises(PagesExhausted, match="do not fit"):
         layer.ensure_capacity(60 + 110, torch.float32, "cpu")
     assert issubclass(PagesExhausted, RuntimeError)
+
+
+# ---------------------------------------------------------------- scratch
+@pytest.mark.parametrize("H,G,line", [(32, 8, 4), (32, 32, 1), (6, 3, 2), (9, 3, 4), (40, 8, 8), (16, 1, 16), (9, 1, 16), (17, 1, 32), (40, 1, 48)])
+def test_workspace_of_known_key_heads(H, G, line):
+    """fp32 scores of whole tiles, ``line`` of them per key head and slot, and never more than the call that does not know the key heads."""
+    f, g = L().b200p_paged_attn_workspace_bytes_of, L().b200p_paged_attn_workspace_bytes
+    assert f(3, H, G, 64, 1000) - f(3, H, G, 64, 200) == 3 * G * line * (1008 - 208) * 4
+    assert f(3, H, G, 64, 0) == g(3, H, 64, 0) and f(3, H, G, 64, 1000) <= g(3, H, 64, 1000)
+    need = f(2, H, G, 64, 64)
+    assert attn(H=H, G=G, mass=OK, bytes=need - 1) == ARG
+    assert f(2, 9, 2, 64, 10) == 0 == f(2, 8, 0, 64, 10) == f(0, 8, 2, 64, 10)
+
+
+def observed_calls(monkeypatch, L, heads=32, kv=8, D=8, offset=0, behind=0, **kw):
+    """The attention calls with weights that a portion of L tokens makes: (row, slot, workspace bytes) each."""
+    from mlx_parallm_b200.models import paged
+    calls = []
+    b = book(**kw)
+    layer = paged.PagedLayer(b, heads, kv, D)
+    layer._offsets = [offset] * b.rows
+    b.behind = behind
+    layer.kpages = layer.vpages = torch.zeros(1, dtype=torch.float16)
+    layer.mass = torch.zeros(1)
+    for name in ("paged_append", "paged_gather", "attn"):
+        monkeypatch.setattr(paged.ops, name, lambda *a, **k: None)
+    monkeypatch.setattr(paged.ops, "paged_attn", lambda q, k, v, table, row, slot, out, scale, mass=None, workspace=None, **kw: calls.append(
+        (row.tolist(), slot.tolist(), workspace.numel())) if mass is not None else None)
+    row = torch.arange(b.rows, dtype=torch.int32).repeat_interleave(L)
+    slot = torch.arange(L, dtype=torch.int32).repeat(b.rows) + offset
+    q = torch.empty((b.rows * L, heads * D), dtype=torch.float16)
+    layer.append_and_attend(None, q, torch.empty_like(q), (row, slot, slot), b.rows, L, heads, None, 1.0, None, None, 1e-6, None, False)
+    return calls
+
+
+@pytest.mark.parametrize("kw,L", [(dict(rows=64, max_tokens=16384, keep=1000), 100), (dict(rows=16, max_tokens=131072, keep=1000), 40),
+                                  (dict(rows=64, max_tokens=16384, keep=1000, window=500, first=4), 100), (dict(rows=3, max_tokens=200, keep=100), 20)], ids=str)
+def test_weights_of_a_prompt_take_a_bounded_workspace(monkeypatch, kw, L):
+    """Every row's last tokens in order, once each, in calls whose scratch does not grow with the table and the batch (a single token per row, which
+    a decode step has as well, is the least)."""
+    from mlx_parallm_b200.models import paged
+    from mlx_parallm_b200.ops import paged_attn_workspace_bytes
+    calls = observed_calls(monkeypatch, L, **kw)
+    keys = min(kw["max_tokens"], 536 if "window" in kw else 1 << 30)
+    assert max(c[2] for c in calls) <= max(paged.OBSERVED_BYTES + (16 << 20), paged_attn_workspace_bytes(kw["rows"], 32, 8, keys, 8))
+    seen = [[] for _ in range(kw["rows"])]
+    for rows, slots, _ in calls:
+        assert len(rows) < 65536
+        for r, s in zip(rows, slots):
+            seen[r].append(s)
+    assert seen == [list(range(L - min(L, 32), L))] * kw["rows"]
+
+
+def test_weights_of_more_tokens_than_a_call_takes(monkeypatch):
+    calls = observed_calls(monkeypatch, 32, heads=1, kv=1, rows=3000, max_tokens=64, keep=40)
+    assert sum(len(c[0]) for c in calls) == 3000 * 32 and max(len(c[0]) for c in calls) < 65536
