@@ -336,7 +336,8 @@ int b200p_gemm_set_path(int path);
  * last call (which clears it).  Synchronises the device. */
 int b200p_gemm_tc_fault(void);
 
-/* t_row[t] = rows[e], t_pos[t] = lengths[rows[e]] + (t - cu[e]), t_off[t] = t - cu[e] for the entry e that owns token t */
+/* t_row[t] = rows[e], t_pos[t] = lengths[rows[e]] + (t - cu[e]), t_off[t] = t - cu[e] for the entry e that owns token t
+ * (rows[e] < 0: an entry whose tokens are idle; lengths is not read for it) */
 int b200p_ragged_plan(const int32_t* cu, const int32_t* rows, const int32_t* lengths, int32_t* t_row, int32_t* t_pos,
                       int32_t* t_off, int nb, int64_t M, void* stream);
 /* end of a step: lengths[rows[e]] += cu[e+1] - cu[e]; last_token[rows[e]] = ids[cu[e+1] - 1] (entries with no token: nothing) */
@@ -673,6 +674,8 @@ int b200p_paged_compact(void* kpages, void* vpages, float* mass, const int32_t* 
 int b200p_paged_gather(const void* kpages, const void* vpages, const int32_t* table, const int32_t* row_of, const int32_t* lengths,
                        void* kcache, void* vcache, int extra, int64_t count, int G, int D, int64_t P, int page, int rows, int width,
                        int64_t Tcap, int dtype, void* stream);
+/* End of a step: lengths[r] and positions[r] grow by delta for every r < count with rows[r] >= 0; the others stay as they are. */
+int b200p_paged_advance(int32_t* lengths, int32_t* positions, const int32_t* rows, int64_t count, int32_t delta, void* stream);
 /* *count = how often a call on the current device met a row, slot or page id that names no place since the last reset; reset != 0 clears it.
  * Synchronises `stream`; not capturable. */
 int b200p_paged_fault_count(unsigned int* count, int reset, void* stream);

@@ -148,6 +148,7 @@ SIGNATURES = {
     "b200p_paged_select": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "b200p_paged_compact": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "b200p_paged_gather": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _i32, _i64, _i32, _vp]),
+    "b200p_paged_advance": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp]),
     "b200p_paged_fault_count": (_i32, [C.POINTER(C.c_uint), _i32, _vp]),
 }
 

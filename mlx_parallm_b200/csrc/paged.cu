@@ -616,6 +616,15 @@ paged_gather_kernel(const uint4* kp, const uint4* vp, PageTable pt, const int32_
   if (missing) atomicAdd(&g_paged_fault, 1u);
 }
 
+// ------------------------------------------------------------------------------------------------ counters
+__global__ void paged_advance_kernel(int32_t* lengths, int32_t* positions, const int32_t* rows, int64_t count, int32_t delta) {
+  pdl_wait();
+  const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (r >= count || rows[r] < 0) return;
+  lengths[r] += delta;
+  positions[r] += delta;
+}
+
 }  // namespace b200p
 
 using namespace b200p;
@@ -771,6 +780,16 @@ extern "C" int b200p_paged_gather(const void* kpages, const void* vpages, const 
   launch_pdl(paged_gather_kernel, dim3((unsigned)((longest + slots - 1) / slots), (unsigned)G, (unsigned)count), GATHER_THREADS, 0, (cudaStream_t)stream,
              (const uint4*)kpages, (const uint4*)vpages, pt, row_of, lengths, (uint4*)kcache, (uint4*)vcache, extra, G, chunks, inv, slots, Tcap);
   B200P_LAUNCH_CHECK("paged_gather_kernel");
+  return B200P_OK;
+}
+
+extern "C" int b200p_paged_advance(int32_t* lengths, int32_t* positions, const int32_t* rows, int64_t count, int32_t delta, void* stream) {
+  PdlClass pdl_cls(32);
+  B200P_REQUIRE(lengths && positions && rows, B200P_ERR_ARG, "null pointer");
+  B200P_REQUIRE(count >= 0 && count < (1ll << 31), B200P_ERR_ARG, "bad number of rows %lld", (long long)count);
+  if (count == 0) return B200P_OK;
+  launch_pdl(paged_advance_kernel, (unsigned)((count + 255) / 256), 256, 0, (cudaStream_t)stream, lengths, positions, rows, count, delta);
+  B200P_LAUNCH_CHECK("paged_advance_kernel");
   return B200P_OK;
 }
 

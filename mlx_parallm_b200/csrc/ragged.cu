@@ -18,7 +18,7 @@ __global__ void ragged_plan_kernel(const int32_t* __restrict__ cu, const int32_t
   const int off = (int)(t - cu[lo]);
   t_row[t] = r;
   t_off[t] = off;
-  t_pos[t] = lengths[r] + off;
+  t_pos[t] = (r < 0 ? 0 : lengths[r]) + off;      // (a negative row: idle, without a history)
 }
 
 __global__ void ragged_advance_kernel(int32_t* __restrict__ lengths, int32_t* __restrict__ last_token,

@@ -23,7 +23,7 @@ applied at load time by ``tp.shard_*`` and adds one all-reduce after each row-sp
 from __future__ import annotations
 
 import threading
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
@@ -374,6 +374,14 @@ class DecoderModel:
         self.rope_rates()                                               # (not inside a capture)
         return [PagedLayer(book, l.self_attn.n_heads, l.self_attn.n_kv_heads, self.head_dim) for l in self.model.layers]
 
+    def release_rows(self, cache: List[PagedLayer], rows: Sequence[int]):
+        """Rows of a cache in pages that have ended: their pages go back to the pool, and until the cache is reset the next steps leave them out (what
+        those steps return for them means nothing).  The others' captured decode step stays valid."""
+        if not isinstance(cache[0], PagedLayer):
+            raise NotImplementedError("every row of a dense cache of this model takes a token in every step")
+        with self._lock:
+            release_rows(cache, [int(r) for r in rows])
+
     def rope_rates(self) -> torch.Tensor:
         """fp32 [head_dim / 2]: the angle of pair i at position p is p * rates[i]."""
         if self._rope_rates is None:
@@ -408,7 +416,7 @@ class DecoderModel:
                       if self._fast16 and M <= ACC32_MAX_ROWS and 2 * inter_local * args.hidden_size <= GATE_UP_ACC32_MAX_WEIGHTS
                       else None),
                 q=torch.empty((M, att.n_heads * att.head_dim), dtype=dt, device=dev),
-                att=torch.empty((M, att.n_heads * att.head_dim), dtype=dt, device=dev),
+                att=torch.zeros((M, att.n_heads * att.head_dim), dtype=dt, device=dev),      # (idle rows' stay as they are)
                 act=torch.empty((M, inter_local), dtype=dt, device=dev),
                 xl=torch.empty((M, args.hidden_size), dtype=dt, device=dev),
                 # split-K tile counters live at the head of the qmm workspace: zero once, kernels self-clean
@@ -607,13 +615,16 @@ def release_rows(caches, rows: List[int]):
 
 
 def advance_counters(caches, L: int):
-    """Every distinct device counter of the caches (lengths; a paged cache's positions too) += L."""
+    """Every distinct device counter of the caches (lengths; of a paged cache the positions too, but not those of idle rows) += L."""
     seen = set()
     for c in caches:
-        for t in c.counters():
-            if t.data_ptr() not in seen:
-                seen.add(t.data_ptr())
-                ops.advance_lengths(t, L)
+        t = c.counters()
+        if t[0].data_ptr() not in seen:
+            seen.add(t[0].data_ptr())
+            if isinstance(c, PagedLayer):
+                ops.paged_advance(*t, c.book.row_index, L)
+            else:
+                ops.advance_lengths(t[0], L)
 
 
 def advance_cache(caches: List[BatchedKVCache], L: int):

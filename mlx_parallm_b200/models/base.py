@@ -89,7 +89,7 @@ class RowState:
         self._lengths_shared = True
 
     def counters(self) -> tuple:
-        """Device counters a step adds its tokens to."""
+        """Device counters a step adds its tokens to (a paged cache: lengths and positions)."""
         return (self._lengths,)
 
     def _sync_lengths(self):

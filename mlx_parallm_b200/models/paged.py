@@ -55,7 +55,8 @@ class PageBook:
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros((rows,), dtype=torch.int32, device=device)
         self.positions = torch.zeros((rows,), dtype=torch.int32, device=device)
-        self.row_index = torch.arange(rows, dtype=torch.int32, device=device)
+        self.row_index = torch.arange(rows, dtype=torch.int32, device=device)      # -1: a row that was given back, whose tokens are idle
+        self.live = [True] * rows
         self.free: List[int] = list(range(self.pages - 1, -1, -1))
         self.owned: List[List[int]] = [[] for _ in range(rows)]
         self.evicted = [0] * rows              # how far a row's positions are ahead of its slots
@@ -81,6 +82,18 @@ class PageBook:
                 at = len(self.owned[r])
                 self.owned[r] += new
                 self.table[r, at:at + k] = torch.tensor(new, dtype=torch.int32).to(self.device)
+
+    def release(self, rows: List[int]) -> None:
+        """Rows that are given back are idle until the cache is reset: they take no pages and their counters stay at 0."""
+        for r in rows:
+            if self.live[r]:
+                self.live[r] = False
+                self.row_index[r] = -1
+
+    def revive(self) -> None:
+        if not all(self.live):
+            self.live = [True] * self.rows
+            self.row_index.copy_(torch.arange(self.rows, dtype=torch.int32))
 
     def shrink(self, counts: List[int]) -> None:
         """Take back the pages that rows of ``counts[r]`` tokens do not need."""
@@ -174,19 +187,25 @@ class PagedLayer(RowState):
         super().reset(None)
         self.book.positions.zero_()
         self.book.shrink([0] * self.batch_size)
+        self.book.revive()
 
     def release_rows_host(self, rows: List[int]):
         super().release_rows_host(rows)
         for r in rows:
             self.book.evicted[r] = 0
+        self.book.release(rows)
         self.book.shrink(self._offsets)
+
+    def advance_host(self, L: int):
+        self._offsets = [o + L if live else 0 for o, live in zip(self._offsets, self.book.live)]
+        self.offset = max(self._offsets)
 
     def _sync_lengths(self):
         super()._sync_lengths()
         self.book.positions.copy_(torch.tensor([n + e for n, e in zip(self._offsets, self.book.evicted)], dtype=torch.int32))
 
     def ensure_capacity(self, needed: int, dtype, device) -> bool:
-        """``needed``: the longest row's tokens after the coming step; the other rows grow by as many."""
+        """``needed``: the longest row's tokens after the coming step; the other rows in use grow by as many."""
         moved = False
         if self.kpages is None or self.kpages.dtype != dtype:
             shape = (self.book.pages, self.n_kv_heads, self.book.page, self.head_dim)
@@ -204,7 +223,7 @@ class PagedLayer(RowState):
                     raise PagesExhausted(f"{new} tokens at once do not fit a paged cache of {room} per row beside the {self.book.first} first and "
                                          f"{self.book.recent} recent ones it keeps")
                 self.book.cut(left, self.book.first, self.book.recent)
-            self.book.room_for([n + new for n in self._offsets])
+            self.book.room_for([n + new if live else 0 for n, live in zip(self._offsets, self.book.live)])
         return moved
 
     # -- the layer's part of a step -----------------------------------------------------------------------------------
@@ -229,6 +248,8 @@ class PagedLayer(RowState):
             dense = book.scratch("dense", (2, B, G, cap, D), self.kpages.dtype)
             ops.paged_gather(self.kpages, self.vpages, book.table, book.row_index, book.lengths, dense[0], dense[1], extra=L)
             ops.attn(q, dense[0], dense[1], book.lengths, out, B, L, heads, G, D, scale, workspace=attn_workspace, out_perm=out_perm)
+        if not all(book.live):                                          # (a step's are what they were: finite)
+            out.view(B, L, -1)[[not live for live in book.live]] = 0
         if self.mass is not None and observed > 0:                      # what the prompt's last tokens look at
             # as many at once as their scores have room for, every row's in order
             size = lambda n: ops.paged_attn_workspace_bytes(n * B, heads, D, book.weighed, G)

@@ -915,6 +915,15 @@ def paged_gather(kpages, vpages, table, rows, lengths, kcache, vcache, extra: in
         P, page, R, width, shape[2], dtype_code(dt), _stream()))
 
 
+def paged_advance(lengths, positions, rows, delta: int):
+    """End of a step: both counters (int32) of every row whose entry of ``rows`` (int32) is not negative grow by ``delta`` (b200p_paged_advance)."""
+    _here(lengths, positions, rows)
+    if any(t.dtype is not _I32 or t.numel() != rows.numel() for t in (lengths, positions, rows)):
+        _refuse("lengths, positions and rows are int32, one for each row")
+    _call("b200p_paged_advance", lambda: lib().b200p_paged_advance(
+        lengths.data_ptr(), positions.data_ptr(), rows.data_ptr(), rows.numel(), int(delta), _stream()))
+
+
 def paged_fault_count(reset: bool = False) -> int:
     """How often a paged call on the current device met a row, slot or page id that names no place since the last reset.  Synchronises the
     current stream: call it at generation boundaries, never under graph capture."""

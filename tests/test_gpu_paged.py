@@ -739,3 +739,30 @@ def test_refusals(ops):
     small = torch.empty((16,), dtype=torch.uint8, device="cuda")
     with pytest.raises(B200PError):
         A(mass=ms, workspace=small)
+
+
+def test_advance_of_the_rows_in_use(ops):
+    """Counters of rows whose index is negative stay; one launch, captured and replayed."""
+    n = 700
+    rows = torch.arange(n, dtype=torch.int32)
+    rows[torch.tensor([0, 5, 255, 256, 699])] = i32([-1, -7, -1, -2, -1])
+    a, b = torch.arange(n, dtype=torch.int32).cuda(), (3 * torch.arange(n, dtype=torch.int32)).cuda()
+    rows = rows.cuda()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.paged_advance(a, b, rows, 7)
+    g.replay()
+    ops.paged_advance(a, b, rows, -2)
+    up = torch.where(rows.cpu() < 0, 0, 5)
+    assert torch.equal(a.cpu(), torch.arange(n) + up) and torch.equal(b.cpu(), 3 * torch.arange(n) + up)
+    for bad in (dict(lengths=a[:5]), dict(positions=b.long()), dict(rows=rows[::2])):
+        with pytest.raises(ValueError):
+            ops.paged_advance(**{**dict(lengths=a, positions=b, rows=rows, delta=1), **bad})
+
+
+def test_plan_of_idle_entries(ops):
+    """An entry of a negative row (next to others): its tokens are idle, its history is not looked at."""
+    cu, rows, lengths = i32([0, 3, 5, 9]).cuda(), i32([1, -1, 0]).cuda(), i32([40, 7]).cuda()
+    row, pos, off = (torch.full((9,), 99, dtype=torch.int32, device="cuda") for _ in range(3))
+    ops.ragged_plan(cu, rows, lengths, row, pos, off, 3, 9)
+    assert row.tolist() == [1] * 3 + [-1] * 2 + [0] * 4 and pos.tolist() == [7, 8, 9, 0, 1, 40, 41, 42, 43] and off.tolist() == [0, 1, 2, 0, 1, 0, 1, 2, 3]

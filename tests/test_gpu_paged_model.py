@@ -199,3 +199,51 @@ def test_weights_of_a_prompts_last_tokens_in_small_calls(monkeypatch, window):
         assert all(abs(float(m.sum()) - 3 * 60 * c.n_heads) <= 1e-4 * 180 * c.n_heads for m, c in zip(out[-1], cache))
     for a, b, c in zip(*out):
         assert float((a - b).abs().max()) <= LOGIT_TOL * float(a.abs().max()) and float((a - c).abs().max()) <= LOGIT_TOL * float(a.abs().max())
+
+
+@pytest.mark.parametrize("keep", [0, 24])
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "captured"])
+def test_rows_given_back_stay_idle(graph, keep):
+    """A row is given back between two replays of a step: its counters stay at nothing and it takes no page, the others' logits are the oracle's, and
+    a portion of a prompt and (keep) a cut pass it by.  Nothing meets a place that does not exist."""
+    from mlx_parallm_b200 import ops
+    from mlx_parallm_b200.utils import DecodeSession
+    cfg, om, gm = make_pair("small-llama", dtype="float16")
+    ids = prompts_for(cfg, 3, 60, seed=11)
+    ops.paged_fault_count(reset=True)
+    cache = gm.make_paged_cache(3, 48, page=16, pages=8, keep=keep, first=2, recent=8)
+    book = cache[0].book
+    exp = om.forward(ids, om.make_cache(3))
+    gm(torch.from_numpy(ids[:, :20]), cache=cache, last_only=True)
+    session = DecodeSession(gm, cache, 3, True, use_graph=graph)
+
+    def step(i, rows):
+        session.tok.copy_(torch.from_numpy(ids[:, i]).to(torch.int32))
+        session.run()
+        assert bool(torch.isfinite(session.logits).all())
+        if i < 48:                                                  # (cuts change what is seen)
+            assert rel_err(session.logits[rows].cpu().numpy(), exp[rows, i]) < LOGIT_TOL
+
+    for i in range(20, 30):
+        step(i, [0, 1, 2])
+    gm.release_rows(cache, [1])
+    assert book.row_index.tolist() == [0, -1, 2] and book.owned[1] == [] and len(book.free) == 4
+    for i in range(30, 34):
+        step(i, [0, 2])
+    got = gm(torch.from_numpy(ids[:, 34:40]), cache=cache).cpu().numpy()      # a portion
+    assert rel_err(got[[0, 2]], exp[[0, 2], 34:40]) < LOGIT_TOL and np.isfinite(got).all()
+    for i in range(40, 60 if keep else 48):
+        step(i, [0, 2])
+    n = 60 if keep else 48
+    assert book.positions.tolist() == [n, 0, n] and book.lengths.tolist() == cache[0].offsets == [min(n, cache[0].offsets[0]), 0, cache[0].offsets[0]]
+    assert book.owned[1] == [] and int(book.table[1].max()) == -1 and ops.paged_fault_count(reset=True) == 0
+    for c in cache:
+        c.reset(3)
+    again = gm(torch.from_numpy(ids[:, :20]), cache=cache).cpu().numpy()
+    assert rel_err(again, exp[:, :20]) < LOGIT_TOL
+
+
+def test_dense_rows_are_not_given_back():
+    cfg, _, gm = make_pair("tiny-llama", dtype="float16")
+    with pytest.raises(NotImplementedError):
+        gm.release_rows(gm.make_cache(2), [1])

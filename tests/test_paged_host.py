@@ -317,3 +317,46 @@ def test_weights_of_a_prompt_take_a_bounded_workspace(monkeypatch, kw, L):
 def test_weights_of_more_tokens_than_a_call_takes(monkeypatch):
     calls = observed_calls(monkeypatch, 32, heads=1, kv=1, rows=3000, max_tokens=64, keep=40)
     assert sum(len(c[0]) for c in calls) == 3000 * 32 and max(len(c[0]) for c in calls) < 65536
+
+
+# ---------------------------------------------------------------- rows that were given back
+def test_a_row_that_was_given_back_takes_no_page_again():
+    """Two rows over a pool that holds one and a bit: after row 1 is given back, row 0 has the pool to itself, step by step to its last place."""
+    from mlx_parallm_b200.models._transformer import prepare_cache, release_rows
+    from mlx_parallm_b200.models.paged import PagedLayer, PagesExhausted
+    b = book(rows=2, max_tokens=64, pages=4)
+    layers = [PagedLayer(b, 4, 2, 64) for _ in range(2)]
+
+    def step(n):
+        prepare_cache(layers, 2, n, torch.float32, "cpu")
+        for c in layers:
+            c.advance_host(n)
+
+    step(20)
+    assert [len(o) for o in b.owned] == [2, 2] and b.row_index.tolist() == [0, 1]
+    release_rows(layers, [1])
+    assert b.row_index.tolist() == [0, -1] and [len(o) for o in b.owned] == [2, 0] and len(b.free) == 2
+    where = b.row_index.data_ptr()
+    for n in range(21, 65):
+        step(1)
+        assert [len(o) for o in b.owned] == [-(-n // 16), 0] and all(c.offsets == [n, 0] for c in layers)
+        assert int(b.table[1].max()) == -1
+    with pytest.raises(PagesExhausted):
+        step(1)
+    release_rows(layers, [1, 0])
+    step(3)
+    assert b.row_index.tolist() == [-1, -1] and len(b.free) == 4 and layers[1].offsets == [0, 0]
+    for c in layers:
+        c.reset(2)
+    assert b.row_index.tolist() == [0, 1] and b.row_index.data_ptr() == where
+    step(5)
+    assert [len(o) for o in b.owned] == [1, 1] and layers[0].offsets == [5, 5]
+
+
+def test_advance_refuses():
+    f = L().b200p_paged_advance
+    assert f(0, OK, OK, 4, 1, 0) == ARG and f(OK, 0, OK, 4, 1, 0) == ARG and f(OK, OK, 0, 4, 1, 0) == ARG and f(OK, OK, OK, -1, 1, 0) == ARG
+    assert f(OK, OK, OK, 0, 1, 0) == 0
+    from mlx_parallm_b200 import ops
+    with pytest.raises(_lib.B200PError):
+        ops.paged_advance(torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 1)
