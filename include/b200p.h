@@ -632,7 +632,9 @@ int b200p_tanh_norm(const float* h, const float* alpha, const float* w, const fl
  * re-zeroing of qkv_f32), t_slot (where they lie in the row) and, for the rotation, t_pos (their position in the text, which differs from the slot
  * once tokens before them were evicted).
  * An id outside [0, P) (and a row or slot outside the table) names no place: nothing is written there, keys there count as masked, and
- * b200p_paged_fault_count counts the meeting.
+ * b200p_paged_fault_count counts the meeting.  The attention of a token whose slot is behind the table, and the selection, closing up and dense view
+ * of a row whose length is, go by the slots that the table has; each such token, and each such row of a call, counts once.  A token at a negative
+ * slot sees nothing and is no meeting, nor is a row of negative length, which is an empty one.
  * mass fp32 [P, G, page] (optional) is the attention weight that every cached token has received from later queries. */
 
 /* Step 1: qkv [M, >= (H + 2 G) D] = [q | k | v] (row stride ldq elements) in `dtype`, or (qkv_f32 = 1, 16-bit dtypes) the projection's fp32
@@ -669,7 +671,7 @@ int b200p_paged_select(const float* mass, const int32_t* table, const int32_t* l
 int b200p_paged_compact(void* kpages, void* vpages, float* mass, const int32_t* table, const int32_t* lengths, const int32_t* kept, int64_t P,
                         int G, int D, int page, int rows, int width, int keep, int dtype, void* stream);
 /* Dense view: slots j < min(lengths[r] + extra, Tcap) of row r = row_of[i] go to kcache / vcache `dtype` [count, G, Tcap, D] at [i, :, j]
- * (row_of[i] < 0: nothing); what lies behind stays as it was.  Prompt attention (b200p_attn) then reads them: append the portion, gather
+ * (row_of[i] < 0: nothing); what lies behind stays as it was, as do slots behind the table.  Prompt attention (b200p_attn) then reads them: append the portion, gather
  * with extra = its tokens. */
 int b200p_paged_gather(const void* kpages, const void* vpages, const int32_t* table, const int32_t* row_of, const int32_t* lengths,
                        void* kcache, void* vcache, int extra, int64_t count, int G, int D, int64_t P, int page, int rows, int width,

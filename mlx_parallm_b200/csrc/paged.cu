@@ -12,7 +12,8 @@ namespace b200p {
 namespace cg = cooperative_groups;
 int sm_count();
 
-// Calls of the append and the eviction that met an id that names no page where they needed one (b200p_paged_fault_count).
+// How often the append, the eviction and the dense view met an id that names no page where they needed one, or a row longer than the table
+// (b200p_paged_fault_count).
 __device__ unsigned int g_paged_fault = 0;
 
 int paged_attn_faults(unsigned int* count, int reset, cudaStream_t st);
@@ -287,6 +288,7 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
   const int g = blockIdx.y, r = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
   int n = lengths[r];
+  if (n > table_slots(pt) && g == 0 && rank == 0 && tid == 0) atomicAdd(&g_paged_fault, 1u);
   n = n < 0 ? 0 : (n > table_slots(pt) ? table_slots(pt) : n);
   int32_t* out = kept + ((int64_t)r * G + g) * keep;
   if (n <= keep) {                                                // the same for the whole cluster
@@ -463,6 +465,7 @@ paged_compact_kernel(uint4* kp, uint4* vp, float* mass, PageTable pt, const int3
   uint4* pages = values ? vp : kp;
   pdl_wait();
   int n = lengths[r];
+  if (n > table_slots(pt) && blockIdx.y == 0 && rank == 0 && tid == 0) atomicAdd(&g_paged_fault, 1u);
   n = n > table_slots(pt) ? table_slots(pt) : n;
   const int32_t* list = kept + ((int64_t)r * G + g) * keep;
   if (n <= 1) return;                                             // nothing can move: the same for the whole cluster
@@ -579,6 +582,7 @@ paged_gather_kernel(const uint4* kp, const uint4* vp, PageTable pt, const int32_
     if (threadIdx.x == 0 && blockIdx.x == 0 && g == 0) atomicAdd(&g_paged_fault, 1u);
     return;
   }
+  if (lengths[r] > table_slots(pt) && threadIdx.x == 0 && blockIdx.x == 0 && g == 0) atomicAdd(&g_paged_fault, 1u);
   int64_t n = (int64_t)lengths[r] + extra;
   if (n > table_slots(pt)) n = table_slots(pt);
   if (n > Tcap) n = Tcap;

@@ -16,7 +16,7 @@ namespace b200p {
 
 int sm_count();
 
-// tiles of keys that met an id that names no page (b200p_paged_fault_count; such keys count as masked), and tokens of rows behind the table
+// tiles of keys that met an id that names no page (b200p_paged_fault_count; such keys count as masked), and tokens of rows or at slots behind the table
 __device__ unsigned int g_paged_attn_fault = 0;
 
 int paged_attn_faults(unsigned int* count, int reset, cudaStream_t st) {
@@ -515,7 +515,7 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
     const Token tok(a, t, W);
     mine += tok.units * items;
     live += tok.units > 0;
-    if (blockIdx.x == 0 && a.t_row[t] >= a.pt.rows) atomicAdd(&g_paged_attn_fault, 1u);
+    if (blockIdx.x == 0 && (a.t_row[t] >= a.pt.rows || (a.t_row[t] >= 0 && a.t_slot[t] >= table_slots(a.pt)))) atomicAdd(&g_paged_attn_fault, 1u);
     if (a.M <= PA_TOKENS) {
       s.tok.row[t] = tok.row;
       s.tok.slots[t] = tok.span.n;

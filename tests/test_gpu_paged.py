@@ -766,3 +766,41 @@ def test_plan_of_idle_entries(ops):
     row, pos, off = (torch.full((9,), 99, dtype=torch.int32, device="cuda") for _ in range(3))
     ops.ragged_plan(cu, rows, lengths, row, pos, off, 3, 9)
     assert row.tolist() == [1] * 3 + [-1] * 2 + [0] * 4 and pos.tolist() == [7, 8, 9, 0, 1, 40, 41, 42, 43] and off.tolist() == [0, 1, 2, 0, 1, 0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("f32", 40)])
+def test_slots_behind_the_table_are_counted(ops, dtype, D):
+    """A token whose slot is behind the table sees what its row holds, and each is counted once; one at the last slot, and a negative one, are not."""
+    c = Cache([64, 64, 64, 64], 16, 2, D, DT[dtype], 61)
+    for n in (0, 600):                                              # few tokens, and more than a CTA keeps
+        row, slot = i32([0, 1, 2, 3] + [-1] * n), i32([64, 63, (1 << 31) - 1, -1] + [1 << 20] * n)
+        q = c.normal(4 + n, 8 * D).to(c.dtype)
+        for mass in (False, True):
+            _check_attn(ops, c, q, row, slot, 8, 0, 0, mass, 0.2)
+            assert ops.paged_fault_count(reset=True) == 2
+    _check_attn(ops, c, c.normal(3, 8 * D).to(c.dtype), i32([0, 1, 2]), i32([63, 62, -3]), 8, 1, 5, True, 0.2)
+    assert ops.paged_fault_count(reset=True) == 0
+
+
+def test_lengths_behind_the_table_are_counted(ops):
+    """Selection, closing up and the dense view take such a row for full, once counted in each call; ``extra`` behind the table's end is not."""
+    c = Cache([64, 64, 40], 16, 2, 64, torch.bfloat16, 62)
+    ln, keep = i32([65, 64, 1 << 30]), 30
+    k, v, table, ms = c.cuda()
+    kept = torch.empty((3, 2, keep), dtype=torch.int32, device="cuda")
+    c.table[2, 3] = c.table[2, 2]                                   # (a page for each of row 2's slots)
+    table.copy_(c.table)
+    ops.paged_select(ms, table, ln.cuda(), kept, first=2, recent=4)
+    assert ops.paged_fault_count(reset=True) == 2
+    exp = po.select(c.mass, c.table, ln, keep, 2, 4)
+    assert torch.equal(kept.cpu().long(), exp)
+    kept[2] = torch.arange(keep, dtype=torch.int32)                 # (nothing moves in the row with a page twice)
+    ops.paged_compact(k, v, table, ln.cuda(), kept, mass=ms)
+    assert ops.paged_fault_count(reset=True) == 2
+    ek, ev, em = po.compact(c.k, c.v, c.mass, c.table, ln.clamp(max=64), kept.cpu().long())
+    assert same(k, ek) and same(v, ev) and same(ms, em)
+    dk = torch.full((4, 2, 80, 64), 3.0, dtype=c.dtype)
+    gk, gv = dk.cuda(), dk.cuda()
+    ops.paged_gather(k, v, table, i32([0, 1, 0, -1]).cuda(), ln.cuda(), gk, gv, extra=9)
+    assert ops.paged_fault_count(reset=True) == 2                   # (row 0, twice)
+    assert same(gk, po.gather(ek, c.table, i32([0, 1, 0, -1]), ln, dk, 9))
