@@ -9,7 +9,7 @@ row takes pages as it grows and gives them back, so memory follows what the rows
     the layers then add up the attention weight every token receives, and each key head keeps tokens of its own.
 
 Decode steps read the pages (b200p_paged_attn); prompts are attended to through a dense view of their rows (b200p_paged_gather) by the
-prompt kernels of dense caches, or token by token where a window hides part of a row.  The device table and counters keep their
+prompt kernels of dense caches, or token by token once the window hides part of a row.  The device table and counters keep their
 addresses, so a captured decode step stays valid while rows grow, shrink and change hands.
 """
 from __future__ import annotations
@@ -240,7 +240,7 @@ class PagedLayer(RowState):
                            mass=self.mass if observed or not book.behind else None, workspace=book.workspace(B, heads, G, D, book.weighed),
                            out_perm=out_perm)
             return
-        if book.window:
+        if book.window and max(self._offsets) + L > book.window + book.first:      # (until then the window hides nothing)
             ops.paged_attn(q, self.kpages, self.vpages, book.table, row, slot, out, scale, first=book.first, window=book.window,
                            workspace=book.workspace(B * L, heads, G, D, 0), out_perm=out_perm)
         else:

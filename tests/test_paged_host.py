@@ -360,3 +360,22 @@ def test_advance_refuses():
     from mlx_parallm_b200 import ops
     with pytest.raises(_lib.B200PError):
         ops.paged_advance(torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 1)
+
+
+@pytest.mark.parametrize("window,first,offset,n,hides", [(40, 0, 0, 40, False), (40, 0, 0, 41, True), (40, 4, 10, 34, False), (40, 4, 10, 35, True),
+                                                        (0, 5, 60, 30, False), (1, 0, 0, 2, True)])
+def test_prompts_whose_window_hides_nothing_go_through_the_dense_view(monkeypatch, window, first, offset, n, hides):
+    """A token at slot s sees all of its row while s < window + first: until then the window takes no prompt from the prompt kernels."""
+    from mlx_parallm_b200.models import paged
+    said = []
+    real = {name: getattr(paged.ops, name) for name in ("paged_append", "paged_gather", "attn", "paged_attn")}
+    b = book(window=window, first=first)
+    layer = paged.PagedLayer(b, 4, 2, 8)
+    layer._offsets = [offset, offset // 2, offset]
+    layer.kpages = torch.zeros(1, dtype=torch.float16)
+    for name in real:
+        monkeypatch.setattr(paged.ops, name, lambda *a, _name=name, **k: said.append(_name))
+    q = torch.empty((3 * n, 32), dtype=torch.float16)
+    t = torch.zeros(3 * n, dtype=torch.int32)
+    layer.append_and_attend(None, q, torch.empty_like(q), (t, t, t), 3, n, 4, None, 1.0, None, None, 1e-6, None, False)
+    assert said == (["paged_append", "paged_attn"] if hides else ["paged_append", "paged_gather", "attn"])
