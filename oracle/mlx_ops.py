@@ -224,9 +224,10 @@ def rope(x, offset, base: float, scale: float = 1.0, dtype: str = "float32") -> 
     return round_to(out, dtype)
 
 
-def sdpa(q, k, v, scale: float, mask=None, dtype: str = "float32") -> np.ndarray:
+def sdpa(q, k, v, scale: float, mask=None, dtype: str = "float32", received=None) -> np.ndarray:
     """mx.fast.scaled_dot_product_attention (A.6; llama.py:139-141, qwen3.py:111-113).
-    q [B,Hq,Lq,D], k/v [B,Hkv,T,D]; GQA: q head h uses kv head h // (Hq/Hkv); fp32 softmax."""
+    q [B,Hq,Lq,D], k/v [B,Hkv,T,D]; GQA: q head h uses kv head h // (Hq/Hkv); fp32 softmax.  ``mask`` additive: [L,T], [B,L,T] or, for masks
+    that differ between kv heads, [B,Hkv,L,T].  ``received`` takes the weights [B,Hkv,Lq,T], summed over the query heads of a kv head."""
     q = np.asarray(q, np.float32)
     k = np.asarray(k, np.float32)
     v = np.asarray(v, np.float32)
@@ -238,11 +239,16 @@ def sdpa(q, k, v, scale: float, mask=None, dtype: str = "float32") -> np.ndarray
     s = np.matmul(qg, k.transpose(0, 1, 3, 2)).reshape(B, Hkv, G, Lq, T)
     if mask is not None:
         m = np.asarray(mask, np.float32)
-        m = m.reshape(m.shape[0], 1, 1, *m.shape[-2:]) if m.ndim == 3 else m.reshape(1, 1, 1, *m.shape[-2:])
+        if m.ndim == 4:
+            m = m[:, :, None]
+        else:
+            m = m.reshape(m.shape[0], 1, 1, *m.shape[-2:]) if m.ndim == 3 else m.reshape(1, 1, 1, *m.shape[-2:])
         s = s + m
     s = s - s.max(-1, keepdims=True)
     p = np.exp(s)
     p = p / p.sum(-1, keepdims=True)
+    if received is not None:
+        received.append(p.sum(2))
     o = np.matmul(p.reshape(B, Hkv, G * Lq, T), v).reshape(B, Hq, Lq, D)
     return round_to(o, dtype)
 

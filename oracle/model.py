@@ -201,7 +201,11 @@ class OracleModel:
         return y
 
     # -- forward ---------------------------------------------------------------------------
-    def forward(self, inputs: np.ndarray, cache: Optional[list] = None, last_only: bool = False) -> np.ndarray:
+    def forward(self, inputs: np.ndarray, cache: Optional[list] = None, last_only: bool = False, visible=None,
+                received: Optional[list] = None) -> np.ndarray:
+        """``visible(layer)`` -> bool [B, Hkv (or 1), L, T], which of the cached tokens a token sees, in place of all before it (the reference
+        has no such mask; caches with a window or evicted tokens are held against it); ``received``: one entry per layer, the weights
+        [B, Hkv, L, T] that the tokens gave."""
         c = self.cfg
         T = c.dtype
         ids = np.asarray(inputs)
@@ -240,7 +244,9 @@ class OracleModel:
             if kv is not None and self.numerics == "reference":
                 cur = "float32"                                          # MLX's promotion
             odt = cur if self.numerics == "reference" else T
-            o = ops.sdpa(q, kf, vf, D ** -0.5, mask, odt)
+            if visible is not None:
+                mask = np.where(visible(i), np.float32(0), np.float32(-1e9))
+            o = ops.sdpa(q, kf, vf, D ** -0.5, mask, odt, received)
             o = o.transpose(0, 2, 1, 3).reshape(B, L, H * D)
             r = self._linear(p + "self_attn.o_proj", o, cur if self.numerics == "reference" else None)
             if self.tp_allreduce is not None:

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from helpers import greedy_report, make_pair, prompts_for, rel_err
-from oracle.model import generate_step as oracle_generate_step
+from oracle.model import OracleModel, generate_step as oracle_generate_step
 
 pytestmark = pytest.mark.gpu
 
@@ -247,3 +247,145 @@ def test_dense_rows_are_not_given_back():
     cfg, _, gm = make_pair("tiny-llama", dtype="float16")
     with pytest.raises(NotImplementedError):
         gm.release_rows(gm.make_cache(2), [1])
+
+
+# ---------------------------------------------------------------- windows, cuts and dense caches, logit by logit
+# Tolerance of the next tests: |engine - oracle| <= |engine - the oracle with the engine's rounding points| + |that - the oracle|.  LOGIT_TOL is for
+# the first; the second is computed.  (bf16 needs it: half a step is 2^-8, and for tiny-qwen3's 61440 logits behind a window the rounding points alone,
+# numerics="mirror", are 0.0053 from the oracle, whose own 16-bit projections are rounded before the norm, behind it and behind the rotation, where the
+# engine rounds once.)
+def mirror_of(om):
+    return OracleModel(om.cfg, om.w, numerics="mirror")
+
+
+def window_mask(L, offset, first, window):
+    """bool [1, 1, L, offset + L]: token t at position offset + t sees j <= its own with j < first or j > its own - window."""
+    s, j = offset + np.arange(L)[:, None], np.arange(offset + L)[None, :]
+    return ((j <= s) & ((j < first) | (j > s - window)))[None, None]
+
+
+@pytest.mark.parametrize("keep", [0, 60], ids=["plain", "weighed"])
+@pytest.mark.parametrize("name,dtype", MODELS)
+def test_logits_behind_a_window(name, dtype, keep):
+    """Prompts that end where the window (16, and 2 first tokens) hides nothing yet, one token further, and long ones, in one piece, in portions and
+    token by token: every position's logits against the oracle under the window's mask."""
+    cfg, om, gm = make_pair(name, dtype=dtype)
+    ids = prompts_for(cfg, 2, 60, seed=21)
+    full = om.forward(ids, om.make_cache(2), visible=lambda layer: window_mask(60, 0, 2, 16))
+    plain = om.forward(ids, om.make_cache(2))
+    assert rel_err(full[:, :18], plain[:, :18]) < 1e-5 and rel_err(full[:, 18:], plain[:, 18:]) > 10 * LOGIT_TOL
+    mi = mirror_of(om)
+    tol = LOGIT_TOL + rel_err(mi.forward(ids, mi.make_cache(2), visible=lambda layer: window_mask(60, 0, 2, 16)), full)
+    t = torch.from_numpy(ids)
+    for cuts in ([18, 19, 20, 44, 45, 46, 60], [19, 60], [5, 18, 19, 60], [60]):
+        cache = gm.make_paged_cache(2, 64, page=16, window=16, first=2, keep=keep)
+        at = [0] + cuts
+        got = torch.cat([gm(t[:, a:b], cache=cache) for a, b in zip(at, at[1:])], 1).cpu().numpy()
+        assert rel_err(got, full) < tol, cuts
+
+
+# What every slot receives, relative to the largest: weights move by twice what their scores do; q and k carry half a step of their type each, of products
+# up to 8.3 in these models (|q| |k| scale), and the layers before them an error below LOGIT_TOL.
+RECEIVED_TOL = {"float16": 3e-2, "float32": 3e-2, "bfloat16": 0.15}
+
+
+@pytest.mark.parametrize("window", [0, 20])
+@pytest.mark.parametrize("name,dtype", [("small-llama", "float16"), ("tiny-qwen3", "bfloat16"), ("tiny-llama", "float32")])
+def test_logits_across_cuts(monkeypatch, name, dtype, window):
+    """Steps through two cuts of full rows.  At each the cache has added up the weights that the oracle gives, keeps what the selection's definition
+    says (the 2 first, the 8 newest, the most attended between, per layer and key head), and afterwards the logits are those of the oracle with everything
+    else hidden and the tokens kept at their positions in the text."""
+    import paged_oracle as po
+    from mlx_parallm_b200 import ops
+    cfg, om, gm = make_pair(name, dtype=dtype)
+    B, prompt, total, keep, observe = 2, 30, 96, 24, 10
+    ids = prompts_for(cfg, B, total, seed=31)
+    cache, oc = gm.make_paged_cache(B, 48, page=16, keep=keep, first=2, recent=8, observe=observe, window=window), om.make_cache(B)
+    mi = mirror_of(om)
+    mc = mi.make_cache(B)
+    G, layers = cache[0].n_kv_heads, len(cache)
+    cut, evict = [], ops.paged_evict
+
+    def spy(k, v, mass, table, lengths, kept, first=0, recent=0):
+        before = [t.cpu().clone() for t in (mass, table, lengths)]
+        evict(k, v, mass, table, lengths, kept, first=first, recent=recent)
+        cut.append((*before, kept.cpu().clone(), first, recent))
+        return kept
+
+    monkeypatch.setattr(ops, "paged_evict", spy)
+    alive = [[[list(range(prompt)) for _ in range(G)] for _ in range(B)] for _ in range(layers)]       # positions, by slot
+    received = [np.zeros((B, G, total)) for _ in range(layers)]
+
+    def seen(layer, n):
+        """Of n tokens, which the token behind them sees."""
+        m = np.zeros((B, G, 1, n + 1), bool)
+        for b in range(B):
+            for g in range(G):
+                a = alive[layer][b][g] + [n]
+                m[b, g, 0, [p for s, p in enumerate(a) if not window or s < 2 or s >= len(a) - window]] = True
+        return m
+
+    gm(torch.from_numpy(ids[:, :prompt]), cache=cache, last_only=True)
+    w = []
+    om.forward(ids[:, :prompt], oc, visible=lambda layer: window_mask(prompt, 0, 2, window or total), received=w)
+    mi.forward(ids[:, :prompt], mc, visible=lambda layer: window_mask(prompt, 0, 2, window or total))
+    for layer in range(layers):
+        received[layer][:, :, :prompt] += w[layer][:, :, -observe:].sum(2)
+    cuts = 0
+    for n in range(prompt, total):
+        got = gm(torch.from_numpy(ids[:, n:n + 1]), cache=cache).cpu().numpy()
+        if cut:
+            assert len(cut) == layers
+            cuts += 1
+            for layer, (mass, table, lengths, kept, first, recent) in enumerate(cut):
+                assert (first, recent) == (2, 8) and lengths.tolist() == [48] * B and kept.shape == (B, G, keep)
+                assert torch.equal(kept.long(), po.select(mass, table, lengths, keep, 2, 8))
+                for b in range(B):
+                    here = torch.cat([mass[p] for p in table[b] if p >= 0], 1)[:, :48].numpy()
+                    for g in range(G):
+                        exp = received[layer][b, g, alive[layer][b][g]]
+                        assert np.abs(here[g] - exp).max() <= RECEIVED_TOL[dtype] * exp.max(), (n, layer, b, g)
+                        assert kept[b, g, :2].tolist() == [0, 1] and kept[b, g, -8:].tolist() == list(range(40, 48))
+                        alive[layer][b][g] = [alive[layer][b][g][s] for s in kept[b, g].tolist()]
+            cut.clear()
+        w = []
+        exp = om.forward(ids[:, n:n + 1], oc, visible=lambda layer: seen(layer, n), received=w)
+        rounded = mi.forward(ids[:, n:n + 1], mc, visible=lambda layer: seen(layer, n))
+        assert rel_err(got, exp) < LOGIT_TOL + rel_err(rounded, exp), n
+        for layer in range(layers):
+            received[layer][:, :, :n + 1] += w[layer][:, :, 0]
+            for b in range(B):
+                for g in range(G):
+                    alive[layer][b][g].append(n)
+        assert cache[0].offsets == [len(alive[0][0][0])] * B and cache[0].book.positions.tolist() == [n + 1] * B
+    assert cuts == 2                                                # at 48 tokens, and 24 further on
+
+
+@pytest.mark.parametrize("name,dtype", MODELS)
+def test_logits_of_dense_caches(name, dtype):
+    """The same prompt, portion and steps over a dense cache and over pages: each within LOGIT_TOL of exact, so twice that of each other."""
+    cfg, _, gm = make_pair(name, dtype=dtype)
+    t = torch.from_numpy(prompts_for(cfg, 3, 40, seed=41))
+    out = []
+    for cache in (gm.make_cache(3), gm.make_paged_cache(3, 40, page=16), gm.make_paged_cache(3, 48, page=48, window=100, keep=40)):
+        out.append(torch.cat([gm(t[:, a:b], cache=cache) for a, b in ((0, 25), (25, 37), (37, 38), (38, 39), (39, 40))], 1).cpu().numpy())
+    print(f"{name} {dtype}: pages against dense {rel_err(out[1], out[0]):.2e} {rel_err(out[2], out[0]):.2e}")
+    assert rel_err(out[1], out[0]) < 2 * LOGIT_TOL and rel_err(out[2], out[0]) < 2 * LOGIT_TOL
+
+
+def test_logits_with_adapters():
+    """LoRA on q and v of every layer, prompts and steps over pages, against the oracle with the same adapters."""
+    from test_gpu_lora import _adapters
+    cfg, om, gm = make_pair("small-llama", dtype="float16")
+    ad = _adapters(cfg, 8, np.random.default_rng(5), layers=range(cfg["num_hidden_layers"]))
+    for k in ad:
+        if k.endswith("lora_a"):
+            pre = k[:-len(".lora_a")]
+            om.lora[pre] = (ad[k].float().numpy(), ad[pre + ".lora_b"].float().numpy(), 10.0)
+    ids = prompts_for(cfg, 2, 24, seed=51)
+    base = gm(torch.from_numpy(ids), cache=gm.make_paged_cache(2, 32, page=16)).cpu().numpy()
+    gm.apply_lora(ad, 10.0)
+    exp = om.forward(ids, om.make_cache(2))
+    cache = gm.make_paged_cache(2, 32, page=16, keep=20)
+    got = torch.cat([gm(torch.from_numpy(ids[:, a:b]), cache=cache) for a, b in ((0, 21), (21, 22), (22, 24))], 1).cpu().numpy()
+    assert rel_err(got, exp) < LOGIT_TOL and rel_err(got, base) > 1e-3
