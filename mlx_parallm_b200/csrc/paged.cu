@@ -265,7 +265,8 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
 // its keys' digits, then adds up all CTAs' counts of its share of the digits through distributed shared memory and hands the sums to the others' copies;
 // the digit in which the need-th lies is found from the sums.  Then each warp counts what it keeps of its slots, and with the counts before it (of the keys
 // equal to the last one the lowest slots are kept) it writes them in order.  Bound by its few barriers: the weights are 4 bytes a slot.
-// (One CTA, 8 bits at a time from global memory: 40001 slots of 8 heads took 230 us.)
+// (One CTA, 8 bits at a time from global memory: 40001 slots of 8 heads took 230 us, now 21.)  Whether the keys are held goes by the table's width,
+// which the host knows, not by the rows' lengths: 64 rows of 4096 of 8 heads take 31.8 us, and 63.6 in a table of 65536 slots.
 constexpr int SEL_MAX_CLUSTER = 8, SEL_BINS = 2048;
 
 struct SelShared {
@@ -442,10 +443,10 @@ paged_select_kernel(const float* mass, PageTable pt, const int32_t* lengths, int
 
 // A CTA or a cluster of them per row, key head and kind (keys or values; the weights go with the keys) closes the kept slots up in rounds: a round's lines
 // go to shared memory, then (everybody has read that round) to their places.  One CTA keeps four rounds of 16 KB under way; a cluster, whose barriers cost 2
-// us, takes rounds of 80 KB (one row of 8 heads cut from 40001 to 5000 tokens, selection and all, in rounds of 16 KB 43 us, 80 KB 38, 160 KB and half the
+// us, takes rounds of 80 KB (one row of 8 heads cut from 40001 to 5000 tokens, selection and all, in rounds of 16 KB 43 us, 80 KB 39, 160 KB and half the
 // CTAs per SM 46).  A slot never moves up and the kept ones ascend, so no later round reads a place that an earlier one wrote.  Where lines come from and
 // go to is looked up for MOVE_LINES of them at once: a look at the list, then the table, then the line, round by round, made every round wait 5 us (16 rows
-// of 8 heads cut from 4096 to 2048 tokens: 160 us, now 69).  Bound by HBM where rows and heads are many.
+// of 8 heads cut from 4096 to 2048 tokens: 160 us, now 70).  Bound by HBM where rows and heads are many.
 constexpr int MOVE_THREADS = 256, MOVE_STAGES = 4, MOVE_LINES = 2048, MOVE_MAX_CLUSTER = 8;
 constexpr int MOVE_UNITS_ONE = 4, MOVE_UNITS_CLUSTER = 20;        // 16-byte pieces of a thread in a round
 // shared memory of a CTA's share: the ring's stages that its rounds use, and the lists of its lines

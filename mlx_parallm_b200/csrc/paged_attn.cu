@@ -82,7 +82,7 @@ struct PagedAttn {
 // The work is cut evenly however unequal the rows are: every token's visible tiles are counted in units of one tile per warp, the units of all
 // (token, key head, block of query heads) items are laid end to end, and each resident CTA takes an equal share of that line.  An item in one share is
 // finished there; of one that is cut every share leaves a part, and a second launch joins them.  (One CTA per item left the GPU idle behind the longest
-// rows: 64 rows of 130 to 500 tokens took 108 us, 16 of 8192 940.  Joining in the CTA whose part comes last, by counters, cost a row of 1000 tokens 3.7 us
+// rows: 64 rows of 128 to 500 tokens took 108 us, 16 of 8192 940.  Joining in the CTA whose part comes last, by counters, cost a row of 1000 tokens 3.7 us
 // of fences and atomics in a row; the second launch costs it less.  SMs differ by a quarter in what they get of the memory's bandwidth, so that of 16 rows of
 // 8192 tokens the first CTAs are done after 63 us and the last after 90; a counter of small shares for whoever comes first evened that out but cost more than
 // it gave: 106 us in all against 95.)
@@ -106,8 +106,8 @@ constexpr int PA_TOKENS = 512;         // up to so many tokens a CTA keeps all o
 
 // Where every CTA's share is long (PA_LAST_UNITS units, some 50 us in all) it gives a part away: PA_LAST_PERCENT of the line, its end, is cut into small
 // shares for 3/4 as many more CTAs, which the hardware starts where the first ones have ended.  (16 rows of 8192 tokens 95.1 -> 90.0 us, 128 of 1000
-// 96.1 -> 90.9, 64 of 1000 52.4 -> 51.8; 64 of 500, below the bound, 31.3, and 33.5 with it.  CTAs that find no share, where the table has room for long rows
-// and the rows are short: 0.3 us at most.)
+// 96.1 -> 90.9, 64 of 1000 52.4 -> 51.8 in a captured graph; launched one by one 16 of 8192 96.0 -> 94.2.  64 of 500, below the bound, 31.3, and 33.5 with it.
+// CTAs that find no share, where the table has room for long rows and the rows are short: 0.3 us at most.)
 constexpr int PA_LAST_UNITS = 24, PA_LAST_PERCENT = 12;
 __host__ __device__ inline int last_ctas(int ctas) { return ctas * 3 / 4; }
 
@@ -884,7 +884,7 @@ paged_attn_join_kernel(const __grid_constant__ PagedAttn a, int rows_log2) {
 // sums come from the parts again (a warp per head, a lane per part), which needs no word from the join.  The slices of a row's first token in the call do so
 // for all of the row's tokens and all of their heads in turn, the others leave, so that a slot's weights are added by one thread in one order (unless rows
 // share its page).
-// 12 rows of 3333 tokens, 64 heads: 26.1 us for the launch before, 5.8 for this one (9.0 with a CTA for every head).  (Atomics of all tokens at once took 1.4
+// 12 rows of 972 to 3333 tokens, 64 heads: 26.1 us for the launch before, 5.8 for this one (9.0 with a CTA for every head).  (Atomics of all tokens at once took 1.4
 // less there, and 50 for the last 32 of 2048 tokens instead of 115; four tokens of a row at a time 88 there, but 2 more for the 12 rows.)
 template <typename T, int NQ, int ROWS>
 __global__ void __launch_bounds__(256)

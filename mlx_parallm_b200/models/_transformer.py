@@ -367,7 +367,8 @@ class DecoderModel:
         """A cache in pages (models/paged.py) for ``batch_size`` rows of up to ``max_tokens`` tokens, drawn from ``pages`` pages of ``page`` tokens
         (None: as many as all rows need).  ``window`` > 0: a token sees the last ``window`` tokens and the ``first`` first ones.  ``keep`` > 0: a row
         that is full is cut to ``keep`` tokens, the ``first`` first, the ``recent`` newest (None: half of the others) and the most attended
-        ones; the weights of decode steps and of a prompt's last ``observe`` tokens count."""
+        ones; the weights of decode steps and of a prompt's last ``observe`` tokens count.  (Left padding is fed as tokens: the first tokens of a padded row
+        are its padding.)"""
         if self.device is None:
             raise RuntimeError("load the model's weights first")
         book = PageBook(batch_size, max_tokens, self.device, page, pages, window, first, keep, recent, observe)
