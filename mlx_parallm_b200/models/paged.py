@@ -190,6 +190,8 @@ class PagedLayer(RowState):
         self.book.revive()
 
     def release_rows_host(self, rows: List[int]):
+        if any(not 0 <= r < self.batch_size for r in rows):
+            raise ValueError(f"rows of this cache are 0 to {self.batch_size - 1}: got {list(rows)}")
         super().release_rows_host(rows)
         for r in rows:
             self.book.evicted[r] = 0

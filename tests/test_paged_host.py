@@ -353,6 +353,23 @@ def test_a_row_that_was_given_back_takes_no_page_again():
     assert [len(o) for o in b.owned] == [1, 1] and layers[0].offsets == [5, 5]
 
 
+@pytest.mark.parametrize("rows", [[1, 3], [0, -1], [7]], ids=str)
+def test_rows_that_do_not_exist_are_not_given_back(rows):
+    """Refused before anything of the others is given back."""
+    from mlx_parallm_b200.models._transformer import release_rows
+    from mlx_parallm_b200.models.paged import PagedLayer
+    b = book()
+    layers = [PagedLayer(b, 4, 2, 64) for _ in range(2)]
+    for c in layers:
+        c._offsets = [5, 20, 9]
+    b.room_for([5, 20, 9])
+    layers[0]._sync_lengths()
+    with pytest.raises(ValueError):
+        release_rows(layers, rows)
+    assert all(c.offsets == [5, 20, 9] for c in layers) and b.lengths.tolist() == [5, 20, 9] and b.row_index.tolist() == [0, 1, 2]
+    assert [len(o) for o in b.owned] == [1, 2, 1]
+
+
 def test_advance_refuses():
     f = L().b200p_paged_advance
     assert f(0, OK, OK, 4, 1, 0) == ARG and f(OK, 0, OK, 4, 1, 0) == ARG and f(OK, OK, 0, 4, 1, 0) == ARG and f(OK, OK, OK, -1, 1, 0) == ARG
