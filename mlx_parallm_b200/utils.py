@@ -414,6 +414,18 @@ def generate_step(
 
 
 # --------------------------------------------------------------------------------- text front-ends
+def _first_tokens(run, n: int):
+    """zip(run, range(n)), which looks for one token more than it gives: the step that runs ahead of it is launched, and its random numbers are
+    used up.  A cache in pages that has no room for that step has given all that was asked for."""
+    for i in range(n):
+        yield next(run), i
+    try:
+        next(run)
+    except PagesExhausted:
+        if n == 0:
+            raise
+
+
 def stream_generate(model, tokenizer, prompt: str, max_tokens: int = 100, **kwargs):
     """utils.py:429-471."""
     if not isinstance(tokenizer, TokenizerWrapper):
@@ -422,7 +434,7 @@ def stream_generate(model, tokenizer, prompt: str, max_tokens: int = 100, **kwar
     detokenizer = tokenizer.detokenizer
     detokenizer.reset()
     kwargs = _presize(kwargs, model, prompt_tokens, max_tokens)
-    for (token, prob), n in zip(generate_step(prompt_tokens, model, **kwargs), range(max_tokens)):
+    for (token, prob), n in _first_tokens(generate_step(prompt_tokens, model, **kwargs), max_tokens):
         token_item = token.item()
         if token_item == tokenizer.eos_token_id:
             break
@@ -447,7 +459,7 @@ def generate(model, tokenizer, prompt: str, max_tokens: int = 100, verbose: bool
     n = -1
     prompt_time = 0.0
     kwargs = _presize(kwargs, model, prompt_tokens, max_tokens)
-    for (token, prob), n in zip(generate_step(prompt_tokens, model, **kwargs), range(max_tokens)):
+    for (token, prob), n in _first_tokens(generate_step(prompt_tokens, model, **kwargs), max_tokens):
         if n == 0:
             prompt_time = time.perf_counter() - tic
             tic = time.perf_counter()
@@ -499,7 +511,7 @@ def batch_generate(model, tokenizer, prompts: List[str], max_tokens: int = 100, 
     output_toks = []
     prompt_time = 0.0
     kwargs = _presize(kwargs, model, prompts_toks, max_tokens)
-    for (tokens, _), n in zip(generate_step(prompts_toks, model, **kwargs), range(max_tokens)):
+    for (tokens, _), n in _first_tokens(generate_step(prompts_toks, model, **kwargs), max_tokens):
         if n == 0:
             tokens[0, 0].item()                      # first token materialised = prefill done
             prompt_time = time.perf_counter() - tic
@@ -532,7 +544,7 @@ def batch_stream_generate_text(model, tokenizer, prompts_tokens, max_tokens: int
     counts = [0] * batch_size
     eos_token_id = tokenizer.eos_token_id
     gs_kwargs = _presize({k: v for k, v in kwargs.items() if k != "repetition_penalty"}, model, prompts_tokens, max_tokens)
-    for (batch_next, _), _ in zip(generate_step(prompts_tokens, model, **gs_kwargs), range(max_tokens)):
+    for (batch_next, _), _ in _first_tokens(generate_step(prompts_tokens, model, **gs_kwargs), max_tokens):
         ids = batch_next.view(-1).tolist()           # ONE D2H per step (the reference does B .item() syncs)
         deltas: List[Tuple[Optional[str], Optional[str]]] = [(None, None)] * batch_size
         any_active = False

@@ -249,6 +249,23 @@ def test_dense_rows_are_not_given_back():
         gm.release_rows(gm.make_cache(2), [1])
 
 
+def test_front_ends_use_the_last_place():
+    """prompt + max_tokens - 1 places: the last token needs none."""
+    from fake_tokenizer import FakeTokenizer
+    from mlx_parallm_b200.tokenizer_utils import TokenizerWrapper
+    from mlx_parallm_b200.utils import batch_generate, batch_stream_generate_text, generate, stream_generate
+    cfg, _, gm = make_pair("tiny-llama", dtype="float16")
+    ids = prompts_for(cfg, 2, 28)
+    texts = [" ".join(f"w{i}" for i in row) for row in ids]
+    tok = TokenizerWrapper(FakeTokenizer(cfg["vocab_size"], eos_token_id=cfg["vocab_size"] + 1))      # (never said)
+    make = lambda rows: gm.make_paged_cache(rows, 48, page=16)
+    assert len(generate(gm, tok, texts[0], max_tokens=21, cache=make(1)).split()) == 21
+    assert len("".join(stream_generate(gm, tok, texts[0], max_tokens=21, cache=make(1))).split()) == 21
+    assert [len(t.split()) for t in batch_generate(gm, tok, texts, max_tokens=21, format_prompts=False, cache=make(2))] == [21, 21]
+    said = list(batch_stream_generate_text(gm, tok, ids, 21, cache=make(2)))
+    assert len(said) == 21 and all(reason == "length" for _, reason in said[-1])
+
+
 # ---------------------------------------------------------------- windows, cuts and dense caches, logit by logit
 # Tolerance of the next tests: |engine - oracle| <= |engine - the oracle with the engine's rounding points| + |that - the oracle|.  LOGIT_TOL is for
 # the first; the second is computed.  (bf16 needs it: half a step is 2^-8, and for tiny-qwen3's 61440 logits behind a window the rounding points alone,

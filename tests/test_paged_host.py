@@ -396,3 +396,35 @@ def test_prompts_whose_window_hides_nothing_go_through_the_dense_view(monkeypatc
     t = torch.zeros(3 * n, dtype=torch.int32)
     layer.append_and_attend(None, q, torch.empty_like(q), (t, t, t), 3, n, 4, None, 1.0, None, None, 1e-6, None, False)
     assert said == (["paged_append", "paged_attn"] if hides else ["paged_append", "paged_gather", "attn"])
+
+
+@pytest.mark.parametrize("n", [1, 2, 6])
+def test_front_ends_end_with_all_of_their_tokens(monkeypatch, n):
+    """prompt + n - 1 places are enough for n tokens, through a front-end too: it looks for one token more (the step that runs ahead, whose random
+    numbers later generations do not share) and misses nothing."""
+    from fake_tokenizer import FakeTokenizer
+    from mlx_parallm_b200 import utils
+    from mlx_parallm_b200.models.paged import PagesExhausted
+    monkeypatch.setattr(utils.ops, "check_waits", lambda: None)
+    step = _Step(n - 1)
+    monkeypatch.setattr(utils, "_decode_step_for", lambda *a: step)
+    cache = [type("C", (), {"_lengths": 1})()]
+    tok = utils.TokenizerWrapper(FakeTokenizer(1000))
+    words = " ".join(f"w{i}" for i in range(10, 10 + n))
+    kw = dict(max_tokens=n, cache=cache)
+
+    def again():
+        step.n = 0
+        return step
+
+    assert again() and utils.generate(_Model(), tok, "w1 w2", **kw) == words
+    assert again() and "".join(utils.stream_generate(_Model(), tok, "w1 w2", **kw)).split() == words.split()
+    assert again() and utils.batch_generate(_Model(), tok, ["w1 w2"], format_prompts=False, **kw) == [words]
+    assert again() and len(list(utils.batch_stream_generate_text(_Model(), tok, [[1, 2]], **kw))) == n
+    with pytest.raises(PagesExhausted):
+        again() and utils.generate(_Model(), tok, "w1 w2", max_tokens=n + 1, cache=cache)
+    # the step ahead of the last token is launched as ever
+    for room, steps in ((50, n + 1), (n, n)):
+        again().room = room
+        utils.generate(_Model(), tok, "w1 w2", **kw)
+        assert step.n == steps
