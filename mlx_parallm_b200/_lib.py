@@ -53,6 +53,7 @@ SIGNATURES = {
     "b200p_argmax_partial": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "b200p_argmax_merge": (_i32, [_vp, _vp, _vp, _i32, _i64, _vp]),
     "b200p_sample_top_p": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _f32, _f32, _u64, _u64, _vp]),
+    "b200p_token_logprobs": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _f32, _i32, _vp]),
     "b200p_symm_alloc": (_i32, [C.POINTER(_vp), _sz]),
     "b200p_symm_free": (_i32, [_vp]),
     "b200p_ipc_export": (_i32, [_vp, _vp]),
@@ -155,14 +156,14 @@ SIGNATURES = {
 # Translation units a model family needs (csrc/*.cu): the library can be linked from a subset, so that a fresh checkout
 # that serves one design compiles that design's kernels only.  ``None`` = every unit (libb200parallm.so).
 UNIT_SETS = {
-    "sequence": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "delta_rule", "latent_attn", "sampler"),
-    "sequence_moe": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "delta_rule", "sink_attn", "moe", "sampler"),
-    "sequence_ssm": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "delta_rule", "ssm", "diff_attn", "moe", "sampler"),
+    "sequence": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "delta_rule", "latent_attn", "sampler", "logprobs"),
+    "sequence_moe": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "delta_rule", "sink_attn", "moe", "sampler", "logprobs"),
+    "sequence_ssm": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "delta_rule", "ssm", "diff_attn", "moe", "sampler", "logprobs"),
     "sequence_hyper": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "hyper", "delta_rule", "latent_attn", "sink_attn", "moe",
-                       "sampler"),
+                       "sampler", "logprobs"),
     "sequence_post": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "post_norm", "latent_attn", "row_attn_prep", "mix_attn", "moe",
-                      "sampler"),
-    "sequence_rows": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "row_attn_prep", "sink_attn", "moe", "sampler"),
+                      "sampler", "logprobs"),
+    "sequence_rows": ("runtime", "dense_gemm", "dense_gemm_tc", "ragged", "row_attn_prep", "sink_attn", "moe", "sampler", "logprobs"),
 }
 GEMM_STORE, GEMM_STORE_F32, GEMM_GLU_CLAMP, GEMM_GLU_GELU_TANH, GEMM_GLU_SILU, GEMM_RELU_SQ, GEMM_XIELU, GEMM_CAP_F32 = 0, 1, 2, 3, 4, 5, 6, 7
 GEMM_CHAINED = 0x100                                # b200p_gemm: other kernels surround the product (include/b200p.h)

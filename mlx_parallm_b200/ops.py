@@ -6,7 +6,7 @@ none of them has a CPU or eager-PyTorch fallback -- a CPU tensor raises.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import os
 
@@ -265,6 +265,47 @@ def sample_top_p(logits, temperature, top_p, seed, offset, out=None, probs_out=N
         out = torch.empty((B,), dtype=torch.int32, device=logits.device)
     _call("b200p_sample_top_p", lambda: lib().b200p_sample_top_p(_p(logits), _p(out), _p(probs_out), B, V, logits.stride(0), float(temperature),
                                    float(top_p), int(seed) & (2**64 - 1), int(offset) & (2**64 - 1), _stream()))
+    return out
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs gives for M rows of logits."""
+    logprob: Optional[torch.Tensor]           # float32 [M]: of the given tokens (None: none were given)
+    entropy: torch.Tensor                     # float32 [M]
+    top_ids: torch.Tensor                     # int32 [M, top]: the most likely tokens, the lowest id first among equal ones
+    top_logprobs: torch.Tensor                # float32 [M, top]
+
+
+def token_logprobs(logits, tokens=None, top: int = 0, temperature: float = 1.0, out: Optional[TokenLogprobs] = None) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` (int32 [M]; negative: no token, 0) under softmax(logits / temperature), every row's entropy and its ``top`` <= 32 most
+    likely tokens (b200p_token_logprobs).  ``logits`` [M, V] float32, float16 or bfloat16, a slice of columns or a row stride are fine."""
+    dev = logits.get_device()
+    if dev < 0 or dev != _device_index() or (tokens is not None and tokens.get_device() != dev):
+        _dev(logits, tokens)
+        raise ValueError("logits and tokens lie on the current device")
+    if logits.dim() != 2:
+        raise ValueError(f"logits are [M, V]: got {tuple(logits.shape)}")
+    (M, V), (ld, inner) = logits.shape, logits.stride()
+    if (V > 1 and inner != 1) or (M > 1 and ld < V):
+        raise ValueError(f"rows of logits have neighbouring columns and do not overlap: got strides {logits.stride()}")
+    if tokens is not None and (tokens.dtype is not torch.int32 or tokens.numel() != M or not tokens.is_contiguous()):
+        raise ValueError(f"tokens are int32 [{M}]: got {tokens.dtype} {tuple(tokens.shape)}")
+    if out is None:
+        if not 0 <= top <= V:
+            raise ValueError(f"{top} alternatives of {V}")
+        at = logits.device
+        out = TokenLogprobs(None if tokens is None else torch.empty(M, dtype=torch.float32, device=at), torch.empty(M, dtype=torch.float32, device=at),
+                            torch.empty((M, top), dtype=torch.int32, device=at), torch.empty((M, top), dtype=torch.float32, device=at))
+    else:
+        if (out.logprob is None) != (tokens is None):
+            raise ValueError("logprob belongs to tokens")
+        for t, shape, dt in ((out.logprob, (M,), torch.float32), (out.entropy, (M,), torch.float32), (out.top_ids, (M, top), torch.int32),
+                             (out.top_logprobs, (M, top), torch.float32)):
+            if t is not None and (t.shape != shape or t.dtype is not dt or not t.is_contiguous() or t.get_device() != dev):
+                raise ValueError(f"an output is {dt} {shape} beside the logits: got {t.dtype} {tuple(t.shape)}")
+    _call("b200p_token_logprobs", lambda: lib().b200p_token_logprobs(
+        logits.data_ptr(), _p(tokens), _p(out.logprob), out.entropy.data_ptr(), out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), M, V,
+        ld if M > 1 else V, top, float(temperature), dtype_code(logits.dtype), _stream()))
     return out
 
 
