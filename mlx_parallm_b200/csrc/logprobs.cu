@@ -23,10 +23,11 @@ namespace b200p {
 
 int sm_count();
 
-constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
+constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_TOP = 32;             // alternatives at most: a group of threads each, and a rank that a warp can hold
 constexpr int LP_CLUSTER = 8;
-constexpr int LP_GROUPS = LP_WARPS * LP_CLUSTER;
+constexpr int LP_GROUPS = 64;
+static_assert(LP_WARPS * LP_CLUSTER == LP_GROUPS, "a warp is a group in the largest cluster");
 constexpr int LP_LIST = 1024;          // values that reach the bound; more are selected from digit by digit
 
 __device__ __forceinline__ float lp_exp2(float x) {
@@ -130,7 +131,7 @@ __device__ __noinline__ void lp_select(const RowParts<T>& p, LpShared& s, int k)
   if (threadIdx.x == 0) s.prefix = 0u, s.need = k;
 #pragma unroll 1
   for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) s.hist[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < 256; i += LP_THREADS) s.hist[i] = 0;
     __syncthreads();
     const uint32_t prefix = s.prefix;
     auto count = [&](float x, bool here) {                          // by whole warps
@@ -199,7 +200,7 @@ __device__ __noinline__ void lp_first_equal(const RowParts<T>& p, LpShared& s, i
 
 // grid (S * rows), clusters of S.  512 threads: two CTAs of an SM take turns, one streams while the other ends its row.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 2)
+__global__ void __launch_bounds__(LP_THREADS, 4)
 token_logprobs_kernel(const __grid_constant__ LogProbs a) {
   __shared__ LpShared s;
   cg::cluster_group cluster = cg::this_cluster();
@@ -249,7 +250,7 @@ token_logprobs_kernel(const __grid_constant__ LogProbs a) {
   // ---- the threads' maxima and sums become the row's ------------------------------------------------------------------------
   const float mine = sum.m;
   float high = mine;
-  const int lanes = S == 1 ? 8 : S == 2 ? 16 : 32;                  // of a group: 64 groups, 128 of 8 CTAs
+  const int lanes = 32 / LP_CLUSTER * (int)S;                       // of a group
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     if (TOP && o == lanes && (lane & (lanes - 1)) == 0) s.group[rank * (LP_THREADS / lanes) + threadIdx.x / lanes] = high;
@@ -363,7 +364,7 @@ token_logprobs_kernel(const __grid_constant__ LogProbs a) {
 template <typename T>
 static int launch_logprobs(const LogProbs& a, int64_t M, cudaStream_t st) {
   int S = LP_CLUSTER;
-  while (S > 1 && M * S > 2 * sm_count()) S >>= 1;                  // one wave
+  while (S > 1 && M * S > 4 * sm_count()) S >>= 1;                  // one wave
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(M * S));
   cfg.blockDim = dim3(LP_THREADS);
