@@ -6,10 +6,9 @@
 // t = sum e_i u_i, which become f s and f (t + d s) when m grows by -d and f = exp(d / T).  Then log p_i = (x_i - m) / T - log s and
 // H = log s - t / (T s).  All of it is fp32; nothing of the row is written.
 //
-// The alternatives come out of the same pass: the k-th largest of the maxima of 64 groups of threads (128 in clusters of 8) is no larger than the
-// row's k-th largest value, and only few values are as large (some 24 for k = 20).  A thread whose maximum reaches it has its values read
-// again, a lane per vector; what reaches the bound goes into a list, which is ranked by counting.  Rows in which too many do
-// (equal values) are selected from digit by digit.
+// The alternatives come out of the same pass: the k-th largest of the maxima of 64 groups of threads is no larger than the row's k-th largest
+// value, and only few values are as large (some 24 for k = 20).  A thread whose maximum reaches it has its values read again, a lane per vector; what reaches
+// the bound goes into a list, which is ranked by counting.  Rows in which too many do (equal values) are selected from digit by digit.
 //
 // A row is split over the CTAs of a cluster where the rows are few, as in sampler.cu.
 #include <cooperative_groups.h>
@@ -105,7 +104,7 @@ struct LpSums {
 struct LpShared {
   float4 part[LP_WARPS > LP_CLUSTER ? LP_WARPS : LP_CLUSTER];      // m, s, t of the warps, then (in the first CTA) of the cluster's CTAs
   float4 cta[LP_CLUSTER];
-  float group[LP_GROUPS];
+  alignas(16) float group[LP_GROUPS];
   float bound, m, log_s;
   int count;
   uint2 list[LP_LIST];                 // key and index
@@ -198,7 +197,10 @@ __device__ __noinline__ void lp_first_equal(const RowParts<T>& p, LpShared& s, i
   }
 }
 
-// grid (S * rows), clusters of S.  512 threads: two CTAs of an SM take turns, one streams while the other ends its row.
+// grid (S * rows), clusters of S: as many CTAs to a row as fit the GPU side by side, four per SM, with two vectors or more for a thread (us, device: 1 row of
+// 128256 in 1 / 2 / 4 / 8 CTAs, 20 alternatives 20.6 / 13.2 / 8.4 / 6.7; 64 rows of 32000 bf16 without 4.9 / 4.0 / 3.8 / 5.2; 333 rows of 50257 bf16
+// 13.4 / 14.2 / 15.8 / 20.3).  Four CTAs of 256 threads and not two of 512: 333 rows with 8 alternatives 22.0 -> 17.1, 1500 rows of 151936 144.6 -> 139.9,
+// 99 % of the copy's bandwidth.  (Eight vectors of a thread under way through shared memory instead of four through registers gave nothing.)
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_THREADS, 4)
 token_logprobs_kernel(const __grid_constant__ LogProbs a) {
@@ -295,13 +297,14 @@ token_logprobs_kernel(const __grid_constant__ LogProbs a) {
   if (!TOP) return;
 
   // ---- the bound, and what reaches it ----------------------------------------------------------------------------------------
-  const int n = groups * (int)S;
-  if ((int)threadIdx.x < n) {
+  if (threadIdx.x < LP_GROUPS) {
     const float x = s.group[threadIdx.x];
     int above = 0;
-    for (int j = 0; j < n; ++j) {
-      const float y = s.group[j];
-      above += y > x || (y == x && j < (int)threadIdx.x);
+#pragma unroll
+    for (int j = 0; j < LP_GROUPS; j += 4) {
+      const float4 y = *reinterpret_cast<const float4*>(s.group + j);
+      above += (y.x > x || (y.x == x && j < (int)threadIdx.x)) + (y.y > x || (y.y == x && j + 1 < (int)threadIdx.x)) +
+               (y.z > x || (y.z == x && j + 2 < (int)threadIdx.x)) + (y.w > x || (y.w == x && j + 3 < (int)threadIdx.x));
     }
     if (above == a.top - 1) s.bound = x;
   }
@@ -364,7 +367,8 @@ token_logprobs_kernel(const __grid_constant__ LogProbs a) {
 template <typename T>
 static int launch_logprobs(const LogProbs& a, int64_t M, cudaStream_t st) {
   int S = LP_CLUSTER;
-  while (S > 1 && M * S > 4 * sm_count()) S >>= 1;                  // one wave
+  const int64_t vectors = a.V / RowParts<T>::E;
+  while (S > 1 && (M * S > 4 * sm_count() || vectors < 2 * S * LP_THREADS)) S >>= 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(M * S));
   cfg.blockDim = dim3(LP_THREADS);
