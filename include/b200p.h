@@ -164,6 +164,21 @@ int b200p_silu_mul(float* gu, void* out, int64_t M, int64_t I, int64_t ldg, int6
  * is rounded to `dtype` first, as MLX's astype does).  16-bit types only. */
 int b200p_lora_add(const void* x, const void* At, const void* Bt, void* y, int64_t M, int64_t N, int64_t K, int64_t ldx,
                    int64_t ldy, int64_t col0, float scale, int dtype, int out_f32, void* stream);
+/* Rows of a batch in the order of a group each (adapters, shared prompts): plan int32 = [tiles, rows in groups, rows whose index is behind the last group,
+ * tile | the rows in order | per tile of up to `tile` rows of one group: group, first place in the order, rows, the group's first place].  index int32 [M]: a
+ * row's group, negative: none (so is one behind the last).  A plan stays good until index changes; `plan_ints` >= b200p_row_groups_ints(M, groups, tile),
+ * 16-byte aligned.  M <= 2^20, groups <= 1024. */
+int b200p_row_groups(const int32_t* index, int32_t* plan, int64_t M, int groups, int tile, int64_t plan_ints, void* stream);
+int64_t b200p_row_groups_ints(int64_t M, int64_t groups, int64_t tile);      /* 0: no such plan */
+/* LoRA with an adapter of its own for every row:  y[m, columns of target t] += scales[i] * (x[m] . A[i, t]^T) . B[i]^T, i = the row's group in `plan`; rows
+ * without one are not touched.  x `dtype` (16-bit) [M, K] (row stride ldx); a `dtype` [adapters, targets, R, K] (lora_a transposed; its k axis permuted like x
+ * when x is PERM8), b `dtype` [adapters, sum of the targets' columns, R] (lora_b transposed, target after target), the ranks filled up to R, a multiple of 16,
+ * with zeros; targets * R <= 256.  host_columns (host memory) = first column in y and number of columns (a multiple of 8) of every target, which do not
+ * overlap; y float (y_f32) or `dtype`, row stride ldy.  Sums are fp32, y is rounded once.  `tile` is the plan's: 16 or 64, b200p_lora_rows_tile(M, adapters)
+ * the better one.  K a multiple of 8; x, its rows, a, b and plan 16-byte aligned; ldy and first columns multiples of 4, y aligned to four elements. */
+int b200p_lora_rows(const void* x, const int32_t* plan, const void* a, const void* b, const float* scales, void* y, const int32_t* host_columns, int64_t M,
+                    int adapters, int tile, int targets, int R, int64_t K, int64_t ldx, int64_t ldy, int dtype, int y_f32, void* stream);
+int b200p_lora_rows_tile(int64_t M, int groups);
 /* Rows that b200p_rope_kv_append could NOT append because lengths[b] + l reached Tcap (their K / V are dropped and the
  * attention of that step reads a stale slot): *count = number of (token, V head) pairs since the last reset on the current
  * device; reset != 0 clears it.  Synchronises `stream`; not capturable.  The Python surface (models/base.py) grows the cache

@@ -43,6 +43,10 @@ SIGNATURES = {
                                     _f32, _f32, _f32, _i32, _i32, _vp]),
     "b200p_silu_mul": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _vp]),
     "b200p_lora_add": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _vp]),
+    "b200p_row_groups_ints": (_i64, [_i64, _i64, _i64]),
+    "b200p_row_groups": (_i32, [_vp, _vp, _i64, _i32, _i32, _i64, _vp]),
+    "b200p_lora_rows_tile": (_i32, [_i64, _i32]),
+    "b200p_lora_rows": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _vp]),
     "b200p_advance_lengths": (_i32, [_vp, _i64, _i32, _vp]),
     "b200p_kv_overflow_count": (_i32, [C.POINTER(C.c_uint), _i32, _vp]),
     "b200p_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i64, _f32, _i32, _i32, _vp, _sz, _vp]),

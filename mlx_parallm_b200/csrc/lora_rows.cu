@@ -1,0 +1,389 @@
+// Low-rank updates with an adapter of its own for every row (b200p_row_groups, b200p_lora_rows): requests under many adapters in one batch.
+//
+//   y[m, columns of target t] += s_i ((x_m A_{i,t}^T) B_{i,t}^T),   i = the row's adapter; rows without one stay as they are
+//
+// The rows are put in the order of their adapters once per batch (row_groups_kernel); the layers then go by tiles of 16 or 64 rows of one adapter.
+// A cluster of CTAs has a tile: every CTA takes a part of K for z = x A^T, the parts meet through distributed shared memory, and every CTA has all of
+// z for its part of the columns.  So both products are one launch, an adapter is read once for a tile, and even a single row has eight SMs.
+// z is fp32; for the second product its rows are scaled by a power of two and split into two f16 or three bf16 numbers, which carry 22 and 24 of its bits,
+// so that the update is as exact as its sums; it is added to y in fp32 and rounded once where y is 16-bit.
+#include <cooperative_groups.h>
+
+#include <atomic>
+
+#include "mma_util.cuh"
+#include "rowgroups.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace b200p {
+
+int sm_count();
+
+// ------------------------------------------------------------------------------------------------ the plan
+constexpr int RG_WARPS = 16;
+
+// A stable counting sort by one CTA: every warp counts its run of rows by group, the counts become places, and the warps go over their rows again.
+// (8000 rows of 7 groups: a launch per batch, not per layer.)
+__global__ void __launch_bounds__(RG_WARPS * 32)
+row_groups_kernel(const int32_t* index, int32_t* plan, int M, int groups, int tile) {
+  extern __shared__ int s_count[];               // [RG_WARPS][groups]
+  __shared__ int s_begin[RG_GROUPS], s_tile[RG_GROUPS], s_size[RG_GROUPS], s_bad;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  for (int i = threadIdx.x; i < RG_WARPS * groups; i += RG_WARPS * 32) s_count[i] = 0;
+  if (threadIdx.x == 0) s_bad = 0;
+  __syncthreads();
+  const int run = (M + RG_WARPS * 32 - 1) / (RG_WARPS * 32) * 32, r0 = min(M, warp * run), r1 = min(M, r0 + run);
+  int* count = s_count + warp * groups;
+  for (int base = r0; base < r1; base += 32) {
+    const int i = base + lane, g = i < r1 ? index[i] : -1;
+    const unsigned same = __match_any_sync(~0u, g), bad = __ballot_sync(~0u, g >= groups);
+    if (g >= 0 && g < groups && lane == __ffs(same) - 1) count[g] += __popc(same);
+    if (bad && lane == 0) atomicAdd(&s_bad, __popc(bad));
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < groups; g += RG_WARPS * 32) {
+    int sum = 0;
+    for (int w = 0; w < RG_WARPS; ++w) {
+      const int n = s_count[w * groups + g];
+      s_count[w * groups + g] = sum;
+      sum += n;
+    }
+    s_size[g] = sum;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int rows = 0, tiles = 0;
+    for (int base = 0; base < groups; base += 32) {
+      const int g = base + lane, n = g < groups ? s_size[g] : 0, k = (n + tile - 1) / tile;
+      int a = n, b = k;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(~0u, a, o), y = __shfl_up_sync(~0u, b, o);
+        if (lane >= o) a += x, b += y;
+      }
+      if (g < groups) s_begin[g] = rows + a - n, s_tile[g] = tiles + b - k;
+      rows += __shfl_sync(~0u, a, 31), tiles += __shfl_sync(~0u, b, 31);
+    }
+    if (lane == 0) plan[0] = tiles, plan[1] = rows, plan[2] = s_bad, plan[3] = tile;
+  }
+  __syncthreads();
+  int32_t* order = plan + RG_HEAD;
+  int4* tiles = reinterpret_cast<int4*>(order + (M + 3) / 4 * 4);
+  for (int g = threadIdx.x; g < groups; g += RG_WARPS * 32)
+    for (int k = 0; k * tile < s_size[g]; ++k) tiles[s_tile[g] + k] = make_int4(g, s_begin[g] + k * tile, min(tile, s_size[g] - k * tile), s_begin[g]);
+  for (int base = r0; base < r1; base += 32) {
+    const int i = base + lane, g = i < r1 ? index[i] : -1;
+    const bool in = g >= 0 && g < groups;
+    const unsigned same = __match_any_sync(~0u, g);
+    if (in) order[s_begin[g] + count[g] + __popc(same & ((1u << lane) - 1u))] = i;
+    __syncwarp();
+    if (in && lane == __ffs(same) - 1) count[g] += __popc(same);
+    __syncwarp();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the update
+constexpr int LW_WARPS = 8, LW_THREADS = LW_WARPS * 32;
+constexpr int LW_TARGETS = 4, LW_CLUSTER = 8, LW_RANKS = 256;     // targets, CTAs of a tile, ranks of all targets at most
+
+struct LoraRows {
+  const void *x, *a, *b;
+  const float* scales;
+  void* y;
+  RowGroups plan;
+  int64_t ldx, ldy;
+  int K, R, N, targets, steps;                   // rank of a target, columns of all targets, 32 of K each
+  int col0[LW_TARGETS], start[LW_TARGETS + 1], tile0[LW_TARGETS + 1];      // first column of y, of b; first run of 16 columns
+};
+
+template <typename T> struct LwParts { static constexpr int N = 2; };
+template <> struct LwParts<__nv_bfloat16> { static constexpr int N = 3; };
+// a row's room for its parts of z, which the split z takes over
+template <typename T>
+__host__ __device__ constexpr int lw_part_floats(int ranks) {
+  return LwParts<T>::N * (ranks + 8) / 2 > LW_WARPS * 32 ? LwParts<T>::N * (ranks + 8) / 2 : LW_WARPS * 32;
+}
+
+// MB blocks of 16 rows; YT: y's type.  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits this CTA's part of K.
+// Operands come straight from memory, 16 bytes a lane: the order of k within a product is free as long as both operands have the same.
+template <typename T, typename YT, int MB>
+__global__ void __launch_bounds__(LW_THREADS, MB == 1 ? 4 : 2)
+lora_rows_kernel(const __grid_constant__ LoraRows p) {
+  constexpr int ROWS = 16 * MB, PARTS = LwParts<T>::N;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_row[ROWS];
+  __shared__ float s_factor[ROWS][LW_TARGETS];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), C = (int)cluster.num_blocks();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int TR = p.targets * p.R, wn = TR > 128 ? 8 : TR > 64 ? 4 : TR > 32 ? 2 : 1, wk = LW_WARPS / wn, ranks = wn * 32;
+  float* s_part = reinterpret_cast<float*>(smem);                 // [wk][ROWS][ranks], then sums of this CTA in its first [ROWS][ranks]
+  float* s_z = s_part + lw_part_floats<T>(ranks) * ROWS;          // [ROWS][ranks]
+  T* s_split = reinterpret_cast<T*>(s_part);                      // [PARTS][ROWS][ranks + 8], once the sums are read
+  pdl_wait();
+  const int tile_index = blockIdx.x / C;
+  if (tile_index >= p.plan.tiles()) return;                       // (the whole cluster)
+  const int4 tile = p.plan.tile(tile_index);
+  if ((int)threadIdx.x < ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
+  const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.x * p.N * p.R;
+  const int runs = p.tile0[p.targets], run0 = (int)((int64_t)runs * rank / C), run1 = (int)((int64_t)runs * (rank + 1) / C);
+  __syncthreads();
+
+  // ---- this CTA's part of z ---------------------------------------------------------------------------------------------------
+  float acc[MB][4][4];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+  const int my_n = warp % wn * 32, my_k = warp / wn;
+  if (my_n < TR) {
+    const T* xr[MB][2];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = s_row[16 * i + 8 * h + g];
+        xr[i][h] = row < 0 ? nullptr : reinterpret_cast<const T*>(p.x) + (int64_t)row * p.ldx + 8 * t;
+      }
+    const T* ar[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = my_n + 8 * j + g;
+      ar[j] = n < TR ? reinterpret_cast<const T*>(p.a) + ((int64_t)tile.x * TR + n) * p.K + 8 * t : nullptr;
+    }
+    const int s0 = (int)((int64_t)p.steps * rank / C), s1 = (int)((int64_t)p.steps * (rank + 1) / C);
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll(MB == 1 ? 2 : 1)
+    for (int s = s0 + my_k; s < s1; s += wk) {
+      const bool in = s * 32 + 8 * t < p.K;
+      uint4 av[4], xv[MB][2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) av[j] = in && ar[j] ? *reinterpret_cast<const uint4*>(ar[j] + s * 32) : zero;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) xv[i][h] = in && xr[i][h] ? *reinterpret_cast<const uint4*>(xr[i][h] + s * 32) : zero;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const uint32_t lo[4] = {xv[i][0].x, xv[i][1].x, xv[i][0].y, xv[i][1].y}, hi[4] = {xv[i][0].z, xv[i][1].z, xv[i][0].w, xv[i][1].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          mma16816<T>(acc[i][j], lo, av[j].x, av[j].y);
+          mma16816<T>(acc[i][j], hi, av[j].z, av[j].w);
+        }
+      }
+    }
+  }
+  {
+    float* part = s_part + my_k * ROWS * ranks + my_n;
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        *reinterpret_cast<float2*>(part + (16 * i + g) * ranks + 8 * j + 2 * t) = make_float2(acc[i][j][0], acc[i][j][1]);
+        *reinterpret_cast<float2*>(part + (16 * i + 8 + g) * ranks + 8 * j + 2 * t) = make_float2(acc[i][j][2], acc[i][j][3]);
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < ROWS * ranks; i += LW_THREADS) {
+    float sum = 0.f;
+    for (int k = 0; k < wk; ++k) sum += s_part[k * ROWS * ranks + i];
+    s_part[i] = sum;                                              // (nobody else looks at place i of the first part)
+  }
+  if (C > 1) cluster.sync();
+  else __syncthreads();
+  for (int i = threadIdx.x; i < ROWS * ranks; i += LW_THREADS) {
+    float sum = 0.f;
+    for (int r = 0; r < C; ++r) sum += cluster.map_shared_rank(s_part, r)[i];       // in one order everywhere
+    s_z[i] = sum;
+  }
+  if (C > 1) cluster.sync();                                      // all have read: what lies there may go
+  else __syncthreads();
+  pdl_launch_dependents();
+
+  // ---- z as 16-bit numbers: a warp per row and target -------------------------------------------------------------------------
+  const int ld = ranks + 8;
+  for (int i = warp; i < ROWS * p.targets; i += LW_WARPS) {
+    const int row = i / p.targets, target = i - row * p.targets;
+    const float* z = s_z + row * ranks + target * p.R;
+    float top = 0.f;
+    for (int r = lane; r < p.R; r += 32) top = fmaxf(top, fabsf(z[r]));
+    top = warp_max(top);
+    // 2^e with top 2^-e in [1, 2); 1 for a row of zeros or one that is not finite
+    const uint32_t e = __float_as_uint(top) >> 23;
+    const bool plain = e < 1 || e > 252;
+    const float down = plain ? 1.f : __uint_as_float((254u - e) << 23), up = plain ? 1.f : __uint_as_float(e << 23);
+    if (lane == 0) s_factor[row][target] = up * p.scales[tile.x];
+    for (int r = lane; r < p.R; r += 32) {
+      float v = z[r] * down;
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) {
+        const T h = Tr<T>::from_f(v);
+        s_split[(k * ROWS + row) * ld + target * p.R + r] = h;
+        v -= Tr<T>::to_f(h);
+      }
+    }
+  }
+  __syncthreads();
+
+  // ---- this CTA's columns: 16 at a time, of which a lane gets four neighbours ---------------------------------------------------
+#pragma unroll 1
+  for (int run = run0 + warp; run < run1; run += LW_WARPS) {
+    int target = 0;
+#pragma unroll
+    for (int k = 1; k < LW_TARGETS; ++k)
+      if (k < p.targets && run >= p.tile0[k]) target = k;
+    const int width = p.start[target + 1] - p.start[target], c0 = (run - p.tile0[target]) * 16;
+    // column j of the two products' eight: 4 (j / 2) + j % 2, and two further
+    const int n0 = c0 + 4 * (g >> 1) + (g & 1);
+    const T* b0 = b + (int64_t)(p.start[target] + n0) * p.R + 4 * t;
+    const bool in0 = n0 < width, in1 = n0 + 2 < width;
+    const int col = c0 + 4 * t;
+    const bool in = col < width;
+    float d[MB][2][4];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) d[i][h][0] = d[i][h][1] = d[i][h][2] = d[i][h][3] = 0.f;
+    for (int k = 0; k < p.R; k += 16) {
+      const uint2 zero = make_uint2(0, 0);
+      const uint2 w0 = in0 ? *reinterpret_cast<const uint2*>(b0 + k) : zero, w1 = in1 ? *reinterpret_cast<const uint2*>(b0 + 2 * p.R + k) : zero;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          const T* z = s_split + (part * ROWS + 16 * i + g) * ld + target * p.R + k + 4 * t;
+          const uint2 lo = *reinterpret_cast<const uint2*>(z), hi = *reinterpret_cast<const uint2*>(z + 8 * ld);
+          const uint32_t f[4] = {lo.x, hi.x, lo.y, hi.y};
+          mma16816<T>(d[i][0], f, w0.x, w0.y);
+          mma16816<T>(d[i][1], f, w1.x, w1.y);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = 16 * i + 8 * h + g, row = s_row[at];
+        if (row < 0 || !in) continue;
+        const float f = s_factor[at][target];
+        YT* y = reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + p.col0[target] + col;
+        if constexpr (sizeof(YT) == 4) {
+          float4 v = *reinterpret_cast<float4*>(y);
+          v.x = fmaf(f, d[i][0][2 * h], v.x), v.y = fmaf(f, d[i][0][2 * h + 1], v.y);
+          v.z = fmaf(f, d[i][1][2 * h], v.z), v.w = fmaf(f, d[i][1][2 * h + 1], v.w);
+          *reinterpret_cast<float4*>(y) = v;
+        } else {
+          uint2 raw = *reinterpret_cast<uint2*>(y);
+          const YT* e = reinterpret_cast<const YT*>(&raw);
+          raw = make_uint2(pack2<YT>(fmaf(f, d[i][0][2 * h], Tr<YT>::to_f(e[0])), fmaf(f, d[i][0][2 * h + 1], Tr<YT>::to_f(e[1]))),
+                           pack2<YT>(fmaf(f, d[i][1][2 * h], Tr<YT>::to_f(e[2])), fmaf(f, d[i][1][2 * h + 1], Tr<YT>::to_f(e[3]))));
+          *reinterpret_cast<uint2*>(y) = raw;
+        }
+      }
+  }
+}
+
+template <typename T, typename YT, int MB>
+static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
+  auto kern = lora_rows_kernel<T, YT, MB>;
+  static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
+  int dev = 0;
+  cudaError_t ae = cudaGetDevice(&dev);
+  if (ae == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
+    ae = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (lw_part_floats<T>(LW_RANKS) + LW_RANKS) * 16 * MB * 4);
+    if (ae == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
+  }
+  if (ae != cudaSuccess) return cuda_fail(ae, "cudaFuncSetAttribute(lora_rows_kernel)");
+  const int TR = p.targets * p.R, ranks = TR > 128 ? 256 : TR > 64 ? 128 : TR > 32 ? 64 : 32;
+  int C = LW_CLUSTER;
+  while (C > 1 && tiles * C > 4 * sm_count()) C >>= 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * C));
+  cfg.blockDim = dim3(LW_THREADS);
+  cfg.dynamicSmemBytes = (size_t)(lw_part_floats<T>(ranks) + ranks) * 16 * MB * 4;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  return e == cudaSuccess ? B200P_OK : cuda_fail(e, "lora_rows_kernel");
+}
+
+}  // namespace b200p
+
+using namespace b200p;
+
+extern "C" int64_t b200p_row_groups_ints(int64_t M, int64_t groups, int64_t tile) {
+  if (M < 0 || M > RG_ROWS || groups <= 0 || groups > RG_GROUPS || tile <= 0) return 0;
+  return row_group_ints(M, groups, tile);
+}
+
+extern "C" int b200p_row_groups(const int32_t* index, int32_t* plan, int64_t M, int groups, int tile, int64_t plan_ints, void* stream) {
+  PdlClass pdl_cls(64);
+  B200P_REQUIRE(M >= 0 && M <= RG_ROWS, B200P_ERR_ARG, "bad shape: %lld rows, at most 2^20", (long long)M);
+  B200P_REQUIRE(groups > 0 && groups <= RG_GROUPS, B200P_ERR_ARG, "%d groups: 1 to %d", groups, RG_GROUPS);
+  B200P_REQUIRE(tile > 0 && tile <= RG_ROWS, B200P_ERR_ARG, "%d rows of a tile", tile);
+  B200P_REQUIRE(plan && (index || M == 0), B200P_ERR_ARG, "null pointer");
+  B200P_REQUIRE(plan_ints >= row_group_ints(M, groups, tile), B200P_ERR_ARG, "a plan of %lld rows in %d groups has %lld integers, got room for %lld", (long long)M,
+                groups, (long long)row_group_ints(M, groups, tile), (long long)plan_ints);
+  B200P_REQUIRE(aligned(plan, 16) && aligned(index, 4), B200P_ERR_ALIGN, "the plan must be 16-byte aligned, the index to its type");
+  if (groups > 512) {                                             // (more than every launch may have)
+    const cudaError_t e = cudaFuncSetAttribute(row_groups_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RG_WARPS * RG_GROUPS * 4);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(row_groups_kernel)");
+  }
+  launch_pdl(row_groups_kernel, 1u, RG_WARPS * 32, (size_t)RG_WARPS * groups * 4, (cudaStream_t)stream, index, plan, (int)M, groups, tile);
+  B200P_LAUNCH_CHECK("row_groups_kernel");
+  return B200P_OK;
+}
+
+// Tiles of 64 rows read an adapter a quarter as often as tiles of 16, which spread few rows over more SMs.
+extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1024 && M >= 16ll * groups ? 64 : 16; }
+
+extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a, const void* b, const float* scales, void* y, const int32_t* host_columns,
+                               int64_t M, int adapters, int tile, int targets, int R, int64_t K, int64_t ldx, int64_t ldy, int dtype, int y_f32,
+                               void* stream) {
+  PdlClass pdl_cls(64);
+  B200P_REQUIRE(dtype == B200P_F16 || dtype == B200P_BF16, B200P_ERR_ARG, "adapters and their inputs are 16-bit");
+  B200P_REQUIRE(M >= 0 && M <= RG_ROWS && adapters > 0 && adapters <= RG_GROUPS, B200P_ERR_ARG, "bad shape: %lld rows, %d adapters", (long long)M, adapters);
+  B200P_REQUIRE(tile == 16 || tile == 64, B200P_ERR_ARG, "the plan's tiles have 16 or 64 rows, not %d", tile);
+  B200P_REQUIRE(targets > 0 && targets <= LW_TARGETS, B200P_ERR_ARG, "%d targets: 1 to %d", targets, LW_TARGETS);
+  B200P_REQUIRE(R > 0 && R % 16 == 0 && R * targets <= LW_RANKS, B200P_ERR_ARG, "%d targets of rank %d: a multiple of 16, %d in all at most", targets, R,
+                LW_RANKS);
+  B200P_REQUIRE(K > 0 && K % 8 == 0 && K < (1ll << 24) && ldx >= K, B200P_ERR_ARG, "bad K %lld: a multiple of 8, not above ldx", (long long)K);
+  B200P_REQUIRE(host_columns, B200P_ERR_ARG, "null pointer");
+  LoraRows p{};
+  for (int t = 0; t < targets; ++t) {
+    const int64_t col = host_columns[2 * t], width = host_columns[2 * t + 1];
+    B200P_REQUIRE(col >= 0 && width > 0 && width % 8 == 0 && col + width <= ldy, B200P_ERR_ARG, "target %d: columns %lld to %lld of %lld, a multiple of 8", t,
+                  (long long)col, (long long)(col + width), (long long)ldy);
+    B200P_REQUIRE(col % 4 == 0, B200P_ERR_ALIGN, "a target's first column is a multiple of 4");
+    for (int u = 0; u < t; ++u)
+      B200P_REQUIRE(col + width <= host_columns[2 * u] || col >= (int64_t)host_columns[2 * u] + host_columns[2 * u + 1], B200P_ERR_ARG, "targets overlap");
+    p.col0[t] = (int)col, p.start[t + 1] = p.start[t] + (int)width, p.tile0[t + 1] = p.tile0[t] + (int)((width + 15) / 16);
+  }
+  if (M == 0) return B200P_OK;
+  B200P_REQUIRE(x && plan && a && b && scales && y, B200P_ERR_ARG, "null pointer");
+  B200P_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && aligned(plan, 16) && ldx % 8 == 0, B200P_ERR_ALIGN,
+                "x, its rows, the adapters and the plan must be 16-byte aligned");
+  B200P_REQUIRE(aligned(y, y_f32 ? 16 : 8) && ldy % 4 == 0, B200P_ERR_ALIGN, "four neighbours of y must be aligned");
+  p.x = x, p.a = a, p.b = b, p.scales = scales, p.y = y, p.plan = RowGroups{plan, (int)M}, p.ldx = ldx, p.ldy = ldy;
+  p.K = (int)K, p.R = R, p.N = p.start[targets], p.targets = targets, p.steps = (int)((K + 31) / 32);
+  const int64_t tiles = row_group_tiles(M, adapters, tile);
+  cudaStream_t st = (cudaStream_t)stream;
+#define LW_GO(T, MB) return y_f32 ? launch_lora_rows<T, float, MB>(p, tiles, st) : launch_lora_rows<T, T, MB>(p, tiles, st)
+  if (dtype == B200P_F16) {
+    if (tile == 16) LW_GO(__half, 1);
+    LW_GO(__half, 4);
+  }
+  if (tile == 16) LW_GO(__nv_bfloat16, 1);
+  LW_GO(__nv_bfloat16, 4);
+#undef LW_GO
+}

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 from typing import NamedTuple, Optional
 
+import functools
 import os
 
 import torch
@@ -198,6 +199,87 @@ def lora_add(x, At, Bt, y, col0: int, scale: float):
     _call("b200p_lora_add", lambda: lib().b200p_lora_add(_p(x), _p(At), _p(Bt), _p(y), M, N, K, x.stride(0), y.stride(0), int(col0),
                                                          float(scale), dtype_code(x.dtype), 1 if y.dtype == torch.float32 else 0,
                                                          _stream()))
+    return y
+
+
+class RowPlan(NamedTuple):
+    """The rows of a batch in the order of their groups (row_groups)."""
+    data: torch.Tensor                        # int32 (b200p_row_groups)
+    rows: int
+    groups: int
+    tile: int
+
+
+def row_groups(index, groups: int, tile: int, out: Optional[RowPlan] = None) -> RowPlan:
+    """Plan of a batch whose row m belongs to group ``index[m]`` (int32; negative or not below ``groups``: to none), in tiles of up to ``tile`` rows
+    (b200p_row_groups).  It stays good until the index changes; ``out`` is written anew, e.g. inside a captured step."""
+    _dev(index)
+    M = index.numel()
+    if index.dtype is not torch.int32 or index.dim() != 1 or not index.is_contiguous() or index.get_device() != _device_index():
+        raise ValueError(f"the index is int32 [rows] on the current device: got {index.dtype} {tuple(index.shape)}")
+    if out is None:
+        n = lib().b200p_row_groups_ints(M, int(groups), int(tile))
+        if n == 0:
+            raise ValueError(f"no plan of {M} rows in {groups} groups and tiles of {tile}: at most 2^20 rows and 1024 groups")
+        out = RowPlan(torch.empty((n,), dtype=torch.int32, device=index.device), M, int(groups), int(tile))
+    elif (out.rows, out.groups, out.tile) != (M, groups, tile):
+        raise ValueError(f"a plan of {out.rows} rows in {out.groups} groups and tiles of {out.tile} is not one of {M}, {groups} and {tile}")
+    _plan(out, index.get_device())
+    _call("b200p_row_groups", lambda: lib().b200p_row_groups(_p(index), out.data.data_ptr(), M, out.groups, out.tile, out.data.numel(), _stream()))
+    return out
+
+
+def _plan(plan: RowPlan, dev: int):
+    d = plan.data
+    if d.dtype is not torch.int32 or d.get_device() != dev or not d.is_contiguous():
+        raise ValueError("a plan is contiguous int32 beside the rows it groups")
+    if plan.tile < 1 or d.numel() < 4 + (plan.rows + 3) // 4 * 4 + 4 * (plan.rows // plan.tile + min(plan.rows, plan.groups)):
+        raise ValueError(f"{d.numel()} integers are no plan of {plan.rows} rows in {plan.groups} groups and tiles of {plan.tile}")
+
+
+def lora_tile(rows: int, adapters: int) -> int:
+    """Tile of the row_groups plan that lora_rows is fastest with."""
+    return lib().b200p_lora_rows_tile(int(rows), int(adapters))
+
+
+@functools.lru_cache(maxsize=64)
+def _columns(columns: tuple):
+    import ctypes as C
+    flat = [int(v) for pair in columns for v in pair]
+    if any(len(pair) != 2 for pair in columns) or any(not 0 <= v < 2**31 for v in flat):
+        raise ValueError(f"columns are (first, number) of every target: got {columns}")
+    return (C.c_int32 * len(flat))(*flat)
+
+
+def lora_rows(x, plan: RowPlan, a, b, scales, columns, y):
+    """y[m, columns] += scales[i] * (x[m] a[i]^T) b[i]^T for every row m that ``plan`` gives an adapter i (b200p_lora_rows): ``x`` [M, K], ``a`` [adapters,
+    targets, R, K], ``b`` [adapters, sum of the targets' columns, R] in one 16-bit type, ``scales`` float32 [adapters], ``columns`` = ((first column in y, number
+    of columns), ...) of the targets, ``y`` [M, N] of that type or float32."""
+    import ctypes as C
+    dev = x.get_device()
+    if dev < 0 or dev != _device_index() or any(t.get_device() != dev for t in (a, b, scales, y)):
+        _dev(x, a, b, scales, y)
+        raise ValueError("x, adapters and y lie on the current device")
+    _plan(plan, dev)
+    M, K = x.shape
+    (ldx, inner), (ldy, y_inner) = x.stride(), y.stride()
+    n, targets, R, ka = a.shape
+    dt, columns = x.dtype, tuple(columns)
+    held = _columns(columns)
+    if a.dtype is not dt or b.dtype is not dt or y.dtype not in (dt, torch.float32):
+        raise ValueError(f"x, a, b are of one 16-bit type, y of it or float32: got {dt}, {a.dtype}, {b.dtype}, {y.dtype}")
+    if scales.dtype is not torch.float32 or scales.shape != (n,) or not (a.is_contiguous() and b.is_contiguous() and scales.is_contiguous()):
+        raise ValueError(f"contiguous adapters, scales float32 [{n}]: got {scales.dtype} {tuple(scales.shape)}")
+    if ka != K or len(columns) != targets or b.shape != (n, sum(w for _, w in columns), R):
+        raise ValueError(f"a [adapters, targets, R, {K}] and b [adapters, {sum(w for _, w in columns)}, R] of {len(columns)} targets: got {tuple(a.shape)} and "
+                         f"{tuple(b.shape)}")
+    if y.shape[0] != M or inner != 1 or y_inner != 1 or (M > 1 and (ldx < K or ldy < y.shape[1])) or (plan.rows, plan.groups) != (M, n):
+        raise ValueError(f"rows of x, y and the plan: got {tuple(x.shape)}, {tuple(y.shape)}, {plan.rows} rows in {plan.groups} groups of {n} adapters")
+    if any(c + w > y.shape[1] for c, w in columns):
+        raise ValueError(f"columns {columns} of {y.shape[1]}")
+    _call("b200p_lora_rows", lambda: lib().b200p_lora_rows(
+        x.data_ptr(), plan.data.data_ptr(), a.data_ptr(), b.data_ptr(), scales.data_ptr(), y.data_ptr(), C.addressof(held), M, n, plan.tile, targets, R, K,
+        ldx if M > 1 else K, ldy if M > 1 else y.shape[1], dtype_code(dt), 0 if y.dtype is dt else 1, _stream()))
     return y
 
 

@@ -24,3 +24,41 @@ def test_token_logprobs_refuses_before_it_launches():
 def test_no_cpu_fallback():
     with pytest.raises(_lib.B200PError):
         ops.token_logprobs(torch.zeros((2, 8)), torch.zeros((2,), dtype=torch.int32))
+
+
+def test_row_groups_refuses_before_it_launches():
+    L = _lib.lib()
+    assert L.b200p_row_groups_ints(10, 3, 16) == 4 + 12 + 4 * 3 and L.b200p_row_groups_ints(100, 3, 16) == 4 + 100 + 4 * (6 + 3)
+    for bad in ((-1, 3, 16), ((1 << 20) + 1, 3, 16), (10, 0, 16), (10, 1025, 16), (10, 3, 0)):
+        assert L.b200p_row_groups_ints(*bad) == 0
+    ok = dict(index=256, plan=256, M=10, groups=3, tile=16, ints=1000)
+
+    def call(**kw):
+        a = dict(ok, **kw)
+        return L.b200p_row_groups(a["index"], a["plan"], a["M"], a["groups"], a["tile"], a["ints"], 0)
+
+    for bad in (dict(M=-1), dict(M=(1 << 20) + 1), dict(groups=0), dict(groups=1025), dict(tile=0), dict(plan=0), dict(index=0), dict(ints=27)):
+        assert call(**bad) == -1, bad
+    assert call(plan=260) == -2 and call(index=258) == -2
+
+
+def test_lora_rows_refuses_before_it_launches():
+    import ctypes as C
+    f = _lib.lib().b200p_lora_rows
+    ok = dict(x=256, plan=256, a=256, b=256, scales=256, y=256, columns=(0, 64, 128, 8), M=4, adapters=2, tile=16, targets=2, R=16, K=64, ldx=64, ldy=136,
+              dtype=_lib.F16, f32=1)
+
+    def call(**kw):
+        a = dict(ok, **kw)
+        held = (C.c_int32 * len(a["columns"]))(*a["columns"])
+        return f(a["x"], a["plan"], a["a"], a["b"], a["scales"], a["y"], C.addressof(held), a["M"], a["adapters"], a["tile"], a["targets"], a["R"], a["K"],
+                 a["ldx"], a["ldy"], a["dtype"], a["f32"], 0)
+
+    for bad in (dict(dtype=_lib.F32), dict(dtype=7), dict(M=-1), dict(M=(1 << 20) + 1), dict(adapters=0), dict(adapters=1025), dict(tile=32), dict(targets=0),
+                dict(targets=5, columns=(0, 8) * 5), dict(R=0), dict(R=24), dict(R=144), dict(K=0), dict(K=12), dict(ldx=56), dict(columns=(0, 64, 128, 16)),
+                dict(columns=(0, 64, 60, 8)), dict(columns=(0, 0, 64, 8)), dict(columns=(-8, 64, 64, 8)), dict(columns=(0, 60, 64, 8)), dict(x=0), dict(plan=0),
+                dict(a=0), dict(b=0), dict(scales=0), dict(y=0)):
+        assert call(**bad) == -1, bad
+    for bad in (dict(columns=(2, 64, 128, 8)), dict(x=264), dict(a=264), dict(b=264), dict(plan=264), dict(ldx=68), dict(y=264), dict(ldy=137)):
+        assert call(**bad) == -2, bad
+    assert call(M=0) == 0
