@@ -173,7 +173,7 @@ int64_t b200p_row_groups_ints(int64_t M, int64_t groups, int64_t tile);      /* 
 /* LoRA with an adapter of its own for every row:  y[m, columns of target t] += scales[i] * (x[m] . A[i, t]^T) . B[i]^T, i = the row's group in `plan`; rows
  * without one are not touched.  x `dtype` (16-bit) [M, K] (row stride ldx); a `dtype` [adapters, targets, R, K] (lora_a transposed; its k axis permuted like x
  * when x is PERM8), b `dtype` [adapters, sum of the targets' columns, R] (lora_b transposed, target after target), the ranks filled up to R, a multiple of 16,
- * with zeros; targets * R <= 256.  host_columns (host memory) = first column in y and number of columns (a multiple of 8) of every target, which do not
+ * 64 at most, with zeros; 4 targets at most.  host_columns (host memory) = first column in y and number of columns (a multiple of 8) of every target, which do not
  * overlap; y float (y_f32) or `dtype`, row stride ldy.  Sums are fp32, y is rounded once.  `tile` is the plan's: 16 or 64, b200p_lora_rows_tile(M, adapters)
  * the better one.  K a multiple of 8; x, its rows, a, b and plan 16-byte aligned; ldy and first columns multiples of 4, y aligned to four elements. */
 int b200p_lora_rows(const void* x, const int32_t* plan, const void* a, const void* b, const float* scales, void* y, const int32_t* host_columns, int64_t M,

@@ -87,7 +87,8 @@ row_groups_kernel(const int32_t* index, int32_t* plan, int M, int groups, int ti
 
 // ------------------------------------------------------------------------------------------------ the update
 constexpr int LW_WARPS = 8, LW_THREADS = LW_WARPS * 32;
-constexpr int LW_TARGETS = 4, LW_CLUSTER = 8, LW_RANKS = 256;     // targets, CTAs of a tile, ranks of all targets at most
+// targets, CTAs of a tile, ranks of a target at most
+constexpr int LW_TARGETS = 4, LW_CLUSTER = 8, LW_RANK = 64, LW_RANKS = LW_RANK * LW_TARGETS;
 
 struct LoraRows {
   const void *x, *a, *b;
@@ -101,35 +102,70 @@ struct LoraRows {
 
 template <typename T> struct LwParts { static constexpr int N = 2; };
 template <> struct LwParts<__nv_bfloat16> { static constexpr int N = 3; };
-// a row's room for its parts of z, which the split z takes over
-template <typename T>
-__host__ __device__ constexpr int lw_part_floats(int ranks) {
-  return LwParts<T>::N * (ranks + 8) / 2 > LW_WARPS * 32 ? LwParts<T>::N * (ranks + 8) / 2 : LW_WARPS * 32;
+// Shared floats of a row: the warps' parts of z, of which the first becomes this CTA's, and the split z, which has room behind it (16 rows) or takes the
+// parts' place when the whole cluster has read them (64 rows: two CTAs fit an SM).
+template <typename T, int MB>
+__host__ __device__ constexpr int lw_row_floats(int ranks) {
+  const int split = LwParts<T>::N * (ranks + 8) / 2 + (MB == 1 ? ranks : 0);
+  return split > LW_WARPS * 32 ? split : LW_WARPS * 32;
 }
 
-// MB blocks of 16 rows; YT: y's type.  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits this CTA's part of K.
-// Operands come straight from memory, 16 bytes a lane: the order of k within a product is free as long as both operands have the same.
-template <typename T, typename YT, int MB>
-__global__ void __launch_bounds__(LW_THREADS, MB == 1 ? 4 : 2)
+__host__ __device__ constexpr int lw_ctas(int mb, int ks) { return mb == 1 && ks < 4 ? 3 : 2; }      // of an SM
+
+__device__ __forceinline__ void red_add4(float* p, float a, float b, float c, float d) {
+  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+// What a lane needs of b for a run of 16 columns: R ranks of its two columns in the products' order, column j of the two products' eight being
+// 4 (j / 2) + j % 2 and two further, so that a lane's four results are neighbours.
+template <typename T, int KS>
+struct LwRun {
+  int target, col, width;
+  uint2 w[KS][2];
+  __device__ __forceinline__ void load(const LoraRows& p, const T* b, int run, int run1) {
+    if (run >= run1) return;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    target = 0;
+#pragma unroll
+    for (int k = 1; k < LW_TARGETS; ++k)
+      if (k < p.targets && run >= p.tile0[k]) target = k;
+    width = p.start[target + 1] - p.start[target];
+    const int c0 = (run - p.tile0[target]) * 16;
+    col = c0 + 4 * t;
+    const int n0 = c0 + 4 * (g >> 1) + (g & 1);
+    const T* at = b + (int64_t)(p.start[target] + n0) * p.R + 4 * t;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[k][h] = n0 + 2 * h < width && 16 * k < p.R ? *reinterpret_cast<const uint2*>(at + 2 * h * p.R + 16 * k) : make_uint2(0, 0);
+  }
+};
+
+// MB blocks of 16 rows; YT: y's type; KS: 16 ranks each (R or more).  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits
+// this CTA's part of K.  Operands come straight from memory, 16 bytes a lane: the order of k within a product is free as long as both operands have the same.
+template <typename T, typename YT, int MB, int KS>
+__global__ void __launch_bounds__(LW_THREADS, lw_ctas(MB, KS))
 lora_rows_kernel(const __grid_constant__ LoraRows p) {
-  constexpr int ROWS = 16 * MB, PARTS = LwParts<T>::N;
+  constexpr int ROWS = 16 * MB, PARTS = LwParts<T>::N, NZ = (16 * KS + 31) / 32;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int s_row[ROWS];
   __shared__ float s_factor[ROWS][LW_TARGETS];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), C = (int)cluster.num_blocks();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int TR = p.targets * p.R, wn = TR > 128 ? 8 : TR > 64 ? 4 : TR > 32 ? 2 : 1, wk = LW_WARPS / wn, ranks = wn * 32;
-  float* s_part = reinterpret_cast<float*>(smem);                 // [wk][ROWS][ranks], then sums of this CTA in its first [ROWS][ranks]
-  float* s_z = s_part + lw_part_floats<T>(ranks) * ROWS;          // [ROWS][ranks]
-  T* s_split = reinterpret_cast<T*>(s_part);                      // [PARTS][ROWS][ranks + 8], once the sums are read
+  const int TR = p.targets * p.R, wn = TR > 128 ? 8 : TR > 64 ? 4 : TR > 32 ? 2 : 1, wk = LW_WARPS / wn, ranks = wn * 32, ld = ranks + 8;
+  float* s_part = reinterpret_cast<float*>(smem);                 // [wk][ROWS][ranks]
+  T* s_split = reinterpret_cast<T*>(s_part + (MB == 1 ? ROWS * ranks : 0));      // [PARTS][ROWS][ld]
   pdl_wait();
-  const int tile_index = blockIdx.x / C;
-  if (tile_index >= p.plan.tiles()) return;                       // (the whole cluster)
-  const int4 tile = p.plan.tile(tile_index);
-  if ((int)threadIdx.x < ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
+  const int tile_index = blockIdx.x / C, tiles = p.plan.tiles();
+  const int4 tile = p.plan.tile(tile_index);                      // (the plan has room for every tile of the grid)
+  if (tile_index >= tiles) return;                                // (the whole cluster)
   const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.x * p.N * p.R;
   const int runs = p.tile0[p.targets], run0 = (int)((int64_t)runs * rank / C), run1 = (int)((int64_t)runs * (rank + 1) / C);
+  LwRun<T, KS> cur, next;
+  cur.load(p, b, run0 + warp, run1);                              // on its way beside the first product
+  if ((int)threadIdx.x < ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
   __syncthreads();
 
   // ---- this CTA's part of z ---------------------------------------------------------------------------------------------------
@@ -188,78 +224,116 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
       }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < ROWS * ranks; i += LW_THREADS) {
+  for (int i = threadIdx.x; i < tile.z * ranks; i += LW_THREADS) {
     float sum = 0.f;
     for (int k = 0; k < wk; ++k) sum += s_part[k * ROWS * ranks + i];
     s_part[i] = sum;                                              // (nobody else looks at place i of the first part)
   }
   if (C > 1) cluster.sync();
   else __syncthreads();
-  for (int i = threadIdx.x; i < ROWS * ranks; i += LW_THREADS) {
-    float sum = 0.f;
-    for (int r = 0; r < C; ++r) sum += cluster.map_shared_rank(s_part, r)[i];       // in one order everywhere
-    s_z[i] = sum;
-  }
-  if (C > 1) cluster.sync();                                      // all have read: what lies there may go
-  else __syncthreads();
-  pdl_launch_dependents();
 
-  // ---- z as 16-bit numbers: a warp per row and target -------------------------------------------------------------------------
-  const int ld = ranks + 8;
-  for (int i = warp; i < ROWS * p.targets; i += LW_WARPS) {
+  // ---- z of all CTAs, as 16-bit numbers: a warp per row and target ---------------------------------------------------------------
+  auto whole = [&](int i, float (&z)[NZ]) {
+    const int row = i / p.targets, at = row * ranks + (i - row * p.targets) * p.R;
+#pragma unroll
+    for (int k = 0; k < NZ; ++k) {
+      z[k] = 0.f;
+      if (32 * k >= p.R) continue;
+      float v[LW_CLUSTER];
+#pragma unroll
+      for (int r = 0; r < LW_CLUSTER; ++r) v[r] = r < C && 32 * k + lane < p.R ? cluster.map_shared_rank(s_part, r)[at + 32 * k + lane] : 0.f;
+#pragma unroll
+      for (int r = 0; r < LW_CLUSTER; ++r) z[k] += v[r];           // in one order everywhere
+    }
+  };
+  auto split = [&](int i, const float (&z)[NZ]) {
     const int row = i / p.targets, target = i - row * p.targets;
-    const float* z = s_z + row * ranks + target * p.R;
     float top = 0.f;
-    for (int r = lane; r < p.R; r += 32) top = fmaxf(top, fabsf(z[r]));
+#pragma unroll
+    for (int k = 0; k < NZ; ++k) top = fmaxf(top, fabsf(z[k]));
     top = warp_max(top);
     // 2^e with top 2^-e in [1, 2); 1 for a row of zeros or one that is not finite
     const uint32_t e = __float_as_uint(top) >> 23;
     const bool plain = e < 1 || e > 252;
     const float down = plain ? 1.f : __uint_as_float((254u - e) << 23), up = plain ? 1.f : __uint_as_float(e << 23);
     if (lane == 0) s_factor[row][target] = up * p.scales[tile.x];
-    for (int r = lane; r < p.R; r += 32) {
-      float v = z[r] * down;
 #pragma unroll
-      for (int k = 0; k < PARTS; ++k) {
+    for (int k = 0; k < NZ; ++k) {
+      if (32 * k + lane >= p.R) continue;
+      float v = z[k] * down;
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
         const T h = Tr<T>::from_f(v);
-        s_split[(k * ROWS + row) * ld + target * p.R + r] = h;
+        s_split[(part * ROWS + row) * ld + target * p.R + 32 * k + lane] = h;
         v -= Tr<T>::to_f(h);
       }
     }
+  };
+  if constexpr (MB == 1) {
+    for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
+      float z[NZ];
+      whole(i, z);
+      split(i, z);
+    }
+    if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    __syncthreads();
+  } else {
+    // (a sum that is needed again takes the first part's place in this CTA when the others have read it)
+    float* s_z = s_part + lw_row_floats<T, MB>(ranks) * ROWS;
+    for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
+      float z[NZ];
+      whole(i, z);
+      const int row = i / p.targets, at = row * ranks + (i - row * p.targets) * p.R;
+#pragma unroll
+      for (int k = 0; k < NZ; ++k)
+        if (32 * k + lane < p.R) s_z[at + 32 * k + lane] = z[k];
+    }
+    if (C > 1) cluster.sync();                                    // all have read: what lies there may go
+    else __syncthreads();
+    for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
+      float z[NZ];
+      const int row = i / p.targets, at = row * ranks + (i - row * p.targets) * p.R;
+#pragma unroll
+      for (int k = 0; k < NZ; ++k) z[k] = 32 * k + lane < p.R ? s_z[at + 32 * k + lane] : 0.f;
+      split(i, z);
+    }
+    __syncthreads();
   }
-  __syncthreads();
+  pdl_launch_dependents();
 
-  // ---- this CTA's columns: 16 at a time, of which a lane gets four neighbours ---------------------------------------------------
+  // ---- this CTA's columns: 16 at a time, of which a lane has four neighbours -----------------------------------------------------
 #pragma unroll 1
   for (int run = run0 + warp; run < run1; run += LW_WARPS) {
-    int target = 0;
+    next.load(p, b, run + LW_WARPS, run1);
+    const bool in = cur.col < cur.width;
+    const int64_t col = p.col0[cur.target] + cur.col;
+    uint2 old[MB][2];                                             // 16-bit y, on its way beside the products (fp32 is added in memory)
+    if constexpr (sizeof(YT) == 2) {
 #pragma unroll
-    for (int k = 1; k < LW_TARGETS; ++k)
-      if (k < p.targets && run >= p.tile0[k]) target = k;
-    const int width = p.start[target + 1] - p.start[target], c0 = (run - p.tile0[target]) * 16;
-    // column j of the two products' eight: 4 (j / 2) + j % 2, and two further
-    const int n0 = c0 + 4 * (g >> 1) + (g & 1);
-    const T* b0 = b + (int64_t)(p.start[target] + n0) * p.R + 4 * t;
-    const bool in0 = n0 < width, in1 = n0 + 2 < width;
-    const int col = c0 + 4 * t;
-    const bool in = col < width;
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = s_row[16 * i + 8 * h + g];
+          old[i][h] = row >= 0 && in ? *reinterpret_cast<const uint2*>(reinterpret_cast<const YT*>(p.y) + (int64_t)row * p.ldy + col) : make_uint2(0, 0);
+        }
+    }
     float d[MB][2][4];
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) d[i][h][0] = d[i][h][1] = d[i][h][2] = d[i][h][3] = 0.f;
-    for (int k = 0; k < p.R; k += 16) {
-      const uint2 zero = make_uint2(0, 0);
-      const uint2 w0 = in0 ? *reinterpret_cast<const uint2*>(b0 + k) : zero, w1 = in1 ? *reinterpret_cast<const uint2*>(b0 + 2 * p.R + k) : zero;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      if (16 * k >= p.R) break;
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          const T* z = s_split + (part * ROWS + 16 * i + g) * ld + target * p.R + k + 4 * t;
+          const T* z = s_split + (part * ROWS + 16 * i + g) * ld + cur.target * p.R + 16 * k + 4 * t;
           const uint2 lo = *reinterpret_cast<const uint2*>(z), hi = *reinterpret_cast<const uint2*>(z + 8 * ld);
           const uint32_t f[4] = {lo.x, hi.x, lo.y, hi.y};
-          mma16816<T>(d[i][0], f, w0.x, w0.y);
-          mma16816<T>(d[i][1], f, w1.x, w1.y);
+          mma16816<T>(d[i][0], f, cur.w[k][0].x, cur.w[k][0].y);
+          mma16816<T>(d[i][1], f, cur.w[k][1].x, cur.w[k][1].y);
         }
     }
 #pragma unroll
@@ -268,42 +342,39 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
       for (int h = 0; h < 2; ++h) {
         const int at = 16 * i + 8 * h + g, row = s_row[at];
         if (row < 0 || !in) continue;
-        const float f = s_factor[at][target];
-        YT* y = reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + p.col0[target] + col;
+        const float f = s_factor[at][cur.target];
+        YT* y = reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + col;
         if constexpr (sizeof(YT) == 4) {
-          float4 v = *reinterpret_cast<float4*>(y);
-          v.x = fmaf(f, d[i][0][2 * h], v.x), v.y = fmaf(f, d[i][0][2 * h + 1], v.y);
-          v.z = fmaf(f, d[i][1][2 * h], v.z), v.w = fmaf(f, d[i][1][2 * h + 1], v.w);
-          *reinterpret_cast<float4*>(y) = v;
+          red_add4(y, f * d[i][0][2 * h], f * d[i][0][2 * h + 1], f * d[i][1][2 * h], f * d[i][1][2 * h + 1]);
         } else {
-          uint2 raw = *reinterpret_cast<uint2*>(y);
-          const YT* e = reinterpret_cast<const YT*>(&raw);
-          raw = make_uint2(pack2<YT>(fmaf(f, d[i][0][2 * h], Tr<YT>::to_f(e[0])), fmaf(f, d[i][0][2 * h + 1], Tr<YT>::to_f(e[1]))),
-                           pack2<YT>(fmaf(f, d[i][1][2 * h], Tr<YT>::to_f(e[2])), fmaf(f, d[i][1][2 * h + 1], Tr<YT>::to_f(e[3]))));
-          *reinterpret_cast<uint2*>(y) = raw;
+          const YT* e = reinterpret_cast<const YT*>(&old[i][h]);
+          *reinterpret_cast<uint2*>(y) = make_uint2(pack2<YT>(fmaf(f, d[i][0][2 * h], Tr<YT>::to_f(e[0])), fmaf(f, d[i][0][2 * h + 1], Tr<YT>::to_f(e[1]))),
+                                                    pack2<YT>(fmaf(f, d[i][1][2 * h], Tr<YT>::to_f(e[2])), fmaf(f, d[i][1][2 * h + 1], Tr<YT>::to_f(e[3]))));
         }
       }
+    cur = next;
   }
+  if (MB == 1 && C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // nobody leaves before all have read
 }
 
-template <typename T, typename YT, int MB>
-static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
-  auto kern = lora_rows_kernel<T, YT, MB>;
+template <typename T, typename YT, int MB, int KS>
+static int launch_lora_rows_of(const LoraRows& p, int64_t tiles, cudaStream_t st) {
+  auto kern = lora_rows_kernel<T, YT, MB, KS>;
   static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
   int dev = 0;
   cudaError_t ae = cudaGetDevice(&dev);
   if (ae == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
-    ae = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (lw_part_floats<T>(LW_RANKS) + LW_RANKS) * 16 * MB * 4);
+    ae = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (lw_row_floats<T, MB>(LW_RANKS) + (MB > 1 ? LW_RANKS : 0)) * 16 * MB * 4);
     if (ae == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   if (ae != cudaSuccess) return cuda_fail(ae, "cudaFuncSetAttribute(lora_rows_kernel)");
   const int TR = p.targets * p.R, ranks = TR > 128 ? 256 : TR > 64 ? 128 : TR > 32 ? 64 : 32;
   int C = LW_CLUSTER;
-  while (C > 1 && tiles * C > 4 * sm_count()) C >>= 1;
+  while (C > 1 && tiles * C > (int64_t)lw_ctas(MB, KS) * sm_count()) C >>= 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C));
   cfg.blockDim = dim3(LW_THREADS);
-  cfg.dynamicSmemBytes = (size_t)(lw_part_floats<T>(ranks) + ranks) * 16 * MB * 4;
+  cfg.dynamicSmemBytes = (size_t)(lw_row_floats<T, MB>(ranks) + (MB > 1 ? ranks : 0)) * 16 * MB * 4;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -315,6 +386,13 @@ static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   return e == cudaSuccess ? B200P_OK : cuda_fail(e, "lora_rows_kernel");
+}
+
+template <typename T, typename YT, int MB>
+static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
+  if (p.R == 16) return launch_lora_rows_of<T, YT, MB, 1>(p, tiles, st);
+  if (p.R == 32) return launch_lora_rows_of<T, YT, MB, 2>(p, tiles, st);
+  return launch_lora_rows_of<T, YT, MB, 4>(p, tiles, st);
 }
 
 }  // namespace b200p
@@ -355,8 +433,7 @@ extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a
   B200P_REQUIRE(M >= 0 && M <= RG_ROWS && adapters > 0 && adapters <= RG_GROUPS, B200P_ERR_ARG, "bad shape: %lld rows, %d adapters", (long long)M, adapters);
   B200P_REQUIRE(tile == 16 || tile == 64, B200P_ERR_ARG, "the plan's tiles have 16 or 64 rows, not %d", tile);
   B200P_REQUIRE(targets > 0 && targets <= LW_TARGETS, B200P_ERR_ARG, "%d targets: 1 to %d", targets, LW_TARGETS);
-  B200P_REQUIRE(R > 0 && R % 16 == 0 && R * targets <= LW_RANKS, B200P_ERR_ARG, "%d targets of rank %d: a multiple of 16, %d in all at most", targets, R,
-                LW_RANKS);
+  B200P_REQUIRE(R > 0 && R % 16 == 0 && R <= LW_RANK, B200P_ERR_ARG, "rank %d: a multiple of 16, %d at most", R, LW_RANK);
   B200P_REQUIRE(K > 0 && K % 8 == 0 && K < (1ll << 24) && ldx >= K, B200P_ERR_ARG, "bad K %lld: a multiple of 8, not above ldx", (long long)K);
   B200P_REQUIRE(host_columns, B200P_ERR_ARG, "null pointer");
   LoraRows p{};

@@ -130,8 +130,7 @@ def test_inner_sizes(K, tile, dtype):
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("tile", [16, 64])
-@pytest.mark.parametrize("R,targets", [(16, 1), (16, 2), (16, 3), (16, 4), (32, 1), (32, 2), (32, 4), (48, 1), (48, 2), (48, 3), (64, 1), (64, 2), (64, 3), (64, 4),
-                                       (80, 3), (96, 2), (128, 2), (256, 1), (240, 1)])
+@pytest.mark.parametrize("R,targets", [(16, 1), (16, 2), (16, 3), (16, 4), (32, 1), (32, 2), (32, 4), (48, 1), (48, 2), (48, 3), (64, 1), (64, 2), (64, 3), (64, 4)])
 def test_ranks_and_targets(R, targets, tile, dtype):
     check(index_of(50, 2), *make(50, 2, 320, R, (72, 8, 16, 200)[:targets], dtype, out="16" if R % 32 else "f32", seed=R), tile)
 
@@ -230,7 +229,7 @@ def test_refusals():
     index = index_of(8, 2).cuda()
     plan = ops.row_groups(index, 2, 16)
     keep = y.clone()
-    for bad in (dict(x=x.float()), dict(x=x[:, ::2]), dict(x=x[:7]), dict(x=x[:, 1:]), dict(a=a.bfloat16()), dict(a=a[:, :, :8]), dict(a=a[:1]),
+    for bad in (dict(x=x.float()), dict(x=x[:, ::2]), dict(x=x[:7]), dict(x=x[:, 1:]), dict(a=a.bfloat16()), dict(a=a[:, :, :8]), dict(a=a[:1]), dict(a=torch.zeros((2, 2, 80, 64), device="cuda").half(), b=torch.zeros((2, 40, 80), device="cuda").half()),
                 dict(b=b[:, :39]), dict(b=b.float()), dict(scales=s.half()), dict(scales=s[:1]), dict(y=y.bfloat16()), dict(y=y[:7]), dict(y=y[:, :40]),
                 dict(columns=columns[:1]), dict(columns=((0, 32), (30, 8))), dict(columns=((0, 36), (40, 4))), dict(columns=((2, 32), (40, 8))),
                 dict(columns=((0, 32), (60, 8))), dict(columns=((-8, 32), (40, 8))), dict(x=x.cpu()), dict(plan=plan._replace(rows=9)),

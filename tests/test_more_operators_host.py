@@ -55,7 +55,7 @@ def test_lora_rows_refuses_before_it_launches():
                  a["ldx"], a["ldy"], a["dtype"], a["f32"], 0)
 
     for bad in (dict(dtype=_lib.F32), dict(dtype=7), dict(M=-1), dict(M=(1 << 20) + 1), dict(adapters=0), dict(adapters=1025), dict(tile=32), dict(targets=0),
-                dict(targets=5, columns=(0, 8) * 5), dict(R=0), dict(R=24), dict(R=144), dict(K=0), dict(K=12), dict(ldx=56), dict(columns=(0, 64, 128, 16)),
+                dict(targets=5, columns=(0, 8) * 5), dict(R=0), dict(R=24), dict(R=80), dict(K=0), dict(K=12), dict(ldx=56), dict(columns=(0, 64, 128, 16)),
                 dict(columns=(0, 64, 60, 8)), dict(columns=(0, 0, 64, 8)), dict(columns=(-8, 64, 64, 8)), dict(columns=(0, 60, 64, 8)), dict(x=0), dict(plan=0),
                 dict(a=0), dict(b=0), dict(scales=0), dict(y=0)):
         assert call(**bad) == -1, bad
