@@ -100,54 +100,50 @@ struct LoraRows {
   int col0[LW_TARGETS], start[LW_TARGETS + 1], tile0[LW_TARGETS + 1];      // first column of y, of b; first run of 16 columns
 };
 
-template <typename T> struct LwParts { static constexpr int N = 2; };
-template <> struct LwParts<__nv_bfloat16> { static constexpr int N = 3; };
+// (two bf16 numbers where y is rounded to bf16: 16 bits of z against y's 8)
+template <typename T, typename YT> struct LwParts { static constexpr int N = std::is_same<T, __nv_bfloat16>::value && sizeof(YT) == 4 ? 3 : 2; };
 // Shared floats of a row: the warps' parts of z, of which the first becomes this CTA's, and the split z, which has room behind it (16 rows) or takes the
 // parts' place when the whole cluster has read them (64 rows: two CTAs fit an SM).
-template <typename T, int MB>
+template <typename T, typename YT, int MB>
 __host__ __device__ constexpr int lw_row_floats(int ranks) {
-  const int split = LwParts<T>::N * (ranks + 8) / 2 + (MB == 1 ? ranks : 0);
+  const int split = LwParts<T, YT>::N * (ranks + 8) / 2 + (MB == 1 ? ranks : 0);
   return split > LW_WARPS * 32 ? split : LW_WARPS * 32;
 }
-
-__host__ __device__ constexpr int lw_ctas(int mb, int ks) { return mb == 1 && ks < 4 ? 3 : 2; }      // of an SM
 
 __device__ __forceinline__ void red_add4(float* p, float a, float b, float c, float d) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
-// What a lane needs of b for a run of 16 columns: R ranks of its two columns in the products' order, column j of the two products' eight being
-// 4 (j / 2) + j % 2 and two further, so that a lane's four results are neighbours.
-template <typename T, int KS>
+// A run of 16 columns: a lane's four are neighbours, as the two products' column j is 4 (j / 2) + j % 2 and two further.
 struct LwRun {
-  int target, col, width;
-  uint2 w[KS][2];
-  __device__ __forceinline__ void load(const LoraRows& p, const T* b, int run, int run1) {
-    if (run >= run1) return;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    target = 0;
+  int target, c0, width;
+  __device__ __forceinline__ LwRun(const LoraRows& p, int run) : target(0) {
 #pragma unroll
     for (int k = 1; k < LW_TARGETS; ++k)
       if (k < p.targets && run >= p.tile0[k]) target = k;
     width = p.start[target + 1] - p.start[target];
-    const int c0 = (run - p.tile0[target]) * 16;
-    col = c0 + 4 * t;
-    const int n0 = c0 + 4 * (g >> 1) + (g & 1);
-    const T* at = b + (int64_t)(p.start[target] + n0) * p.R + 4 * t;
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        w[k][h] = n0 + 2 * h < width && 16 * k < p.R ? *reinterpret_cast<const uint2*>(at + 2 * h * p.R + 16 * k) : make_uint2(0, 0);
+    c0 = (run - p.tile0[target]) * 16;
   }
 };
+template <typename T, int KS>
+__device__ __forceinline__ void lw_load(const LoraRows& p, const T* b, int run, int run1, uint2 (&w)[KS][2]) {
+  if (run >= run1) return;
+  const LwRun r(p, run);
+  const int lane = threadIdx.x & 31, g = lane >> 2, n0 = r.c0 + 4 * (g >> 1) + (g & 1);
+  const T* at = b + (int64_t)(p.start[r.target] + n0) * p.R + 4 * (lane & 3);
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      w[k][h] = n0 + 2 * h < r.width && 16 * k < p.R ? *reinterpret_cast<const uint2*>(at + 2 * h * p.R + 16 * k) : make_uint2(0, 0);
+}
 
 // MB blocks of 16 rows; YT: y's type; KS: 16 ranks each (R or more).  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits
 // this CTA's part of K.  Operands come straight from memory, 16 bytes a lane: the order of k within a product is free as long as both operands have the same.
 template <typename T, typename YT, int MB, int KS>
-__global__ void __launch_bounds__(LW_THREADS, lw_ctas(MB, KS))
+__global__ void __launch_bounds__(LW_THREADS, 2)
 lora_rows_kernel(const __grid_constant__ LoraRows p) {
-  constexpr int ROWS = 16 * MB, PARTS = LwParts<T>::N, NZ = (16 * KS + 31) / 32;
+  constexpr int ROWS = 16 * MB, PARTS = LwParts<T, YT>::N, NZ = (16 * KS + 31) / 32;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int s_row[ROWS];
   __shared__ float s_factor[ROWS][LW_TARGETS];
@@ -163,8 +159,6 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
   if (tile_index >= tiles) return;                                // (the whole cluster)
   const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.x * p.N * p.R;
   const int runs = p.tile0[p.targets], run0 = (int)((int64_t)runs * rank / C), run1 = (int)((int64_t)runs * (rank + 1) / C);
-  LwRun<T, KS> cur, next;
-  cur.load(p, b, run0 + warp, run1);                              // on its way beside the first product
   if ((int)threadIdx.x < ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
   __syncthreads();
 
@@ -192,27 +186,39 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
     }
     const int s0 = (int)((int64_t)p.steps * rank / C), s1 = (int)((int64_t)p.steps * (rank + 1) / C);
     const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll(MB == 1 ? 2 : 1)
-    for (int s = s0 + my_k; s < s1; s += wk) {
-      const bool in = s * 32 + 8 * t < p.K;
-      uint4 av[4], xv[MB][2];
+    constexpr int DEEP = MB == 1 ? 4 : 1;                         // steps whose loads are under way together
+#pragma unroll 1
+    for (int s = s0 + my_k; s < s1; s += DEEP * wk) {
+      uint4 av[DEEP][4], xv[DEEP][MB][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) av[j] = in && ar[j] ? *reinterpret_cast<const uint4*>(ar[j] + s * 32) : zero;
+      for (int u = 0; u < DEEP; ++u) {
+        const int k = (s + u * wk) * 32;
+        const bool in = s + u * wk < s1 && k + 8 * t < p.K;
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
+        for (int j = 0; j < 4; ++j) av[u][j] = in && ar[j] ? *reinterpret_cast<const uint4*>(ar[j] + k) : zero;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) xv[i][h] = in && xr[i][h] ? *reinterpret_cast<const uint4*>(xr[i][h] + s * 32) : zero;
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const uint32_t lo[4] = {xv[i][0].x, xv[i][1].x, xv[i][0].y, xv[i][1].y}, hi[4] = {xv[i][0].z, xv[i][1].z, xv[i][0].w, xv[i][1].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma16816<T>(acc[i][j], lo, av[j].x, av[j].y);
-          mma16816<T>(acc[i][j], hi, av[j].z, av[j].w);
-        }
+          for (int h = 0; h < 2; ++h) xv[u][i][h] = in && xr[i][h] ? *reinterpret_cast<const uint4*>(xr[i][h] + k) : zero;
       }
+#pragma unroll
+      for (int u = 0; u < DEEP; ++u)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          const uint32_t lo[4] = {xv[u][i][0].x, xv[u][i][1].x, xv[u][i][0].y, xv[u][i][1].y};
+          const uint32_t hi[4] = {xv[u][i][0].z, xv[u][i][1].z, xv[u][i][0].w, xv[u][i][1].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            mma16816<T>(acc[i][j], lo, av[u][j].x, av[u][j].y);
+            mma16816<T>(acc[i][j], hi, av[u][j].z, av[u][j].w);
+          }
+        }
     }
   }
+  constexpr int AHEAD = MB == 1 ? 8 / KS : 1;                      // runs whose b is under way
+  uint2 w[AHEAD][KS][2];
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) lw_load<T, KS>(p, b, run0 + warp + u * LW_WARPS, run1, w[u]);
   {
     float* part = s_part + my_k * ROWS * ranks + my_n;
 #pragma unroll
@@ -226,7 +232,9 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
   __syncthreads();
   for (int i = threadIdx.x; i < tile.z * ranks; i += LW_THREADS) {
     float sum = 0.f;
-    for (int k = 0; k < wk; ++k) sum += s_part[k * ROWS * ranks + i];
+#pragma unroll
+    for (int k = 0; k < LW_WARPS; ++k)
+      if (k < wk) sum += s_part[k * ROWS * ranks + i];
     s_part[i] = sum;                                              // (nobody else looks at place i of the first part)
   }
   if (C > 1) cluster.sync();
@@ -279,7 +287,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
     __syncthreads();
   } else {
     // (a sum that is needed again takes the first part's place in this CTA when the others have read it)
-    float* s_z = s_part + lw_row_floats<T, MB>(ranks) * ROWS;
+    float* s_z = s_part + lw_row_floats<T, YT, MB>(ranks) * ROWS;
     for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
       float z[NZ];
       whole(i, z);
@@ -303,56 +311,61 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
 
   // ---- this CTA's columns: 16 at a time, of which a lane has four neighbours -----------------------------------------------------
 #pragma unroll 1
-  for (int run = run0 + warp; run < run1; run += LW_WARPS) {
-    next.load(p, b, run + LW_WARPS, run1);
-    const bool in = cur.col < cur.width;
-    const int64_t col = p.col0[cur.target] + cur.col;
-    uint2 old[MB][2];                                             // 16-bit y, on its way beside the products (fp32 is added in memory)
-    if constexpr (sizeof(YT) == 2) {
+  for (int first = run0 + warp; first < run1; first += AHEAD * LW_WARPS) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int run = first + u * LW_WARPS;
+      if (run >= run1) break;
+      const LwRun r(p, run);
+      const bool in = r.c0 + 4 * t < r.width;
+      const int64_t col = p.col0[r.target] + r.c0 + 4 * t;
+      uint2 old[MB][2];                                           // 16-bit y, on its way beside the products (fp32 is added in memory)
+      if constexpr (sizeof(YT) == 2) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = s_row[16 * i + 8 * h + g];
+            old[i][h] = row >= 0 && in ? *reinterpret_cast<const uint2*>(reinterpret_cast<const YT*>(p.y) + (int64_t)row * p.ldy + col) : make_uint2(0, 0);
+          }
+      }
+      float d[MB][2][4];
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) d[i][h][0] = d[i][h][1] = d[i][h][2] = d[i][h][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if (16 * k >= p.R) break;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) {
+            const T* z = s_split + (part * ROWS + 16 * i + g) * ld + r.target * p.R + 16 * k + 4 * t;
+            const uint2 lo = *reinterpret_cast<const uint2*>(z), hi = *reinterpret_cast<const uint2*>(z + 8 * ld);
+            const uint32_t f[4] = {lo.x, hi.x, lo.y, hi.y};
+            mma16816<T>(d[i][0], f, w[u][k][0].x, w[u][k][0].y);
+            mma16816<T>(d[i][1], f, w[u][k][1].x, w[u][k][1].y);
+          }
+      }
+      lw_load<T, KS>(p, b, run + AHEAD * LW_WARPS, run1, w[u]);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int row = s_row[16 * i + 8 * h + g];
-          old[i][h] = row >= 0 && in ? *reinterpret_cast<const uint2*>(reinterpret_cast<const YT*>(p.y) + (int64_t)row * p.ldy + col) : make_uint2(0, 0);
+          const int at = 16 * i + 8 * h + g, row = s_row[at];
+          if (row < 0 || !in) continue;
+          const float f = s_factor[at][r.target];
+          YT* y = reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + col;
+          if constexpr (sizeof(YT) == 4) {
+            red_add4(y, f * d[i][0][2 * h], f * d[i][0][2 * h + 1], f * d[i][1][2 * h], f * d[i][1][2 * h + 1]);
+          } else {
+            const YT* e = reinterpret_cast<const YT*>(&old[i][h]);
+            *reinterpret_cast<uint2*>(y) = make_uint2(pack2<YT>(fmaf(f, d[i][0][2 * h], Tr<YT>::to_f(e[0])), fmaf(f, d[i][0][2 * h + 1], Tr<YT>::to_f(e[1]))),
+                                                      pack2<YT>(fmaf(f, d[i][1][2 * h], Tr<YT>::to_f(e[2])), fmaf(f, d[i][1][2 * h + 1], Tr<YT>::to_f(e[3]))));
+          }
         }
     }
-    float d[MB][2][4];
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) d[i][h][0] = d[i][h][1] = d[i][h][2] = d[i][h][3] = 0.f;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      if (16 * k >= p.R) break;
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-          const T* z = s_split + (part * ROWS + 16 * i + g) * ld + cur.target * p.R + 16 * k + 4 * t;
-          const uint2 lo = *reinterpret_cast<const uint2*>(z), hi = *reinterpret_cast<const uint2*>(z + 8 * ld);
-          const uint32_t f[4] = {lo.x, hi.x, lo.y, hi.y};
-          mma16816<T>(d[i][0], f, cur.w[k][0].x, cur.w[k][0].y);
-          mma16816<T>(d[i][1], f, cur.w[k][1].x, cur.w[k][1].y);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int at = 16 * i + 8 * h + g, row = s_row[at];
-        if (row < 0 || !in) continue;
-        const float f = s_factor[at][cur.target];
-        YT* y = reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + col;
-        if constexpr (sizeof(YT) == 4) {
-          red_add4(y, f * d[i][0][2 * h], f * d[i][0][2 * h + 1], f * d[i][1][2 * h], f * d[i][1][2 * h + 1]);
-        } else {
-          const YT* e = reinterpret_cast<const YT*>(&old[i][h]);
-          *reinterpret_cast<uint2*>(y) = make_uint2(pack2<YT>(fmaf(f, d[i][0][2 * h], Tr<YT>::to_f(e[0])), fmaf(f, d[i][0][2 * h + 1], Tr<YT>::to_f(e[1]))),
-                                                    pack2<YT>(fmaf(f, d[i][1][2 * h], Tr<YT>::to_f(e[2])), fmaf(f, d[i][1][2 * h + 1], Tr<YT>::to_f(e[3]))));
-        }
-      }
-    cur = next;
   }
   if (MB == 1 && C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // nobody leaves before all have read
 }
@@ -364,17 +377,17 @@ static int launch_lora_rows_of(const LoraRows& p, int64_t tiles, cudaStream_t st
   int dev = 0;
   cudaError_t ae = cudaGetDevice(&dev);
   if (ae == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
-    ae = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (lw_row_floats<T, MB>(LW_RANKS) + (MB > 1 ? LW_RANKS : 0)) * 16 * MB * 4);
+    ae = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (lw_row_floats<T, YT, MB>(LW_RANKS) + (MB > 1 ? LW_RANKS : 0)) * 16 * MB * 4);
     if (ae == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   if (ae != cudaSuccess) return cuda_fail(ae, "cudaFuncSetAttribute(lora_rows_kernel)");
   const int TR = p.targets * p.R, ranks = TR > 128 ? 256 : TR > 64 ? 128 : TR > 32 ? 64 : 32;
   int C = LW_CLUSTER;
-  while (C > 1 && tiles * C > (int64_t)lw_ctas(MB, KS) * sm_count()) C >>= 1;
+  while (C > 1 && tiles * C > 2 * sm_count()) C >>= 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C));
   cfg.blockDim = dim3(LW_THREADS);
-  cfg.dynamicSmemBytes = (size_t)(lw_row_floats<T, MB>(ranks) + (MB > 1 ? ranks : 0)) * 16 * MB * 4;
+  cfg.dynamicSmemBytes = (size_t)(lw_row_floats<T, YT, MB>(ranks) + (MB > 1 ? ranks : 0)) * 16 * MB * 4;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
