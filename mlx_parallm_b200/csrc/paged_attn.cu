@@ -77,7 +77,13 @@ struct PagedAttn {
   uint64_t inv_tpp;    // 2^36 / (tiles of a page, 256 at most), rounded up: tile * inv_tpp >> 36 is the page's index for any tile below 2^26
   int tpp, last;       // tiles of a page; CTAs for small shares at the line's end
   int cap, pitch;      // visible slots a token can have, in whole tiles; heads of a line of scores, a power of two
+  // behind shared slots (paged_shared.cuh): a token's group, the groups' shared slots, the parts of items that lie in one share
+  const int32_t *index, *prefix;
+  int groups;
+  float* whole;        // [M, items, rows of a block, D + 4]
 };
+
+__device__ __forceinline__ int shared_slots(const int32_t* index, const int32_t* prefix, int groups, const PageTable& pt, int t, int seen);
 
 // The work is cut evenly however unequal the rows are: every token's visible tiles are counted in units of one tile per warp, the units of all
 // (token, key head, block of query heads) items are laid end to end, and each resident CTA takes an equal share of that line.  An item in one share is
@@ -90,15 +96,20 @@ struct Token {
   int row, units;
   Span span;
   __device__ Token() : row(-1), units(0), span(0, 0, 0) {}
-  __device__ Token(const PagedAttn& a, int row_, int slots, int warps) : row(row_), units(0), span(0, 0, 0) {
+  // from > 0: only the slots from there on
+  __device__ Token(const PagedAttn& a, int row_, int slots, int from, int warps) : row(row_), units(0), span(0, 0, 0) {
     if (row >= 0) {
-      span = Span(slots, a.first, a.window);
+      span = from == 0 ? Span(slots, a.first, a.window) : slots > from ? Span(slots, 0, slots - from) : Span(0, 0, 0);
       units = span.tiles > warps ? (span.tiles + warps - 1) / warps : 1;      // a token that sees nothing: one, for its zeros
     }
   }
-  __device__ Token(const PagedAttn& a, int t, int warps) : Token() {
+  template <bool TAIL>
+  static __device__ Token of(const PagedAttn& a, int t, int warps, int* begins = nullptr) {
     const int r = a.t_row[t];
-    if (r >= 0 && r < a.pt.rows) *this = Token(a, r, slots_seen(a.pt, a.t_slot[t]), warps);
+    if (r < 0 || r >= a.pt.rows) return Token();
+    const int n = slots_seen(a.pt, a.t_slot[t]), from = TAIL ? shared_slots(a.index, a.prefix, a.groups, a.pt, t, n) : 0;
+    if (TAIL && begins) *begins = from;
+    return Token(a, r, n, from, warps);
   }
 };
 
@@ -135,19 +146,21 @@ struct Shares {
 
 // The tokens of a call of up to PA_TOKENS: their rows and where their slots end.  (Under a full stream of keys a look at global memory
 // takes 2 to 3 us, L2 hit or not.)
+template <bool TAIL>
 struct Tokens {
-  int row[PA_TOKENS], slots[PA_TOKENS];
+  int row[PA_TOKENS], slots[PA_TOKENS], from[TAIL ? PA_TOKENS : 1];
 };
 
 // A position in a share: the token, and of its units the run [a, b) of one item.
+template <bool TAIL>
 struct Cursor {
   unsigned u, end, base;
   int t, item, a, b;
   Token tok;
-  __device__ void load(const PagedAttn& p, const Tokens& ts, int warps) {
-    tok = p.M <= PA_TOKENS ? Token(p, ts.row[t], ts.slots[t], warps) : Token(p, t, warps);
+  __device__ void load(const PagedAttn& p, const Tokens<TAIL>& ts, int warps) {
+    tok = p.M <= PA_TOKENS ? Token(p, ts.row[t], ts.slots[t], TAIL ? ts.from[t] : 0, warps) : Token::of<TAIL>(p, t, warps);
   }
-  __device__ bool next(const PagedAttn& p, const Tokens& ts, int items, int warps) {
+  __device__ bool next(const PagedAttn& p, const Tokens<TAIL>& ts, int items, int warps) {
     if (u >= end) return false;
     while (u - base >= (unsigned)(tok.units * items)) {
       base += tok.units * items;
@@ -475,11 +488,11 @@ __device__ __forceinline__ void store_row4(T* out, int d, float4 v, int perm) {
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
-template <int W>
+template <int W, bool TAIL>
 struct Plan {
   unsigned sum[W], live[W], base;
   int t, part[W];
-  Tokens tok;
+  Tokens<TAIL> tok;
   Run run[4];
 };
 
@@ -488,13 +501,16 @@ __device__ __forceinline__ void meet(int barrier) { asm volatile("barrier.cta.sy
 
 // W warps that stream and multiply, and one that works out what they do next.  They meet at the end of every run.
 // The code has to stay small: it is fetched through the memory that streams the keys, and when it had 90 KB every seldom taken path took microseconds.
-template <typename E>
+// TAIL: only the slots behind the shared ones; every item leaves parts for the launch that joins them with those of the shared slots.  The launch before
+// this one (paged_prefix_kernel) waits for everything older before it lets this one begin, and writes nothing that is read here, so this one waits
+// for it at its end.
+template <typename E, bool TAIL>
 __global__ void __launch_bounds__(E::WARPS * 32 + 32, E::CTAS)
 paged_attn_kernel(const __grid_constant__ PagedAttn a) {
   using T = typename E::T;
   constexpr int W = E::WARPS, THREADS = W * 32;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ Plan<W> s;
+  __shared__ Plan<W, TAIL> s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = E::dim(a), chunks = D * (int)sizeof(T) / 16;
   const int per = a.H / a.G, blocks = (per + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
@@ -504,7 +520,7 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
     if (line < tables) prefetch_l2(reinterpret_cast<const uint8_t*>(a.pt.table) + line * 128);
     else if (line - tables < queries) prefetch_l2(reinterpret_cast<const uint8_t*>(a.q) + (line - tables) * 128);
   }
-  pdl_wait();
+  if (!TAIL) pdl_wait();
 
   // ---- the plan: units of all tokens, the shares, the token in which this CTA's begins -------------------------------------
   const int chunk = (a.M + THREADS - 1) / THREADS;
@@ -512,13 +528,15 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
   unsigned mine = 0, live = 0;
 #pragma unroll 1
   for (int t = t0; t < t1; ++t) {
-    const Token tok(a, t, W);
+    int from = 0;
+    const Token tok = Token::of<TAIL>(a, t, W, &from);
     mine += tok.units * items;
     live += tok.units > 0;
     if (blockIdx.x == 0 && (a.t_row[t] >= a.pt.rows || (a.t_row[t] >= 0 && a.t_slot[t] >= table_slots(a.pt)))) atomicAdd(&g_paged_attn_fault, 1u);
     if (a.M <= PA_TOKENS) {
       s.tok.row[t] = tok.row;
-      s.tok.slots[t] = tok.span.n;
+      s.tok.slots[t] = TAIL && tok.row >= 0 ? slots_seen(a.pt, a.t_slot[t]) : tok.span.n;
+      if (TAIL) s.tok.from[t] = from;
     }
   }
   unsigned before = mine;
@@ -543,11 +561,14 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
   }
   pdl_launch_dependents();                                        // (the join waits for this launch's end; until then it has no room anyway)
   const Shares sh(U, n_items, gridDim.x - a.last, a.last);
-  if (blockIdx.x >= sh.n) return;
+  if (blockIdx.x >= sh.n) {
+    if (TAIL) pdl_wait();
+    return;
+  }
   const unsigned ub = sh.begin(blockIdx.x);
 #pragma unroll 1
   for (int t = t0; t < t1; ++t) {
-    const unsigned n = (a.M <= PA_TOKENS ? Token(a, s.tok.row[t], s.tok.slots[t], W) : Token(a, t, W)).units * items;
+    const unsigned n = (a.M <= PA_TOKENS ? Token(a, s.tok.row[t], s.tok.slots[t], TAIL ? s.tok.from[t] : 0, W) : Token::of<TAIL>(a, t, W)).units * items;
     if (ub - before < n) {
       s.t = t;
       s.base = before;
@@ -558,7 +579,7 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
 
   // ---- the warp for the runs and the parts ----------------------------------------------------------------------------------
   if (warp == W) {
-    Cursor c;
+    Cursor<TAIL> c;
     c.u = ub, c.end = sh.begin(blockIdx.x + 1), c.base = s.base, c.t = s.t;
     c.load(a, s.tok, W);
     // runs 0 to 2 before the others start, then run n + 3 when run n has ended
@@ -581,7 +602,10 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
       if (n < 2) continue;
       if (n == 2) __syncthreads();
       meet<THREADS + 32>(2);                                      // the end of run n - 2
-      if (s.run[(n - 1) & 3].tile < 0) return;
+      if (s.run[(n - 1) & 3].tile < 0) {
+        if (TAIL) pdl_wait();
+        return;
+      }
     }
   }
 
@@ -717,8 +741,8 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
     const int part = (warp * E::STAGES + ld_stage) * E::tile_bytes(D);
     if (lane == 0) s.part[warp] = part;
     const int head = r.head;
-    const bool cut = r.part >= 0;
-    float* rec = a.rec + (int64_t)r.part * E::ROWS * (D + 4);
+    const bool cut = TAIL || r.part >= 0;
+    float* rec = (TAIL && r.part < 0 ? a.whole + (int64_t)r.line * E::ROWS * (D + 4) : a.rec + (int64_t)r.part * E::ROWS * (D + 4));
 #pragma unroll 1
     for (int pass = 0; pass * 8 < rows; ++pass) {
       e.publish(reinterpret_cast<float*>(smem + E::Q_BYTES + part), pass, D);
@@ -764,7 +788,10 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
       if (pass * 8 + 8 < rows) meet<THREADS>(1);
     }
     meet<THREADS + 32>(2);
-    if (!more) return;
+    if (!more) {
+      if (TAIL) pdl_wait();
+      return;
+    }
   }
 }
 
@@ -1019,6 +1046,12 @@ paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks,
   }
 }
 
+}  // namespace b200p
+
+#include "paged_shared.cuh"
+
+namespace b200p {
+
 // ------------------------------------------------------------------------------------------------ host
 // visible slots a token can have, in whole tiles
 static int64_t visible_cap(int64_t slots, int64_t first, int64_t window) {
@@ -1032,13 +1065,14 @@ static size_t parts_bytes(int64_t M, int H) { return round256((size_t)M * H * 8)
 static size_t rec_bytes(int D) { return round256((size_t)(2 * sm_count() + last_ctas(2 * sm_count())) * 2 * 16 * (D + 4) * 4); }
 static size_t stat_bytes(int64_t M, int H) { return round256((size_t)M * H * 8); }
 
-template <typename E>
-static int launch_paged(PagedAttn a, cudaStream_t st) {
+// The streaming launch; its grid and what it needs to know are written into a.
+template <typename E, bool TAIL>
+static int launch_stream(PagedAttn& a, cudaStream_t st) {
   const int smem = E::Q_BYTES + E::WARPS * E::STAGES * E::tile_bytes(a.D);
   const int blocks = (a.H / a.G + E::ROWS - 1) / E::ROWS, items = a.G * blocks;
   B200P_REQUIRE((int64_t)a.M * items * (a.cap / PA_TILE / E::WARPS + 1) < (1ll << 31) && (int64_t)a.M * a.H < (1ll << 31) && items < 65536, B200P_ERR_ARG,
                 "%d tokens of %d key heads over %d slots: too many for one call", a.M, a.G, a.cap);
-  auto kern = paged_attn_kernel<E>;
+  auto kern = paged_attn_kernel<E, TAIL>;
   static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1057,8 +1091,15 @@ static int launch_paged(PagedAttn a, cudaStream_t st) {
   while (a.pitch < E::ROWS && a.pitch < a.H / a.G) a.pitch *= 2;
   launch_pdl(kern, (unsigned)grid, E::WARPS * 32 + 32, smem, st, a);
   B200P_LAUNCH_CHECK("paged_attn_kernel");
+  return B200P_OK;
+}
+
+template <typename E>
+static int launch_paged(PagedAttn a, cudaStream_t st) {
+  const int rc = launch_stream<E, false>(a, st);
+  if (rc) return rc;
   using T = typename E::T;
-  const int per = a.H / a.G, rows_log2 = E::ROWS == 4 ? 2 : E::ROWS == 8 ? 3 : 4;
+  const int per = a.H / a.G, blocks = (per + E::ROWS - 1) / E::ROWS, items = a.G * blocks, rows_log2 = E::ROWS == 4 ? 2 : E::ROWS == 8 ? 3 : 4;
   const dim3 heads((unsigned)per, (unsigned)a.G, (unsigned)a.M);
   const bool few = (int64_t)a.M * a.H <= 4 * sm_count();             // CTAs of the join
   if (a.mass) {
@@ -1093,6 +1134,61 @@ static int launch_paged_type(const PagedAttn& a, cudaStream_t st) {
   const bool four = a.H / a.G <= 4;
   if (a.D <= 128) return four ? launch_paged<FmaEngine<T, 1, 4>>(a, st) : launch_paged<FmaEngine<T, 1, 8>>(a, st);
   return four ? launch_paged<FmaEngine<T, 2, 4>>(a, st) : launch_paged<FmaEngine<T, 2, 8>>(a, st);
+}
+
+// ---- behind shared slots ------------------------------------------------------------------------------------------------------
+// Which calls go by groups: those that the matrix instructions serve.  (fp32 and other sizes are bound by their FMAs, of which sharing saves none.)
+static bool shared_served(int H, int G, int D, int dtype) {
+  return dtype != B200P_F32 && H / G <= PS_ROWS && (D == 64 || D == 80 || D == 96 || D == 128 || D == 256);
+}
+static int shared_tile(int H, int G) { return H / G < PS_ROWS ? PS_ROWS / (H / G) : 1; }
+static int64_t shared_rows(int H, int G) {                          // of a token's items with the rows that blocks are filled up to
+  const int per = H / G;
+  return (int64_t)G * (per <= 8 ? 8 : (per + 15) / 16 * 16);
+}
+static size_t whole_bytes(int64_t M, int H, int G, int D) { return round256((size_t)M * shared_rows(H, G) * (D + 4) * 4); }
+static size_t prefix_bytes(int64_t M, int H, int G, int D, int groups) {
+  return round256(((size_t)row_group_tiles(M, groups, shared_tile(H, G)) * G + sm_count()) * PS_ROWS * (D + 4) * 4);
+}
+static size_t info_bytes(int64_t M) { return round256((size_t)M * 16 + 16); }
+
+template <typename T, int D, int NB>
+static int launch_shared(PagedAttn a, PagedPrefix p, int64_t tiles, cudaStream_t st) {
+  using E = TcEngine<T, D, NB>;
+  auto kern = paged_prefix_kernel<T, D>;
+  static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixTile<T, D>::SMEM);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_prefix_kernel)");
+  const int64_t slots = (int64_t)a.pt.width * a.pt.page, units = tiles * a.G * ((slots + PrefixTile<T, D>::KT - 1) / PrefixTile<T, D>::KT);
+  B200P_REQUIRE(units < (1ll << 31), B200P_ERR_ARG, "%lld tiles of %d key heads over %lld slots: too many for one call", (long long)tiles, a.G, (long long)slots);
+  const unsigned ctas = (unsigned)(units < sm_count() ? units : sm_count());
+  p.tpp = a.pt.page / PA_TILE;
+  p.inv_tpp = ((1ull << 36) + p.tpp - 1) / p.tpp;
+  launch_pdl(kern, ctas, PS_WARPS * 32, PrefixTile<T, D>::SMEM, st, p);
+  B200P_LAUNCH_CHECK("paged_prefix_kernel");
+  const int rc = launch_stream<E, true>(a, st);
+  if (rc) return rc;
+  const dim3 heads((unsigned)(a.H / a.G), (unsigned)a.G, (unsigned)a.M);
+  launch_pdl(paged_shared_join_kernel<T, D <= 128 ? 1 : 2, E::ROWS, 4>, heads, 4 * 32, 0, st, a, p, (int)ctas);
+  B200P_LAUNCH_CHECK("paged_shared_join_kernel");
+  return B200P_OK;
+}
+
+template <typename T>
+static int launch_shared_type(const PagedAttn& a, const PagedPrefix& p, int64_t tiles, cudaStream_t st) {
+  const bool few = a.H / a.G <= 8;
+  switch (a.D) {
+    case 64: return few ? launch_shared<T, 64, 1>(a, p, tiles, st) : launch_shared<T, 64, 2>(a, p, tiles, st);
+    case 80: return few ? launch_shared<T, 80, 1>(a, p, tiles, st) : launch_shared<T, 80, 2>(a, p, tiles, st);
+    case 96: return few ? launch_shared<T, 96, 1>(a, p, tiles, st) : launch_shared<T, 96, 2>(a, p, tiles, st);
+    case 128: return few ? launch_shared<T, 128, 1>(a, p, tiles, st) : launch_shared<T, 128, 2>(a, p, tiles, st);
+    default: return launch_shared<T, 256, 1>(a, p, tiles, st);
+  }
 }
 
 }  // namespace b200p
@@ -1151,4 +1247,53 @@ extern "C" int b200p_paged_attn(const void* q, const void* kpages, const void* v
   a.scores = (float*)(ws + stat_bytes(M, H));
   B200P_DISPATCH_DTYPE(dtype, T, return (launch_paged_type<T>(a, (cudaStream_t)stream)));
   return B200P_OK;
+}
+
+extern "C" int b200p_paged_attn_shared_tile(int H, int G) { return G > 0 && H >= G && H % G == 0 ? shared_tile(H, G) : 0; }
+
+extern "C" size_t b200p_paged_attn_shared_workspace_bytes(int64_t M, int H, int G, int D, int groups) {
+  if (M <= 0 || G <= 0 || H < G || H % G || D <= 0 || groups <= 0 || groups > RG_GROUPS) return 0;
+  return workspace_bytes(M, H, D, 0, 0) + whole_bytes(M, H, G, D) + prefix_bytes(M, H, G, D, groups) + info_bytes(M);
+}
+
+extern "C" int b200p_paged_attn_shared(const void* q, const void* kpages, const void* vpages, const int32_t* table, const int32_t* t_row,
+                                       const int32_t* t_slot, void* out, const int32_t* index, const int32_t* prefix, const int32_t* plan, int64_t M, int H,
+                                       int G, int D, int groups, int tile, int64_t P, int page, int rows, int width, float scale, int dtype, int flags,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+  B200P_REQUIRE(M == 0 || (index && prefix && plan), B200P_ERR_ARG, "null pointer");
+  B200P_REQUIRE(groups > 0 && groups <= RG_GROUPS, B200P_ERR_ARG, "%d groups: 1 to %d", groups, RG_GROUPS);
+  B200P_REQUIRE(G > 0 && H > 0 && H % G == 0, B200P_ERR_ARG, "bad head counts %d/%d", H, G);
+  B200P_REQUIRE(tile == shared_tile(H, G), B200P_ERR_ARG, "the plan's tiles have %d rows for these heads, not %d", shared_tile(H, G), tile);
+  B200P_REQUIRE(aligned(plan, 16), B200P_ERR_ALIGN, "the plan must be 16-byte aligned");
+  B200P_REQUIRE(M <= 0 || (workspace && workspace_bytes >= b200p_paged_attn_shared_workspace_bytes(M, H, G, D, groups)), B200P_ERR_ARG,
+                "workspace of paged attention behind shared slots too small");
+  if (M <= 0 || !shared_served(H, G, D, dtype))                     // (the other checks are paged attention's)
+    return b200p_paged_attn(q, kpages, vpages, nullptr, table, t_row, t_slot, out, M, H, G, D, P, page, rows, width, scale, 0, 0, dtype, flags, workspace,
+                            workspace_bytes, stream);
+  PdlClass pdl_cls(8);
+  const PageTable pt{table, P, rows, width, page};
+  const int rc = check_pages(kpages, vpages, pt, G, D, dtype);
+  if (rc) return rc;
+  B200P_REQUIRE(q && out && t_row && t_slot, B200P_ERR_ARG, "null pointer");
+  B200P_REQUIRE(M < 65536, B200P_ERR_ARG, "bad shape: %lld tokens", (long long)M);
+  B200P_REQUIRE((flags & ~B200P_OUT_PERM8) == 0, B200P_ERR_ARG, "unknown flags 0x%x", flags);
+  B200P_REQUIRE(aligned(q, 16) && aligned(out, 16), B200P_ERR_ALIGN, "q and out must be 16-byte aligned");
+  B200P_REQUIRE(aligned(workspace, 256), B200P_ERR_ARG, "workspace not aligned to 256 bytes");
+  PagedAttn a{};
+  a.q = q, a.k = kpages, a.v = vpages, a.out = out, a.pt = pt, a.t_row = t_row, a.t_slot = t_slot;
+  a.M = (int)M, a.H = H, a.G = G, a.D = D, a.out_perm = (flags & B200P_OUT_PERM8) ? 1 : 0;
+  a.scale_log2e = scale * 1.4426950408889634f, a.cap = (int)visible_cap((int64_t)width * page, 0, 0);
+  a.index = index, a.prefix = prefix, a.groups = groups;
+  uint8_t* ws = (uint8_t*)workspace;
+  a.parts = (uint2*)ws;
+  a.rec = (float*)(ws += parts_bytes(M, H));
+  a.whole = (float*)(ws += rec_bytes(D));
+  PagedPrefix p{};
+  p.q = q, p.k = kpages, p.v = vpages, p.pt = pt, p.t_row = t_row, p.t_slot = t_slot, p.index = index, p.prefix = prefix;
+  p.plan = RowGroups{plan, (int)M}, p.M = (int)M, p.H = H, p.G = G, p.groups = groups, p.scale_log2e = a.scale_log2e;
+  p.rec = (float*)(ws += whole_bytes(M, H, G, D));
+  p.info = (int4*)(ws += prefix_bytes(M, H, G, D, groups));
+  p.total = (unsigned*)(p.info + M);
+  const int64_t tiles = row_group_tiles(M, groups, tile);
+  return dtype == B200P_F16 ? launch_shared_type<__half>(a, p, tiles, (cudaStream_t)stream) : launch_shared_type<__nv_bfloat16>(a, p, tiles, (cudaStream_t)stream);
 }

@@ -1,0 +1,367 @@
+// Attention of single tokens of rows whose first slots lie in the same pages (b200p_paged_attn_shared); part of paged_attn.cu.
+//
+//   o = sum_j p_j v_j over a group's shared slots and the row's own ones: either part leaves its maximum m, sum l and unnormalised output, and
+//   o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i,  m = max m_i
+//
+// The shared slots are read once for a tile of up to PS_ROWS query heads of the group's tokens, instead of once for every token: products of 128 rows,
+// which the matrix instructions bound and not the memory.  The own slots go through paged_attn_kernel behind the shared ones, beside this kernel on the same
+// SMs, and a third launch joins the parts of both.
+#pragma once
+#include "rowgroups.cuh"
+
+namespace b200p {
+
+constexpr int PS_ROWS = 128, PS_WARPS = 8;       // query rows of a tile: tokens x query heads of a key head; a warp has 16
+
+struct PagedPrefix {
+  const void *q, *k, *v;
+  PageTable pt;
+  const int32_t *t_row, *t_slot, *index, *prefix;
+  RowGroups plan;
+  int M, H, G, groups;
+  float scale_log2e;
+  uint64_t inv_tpp;
+  int tpp;
+  float* rec;            // [items + CTAs, PS_ROWS, D + 4] parts, of item i in CTA c the one at i + c
+  int4* info;            // [M] the token's tile, its place in it, the tile's first unit, units of an item (0: no shared slot)
+  unsigned* total;       // units of all
+};
+
+// The units (KT shared keys of a tile of tokens and a key head) of all items lie end to end and every CTA has an equal part of them, as in
+// paged_attn_kernel.
+struct PrefixShares {
+  unsigned n, q, r;
+  __device__ PrefixShares(unsigned U, unsigned ctas) : n(min(U, ctas)) {
+    q = n ? U / n : 1;
+    r = U - q * n;
+  }
+  __device__ unsigned begin(unsigned c) const { return c * q + min(c, r); }
+  __device__ unsigned of(unsigned u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
+};
+
+// The slots that a token has in common with its group (of those that the table has).  0: it belongs to none, or stands before their end and reads what it
+// sees by itself.
+__device__ __forceinline__ int shared_slots(const int32_t* index, const int32_t* prefix, int groups, const PageTable& pt, int t, int seen) {
+  const int g = index[t];
+  if ((unsigned)g >= (unsigned)groups) return 0;
+  const int n = min(max(prefix[g], 0), table_slots(pt));
+  return seen < n ? 0 : n;
+}
+
+template <typename T, int D>
+struct PrefixTile {
+  static constexpr int KT = D > 128 ? 32 : 64, STAGES = 3, CHUNKS = D / 8, PIECES = CHUNKS % 8 ? (CHUNKS | 1) : CHUNKS, LINE = PIECES * 16;
+  static constexpr int KV_BYTES = KT * LINE, STAGE = 2 * KV_BYTES, Q_BYTES = PS_ROWS * LINE, SMEM = Q_BYTES + STAGES * STAGE;
+  static __device__ __forceinline__ uint32_t at(int line, int c) { return (uint32_t)(line * LINE + ((CHUNKS % 8 ? c : c ^ (line & 7)) << 4)); }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PS_WARPS * 32, 1)
+paged_prefix_kernel(const __grid_constant__ PagedPrefix a) {
+  using P = PrefixTile<T, D>;
+  constexpr int KT = P::KT, THREADS = PS_WARPS * 32, CHUNKS = P::CHUNKS, NP = KT / 16;
+  // f16: weights up to 2^14 and not 1, so that small ones keep their bits
+  constexpr float SHIFT = std::is_same<T, __half>::value ? 14.f : 0.f;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ unsigned s_sum[PS_WARPS], s_base;
+  __shared__ int s_tile, s_token[PS_ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qr = lane >> 2, qc = lane & 3, mat = lane >> 3, r8 = lane & 7;
+  const int per = a.H / a.G;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- the plan: units of all tiles, this CTA's part ---------------------------------------------------------------------------
+  auto shared = [&](const int4& tile) { return min(max(a.prefix[tile.x], 0), table_slots(a.pt)); };
+  auto live = [&](const int4& tile) {                               // the row of a member that holds the shared slots; -1: none does
+    const int common = shared(tile);
+    for (int i = 0; i < tile.z; ++i) {
+      const int t = a.plan.order()[tile.y + i], row = a.t_row[t];
+      if (row >= 0 && row < a.pt.rows && slots_seen(a.pt, a.t_slot[t]) >= common) return row;
+    }
+    return -1;
+  };
+  auto units = [&](const int4& tile) { return live(tile) < 0 ? 0 : (shared(tile) + KT - 1) / KT; };
+  const int tiles = a.plan.tiles(), chunk = (tiles + THREADS - 1) / THREADS;
+  const int i0 = min(tiles, (int)threadIdx.x * chunk), i1 = min(tiles, i0 + chunk);
+  unsigned mine = 0;
+  for (int i = i0; i < i1; ++i) mine += units(a.plan.tile(i)) * a.G;
+  unsigned before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned x = __shfl_up_sync(~0u, before, o);
+    if (lane >= o) before += x;
+  }
+  if (lane == 31) s_sum[warp] = before;
+  __syncthreads();
+  before -= mine;
+  unsigned U = 0;
+#pragma unroll
+  for (int w = 0; w < PS_WARPS; ++w) {
+    if (w < warp) before += s_sum[w];
+    U += s_sum[w];
+  }
+  const PrefixShares sh(U, gridDim.x);
+  unsigned u = sh.begin(blockIdx.x);
+  const unsigned end = sh.begin(blockIdx.x + 1);
+  for (int i = i0; i < i1; ++i) {
+    const int4 tile = a.plan.tile(i);
+    const int n = units(tile);
+    if (u - before < n * (unsigned)a.G) s_tile = i, s_base = before;
+    if (blockIdx.x == 0)                                            // for the join
+      for (int k = 0; k < tile.z; ++k) a.info[a.plan.order()[tile.y + k]] = make_int4(i, k, (int)before, n);
+    before += n * a.G;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.total = U;
+  if (blockIdx.x >= sh.n) return;
+  __syncthreads();
+  int ti = s_tile;
+  unsigned base = s_base;
+
+  const uint32_t qs = (uint32_t)__cvta_generic_to_shared(smem), ring = qs + P::Q_BYTES;
+  while (u < end) {
+    // ---- the next item: a tile of tokens and a key head --------------------------------------------------------------------------
+    int4 tile = a.plan.tile(ti);
+    int n = units(tile);
+    while (u - base >= n * (unsigned)a.G) {
+      base += n * a.G;
+      tile = a.plan.tile(++ti);
+      n = units(tile);
+    }
+    const int g = (int)((u - base) / (unsigned)n), first = (int)(u - base) - g * n, last = min(n, first + (int)(end - u)), item = ti * a.G + g;
+    const int rows = tile.z * per, common = shared(tile);
+    const int32_t* table = a.pt.table + (int64_t)live(tile) * a.pt.width;
+    __syncthreads();                                                // the item before this one is done with shared memory
+    if ((int)threadIdx.x < PS_ROWS) {
+      const int k = (int)threadIdx.x / per;
+      s_token[threadIdx.x] = k < tile.z ? a.plan.order()[tile.y + k] : -1;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < PS_ROWS * CHUNKS; x += THREADS) {
+      const int r = x / CHUNKS, c = x - r * CHUNKS, token = s_token[r];
+      const uint4* src = reinterpret_cast<const uint4*>(a.q) + ((int64_t)(token < 0 ? 0 : token) * a.H + (int64_t)g * per + r % per) * CHUNKS + c;
+      cp_async16(qs + P::at(r, c), src, token >= 0);
+    }
+    // 16 keys at a time lie in one page; their page is looked up a tile ahead
+    int id[NP];
+    unsigned paged = 0;                                             // of every stage's 16 keys each: whether they have a page
+    auto seek = [&](int tile_u) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int kt = tile_u * NP + i, index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 36);
+        id[i] = tile_u < last && kt * 16 < common ? table[index] : -1;
+      }
+    };
+    auto issue = [&](int tile_u) {
+      if (tile_u < last) {
+        const int stage = tile_u % P::STAGES;
+        const uint32_t ks = ring + (uint32_t)stage * P::STAGE;
+        paged &= ~(((1u << NP) - 1u) << (NP * stage));
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int kt = tile_u * NP + i, index = (int)((uint64_t)(unsigned)kt * a.inv_tpp >> 36);
+          const bool page = (unsigned)id[i] < (unsigned)a.pt.P;
+          const int64_t line = (((int64_t)(page ? id[i] : 0) * a.G + g) * a.tpp + (page ? kt - index * a.tpp : 0)) * 16;
+          paged |= (page ? 1u : 0u) << (NP * stage + i);
+          if (!page && kt * 16 < common && threadIdx.x == 0) atomicAdd(&g_paged_attn_fault, 1u);
+#pragma unroll
+          for (int x = threadIdx.x; x < 16 * CHUNKS; x += THREADS) {
+            const int key = x / CHUNKS, c = x - key * CHUNKS;
+            const bool ok = page && kt * 16 + key < common;
+            const int64_t from = line * CHUNKS + (ok ? x : 0);
+            cp_async16(ks + P::at(16 * i + key, c), reinterpret_cast<const uint4*>(a.k) + from, ok);
+            cp_async16(ks + P::KV_BYTES + P::at(16 * i + key, c), reinterpret_cast<const uint4*>(a.v) + from, ok);
+          }
+        }
+        seek(tile_u + 1);
+      }
+      cp_async_commit();
+    };
+    seek(first);
+    for (int s = 0; s < P::STAGES - 1; ++s) issue(first + s);
+
+    float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    const bool works = 16 * warp < rows;
+#pragma unroll 1
+    for (int v = first; v < last; ++v) {
+      cp_async_wait<P::STAGES - 2>();
+      __syncthreads();
+      const unsigned paged_now = paged >> (NP * (v % P::STAGES)) & ((1u << NP) - 1u);
+      issue(v + P::STAGES - 1);                                     // (into the stage that all were done with at this barrier)
+      if (!works) continue;
+      const uint32_t ks = ring + (uint32_t)(v % P::STAGES) * P::STAGE, vs = ks + P::KV_BYTES;
+      float s[KT / 8][4];
+#pragma unroll
+      for (int j = 0; j < KT / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t qf[4];
+        ldsm_x4(qs + P::at(16 * warp + r8 + 8 * (mat & 1), 2 * k + (mat >> 1)), qf);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          uint32_t kf[4];
+          ldsm_x4(ks + P::at(16 * j + r8 + 8 * (mat >> 1), 2 * k + (mat & 1)), kf);
+          mma16816<T>(s[2 * j], qf, kf[0], kf[1]);
+          mma16816<T>(s[2 * j + 1], qf, kf[2], kf[3]);
+        }
+      }
+      const unsigned pages = paged_now;
+      const bool whole = (v + 1) * KT <= common && pages == (1u << NP) - 1u;
+      float f[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float t = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = s[j][2 * h + e] * a.scale_log2e;
+            if (!whole && (v * KT + 8 * j + 2 * qc + e >= common || !(pages >> (j / 2) & 1u))) x = -INFINITY;
+            s[j][2 * h + e] = x;
+            t = fmaxf(t, x);
+          }
+        t = fmaxf(t, __shfl_xor_sync(~0u, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(~0u, t, 2));
+        t = fmaxf(t - SHIFT, m[h]);
+        const float ref = t == -INFINITY ? 0.f : t;
+        f[h] = raise2(m[h] - ref);
+        m[h] = t;
+        l[h] *= f[h];
+#pragma unroll
+        for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) s[j][2 * h + e] = raise2(s[j][2 * h + e] - ref);
+      }
+      if (__any_sync(~0u, f[0] != 1.f || f[1] != 1.f)) {            // a maximum grew (or is not a number)
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) o[j][0] *= f[0], o[j][1] *= f[0], o[j][2] *= f[1], o[j][3] *= f[1];
+      }
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        // The weights multiply the values as 16-bit numbers, and their sum is that of the rounded ones: each is off by half a step, at random, which
+        // leaves the output's own rounding the larger error; two numbers each would cost half as many products again.
+        uint32_t pf[4] = {pack2<T>(s[2 * j][0], s[2 * j][1]), pack2<T>(s[2 * j][2], s[2 * j][3]), pack2<T>(s[2 * j + 1][0], s[2 * j + 1][1]),
+                          pack2<T>(s[2 * j + 1][2], s[2 * j + 1][3])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const T* p = reinterpret_cast<const T*>(&pf[e]);
+          l[e & 1] += Tr<T>::to_f(p[0]) + Tr<T>::to_f(p[1]);
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t vf[4];
+          ldsm_x4_trans(vs + P::at(16 * j + r8 + 8 * (mat & 1), 2 * k + (mat >> 1)), vf);
+          mma16816<T>(o[2 * k], pf, vf[0], vf[1]);
+          mma16816<T>(o[2 * k + 1], pf, vf[2], vf[3]);
+        }
+      }
+    }
+    cp_async_wait<0>();
+    // ---- the part ---------------------------------------------------------------------------------------------------------------
+    if (works) {
+      float* rec = a.rec + ((int64_t)item + blockIdx.x) * PS_ROWS * (D + 4);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float sum = l[h];
+        sum += __shfl_xor_sync(~0u, sum, 1);
+        sum += __shfl_xor_sync(~0u, sum, 2);
+        float* row = rec + (16 * warp + 8 * h + qr) * (D + 4);
+        if (qc == 0) *reinterpret_cast<float2*>(row) = make_float2(m[h], sum);
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(row + 4 + 8 * j + 2 * qc) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+      }
+    }
+    u += last - first;
+  }
+}
+
+// A CTA per token and query head joins the parts of the shared slots and of the own ones: a warp takes them in turn, then the warps become one.
+template <typename T, int NQ, int ROWS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32)
+paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ PagedPrefix p, int prefix_ctas) {
+  __shared__ float2 s_ml[WARPS];
+  __shared__ float4 s_o[WARPS][32 * NQ];
+  const int r = blockIdx.x, g = blockIdx.y, t = blockIdx.z, per = gridDim.x, blocks = (per + ROWS - 1) / ROWS, warp = threadIdx.x >> 5,
+            lane = threadIdx.x & 31, D = a.D;
+  pdl_wait();
+  const int64_t line = ((int64_t)t * a.G + g) * blocks + r / ROWS;
+  const int row = a.t_row[t];
+  const uint2 parts = a.parts[line];
+  const bool member = shared_slots(p.index, p.prefix, p.groups, a.pt, t, slots_seen(a.pt, a.t_slot[t])) > 0;
+  const int4 info = p.info[member ? t : 0];
+  const unsigned total = *p.total;
+  if (row < 0 || row >= a.pt.rows) return;
+  int heads = 0, item = 0, c0 = 0;                                  // parts of the shared slots
+  if (member) {
+    const PrefixShares sh(total, prefix_ctas);
+    const unsigned u = (unsigned)info.z + (unsigned)g * info.w;
+    c0 = (int)sh.of(u);
+    heads = (int)sh.of(u + info.w - 1) - c0 + 1;
+    item = info.x * a.G + g;
+  }
+  const int all = heads + (int)parts.y;
+  auto at = [&](int i) -> const float* {
+    if (i < heads) return p.rec + ((int64_t)(item + c0 + i) * PS_ROWS + info.y * per + r) * (D + 4);
+    if (parts.y == 1) return a.whole + (line * ROWS + r % ROWS) * (D + 4);
+    return part_at(a, parts.x, i - heads, ROWS, r % ROWS);
+  };
+  constexpr int AHEAD = 4;
+  float M = -INFINITY, L = 0.f;
+  float4 acc[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i0 = warp; i0 < all; i0 += AHEAD * WARPS) {
+    float2 ml[AHEAD];
+    float4 y[AHEAD][NQ];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const bool in = i0 + k * WARPS < all;
+      const float* from = at(in ? i0 + k * WARPS : i0);
+      ml[k] = in ? *reinterpret_cast<const float2*>(from) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+        y[k][x] = in && 4 * lane + 128 * x < D ? *reinterpret_cast<const float4*>(from + 4 + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top = M;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) top = fmaxf(top, ml[k].x);
+    const float ref = top == -INFINITY ? 0.f : top, f = raise2(M - ref);
+    M = top;
+    L *= f;
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) acc[x].x *= f, acc[x].y *= f, acc[x].z *= f, acc[x].w *= f;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const float w = raise2(ml[k].x - ref);
+      L += ml[k].y * w;
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) acc[x].x += y[k][x].x * w, acc[x].y += y[k][x].y * w, acc[x].z += y[k][x].z * w, acc[x].w += y[k][x].w * w;
+    }
+  }
+  if (lane == 0) s_ml[warp] = make_float2(M, L);
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) s_o[warp][lane + 32 * x] = acc[x];
+  __syncthreads();
+  const int d = 4 * threadIdx.x;
+  if (d >= D) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_ml[w].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const float f = raise2(s_ml[w].x - ref);
+    const float4 y = s_o[w][threadIdx.x];
+    sum += s_ml[w].y * f;
+    o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  store_row4<T>(reinterpret_cast<T*>(a.out) + ((int64_t)t * a.H + (int64_t)g * per + r) * D, d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv),
+                a.out_perm);
+}
+
+}  // namespace b200p

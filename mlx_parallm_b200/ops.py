@@ -995,6 +995,36 @@ def paged_attn(q, kpages, vpages, table, t_row, t_slot, out, scale: float, first
     return out
 
 
+def paged_attn_shared_tile(H: int, G: int) -> int:
+    """Tile of the row_groups plan that paged_attn_shared goes by."""
+    return lib().b200p_paged_attn_shared_tile(int(H), int(G))
+
+
+def paged_attn_shared_workspace_bytes(M: int, H: int, G: int, D: int, groups: int) -> int:
+    return int(lib().b200p_paged_attn_shared_workspace_bytes(int(M), int(H), int(G), int(D), int(groups)))
+
+
+def paged_attn_shared(q, kpages, vpages, table, t_row, t_slot, out, scale: float, group, prefix, plan: RowPlan, workspace=None, out_perm: bool = False):
+    """paged_attn of tokens whose rows have their first slots in common: the first ``prefix[g]`` slots (int32 [groups]) of the tokens with ``group[t]`` = g
+    (int32 [M]; negative: of no group) lie in the same pages and are read once for many tokens (b200p_paged_attn_shared).  ``plan``: row_groups(group, groups,
+    paged_attn_shared_tile(H, G))."""
+    P, G, page, D, rows, width = _paged(kpages, vpages, table, None, q, out, t_row, t_slot, group, prefix, plan.data, workspace)
+    M, n, dt = t_row.numel(), q.numel(), kpages.dtype
+    H = n // (M * D) if M else G
+    if q.dtype is not dt or out.dtype is not dt or n != M * H * D or out.numel() != n:
+        _refuse(f"q and out are [{M}, heads * {D}] in the pages' dtype: got {tuple(q.shape)} and {tuple(out.shape)}")
+    _tokens(M, t_row, t_slot, group)
+    _plan(plan, q.get_device())
+    groups = prefix.numel()
+    if prefix.dtype is not _I32 or plan.rows != M or plan.groups != groups:
+        _refuse(f"prefix is int32 [groups], the plan of {M} tokens in {groups} groups: got {prefix.dtype}, {plan.rows} in {plan.groups}")
+    _call("b200p_paged_attn_shared", lambda: lib().b200p_paged_attn_shared(
+        q.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), table.data_ptr(), t_row.data_ptr(), t_slot.data_ptr(), out.data_ptr(), group.data_ptr(),
+        prefix.data_ptr(), plan.data.data_ptr(), M, H, G, D, groups, plan.tile, P, page, rows, width, float(scale), dtype_code(dt),
+        _lib.OUT_PERM8 if out_perm else 0, _p(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), _stream()))
+    return out
+
+
 def paged_select(mass, table, lengths, kept, first: int = 0, recent: int = 0):
     """``kept`` int32 [rows, G, keep]: which slots every row's key heads keep when the row is cut to ``keep`` tokens (b200p_paged_select)."""
     _here(mass, table, lengths, kept)

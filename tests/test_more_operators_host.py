@@ -62,3 +62,26 @@ def test_lora_rows_refuses_before_it_launches():
     for bad in (dict(columns=(2, 64, 128, 8)), dict(x=264), dict(a=264), dict(b=264), dict(plan=264), dict(ldx=68), dict(y=264), dict(ldy=137)):
         assert call(**bad) == -2, bad
     assert call(M=0) == 0
+
+
+def test_paged_attn_shared_refuses_before_it_launches():
+    L = _lib.lib()
+    assert [L.b200p_paged_attn_shared_tile(*x) for x in ((32, 8), (40, 8), (8, 8), (64, 1), (129, 1), (300, 1), (7, 2), (4, 0))] == [32, 25, 128, 2, 1, 1, 0, 0]
+    size = L.b200p_paged_attn_shared_workspace_bytes
+    assert size(4, 8, 2, 64, 1) > 0 and [size(*x) for x in ((0, 8, 2, 64, 1), (4, 7, 2, 64, 1), (4, 8, 2, 64, 0), (4, 8, 2, 64, 1025))] == [0] * 4
+    ok = dict(q=256, k=256, v=256, table=256, row=256, slot=256, out=256, index=256, prefix=256, plan=256, M=4, H=8, G=2, D=64, groups=1, tile=32, P=9, page=16,
+              rows=4, width=8, dtype=_lib.F16, flags=0, ws=256, bytes=1 << 30)
+
+    def call(**kw):
+        a = dict(ok, **kw)
+        return L.b200p_paged_attn_shared(a["q"], a["k"], a["v"], a["table"], a["row"], a["slot"], a["out"], a["index"], a["prefix"], a["plan"], a["M"], a["H"],
+                                         a["G"], a["D"], a["groups"], a["tile"], a["P"], a["page"], a["rows"], a["width"], 1.0, a["dtype"], a["flags"], a["ws"],
+                                         a["bytes"], 0)
+
+    for bad in (dict(q=0), dict(k=0), dict(table=0), dict(row=0), dict(slot=0), dict(out=0), dict(index=0), dict(prefix=0), dict(plan=0), dict(M=-1), dict(M=65536),
+                dict(H=7), dict(G=0), dict(D=12), dict(D=264), dict(groups=0), dict(groups=1025), dict(tile=16), dict(P=0), dict(page=24), dict(page=8192),
+                dict(rows=0), dict(width=0), dict(width=1 << 27), dict(dtype=9), dict(flags=2), dict(ws=0), dict(ws=128), dict(bytes=1000),
+                dict(dtype=_lib.F32, bytes=1000)):
+        assert call(**bad) == -1, bad
+    for bad in (dict(q=264), dict(out=264), dict(k=264), dict(plan=264)):
+        assert call(**bad) == -2, bad
