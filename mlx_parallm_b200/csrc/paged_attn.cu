@@ -1049,6 +1049,7 @@ paged_attn_mass_kernel(const __grid_constant__ PagedAttn a, int per, int blocks,
 }  // namespace b200p
 
 #include "paged_shared.cuh"
+#include "paged_prefix_tc.cuh"
 
 namespace b200p {
 
@@ -1148,33 +1149,67 @@ static int64_t shared_rows(int H, int G) {                          // of a toke
 }
 static size_t whole_bytes(int64_t M, int H, int G, int D) { return round256((size_t)M * shared_rows(H, G) * (D + 4) * 4); }
 static size_t prefix_bytes(int64_t M, int H, int G, int D, int groups) {
-  return round256(((size_t)row_group_tiles(M, groups, shared_tile(H, G)) * G + sm_count()) * PS_ROWS * (D + 4) * 4);
+  return round256(((size_t)row_group_tiles(M, groups, shared_tile(H, G)) * G + sm_count()) * PS_ROWS * (D + 4) * 4);      // (halves as items: no more)
 }
 static size_t info_bytes(int64_t M) { return round256((size_t)M * 16 + 16); }
+
+template <typename K>
+static int shared_memory_of(K kern, int bytes, std::atomic<uint64_t>& ready, const char* what) {      // ready: devices whose copy of the kernel has it
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
+  }
+  return e == cudaSuccess ? B200P_OK : cuda_fail(e, what);
+}
+
+// tcgen05: copies of whole boxes of keys by 32-bit lines, and a scale that keeps the scores' order
+template <typename T>
+static int launch_prefix_tc(const PagedPrefix& p, unsigned ctas, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
+  auto kern = paged_prefix_tc_kernel<T>;
+  if (const int rc = shared_memory_of(kern, FT_SMEM, ready, "cudaFuncSetAttribute(paged_prefix_tc_kernel)")) return rc;
+  TcEncodeFn enc = tc_get_encode();
+  B200P_REQUIRE(enc != nullptr, B200P_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  const CUtensorMapDataType dt = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  PagedPrefix q = p;
+  if (const int rc = wait_word(WAIT_ATTN_TC, &q.wait_word)) return rc;
+  q.box = q.pt.page % 128 == 0 ? 128 : q.pt.page % 64 == 0 ? 64 : q.pt.page % 32 == 0 ? 32 : 16;
+  CUtensorMap tm[2];
+  for (int i = 0; i < 2; ++i)
+    if (const int rc = tc_encode_2d(enc, &tm[i], dt, i ? q.v : q.k, FT_D, (uint64_t)q.pt.P * q.G * q.pt.page, FT_D * 2, 64, (uint32_t)q.box,
+                                    CU_TENSOR_MAP_SWIZZLE_128B, "cuTensorMapEncodeTiled(pages)"))
+      return rc;
+  launch_pdl(kern, ctas, FT_THREADS, FT_SMEM, st, tm[0], tm[1], q);
+  B200P_LAUNCH_CHECK("paged_prefix_tc_kernel");
+  return B200P_OK;
+}
 
 template <typename T, int D, int NB>
 static int launch_shared(PagedAttn a, PagedPrefix p, int64_t tiles, cudaStream_t st) {
   using E = TcEngine<T, D, NB>;
-  auto kern = paged_prefix_kernel<T, D>;
-  static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixTile<T, D>::SMEM);
-    if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
-  }
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_prefix_kernel)");
-  const int64_t slots = (int64_t)a.pt.width * a.pt.page, units = tiles * a.G * ((slots + PrefixTile<T, D>::KT - 1) / PrefixTile<T, D>::KT);
+  const bool tc = D == FT_D && p.scale_log2e >= 1e-30f && p.scale_log2e <= 1e30f && a.pt.P * a.G * a.pt.page < (1ll << 31) - FT_KEYS;
+  const int64_t slots = (int64_t)a.pt.width * a.pt.page, kt = tc ? FT_KEYS : PrefixTile<T, D>::KT, units = tiles * a.G * (tc ? 1 : 2) * ((slots + kt - 1) / kt);
   B200P_REQUIRE(units < (1ll << 31), B200P_ERR_ARG, "%lld tiles of %d key heads over %lld slots: too many for one call", (long long)tiles, a.G, (long long)slots);
   const unsigned ctas = (unsigned)(units < sm_count() ? units : sm_count());
   p.tpp = a.pt.page / PA_TILE;
   p.inv_tpp = ((1ull << 36) + p.tpp - 1) / p.tpp;
-  launch_pdl(kern, ctas, PS_WARPS * 32, PrefixTile<T, D>::SMEM, st, p);
-  B200P_LAUNCH_CHECK("paged_prefix_kernel");
-  const int rc = launch_stream<E, true>(a, st);
-  if (rc) return rc;
+  int rc;
+  if (tc) {
+    if constexpr (D == FT_D) {
+      if ((rc = launch_prefix_tc<T>(p, ctas, st))) return rc;
+    }
+  } else {
+    static std::atomic<uint64_t> ready{0};
+    auto kern = paged_prefix_kernel<T, D>;
+    if ((rc = shared_memory_of(kern, PrefixTile<T, D>::SMEM, ready, "cudaFuncSetAttribute(paged_prefix_kernel)"))) return rc;
+    launch_pdl(kern, ctas, PS_WARPS * 32, PrefixTile<T, D>::SMEM, st, p);
+    B200P_LAUNCH_CHECK("paged_prefix_kernel");
+  }
+  if ((rc = launch_stream<E, true>(a, st))) return rc;
   const dim3 heads((unsigned)(a.H / a.G), (unsigned)a.G, (unsigned)a.M);
-  launch_pdl(paged_shared_join_kernel<T, D <= 128 ? 1 : 2, E::ROWS, 4>, heads, 4 * 32, 0, st, a, p, (int)ctas);
+  launch_pdl(paged_shared_join_kernel<T, D <= 128 ? 1 : 2, E::ROWS, 4>, heads, 4 * 32, 0, st, a, p, (int)ctas, tc ? PS_ROWS : PS_HALF);
   B200P_LAUNCH_CHECK("paged_shared_join_kernel");
   return B200P_OK;
 }

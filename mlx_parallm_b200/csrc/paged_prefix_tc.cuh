@@ -1,0 +1,310 @@
+// The shared slots of b200p_paged_attn_shared on tcgen05, 16-bit caches, head_dim 128 (part of paged_attn.cu): attn_prefill_tc.cu's two tiles of 128 rows that
+// take turns, here the two halves of a tile of query heads of a group's tokens, over keys in pages and without a mask but for the last.
+//
+// The 128 keys of a step come as boxes of 16 to 128 keys that lie in one page each; their ids are looked up a step ahead, a lane per box, and a box without
+// a page is fetched from behind the pages, where the copy brings zeros.  A CTA's part of the work is runs of steps of one item after the other, each of
+// which leaves a part.  Products, softmax and roles are those of the prompt kernel; the maximum is held 14 lower for f16, so that weights reach 2^14 and small
+// ones keep their bits.
+#pragma once
+#include "attn_tc.cuh"
+
+namespace b200p {
+
+template <typename T>
+__global__ void __launch_bounds__(FT_THREADS, 1)
+paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const __grid_constant__ PagedPrefix a) {
+  constexpr float SHIFT = std::is_same<T, __half>::value ? 14.f : 0.f;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ PrefixPlan s_plan;
+  const uint32_t raw = smem_u32(smem);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t ring = base + 2 * FT_TILE_BYTES;
+  AttnTcShared* sh = reinterpret_cast<AttnTcShared*>(smem + (base - raw) + (2 + FT_RING) * FT_TILE_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&sh->q_full), 8);
+    for (int s = 0; s < FT_RING; ++s) { mbar_init(smem_u32(&sh->kv_full[s]), 1); mbar_init(smem_u32(&sh->kv_empty[s]), 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&sh->s_full[i]), 1); mbar_init(smem_u32(&sh->p_full[i]), 4); mbar_init(smem_u32(&sh->o_full[i]), 1); }
+    sh->abort = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmk);
+    tma_prefetch_desc(&tmv);
+  }
+  if (warp == 8) tmem_alloc(smem_u32(&sh->tmem_base), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;                     // S of half i at 128 i (P over its first 64), O of half i at 256 + 128 i
+  pdl_wait();
+  pdl_launch_dependents();
+  PrefixCursor<FT_KEYS, false> cursor = prefix_plan<FT_THREADS, FT_KEYS, false>(a, s_plan);
+  auto wait = [&](uint64_t& bar, uint32_t parity, int role) { return mbar_wait_warp(smem_u32(&bar), parity, &sh->abort, a.wait_word, role); };
+  PrefixRun run;
+  bool ok = true;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ft_regs_other(true)));
+    if (warp == 9) {
+      // ===================================== TMA producer =====================================
+      const int boxes = FT_KEYS / a.box, page = a.pt.page;
+      int slot = 0;
+      uint32_t ph = 0;
+      while (ok && cursor.next(a, run)) {
+        const int32_t* table = a.pt.table + (int64_t)run.table_row * a.pt.width;
+        const int nowhere = (int)(a.pt.P * a.G * page);    // behind the pages: zeros (the host has checked that it fits)
+        auto seek = [&](int u) {                           // the line of this lane's box
+          const int key = u * FT_KEYS + lane * a.box;
+          if (lane >= boxes || u >= run.last || key >= run.common) return nowhere;
+          const int index = key / page, id = table[index];
+          if ((unsigned)id >= (unsigned)a.pt.P) {
+            atomicAdd(&g_paged_attn_fault, 1u);
+            return nowhere;
+          }
+          return (id * a.G + run.g) * page + key - index * page;
+        };
+        int line = seek(run.first);
+        for (int u = run.first; ok && u < run.last; ++u) {
+          const int ahead = seek(u + 1);
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv) {
+            if (!(ok = wait(sh->kv_empty[slot], ph ^ 1u, 0))) break;
+            const uint32_t bar = smem_u32(&sh->kv_full[slot]), dst = ring + slot * FT_TILE_BYTES;
+            const CUtensorMap* m = kv ? &tmv : &tmk;
+            if (lane == 0) mbar_arrive_expect_tx(bar, FT_TILE_BYTES);
+#pragma unroll 1
+            for (int b = 0; b < boxes; ++b) {
+              const int at = __shfl_sync(~0u, line, b);
+              if (lane == 0) {
+                tma_load_2d(dst + b * a.box * 128, m, 0, at, bar);
+                tma_load_2d(dst + FT_HALF + b * a.box * 128, m, 64, at, bar);
+              }
+            }
+            __syncwarp();
+            if (++slot == FT_RING) { slot = 0; ph ^= 1u; }
+          }
+          line = ahead;
+        }
+      }
+    } else if (warp == 8) {
+      // ===================================== MMA issuer =======================================
+      constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+      constexpr uint32_t idesc_pv = idesc | (1u << 16);    // B is N-major
+      auto qk = [&](int i, int slot) {
+        const uint64_t ad = make_desc_sw128(base + i * FT_TILE_BYTES), bd = make_desc_sw128(ring + slot * FT_TILE_BYTES);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {                      // 16 k = 32 bytes of a 128-byte row; k 4..7 in the other half of the operand
+          const uint64_t off = (uint64_t)((k & 3) * 2 + (k >> 2) * (FT_HALF >> 4));
+          ft_mma_ss(tmem + 128 * i, ad + off, bd + off, idesc, k ? 1u : 0u);
+        }
+      };
+      auto pv = [&](int i, int slot, uint32_t acc) {
+        const uint64_t bd = ft_desc_n_major(ring + slot * FT_TILE_BYTES);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)                        // 16 keys = 2048 bytes; P: 8 columns
+          umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, bd + (uint64_t)(k * (2048 >> 4)), idesc_pv, (k || acc) ? 1u : 0u);
+      };
+      int slot = 0, round = 0;
+      uint32_t ph = 0, pph[2] = {0, 0};                    // phases of `slot` and of the probabilities' barriers
+      while (ok && cursor.next(a, run)) {
+        const int both = run.rows > PS_HALF ? 2 : 1, steps = run.last - run.first;
+        const int k0 = slot;
+        if (!(ok = wait(sh->q_full, (uint32_t)(round & 1), 1) && wait(sh->kv_full[k0], ph, 1))) break;
+        ++round;
+        if (++slot == FT_RING) { slot = 0; ph ^= 1u; }
+        tc_fence_after();
+        if (elect_one()) {
+          for (int i = 0; i < both; ++i) {
+            qk(i, k0);
+            umma_commit(smem_u32(&sh->s_full[i]));
+          }
+          umma_commit(smem_u32(&sh->kv_empty[k0]));
+        }
+        __syncwarp();
+        for (int j = 0; j < steps && ok; ++j) {
+          const int vslot = slot;
+          if (!(ok = wait(sh->kv_full[vslot], ph, 1))) break;
+          if (++slot == FT_RING) { slot = 0; ph ^= 1u; }
+          const int left = run.common - (run.first + j) * FT_KEYS;
+          if (left < FT_KEYS) {
+            // the weights of keys behind the shared ones are zero, but what lies there may not be finite: zero those rows of V
+            for (int c = lane; c < (FT_KEYS - left) * 16; c += 32) {
+              const int row = left + (c >> 4), hf = (c >> 3) & 1, ch = c & 7;
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + vslot * FT_TILE_BYTES + hf * FT_HALF + row * 128 + ch * 16), "r"(0) : "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          const bool more = j + 1 < steps;
+          const int kslot = slot;
+          if (more) {
+            if (!(ok = wait(sh->kv_full[kslot], ph, 1))) break;
+            if (++slot == FT_RING) { slot = 0; ph ^= 1u; }
+          }
+          for (int i = 0; i < both; ++i) {
+            if (!(ok = wait(sh->p_full[i], pph[i], 1))) break;
+            pph[i] ^= 1u;
+            tc_fence_after();
+            if (elect_one()) {
+              pv(i, vslot, j > 0 ? 1u : 0u);
+              if (i == both - 1) umma_commit(smem_u32(&sh->kv_empty[vslot]));
+              if (more) {
+                qk(i, kslot);
+                umma_commit(smem_u32(&sh->s_full[i]));
+                if (i == both - 1) umma_commit(smem_u32(&sh->kv_empty[kslot]));
+              } else {
+                umma_commit(smem_u32(&sh->o_full[i]));
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(ft_regs_softmax(true)));
+    // ===================================== softmax and parts ================================
+    const int i = warp >> 2, q = warp & 3, per = a.H / a.G;
+    const int r = q * 32 + lane;                           // row of the half = TMEM lane
+    const uint32_t s_addr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(128 * i), o_addr = s_addr + 256;
+    const float2 sc2 = make_float2(a.scale_log2e, a.scale_log2e);
+    uint32_t sph = 0, oph = 0, round = 0;
+    while (ok && cursor.next(a, run)) {
+      // (all products of the run before have been waited for by the half that both runs have, or were not made: the queries' place is free)
+      const bool mine = i == 0 || run.rows > PS_HALF;
+      const int at = PS_HALF * i + r;
+      if (mine) {
+        const bool live = at < run.rows;
+        const int token = live ? a.plan.order()[run.tile.y + at / per] : 0;
+        const uint4* src = reinterpret_cast<const uint4*>(a.q) + ((int64_t)token * a.H + (int64_t)run.g * per + (live ? at % per : 0)) * 16;
+        const uint32_t dst = base + i * FT_TILE_BYTES + r * 128;
+        uint4 x[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) x[c] = live ? src[c] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * FT_HALF + (((c & 7) ^ (r & 7)) << 4)), "r"(x[c].x), "r"(x[c].y),
+                       "r"(x[c].z), "r"(x[c].w)
+                       : "memory");
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh->q_full));
+      // whether every key of the run has a page: seldom not, and then the scores look theirs up
+      const int32_t* table = a.pt.table + (int64_t)run.table_row * a.pt.width;
+      bool bad = false;
+      for (int p = run.first * FT_KEYS / a.pt.page + lane; p <= (min(run.common, run.last * FT_KEYS) - 1) / a.pt.page; p += 32)
+        bad |= (unsigned)table[p] >= (unsigned)a.pt.P;
+      bad = __any_sync(~0u, bad);
+      if (!mine) {                                         // (an arrival for the next run would count for this one until all of its are in)
+        ok = wait(sh->q_full, round & 1u, 2 + i);
+        ++round;
+        continue;
+      }
+      ++round;
+      float m = -INFINITY, sum = 0.f;
+      for (int u = run.first; u < run.last; ++u) {
+        if (!(ok = wait(sh->s_full[i], sph, 2 + i))) break;
+        sph ^= 1u;
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, s + 32 * c);
+        tmem_ld_wait();
+        const int n = run.common - u * FT_KEYS;            // shared keys from this step's first on
+        if (n < FT_KEYS || bad) {
+          unsigned pages = 0xffu;                          // which 16 keys have a page
+          if (bad) {
+            pages = 0;
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c)
+              if (16 * c < n) pages |= ((unsigned)table[(u * FT_KEYS + 16 * c) / a.pt.page] < (unsigned)a.pt.P ? 1u : 0u) << c;
+          }
+#pragma unroll
+          for (int c = 0; c < 128; ++c) s[c] = c < n && (pages >> (c / 16) & 1u) ? s[c] : -INFINITY;
+        }
+        float t0 = max3(s[0], s[1], s[2]), t1 = max3(s[3], s[4], s[5]), t2 = max3(s[6], s[7], s[8]), t3 = max3(s[9], s[10], s[11]);
+#pragma unroll
+        for (int c = 12; c + 8 <= 128; c += 8) {
+          t0 = max3(t0, s[c], s[c + 1]);
+          t1 = max3(t1, s[c + 2], s[c + 3]);
+          t2 = max3(t2, s[c + 4], s[c + 5]);
+          t3 = max3(t3, s[c + 6], s[c + 7]);
+        }
+        t0 = max3(t0, s[124], s[125]);
+        t1 = max3(t1, s[126], s[127]);
+        const float mt = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * a.scale_log2e - SHIFT;      // (the host sends positive scales here)
+        const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.f : mn, f = ex2(m - ref);
+        const bool rescale = u > run.first && __any_sync(~0u, mn > m);
+        m = mn;
+        const float2 nm2 = make_float2(-ref, -ref);
+        float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float2 x = __ffma2_rn(make_float2(s[64 * h + 2 * c], s[64 * h + 2 * c + 1]), sc2, nm2);
+            w[c] = ft_pack<T>(ex2(x.x), ex2(x.y));
+            const float2 e = ft_unpack<T>(w[c]);           // the sum is that of the weights as the product uses them
+            if (c & 1) a1 = __fadd2_rn(a1, e); else a0 = __fadd2_rn(a0, e);
+          }
+          tmem_st32(s_addr + 32 * h, w);
+        }
+        if (rescale) {
+          const float2 f2 = make_float2(f, f);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float o[2][32];
+            tmem_ld32(o_addr + 64 * h, o[0]);
+            tmem_ld32(o_addr + 64 * h + 32, o[1]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t w[32];
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                const float2 y = __fmul2_rn(make_float2(o[c][k], o[c][k + 1]), f2);
+                w[k] = __float_as_uint(y.x);
+                w[k + 1] = __float_as_uint(y.y);
+              }
+              tmem_st32(o_addr + 64 * h + 32 * c, w);
+            }
+          }
+        }
+        tmem_st_wait();
+        sum = sum * f + ((a0.x + a0.y) + (a1.x + a1.y));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh->p_full[i]));
+      }
+      if (ok) ok = wait(sh->o_full[i], oph, 2 + i);
+      oph ^= 1u;
+      if (ok) {
+        tc_fence_after();
+        float* row = a.rec + (((int64_t)run.item + blockIdx.x) * PS_ROWS + at) * (FT_D + 4);
+        const bool live = at < run.rows;
+        if (live) *reinterpret_cast<float2*>(row) = make_float2(m, sum);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          tmem_ld32(o_addr + 32 * c, o);
+          tmem_ld_wait();
+          if (!live) continue;
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(row + 4 + 32 * c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        }
+        tc_fence_before();                                 // (the next run's first products write there again)
+      }
+    }
+  }
+  if (sh->abort) wait_settle();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace b200p

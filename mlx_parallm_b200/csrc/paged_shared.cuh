@@ -3,15 +3,16 @@
 //   o = sum_j p_j v_j over a group's shared slots and the row's own ones: either part leaves its maximum m, sum l and unnormalised output, and
 //   o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i,  m = max m_i
 //
-// The shared slots are read once for a tile of up to PS_ROWS query heads of the group's tokens, instead of once for every token: products of 128 rows,
-// which the matrix instructions bound and not the memory.  The own slots go through paged_attn_kernel behind the shared ones, beside this kernel on the same
-// SMs, and a third launch joins the parts of both.
+// The shared slots are read once for a tile of up to PS_ROWS query heads of the group's tokens, instead of once for every token: products of many rows,
+// which the matrix instructions bound and not the memory.  The own slots go through paged_attn_kernel behind the shared ones, and a third launch joins the
+// parts of both.
 #pragma once
 #include "rowgroups.cuh"
 
 namespace b200p {
 
-constexpr int PS_ROWS = 128, PS_WARPS = 8;       // query rows of a tile: tokens x query heads of a key head; a warp has 16
+constexpr int PS_ROWS = 256;                     // query rows of a tile: tokens x query heads of a key head
+constexpr int PS_HALF = 128, PS_WARPS = 8;       // of which paged_prefix_kernel takes 128 at a time, 16 to a warp
 
 struct PagedPrefix {
   const void *q, *k, *v;
@@ -22,12 +23,14 @@ struct PagedPrefix {
   float scale_log2e;
   uint64_t inv_tpp;
   int tpp;
-  float* rec;            // [items + CTAs, PS_ROWS, D + 4] parts, of item i in CTA c the one at i + c
-  int4* info;            // [M] the token's tile, its place in it, the tile's first unit, units of an item (0: no shared slot)
+  float* rec;            // [items + CTAs, rows of an item, D + 4] parts, of item i in CTA c the one at i + c
+  int4* info;            // [M] the token's tile, its place in it (and in the upper half the tile's items per key head), the tile's first unit, units of an item
   unsigned* total;       // units of all
+  int* wait_word;
+  int box;               // keys that one copy brings: they lie in one page
 };
 
-// The units (KT shared keys of a tile of tokens and a key head) of all items lie end to end and every CTA has an equal part of them, as in
+// The units (KT shared keys of an item: the rows of a tile, or of a half of it, and a key head) lie end to end and every CTA has an equal part of them, as in
 // paged_attn_kernel.
 struct PrefixShares {
   unsigned n, q, r;
@@ -35,7 +38,7 @@ struct PrefixShares {
     q = n ? U / n : 1;
     r = U - q * n;
   }
-  __device__ unsigned begin(unsigned c) const { return c * q + min(c, r); }
+  __device__ unsigned begin(unsigned c) const { return c < n ? c * q + min(c, r) : q * n + r; }
   __device__ unsigned of(unsigned u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
 };
 
@@ -48,10 +51,101 @@ __device__ __forceinline__ int shared_slots(const int32_t* index, const int32_t*
   return seen < n ? 0 : n;
 }
 
+// A run of an item's units.
+struct PrefixRun {
+  int4 tile;
+  int ti, n, common, table_row;        // the tile, units of an item, shared slots, the table row that has their pages
+  int g, half, first, last, item, rows;  // key head, half, units [first, last), number of the item, query rows of the tile
+};
+
+// SPLIT: an item has half of a tile's rows (where it has more than that), else all of them.
+template <int KT, bool SPLIT>
+struct PrefixCursor {
+  unsigned u, end, base;
+  int ti;
+  static __device__ __forceinline__ void look(const PagedPrefix& a, int i, PrefixRun& r) {
+    r.tile = a.plan.tile(i);
+    r.ti = i;
+    r.common = min(max(a.prefix[r.tile.x], 0), table_slots(a.pt));
+    r.table_row = -1;                                               // that of the first member that holds the shared slots
+    for (int k = 0; k < r.tile.z && r.table_row < 0; ++k) {
+      const int t = a.plan.order()[r.tile.y + k], row = a.t_row[t];
+      if (row >= 0 && row < a.pt.rows && slots_seen(a.pt, a.t_slot[t]) >= r.common) r.table_row = row;
+    }
+    r.n = r.table_row < 0 ? 0 : (r.common + KT - 1) / KT;
+    r.rows = r.tile.z * (a.H / a.G);
+  }
+  static __device__ __forceinline__ int halves(const PrefixRun& r) { return SPLIT && r.rows > PS_HALF ? 2 : 1; }
+  static __device__ __forceinline__ unsigned units(const PagedPrefix& a, const PrefixRun& r) { return (unsigned)r.n * a.G * halves(r); }
+  __device__ bool next(const PagedPrefix& a, PrefixRun& r) {
+    if (u >= end) return false;
+    look(a, ti, r);
+    while (u - base >= units(a, r)) {
+      base += units(a, r);
+      look(a, ++ti, r);
+    }
+    const int at = (int)((u - base) / (unsigned)r.n), h = halves(r);
+    r.g = at / h, r.half = at - r.g * h;
+    r.first = (int)(u - base) - at * r.n, r.last = min(r.n, r.first + (int)(end - u));
+    r.item = SPLIT ? (ti * a.G + r.g) * 2 + r.half : ti * a.G + r.g;
+    u += r.last - r.first;
+    return true;
+  }
+};
+
+// By the whole CTA: units of all tiles, this CTA's part, and (by the first CTA) what the join has to know of every token.
+struct PrefixPlan {
+  unsigned sum[16], base;
+  int tile;
+};
+template <int THREADS, int KT, bool SPLIT>
+__device__ __forceinline__ PrefixCursor<KT, SPLIT> prefix_plan(const PagedPrefix& a, PrefixPlan& s) {
+  using C = PrefixCursor<KT, SPLIT>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = a.plan.tiles(), chunk = (tiles + THREADS - 1) / THREADS;
+  const int i0 = min(tiles, (int)threadIdx.x * chunk), i1 = min(tiles, i0 + chunk);
+  PrefixRun r;
+  unsigned mine = 0;
+  for (int i = i0; i < i1; ++i) {
+    C::look(a, i, r);
+    mine += C::units(a, r);
+  }
+  unsigned before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned x = __shfl_up_sync(~0u, before, o);
+    if (lane >= o) before += x;
+  }
+  if (lane == 31) s.sum[warp] = before;
+  __syncthreads();
+  before -= mine;
+  unsigned U = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += s.sum[w];
+    U += s.sum[w];
+  }
+  const PrefixShares sh(U, gridDim.x);
+  C c;
+  c.u = sh.begin(blockIdx.x), c.end = sh.begin(blockIdx.x + 1);
+  for (int i = i0; i < i1; ++i) {
+    if (i0 + 1 < i1) C::look(a, i, r);
+    const unsigned n = C::units(a, r);
+    if (c.u - before < n) s.tile = i, s.base = before;
+    if (blockIdx.x == 0)
+      for (int k = 0; k < r.tile.z; ++k) a.info[a.plan.order()[r.tile.y + k]] = make_int4(i, k | C::halves(r) << 16, (int)before, r.n);
+    before += n;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.total = U;
+  __syncthreads();
+  c.ti = s.tile, c.base = s.base;                                   // (where there is nothing to do nobody looks at them)
+  return c;
+}
+
 template <typename T, int D>
 struct PrefixTile {
   static constexpr int KT = D > 128 ? 32 : 64, STAGES = 3, CHUNKS = D / 8, PIECES = CHUNKS % 8 ? (CHUNKS | 1) : CHUNKS, LINE = PIECES * 16;
-  static constexpr int KV_BYTES = KT * LINE, STAGE = 2 * KV_BYTES, Q_BYTES = PS_ROWS * LINE, SMEM = Q_BYTES + STAGES * STAGE;
+  static constexpr int KV_BYTES = KT * LINE, STAGE = 2 * KV_BYTES, Q_BYTES = PS_HALF * LINE, SMEM = Q_BYTES + STAGES * STAGE;
   static __device__ __forceinline__ uint32_t at(int line, int c) { return (uint32_t)(line * LINE + ((CHUNKS % 8 ? c : c ^ (line & 7)) << 4)); }
 };
 
@@ -63,82 +157,27 @@ paged_prefix_kernel(const __grid_constant__ PagedPrefix a) {
   // f16: weights up to 2^14 and not 1, so that small ones keep their bits
   constexpr float SHIFT = std::is_same<T, __half>::value ? 14.f : 0.f;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ unsigned s_sum[PS_WARPS], s_base;
-  __shared__ int s_tile, s_token[PS_ROWS];
+  __shared__ PrefixPlan s_plan;
+  __shared__ int s_token[PS_HALF];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qr = lane >> 2, qc = lane & 3, mat = lane >> 3, r8 = lane & 7;
   const int per = a.H / a.G;
   pdl_wait();
   pdl_launch_dependents();
-
-  // ---- the plan: units of all tiles, this CTA's part ---------------------------------------------------------------------------
-  auto shared = [&](const int4& tile) { return min(max(a.prefix[tile.x], 0), table_slots(a.pt)); };
-  auto live = [&](const int4& tile) {                               // the row of a member that holds the shared slots; -1: none does
-    const int common = shared(tile);
-    for (int i = 0; i < tile.z; ++i) {
-      const int t = a.plan.order()[tile.y + i], row = a.t_row[t];
-      if (row >= 0 && row < a.pt.rows && slots_seen(a.pt, a.t_slot[t]) >= common) return row;
-    }
-    return -1;
-  };
-  auto units = [&](const int4& tile) { return live(tile) < 0 ? 0 : (shared(tile) + KT - 1) / KT; };
-  const int tiles = a.plan.tiles(), chunk = (tiles + THREADS - 1) / THREADS;
-  const int i0 = min(tiles, (int)threadIdx.x * chunk), i1 = min(tiles, i0 + chunk);
-  unsigned mine = 0;
-  for (int i = i0; i < i1; ++i) mine += units(a.plan.tile(i)) * a.G;
-  unsigned before = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned x = __shfl_up_sync(~0u, before, o);
-    if (lane >= o) before += x;
-  }
-  if (lane == 31) s_sum[warp] = before;
-  __syncthreads();
-  before -= mine;
-  unsigned U = 0;
-#pragma unroll
-  for (int w = 0; w < PS_WARPS; ++w) {
-    if (w < warp) before += s_sum[w];
-    U += s_sum[w];
-  }
-  const PrefixShares sh(U, gridDim.x);
-  unsigned u = sh.begin(blockIdx.x);
-  const unsigned end = sh.begin(blockIdx.x + 1);
-  for (int i = i0; i < i1; ++i) {
-    const int4 tile = a.plan.tile(i);
-    const int n = units(tile);
-    if (u - before < n * (unsigned)a.G) s_tile = i, s_base = before;
-    if (blockIdx.x == 0)                                            // for the join
-      for (int k = 0; k < tile.z; ++k) a.info[a.plan.order()[tile.y + k]] = make_int4(i, k, (int)before, n);
-    before += n * a.G;
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.total = U;
-  if (blockIdx.x >= sh.n) return;
-  __syncthreads();
-  int ti = s_tile;
-  unsigned base = s_base;
-
+  PrefixCursor<KT, true> cursor = prefix_plan<THREADS, KT, true>(a, s_plan);
   const uint32_t qs = (uint32_t)__cvta_generic_to_shared(smem), ring = qs + P::Q_BYTES;
-  while (u < end) {
-    // ---- the next item: a tile of tokens and a key head --------------------------------------------------------------------------
-    int4 tile = a.plan.tile(ti);
-    int n = units(tile);
-    while (u - base >= n * (unsigned)a.G) {
-      base += n * a.G;
-      tile = a.plan.tile(++ti);
-      n = units(tile);
-    }
-    const int g = (int)((u - base) / (unsigned)n), first = (int)(u - base) - g * n, last = min(n, first + (int)(end - u)), item = ti * a.G + g;
-    const int rows = tile.z * per, common = shared(tile);
-    const int32_t* table = a.pt.table + (int64_t)live(tile) * a.pt.width;
+  PrefixRun run;
+  while (cursor.next(a, run)) {
+    const int first = run.first, last = run.last, g = run.g, common = run.common, rows = run.rows - PS_HALF * run.half, r0 = PS_HALF * run.half;
+    const int32_t* table = a.pt.table + (int64_t)run.table_row * a.pt.width;
     __syncthreads();                                                // the item before this one is done with shared memory
-    if ((int)threadIdx.x < PS_ROWS) {
-      const int k = (int)threadIdx.x / per;
-      s_token[threadIdx.x] = k < tile.z ? a.plan.order()[tile.y + k] : -1;
+    if ((int)threadIdx.x < PS_HALF) {
+      const int k = (r0 + (int)threadIdx.x) / per;
+      s_token[threadIdx.x] = k < run.tile.z ? a.plan.order()[run.tile.y + k] : -1;
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < PS_ROWS * CHUNKS; x += THREADS) {
+    for (int x = threadIdx.x; x < PS_HALF * CHUNKS; x += THREADS) {
       const int r = x / CHUNKS, c = x - r * CHUNKS, token = s_token[r];
-      const uint4* src = reinterpret_cast<const uint4*>(a.q) + ((int64_t)(token < 0 ? 0 : token) * a.H + (int64_t)g * per + r % per) * CHUNKS + c;
+      const uint4* src = reinterpret_cast<const uint4*>(a.q) + ((int64_t)(token < 0 ? 0 : token) * a.H + (int64_t)g * per + (r0 + r) % per) * CHUNKS + c;
       cp_async16(qs + P::at(r, c), src, token >= 0);
     }
     // 16 keys at a time lie in one page; their page is looked up a tile ahead
@@ -260,7 +299,7 @@ paged_prefix_kernel(const __grid_constant__ PagedPrefix a) {
     cp_async_wait<0>();
     // ---- the part ---------------------------------------------------------------------------------------------------------------
     if (works) {
-      float* rec = a.rec + ((int64_t)item + blockIdx.x) * PS_ROWS * (D + 4);
+      float* rec = a.rec + ((int64_t)run.item + blockIdx.x) * PS_HALF * (D + 4);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float sum = l[h];
@@ -272,14 +311,13 @@ paged_prefix_kernel(const __grid_constant__ PagedPrefix a) {
         for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(row + 4 + 8 * j + 2 * qc) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
       }
     }
-    u += last - first;
   }
 }
 
 // A CTA per token and query head joins the parts of the shared slots and of the own ones: a warp takes them in turn, then the warps become one.
 template <typename T, int NQ, int ROWS, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
-paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ PagedPrefix p, int prefix_ctas) {
+paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ PagedPrefix p, int prefix_ctas, int item_rows) {
   __shared__ float2 s_ml[WARPS];
   __shared__ float4 s_o[WARPS][32 * NQ];
   const int r = blockIdx.x, g = blockIdx.y, t = blockIdx.z, per = gridDim.x, blocks = (per + ROWS - 1) / ROWS, warp = threadIdx.x >> 5,
@@ -292,17 +330,20 @@ paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_const
   const int4 info = p.info[member ? t : 0];
   const unsigned total = *p.total;
   if (row < 0 || row >= a.pt.rows) return;
-  int heads = 0, item = 0, c0 = 0;                                  // parts of the shared slots
+  int heads = 0, c0 = 0;                                            // parts of the shared slots
+  int64_t from = 0;                                                 // the first of them
   if (member) {
     const PrefixShares sh(total, prefix_ctas);
-    const unsigned u = (unsigned)info.z + (unsigned)g * info.w;
+    const int halves = info.y >> 16, at = (info.y & 0xffff) * per + r, half = halves > 1 && at >= PS_HALF ? 1 : 0;
+    const unsigned u = (unsigned)info.z + (unsigned)((g * halves + half) * info.w);
     c0 = (int)sh.of(u);
     heads = (int)sh.of(u + info.w - 1) - c0 + 1;
-    item = info.x * a.G + g;
+    from = (int64_t)(item_rows == PS_HALF ? (info.x * a.G + g) * 2 + half : info.x * a.G + g) + c0;
+    from = from * item_rows + at - PS_HALF * half;
   }
   const int all = heads + (int)parts.y;
   auto at = [&](int i) -> const float* {
-    if (i < heads) return p.rec + ((int64_t)(item + c0 + i) * PS_ROWS + info.y * per + r) * (D + 4);
+    if (i < heads) return p.rec + (from + (int64_t)i * item_rows) * (D + 4);
     if (parts.y == 1) return a.whole + (line * ROWS + r % ROWS) * (D + 4);
     return part_at(a, parts.x, i - heads, ROWS, r % ROWS);
   };
