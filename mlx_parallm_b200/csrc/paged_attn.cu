@@ -1149,7 +1149,7 @@ static int64_t shared_rows(int H, int G) {                          // of a toke
 }
 static size_t whole_bytes(int64_t M, int H, int G, int D) { return round256((size_t)M * shared_rows(H, G) * (D + 4) * 4); }
 static size_t prefix_bytes(int64_t M, int H, int G, int D, int groups) {
-  return round256(((size_t)row_group_tiles(M, groups, shared_tile(H, G)) * G + sm_count()) * PS_ROWS * (D + 4) * 4);      // (halves as items: no more)
+  return round256(((size_t)row_group_tiles(M, groups, shared_tile(H, G)) * G + sm_count()) * PS_ROWS * (D + PS_HEAD) * 4);      // (halves as items: no more)
 }
 static size_t info_bytes(int64_t M) { return round256((size_t)M * 16 + 16); }
 
@@ -1208,8 +1208,11 @@ static int launch_shared(PagedAttn a, PagedPrefix p, int64_t tiles, cudaStream_t
     B200P_LAUNCH_CHECK("paged_prefix_kernel");
   }
   if ((rc = launch_stream<E, true>(a, st))) return rc;
-  const dim3 heads((unsigned)(a.H / a.G), (unsigned)a.G, (unsigned)a.M);
-  launch_pdl(paged_shared_join_kernel<T, D <= 128 ? 1 : 2, E::ROWS, 4>, heads, 4 * 32, 0, st, a, p, (int)ctas, tc ? PS_ROWS : PS_HALF);
+  // warps per query head: eight where the heads are few, else two
+  constexpr int NQ = D <= 128 ? 1 : 2;
+  const int W = (int64_t)a.M * a.H <= 4 * sm_count() ? 8 : 2, rows = tc ? PS_ROWS : PS_HALF;
+  const dim3 grid((unsigned)((a.H * W + 7) / 8), (unsigned)a.M);
+  launch_pdl(W == 8 ? paged_shared_join_kernel<T, NQ, E::ROWS, 8> : paged_shared_join_kernel<T, NQ, E::ROWS, 2>, grid, 256, 0, st, a, p, (int)ctas, rows);
   B200P_LAUNCH_CHECK("paged_shared_join_kernel");
   return B200P_OK;
 }

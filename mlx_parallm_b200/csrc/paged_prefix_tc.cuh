@@ -13,9 +13,10 @@ namespace b200p {
 template <typename T>
 __global__ void __launch_bounds__(FT_THREADS, 1)
 paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const __grid_constant__ PagedPrefix a) {
-  constexpr float SHIFT = std::is_same<T, __half>::value ? 14.f : 0.f;
+  constexpr float SHIFT = std::is_same<T, __half>::value ? 8.f : 0.f, LAG = 6.f;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ PrefixPlan s_plan;
+  __shared__ struct { PrefixCursor<FT_KEYS, false> cursor; PrefixRun run; } s_kept[8];      // the steps' loop has no registers for them
   const uint32_t raw = smem_u32(smem);
   const uint32_t base = (raw + 1023u) & ~1023u;
   const uint32_t ring = base + 2 * FT_TILE_BYTES;
@@ -37,9 +38,9 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
   const uint32_t tmem = sh->tmem_base;                     // S of half i at 128 i (P over its first 64), O of half i at 256 + 128 i
   pdl_wait();
   pdl_launch_dependents();
-  PrefixCursor<FT_KEYS, false> cursor = prefix_plan<FT_THREADS, FT_KEYS, false>(a, s_plan);
-  auto wait = [&](uint64_t& bar, uint32_t parity, int role) { return mbar_wait_warp(smem_u32(&bar), parity, &sh->abort, a.wait_word, role); };
   PrefixRun run;
+  PrefixCursor<FT_KEYS, false> cursor = prefix_plan<FT_THREADS, FT_KEYS, false>(a, s_plan, run);
+  auto wait = [&](uint64_t& bar, uint32_t parity, int role) { return mbar_wait_warp(smem_u32(&bar), parity, &sh->abort, a.wait_word, role); };
   bool ok = true;
 
   if (warp >= 8) {
@@ -173,19 +174,24 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
       // (all products of the run before have been waited for by the half that both runs have, or were not made: the queries' place is free)
       const bool mine = i == 0 || run.rows > PS_HALF;
       const int at = PS_HALF * i + r;
+      cursor.tell(a, run, at);
       if (mine) {
-        const bool live = at < run.rows;
-        const int token = live ? a.plan.order()[run.tile.y + at / per] : 0;
-        const uint4* src = reinterpret_cast<const uint4*>(a.q) + ((int64_t)token * a.H + (int64_t)run.g * per + (live ? at % per : 0)) * 16;
-        const uint32_t dst = base + i * FT_TILE_BYTES + r * 128;
+        // 16 lanes have a row, so that a load is two whole rows (a row per lane: 16 loads of 32 lines each, 9100 cycles instead of CYC)
+        const int64_t line = at < run.rows ? ((int64_t)a.plan.order()[run.tile.y + at / per] * a.H + (int64_t)run.g * per + at % per) * 16 : -1;
+        const int c = lane & 15;
         uint4 x[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) x[c] = live ? src[c] : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < 16; ++k) {
+          const int64_t from = __shfl_sync(~0u, line, 2 * k + (lane >> 4));
+          x[k] = from >= 0 ? reinterpret_cast<const uint4*>(a.q)[from + c] : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * FT_HALF + (((c & 7) ^ (r & 7)) << 4)), "r"(x[c].x), "r"(x[c].y),
-                       "r"(x[c].z), "r"(x[c].w)
+        for (int k = 0; k < 16; ++k) {
+          const int row = q * 32 + 2 * k + (lane >> 4);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(base + i * FT_TILE_BYTES + (c >> 3) * FT_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)),
+                       "r"(x[k].x), "r"(x[k].y), "r"(x[k].z), "r"(x[k].w)
                        : "memory");
+        }
         fence_proxy_async_smem();
       }
       __syncwarp();
@@ -202,8 +208,11 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
         continue;
       }
       ++round;
+      if (lane == 0) s_kept[warp].cursor = cursor, s_kept[warp].run = run;
+      __syncwarp();
+      const int common = run.common, first = run.first, last = run.last;
       float m = -INFINITY, sum = 0.f;
-      for (int u = run.first; u < run.last; ++u) {
+      for (int u = first; u < last; ++u) {
         if (!(ok = wait(sh->s_full[i], sph, 2 + i))) break;
         sph ^= 1u;
         tc_fence_after();
@@ -211,7 +220,7 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, s + 32 * c);
         tmem_ld_wait();
-        const int n = run.common - u * FT_KEYS;            // shared keys from this step's first on
+        const int n = common - u * FT_KEYS;            // shared keys from this step's first on
         if (n < FT_KEYS || bad) {
           unsigned pages = 0xffu;                          // which 16 keys have a page
           if (bad) {
@@ -234,8 +243,8 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
         t0 = max3(t0, s[124], s[125]);
         t1 = max3(t1, s[126], s[127]);
         const float mt = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * a.scale_log2e - SHIFT;      // (the host sends positive scales here)
-        const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.f : mn, f = ex2(m - ref);
-        const bool rescale = u > run.first && __any_sync(~0u, mn > m);
+        const float mn = mt > m + LAG ? mt : m, ref = mn == -INFINITY ? 0.f : mn, f = ex2(m - ref);
+        const bool rescale = u > first && __any_sync(~0u, mn > m);
         m = mn;
         const float2 nm2 = make_float2(-ref, -ref);
         float2 a0 = make_float2(0.f, 0.f), a1 = a0;
@@ -280,19 +289,34 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
       }
       if (ok) ok = wait(sh->o_full[i], oph, 2 + i);
       oph ^= 1u;
+      cursor = s_kept[warp].cursor, run = s_kept[warp].run;
       if (ok) {
         tc_fence_after();
-        float* row = a.rec + (((int64_t)run.item + blockIdx.x) * PS_ROWS + at) * (FT_D + 4);
-        const bool live = at < run.rows;
-        if (live) *reinterpret_cast<float2*>(row) = make_float2(m, sum);
+        // A row's outputs are in a lane: 32 columns at a time go through the warp's own place among the queries, which nobody reads any more, so that
+        // lines are written whole.
+        float* part = a.rec + (((int64_t)run.item + blockIdx.x) * PS_ROWS + PS_HALF * i + 32 * q) * (FT_D + PS_HEAD);
+        const int rows = min(32, run.rows - PS_HALF * i - 32 * q);
+        if (lane < rows) *reinterpret_cast<float2*>(part + lane * (FT_D + PS_HEAD)) = make_float2(m, sum);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+          const uint32_t own = base + i * FT_TILE_BYTES + (c & 1) * FT_HALF + q * 4096;
           float o[32];
           tmem_ld32(o_addr + 32 * c, o);
           tmem_ld_wait();
-          if (!live) continue;
+          if (rows <= 0) continue;
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(row + 4 + 32 * c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          for (int k = 0; k < 8; ++k)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(own + lane * 128 + ((k ^ (lane & 7)) << 4)), "f"(o[4 * k]), "f"(o[4 * k + 1]),
+                         "f"(o[4 * k + 2]), "f"(o[4 * k + 3])
+                         : "memory");
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int row = 4 * k + (lane >> 3), ch = lane & 7;
+            const uint4 y = lds128(own + row * 128 + ((ch ^ (row & 7)) << 4));
+            if (row < rows) *reinterpret_cast<uint4*>(part + row * (FT_D + PS_HEAD) + PS_HEAD + 32 * c + 4 * ch) = y;
+          }
+          __syncwarp();
         }
         tc_fence_before();                                 // (the next run's first products write there again)
       }

@@ -11,6 +11,7 @@
 
 namespace b200p {
 
+constexpr int PS_HEAD = 8;                       // floats before a part's outputs: maximum, sum (whole sectors of 32 bytes behind them)
 constexpr int PS_ROWS = 256;                     // query rows of a tile: tokens x query heads of a key head
 constexpr int PS_HALF = 128, PS_WARPS = 8;       // of which paged_prefix_kernel takes 128 at a time, 16 to a warp
 
@@ -23,8 +24,9 @@ struct PagedPrefix {
   float scale_log2e;
   uint64_t inv_tpp;
   int tpp;
-  float* rec;            // [items + CTAs, rows of an item, D + 4] parts, of item i in CTA c the one at i + c
-  int4* info;            // [M] the token's tile, its place in it (and in the upper half the tile's items per key head), the tile's first unit, units of an item
+  float* rec;            // [items + CTAs, rows of an item, PS_HEAD + D] parts, of item i in CTA c the one at i + c
+  int4* info;            // [M] the token's tile, its place in it (and in the upper half the tile's items per key head), the tile's first unit, units of an item (0:
+                         // the token reads by itself)
   unsigned* total;       // units of all
   int* wait_word;
   int box;               // keys that one copy brings: they lie in one page
@@ -79,7 +81,7 @@ struct PrefixCursor {
   static __device__ __forceinline__ unsigned units(const PagedPrefix& a, const PrefixRun& r) { return (unsigned)r.n * a.G * halves(r); }
   __device__ bool next(const PagedPrefix& a, PrefixRun& r) {
     if (u >= end) return false;
-    look(a, ti, r);
+    if (r.ti != ti) look(a, ti, r);                                 // (the plan has looked at the first)
     while (u - base >= units(a, r)) {
       base += units(a, r);
       look(a, ++ti, r);
@@ -91,15 +93,23 @@ struct PrefixCursor {
     u += r.last - r.first;
     return true;
   }
+  // what the join has to know of the tile's tokens, by the threads of the CTA that begins its first item
+  __device__ __forceinline__ void tell(const PagedPrefix& a, const PrefixRun& r, int thread) const {
+    if (r.g == 0 && r.half == 0 && r.first == 0 && thread < r.tile.z) {
+      const int t = a.plan.order()[r.tile.y + thread];
+      const bool shares = slots_seen(a.pt, a.t_slot[t]) >= r.common;
+      a.info[t] = make_int4(r.ti, thread | halves(r) << 16, (int)base, shares ? r.n : 0);
+    }
+  }
 };
 
-// By the whole CTA: units of all tiles, this CTA's part, and (by the first CTA) what the join has to know of every token.
+// By the whole CTA: units of all tiles and this CTA's part.
 struct PrefixPlan {
   unsigned sum[16], base;
-  int tile;
+  PrefixRun first;
 };
 template <int THREADS, int KT, bool SPLIT>
-__device__ __forceinline__ PrefixCursor<KT, SPLIT> prefix_plan(const PagedPrefix& a, PrefixPlan& s) {
+__device__ __forceinline__ PrefixCursor<KT, SPLIT> prefix_plan(const PagedPrefix& a, PrefixPlan& s, PrefixRun& first) {
   using C = PrefixCursor<KT, SPLIT>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = a.plan.tiles(), chunk = (tiles + THREADS - 1) / THREADS;
@@ -131,14 +141,15 @@ __device__ __forceinline__ PrefixCursor<KT, SPLIT> prefix_plan(const PagedPrefix
   for (int i = i0; i < i1; ++i) {
     if (i0 + 1 < i1) C::look(a, i, r);
     const unsigned n = C::units(a, r);
-    if (c.u - before < n) s.tile = i, s.base = before;
-    if (blockIdx.x == 0)
-      for (int k = 0; k < r.tile.z; ++k) a.info[a.plan.order()[r.tile.y + k]] = make_int4(i, k | C::halves(r) << 16, (int)before, r.n);
+    if (c.u - before < n) s.first = r, s.base = before;
+    if (n == 0 && blockIdx.x == 0)                                  // nobody will go through this tile
+      for (int k = 0; k < r.tile.z; ++k) a.info[a.plan.order()[r.tile.y + k]] = make_int4(0, 0, 0, 0);
     before += n;
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.total = U;
   __syncthreads();
-  c.ti = s.tile, c.base = s.base;                                   // (where there is nothing to do nobody looks at them)
+  first = s.first;                                                  // (where there is nothing to do nobody looks at it)
+  c.ti = first.ti, c.base = s.base;
   return c;
 }
 
@@ -163,12 +174,13 @@ paged_prefix_kernel(const __grid_constant__ PagedPrefix a) {
   const int per = a.H / a.G;
   pdl_wait();
   pdl_launch_dependents();
-  PrefixCursor<KT, true> cursor = prefix_plan<THREADS, KT, true>(a, s_plan);
-  const uint32_t qs = (uint32_t)__cvta_generic_to_shared(smem), ring = qs + P::Q_BYTES;
   PrefixRun run;
+  PrefixCursor<KT, true> cursor = prefix_plan<THREADS, KT, true>(a, s_plan, run);
+  const uint32_t qs = (uint32_t)__cvta_generic_to_shared(smem), ring = qs + P::Q_BYTES;
   while (cursor.next(a, run)) {
     const int first = run.first, last = run.last, g = run.g, common = run.common, rows = run.rows - PS_HALF * run.half, r0 = PS_HALF * run.half;
     const int32_t* table = a.pt.table + (int64_t)run.table_row * a.pt.width;
+    cursor.tell(a, run, threadIdx.x);
     __syncthreads();                                                // the item before this one is done with shared memory
     if ((int)threadIdx.x < PS_HALF) {
       const int k = (r0 + (int)threadIdx.x) / per;
@@ -299,53 +311,53 @@ paged_prefix_kernel(const __grid_constant__ PagedPrefix a) {
     cp_async_wait<0>();
     // ---- the part ---------------------------------------------------------------------------------------------------------------
     if (works) {
-      float* rec = a.rec + ((int64_t)run.item + blockIdx.x) * PS_HALF * (D + 4);
+      float* rec = a.rec + ((int64_t)run.item + blockIdx.x) * PS_HALF * (D + PS_HEAD);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float sum = l[h];
         sum += __shfl_xor_sync(~0u, sum, 1);
         sum += __shfl_xor_sync(~0u, sum, 2);
-        float* row = rec + (16 * warp + 8 * h + qr) * (D + 4);
+        float* row = rec + (16 * warp + 8 * h + qr) * (D + PS_HEAD);
         if (qc == 0) *reinterpret_cast<float2*>(row) = make_float2(m[h], sum);
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(row + 4 + 8 * j + 2 * qc) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+        for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(row + PS_HEAD + 8 * j + 2 * qc) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
       }
     }
   }
 }
 
-// A CTA per token and query head joins the parts of the shared slots and of the own ones: a warp takes them in turn, then the warps become one.
-template <typename T, int NQ, int ROWS, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32)
+// The parts of the shared slots and of the own ones become a token's outputs: W warps per query head, a CTA of 8.
+template <typename T, int NQ, int ROWS, int W>
+__global__ void __launch_bounds__(256)
 paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ PagedPrefix p, int prefix_ctas, int item_rows) {
-  __shared__ float2 s_ml[WARPS];
-  __shared__ float4 s_o[WARPS][32 * NQ];
-  const int r = blockIdx.x, g = blockIdx.y, t = blockIdx.z, per = gridDim.x, blocks = (per + ROWS - 1) / ROWS, warp = threadIdx.x >> 5,
-            lane = threadIdx.x & 31, D = a.D;
+  __shared__ float2 s_ml[8];
+  __shared__ float4 s_o[W > 1 ? 8 : 1][32 * NQ];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = a.D, per = a.H / a.G, blocks = (per + ROWS - 1) / ROWS, t = blockIdx.y;
+  const int head = (int)blockIdx.x * (8 / W) + warp / W, g = head / per, r = head - g * per;
   pdl_wait();
-  const int64_t line = ((int64_t)t * a.G + g) * blocks + r / ROWS;
-  const int row = a.t_row[t];
+  const bool here = head < a.H;
+  const int64_t line = ((int64_t)t * a.G + (here ? g : 0)) * blocks + (here ? r / ROWS : 0);
+  const int row = a.t_row[t], group = p.index[t];
   const uint2 parts = a.parts[line];
-  const bool member = shared_slots(p.index, p.prefix, p.groups, a.pt, t, slots_seen(a.pt, a.t_slot[t])) > 0;
-  const int4 info = p.info[member ? t : 0];
+  const int4 info = p.info[t];                                      // (written for tokens of groups)
   const unsigned total = *p.total;
   if (row < 0 || row >= a.pt.rows) return;
   int heads = 0, c0 = 0;                                            // parts of the shared slots
-  int64_t from = 0;                                                 // the first of them
-  if (member) {
+  int64_t row0 = 0;                                                 // its row in the first of them
+  if ((unsigned)group < (unsigned)p.groups && info.w > 0) {
     const PrefixShares sh(total, prefix_ctas);
     const int halves = info.y >> 16, at = (info.y & 0xffff) * per + r, half = halves > 1 && at >= PS_HALF ? 1 : 0;
     const unsigned u = (unsigned)info.z + (unsigned)((g * halves + half) * info.w);
     c0 = (int)sh.of(u);
     heads = (int)sh.of(u + info.w - 1) - c0 + 1;
-    from = (int64_t)(item_rows == PS_HALF ? (info.x * a.G + g) * 2 + half : info.x * a.G + g) + c0;
-    from = from * item_rows + at - PS_HALF * half;
+    row0 = (int64_t)(item_rows == PS_HALF ? (info.x * a.G + g) * 2 + half : info.x * a.G + g) + c0;
+    row0 = row0 * item_rows + at - PS_HALF * half;
   }
-  const int all = heads + (int)parts.y;
-  auto at = [&](int i) -> const float* {
-    if (i < heads) return p.rec + (from + (int64_t)i * item_rows) * (D + 4);
-    if (parts.y == 1) return a.whole + (line * ROWS + r % ROWS) * (D + 4);
-    return part_at(a, parts.x, i - heads, ROWS, r % ROWS);
+  const int all = here ? heads + (int)parts.y : 0;
+  auto at = [&](int i) -> const float* {                            // its outputs; maximum and sum stand before them
+    if (i < heads) return p.rec + (row0 + (int64_t)i * item_rows) * (D + PS_HEAD) + PS_HEAD;
+    if (parts.y == 1) return a.whole + (line * ROWS + r % ROWS) * (D + 4) + 4;
+    return part_at(a, parts.x, i - heads, ROWS, r % ROWS) + 4;
   };
   constexpr int AHEAD = 4;
   float M = -INFINITY, L = 0.f;
@@ -353,17 +365,18 @@ paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_const
 #pragma unroll
   for (int x = 0; x < NQ; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-  for (int i0 = warp; i0 < all; i0 += AHEAD * WARPS) {
+  for (int i0 = warp % W; i0 < all; i0 += AHEAD * W) {
     float2 ml[AHEAD];
     float4 y[AHEAD][NQ];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const bool in = i0 + k * WARPS < all;
-      const float* from = at(in ? i0 + k * WARPS : i0);
-      ml[k] = in ? *reinterpret_cast<const float2*>(from) : make_float2(-INFINITY, 0.f);
+      const int i = i0 + k * W;
+      const bool in = i < all;
+      const float* from = at(in ? i : i0);
+      ml[k] = in ? *reinterpret_cast<const float2*>(from - (i < heads ? PS_HEAD : 4)) : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int x = 0; x < NQ; ++x)
-        y[k][x] = in && 4 * lane + 128 * x < D ? *reinterpret_cast<const float4*>(from + 4 + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+        y[k][x] = in && 4 * lane + 128 * x < D ? *reinterpret_cast<const float4*>(from + 4 * lane + 128 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float top = M;
 #pragma unroll
@@ -381,28 +394,39 @@ paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_const
       for (int x = 0; x < NQ; ++x) acc[x].x += y[k][x].x * w, acc[x].y += y[k][x].y * w, acc[x].z += y[k][x].z * w, acc[x].w += y[k][x].w * w;
     }
   }
-  if (lane == 0) s_ml[warp] = make_float2(M, L);
+  if constexpr (W > 1) {
+    if (lane == 0) s_ml[warp] = make_float2(M, L);
 #pragma unroll
-  for (int x = 0; x < NQ; ++x) s_o[warp][lane + 32 * x] = acc[x];
-  __syncthreads();
-  const int d = 4 * threadIdx.x;
-  if (d >= D) return;
-  float top = -INFINITY;
+    for (int x = 0; x < NQ; ++x) s_o[warp][lane + 32 * x] = acc[x];
+    __syncthreads();
+    if (warp % W) return;                                           // the first warp of a head goes on
+    float top = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_ml[w].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[warp + w].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    L = 0.f;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    const float f = raise2(s_ml[w].x - ref);
-    const float4 y = s_o[w][threadIdx.x];
-    sum += s_ml[w].y * f;
-    o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
+    for (int x = 0; x < NQ; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = raise2(s_ml[warp + w].x - ref);
+      L += s_ml[warp + w].y * f;
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        const float4 y = s_o[warp + w][lane + 32 * x];
+        acc[x].x += y.x * f, acc[x].y += y.y * f, acc[x].z += y.z * f, acc[x].w += y.w * f;
+      }
+    }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  store_row4<T>(reinterpret_cast<T*>(a.out) + ((int64_t)t * a.H + (int64_t)g * per + r) * D, d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv),
-                a.out_perm);
+  if (!here) return;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const int d = 4 * lane + 128 * x;
+    if (d < D)
+      store_row4<T>(reinterpret_cast<T*>(a.out) + ((int64_t)t * a.H + head) * D, d, make_float4(acc[x].x * inv, acc[x].y * inv, acc[x].z * inv, acc[x].w * inv),
+                    a.out_perm);
+  }
 }
 
 }  // namespace b200p
