@@ -62,6 +62,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from .. import ops
+from ..ops import TokenLogprobs
 import math
 
 from .._lib import (GATE_SIGMOID, GATE_SILU, GEMM_CAP_F32, GEMM_GLU_CLAMP, GEMM_GLU_GELU_TANH, GEMM_GLU_SILU, GEMM_RELU_SQ, GEMM_STORE,
@@ -1306,7 +1307,8 @@ class SequenceModel:
         with self._lock:
             return self._forward_ragged_locked(seqs, cache, rows, want)
 
-    def _forward_ragged_locked(self, seqs, cache, rows, want):
+    def _forward_ragged_locked(self, seqs, cache, rows, want, sink=None):
+        """``sink(rows, where, arena)``: gets the residual rows of the wanted positions (entry, place in want[entry]) instead of their logits being returned."""
         from ._transformer import advance_rows, prepare_rows
         nb = len(seqs)
         rows = list(range(nb)) if rows is None else [int(r) for r in rows]
@@ -1348,11 +1350,16 @@ class SequenceModel:
                         where.append((i, k))
             if pick:
                 hs = a["h"][:M].index_select(0, torch.tensor(pick, dtype=torch.int64, device=dev))
-                lg = self._head(hs, a)
-                for j, (i, k) in enumerate(where):
-                    outs[i][k] = lg[j]
+                if sink is not None:
+                    sink(hs, where, a)
+                else:
+                    lg = self._head(hs, a)
+                    for j, (i, k) in enumerate(where):
+                        outs[i][k] = lg[j]
             for i in range(nb):
                 done[i] += take[i]
+        if sink is not None:
+            return None
         flat_out = [t for o in outs for t in o]
         if any(t is None for t in flat_out):
             raise ValueError("a wanted position lies outside its entry's tokens")
@@ -1379,6 +1386,36 @@ class SequenceModel:
         for b in range(B):
             out[b, L - n[b]:] = lg[o:o + n[b]]
             o += n[b]
+        return out
+
+    def score(self, inputs, top: int = 0, temperature: float = 1.0, cache: Optional[List[RowState]] = None, prompt_lengths=None) -> TokenLogprobs:
+        """DecoderModel.score for packed prompts: row b's entries are those of its last prompt_lengths[b] ids, the others are 0."""
+        from ._transformer import SCORE_BYTES, empty_logprobs
+        inputs = inputs if isinstance(inputs, torch.Tensor) else torch.as_tensor(inputs)
+        B, L = inputs.shape
+        host = inputs.tolist()
+        n = [L] * B if prompt_lengths is None else [int(v) for v in prompt_lengths]
+        out = empty_logprobs((B, L), top, self.device)
+        for t in out:
+            t.zero_()
+        flat = TokenLogprobs(*(t.view(B * L, *t.shape[2:]) for t in out))
+        V = self.lm_head.out_features
+
+        def sink(hs, where, a):
+            at = [(i, L - n[i] + k) for i, k in where]
+            place = torch.tensor([i * L + l for i, l in at], dtype=torch.int64, device=self.device)
+            tokens = torch.tensor([host[i][l + 1] if l + 1 < L else -1 for i, l in at], dtype=torch.int32, device=self.device)
+            M = len(at)
+            step = max(1, min(M, SCORE_BYTES // (4 * V)))
+            for r in range(0, M, step):
+                got = ops.token_logprobs(self._head(hs[r:r + step], a), tokens[r:r + step], top, temperature)
+                for t, v in zip(flat, got):
+                    t[place[r:r + step]] = v
+
+        with self._lock:
+            if cache is None:
+                cache = self.make_cache(B, step=max(L, 1))
+            self._forward_ragged_locked([host[b][L - n[b]:] for b in range(B)], cache, None, [list(range(k)) for k in n], sink)
         return out
 
     def release_rows(self, cache: List[RowState], rows: Sequence[int]):

@@ -28,11 +28,13 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from .. import ops
+from ..ops import TokenLogprobs
 from .._lib import EPI_ADD_RESIDUAL, EPI_SILU_MUL, EPI_STORE, EPI_STORE_F32
 from .base import BatchedKVCache, PagedKVCache
-from .paged import PageBook, PagedLayer
+from .paged import PageBook, PagedLayer, PagesExhausted
 
 MAX_TOKENS_PER_FORWARD = 8192     # chunk size (B*L) of one prefill pass through the layers
+SCORE_BYTES = 256 << 20           # logits that scoring holds at a time (one row at least)
 # Up to this many rows the fused q|k|v projection accumulates in an fp32 buffer through the stream-K kernel (csrc/qmm_sk.cu:
 # partial tiles summed by TMA reduce-adds, no tail; rope_kv_append rounds to the storage type and re-zeroes the buffer).
 # q|k|v has 24 output tiles for 148 SMs, so it must split K; measured at 64 rows: 16.8 us through the
@@ -106,6 +108,7 @@ class Attention:
         self.o_proj = QuantizedLinear(self.n_heads * head_dim, h, gs, bits)
         self.qkv_proj = QuantizedLinear(h, (self.n_heads + 2 * self.n_kv_heads) * head_dim, gs, bits)
         self.lora: Dict[str, tuple] = {}      # "q_proj" / "v_proj" -> (At [16,K], Bt [N,16], scale): set by apply_lora
+        self.loras: Optional[tuple] = None    # (a [n, targets, R, K], b [n, columns, R], scales [n], columns): set by apply_loras
         self.q_norm = RMSNorm(head_dim, args.rms_norm_eps) if qk_norm else None
         self.k_norm = RMSNorm(head_dim, args.rms_norm_eps) if qk_norm else None
 
@@ -177,6 +180,7 @@ class DecoderModel:
         self.device: Optional[torch.device] = None
         self._rope_rates: Optional[torch.Tensor] = None
         self._arenas: Dict[int, dict] = {}
+        self._adapters = 0                    # adapters that apply_loras holds
         # One forward at a time per model instance: the scratch arenas, the self-cleaning qmm
         # workspace and the fp32 accumulators are shared by every caller of this model, and the reference server runs
         # generate_step from an executor thread and from the event loop at once (utils.py:1345 vs server/main.py:1358).
@@ -291,6 +295,8 @@ class DecoderModel:
         model's forward lock, so a generation in flight sees either the old or the new set, never a mix."""
         if not self._fast16:
             raise NotImplementedError("LoRA needs a 16-bit model (b200p_lora_add)")
+        if adapters and self._adapters:
+            raise RuntimeError("adapters for single rows are held: apply_loras([], []) first")
         new_sets = []
         for i, layer in enumerate(self.model.layers):
             new_sets.append({})
@@ -323,6 +329,86 @@ class DecoderModel:
                 layer.self_attn.lora = st
             self._arenas.clear()          # captured decode graphs hold the old adapter pointers: force a re-capture
         return self
+
+    def apply_loras(self, adapters: Sequence[Dict[str, torch.Tensor]], scales: Sequence[float], keys=("self_attn.q_proj", "self_attn.v_proj")):
+        """Hold several mlx_lm-format adapters at once, each in apply_lora's form; ``bind_adapters`` (or ``generate_step(adapters=)``) says which row of a
+        batch goes under which (b200p_lora_rows).  ``keys``: any of self_attn.q_proj, k_proj and v_proj; ranks up to 64 and layers may differ between
+        adapters.  [] drops them.  A cache bound before keeps its numbers: rows of an adapter that is gone have none."""
+        if not self._fast16:
+            raise NotImplementedError("LoRA needs a 16-bit model (b200p_lora_rows)")
+        if len(adapters) != len(scales):
+            raise ValueError(f"{len(adapters)} adapters and {len(scales)} scales")
+        if len(adapters) > 1024:
+            raise ValueError("at most 1024 adapters at once")
+        names = [k.split(".")[-1] for k in keys]
+        if any(k not in ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj") for k in keys) or len(set(names)) != len(names):
+            raise NotImplementedError(f"LoRA on {tuple(keys)} is not built (q_proj, k_proj, v_proj)")
+        if adapters and any(layer.self_attn.lora for layer in self.layers):
+            raise RuntimeError("an adapter for all rows is applied: apply_lora({}) first")
+        held = []
+        for i, layer in enumerate(self.model.layers):
+            at = layer.self_attn
+            widths = [getattr(at, n).weight.shape[0] for n in names]
+            first = {"q_proj": 0, "k_proj": at.n_heads * at.head_dim, "v_proj": (at.n_heads + at.n_kv_heads) * at.head_dim}
+            pre = [f"model.layers.{i}.{k}." for k in keys]
+            ranks = [ad[q + "lora_a"].shape[1] for ad in adapters for q in pre if q + "lora_a" in ad]
+            if not ranks:
+                held.append(None)
+                continue
+            K, R = at.q_proj.in_features, -(-max(ranks) // 16) * 16
+            if R > 64:
+                raise NotImplementedError(f"LoRA rank {max(ranks)} > 64")
+            a = torch.zeros((len(adapters), len(keys), R, K), dtype=self.dtype, device=self.device)
+            b = torch.zeros((len(adapters), sum(widths), R), dtype=self.dtype, device=self.device)
+            for j, ad in enumerate(adapters):
+                row = 0
+                for k, (q, width) in enumerate(zip(pre, widths)):
+                    if q + "lora_a" in ad:
+                        A, Bm = ad[q + "lora_a"].to(self.device, self.dtype), ad[q + "lora_b"].to(self.device, self.dtype)      # [K, r], [r, N]
+                        if Bm.shape[1] != width:                        # full-width adapter on a column shard
+                            if Bm.shape[1] != width * self.tp_world:
+                                raise ValueError(f"{q}lora_b: {Bm.shape[1]} output columns do not match the projection ({width} x tp {self.tp_world})")
+                            Bm = Bm[:, self.tp_rank * width:(self.tp_rank + 1) * width]
+                        if A.shape[0] != K or A.shape[1] != Bm.shape[0]:
+                            raise ValueError(f"{q}lora_a {tuple(A.shape)} and lora_b {tuple(Bm.shape)} of a projection of {K} inputs")
+                        a[j, k, :A.shape[1]] = A.t()
+                        b[j, row:row + width, :A.shape[1]] = Bm.t()
+                    row += width
+            if self._perm8:                                            # x arrives as [0,4,1,5,2,6,3,7] inside each group of 8
+                a = a.view(*a.shape[:3], K // 8, 8)[..., [0, 4, 1, 5, 2, 6, 3, 7]].reshape(a.shape).contiguous()
+            held.append((a, b, torch.tensor([float(s) for s in scales], dtype=torch.float32, device=self.device),
+                         tuple((first[n], w) for n, w in zip(names, widths))))
+        with self._lock:
+            for layer, st in zip(self.model.layers, held):
+                layer.self_attn.loras = st
+            self._adapters = len(adapters)
+            self._arenas.clear()          # captured decode graphs hold the old adapters' pointers
+        return self
+
+    def bind_adapters(self, cache, adapters: Optional[Sequence[int]]):
+        """Row r of ``cache`` goes under adapter ``adapters[r]`` of apply_loras (-1: under none) until the cache is reset; None: no row under any.  What a row
+        holds already keeps the keys and values that it was given."""
+        first = cache[0]
+        if adapters is None:
+            first.adapter_rows = None
+            return
+        rows = [int(v) for v in adapters]
+        if len(rows) != first.batch_size or any(not -1 <= v < self._adapters for v in rows):
+            raise ValueError(f"one of the {self._adapters} adapters (or -1) for each of the {first.batch_size} rows: got {rows}")
+        with self._lock:
+            if first.adapter_index is None or first.adapter_index.numel() != len(rows):
+                first.adapter_index = torch.empty((len(rows),), dtype=torch.int32, device=self.device)
+            first.adapter_index.copy_(torch.tensor(rows, dtype=torch.int32))
+            first.adapter_rows = rows
+
+    def _adapter_plan(self, cache, B: int, L: int, a: dict):
+        """The step's tokens in the order of their adapters (None: no row is under one)."""
+        if not self._adapters or cache[0].adapter_rows is None:
+            return None
+        index = cache[0].adapter_index
+        if L == 1:
+            return ops.row_groups(index, self._adapters, a["adapter_plan"].tile, out=a["adapter_plan"])
+        return ops.row_groups(index.repeat_interleave(L), self._adapters, ops.lora_tile(B * L, self._adapters))
 
     def set_tensor_parallel(self, rank: int, world: int, allreduce):
         """allreduce(tensor_f32) sums in place across ranks on the current stream."""
@@ -375,6 +461,44 @@ class DecoderModel:
         self.rope_rates()                                               # (not inside a capture)
         return [PagedLayer(book, l.self_attn.n_heads, l.self_attn.n_kv_heads, self.head_dim) for l in self.model.layers]
 
+    def share_prompt(self, cache: List[PagedLayer], prompts, groups: Sequence[Sequence[int]]) -> torch.Tensor:
+        """Rows that begin with the same prompt: ``prompts`` int [n, L], read once each, ``groups[i]`` the empty rows of ``cache`` (in pages, without a window or
+        ``keep``) that go on from prompt i.  They have its whole pages together, which a decode step then reads once for all of them
+        (b200p_paged_attn_shared); the rows of a group are under one adapter.  -> logits float32 [n, V] of the prompts' last tokens."""
+        if not isinstance(cache[0], PagedLayer):
+            raise NotImplementedError("rows of a dense cache share no pages")
+        prompts = prompts if isinstance(prompts, torch.Tensor) else torch.as_tensor(prompts)
+        groups, book, first = [[int(r) for r in g] for g in groups], cache[0].book, cache[0]
+        rows = [r for g in groups for r in g]
+        if prompts.dim() != 2 or prompts.shape[0] != len(groups) or not prompts.numel() or any(not g for g in groups):
+            raise ValueError(f"prompts are [n, L], with rows for each: got {tuple(prompts.shape)} and {len(groups)} groups")
+        if len(set(rows)) != len(rows) or any(not 0 <= r < book.rows for r in rows):
+            raise ValueError(f"a row has one prompt, and rows are 0 to {book.rows - 1}: got {groups}")
+        if book.window or book.keep:
+            raise NotImplementedError("rows of a cache with a window, or whose rows are cut, share no pages")
+        if any(first._offsets[r] or not book.live[r] for r in rows):
+            raise ValueError("rows that share a prompt are empty and in use")
+        bound = first.adapter_rows
+        if bound is not None and any(bound[r] != bound[g[0]] for g in groups for r in g):
+            raise ValueError("the rows of a group are under one adapter: its keys and values are the prompt's")
+        n, L = prompts.shape
+        with self._lock:
+            prepare_cache(cache, book.rows, 0, self.dtype, self.device)            # (the pages of every layer)
+            if L + 1 > book.max_tokens:
+                raise PagesExhausted(f"a prompt of {L} tokens does not fit a paged cache of {book.max_tokens} per row")
+            side = PageBook(n, L, self.device, book.page, book.pages, of=book)
+            layers = [PagedLayer(side, c.n_heads, c.n_kv_heads, c.head_dim) for c in cache]
+            for mine, c in zip(layers, cache):
+                mine.kpages, mine.vpages = c.kpages, c.vpages
+            if bound is not None:
+                self.bind_adapters(layers, [bound[g[0]] for g in groups])
+            try:
+                logits = self(prompts, cache=layers, last_only=True)[:, -1, :]
+                book.adopt(side, groups, L)
+            finally:
+                side.shrink([0] * n)                                    # (what was adopted is the rows' own)
+            return logits
+
     def release_rows(self, cache: List[PagedLayer], rows: Sequence[int]):
         """Rows of a cache in pages that have ended: their pages go back to the pool, and until the cache is reset the next steps leave them out (what
         those steps return for them means nothing).  The others' captured decode step stays valid."""
@@ -424,6 +548,9 @@ class DecoderModel:
                 ws=torch.zeros((ws_q,), dtype=torch.uint8, device=dev),
                 ws_attn=torch.empty((ws_a,), dtype=torch.uint8, device=dev),
             )
+            if self._adapters and M == B:      # (where a captured step knows it)
+                n, tile = self._adapters, ops.lora_tile(M, self._adapters)
+                a["adapter_plan"] = ops.row_groups(torch.full((M,), -1, dtype=torch.int32, device=dev), n, tile)
             fx = getattr(self, "_tp_fused", None)
             if fx is not None and fx.mode == "rows":
                 a["x"] = fx.x_view(M, dt)          # filled on every rank by the row-sharded exchange (tp.PeerExchange)
@@ -449,6 +576,7 @@ class DecoderModel:
         rows_mode = fx is not None and fx.mode == "rows"
         a["x_final"] = False
         paged = cache[0].book.tokens(B, L) if isinstance(cache[0], PagedLayer) else None
+        adapters = self._adapter_plan(cache, B, L, a)
         for li, (layer, c) in enumerate(zip(layers, cache)):
             at, mlp = layer.self_attn, layer.mlp
             lengths = c.lengths(self.device)
@@ -461,6 +589,9 @@ class DecoderModel:
                 for name, (At, Bt, scale) in at.lora.items():
                     col0 = 0 if name == "q_proj" else (at.n_heads + at.n_kv_heads) * at.head_dim
                     ops.lora_add(a["x"], At, Bt, qkv_buf, col0, scale)
+            if adapters is not None and at.loras is not None:           # every row under an adapter of its own
+                la, lb, scales, columns = at.loras
+                ops.lora_rows(a["x"], adapters, la, lb, scales, columns, qkv_buf)
             if paged is not None:
                 c.append_and_attend(qkv_buf, a["q"], a["att"], paged, B, L, at.n_heads, self.rope_rates(), at.scale,
                                     at.q_norm.weight if at.q_norm else None, at.k_norm.weight if at.k_norm else None,
@@ -526,13 +657,58 @@ class DecoderModel:
         head = self.lm_head if self.lm_head is not None else self.model.embed_tokens
         return QuantizedLinear.__call__(head, x, EPI_STORE_F32, out=logits_out, workspace=a["ws"], x_perm=self._perm8)
 
+    def _score_rows(self, h_rows, tokens, top: int, temperature: float, a: dict) -> TokenLogprobs:
+        """token_logprobs of the rows' logits, of which SCORE_BYTES are held at a time."""
+        head = self.lm_head if self.lm_head is not None else self.model.embed_tokens
+        M, V = h_rows.shape[0], head.out_features
+        out = empty_logprobs((M,), top, self.device)
+        n = max(1, min(M, SCORE_BYTES // (4 * V)))
+        need = max(ops.qmm_workspace_bytes(m, V, self.args.hidden_size) for m in {n, M % n or n})
+        if a["ws"].numel() < need:
+            a = dict(a, ws=torch.zeros((need,), dtype=torch.uint8, device=self.device))
+        logits = torch.empty((n, V), dtype=torch.float32, device=self.device)
+        for r in range(0, M, n):
+            part = logits[:min(n, M - r)]
+            self._head(h_rows[r:r + n], a, logits_out=part)
+            ops.token_logprobs(part, tokens[r:r + n], top, temperature, out=TokenLogprobs(*(t[r:r + n] for t in out)))
+        return out
+
+    def score(self, inputs, top: int = 0, temperature: float = 1.0, cache=None, adapters: Optional[Sequence[int]] = None) -> TokenLogprobs:
+        """How likely a text's own tokens were (the server's echoed log probabilities and perplexities, server/main.py:458-659; GRPO's,
+        rl_training/grpo_trainer.py:74-120): inputs int [B, L] -> TokenLogprobs of [B, L] entries, entry l about what follows token l -- the log probability of
+        token l + 1 (0 behind the last one), the entropy, the ``top`` most likely tokens ([B, L, top]).  The logits of one portion of rows are held at a
+        time, never those of all.  ``cache``: the text goes on where its rows stand; ``adapters``: every row's (bind_adapters)."""
+        if self.tp_world > 1:
+            raise NotImplementedError("scoring needs the whole vocabulary on one rank")
+        inputs = inputs if isinstance(inputs, torch.Tensor) else torch.as_tensor(inputs)
+        with self._lock:
+            ids = inputs.to(self.device).to(torch.int32).contiguous()
+            B, L = ids.shape
+            out = empty_logprobs((B, L), top, self.device)
+            if not B * L:
+                return out
+            following = torch.cat([ids[:, 1:], ids.new_full((B, 1), -1)], 1)
+
+            def take(l0, l1, rows, a):
+                part = self._score_rows(rows, following[:, l0:l1].reshape(-1), top, temperature, a)
+                for t, v in zip(out, part):
+                    t[:, l0:l1] = v.view(B, l1 - l0, *v.shape[1:])
+
+            if cache is None:
+                cache = self.make_cache(B, step=max(L, 1))
+            if adapters is not None:
+                self.bind_adapters(cache, adapters)
+            self._forward_locked(ids, cache, False, take)
+            return out
+
     def __call__(self, inputs, cache: Optional[List[BatchedKVCache]] = None, last_only: bool = False):
         """inputs int [B, L] -> logits float32 [B, L, V] (or [B, 1, V] with last_only, the only rows
         generate_step reads, utils.py:404).  Under TP the vocab axis is this rank's shard."""
         with self._lock:
             return self._forward_locked(inputs, cache, last_only)
 
-    def _forward_locked(self, inputs, cache, last_only):
+    def _forward_locked(self, inputs, cache, last_only, take=None):
+        """``take(l0, l1, rows, arena)``: gets the residual rows of tokens l0 to l1 instead of their logits being returned."""
         if not isinstance(inputs, torch.Tensor):
             inputs = torch.as_tensor(inputs)
         inputs = inputs.to(self.device)
@@ -555,13 +731,21 @@ class DecoderModel:
             self._layers_forward(chunk, B, n, cache, a)
             advance_cache(cache, n)
             src = a["x"] if a.get("x_final") else a["h"]      # row-sharded TP: x already holds final_norm(h) on every rank
-            if last_only:
+            if take is not None:
+                take(l0, l1, src, a)
+            elif last_only:
                 if l1 == L:
                     last = src if n == 1 else src.view(B, n, -1)[:, -1, :].contiguous()
                     return (self._head(None, a, x_rows=last) if a.get("x_final") else self._head(last, a)).view(B, 1, -1)
             else:
                 outs.append((self._head(None, a, x_rows=src) if a.get("x_final") else self._head(src, a)).view(B, n, -1))
-        return outs[0] if len(outs) == 1 else torch.cat(outs, 1)
+        if take is None:
+            return outs[0] if len(outs) == 1 else torch.cat(outs, 1)
+
+
+def empty_logprobs(shape: tuple, top: int, device) -> TokenLogprobs:
+    new = lambda *extra, dt=torch.float32: torch.empty((*shape, *extra), dtype=dt, device=device)
+    return TokenLogprobs(new(), new(), new(top, dt=torch.int32), new(top))
 
 
 # ---------------------------------------------------------------------------------------------------

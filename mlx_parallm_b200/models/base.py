@@ -36,6 +36,8 @@ class RowState:
         self._offsets: List[int] = [0] * batch_size
         self._lengths: Optional[torch.Tensor] = None     # device int32 [B]; may be shared across layers
         self._lengths_shared = False
+        self.adapter_rows: Optional[List[int]] = None    # in a group's first entry: every row's adapter (DecoderModel.bind_adapters); None: none
+        self.adapter_index: Optional[torch.Tensor] = None     # the same on the device; kept over resets
 
     @property
     def offsets(self):
@@ -60,6 +62,7 @@ class RowState:
 
     def reset(self, batch_size: int | None = None):
         """base.py:52-64 / 145-148: keep buffers when the batch size is unchanged."""
+        self.adapter_rows = None
         if batch_size is not None and batch_size != self.batch_size:
             self.batch_size = batch_size
             self._drop_buffers()

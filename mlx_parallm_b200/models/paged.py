@@ -8,13 +8,16 @@ row takes pages as it grows and gives them back, so memory follows what the rows
   - cut rows that have no room left to the tokens that were attended to most (``keep``, with the ``first`` and the ``recent`` newest ones):
     the layers then add up the attention weight every token receives, and each key head keeps tokens of its own.
 
+Rows may also share the pages of a prompt (DecoderModel.share_prompt): its whole pages stand in the table of every one of them, are read once for all in
+a decode step (b200p_paged_attn_shared) and are given back with the last.
+
 Decode steps read the pages (b200p_paged_attn); prompts are attended to through a dense view of their rows (b200p_paged_gather) by the
 prompt kernels of dense caches, or token by token once the window hides part of a row.  The device table and counters keep their
 addresses, so a captured decode step stays valid while rows grow, shrink and change hands.
 """
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import Dict, List, Optional
 
 import torch
 
@@ -22,6 +25,9 @@ from .. import ops
 from .base import RowState
 
 
+# Keys and values of shared pages that a layer's decode step need not read again from which on it goes by groups: below, the third launch and the
+# groups' plan cost more than the reading (SHAREFIG)
+SHARED_BYTES = 16 << 20
 OBSERVED_BYTES = 256 << 20        # workspace of a call that adds up the weights of a prompt's last tokens (one token per row at least)
 
 
@@ -34,7 +40,8 @@ class PageBook:
     use) and ``positions`` (places in the text: larger than the length once tokens were evicted), and the list of free pages."""
 
     def __init__(self, rows: int, max_tokens: int, device, page: int = 64, pages: Optional[int] = None, window: int = 0, first: int = 0, keep: int = 0,
-                 recent: Optional[int] = None, observe: int = 32):
+                 recent: Optional[int] = None, observe: int = 32, of: Optional["PageBook"] = None):
+        """``of``: a book whose pages this one draws on."""
         if page < 16 or page % 16 or page > 4096:
             raise ValueError(f"a page holds a multiple of 16 tokens, 4096 at most: got {page}")
         if rows < 1 or max_tokens < 1:
@@ -57,7 +64,15 @@ class PageBook:
         self.positions = torch.zeros((rows,), dtype=torch.int32, device=device)
         self.row_index = torch.arange(rows, dtype=torch.int32, device=device)      # -1: a row that was given back, whose tokens are idle
         self.live = [True] * rows
-        self.free: List[int] = list(range(self.pages - 1, -1, -1))
+        self.free: List[int] = list(range(self.pages - 1, -1, -1)) if of is None else of.free
+        self.held: Dict[int, int] = {} if of is None else of.held      # pages that several rows have: how many
+        # rows that share a prompt: every row's group, the groups' shared slots, which rows have them, and whether a step goes by them
+        self.group: Optional[torch.Tensor] = None
+        self.prefix: Optional[torch.Tensor] = None
+        self.plan: Optional[ops.RowPlan] = None
+        self.groups: List[List[int]] = []
+        self.prefixes: List[int] = []
+        self.by_groups = False
         self.owned: List[List[int]] = [[] for _ in range(rows)]
         self.evicted = [0] * rows              # how far a row's positions are ahead of its slots
         self.layers: List["PagedLayer"] = []
@@ -100,9 +115,91 @@ class PageBook:
         for r, n in enumerate(counts):
             left = -(-n // self.page)
             if left < len(self.owned[r]):
-                self.free += reversed(self.owned[r][left:])
+                for p in reversed(self.owned[r][left:]):
+                    n = self.held.get(p, 1) - 1
+                    if n > 1:
+                        self.held[p] = n
+                    elif n == 1:
+                        del self.held[p]
+                    else:
+                        self.free.append(p)
                 del self.owned[r][left:]
                 self.table[r, left:] = -1
+
+    def adopt(self, other: "PageBook", groups: List[List[int]], tokens: int) -> None:
+        """Row i of ``other``, which draws on this book's pages and holds ``tokens`` tokens, becomes all of the rows ``groups[i]``: its whole pages are theirs
+        together, of a last one that is not full everybody but the first gets a copy.  All or nothing: PagesExhausted if the pool is short."""
+        whole, rest = tokens // self.page, tokens % self.page
+        need = sum(len(g) - 1 for g in groups) if rest else 0
+        if need > len(self.free):
+            raise PagesExhausted(f"paged cache exhausted: {need} pages wanted for the rows of a shared prompt, {len(self.free)} of {self.pages} free")
+        source, copies = [], []
+        for i, g in enumerate(groups):
+            pages = other.owned[i]
+            for k, r in enumerate(g):
+                mine = list(pages[:whole])
+                if rest:
+                    mine.append(pages[whole] if k == 0 else self.free.pop())
+                    if k:
+                        source.append(pages[whole])
+                        copies.append(mine[-1])
+                self.owned[r] = mine
+                self.table[r, :len(mine)] = torch.tensor(mine, dtype=torch.int32).to(self.device)
+            if len(g) > 1:
+                for p in pages[:whole]:
+                    self.held[p] = len(g)
+            other.owned[i] = []
+            self.groups.append(list(g))
+            self.prefixes.append(whole * self.page)
+        if copies:
+            at = torch.tensor(source, device=self.device), torch.tensor(copies, device=self.device)
+            for c in self.layers:
+                for pages in (c.kpages, c.vpages):
+                    pages[at[1]] = pages[at[0]]
+        for c in self.layers:
+            for g in groups:
+                for r in g:
+                    c._offsets[r] = tokens
+            c.offset = max(c._offsets)
+        self.layers[0]._sync_lengths()
+        self._regroup()
+
+    def _regroup(self) -> None:
+        """The device's view of the groups, and whether the shared slots are worth a step's going by them.  Once it does, it does so until the cache is reset, so
+        that a captured step stays valid while rows leave."""
+        c = self.layers[0]
+        saved = sum((len(g) - 1) * n for g, n in zip(self.groups, self.prefixes)) * 2 * c.n_kv_heads * c.head_dim * c.kpages.element_size()
+        if not self.by_groups and saved < SHARED_BYTES:
+            return
+        if self.group is None:
+            self.group = torch.empty((self.rows,), dtype=torch.int32, device=self.device)
+            self.prefix = torch.zeros((self.rows,), dtype=torch.int32, device=self.device)
+        index = [-1] * self.rows
+        for i, g in enumerate(self.groups):
+            for r in g:
+                index[r] = i
+        self.group.copy_(torch.tensor(index, dtype=torch.int32))
+        self.prefix.copy_(torch.tensor(self.prefixes + [0] * (self.rows - len(self.prefixes)), dtype=torch.int32))
+        tile = ops.paged_attn_shared_tile(c.n_heads, c.n_kv_heads)
+        self.plan = ops.row_groups(self.group, self.rows, tile, out=self.plan)
+        self.by_groups = True
+
+    def ungroup(self) -> None:
+        self.groups, self.prefixes, self.by_groups = [], [], False
+
+    def leave(self, rows: List[int]) -> None:
+        """Rows that are given back leave their groups (their pages are what ``shrink`` takes; the others' table rows stay)."""
+        if any(r in g for g in self.groups for r in rows):
+            self.groups = [[r for r in g if r not in rows] for g in self.groups]
+            if self.by_groups:
+                self._regroup()
+
+    def shared_workspace(self, H: int, G: int, D: int) -> torch.Tensor:
+        need = ops.paged_attn_shared_workspace_bytes(self.rows, H, G, D, self.rows)
+        t = self._scratch.get("shared")
+        if t is None or t.numel() < need:
+            t = self._scratch["shared"] = torch.empty((need,), dtype=torch.uint8, device=self.device)
+        return t
 
     def cut(self, keep: int, first: int, recent: int) -> None:
         """Every row of more than ``keep`` tokens keeps its ``first`` first and ``recent`` newest ones and the most attended ones between (per
@@ -170,7 +267,8 @@ class PagedLayer(RowState):
         book.layers.append(self)
 
     def buffers(self) -> tuple:
-        return (self.kpages, self.vpages, self.mass, self.book.table)
+        b = self.book
+        return (self.kpages, self.vpages, self.mass, b.table, b.group if b.by_groups else None)
 
     @property
     def capacity(self) -> int:
@@ -187,6 +285,7 @@ class PagedLayer(RowState):
         super().reset(None)
         self.book.positions.zero_()
         self.book.shrink([0] * self.batch_size)
+        self.book.ungroup()
         self.book.revive()
 
     def release_rows_host(self, rows: List[int]):
@@ -196,6 +295,7 @@ class PagedLayer(RowState):
         for r in rows:
             self.book.evicted[r] = 0
         self.book.release(rows)
+        self.book.leave(rows)
         self.book.shrink(self._offsets)
 
     def advance_host(self, L: int):
@@ -237,6 +337,10 @@ class PagedLayer(RowState):
         ops.paged_append(qkv, q, self.kpages, self.vpages, book.table, row, slot, pos, heads, rates=rates, q_norm_w=q_norm, k_norm_w=k_norm, eps=eps,
                          mass=self.mass)
         observed = min(L, max(0, book.observe - book.behind))
+        if L == 1 and book.by_groups:
+            ops.paged_attn_shared(q, self.kpages, self.vpages, book.table, row, slot, out, scale, book.group, book.prefix, book.plan,
+                                  workspace=book.shared_workspace(heads, G, D), out_perm=out_perm)
+            return
         if L == 1:
             ops.paged_attn(q, self.kpages, self.vpages, book.table, row, slot, out, scale, first=book.first, window=book.window,
                            mass=self.mass if observed or not book.behind else None, workspace=book.workspace(B, heads, G, D, book.weighed),

@@ -26,7 +26,7 @@ import threading
 import time
 from collections import OrderedDict
 from pathlib import Path
-from typing import Any, Callable, Dict, Generator, List, Optional, Tuple, Union
+from typing import Any, Callable, Dict, Generator, List, NamedTuple, Optional, Tuple, Union
 
 import numpy as np
 import torch
@@ -221,7 +221,9 @@ class _DecodeStep:
         self._sig = None
 
     def _signature(self):
-        return tuple(tuple(0 if t is None else t.data_ptr() for t in c.buffers()) + (c._lengths.data_ptr(),) for c in self.cache)
+        first = self.cache[0]
+        adapters = 0 if first.adapter_rows is None else first.adapter_index.data_ptr()
+        return (adapters,) + tuple(tuple(0 if t is None else t.data_ptr() for t in c.buffers()) + (c._lengths.data_ptr(),) for c in self.cache)
 
     def set_rows(self, rows: List[int]):
         """Ragged models only: entry i of the next steps continues cache row rows[i] (a batch whose shorter requests have
@@ -326,6 +328,8 @@ def generate_step(
     logit_bias: Optional[Dict[int, float]] = None,
     cache: Optional[List[BatchedKVCache]] = None,
     prompt_lengths: Optional[List[int]] = None,
+    logprobs: Optional[int] = None,
+    adapters: Optional[List[int]] = None,
 ) -> Generator[Tuple[torch.Tensor, torch.Tensor], None, None]:
     """Generator yielding (tokens [B,1] int64, probs [B,1] float32) forever (utils.py:315-427).
 
@@ -335,7 +339,9 @@ def generate_step(
     pages that has no room for that step says so (PagesExhausted) when token n+1 is asked for: prompt + n places give n + 1 tokens.
     ``probs`` is per row (the reference gathers row 0 only).  ``prompt_lengths`` (models with ``supports_ragged``
     only): row b's last prompt_lengths[b] ids are its prompt, the ids before them are left padding and are not fed at all, so a
-    row's tokens do not depend on the other rows of the batch."""
+    row's tokens do not depend on the other rows of the batch.
+    ``logprobs`` = k (0 and up): yields (tokens, probs, ops.TokenLogprobs) with the log probability of every row's token under the model (at temperature 1,
+    after ``logit_bias``), the entropy and the k most likely tokens.  ``adapters``: every row's of model.apply_loras, -1 for none."""
     if repetition_penalty:
         raise NotImplementedError("repetition_penalty not supported.")
     dev = model.device
@@ -349,6 +355,12 @@ def generate_step(
         cache = _kv_pool.get_for(model, B)                                                           # utils.py:390-394
     elif cache and cache[0]._lengths is None:
         bind_cache_group(cache, dev)
+    if logprobs is not None and getattr(model, "tp_world", 1) > 1:
+        raise NotImplementedError("logprobs needs the whole vocabulary on one rank")
+    if adapters is not None:
+        if not hasattr(model, "bind_adapters"):
+            raise NotImplementedError("this model family takes no adapters")
+        model.bind_adapters(cache, adapters)
     greedy = temp == 0
     bias_idx = bias_val = None
     if logit_bias:
@@ -386,6 +398,11 @@ def generate_step(
         if isinstance(cache[0], PagedLayer) and ops.paged_fault_count(reset=True):
             raise RuntimeError("a paged cache's table named pages that do not exist; results of this generation are invalid")
 
+    def said(logits: Optional[torch.Tensor] = None) -> tuple:
+        """What is yielded for the tokens just sampled (from the step's logits, or those given)."""
+        y, p = step.tok.to(torch.int64).view(B, 1), step.probs.clone().view(B, 1)
+        return (y, p) if logprobs is None else (y, p, ops.token_logprobs(step.logits if logits is None else logits, step.tok, top=logprobs))
+
     # prefill (eager, chunked) + first sample
     if prompt_lengths is not None:
         logits = model(y, cache=cache, last_only=True, prompt_lengths=prompt_lengths)[:, -1, :]
@@ -393,8 +410,7 @@ def generate_step(
         logits = model(y, cache=cache, last_only=True)[:, -1, :]
     sample(logits)
     check_exchange()
-    out_y = step.tok.to(torch.int64).view(B, 1)
-    out_p = step.probs.clone().view(B, 1)
+    out = said(logits)
     n_steps = 0
     while True:
         n_steps += 1
@@ -403,14 +419,13 @@ def generate_step(
         try:
             step.run()                               # launches step n+1 (utils.py:422-423)
         except PagesExhausted:                       # no room for the token that is handed out now: the one behind it is the caller's to miss
-            yield out_y, out_p
+            yield out
             raise
         if not step.greedy:
             sample(step.logits)
-        next_y = step.tok.to(torch.int64).view(B, 1)
-        next_p = step.probs.clone().view(B, 1)
-        yield out_y, out_p
-        out_y, out_p = next_y, next_p
+        following = said()
+        yield out
+        out = following
 
 
 # --------------------------------------------------------------------------------- text front-ends
@@ -434,7 +449,7 @@ def stream_generate(model, tokenizer, prompt: str, max_tokens: int = 100, **kwar
     detokenizer = tokenizer.detokenizer
     detokenizer.reset()
     kwargs = _presize(kwargs, model, prompt_tokens, max_tokens)
-    for (token, prob), n in _first_tokens(generate_step(prompt_tokens, model, **kwargs), max_tokens):
+    for (token, prob, *_), n in _first_tokens(generate_step(prompt_tokens, model, **kwargs), max_tokens):
         token_item = token.item()
         if token_item == tokenizer.eos_token_id:
             break
@@ -459,7 +474,7 @@ def generate(model, tokenizer, prompt: str, max_tokens: int = 100, verbose: bool
     n = -1
     prompt_time = 0.0
     kwargs = _presize(kwargs, model, prompt_tokens, max_tokens)
-    for (token, prob), n in _first_tokens(generate_step(prompt_tokens, model, **kwargs), max_tokens):
+    for (token, prob, *_), n in _first_tokens(generate_step(prompt_tokens, model, **kwargs), max_tokens):
         if n == 0:
             prompt_time = time.perf_counter() - tic
             tic = time.perf_counter()
@@ -511,7 +526,7 @@ def batch_generate(model, tokenizer, prompts: List[str], max_tokens: int = 100, 
     output_toks = []
     prompt_time = 0.0
     kwargs = _presize(kwargs, model, prompts_toks, max_tokens)
-    for (tokens, _), n in _first_tokens(generate_step(prompts_toks, model, **kwargs), max_tokens):
+    for (tokens, *_), n in _first_tokens(generate_step(prompts_toks, model, **kwargs), max_tokens):
         if n == 0:
             tokens[0, 0].item()                      # first token materialised = prefill done
             prompt_time = time.perf_counter() - tic
@@ -544,7 +559,7 @@ def batch_stream_generate_text(model, tokenizer, prompts_tokens, max_tokens: int
     counts = [0] * batch_size
     eos_token_id = tokenizer.eos_token_id
     gs_kwargs = _presize({k: v for k, v in kwargs.items() if k != "repetition_penalty"}, model, prompts_tokens, max_tokens)
-    for (batch_next, _), _ in _first_tokens(generate_step(prompts_tokens, model, **gs_kwargs), max_tokens):
+    for (batch_next, *_), _ in _first_tokens(generate_step(prompts_tokens, model, **gs_kwargs), max_tokens):
         ids = batch_next.view(-1).tolist()           # ONE D2H per step (the reference does B .item() syncs)
         deltas: List[Tuple[Optional[str], Optional[str]]] = [(None, None)] * batch_size
         any_active = False
@@ -642,7 +657,7 @@ async def batch_generate_text(model, tokenizer, prompts: List[str], max_tokens: 
         generated = [[] for _ in range(B)]
         active = [True] * B
         counts = [0] * B
-        for step_num, (nxt, _) in enumerate(generate_step(suffix_batch, model, cache=caches, temp=temp, top_p=top_p)):
+        for step_num, (nxt, *_) in enumerate(generate_step(suffix_batch, model, cache=caches, temp=temp, top_p=top_p)):
             if step_num >= max_tokens:
                 break
             ids = nxt.view(-1).tolist()
@@ -664,6 +679,83 @@ async def batch_generate_text(model, tokenizer, prompts: List[str], max_tokens: 
 
 
 batch_generate_text_util = batch_generate_text
+
+
+class Choice(NamedTuple):
+    """One of generate_choices' answers."""
+    text: str
+    tokens: List[int]
+    logprobs: Optional[List[float]]                  # of its tokens (None: not asked for)
+    top_logprobs: Optional[List[Dict[int, float]]]   # per token the most likely ones
+    finish_reason: str                               # "stop" or "length"
+
+
+def generate_choices(model, tokenizer, prompt: str, n: int = 1, max_tokens: int = 100, temp: float = 0.7, top_p: float = 1.0,
+                     logprobs: Optional[int] = None, adapters: Optional[List[int]] = None, page: int = 64) -> List[Choice]:
+    """``n`` answers to one prompt (the server's ``n`` choices, which the reference answers from n copies of the prompt): the prompt is read once per adapter
+    and its pages are shared (model.share_prompt).  ``logprobs`` = k: every token's log probability and the k most likely ones; ``adapters``: every
+    answer's of model.apply_loras (-1: none)."""
+    if n < 1 or max_tokens < 0:
+        raise ValueError(f"{n} answers of {max_tokens} tokens")
+    if adapters is not None and len(adapters) != n:
+        raise ValueError(f"{len(adapters)} adapters for {n} answers")
+    if not hasattr(model, "make_paged_cache"):
+        raise NotImplementedError("choices need a model with a cache in pages")
+    if not isinstance(tokenizer, TokenizerWrapper):
+        tokenizer = TokenizerWrapper(tokenizer)
+    ids = list(tokenizer.encode(prompt))
+    if not ids:
+        raise ValueError("an empty prompt")
+    eos = tokenizer.eos_token_id
+    eos = eos if isinstance(eos, (set, frozenset, list, tuple)) else {eos}
+    by_adapter: Dict[int, List[int]] = {}
+    for r in range(n):
+        by_adapter.setdefault(-1 if adapters is None else int(adapters[r]), []).append(r)
+    groups, head, room = list(by_adapter.values()), len(ids) - 1, len(ids) + max_tokens + 1
+    pages = len(groups) * -(-head // page) + n * (-(-(room - head // page * page) // page))      # the prompts' while they are read, and what each row has by itself
+    cache = model.make_paged_cache(n, room, page=page, pages=pages)
+    if adapters is not None:
+        model.bind_adapters(cache, adapters)
+    if head:
+        model.share_prompt(cache, torch.tensor([ids[:-1]] * len(groups)), groups)
+    run = generate_step(torch.tensor([ids[-1:]] * n), model, temp=temp, top_p=top_p, cache=cache, logprobs=logprobs)
+    tokens, said, tops, open_rows = [[] for _ in range(n)], [[] for _ in range(n)], [[] for _ in range(n)], list(range(n))
+    for (y, _, *more), _ in _first_tokens(run, max_tokens):
+        step = y.view(-1).tolist()
+        lp, alt = (None, None) if logprobs is None else (more[0].logprob.tolist(), list(zip(more[0].top_ids.tolist(), more[0].top_logprobs.tolist())))
+        ended = [r for r in open_rows if step[r] in eos]
+        open_rows = [r for r in open_rows if r not in ended]
+        for r in open_rows:
+            tokens[r].append(step[r])
+            if lp is not None:
+                said[r].append(lp[r])
+                tops[r].append(dict(zip(*alt[r])))
+        if not open_rows:
+            break
+        if ended:
+            model.release_rows(cache, ended)
+    asked = logprobs is not None
+    return [Choice(tokenizer.decode(tokens[r], skip_special_tokens=True), tokens[r], said[r] if asked else None, tops[r] if asked else None,
+                   "length" if r in open_rows else "stop") for r in range(n)]
+
+
+def score_text(model, tokenizer, texts: List[str], top: int = 0) -> List[dict]:
+    """What the server's ``echo`` with log probabilities and its perplexities are made of (server/main.py:458-659): per text its ``tokens``, their
+    ``token_logprobs`` (None for the first), per token the ``top_logprobs`` at its place, and the ``perplexity``."""
+    if not isinstance(tokenizer, TokenizerWrapper):
+        tokenizer = TokenizerWrapper(tokenizer)
+    out = []
+    for text in texts:
+        ids = list(tokenizer.encode(text))
+        if not ids:
+            out.append(dict(tokens=[], token_logprobs=[], top_logprobs=[], perplexity=float("nan")))
+            continue
+        s = model.score(torch.tensor([ids]), top=top)
+        lp = s.logprob[0, :-1].tolist()
+        tops = [dict(zip(i, v)) for i, v in zip(s.top_ids[0, :-1].tolist(), s.top_logprobs[0, :-1].tolist())]
+        out.append(dict(tokens=ids, token_logprobs=[None] + lp, top_logprobs=[None] + tops,
+                        perplexity=float(np.exp(-np.mean(lp))) if lp else float("nan")))
+    return out
 
 
 # --------------------------------------------------------------------------------- loading

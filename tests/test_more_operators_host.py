@@ -85,3 +85,48 @@ def test_paged_attn_shared_refuses_before_it_launches():
         assert call(**bad) == -1, bad
     for bad in (dict(q=264), dict(out=264), dict(k=264), dict(plan=264)):
         assert call(**bad) == -2, bad
+
+
+def test_pages_of_rows_that_share_a_prompt():
+    """Counting of shared pages, on the CPU: whole pages belong to all rows of a group, the last one's tokens are copied, the last row gives pages back."""
+    from mlx_parallm_b200.models.paged import PageBook, PagedLayer, PagesExhausted
+    book = PageBook(5, 64, "cpu", page=16, pages=12)
+    layer = PagedLayer(book, 4, 2, 8)
+    layer.kpages, layer.vpages = torch.randn((12, 2, 16, 8)), torch.randn((12, 2, 16, 8))
+
+    def read(n, tokens):
+        side = PageBook(n, tokens, "cpu", page=16, pages=12, of=book)
+        PagedLayer(side, 4, 2, 8)
+        side.room_for([tokens] * n)
+        return side
+
+    side = read(1, 40)
+    assert len(book.free) == 9 and side.free is book.free
+    held = list(side.owned[0])
+    book.adopt(side, [[0, 2, 3]], 40)
+    side.shrink([0])
+    assert layer._offsets == [40, 0, 40, 40, 0] and book.lengths.tolist() == [40, 0, 40, 40, 0]
+    assert [o[:2] for o in (book.owned[0], book.owned[2], book.owned[3])] == [held[:2]] * 3 and book.owned[0][2] == held[2]
+    assert len({o[2] for o in (book.owned[0], book.owned[2], book.owned[3])}) == 3 and len(book.free) == 7
+    for r in (2, 3):
+        assert book.table[r].tolist() == book.owned[r] + [-1]
+        assert torch.equal(layer.kpages[book.owned[r][2]], layer.kpages[held[2]]) and torch.equal(layer.vpages[book.owned[r][2]], layer.vpages[held[2]])
+    assert book.held == {p: 3 for p in held[:2]} and book.groups == [[0, 2, 3]] and book.prefixes == [32] and not book.by_groups
+    side = read(1, 32)                                              # no rest: nothing is copied
+    book.adopt(side, [[1, 4]], 32)
+    assert book.owned[1] == book.owned[4] and len(book.free) == 5
+    layer.release_rows_host([2])
+    assert book.groups[0] == [0, 3] and len(book.free) == 6 and book.held[held[0]] == 2
+    book.room_for([50, 0, 0, 0, 0])
+    assert len(book.free) == 5
+    layer.release_rows_host([0])
+    assert book.held.keys() == set(book.owned[1]) and len(book.free) == 7
+    layer.release_rows_host([3])
+    assert len(book.free) == 10
+    layer.reset()
+    assert sorted(book.free) == list(range(12)) and not book.held and book.groups == [] and (book.table == -1).all()
+    side = read(2, 40)                                              # 6 pages; 7 rows more want 5 for their rests, and 6 are free
+    book.free[:] = book.free[:2]
+    with pytest.raises(PagesExhausted):
+        book.adopt(side, [[0, 1, 2], [3, 4]], 40)
+    assert all(not o for o in book.owned) and book.groups == [] and len(book.free) == 2
