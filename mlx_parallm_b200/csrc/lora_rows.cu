@@ -102,12 +102,18 @@ struct LoraRows {
 
 // (two bf16 numbers where y is rounded to bf16: 16 bits of z against y's 8)
 template <typename T, typename YT> struct LwParts { static constexpr int N = std::is_same<T, __nv_bfloat16>::value && sizeof(YT) == 4 ? 3 : 2; };
-// Shared floats of a row: the warps' parts of z, of which the first becomes this CTA's, and the split z, which has room behind it (16 rows) or takes the
-// parts' place when the whole cluster has read them (64 rows: two CTAs fit an SM).
-template <typename T, typename YT, int MB>
+// Shared floats of a row: the warps' parts of z, of which the first becomes this CTA's, and the split z behind that.
+template <typename T, typename YT>
 __host__ __device__ constexpr int lw_row_floats(int ranks) {
-  const int split = LwParts<T, YT>::N * (ranks + 8) / 2 + (MB == 1 ? ranks : 0);
+  const int split = LwParts<T, YT>::N * (ranks + 8) / 2 + ranks;
   return split > LW_WARPS * 32 ? split : LW_WARPS * 32;
+}
+
+// up = 2^e, down = 2^-e with top * down in [1, 2); 1 for a row of zeros or one that is not finite
+__device__ __forceinline__ void lw_scale(float top, float& up, float& down) {
+  const uint32_t e = __float_as_uint(top) >> 23;
+  const bool plain = e < 1 || e > 252;
+  down = plain ? 1.f : __uint_as_float((254u - e) << 23), up = plain ? 1.f : __uint_as_float(e << 23);
 }
 
 __device__ __forceinline__ void red_add4(float* p, float a, float b, float c, float d) {
@@ -138,12 +144,12 @@ __device__ __forceinline__ void lw_load(const LoraRows& p, const T* b, int run, 
       w[k][h] = n0 + 2 * h < r.width && 16 * k < p.R ? *reinterpret_cast<const uint2*>(at + 2 * h * p.R + 16 * k) : make_uint2(0, 0);
 }
 
-// MB blocks of 16 rows; YT: y's type; KS: 16 ranks each (R or more).  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits
+// Tiles of 16 rows: decode batches.  YT: y's type; KS: 16 ranks each (R or more).  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits
 // this CTA's part of K.  Operands come straight from memory, 16 bytes a lane: the order of k within a product is free as long as both operands have the same.
-template <typename T, typename YT, int MB, int KS>
+template <typename T, typename YT, int KS>
 __global__ void __launch_bounds__(LW_THREADS, 2)
 lora_rows_kernel(const __grid_constant__ LoraRows p) {
-  constexpr int ROWS = 16 * MB, PARTS = LwParts<T, YT>::N, NZ = (16 * KS + 31) / 32;
+  constexpr int MB = 1, ROWS = 16, PARTS = LwParts<T, YT>::N, NZ = (16 * KS + 31) / 32;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int s_row[ROWS];
   __shared__ float s_factor[ROWS][LW_TARGETS];
@@ -152,7 +158,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int TR = p.targets * p.R, wn = TR > 128 ? 8 : TR > 64 ? 4 : TR > 32 ? 2 : 1, wk = LW_WARPS / wn, ranks = wn * 32, ld = ranks + 8;
   float* s_part = reinterpret_cast<float*>(smem);                 // [wk][ROWS][ranks]
-  T* s_split = reinterpret_cast<T*>(s_part + (MB == 1 ? ROWS * ranks : 0));      // [PARTS][ROWS][ld]
+  T* s_split = reinterpret_cast<T*>(s_part + ROWS * ranks);      // [PARTS][ROWS][ld]
   pdl_wait();
   const int tile_index = blockIdx.x / C, tiles = p.plan.tiles();
   const int4 tile = p.plan.tile(tile_index);                      // (the plan has room for every tile of the grid)
@@ -186,7 +192,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
     }
     const int s0 = (int)((int64_t)p.steps * rank / C), s1 = (int)((int64_t)p.steps * (rank + 1) / C);
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    constexpr int DEEP = MB == 1 ? 4 : 1;                         // steps whose loads are under way together
+    constexpr int DEEP = 4;                         // steps whose loads are under way together
 #pragma unroll 1
     for (int s = s0 + my_k; s < s1; s += DEEP * wk) {
       uint4 av[DEEP][4], xv[DEEP][MB][2];
@@ -215,7 +221,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
         }
     }
   }
-  constexpr int AHEAD = MB == 1 ? 8 / KS : 1;                      // runs whose b is under way
+  constexpr int AHEAD = 8 / KS;                      // runs whose b is under way
   uint2 w[AHEAD][KS][2];
 #pragma unroll
   for (int u = 0; u < AHEAD; ++u) lw_load<T, KS>(p, b, run0 + warp + u * LW_WARPS, run1, w[u]);
@@ -260,10 +266,8 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
 #pragma unroll
     for (int k = 0; k < NZ; ++k) top = fmaxf(top, fabsf(z[k]));
     top = warp_max(top);
-    // 2^e with top 2^-e in [1, 2); 1 for a row of zeros or one that is not finite
-    const uint32_t e = __float_as_uint(top) >> 23;
-    const bool plain = e < 1 || e > 252;
-    const float down = plain ? 1.f : __uint_as_float((254u - e) << 23), up = plain ? 1.f : __uint_as_float(e << 23);
+    float up, down;
+    lw_scale(top, up, down);
     if (lane == 0) s_factor[row][target] = up * p.scales[tile.x];
 #pragma unroll
     for (int k = 0; k < NZ; ++k) {
@@ -277,36 +281,13 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
       }
     }
   };
-  if constexpr (MB == 1) {
-    for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
-      float z[NZ];
-      whole(i, z);
-      split(i, z);
-    }
-    if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    __syncthreads();
-  } else {
-    // (a sum that is needed again takes the first part's place in this CTA when the others have read it)
-    float* s_z = s_part + lw_row_floats<T, YT, MB>(ranks) * ROWS;
-    for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
-      float z[NZ];
-      whole(i, z);
-      const int row = i / p.targets, at = row * ranks + (i - row * p.targets) * p.R;
-#pragma unroll
-      for (int k = 0; k < NZ; ++k)
-        if (32 * k + lane < p.R) s_z[at + 32 * k + lane] = z[k];
-    }
-    if (C > 1) cluster.sync();                                    // all have read: what lies there may go
-    else __syncthreads();
-    for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
-      float z[NZ];
-      const int row = i / p.targets, at = row * ranks + (i - row * p.targets) * p.R;
-#pragma unroll
-      for (int k = 0; k < NZ; ++k) z[k] = 32 * k + lane < p.R ? s_z[at + 32 * k + lane] : 0.f;
-      split(i, z);
-    }
-    __syncthreads();
+  for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
+    float z[NZ];
+    whole(i, z);
+    split(i, z);
   }
+  if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  __syncthreads();
   pdl_launch_dependents();
 
   // ---- this CTA's columns: 16 at a time, of which a lane has four neighbours -----------------------------------------------------
@@ -367,27 +348,304 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
         }
     }
   }
-  if (MB == 1 && C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // nobody leaves before all have read
+  if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // nobody leaves before all have read
 }
 
-template <typename T, typename YT, int MB, int KS>
-static int launch_lora_rows_of(const LoraRows& p, int64_t tiles, cudaStream_t st) {
-  auto kern = lora_rows_kernel<T, YT, MB, KS>;
-  static std::atomic<uint64_t> ready{0};                          // devices whose copy of the kernel has its shared memory
+// Tiles of 64 rows: prompts.  The same steps as products of tiles in shared memory, which copies fill three stages ahead: z = x A^T in steps of 64 of K,
+// then blocks of 64 columns, for which b and the old y come along, y grows in its place in shared memory and leaves by whole lines.
+// RK: ranks of all targets, filled up to 32, 64, 128 or 256.  (As the kernel of 16 rows, with operands straight from memory, 8000 rows of rank 64 took 222 us: a
+// round trip per 32 of K and per 16 columns.)
+constexpr int LP_ROWS = 64, LP_STAGES = 3, LP_COLS = 64;
+template <typename T, typename YT, int RK>
+struct LpShape {
+  static constexpr int MT = RK >= 128 ? 2 : 1, NT = RK == 256 ? 8 : 4, KG = RK == 32 ? 2 : 1;      // a warp's 16-row and 8-rank blocks; warps that share them
+  static constexpr int WM = LP_ROWS / 16 / MT, WN = RK / 8 / NT;
+  static constexpr int PARTS = LwParts<T, YT>::N, LD = RK + 8;
+  static constexpr int STAGE_A = (LP_ROWS + RK) * 128, Z_BYTES = LP_ROWS * RK * 4, SPLIT_BYTES = PARTS * LP_ROWS * LD * 2;
+  static constexpr int Y_PITCH = LP_COLS * (int)sizeof(YT) + 16;
+  static __host__ __device__ constexpr int b_pitch(int R) { return 2 * R + 16; }      // an odd number of 16 bytes: no conflicts
+  static __host__ __device__ constexpr int stage_c(int R) { return LP_COLS * b_pitch(R) + LP_ROWS * Y_PITCH; }
+  static __host__ __device__ constexpr int front(int R) {
+    const int a = LP_STAGES * STAGE_A, c = LP_STAGES * stage_c(R);
+    return a > c ? a > Z_BYTES ? a : Z_BYTES : c > Z_BYTES ? c : Z_BYTES;
+  }
+  static __host__ __device__ constexpr int bytes(int R) { return front(R) + SPLIT_BYTES; }
+  static_assert(WM * WN * KG == LW_WARPS, "eight warps");
+};
+
+template <int N>
+__device__ __forceinline__ void lp_copy(uint32_t dst, const void* src, bool valid) {      // 8 or 16 bytes, zeros where there is nothing
+  const int size = valid ? N : 0;
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
+}
+
+template <typename T, typename YT, int RK>
+__global__ void __launch_bounds__(LW_THREADS, RK == 256 ? 1 : 2)
+lora_prompt_kernel(const __grid_constant__ LoraRows p) {
+  using S = LpShape<T, YT, RK>;
+  constexpr int MT = S::MT, NT = S::NT, PARTS = S::PARTS, LD = S::LD, KSTEPS = 4;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_row[LP_ROWS];
+  __shared__ float s_factor[LP_ROWS][LW_TARGETS];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), C = (int)cluster.num_blocks();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mat = lane >> 3, r8 = lane & 7;
+  const int TR = p.targets * p.R;
+  const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(smem);
+  float* s_z = reinterpret_cast<float*>(smem);                    // [64][RK], over the stages
+  T* s_split = reinterpret_cast<T*>(smem + S::front(p.R));        // [PARTS][64][LD]
+  pdl_wait();
+  const int tile_index = blockIdx.x / C, tiles = p.plan.tiles();
+  const int4 tile = p.plan.tile(tile_index);                      // (the plan has room for every tile of the grid)
+  if (tile_index >= tiles) return;                                // (the whole cluster)
+  if ((int)threadIdx.x < LP_ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
+  __syncthreads();
+
+  // ---- this CTA's part of z ---------------------------------------------------------------------------------------------------
+  {
+    const int steps = (int)((p.K + 63) / 64), k0 = (int)((int64_t)steps * rank / C), k1 = (int)((int64_t)steps * (rank + 1) / C);
+    const int c = threadIdx.x & 7, line = threadIdx.x >> 3;       // this thread's 16 bytes of a line of 64, and its first line
+    const T* xr[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = s_row[line + 32 * i];
+      xr[i] = row < 0 ? nullptr : reinterpret_cast<const T*>(p.x) + (int64_t)row * p.ldx + 8 * c;
+    }
+    const T* ar = reinterpret_cast<const T*>(p.a) + ((int64_t)tile.x * TR + line) * p.K + 8 * c;
+    auto issue = [&](int s) {
+      if (s < k1) {
+        const uint32_t at = s0 + (uint32_t)(s % LP_STAGES) * S::STAGE_A + ((c ^ (line & 7)) << 4);
+        const bool in = s * 64 + 8 * c < p.K;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bool ok = in && xr[i];
+          lp_copy<16>(at + (line + 32 * i) * 128, ok ? xr[i] + s * 64 : reinterpret_cast<const T*>(p.x), ok);
+        }
+#pragma unroll
+        for (int i = 0; i < RK / 32; ++i) {
+          const bool ok = in && line + 32 * i < TR;
+          lp_copy<16>(at + (LP_ROWS + line + 32 * i) * 128, ok ? ar + (int64_t)32 * i * p.K + s * 64 : reinterpret_cast<const T*>(p.a), ok);
+        }
+      }
+      cp_async_commit();
+    };
+    float acc[MT][NT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+    const int kg = warp / (S::WM * S::WN), wm = warp % S::WM, wn = warp / S::WM % S::WN;
+    for (int s = 0; s < LP_STAGES - 1; ++s) issue(k0 + s);
+#pragma unroll 1
+    for (int s = k0; s < k1; ++s) {
+      cp_async_wait<LP_STAGES - 2>();
+      __syncthreads();
+      issue(s + LP_STAGES - 1);
+      const uint32_t xs = s0 + (uint32_t)(s % LP_STAGES) * S::STAGE_A, as = xs + LP_ROWS * 128;
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k) {
+        if (S::KG == 2 && (k & 1) != kg) continue;
+        uint32_t xf[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int row = 16 * (wm * MT + i) + r8 + 8 * (mat & 1);
+          ldsm_x4(xs + row * 128 + (((2 * k + (mat >> 1)) ^ (row & 7)) << 4), xf[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < NT / 2; ++j) {
+          const int n = 8 * NT * wn + 16 * j + r8 + 8 * (mat >> 1);
+          uint32_t af[4];
+          ldsm_x4(as + n * 128 + (((2 * k + (mat & 1)) ^ (n & 7)) << 4), af);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            mma16816<T>(acc[i][2 * j], xf[i], af[0], af[1]);
+            mma16816<T>(acc[i][2 * j + 1], xf[i], af[2], af[3]);
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+#pragma unroll
+    for (int half = 0; half < S::KG; ++half) {
+      if (kg == half) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float2* z = reinterpret_cast<float2*>(s_z + (16 * (wm * MT + i) + 8 * h + g) * RK + 8 * NT * wn + 8 * j + 2 * t);
+              float2 v = make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
+              if (half) {
+                const float2 u = *z;
+                v.x += u.x, v.y += u.y;
+              }
+              *z = v;
+            }
+      }
+      __syncthreads();
+    }
+  }
+  if (C > 1) cluster.sync();
+
+  // ---- z of all CTAs, as 16-bit numbers: a warp per row and target ---------------------------------------------------------------
+  for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
+    const int row = i / p.targets, target = i - row * p.targets, at = row * RK + target * p.R;
+    float z[2] = {0.f, 0.f}, v[2][LW_CLUSTER];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < LW_CLUSTER; ++r) v[k][r] = r < C && 32 * k + lane < p.R ? cluster.map_shared_rank(s_z, r)[at + 32 * k + lane] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < LW_CLUSTER; ++r) z[k] += v[k][r];       // in one order everywhere
+    const float top = warp_max(fmaxf(fabsf(z[0]), fabsf(z[1])));
+    float up, down;
+    lw_scale(top, up, down);
+    if (lane == 0) s_factor[row][target] = up * p.scales[tile.x];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (32 * k + lane >= p.R) continue;
+      float x = z[k] * down;
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
+        const T h = Tr<T>::from_f(x);
+        s_split[(part * LP_ROWS + row) * LD + target * p.R + 32 * k + lane] = h;
+        x -= Tr<T>::to_f(h);
+      }
+    }
+  }
+  if (C > 1) cluster.sync();                                      // all have read: the stages may lie there again
+  else __syncthreads();
+  pdl_launch_dependents();
+
+  // ---- this CTA's columns -------------------------------------------------------------------------------------------------------
+  const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.x * p.N * p.R;
+  int blocks = 0;
+  for (int k = 0; k < p.targets; ++k) blocks += (p.start[k + 1] - p.start[k] + LP_COLS - 1) / LP_COLS;
+  const int b0 = (int)((int64_t)blocks * rank / C), b1 = (int)((int64_t)blocks * (rank + 1) / C);
+  auto place = [&](int block, int& target, int& col) {            // a block's target and first column in it
+    target = 0;
+    for (;;) {
+      const int n = (p.start[target + 1] - p.start[target] + LP_COLS - 1) / LP_COLS;
+      if (block < n) break;
+      block -= n;
+      ++target;
+    }
+    col = block * LP_COLS;
+  };
+  const int pitch = S::b_pitch(p.R), per = p.R / 8;               // 16-byte pieces of a line of b
+  const uint32_t stage_bytes = (uint32_t)S::stage_c(p.R);
+  auto issue = [&](int block) {
+    if (block < b1) {
+      int target, col;
+      place(block, target, col);
+      const int width = p.start[target + 1] - p.start[target];
+      const uint32_t bs = s0 + (uint32_t)(block % LP_STAGES) * stage_bytes, ys = bs + LP_COLS * pitch;
+      for (int x = threadIdx.x; x < LP_COLS * per; x += LW_THREADS) {
+        const int n = x / per, c = x - n * per;
+        const bool ok = col + n < width;
+        lp_copy<16>(bs + n * pitch + c * 16, b + (ok ? (int64_t)(p.start[target] + col + n) * p.R + 8 * c : 0), ok);
+      }
+#pragma unroll
+      for (int k = 0; k < LP_ROWS * 16 / LW_THREADS; ++k) {       // four columns each
+        const int row = (threadIdx.x >> 4) + k * (LW_THREADS / 16), c = 4 * (threadIdx.x & 15);
+        const bool ok = s_row[row] >= 0 && col + c < width;
+        const YT* y = reinterpret_cast<const YT*>(p.y) + (ok ? (int64_t)s_row[row] * p.ldy + p.col0[target] + col + c : 0);
+        lp_copy<4 * sizeof(YT)>(ys + row * S::Y_PITCH + c * (int)sizeof(YT), y, ok);
+      }
+    }
+    cp_async_commit();
+  };
+  for (int s = 0; s < LP_STAGES - 1; ++s) issue(b0 + s);
+  const int wm = warp & 3, wn = warp >> 2;                        // 16 rows, 32 columns
+  uint32_t zf[PARTS][KSTEPS][4];
+  float f0 = 0.f, f1 = 0.f;
+  int held = -1;
+#pragma unroll 1
+  for (int block = b0; block < b1; ++block) {
+    int target, col;
+    place(block, target, col);
+    if (target != held) {                                         // the rows' z of this target stays in registers
+      held = target;
+      f0 = s_factor[16 * wm + g][target], f1 = s_factor[16 * wm + 8 + g][target];
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k)
+          if (16 * k < p.R)
+            ldsm_x4((uint32_t)__cvta_generic_to_shared(s_split) +
+                        ((part * LP_ROWS + 16 * wm + r8 + 8 * (mat & 1)) * LD + target * p.R + 16 * k + 8 * (mat >> 1)) * 2,
+                    zf[part][k]);
+    }
+    cp_async_wait<LP_STAGES - 2>();
+    __syncthreads();
+    issue(block + LP_STAGES - 1);
+    const uint32_t bs = s0 + (uint32_t)(block % LP_STAGES) * stage_bytes;
+    uint8_t* ys = smem + (size_t)(block % LP_STAGES) * stage_bytes + LP_COLS * pitch;
+    float d[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KSTEPS; ++k) {
+      if (16 * k >= p.R) break;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t bf[4];
+        ldsm_x4(bs + (32 * wn + 16 * j + r8 + 8 * (mat >> 1)) * pitch + (2 * k + (mat & 1)) * 16, bf);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          mma16816<T>(d[2 * j], zf[part][k], bf[0], bf[1]);
+          mma16816<T>(d[2 * j + 1], zf[part][k], bf[2], bf[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        YT* y = reinterpret_cast<YT*>(ys + (16 * wm + 8 * h + g) * S::Y_PITCH) + 32 * wn + 8 * j + 2 * t;
+        const float f = h ? f1 : f0;
+        if constexpr (sizeof(YT) == 4) {
+          float2 v = *reinterpret_cast<float2*>(y);
+          v.x = fmaf(f, d[j][2 * h], v.x), v.y = fmaf(f, d[j][2 * h + 1], v.y);
+          *reinterpret_cast<float2*>(y) = v;
+        } else {
+          *reinterpret_cast<uint32_t*>(y) = pack2<YT>(fmaf(f, d[j][2 * h], Tr<YT>::to_f(y[0])), fmaf(f, d[j][2 * h + 1], Tr<YT>::to_f(y[1])));
+        }
+      }
+    __syncthreads();
+    const int width = p.start[target + 1] - p.start[target];
+#pragma unroll
+    for (int k = 0; k < LP_ROWS * 16 / LW_THREADS; ++k) {
+      const int row = (threadIdx.x >> 4) + k * (LW_THREADS / 16), c = 4 * (threadIdx.x & 15);
+      if (s_row[row] < 0 || col + c >= width) continue;
+      YT* y = reinterpret_cast<YT*>(p.y) + (int64_t)s_row[row] * p.ldy + p.col0[target] + col + c;
+      const uint8_t* from = ys + row * S::Y_PITCH + c * (int)sizeof(YT);
+      if constexpr (sizeof(YT) == 4) *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(from);
+      else *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(from);
+    }
+  }
+}
+
+// clusters of C CTAs, as many as fit the GPU at two CTAs per SM
+static int launch_lora(void (*kern)(LoraRows), int most_bytes, int bytes, std::atomic<uint64_t>& ready, const LoraRows& p, int64_t tiles, cudaStream_t st) {
   int dev = 0;
   cudaError_t ae = cudaGetDevice(&dev);
-  if (ae == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
-    ae = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (lw_row_floats<T, YT, MB>(LW_RANKS) + (MB > 1 ? LW_RANKS : 0)) * 16 * MB * 4);
+  if (ae == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {      // ready: devices whose copy of the kernel has its shared memory
+    ae = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_bytes);
     if (ae == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
-  if (ae != cudaSuccess) return cuda_fail(ae, "cudaFuncSetAttribute(lora_rows_kernel)");
-  const int TR = p.targets * p.R, ranks = TR > 128 ? 256 : TR > 64 ? 128 : TR > 32 ? 64 : 32;
+  if (ae != cudaSuccess) return cuda_fail(ae, "cudaFuncSetAttribute(lora kernels)");
   int C = LW_CLUSTER;
   while (C > 1 && tiles * C > 2 * sm_count()) C >>= 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C));
   cfg.blockDim = dim3(LW_THREADS);
-  cfg.dynamicSmemBytes = (size_t)(lw_row_floats<T, YT, MB>(ranks) + (MB > 1 ? ranks : 0)) * 16 * MB * 4;
+  cfg.dynamicSmemBytes = (size_t)bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -398,14 +656,34 @@ static int launch_lora_rows_of(const LoraRows& p, int64_t tiles, cudaStream_t st
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-  return e == cudaSuccess ? B200P_OK : cuda_fail(e, "lora_rows_kernel");
+  return e == cudaSuccess ? B200P_OK : cuda_fail(e, "lora kernels");
 }
 
-template <typename T, typename YT, int MB>
+template <typename T, typename YT, int KS>
 static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
-  if (p.R == 16) return launch_lora_rows_of<T, YT, MB, 1>(p, tiles, st);
-  if (p.R == 32) return launch_lora_rows_of<T, YT, MB, 2>(p, tiles, st);
-  return launch_lora_rows_of<T, YT, MB, 4>(p, tiles, st);
+  static std::atomic<uint64_t> ready{0};
+  const int TR = p.targets * p.R, ranks = TR > 128 ? 256 : TR > 64 ? 128 : TR > 32 ? 64 : 32;
+  return launch_lora(lora_rows_kernel<T, YT, KS>, lw_row_floats<T, YT>(LW_RANKS) * 16 * 4, lw_row_floats<T, YT>(ranks) * 16 * 4, ready, p, tiles, st);
+}
+
+template <typename T, typename YT, int RK>
+static int launch_lora_prompt(const LoraRows& p, int64_t tiles, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
+  return launch_lora(lora_prompt_kernel<T, YT, RK>, LpShape<T, YT, RK>::bytes(LW_RANK), LpShape<T, YT, RK>::bytes(p.R), ready, p, tiles, st);
+}
+
+template <typename T, typename YT>
+static int launch_lora_tiles(const LoraRows& p, int tile, int64_t tiles, cudaStream_t st) {
+  if (tile == 16) {
+    if (p.R == 16) return launch_lora_rows<T, YT, 1>(p, tiles, st);
+    if (p.R == 32) return launch_lora_rows<T, YT, 2>(p, tiles, st);
+    return launch_lora_rows<T, YT, 4>(p, tiles, st);
+  }
+  const int TR = p.targets * p.R;
+  if (TR > 128) return launch_lora_prompt<T, YT, 256>(p, tiles, st);
+  if (TR > 64) return launch_lora_prompt<T, YT, 128>(p, tiles, st);
+  if (TR > 32) return launch_lora_prompt<T, YT, 64>(p, tiles, st);
+  return launch_lora_prompt<T, YT, 32>(p, tiles, st);
 }
 
 }  // namespace b200p
@@ -468,12 +746,6 @@ extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a
   p.K = (int)K, p.R = R, p.N = p.start[targets], p.targets = targets, p.steps = (int)((K + 31) / 32);
   const int64_t tiles = row_group_tiles(M, adapters, tile);
   cudaStream_t st = (cudaStream_t)stream;
-#define LW_GO(T, MB) return y_f32 ? launch_lora_rows<T, float, MB>(p, tiles, st) : launch_lora_rows<T, T, MB>(p, tiles, st)
-  if (dtype == B200P_F16) {
-    if (tile == 16) LW_GO(__half, 1);
-    LW_GO(__half, 4);
-  }
-  if (tile == 16) LW_GO(__nv_bfloat16, 1);
-  LW_GO(__nv_bfloat16, 4);
-#undef LW_GO
+  if (dtype == B200P_F16) return y_f32 ? launch_lora_tiles<__half, float>(p, tile, tiles, st) : launch_lora_tiles<__half, __half>(p, tile, tiles, st);
+  return y_f32 ? launch_lora_tiles<__nv_bfloat16, float>(p, tile, tiles, st) : launch_lora_tiles<__nv_bfloat16, __nv_bfloat16>(p, tile, tiles, st);
 }
