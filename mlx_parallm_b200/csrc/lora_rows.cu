@@ -488,20 +488,32 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
       __syncthreads();
     }
   }
-  if (C > 1) cluster.sync();
-
-  // ---- z of all CTAs, as 16-bit numbers: a warp per row and target ---------------------------------------------------------------
+  // ---- z of all CTAs -----------------------------------------------------------------------------------------------------------
+  if (C > 1) {
+    constexpr int N = LP_ROWS * RK / 4 / LW_THREADS;
+    float4 z[N];
+    cluster.sync();
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < C; ++r) {                                 // in one order everywhere
+      const float4* other = reinterpret_cast<const float4*>(cluster.map_shared_rank(s_z, r));
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float4 v = other[threadIdx.x + k * LW_THREADS];
+        z[k].x += v.x, z[k].y += v.y, z[k].z += v.z, z[k].w += v.w;
+      }
+    }
+    cluster.sync();                                               // all have read
+#pragma unroll
+    for (int k = 0; k < N; ++k) reinterpret_cast<float4*>(s_z)[threadIdx.x + k * LW_THREADS] = z[k];
+    __syncthreads();
+  }
+  // as 16-bit numbers: a warp per row and target
   for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
     const int row = i / p.targets, target = i - row * p.targets, at = row * RK + target * p.R;
-    float z[2] = {0.f, 0.f}, v[2][LW_CLUSTER];
+    float z[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int r = 0; r < LW_CLUSTER; ++r) v[k][r] = r < C && 32 * k + lane < p.R ? cluster.map_shared_rank(s_z, r)[at + 32 * k + lane] : 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int r = 0; r < LW_CLUSTER; ++r) z[k] += v[k][r];       // in one order everywhere
+    for (int k = 0; k < 2; ++k) z[k] = 32 * k + lane < p.R ? s_z[at + 32 * k + lane] : 0.f;
     const float top = warp_max(fmaxf(fabsf(z[0]), fabsf(z[1])));
     float up, down;
     lw_scale(top, up, down);
@@ -518,8 +530,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
       }
     }
   }
-  if (C > 1) cluster.sync();                                      // all have read: the stages may lie there again
-  else __syncthreads();
+  __syncthreads();                                                // (the stages may lie over z again)
   pdl_launch_dependents();
 
   // ---- this CTA's columns -------------------------------------------------------------------------------------------------------
@@ -527,36 +538,52 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   int blocks = 0;
   for (int k = 0; k < p.targets; ++k) blocks += (p.start[k + 1] - p.start[k] + LP_COLS - 1) / LP_COLS;
   const int b0 = (int)((int64_t)blocks * rank / C), b1 = (int)((int64_t)blocks * (rank + 1) / C);
-  auto place = [&](int block, int& target, int& col) {            // a block's target and first column in it
-    target = 0;
-    for (;;) {
-      const int n = (p.start[target + 1] - p.start[target] + LP_COLS - 1) / LP_COLS;
-      if (block < n) break;
-      block -= n;
-      ++target;
-    }
-    col = block * LP_COLS;
+  struct Place {                                                  // of a block: its target and first column in it
+    int target, col, width;
   };
-  const int pitch = S::b_pitch(p.R), per = p.R / 8;               // 16-byte pieces of a line of b
+  auto step = [&](Place& x) {
+    x.col += LP_COLS;
+    if (x.col >= x.width && x.target + 1 < p.targets) ++x.target, x.col = 0, x.width = p.start[x.target + 1] - p.start[x.target];
+  };
+  Place ahead{0, 0, p.start[1]};
+  for (int k = 0; k < b0; ++k) step(ahead);
+  Place here = ahead;
+  const int pitch = S::b_pitch(p.R), per = p.R / 8, pieces = LP_COLS * per;      // 16-byte pieces of a line of b, and of a block: they lie in a row
   const uint32_t stage_bytes = (uint32_t)S::stage_c(p.R);
+  constexpr int BP = LP_COLS * LW_RANK / 8 / LW_THREADS, YP = LP_ROWS * 16 / LW_THREADS;
+  uint32_t b_to[BP];                                              // where this thread's pieces of b go
+#pragma unroll
+  for (int k = 0; k < BP; ++k) {
+    const int x = threadIdx.x + k * LW_THREADS;
+    b_to[k] = (uint32_t)(16 * (x + x / per));
+  }
+  const int c4 = 4 * (threadIdx.x & 15), line = threadIdx.x >> 4;  // its four columns of y, in rows `line`, `line` + 16 and so on
+  YT* y_at[YP];
+#pragma unroll
+  for (int k = 0; k < YP; ++k) {
+    const int row = s_row[line + k * (LW_THREADS / 16)];
+    y_at[k] = row < 0 ? nullptr : reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + c4;
+  }
+  int fill = b0 % LP_STAGES;                                      // the stage of the next block that is fetched
   auto issue = [&](int block) {
     if (block < b1) {
-      int target, col;
-      place(block, target, col);
-      const int width = p.start[target + 1] - p.start[target];
-      const uint32_t bs = s0 + (uint32_t)(block % LP_STAGES) * stage_bytes, ys = bs + LP_COLS * pitch;
-      for (int x = threadIdx.x; x < LP_COLS * per; x += LW_THREADS) {
-        const int n = x / per, c = x - n * per;
-        const bool ok = col + n < width;
-        lp_copy<16>(bs + n * pitch + c * 16, b + (ok ? (int64_t)(p.start[target] + col + n) * p.R + 8 * c : 0), ok);
-      }
+      const uint32_t bs = s0 + (uint32_t)fill * stage_bytes, ys = bs + LP_COLS * pitch;
+      const T* from = b + (int64_t)(p.start[ahead.target] + ahead.col) * p.R;
+      const int some = min(pieces, (ahead.width - ahead.col) * per);
 #pragma unroll
-      for (int k = 0; k < LP_ROWS * 16 / LW_THREADS; ++k) {       // four columns each
-        const int row = (threadIdx.x >> 4) + k * (LW_THREADS / 16), c = 4 * (threadIdx.x & 15);
-        const bool ok = s_row[row] >= 0 && col + c < width;
-        const YT* y = reinterpret_cast<const YT*>(p.y) + (ok ? (int64_t)s_row[row] * p.ldy + p.col0[target] + col + c : 0);
-        lp_copy<4 * sizeof(YT)>(ys + row * S::Y_PITCH + c * (int)sizeof(YT), y, ok);
+      for (int k = 0; k < BP; ++k) {
+        const int x = threadIdx.x + k * LW_THREADS;
+        if (x < pieces) lp_copy<16>(bs + b_to[k], from + (x < some ? 8 * x : 0), x < some);
       }
+      const int64_t col = p.col0[ahead.target] + ahead.col;
+      const bool in = ahead.col + c4 < ahead.width;
+#pragma unroll
+      for (int k = 0; k < YP; ++k) {
+        const bool ok = in && y_at[k];
+        lp_copy<4 * sizeof(YT)>(ys + (line + k * (LW_THREADS / 16)) * S::Y_PITCH + c4 * (int)sizeof(YT), ok ? y_at[k] + col : reinterpret_cast<const YT*>(p.y), ok);
+      }
+      step(ahead);
+      fill = fill + 1 == LP_STAGES ? 0 : fill + 1;
     }
     cp_async_commit();
   };
@@ -565,10 +592,10 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   uint32_t zf[PARTS][KSTEPS][4];
   float f0 = 0.f, f1 = 0.f;
   int held = -1;
+  int stage = b0 % LP_STAGES;
 #pragma unroll 1
   for (int block = b0; block < b1; ++block) {
-    int target, col;
-    place(block, target, col);
+    const int target = here.target, col = here.col, width = here.width;
     if (target != held) {                                         // the rows' z of this target stays in registers
       held = target;
       f0 = s_factor[16 * wm + g][target], f1 = s_factor[16 * wm + 8 + g][target];
@@ -584,8 +611,9 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
     cp_async_wait<LP_STAGES - 2>();
     __syncthreads();
     issue(block + LP_STAGES - 1);
-    const uint32_t bs = s0 + (uint32_t)(block % LP_STAGES) * stage_bytes;
-    uint8_t* ys = smem + (size_t)(block % LP_STAGES) * stage_bytes + LP_COLS * pitch;
+    const uint32_t bs = s0 + (uint32_t)stage * stage_bytes;
+    uint8_t* ys = smem + (size_t)stage * stage_bytes + LP_COLS * pitch;
+    stage = stage + 1 == LP_STAGES ? 0 : stage + 1;
     float d[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
@@ -618,16 +646,15 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
         }
       }
     __syncthreads();
-    const int width = p.start[target + 1] - p.start[target];
+    const int64_t to = p.col0[target] + col;
 #pragma unroll
-    for (int k = 0; k < LP_ROWS * 16 / LW_THREADS; ++k) {
-      const int row = (threadIdx.x >> 4) + k * (LW_THREADS / 16), c = 4 * (threadIdx.x & 15);
-      if (s_row[row] < 0 || col + c >= width) continue;
-      YT* y = reinterpret_cast<YT*>(p.y) + (int64_t)s_row[row] * p.ldy + p.col0[target] + col + c;
-      const uint8_t* from = ys + row * S::Y_PITCH + c * (int)sizeof(YT);
-      if constexpr (sizeof(YT) == 4) *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(from);
-      else *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(from);
+    for (int k = 0; k < YP; ++k) {
+      if (!y_at[k] || col + c4 >= width) continue;
+      const uint8_t* from = ys + (line + k * (LW_THREADS / 16)) * S::Y_PITCH + c4 * (int)sizeof(YT);
+      if constexpr (sizeof(YT) == 4) *reinterpret_cast<uint4*>(y_at[k] + to) = *reinterpret_cast<const uint4*>(from);
+      else *reinterpret_cast<uint2*>(y_at[k] + to) = *reinterpret_cast<const uint2*>(from);
     }
+    step(here);
   }
 }
 
