@@ -151,6 +151,7 @@ SIGNATURES = {
     "b200p_paged_attn_workspace_bytes": (_sz, [_i64, _i32, _i32, _i64]),
     "b200p_paged_attn_workspace_bytes_of": (_sz, [_i64, _i32, _i32, _i32, _i64]),
     "b200p_paged_attn_shared_tile": (_i32, [_i32, _i32]),
+    "b200p_paged_attn_shared_set_path": (_i32, [_i32]),
     "b200p_paged_attn_shared_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32]),
     "b200p_paged_attn_shared": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _f32,
                                        _i32, _i32, _vp, _sz, _vp]),

@@ -355,7 +355,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
 // then blocks of 64 columns, for which b and the old y come along, y grows in its place in shared memory and leaves by whole lines.
 // RK: ranks of all targets, filled up to 32, 64, 128 or 256.  (As the kernel of 16 rows, with operands straight from memory, 8000 rows of rank 64 took 222 us: a
 // round trip per 32 of K and per 16 columns.)
-constexpr int LP_ROWS = 64, LP_STAGES = 3, LP_COLS = 64;
+constexpr int LP_ROWS = 64, LP_COLS = 64;
 template <typename T, typename YT, int RK>
 struct LpShape {
   static constexpr int MT = RK >= 128 ? 2 : 1, NT = RK == 256 ? 8 : 4, KG = RK == 32 ? 2 : 1;      // a warp's 16-row and 8-rank blocks; warps that share them
@@ -365,11 +365,13 @@ struct LpShape {
   static constexpr int Y_PITCH = LP_COLS * (int)sizeof(YT) + 16;
   static __host__ __device__ constexpr int b_pitch(int R) { return 2 * R + 16; }      // an odd number of 16 bytes: no conflicts
   static __host__ __device__ constexpr int stage_c(int R) { return LP_COLS * b_pitch(R) + LP_ROWS * Y_PITCH; }
-  static __host__ __device__ constexpr int front(int R) {
-    const int a = LP_STAGES * STAGE_A, c = LP_STAGES * stage_c(R);
-    return a > c ? a > Z_BYTES ? a : Z_BYTES : c > Z_BYTES ? c : Z_BYTES;
-  }
-  static __host__ __device__ constexpr int bytes(int R) { return front(R) + SPLIT_BYTES; }
+  // what is on its way bounds both parts (8000 rows of rank 64 with three stages each 96 us)
+  static constexpr int ROOM = (RK == 256 ? 216 : 110) * 1024, TOP_R = RK < LW_RANK ? RK : LW_RANK;
+  static __host__ __device__ constexpr int between(int lo, int v, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+  static constexpr int STAGES_A = between(3, ROOM / STAGE_A, 8), STAGES_C = between(3, (ROOM - SPLIT_BYTES) / stage_c(TOP_R), 8);
+  // first the stages of A; then z, or the stages of C, and behind them the split z
+  static constexpr int FRONT = STAGES_C * stage_c(TOP_R) > Z_BYTES ? STAGES_C * stage_c(TOP_R) : Z_BYTES;
+  static constexpr int BYTES = STAGES_A * STAGE_A > FRONT + SPLIT_BYTES ? STAGES_A * STAGE_A : FRONT + SPLIT_BYTES;
   static_assert(WM * WN * KG == LW_WARPS, "eight warps");
 };
 
@@ -394,7 +396,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   const int TR = p.targets * p.R;
   const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(smem);
   float* s_z = reinterpret_cast<float*>(smem);                    // [64][RK], over the stages
-  T* s_split = reinterpret_cast<T*>(smem + S::front(p.R));        // [PARTS][64][LD]
+  T* s_split = reinterpret_cast<T*>(smem + S::FRONT);            // [PARTS][64][LD], over the first stages' end
   pdl_wait();
   const int tile_index = blockIdx.x / C, tiles = p.plan.tiles();
   const int4 tile = p.plan.tile(tile_index);                      // (the plan has room for every tile of the grid)
@@ -415,7 +417,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
     const T* ar = reinterpret_cast<const T*>(p.a) + ((int64_t)tile.x * TR + line) * p.K + 8 * c;
     auto issue = [&](int s) {
       if (s < k1) {
-        const uint32_t at = s0 + (uint32_t)(s % LP_STAGES) * S::STAGE_A + ((c ^ (line & 7)) << 4);
+        const uint32_t at = s0 + (uint32_t)(s % S::STAGES_A) * S::STAGE_A + ((c ^ (line & 7)) << 4);
         const bool in = s * 64 + 8 * c < p.K;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -436,13 +438,13 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
     const int kg = warp / (S::WM * S::WN), wm = warp % S::WM, wn = warp / S::WM % S::WN;
-    for (int s = 0; s < LP_STAGES - 1; ++s) issue(k0 + s);
+    for (int s = 0; s < S::STAGES_A - 1; ++s) issue(k0 + s);
 #pragma unroll 1
     for (int s = k0; s < k1; ++s) {
-      cp_async_wait<LP_STAGES - 2>();
+      cp_async_wait<S::STAGES_A - 2>();
       __syncthreads();
-      issue(s + LP_STAGES - 1);
-      const uint32_t xs = s0 + (uint32_t)(s % LP_STAGES) * S::STAGE_A, as = xs + LP_ROWS * 128;
+      issue(s + S::STAGES_A - 1);
+      const uint32_t xs = s0 + (uint32_t)(s % S::STAGES_A) * S::STAGE_A, as = xs + LP_ROWS * 128;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
         if (S::KG == 2 && (k & 1) != kg) continue;
@@ -564,7 +566,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
     const int row = s_row[line + k * (LW_THREADS / 16)];
     y_at[k] = row < 0 ? nullptr : reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + c4;
   }
-  int fill = b0 % LP_STAGES;                                      // the stage of the next block that is fetched
+  int fill = b0 % S::STAGES_C;                                      // the stage of the next block that is fetched
   auto issue = [&](int block) {
     if (block < b1) {
       const uint32_t bs = s0 + (uint32_t)fill * stage_bytes, ys = bs + LP_COLS * pitch;
@@ -583,16 +585,16 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
         lp_copy<4 * sizeof(YT)>(ys + (line + k * (LW_THREADS / 16)) * S::Y_PITCH + c4 * (int)sizeof(YT), ok ? y_at[k] + col : reinterpret_cast<const YT*>(p.y), ok);
       }
       step(ahead);
-      fill = fill + 1 == LP_STAGES ? 0 : fill + 1;
+      fill = fill + 1 == S::STAGES_C ? 0 : fill + 1;
     }
     cp_async_commit();
   };
-  for (int s = 0; s < LP_STAGES - 1; ++s) issue(b0 + s);
+  for (int s = 0; s < S::STAGES_C - 1; ++s) issue(b0 + s);
   const int wm = warp & 3, wn = warp >> 2;                        // 16 rows, 32 columns
   uint32_t zf[PARTS][KSTEPS][4];
   float f0 = 0.f, f1 = 0.f;
   int held = -1;
-  int stage = b0 % LP_STAGES;
+  int stage = b0 % S::STAGES_C;
 #pragma unroll 1
   for (int block = b0; block < b1; ++block) {
     const int target = here.target, col = here.col, width = here.width;
@@ -608,12 +610,12 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
                         ((part * LP_ROWS + 16 * wm + r8 + 8 * (mat & 1)) * LD + target * p.R + 16 * k + 8 * (mat >> 1)) * 2,
                     zf[part][k]);
     }
-    cp_async_wait<LP_STAGES - 2>();
+    cp_async_wait<S::STAGES_C - 2>();
     __syncthreads();
-    issue(block + LP_STAGES - 1);
+    issue(block + S::STAGES_C - 1);
     const uint32_t bs = s0 + (uint32_t)stage * stage_bytes;
     uint8_t* ys = smem + (size_t)stage * stage_bytes + LP_COLS * pitch;
-    stage = stage + 1 == LP_STAGES ? 0 : stage + 1;
+    stage = stage + 1 == S::STAGES_C ? 0 : stage + 1;
     float d[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
@@ -658,8 +660,10 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   }
 }
 
-// clusters of C CTAs, as many as fit the GPU at two CTAs per SM
-static int launch_lora(void (*kern)(LoraRows), int most_bytes, int bytes, std::atomic<uint64_t>& ready, const LoraRows& p, int64_t tiles, cudaStream_t st) {
+// Clusters of up to C CTAs, as many as fit the GPU at two CTAs per SM.  (us, 64 rows of 64 adapters in clusters of 1 / 2 / 4 / 8: 20.6 / 13.6 / 11.6 / 17.2; 1 row
+// 19.8 / 12.6 / 8.7 / 7.0; 2000 rows in tiles of 64: 66 / 40 / 27 / 32.)
+static int launch_lora(void (*kern)(LoraRows), int most_bytes, int bytes, int C, std::atomic<uint64_t>& ready, const LoraRows& p, int64_t tiles,
+                       cudaStream_t st) {
   int dev = 0;
   cudaError_t ae = cudaGetDevice(&dev);
   if (ae == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {      // ready: devices whose copy of the kernel has its shared memory
@@ -667,7 +671,6 @@ static int launch_lora(void (*kern)(LoraRows), int most_bytes, int bytes, std::a
     if (ae == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   if (ae != cudaSuccess) return cuda_fail(ae, "cudaFuncSetAttribute(lora kernels)");
-  int C = LW_CLUSTER;
   while (C > 1 && tiles * C > 2 * sm_count()) C >>= 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C));
@@ -690,13 +693,13 @@ template <typename T, typename YT, int KS>
 static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   const int TR = p.targets * p.R, ranks = TR > 128 ? 256 : TR > 64 ? 128 : TR > 32 ? 64 : 32;
-  return launch_lora(lora_rows_kernel<T, YT, KS>, lw_row_floats<T, YT>(LW_RANKS) * 16 * 4, lw_row_floats<T, YT>(ranks) * 16 * 4, ready, p, tiles, st);
+  return launch_lora(lora_rows_kernel<T, YT, KS>, lw_row_floats<T, YT>(LW_RANKS) * 16 * 4, lw_row_floats<T, YT>(ranks) * 16 * 4, LW_CLUSTER, ready, p, tiles, st);
 }
 
 template <typename T, typename YT, int RK>
 static int launch_lora_prompt(const LoraRows& p, int64_t tiles, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
-  return launch_lora(lora_prompt_kernel<T, YT, RK>, LpShape<T, YT, RK>::bytes(LW_RANK), LpShape<T, YT, RK>::bytes(p.R), ready, p, tiles, st);
+  return launch_lora(lora_prompt_kernel<T, YT, RK>, LpShape<T, YT, RK>::BYTES, LpShape<T, YT, RK>::BYTES, 4, ready, p, tiles, st);
 }
 
 template <typename T, typename YT>
@@ -740,8 +743,9 @@ extern "C" int b200p_row_groups(const int32_t* index, int32_t* plan, int64_t M, 
   return B200P_OK;
 }
 
-// Tiles of 64 rows read an adapter a quarter as often as tiles of 16, which spread few rows over more SMs.
-extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1024 && M >= 16ll * groups ? 64 : 16; }
+// Tiles of 64 rows read an adapter a quarter as often as tiles of 16, which spread few rows over more SMs and have less to set up.  us, tiles of 16 / 64,
+// 4096 to 5120 columns, 2 adapters: 1000 rows of rank 16 17 / 26, 2000 34 / 32, 8000 115 / 66; rank 64 33 / 57, 64 / 65, 234 / 94.
+extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1500 && M >= 16ll * groups ? 64 : 16; }
 
 extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a, const void* b, const float* scales, void* y, const int32_t* host_columns,
                                int64_t M, int adapters, int tile, int targets, int R, int64_t K, int64_t ldx, int64_t ldy, int dtype, int y_f32,

@@ -1138,9 +1138,15 @@ static int launch_paged_type(const PagedAttn& a, cudaStream_t st) {
 }
 
 // ---- behind shared slots ------------------------------------------------------------------------------------------------------
-// Which calls go by groups: those that the matrix instructions serve.  (fp32 and other sizes are bound by their FMAs, of which sharing saves none.)
-static bool shared_served(int H, int G, int D, int dtype) {
-  return dtype != B200P_F32 && H / G <= PS_ROWS && (D == 64 || D == 80 || D == 96 || D == 128 || D == 256);
+// Which calls go by groups: those that the matrix instructions serve (fp32 and other sizes are bound by their FMAs, of which sharing saves none), and in
+// which the tokens' rows could have keys and values of 32 MiB in common.  Below, the third launch costs more than the reading: us by token / by group, 32 / 8
+// heads of 128, 4 rows behind 900 slots 10.8 / 12.5, 8 behind 1000 (26 MiB) 13.0 / 13.3, 16 behind 512 (30 MiB) 14.0 / 13.9, 8 behind 2000 16.9 / 15.4, 64 behind
+// 1000 47.9 / 30.0, 64 behind 4000 134 / 41.
+static std::atomic<int> g_shared_path{0};                           // 1: by groups wherever it is served, 2: never
+static bool shared_served(int64_t M, int H, int G, int D, int64_t slots, int dtype) {
+  const int path = g_shared_path.load(std::memory_order_relaxed);
+  if (path == 2 || dtype == B200P_F32 || H / G > PS_ROWS || !(D == 64 || D == 80 || D == 96 || D == 128 || D == 256)) return false;
+  return path == 1 || (M - 1) * slots * G * D * 4 >= 32ll << 20;
 }
 static int shared_tile(int H, int G) { return H / G < PS_ROWS ? PS_ROWS / (H / G) : 1; }
 static int64_t shared_rows(int H, int G) {                          // of a token's items with the rows that blocks are filled up to
@@ -1195,6 +1201,7 @@ static int launch_shared(PagedAttn a, PagedPrefix p, int64_t tiles, cudaStream_t
   const unsigned ctas = (unsigned)(units < sm_count() ? units : sm_count());
   p.tpp = a.pt.page / PA_TILE;
   p.inv_tpp = ((1ull << 36) + p.tpp - 1) / p.tpp;
+  p.few = sm_count() / 2;
   int rc;
   if (tc) {
     if constexpr (D == FT_D) {
@@ -1287,6 +1294,12 @@ extern "C" int b200p_paged_attn(const void* q, const void* kpages, const void* v
   return B200P_OK;
 }
 
+extern "C" int b200p_paged_attn_shared_set_path(int path) {
+  B200P_REQUIRE(path >= 0 && path <= 2, B200P_ERR_ARG, "path %d: 0 by the rule, 1 by groups, 2 by tokens", path);
+  g_shared_path.store(path, std::memory_order_relaxed);
+  return B200P_OK;
+}
+
 extern "C" int b200p_paged_attn_shared_tile(int H, int G) { return G > 0 && H >= G && H % G == 0 ? shared_tile(H, G) : 0; }
 
 extern "C" size_t b200p_paged_attn_shared_workspace_bytes(int64_t M, int H, int G, int D, int groups) {
@@ -1305,7 +1318,7 @@ extern "C" int b200p_paged_attn_shared(const void* q, const void* kpages, const 
   B200P_REQUIRE(aligned(plan, 16), B200P_ERR_ALIGN, "the plan must be 16-byte aligned");
   B200P_REQUIRE(M <= 0 || (workspace && workspace_bytes >= b200p_paged_attn_shared_workspace_bytes(M, H, G, D, groups)), B200P_ERR_ARG,
                 "workspace of paged attention behind shared slots too small");
-  if (M <= 0 || !shared_served(H, G, D, dtype))                     // (the other checks are paged attention's)
+  if (M <= 0 || !shared_served(M, H, G, D, (int64_t)width * page, dtype))                     // (the other checks are paged attention's)
     return b200p_paged_attn(q, kpages, vpages, nullptr, table, t_row, t_slot, out, M, H, G, D, P, page, rows, width, scale, 0, 0, dtype, flags, workspace,
                             workspace_bytes, stream);
   PdlClass pdl_cls(8);

@@ -30,13 +30,16 @@ struct PagedPrefix {
   unsigned* total;       // units of all
   int* wait_word;
   int box;               // keys that one copy brings: they lie in one page
+  int few;               // half of the GPU's SMs
 };
 
 // The units (KT shared keys of an item: the rows of a tile, or of a half of it, and a key head) lie end to end and every CTA has an equal part of them, as in
 // paged_attn_kernel.
 struct PrefixShares {
   unsigned n, q, r;
-  __device__ PrefixShares(unsigned U, unsigned ctas) : n(min(U, ctas)) {
+  // A CTA has some 8 us to set up and to leave its part, a unit takes 1.6: four units each, unless half of the GPU is enough for fewer.  What is left of
+  // the GPU begins with the own slots.
+  __device__ PrefixShares(unsigned U, unsigned ctas, unsigned few) : n(min(ctas, max(U / 4, min(U, few)))) {
     q = n ? U / n : 1;
     r = U - q * n;
   }
@@ -135,7 +138,7 @@ __device__ __forceinline__ PrefixCursor<KT, SPLIT> prefix_plan(const PagedPrefix
     if (w < warp) before += s.sum[w];
     U += s.sum[w];
   }
-  const PrefixShares sh(U, gridDim.x);
+  const PrefixShares sh(U, gridDim.x, a.few);
   C c;
   c.u = sh.begin(blockIdx.x), c.end = sh.begin(blockIdx.x + 1);
   for (int i = i0; i < i1; ++i) {
@@ -345,7 +348,7 @@ paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_const
   int heads = 0, c0 = 0;                                            // parts of the shared slots
   int64_t row0 = 0;                                                 // its row in the first of them
   if ((unsigned)group < (unsigned)p.groups && info.w > 0) {
-    const PrefixShares sh(total, prefix_ctas);
+    const PrefixShares sh(total, prefix_ctas, p.few);
     const int halves = info.y >> 16, at = (info.y & 0xffff) * per + r, half = halves > 1 && at >= PS_HALF ? 1 : 0;
     const unsigned u = (unsigned)info.z + (unsigned)((g * halves + half) * info.w);
     c0 = (int)sh.of(u);

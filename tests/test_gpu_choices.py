@@ -8,6 +8,7 @@ import torch
 
 from fake_tokenizer import FakeTokenizer
 from helpers import make_pair, prompts_for, rel_err
+from mlx_parallm_b200 import _lib
 from mlx_parallm_b200.models import _transformer, paged
 from mlx_parallm_b200.utils import generate_choices, generate_step, score_text
 
@@ -27,6 +28,15 @@ def adapters_for(cfg, rank, seed, keys=("self_attn.q_proj", "self_attn.v_proj"),
             out[f"model.layers.{i}.{k}.lora_a"] = torch.randn((h, rank), generator=g) / h ** 0.5
             out[f"model.layers.{i}.{k}.lora_b"] = torch.randn((rank, width[k.split(".")[-1]]), generator=g) * size
     return out
+
+
+@pytest.fixture
+def groups_always(monkeypatch):
+    """Steps go by groups however little their rows share."""
+    monkeypatch.setattr(paged, "SHARED_BYTES", 0)
+    _lib.lib().b200p_paged_attn_shared_set_path(1)
+    yield
+    _lib.lib().b200p_paged_attn_shared_set_path(0)
 
 
 # ---------------------------------------------------------------------------------------------------------------- scoring
@@ -202,10 +212,10 @@ def test_adapters_that_are_refused():
 # ---------------------------------------------------------------------------------------------------------------- shared prompts
 @pytest.mark.parametrize("by_groups", [True, False])
 @pytest.mark.parametrize("name,dtype", MODELS)
-def test_rows_that_share_prompts(name, dtype, by_groups, monkeypatch):
+def test_rows_that_share_prompts(name, dtype, by_groups, request):
     """Steps, a portion and more steps of rows behind shared prompts against the oracle's whole texts."""
     if by_groups:
-        monkeypatch.setattr(paged, "SHARED_BYTES", 0)
+        request.getfixturevalue("groups_always")
     cfg, om, gm = make_pair(name, dtype=dtype)
     heads, tails = prompts_for(cfg, 2, 41), prompts_for(cfg, 6, 14, seed=9)
     groups = [[0, 3, 5], [1, 4]]                                    # row 2 is by itself
@@ -236,7 +246,7 @@ def test_rows_that_share_prompts(name, dtype, by_groups, monkeypatch):
     assert rel_err(gm(torch.from_numpy(texts[:, :20]), cache=cache).cpu(), exp[:, :20]) < LOGIT_TOL
 
 
-def test_greedy_generation_behind_a_shared_prompt(monkeypatch):
+def test_greedy_generation_behind_a_shared_prompt(monkeypatch, groups_always):
     """The captured step over groups gives what the step over pages without them gives, token for token but for near-ties."""
     cfg, om, gm = make_pair("small-llama", dtype="float16")
     head = prompts_for(cfg, 1, 70)
@@ -306,9 +316,8 @@ def test_prompts_that_cannot_be_shared():
 # ---------------------------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("name,dtype,prompt_tokens", [("small-llama", "float16", 90), ("tiny-qwen3", "bfloat16", 33), ("tiny-llama", "float16", 1)])
 @pytest.mark.parametrize("temp", [0.0, 0.9])
-def test_choices_under_adapters_and_their_scores(name, dtype, prompt_tokens, temp, monkeypatch):
+def test_choices_under_adapters_and_their_scores(name, dtype, prompt_tokens, temp, groups_always):
     """Answers to one prompt under several adapters: shared pages, per-row updates and log probabilities in one captured step; scored anew as whole texts."""
-    monkeypatch.setattr(paged, "SHARED_BYTES", 0)
     cfg, om, gm = make_pair(name, dtype=dtype)
     gm.apply_loras([adapters_for(cfg, 8, 1), adapters_for(cfg, 20, 2)], [1.0, 2.0])
     prompt = " ".join(f"w{i}" for i in prompts_for(cfg, 1, prompt_tokens)[0])

@@ -2,10 +2,18 @@
 import pytest
 import torch
 
-from mlx_parallm_b200 import ops
+from mlx_parallm_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(autouse=True)
+def by_groups():
+    """The kernels for groups, whatever the sizes."""
+    _lib.lib().b200p_paged_attn_shared_set_path(1)
+    yield
+    _lib.lib().b200p_paged_attn_shared_set_path(0)
 
 
 class Case:
@@ -303,3 +311,14 @@ def test_refusals():
         with pytest.raises((ValueError, RuntimeError)):
             ops.paged_attn_shared(**dict(args, **bad))
     assert (keep == 7.0).all()
+
+
+@pytest.mark.parametrize("path", [0, 2])
+def test_by_the_rule_and_by_tokens(path):
+    """The rule sends small calls past the groups; by tokens the bits are paged_attn's."""
+    _lib.lib().b200p_paged_attn_shared_set_path(path)
+    small = Case([0] * 5, [160], [161, 170, 190, 200, 210])
+    ws = torch.empty((ops.paged_attn_workspace_bytes(5, 32, 128, 0, 8),), dtype=torch.uint8, device="cuda")
+    plain = ops.paged_attn(small.q, small.k, small.v, small.table, small.row, small.slot, torch.empty_like(small.q), small.scale, workspace=ws)
+    assert torch.equal(small.check(), plain)
+    Case([0] * 12, [1600], [1601 + i for i in range(12)]).check()

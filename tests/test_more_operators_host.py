@@ -67,6 +67,7 @@ def test_lora_rows_refuses_before_it_launches():
 def test_paged_attn_shared_refuses_before_it_launches():
     L = _lib.lib()
     assert [L.b200p_paged_attn_shared_tile(*x) for x in ((32, 8), (40, 8), (8, 8), (64, 1), (129, 1), (300, 1), (7, 2), (4, 0))] == [64, 51, 256, 4, 1, 1, 0, 0]
+    assert L.b200p_paged_attn_shared_set_path(3) == -1 and L.b200p_paged_attn_shared_set_path(-1) == -1 and L.b200p_paged_attn_shared_set_path(0) == 0
     size = L.b200p_paged_attn_shared_workspace_bytes
     assert size(4, 8, 2, 64, 1) > 0 and [size(*x) for x in ((0, 8, 2, 64, 1), (4, 7, 2, 64, 1), (4, 8, 2, 64, 0), (4, 8, 2, 64, 1025))] == [0] * 4
     ok = dict(q=256, k=256, v=256, table=256, row=256, slot=256, out=256, index=256, prefix=256, plan=256, M=4, H=8, G=2, D=64, groups=1, tile=64, P=9, page=16,
