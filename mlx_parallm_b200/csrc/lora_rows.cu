@@ -192,7 +192,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
     }
     const int s0 = (int)((int64_t)p.steps * rank / C), s1 = (int)((int64_t)p.steps * (rank + 1) / C);
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    constexpr int DEEP = 4;                         // steps whose loads are under way together
+    constexpr int DEEP = 2;                         // steps whose loads are under way together
 #pragma unroll 1
     for (int s = s0 + my_k; s < s1; s += DEEP * wk) {
       uint4 av[DEEP][4], xv[DEEP][MB][2];
@@ -221,7 +221,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
         }
     }
   }
-  constexpr int AHEAD = 8 / KS;                      // runs whose b is under way
+  constexpr int AHEAD = 4 / KS;                      // runs whose b is under way
   uint2 w[AHEAD][KS][2];
 #pragma unroll
   for (int u = 0; u < AHEAD; ++u) lw_load<T, KS>(p, b, run0 + warp + u * LW_WARPS, run1, w[u]);
