@@ -84,6 +84,19 @@ template <> __device__ __forceinline__ uint4 lp_nothing<float>() { return make_u
 template <> __device__ __forceinline__ uint4 lp_nothing<__half>() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
 template <> __device__ __forceinline__ uint4 lp_nothing<__nv_bfloat16>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
 
+// Two values at a time where an instruction takes two.
+struct LpPair {
+  float2 s, t;
+  __device__ LpPair() : s(make_float2(0.f, 0.f)), t(s) {}
+  __device__ __forceinline__ void add(float x, float y, float m, float c) {
+    float2 u = __fadd2_rn(make_float2(x, y), make_float2(-m, -m));
+    u.x = lp_max_nan(u.x, -1e30f), u.y = lp_max_nan(u.y, -1e30f);
+    const float2 d = __fmul2_rn(u, make_float2(c, c)), e = make_float2(lp_exp2(d.x), lp_exp2(d.y));
+    s = __fadd2_rn(s, e);
+    t = __ffma2_rn(e, u, t);
+  }
+};
+
 struct LpSums {
   float m, s, t;
   // (m starts at the lowest number, not at minus infinity: a difference to it is a number or minus infinity)
@@ -236,12 +249,15 @@ token_logprobs_kernel(const __grid_constant__ LogProbs a) {
       for (int i = 0; i < E; ++i) top = fmaxf(top, Tr<T>::to_f(e[i]));       // (drops NaN)
     }
     if (top > sum.m) sum.raise(top, c);
+    LpPair pair;
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       const T* e = reinterpret_cast<const T*>(&raw[k]);
 #pragma unroll
-      for (int i = 0; i < E; ++i) sum.add(Tr<T>::to_f(e[i]), c);
+      for (int i = 0; i < E; i += 2) pair.add(Tr<T>::to_f(e[i]), Tr<T>::to_f(e[i + 1]), sum.m, c);
     }
+    sum.s += pair.s.x + pair.s.y;
+    sum.t += pair.t.x + pair.t.y;
   }
   if (rank == 0 && (int)threadIdx.x < p.loose) {
     const float x = Tr<T>::to_f(p.row[p.loose_index(threadIdx.x)]);

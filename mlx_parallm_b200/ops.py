@@ -244,42 +244,41 @@ def lora_tile(rows: int, adapters: int) -> int:
 
 @functools.lru_cache(maxsize=64)
 def _columns(columns: tuple):
+    """(the C array and its address, columns of all targets, one behind the last of y's)"""
     import ctypes as C
     flat = [int(v) for pair in columns for v in pair]
-    if any(len(pair) != 2 for pair in columns) or any(not 0 <= v < 2**31 for v in flat):
+    if not columns or any(len(pair) != 2 for pair in columns) or any(not 0 <= v < 2**31 for v in flat):
         raise ValueError(f"columns are (first, number) of every target: got {columns}")
-    return (C.c_int32 * len(flat))(*flat)
+    held = (C.c_int32 * len(flat))(*flat)
+    return (held, C.addressof(held)), sum(flat[1::2]), max(c + w for c, w in columns)
 
 
 def lora_rows(x, plan: RowPlan, a, b, scales, columns, y):
     """y[m, columns] += scales[i] * (x[m] a[i]^T) b[i]^T for every row m that ``plan`` gives an adapter i (b200p_lora_rows): ``x`` [M, K], ``a`` [adapters,
     targets, R, K], ``b`` [adapters, sum of the targets' columns, R] in one 16-bit type, ``scales`` float32 [adapters], ``columns`` = ((first column in y, number
     of columns), ...) of the targets, ``y`` [M, N] of that type or float32."""
-    import ctypes as C
     dev = x.get_device()
-    if dev < 0 or dev != _device_index() or any(t.get_device() != dev for t in (a, b, scales, y)):
+    if dev < 0 or dev != _device_index() or not a.get_device() == b.get_device() == scales.get_device() == y.get_device() == dev:
         _dev(x, a, b, scales, y)
         raise ValueError("x, adapters and y lie on the current device")
     _plan(plan, dev)
-    M, K = x.shape
+    (M, K), (rows, N), (n, targets, R, ka) = x.shape, y.shape, a.shape
     (ldx, inner), (ldy, y_inner) = x.stride(), y.stride()
-    n, targets, R, ka = a.shape
-    dt, columns = x.dtype, tuple(columns)
-    held = _columns(columns)
-    if a.dtype is not dt or b.dtype is not dt or y.dtype not in (dt, torch.float32):
-        raise ValueError(f"x, a, b are of one 16-bit type, y of it or float32: got {dt}, {a.dtype}, {b.dtype}, {y.dtype}")
+    dt, ydt, columns = x.dtype, y.dtype, tuple(columns)
+    held, total, last = _columns(columns)
+    if a.dtype is not dt or b.dtype is not dt or (ydt is not dt and ydt is not torch.float32):
+        raise ValueError(f"x, a, b are of one 16-bit type, y of it or float32: got {dt}, {a.dtype}, {b.dtype}, {ydt}")
     if scales.dtype is not torch.float32 or scales.shape != (n,) or not (a.is_contiguous() and b.is_contiguous() and scales.is_contiguous()):
         raise ValueError(f"contiguous adapters, scales float32 [{n}]: got {scales.dtype} {tuple(scales.shape)}")
-    if ka != K or len(columns) != targets or b.shape != (n, sum(w for _, w in columns), R):
-        raise ValueError(f"a [adapters, targets, R, {K}] and b [adapters, {sum(w for _, w in columns)}, R] of {len(columns)} targets: got {tuple(a.shape)} and "
-                         f"{tuple(b.shape)}")
-    if y.shape[0] != M or inner != 1 or y_inner != 1 or (M > 1 and (ldx < K or ldy < y.shape[1])) or (plan.rows, plan.groups) != (M, n):
+    if ka != K or len(columns) != targets or b.shape != (n, total, R):
+        raise ValueError(f"a [adapters, targets, R, {K}] and b [adapters, {total}, R] of {len(columns)} targets: got {tuple(a.shape)} and {tuple(b.shape)}")
+    if rows != M or inner != 1 or y_inner != 1 or (M > 1 and (ldx < K or ldy < N)) or plan.rows != M or plan.groups != n:
         raise ValueError(f"rows of x, y and the plan: got {tuple(x.shape)}, {tuple(y.shape)}, {plan.rows} rows in {plan.groups} groups of {n} adapters")
-    if any(c + w > y.shape[1] for c, w in columns):
-        raise ValueError(f"columns {columns} of {y.shape[1]}")
+    if last > N:
+        raise ValueError(f"columns {columns} of {N}")
     _call("b200p_lora_rows", lambda: lib().b200p_lora_rows(
-        x.data_ptr(), plan.data.data_ptr(), a.data_ptr(), b.data_ptr(), scales.data_ptr(), y.data_ptr(), C.addressof(held), M, n, plan.tile, targets, R, K,
-        ldx if M > 1 else K, ldy if M > 1 else y.shape[1], dtype_code(dt), 0 if y.dtype is dt else 1, _stream()))
+        x.data_ptr(), plan.data.data_ptr(), a.data_ptr(), b.data_ptr(), scales.data_ptr(), y.data_ptr(), held[1], M, n, plan.tile, targets, R, K,
+        ldx if M > 1 else K, ldy if M > 1 else N, dtype_code(dt), 0 if ydt is dt else 1, _stream()))
     return y
 
 
@@ -375,9 +374,9 @@ def token_logprobs(logits, tokens=None, top: int = 0, temperature: float = 1.0, 
     if out is None:
         if not 0 <= top <= V:
             raise ValueError(f"{top} alternatives of {V}")
-        at = logits.device
-        out = TokenLogprobs(None if tokens is None else torch.empty(M, dtype=torch.float32, device=at), torch.empty(M, dtype=torch.float32, device=at),
-                            torch.empty((M, top), dtype=torch.int32, device=at), torch.empty((M, top), dtype=torch.float32, device=at))
+        entropy = torch.empty(M, dtype=torch.float32, device=logits.device)      # (new_empty asks less than torch.empty: 1.8 us against 2.5 for two sizes)
+        top_ids = torch.empty((M, top), dtype=torch.int32, device=logits.device) if tokens is None else tokens.new_empty((M, top))
+        out = TokenLogprobs(None if tokens is None else entropy.new_empty((M,)), entropy, top_ids, entropy.new_empty((M, top)))
     else:
         if (out.logprob is None) != (tokens is None):
             raise ValueError("logprob belongs to tokens")
