@@ -212,8 +212,8 @@ __device__ __noinline__ void lp_first_equal(const RowParts<T>& p, LpShared& s, i
 
 // grid (S * rows), clusters of S: as many CTAs to a row as fit the GPU side by side, four per SM, with two vectors or more for a thread (us, device: 1 row of
 // 128256 in 1 / 2 / 4 / 8 CTAs, 20 alternatives 20.6 / 13.2 / 8.4 / 6.7; 64 rows of 32000 bf16 without 4.9 / 4.0 / 3.8 / 5.2; 333 rows of 50257 bf16
-// 13.4 / 14.2 / 15.8 / 20.3).  Four CTAs of 256 threads and not two of 512: 333 rows with 8 alternatives 22.0 -> 17.1, 1500 rows of 151936 144.6 -> 139.9,
-// 99 % of the copy's bandwidth.  (Eight vectors of a thread under way through shared memory instead of four through registers gave nothing.)
+// 13.4 / 14.2 / 15.8 / 20.3).  Four CTAs of 256 threads and not two of 512: 333 rows with 8 alternatives 22.0 -> 17.1 (16.6 with values in pairs), 1500 rows
+// of 151936 144.6 -> 139.9, 99 % of the copy's bandwidth.  (Eight vectors of a thread under way through shared memory instead of four through registers gave nothing.)
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_THREADS, 4)
 token_logprobs_kernel(const __grid_constant__ LogProbs a) {

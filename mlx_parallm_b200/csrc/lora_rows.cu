@@ -144,7 +144,9 @@ __device__ __forceinline__ void lw_load(const LoraRows& p, const T* b, int run, 
       w[k][h] = n0 + 2 * h < r.width && 16 * k < p.R ? *reinterpret_cast<const uint2*>(at + 2 * h * p.R + 16 * k) : make_uint2(0, 0);
 }
 
-// Tiles of 16 rows: decode batches.  YT: y's type; KS: 16 ranks each (R or more).  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits
+// Tiles of 16 rows: decode batches, bound by memory where adapters are many (64 rows of 64 adapters of rank 16, 4096 to 5120: 12.3 us for 29 MB, a floor of 4.6)
+// and by the chain of two products, the parts' meeting and two round trips where they are few (1 row 6.9 us).  Four steps of K and eight runs of 16 columns
+// are under way (two and four: 14.1 us for the 64, 6.8 for the one).  YT: y's type; KS: 16 ranks each (R or more).  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits
 // this CTA's part of K.  Operands come straight from memory, 16 bytes a lane: the order of k within a product is free as long as both operands have the same.
 template <typename T, typename YT, int KS>
 __global__ void __launch_bounds__(LW_THREADS, 2)
@@ -192,7 +194,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
     }
     const int s0 = (int)((int64_t)p.steps * rank / C), s1 = (int)((int64_t)p.steps * (rank + 1) / C);
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    constexpr int DEEP = 2;                         // steps whose loads are under way together
+    constexpr int DEEP = 4;                         // steps whose loads are under way together
 #pragma unroll 1
     for (int s = s0 + my_k; s < s1; s += DEEP * wk) {
       uint4 av[DEEP][4], xv[DEEP][MB][2];
@@ -221,7 +223,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
         }
     }
   }
-  constexpr int AHEAD = 4 / KS;                      // runs whose b is under way
+  constexpr int AHEAD = 8 / KS;                      // runs whose b is under way
   uint2 w[AHEAD][KS][2];
 #pragma unroll
   for (int u = 0; u < AHEAD; ++u) lw_load<T, KS>(p, b, run0 + warp + u * LW_WARPS, run1, w[u]);
@@ -353,8 +355,9 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
 
 // Tiles of 64 rows: prompts.  The same steps as products of tiles in shared memory, which copies fill three stages ahead: z = x A^T in steps of 64 of K,
 // then blocks of 64 columns, for which b and the old y come along, y grows in its place in shared memory and leaves by whole lines.
-// RK: ranks of all targets, filled up to 32, 64, 128 or 256.  (As the kernel of 16 rows, with operands straight from memory, 8000 rows of rank 64 took 222 us: a
-// round trip per 32 of K and per 16 columns.)
+// RK: ranks of all targets, filled up to 32, 64, 128 or 256.  8000 rows of rank 64, 4096 to 5120, 16-bit y: 96 us; the warps' matrix instructions run at 78 % of
+// their rate (943 products a cycle and SM, measured) in the first part and at 60 % in the second, which has two for every product.  (As the kernel of 16
+// rows, with operands straight from memory, 222 us: a round trip per 32 of K and per 16 columns.)
 constexpr int LP_ROWS = 64, LP_COLS = 64;
 template <typename T, typename YT, int RK>
 struct LpShape {

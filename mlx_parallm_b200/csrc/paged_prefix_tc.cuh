@@ -3,8 +3,13 @@
 //
 // The 128 keys of a step come as boxes of 16 to 128 keys that lie in one page each; their ids are looked up a step ahead, a lane per box, and a box without
 // a page is fetched from behind the pages, where the copy brings zeros.  A CTA's part of the work is runs of steps of one item after the other, each of
-// which leaves a part.  Products, softmax and roles are those of the prompt kernel; the maximum is held 14 lower for f16, so that weights reach 2^14 and small
-// ones keep their bits.
+// which leaves a part.  Products, softmax and roles are those of the prompt kernel, but the maximum may lag by 2^6 before outputs are rescaled (a part is few
+// steps, in most of which one of a warp's rows finds a new one: 114 -> 104 thousand cycles for 30 steps), and for f16 it is held 8 lower, so that weights reach
+// 2^14 and small ones keep their bits.  A weight is off by half a step of its type, at random, and their sum is that of the rounded ones: with the output's own
+// rounding 1.2 (bf16) and 1.4 (f16) times that rounding alone.
+//
+// 128 rows in two groups behind 16000 and 12032 slots, 64 / 8 heads (60 GFLOP): 62 us, 3400 cycles a step of 256 rows against 2048 of the tensor core's; of
+// 64 rows behind 4000 slots a CTA has 3.5 steps, and the plan (4000 cycles), queries (5000), first copy (1500) and the part (5000) are most of its time.
 #pragma once
 #include "attn_tc.cuh"
 
@@ -176,7 +181,7 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
       const int at = PS_HALF * i + r;
       cursor.tell(a, run, at);
       if (mine) {
-        // 16 lanes have a row, so that a load is two whole rows (a row per lane: 16 loads of 32 lines each, 9100 cycles instead of CYC)
+        // 16 lanes have a row, so that a load is two whole rows (a row per lane, 32 lines a load: 9100 cycles up to the arrival instead of 5000)
         const int64_t line = at < run.rows ? ((int64_t)a.plan.order()[run.tile.y + at / per] * a.H + (int64_t)run.g * per + at % per) * 16 : -1;
         const int c = lane & 15;
         uint4 x[16];
