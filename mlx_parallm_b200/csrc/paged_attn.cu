@@ -1343,6 +1343,7 @@ extern "C" int b200p_paged_attn_shared(const void* q, const void* kpages, const 
   p.q = q, p.k = kpages, p.v = vpages, p.pt = pt, p.t_row = t_row, p.t_slot = t_slot, p.index = index, p.prefix = prefix;
   p.plan = RowGroups{plan, (int)M}, p.M = (int)M, p.H = H, p.G = G, p.groups = groups, p.scale_log2e = a.scale_log2e;
   p.rec = (float*)(ws += whole_bytes(M, H, G, D));
+  p.rec_rows = (int64_t)(prefix_bytes(M, H, G, D, groups) / ((D + PS_HEAD) * 4));
   p.info = (int4*)(ws += prefix_bytes(M, H, G, D, groups));
   p.total = (unsigned*)(p.info + M);
   const int64_t tiles = row_group_tiles(M, groups, tile);

@@ -31,6 +31,7 @@ struct PagedPrefix {
   int* wait_word;
   int box;               // keys that one copy brings: they lie in one page
   int few;               // half of the GPU's SMs
+  int64_t rec_rows;      // that rec has room for
 };
 
 // The units (KT shared keys of an item: the rows of a tile, or of a half of it, and a key head) lie end to end and every CTA has an equal part of them, as in
@@ -355,6 +356,8 @@ paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_const
     heads = (int)sh.of(u + info.w - 1) - c0 + 1;
     row0 = (int64_t)(item_rows == PS_HALF ? (info.x * a.G + g) * 2 + half : info.x * a.G + g) + c0;
     row0 = row0 * item_rows + at - PS_HALF * half;
+    // (a plan that is not the index's leaves what it likes here: wrong, but nothing behind the workspace is read)
+    if (heads > prefix_ctas || row0 < 0 || row0 + (int64_t)heads * item_rows > p.rec_rows) heads = 0;
   }
   const int all = here ? heads + (int)parts.y : 0;
   auto at = [&](int i) -> const float* {                            // its outputs; maximum and sum stand before them

@@ -174,16 +174,24 @@ class PageBook:
             return
         if self.group is None:
             self.group = torch.empty((self.rows,), dtype=torch.int32, device=self.device)
-            self.prefix = torch.zeros((self.rows,), dtype=torch.int32, device=self.device)
-        index = [-1] * self.rows
-        for i, g in enumerate(self.groups):
+            self.prefix = torch.empty((self.shared_groups,), dtype=torch.int32, device=self.device)
+        index, prefix = [-1] * self.rows, [0] * self.shared_groups
+        together = [(g, n) for g, n in zip(self.groups, self.prefixes) if len(g) > 1][:self.shared_groups]
+        for i, (g, n) in enumerate(together):
+            prefix[i] = n
             for r in g:
                 index[r] = i
         self.group.copy_(torch.tensor(index, dtype=torch.int32))
-        self.prefix.copy_(torch.tensor(self.prefixes + [0] * (self.rows - len(self.prefixes)), dtype=torch.int32))
+        self.prefix.copy_(torch.tensor(prefix, dtype=torch.int32))
         tile = ops.paged_attn_shared_tile(c.n_heads, c.n_kv_heads)
-        self.plan = ops.row_groups(self.group, self.rows, tile, out=self.plan)
+        self.plan = ops.row_groups(self.group, self.shared_groups, tile, out=self.plan)
+        self.shared_workspace(c.n_heads, c.n_kv_heads, c.head_dim)      # (not inside the capture of a step)
         self.by_groups = True
+
+    @property
+    def shared_groups(self) -> int:
+        """Groups of two rows and more that there can be (a plan has 1024 at most: the rows of those behind read by themselves)."""
+        return max(1, min(self.rows // 2, 1024))
 
     def ungroup(self) -> None:
         self.groups, self.prefixes, self.by_groups = [], [], False
@@ -196,7 +204,7 @@ class PageBook:
                 self._regroup()
 
     def shared_workspace(self, H: int, G: int, D: int) -> torch.Tensor:
-        need = ops.paged_attn_shared_workspace_bytes(self.rows, H, G, D, self.rows)
+        need = ops.paged_attn_shared_workspace_bytes(self.rows, H, G, D, self.shared_groups)
         t = self._scratch.get("shared")
         if t is None or t.numel() < need:
             t = self._scratch["shared"] = torch.empty((need,), dtype=torch.uint8, device=self.device)

@@ -695,8 +695,8 @@ def generate_choices(model, tokenizer, prompt: str, n: int = 1, max_tokens: int 
     """``n`` answers to one prompt (the server's ``n`` choices, which the reference answers from n copies of the prompt): the prompt is read once per adapter
     and its pages are shared (model.share_prompt).  ``logprobs`` = k: every token's log probability and the k most likely ones; ``adapters``: every
     answer's of model.apply_loras (-1: none)."""
-    if n < 1 or max_tokens < 0:
-        raise ValueError(f"{n} answers of {max_tokens} tokens")
+    if n < 1 or max_tokens < 0 or page < 1:
+        raise ValueError(f"{n} answers of {max_tokens} tokens in pages of {page}")
     if adapters is not None and len(adapters) != n:
         raise ValueError(f"{len(adapters)} adapters for {n} answers")
     if not hasattr(model, "make_paged_cache"):

@@ -192,6 +192,14 @@ def test_graph_and_streams():
         assert torch.equal(got.top_ids.long().cpu(), ids)
 
 
+def test_rows_farther_apart_than_32_bits_reach():
+    base = torch.empty((2 ** 31 + 5000,), dtype=torch.bfloat16, device="cuda")
+    x = base.as_strided((2, 4001), (2 ** 31 + 8, 1), 3)
+    y, t = make(2, 4001, "bf16")
+    x.copy_(y)
+    check(x, t, 20)
+
+
 def test_refusals():
     x, t = make(4, 100, "f32")
     for bad in (dict(top=33), dict(top=-1), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf)):

@@ -163,6 +163,21 @@ def test_slices_of_wider_tensors():
     check(index_of(1, 3), wide[3:4, 16:272], a, b, s, columns, tall[:1, :y.shape[1]], 16)
 
 
+@pytest.mark.parametrize("tile", [16, 64])
+def test_rows_farther_apart_than_32_bits_reach(tile):
+    x, a, b, s, columns, y = make(3, 2, 128, 16, (64, 32), "bf16", out="16")
+    far = lambda n: torch.zeros((2 ** 31 + 4096,), dtype=torch.bfloat16, device="cuda").as_strided((3, n), (2 ** 30 + 64, 1))
+    wide_x, wide_y = far(128), far(y.shape[1])
+    wide_x.copy_(x), wide_y.copy_(y)
+    check(torch.tensor([1, 0, 1], dtype=torch.int32), wide_x, a, b, s, columns, wide_y, tile)
+
+
+def test_many_rows():
+    check(index_of(5000, 30), *make(5000, 30, 256, 32, (128, 64), "f16", out="16"), 64)
+    check(index_of(5000, 30), *make(5000, 30, 256, 32, (128, 64), "bf16"), 64)
+    check(index_of(5000, 1024), *make(5000, 1024, 128, 16, (64,), "f16"), 16)
+
+
 def test_no_row_has_an_adapter():
     x, a, b, s, columns, y = make(40, 3, 256, 16, (64,), "f16")
     for v in (-1, 3, 2 ** 31 - 1, -2 ** 31):

@@ -240,6 +240,22 @@ def test_scores_of_minus_infinity():
     ops.paged_fault_count(reset=True)
 
 
+@pytest.mark.parametrize("H,G,D,page", [(32, 8, 128, 256), (32, 8, 64, 512)])
+def test_pages_behind_32_bits(H, G, D, page):
+    """A pool of more than 2^31 elements, whose last pages are the ones in use."""
+    c = Case([0] * 9 + [1, 1, -1], [2 * page, page], [2 * page + 1 + 9 * i for i in range(9)] + [page + 5, page + 300, 70], H=H, G=G, D=D, page=page, dtype="f16",
+             poison=False)
+    room = (2 ** 31 + 2 ** 28) // (G * page * D)
+    for name in ("k", "v"):
+        small = getattr(c, name)
+        large = torch.empty((room + c.P, G, page, D), dtype=small.dtype, device="cuda")
+        large[room:] = small
+        setattr(c, name, large)
+    c.table = torch.where(c.table >= 0, c.table + room, c.table)
+    c.P += room
+    c.check()
+
+
 def test_as_paged_attn_does():
     c = Case([0] * 30, [1600], [1601 + 11 * i for i in range(30)])
     got = c.check()
