@@ -1215,11 +1215,11 @@ static int launch_shared(PagedAttn a, PagedPrefix p, int64_t tiles, cudaStream_t
     B200P_LAUNCH_CHECK("paged_prefix_kernel");
   }
   if ((rc = launch_stream<E, true>(a, st))) return rc;
-  // warps per query head: eight where the heads are few, else two
+  // warps per query head: eight where the heads are few, one where they are many
   constexpr int NQ = D <= 128 ? 1 : 2;
-  const int W = (int64_t)a.M * a.H <= 4 * sm_count() ? 8 : 2, rows = tc ? PS_ROWS : PS_HALF;
+  const int W = (int64_t)a.M * a.H <= 4 * sm_count() ? 8 : (int64_t)a.M * a.H <= 32 * sm_count() ? 2 : 1, rows = tc ? PS_ROWS : PS_HALF;
   const dim3 grid((unsigned)((a.H * W + 7) / 8), (unsigned)a.M);
-  launch_pdl(W == 8 ? paged_shared_join_kernel<T, NQ, E::ROWS, 8> : paged_shared_join_kernel<T, NQ, E::ROWS, 2>, grid, 256, 0, st, a, p, (int)ctas, rows);
+  launch_pdl(W == 8 ? paged_shared_join_kernel<T, NQ, E::ROWS, 8> : W == 2 ? paged_shared_join_kernel<T, NQ, E::ROWS, 2> : paged_shared_join_kernel<T, NQ, E::ROWS, 1>, grid, 256, 0, st, a, p, (int)ctas, rows);
   B200P_LAUNCH_CHECK("paged_shared_join_kernel");
   return B200P_OK;
 }

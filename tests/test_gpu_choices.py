@@ -209,6 +209,34 @@ def test_adapters_that_are_refused():
         f32.apply_loras([ok], [1.0])
 
 
+def test_adapters_on_a_tensor_parallel_shard_keep_their_output_columns():
+    """A rank holds A whole and the columns of B that its rows of the projections have."""
+    from mlx_parallm_b200 import synth, tp
+    from mlx_parallm_b200.utils import _get_classes
+    cfg = synth.get_config("small-llama", num_key_value_heads=2)
+    w = synth.random_weights(cfg, seed=1234, dtype="float16")
+    Model, Args = _get_classes(cfg)
+    keys = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj")
+    sets = [adapters_for(cfg, 8, 1, keys), adapters_for(cfg, 20, 2, keys)]
+    full = Model(Args.from_dict(cfg)).load_weights(w, device="cuda").apply_loras(sets, [1.0, 2.0], keys)
+    for rank in range(2):
+        part = Model(Args.from_dict(cfg)).load_weights(tp.shard_weights(w, cfg, rank, 2), device="cuda")
+        part.set_tensor_parallel(rank, 2, None)
+        part.apply_loras(sets, [1.0, 2.0], keys)
+        for lf, lp in zip(full.layers, part.layers):
+            (af, bf, sf, cf), (ap, bp, sp, cp) = lf.self_attn.loras, lp.self_attn.loras
+            assert torch.equal(af, ap) and torch.equal(sf, sp)
+            at = loc = 0
+            for (_, width), (first, n) in zip(cf, cp):
+                assert n == width // 2 and first == loc             # (the shard's fused block is its q, k and v rows)
+                assert torch.equal(bp[:, loc:loc + n], bf[:, at + rank * n:at + (rank + 1) * n])
+                at, loc = at + width, loc + n
+        with pytest.raises(NotImplementedError):
+            part.score(torch.zeros((1, 4), dtype=torch.int64))
+        with pytest.raises(NotImplementedError):
+            next(generate_step(torch.zeros((1, 4), dtype=torch.int64), part, logprobs=1))
+
+
 # ---------------------------------------------------------------------------------------------------------------- shared prompts
 @pytest.mark.parametrize("by_groups", [True, False])
 @pytest.mark.parametrize("name,dtype", MODELS)
