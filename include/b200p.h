@@ -174,7 +174,7 @@ int64_t b200p_row_groups_ints(int64_t M, int64_t groups, int64_t tile);      /* 
  * without one are not touched.  x `dtype` (16-bit) [M, K] (row stride ldx); a `dtype` [adapters, targets, R, K] (lora_a transposed; its k axis permuted like x
  * when x is PERM8), b `dtype` [adapters, sum of the targets' columns, R] (lora_b transposed, target after target), the ranks filled up to R, a multiple of 16,
  * 64 at most, with zeros; 4 targets at most.  host_columns (host memory) = first column in y and number of columns (a multiple of 8) of every target, which do not
- * overlap; y float (y_f32) or `dtype`, row stride ldy.  Sums are fp32, y is rounded once.  `tile` is the plan's: 16 or 64, b200p_lora_rows_tile(M, adapters)
+ * overlap; y float (y_f32) or `dtype`, row stride ldy.  Sums are fp32, y is rounded once.  `tile` is the plan's: 16 or 128, b200p_lora_rows_tile(M, adapters)
  * the better one.  K a multiple of 8; x, its rows, a, b and plan 16-byte aligned; ldy and first columns multiples of 4, y aligned to four elements. */
 int b200p_lora_rows(const void* x, const int32_t* plan, const void* a, const void* b, const float* scales, void* y, const int32_t* host_columns, int64_t M,
                     int adapters, int tile, int targets, int R, int64_t K, int64_t ldx, int64_t ldy, int dtype, int y_f32, void* stream);
@@ -355,8 +355,8 @@ int b200p_gemm_grouped_with(const void* x, const void* w, void* y, const int32_t
  * weights on the MMA's M side and K split where the output is narrow, which adds fp32 partial sums in no fixed order) and fall
  * back to the mma.sync kernels for shapes it declines (K < 64); 1: mma.sync kernels only; 2: the same as 0. */
 int b200p_gemm_set_path(int path);
-/* 0, or 1 + the role (0 loader, 1 MMA issuer, 2 epilogue) whose bounded barrier wait ran out in a tcgen05 dense GEMM since the
- * last call (which clears it).  Synchronises the device. */
+/* 0, or 1 + the role (0 loader, 1 MMA issuer, 2 epilogue) whose bounded barrier wait ran out in a tcgen05 dense GEMM (8 and 9: in
+ * the first or second product of b200p_lora_rows) since the last call (which clears it).  Synchronises the device. */
 int b200p_gemm_tc_fault(void);
 
 /* t_row[t] = rows[e], t_pos[t] = lengths[rows[e]] + (t - cu[e]), t_off[t] = t - cu[e] for the entry e that owns token t

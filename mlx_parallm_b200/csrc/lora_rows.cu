@@ -2,7 +2,7 @@
 //
 //   y[m, columns of target t] += s_i ((x_m A_{i,t}^T) B_{i,t}^T),   i = the row's adapter; rows without one stay as they are
 //
-// The rows are put in the order of their adapters once per batch (row_groups_kernel); the layers then go by tiles of 16 or 64 rows of one adapter.
+// The rows are put in the order of their adapters once per batch (row_groups_kernel); the layers then go by tiles of 16 or 128 rows of one adapter.
 // A cluster of CTAs has a tile: every CTA takes a part of K for z = x A^T, the parts meet through distributed shared memory, and every CTA has all of
 // z for its part of the columns.  So both products are one launch, an adapter is read once for a tile, and even a single row has eight SMs.
 // z is fp32; for the second product its rows are scaled by a power of two and split into two f16 or three bf16 numbers, which carry 22 and 24 of its bits,
@@ -13,6 +13,7 @@
 
 #include "mma_util.cuh"
 #include "rowgroups.cuh"
+#include "tc_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -97,6 +98,8 @@ struct LoraRows {
   RowGroups plan;
   int64_t ldx, ldy;
   int K, R, N, targets, steps;                   // rank of a target, columns of all targets, 32 of K each
+  int sub;                                       // 16-row tiles of a tile of the plan
+  int* wait_word;
   int col0[LW_TARGETS], start[LW_TARGETS + 1], tile0[LW_TARGETS + 1];      // first column of y, of b; first run of 16 columns
 };
 
@@ -162,9 +165,10 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
   float* s_part = reinterpret_cast<float*>(smem);                 // [wk][ROWS][ranks]
   T* s_split = reinterpret_cast<T*>(s_part + ROWS * ranks);      // [PARTS][ROWS][ld]
   pdl_wait();
-  const int tile_index = blockIdx.x / C, tiles = p.plan.tiles();
-  const int4 tile = p.plan.tile(tile_index);                      // (the plan has room for every tile of the grid)
-  if (tile_index >= tiles) return;                                // (the whole cluster)
+  const int tile_index = blockIdx.x / C / p.sub, from = 16 * (blockIdx.x / C - tile_index * p.sub), tiles = p.plan.tiles();
+  int4 tile = p.plan.tile(tile_index);                            // (the plan has room for every tile of the grid)
+  if (tile_index >= tiles || from >= tile.z) return;              // (the whole cluster)
+  tile.y += from, tile.z = min(16, tile.z - from);
   const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.x * p.N * p.R;
   const int runs = p.tile0[p.targets], run0 = (int)((int64_t)runs * rank / C), run1 = (int)((int64_t)runs * (rank + 1) / C);
   if ((int)threadIdx.x < ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
@@ -353,189 +357,211 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
   if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // nobody leaves before all have read
 }
 
-// Tiles of 64 rows: prompts.  The same steps as products of tiles in shared memory, which copies fill three stages ahead: z = x A^T in steps of 64 of K,
-// then blocks of 64 columns, for which b and the old y come along, y grows in its place in shared memory and leaves by whole lines.
-// RK: ranks of all targets, filled up to 32, 64, 128 or 256.  8000 rows of rank 64, 4096 to 5120, 16-bit y: 96 us; the warps' matrix instructions run at 78 % of
-// their rate (943 products a cycle and SM, measured) in the first part and at 60 % in the second, which has two for every product.  (As the kernel of 16
-// rows, with operands straight from memory, 222 us: a round trip per 32 of K and per 16 columns.)
-constexpr int LP_ROWS = 64, LP_COLS = 64;
-template <typename T, typename YT, int RK>
+// Tiles of 128 rows on tcgen05: prompts with 16-bit y and up to three targets.  The same steps, one CTA per SM: rows of x (wherever they lie) and of A come by
+// 16-byte copies into tiles of 64 of K, z = x A^T grows in TMEM, meets the other CTAs' and becomes the operand of the second product, whose blocks of 64 columns
+// take b along with the old y; y grows in its place in shared memory and leaves by whole lines while the next block's product runs.
+// RK: ranks of all targets, filled up to 32, 64, 128 or 256.  8000 rows of rank 64, 4096 to 5120: LPFIG.
+constexpr int LP_ROWS = 128, LP_COLS = 64, LP_TARGETS = 3, LP_STAGES_C = 4;
+template <int RK>
 struct LpShape {
-  static constexpr int MT = RK >= 128 ? 2 : 1, NT = RK == 256 ? 8 : 4, KG = RK == 32 ? 2 : 1;      // a warp's 16-row and 8-rank blocks; warps that share them
-  static constexpr int WM = LP_ROWS / 16 / MT, WN = RK / 8 / NT;
-  static constexpr int PARTS = LwParts<T, YT>::N, LD = RK + 8;
-  static constexpr int STAGE_A = (LP_ROWS + RK) * 128, Z_BYTES = LP_ROWS * RK * 4, SPLIT_BYTES = PARTS * LP_ROWS * LD * 2;
-  static constexpr int Y_PITCH = LP_COLS * (int)sizeof(YT) + 16;
-  static __host__ __device__ constexpr int b_pitch(int R) { return 2 * R + 16; }      // an odd number of 16 bytes: no conflicts
-  static __host__ __device__ constexpr int stage_c(int R) { return LP_COLS * b_pitch(R) + LP_ROWS * Y_PITCH; }
-  // what is on its way bounds both parts (8000 rows of rank 64 with three stages each 96 us)
-  static constexpr int ROOM = (RK == 256 ? 216 : 110) * 1024, TOP_R = RK < LW_RANK ? RK : LW_RANK;
-  static __host__ __device__ constexpr int between(int lo, int v, int hi) { return v < lo ? lo : v > hi ? hi : v; }
-  static constexpr int STAGES_A = between(3, ROOM / STAGE_A, 8), STAGES_C = between(3, (ROOM - SPLIT_BYTES) / stage_c(TOP_R), 8);
-  // first the stages of A; then z, or the stages of C, and behind them the split z
-  static constexpr int FRONT = STAGES_C * stage_c(TOP_R) > Z_BYTES ? STAGES_C * stage_c(TOP_R) : Z_BYTES;
-  static constexpr int BYTES = STAGES_A * STAGE_A > FRONT + SPLIT_BYTES ? STAGES_A * STAGE_A : FRONT + SPLIT_BYTES;
-  static_assert(WM * WN * KG == LW_WARPS, "eight warps");
+  static constexpr int STAGE_A = (LP_ROWS + RK) * 128, STAGES_A = RK == 256 ? 4 : 6, TMEM = RK == 256 ? 256 : 128;
+  static constexpr int B_BYTES = LP_COLS * 128, Y_PITCH = LP_COLS * 2 + 16, STAGE_C = B_BYTES + LP_ROWS * Y_PITCH;
+  static constexpr int Z_TILE = LP_ROWS * 128;                    // of one part of a target's z: 64 ranks a line
+  static __host__ __device__ constexpr int z_pitch(int TR) { return TR + 4; }      // floats; a row per thread without conflicts
+  static __host__ __device__ constexpr int front(int TR) {
+    const int z = LP_ROWS * z_pitch(TR) * 4, c = LP_STAGES_C * STAGE_C;
+    return ((z > c ? z : c) + 1023) / 1024 * 1024;
+  }
+  static __host__ __device__ constexpr int bytes(int TR, int targets) {
+    const int a = STAGES_A * STAGE_A, c = front(TR) + 2 * targets * Z_TILE;
+    return 1024 + (a > c ? a : c);
+  }
+  static_assert(STAGE_C % 1024 == 0 && STAGE_A % 1024 == 0, "tiles at whole swizzles");
 };
 
-template <int N>
-__device__ __forceinline__ void lp_copy(uint32_t dst, const void* src, bool valid) {      // 8 or 16 bytes, zeros where there is nothing
-  const int size = valid ? N : 0;
-  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
+__device__ __forceinline__ void lp_copy(uint32_t dst, const void* src, bool valid) { cp_async16(dst, src, valid); }
+__device__ __forceinline__ void lp_copy8(uint32_t dst, const void* src, bool valid) {
+  const int size = valid ? 8 : 0;                                 // zeros where there is nothing
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
+}
+__device__ __forceinline__ void lp_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void lp_tmem_ld32(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+      "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
 }
 
-template <typename T, typename YT, int RK>
-__global__ void __launch_bounds__(LW_THREADS, RK == 256 ? 1 : 2)
+struct LpBarriers {
+  uint64_t step[6], block[2];                                     // a stage's products, a block's
+  uint32_t tmem;
+  volatile int abort;
+};
+
+// A wait that gives up is reported and everything goes on (the other waits then give up at once): the threads keep meeting at the CTA's and the cluster's
+// barriers, and only the numbers are wrong.
+template <typename T, int RK>
+__global__ void __launch_bounds__(LW_THREADS, 1)
 lora_prompt_kernel(const __grid_constant__ LoraRows p) {
-  using S = LpShape<T, YT, RK>;
-  constexpr int MT = S::MT, NT = S::NT, PARTS = S::PARTS, LD = S::LD, KSTEPS = 4;
+  using S = LpShape<RK>;
+  constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);      // D fp32, 128 rows, K-major operands; N below
+  constexpr uint32_t idesc_z = idesc | ((uint32_t)(RK >> 3) << 17), idesc_y = idesc | ((uint32_t)(LP_COLS >> 3) << 17);
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int s_row[LP_ROWS];
-  __shared__ float s_factor[LP_ROWS][LW_TARGETS];
+  __shared__ float s_factor[LP_TARGETS][LP_ROWS];
+  __shared__ LpBarriers s_bar;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), C = (int)cluster.num_blocks();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mat = lane >> 3, r8 = lane & 7;
-  const int TR = p.targets * p.R;
-  const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(smem);
-  float* s_z = reinterpret_cast<float*>(smem);                    // [64][RK], over the stages
-  T* s_split = reinterpret_cast<T*>(smem + S::FRONT);            // [PARTS][64][LD], over the first stages' end
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int TR = p.targets * p.R, zp = S::z_pitch(TR);
+  const uint32_t raw = smem_u32(smem), s0 = (raw + 1023u) & ~1023u;
+  uint8_t* base = smem + (s0 - raw);                              // (the same offset in every CTA of the cluster)
+  float* s_z = reinterpret_cast<float*>(base);                    // [128][zp], over the first stages
+  const uint32_t zop = s0 + S::front(TR);                         // [part][target] tiles of z
   pdl_wait();
   const int tile_index = blockIdx.x / C, tiles = p.plan.tiles();
   const int4 tile = p.plan.tile(tile_index);                      // (the plan has room for every tile of the grid)
   if (tile_index >= tiles) return;                                // (the whole cluster)
   if ((int)threadIdx.x < LP_ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 6; ++i) mbar_init(smem_u32(&s_bar.step[i]), 1);
+    mbar_init(smem_u32(&s_bar.block[0]), 1);
+    mbar_init(smem_u32(&s_bar.block[1]), 1);
+    s_bar.abort = 0;
+    fence_barrier_init();
+  }
+  // (behind the wait: an older launch on this SM takes its TMEM first)
+  if (warp == 0) tmem_alloc(smem_u32(&s_bar.tmem), S::TMEM);
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_bar.tmem;
+  auto wait = [&](uint64_t& bar, uint32_t parity, int role) { mbar_wait_warp(smem_u32(&bar), parity, &s_bar.abort, p.wait_word, role); };
 
   // ---- this CTA's part of z ---------------------------------------------------------------------------------------------------
+  const int steps = (int)((p.K + 63) / 64), k0 = (int)((int64_t)steps * rank / C), k1 = (int)((int64_t)steps * (rank + 1) / C);
   {
-    const int steps = (int)((p.K + 63) / 64), k0 = (int)((int64_t)steps * rank / C), k1 = (int)((int64_t)steps * (rank + 1) / C);
     const int c = threadIdx.x & 7, line = threadIdx.x >> 3;       // this thread's 16 bytes of a line of 64, and its first line
-    const T* xr[2];
+    const T* xr[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int row = s_row[line + 32 * i];
       xr[i] = row < 0 ? nullptr : reinterpret_cast<const T*>(p.x) + (int64_t)row * p.ldx + 8 * c;
     }
     const T* ar = reinterpret_cast<const T*>(p.a) + ((int64_t)tile.x * TR + line) * p.K + 8 * c;
     auto issue = [&](int s) {
       if (s < k1) {
-        const uint32_t at = s0 + (uint32_t)(s % S::STAGES_A) * S::STAGE_A + ((c ^ (line & 7)) << 4);
+        const uint32_t at = s0 + (uint32_t)((s - k0) % S::STAGES_A) * S::STAGE_A + ((c ^ (line & 7)) << 4);
         const bool in = s * 64 + 8 * c < p.K;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const bool ok = in && xr[i];
-          lp_copy<16>(at + (line + 32 * i) * 128, ok ? xr[i] + s * 64 : reinterpret_cast<const T*>(p.x), ok);
+          lp_copy(at + (line + 32 * i) * 128, ok ? xr[i] + s * 64 : reinterpret_cast<const T*>(p.x), ok);
         }
 #pragma unroll
         for (int i = 0; i < RK / 32; ++i) {
           const bool ok = in && line + 32 * i < TR;
-          lp_copy<16>(at + (LP_ROWS + line + 32 * i) * 128, ok ? ar + (int64_t)32 * i * p.K + s * 64 : reinterpret_cast<const T*>(p.a), ok);
+          lp_copy(at + (LP_ROWS + line + 32 * i) * 128, ok ? ar + (int64_t)32 * i * p.K + s * 64 : reinterpret_cast<const T*>(p.a), ok);
         }
       }
       cp_async_commit();
     };
-    float acc[MT][NT][4];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
-    const int kg = warp / (S::WM * S::WN), wm = warp % S::WM, wn = warp / S::WM % S::WN;
     for (int s = 0; s < S::STAGES_A - 1; ++s) issue(k0 + s);
 #pragma unroll 1
     for (int s = k0; s < k1; ++s) {
+      const int n = s - k0;
       cp_async_wait<S::STAGES_A - 2>();
+      fence_proxy_async_smem();                                   // this thread's copies, for the products
       __syncthreads();
-      issue(s + S::STAGES_A - 1);
-      const uint32_t xs = s0 + (uint32_t)(s % S::STAGES_A) * S::STAGE_A, as = xs + LP_ROWS * 128;
+      if (warp == 0 && elect_one()) {
+        const uint32_t xs = s0 + (uint32_t)(n % S::STAGES_A) * S::STAGE_A;
+        const uint64_t ad = make_desc_sw128(xs), bd = make_desc_sw128(xs + LP_ROWS * 128);
 #pragma unroll
-      for (int k = 0; k < KSTEPS; ++k) {
-        if (S::KG == 2 && (k & 1) != kg) continue;
-        uint32_t xf[MT][4];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const int row = 16 * (wm * MT + i) + r8 + 8 * (mat & 1);
-          ldsm_x4(xs + row * 128 + (((2 * k + (mat >> 1)) ^ (row & 7)) << 4), xf[i]);
-        }
-#pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
-          const int n = 8 * NT * wn + 16 * j + r8 + 8 * (mat >> 1);
-          uint32_t af[4];
-          ldsm_x4(as + n * 128 + (((2 * k + (mat & 1)) ^ (n & 7)) << 4), af);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            mma16816<T>(acc[i][2 * j], xf[i], af[0], af[1]);
-            mma16816<T>(acc[i][2 * j + 1], xf[i], af[2], af[3]);
-          }
-        }
+        for (int k = 0; k < 4; ++k) lp_mma(tmem, ad + 2 * k, bd + 2 * k, idesc_z, n || k ? 1u : 0u);
+        umma_commit(smem_u32(&s_bar.step[n % S::STAGES_A]));
       }
+      __syncwarp();
+      if (n > 0) wait(s_bar.step[(n - 1) % S::STAGES_A], (uint32_t)((n - 1) / S::STAGES_A) & 1u, 8);      // its stage is the one that is filled now
+      issue(s + S::STAGES_A - 1);
     }
     cp_async_wait<0>();
-    __syncthreads();
+    if (k1 > k0) wait(s_bar.step[(k1 - k0 - 1) % S::STAGES_A], (uint32_t)((k1 - k0 - 1) / S::STAGES_A) & 1u, 8);
+    tc_fence_after();
+    __syncthreads();                                              // the stages are nobody's any more
+    // a thread per row and every other 32 ranks
+    const int row = 32 * (warp & 3) + lane;
+    for (int r = 32 * (warp >> 2); r < TR; r += 64) {
+      float z[32];
+      if (k1 > k0) {
+        lp_tmem_ld32(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + r, z);
+        tmem_ld_wait();
+      } else {
 #pragma unroll
-    for (int half = 0; half < S::KG; ++half) {
-      if (kg == half) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float2* z = reinterpret_cast<float2*>(s_z + (16 * (wm * MT + i) + 8 * h + g) * RK + 8 * NT * wn + 8 * j + 2 * t);
-              float2 v = make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
-              if (half) {
-                const float2 u = *z;
-                v.x += u.x, v.y += u.y;
-              }
-              *z = v;
-            }
+        for (int i = 0; i < 32; ++i) z[i] = 0.f;
       }
-      __syncthreads();
-    }
-  }
-  // ---- z of all CTAs -----------------------------------------------------------------------------------------------------------
-  if (C > 1) {
-    constexpr int N = LP_ROWS * RK / 4 / LW_THREADS;
-    float4 z[N];
-    cluster.sync();
 #pragma unroll
-    for (int k = 0; k < N; ++k) z[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < 32; i += 4)
+        if (r + i < TR) *reinterpret_cast<float4*>(s_z + row * zp + r + i) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+    }
+    tc_fence_before();                                            // (the blocks' products write there again)
+  }
+  if (C > 1) cluster.sync();
+  else __syncthreads();
+
+  // ---- z of all CTAs, as two 16-bit numbers: a thread per row and target ----------------------------------------------------------
+  for (int i = threadIdx.x; i < LP_ROWS * p.targets; i += LW_THREADS) {
+    const int row = i & (LP_ROWS - 1), target = i / LP_ROWS, at = row * zp + target * p.R;
+    float z[LW_RANK];
+#pragma unroll
+    for (int k = 0; k < LW_RANK; ++k) z[k] = 0.f;
     for (int r = 0; r < C; ++r) {                                 // in one order everywhere
-      const float4* other = reinterpret_cast<const float4*>(cluster.map_shared_rank(s_z, r));
+      const float* other = C > 1 ? cluster.map_shared_rank(s_z, r) + at : s_z + at;
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const float4 v = other[threadIdx.x + k * LW_THREADS];
-        z[k].x += v.x, z[k].y += v.y, z[k].z += v.z, z[k].w += v.w;
-      }
+      for (int k = 0; k < LW_RANK; k += 4)
+        if (k < p.R) {
+          const float4 v = *reinterpret_cast<const float4*>(other + k);
+          z[k] += v.x, z[k + 1] += v.y, z[k + 2] += v.z, z[k + 3] += v.w;
+        }
     }
-    cluster.sync();                                               // all have read
+    float top = 0.f, up, down;
 #pragma unroll
-    for (int k = 0; k < N; ++k) reinterpret_cast<float4*>(s_z)[threadIdx.x + k * LW_THREADS] = z[k];
-    __syncthreads();
-  }
-  // as 16-bit numbers: a warp per row and target
-  for (int i = warp; i < tile.z * p.targets; i += LW_WARPS) {
-    const int row = i / p.targets, target = i - row * p.targets, at = row * RK + target * p.R;
-    float z[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) z[k] = 32 * k + lane < p.R ? s_z[at + 32 * k + lane] : 0.f;
-    const float top = warp_max(fmaxf(fabsf(z[0]), fabsf(z[1])));
-    float up, down;
+    for (int k = 0; k < LW_RANK; ++k) top = fmaxf(top, fabsf(z[k]));
     lw_scale(top, up, down);
-    if (lane == 0) s_factor[row][target] = up * p.scales[tile.x];
+    s_factor[target][row] = up * p.scales[tile.x];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (32 * k + lane >= p.R) continue;
-      float x = z[k] * down;
+    for (int k = 0; k < LW_RANK; k += 8)
+      if (k < p.R) {
+        uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int part = 0; part < PARTS; ++part) {
-        const T h = Tr<T>::from_f(x);
-        s_split[(part * LP_ROWS + row) * LD + target * p.R + 32 * k + lane] = h;
-        x -= Tr<T>::to_f(h);
+        for (int e = 0; e < 4; ++e) {
+          const float x = z[k + 2 * e] * down, y = z[k + 2 * e + 1] * down;
+          const T hx = Tr<T>::from_f(x), hy = Tr<T>::from_f(y);
+          hi[e] = pack2<T>(x, y);
+          lo[e] = pack2<T>(x - Tr<T>::to_f(hx), y - Tr<T>::to_f(hy));
+        }
+        const uint32_t to = zop + (uint32_t)target * S::Z_TILE + row * 128 + (((k >> 3) ^ (row & 7)) << 4);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (uint32_t)p.targets * S::Z_TILE), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
       }
-    }
   }
-  __syncthreads();                                                // (the stages may lie over z again)
+  fence_proxy_async_smem();
+  if (C > 1) cluster.sync();                                      // all have read: the stages may lie there again
+  else __syncthreads();
+  tc_fence_after();
   pdl_launch_dependents();
 
   // ---- this CTA's columns -------------------------------------------------------------------------------------------------------
@@ -552,120 +578,113 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   };
   Place ahead{0, 0, p.start[1]};
   for (int k = 0; k < b0; ++k) step(ahead);
-  Place here = ahead;
-  const int pitch = S::b_pitch(p.R), per = p.R / 8, pieces = LP_COLS * per;      // 16-byte pieces of a line of b, and of a block: they lie in a row
-  const uint32_t stage_bytes = (uint32_t)S::stage_c(p.R);
+  Place here = ahead, issued = ahead;                             // the next block to fetch, to store, to multiply
+  const int per = p.R / 8, pieces = LP_COLS * per;                // 16-byte pieces of a line of b, and of a block: they lie in a row
   constexpr int BP = LP_COLS * LW_RANK / 8 / LW_THREADS, YP = LP_ROWS * 16 / LW_THREADS;
   uint32_t b_to[BP];                                              // where this thread's pieces of b go
 #pragma unroll
   for (int k = 0; k < BP; ++k) {
-    const int x = threadIdx.x + k * LW_THREADS;
-    b_to[k] = (uint32_t)(16 * (x + x / per));
+    const int x = threadIdx.x + k * LW_THREADS, n = x / per, c = x - n * per;
+    b_to[k] = (uint32_t)(n * 128 + ((c ^ (n & 7)) << 4));
   }
   const int c4 = 4 * (threadIdx.x & 15), line = threadIdx.x >> 4;  // its four columns of y, in rows `line`, `line` + 16 and so on
-  YT* y_at[YP];
-#pragma unroll
-  for (int k = 0; k < YP; ++k) {
-    const int row = s_row[line + k * (LW_THREADS / 16)];
-    y_at[k] = row < 0 ? nullptr : reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + c4;
-  }
-  int fill = b0 % S::STAGES_C;                                      // the stage of the next block that is fetched
+  auto y_of = [&](int k) { return s_row[line + k * (LW_THREADS / 16)]; };
   auto issue = [&](int block) {
     if (block < b1) {
-      const uint32_t bs = s0 + (uint32_t)fill * stage_bytes, ys = bs + LP_COLS * pitch;
+      const uint32_t bs = s0 + (uint32_t)((block - b0) % LP_STAGES_C) * S::STAGE_C, ys = bs + S::B_BYTES;
       const T* from = b + (int64_t)(p.start[ahead.target] + ahead.col) * p.R;
       const int some = min(pieces, (ahead.width - ahead.col) * per);
 #pragma unroll
       for (int k = 0; k < BP; ++k) {
         const int x = threadIdx.x + k * LW_THREADS;
-        if (x < pieces) lp_copy<16>(bs + b_to[k], from + (x < some ? 8 * x : 0), x < some);
+        if (x < pieces) lp_copy(bs + b_to[k], from + (x < some ? 8 * x : 0), x < some);
       }
-      const int64_t col = p.col0[ahead.target] + ahead.col;
+      const T* y = reinterpret_cast<const T*>(p.y) + p.col0[ahead.target] + ahead.col + c4;
       const bool in = ahead.col + c4 < ahead.width;
 #pragma unroll
       for (int k = 0; k < YP; ++k) {
-        const bool ok = in && y_at[k];
-        lp_copy<4 * sizeof(YT)>(ys + (line + k * (LW_THREADS / 16)) * S::Y_PITCH + c4 * (int)sizeof(YT), ok ? y_at[k] + col : reinterpret_cast<const YT*>(p.y), ok);
+        const int row = y_of(k);
+        const bool ok = in && row >= 0;
+        lp_copy8(ys + (line + k * (LW_THREADS / 16)) * S::Y_PITCH + c4 * 2, ok ? y + (int64_t)row * p.ldy : reinterpret_cast<const T*>(p.y), ok);
       }
       step(ahead);
-      fill = fill + 1 == S::STAGES_C ? 0 : fill + 1;
     }
     cp_async_commit();
   };
-  for (int s = 0; s < S::STAGES_C - 1; ++s) issue(b0 + s);
-  const int wm = warp & 3, wn = warp >> 2;                        // 16 rows, 32 columns
-  uint32_t zf[PARTS][KSTEPS][4];
-  float f0 = 0.f, f1 = 0.f;
-  int held = -1;
-  int stage = b0 % S::STAGES_C;
+  auto multiply = [&](int block) {                                // by one thread
+    const int n = block - b0;
+    const uint64_t bd = make_desc_sw128(s0 + (uint32_t)(n % LP_STAGES_C) * S::STAGE_C);
+    for (int part = 0; part < 2; ++part) {
+      const uint64_t ad = make_desc_sw128(zop + (uint32_t)(part * p.targets + issued.target) * S::Z_TILE);
+#pragma unroll
+      for (int k = 0; k < LW_RANK / 16; ++k)
+        if (16 * k < p.R) lp_mma(tmem + LP_COLS * (n & 1), ad + 2 * k, bd + 2 * k, idesc_y, part || k ? 1u : 0u);
+    }
+    umma_commit(smem_u32(&s_bar.block[n & 1]));
+  };
+  for (int s = 0; s < LP_STAGES_C - 1; ++s) issue(b0 + s);
 #pragma unroll 1
-  for (int block = b0; block < b1; ++block) {
-    const int target = here.target, col = here.col, width = here.width;
-    if (target != held) {                                         // the rows' z of this target stays in registers
-      held = target;
-      f0 = s_factor[16 * wm + g][target], f1 = s_factor[16 * wm + 8 + g][target];
-#pragma unroll
-      for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-        for (int k = 0; k < KSTEPS; ++k)
-          if (16 * k < p.R)
-            ldsm_x4((uint32_t)__cvta_generic_to_shared(s_split) +
-                        ((part * LP_ROWS + 16 * wm + r8 + 8 * (mat & 1)) * LD + target * p.R + 16 * k + 8 * (mat >> 1)) * 2,
-                    zf[part][k]);
-    }
-    cp_async_wait<S::STAGES_C - 2>();
+  for (int block = b0 - 1; block < b1; ++block) {
+    // block + 1 is here (of what is under way it is the last but one, or older); all are done with block - 1
+    cp_async_wait<LP_STAGES_C - 3>();
+    fence_proxy_async_smem();
+    tc_fence_before();
     __syncthreads();
-    issue(block + S::STAGES_C - 1);
-    const uint32_t bs = s0 + (uint32_t)stage * stage_bytes;
-    uint8_t* ys = smem + (size_t)stage * stage_bytes + LP_COLS * pitch;
-    stage = stage + 1 == S::STAGES_C ? 0 : stage + 1;
-    float d[4][4];
+    tc_fence_after();
+    if (block + 1 < b1) {
+      if (warp == 0 && elect_one()) multiply(block + 1);
+      __syncwarp();
+      step(issued);
+    }
+    if (block < b0) continue;
+    issue(block + LP_STAGES_C - 1);
+    const int n = block - b0;
+    wait(s_bar.block[n & 1], (uint32_t)(n >> 1) & 1u, 9);
+    tc_fence_after();
+    uint8_t* ys = base + (size_t)(n % LP_STAGES_C) * S::STAGE_C + S::B_BYTES;
+    {
+      const int row = 32 * (warp & 3) + lane, c0 = 32 * (warp >> 2);
+      float d[32];
+      lp_tmem_ld32(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + LP_COLS * (n & 1) + c0, d);
+      tmem_ld_wait();
+      const float f = s_factor[here.target][row];
+      uint4* y = reinterpret_cast<uint4*>(ys + row * S::Y_PITCH + c0 * 2);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
-#pragma unroll
-    for (int k = 0; k < KSTEPS; ++k) {
-      if (16 * k >= p.R) break;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t bf[4];
-        ldsm_x4(bs + (32 * wn + 16 * j + r8 + 8 * (mat >> 1)) * pitch + (2 * k + (mat & 1)) * 16, bf);
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-          mma16816<T>(d[2 * j], zf[part][k], bf[0], bf[1]);
-          mma16816<T>(d[2 * j + 1], zf[part][k], bf[2], bf[3]);
-        }
+      for (int k = 0; k < 4; ++k) {
+        uint4 v = y[k];
+        const T* e = reinterpret_cast<const T*>(&v);
+        const float* x = d + 8 * k;
+        v = make_uint4(pack2<T>(fmaf(f, x[0], Tr<T>::to_f(e[0])), fmaf(f, x[1], Tr<T>::to_f(e[1]))),
+                       pack2<T>(fmaf(f, x[2], Tr<T>::to_f(e[2])), fmaf(f, x[3], Tr<T>::to_f(e[3]))),
+                       pack2<T>(fmaf(f, x[4], Tr<T>::to_f(e[4])), fmaf(f, x[5], Tr<T>::to_f(e[5]))),
+                       pack2<T>(fmaf(f, x[6], Tr<T>::to_f(e[6])), fmaf(f, x[7], Tr<T>::to_f(e[7]))));
+        y[k] = v;
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        YT* y = reinterpret_cast<YT*>(ys + (16 * wm + 8 * h + g) * S::Y_PITCH) + 32 * wn + 8 * j + 2 * t;
-        const float f = h ? f1 : f0;
-        if constexpr (sizeof(YT) == 4) {
-          float2 v = *reinterpret_cast<float2*>(y);
-          v.x = fmaf(f, d[j][2 * h], v.x), v.y = fmaf(f, d[j][2 * h + 1], v.y);
-          *reinterpret_cast<float2*>(y) = v;
-        } else {
-          *reinterpret_cast<uint32_t*>(y) = pack2<YT>(fmaf(f, d[j][2 * h], Tr<YT>::to_f(y[0])), fmaf(f, d[j][2 * h + 1], Tr<YT>::to_f(y[1])));
-        }
-      }
     __syncthreads();
-    const int64_t to = p.col0[target] + col;
+    T* y = reinterpret_cast<T*>(p.y) + p.col0[here.target] + here.col + c4;
+    if (here.col + c4 < here.width) {
 #pragma unroll
-    for (int k = 0; k < YP; ++k) {
-      if (!y_at[k] || col + c4 >= width) continue;
-      const uint8_t* from = ys + (line + k * (LW_THREADS / 16)) * S::Y_PITCH + c4 * (int)sizeof(YT);
-      if constexpr (sizeof(YT) == 4) *reinterpret_cast<uint4*>(y_at[k] + to) = *reinterpret_cast<const uint4*>(from);
-      else *reinterpret_cast<uint2*>(y_at[k] + to) = *reinterpret_cast<const uint2*>(from);
+      for (int k = 0; k < YP; ++k) {
+        const int row = y_of(k);
+        if (row >= 0) *reinterpret_cast<uint2*>(y + (int64_t)row * p.ldy) = *reinterpret_cast<const uint2*>(ys + (line + k * (LW_THREADS / 16)) * S::Y_PITCH + c4 * 2);
+      }
     }
     step(here);
   }
+  cp_async_wait<0>();
+  if (s_bar.abort) wait_settle();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::TMEM);
+  }
 }
 
-// Clusters of up to C CTAs, as many as fit the GPU at two CTAs per SM.  (us, 64 rows of 64 adapters in clusters of 1 / 2 / 4 / 8: 20.6 / 13.6 / 11.6 / 17.2; 1 row
-// 19.8 / 12.6 / 8.7 / 7.0; 2000 rows in tiles of 64: 66 / 40 / 27 / 32.)
-static int launch_lora(void (*kern)(LoraRows), int most_bytes, int bytes, int C, std::atomic<uint64_t>& ready, const LoraRows& p, int64_t tiles,
+// Clusters of up to C CTAs, as many as fit the GPU.  (us, 64 rows of 64 adapters in clusters of 1 / 2 / 4 / 8: 20.6 / 13.6 / 11.6 / 17.2; 1 row 19.8 / 12.6 / 8.7 /
+// 7.0.)
+static int launch_lora(void (*kern)(LoraRows), int most_bytes, int bytes, int C, int per_sm, std::atomic<uint64_t>& ready, const LoraRows& p, int64_t tiles,
                        cudaStream_t st) {
   int dev = 0;
   cudaError_t ae = cudaGetDevice(&dev);
@@ -674,7 +693,7 @@ static int launch_lora(void (*kern)(LoraRows), int most_bytes, int bytes, int C,
     if (ae == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   if (ae != cudaSuccess) return cuda_fail(ae, "cudaFuncSetAttribute(lora kernels)");
-  while (C > 1 && tiles * C > 2 * sm_count()) C >>= 1;
+  while (C > 1 && tiles * C > (int64_t)per_sm * sm_count()) C >>= 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C));
   cfg.blockDim = dim3(LW_THREADS);
@@ -696,27 +715,33 @@ template <typename T, typename YT, int KS>
 static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   const int TR = p.targets * p.R, ranks = TR > 128 ? 256 : TR > 64 ? 128 : TR > 32 ? 64 : 32;
-  return launch_lora(lora_rows_kernel<T, YT, KS>, lw_row_floats<T, YT>(LW_RANKS) * 16 * 4, lw_row_floats<T, YT>(ranks) * 16 * 4, LW_CLUSTER, ready, p, tiles, st);
+  return launch_lora(lora_rows_kernel<T, YT, KS>, lw_row_floats<T, YT>(LW_RANKS) * 16 * 4, lw_row_floats<T, YT>(ranks) * 16 * 4, LW_CLUSTER, 2, ready, p,
+                     tiles * p.sub, st);
 }
 
-template <typename T, typename YT, int RK>
-static int launch_lora_prompt(const LoraRows& p, int64_t tiles, cudaStream_t st) {
+template <typename T, int RK>
+static int launch_lora_prompt(LoraRows p, int64_t tiles, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
-  return launch_lora(lora_prompt_kernel<T, YT, RK>, LpShape<T, YT, RK>::BYTES, LpShape<T, YT, RK>::BYTES, 4, ready, p, tiles, st);
+  if (const int rc = wait_word(WAIT_GEMM_TC, &p.wait_word)) return rc;
+  const int most = RK < LW_RANK * LP_TARGETS ? RK : LW_RANK * LP_TARGETS;
+  return launch_lora(lora_prompt_kernel<T, RK>, LpShape<RK>::bytes(most, LP_TARGETS), LpShape<RK>::bytes(p.targets * p.R, p.targets), 4, 1, ready, p, tiles, st);
 }
 
 template <typename T, typename YT>
-static int launch_lora_tiles(const LoraRows& p, int tile, int64_t tiles, cudaStream_t st) {
-  if (tile == 16) {
-    if (p.R == 16) return launch_lora_rows<T, YT, 1>(p, tiles, st);
-    if (p.R == 32) return launch_lora_rows<T, YT, 2>(p, tiles, st);
-    return launch_lora_rows<T, YT, 4>(p, tiles, st);
-  }
+static int launch_lora_tiles(LoraRows p, int tile, int64_t tiles, cudaStream_t st) {
   const int TR = p.targets * p.R;
-  if (TR > 128) return launch_lora_prompt<T, YT, 256>(p, tiles, st);
-  if (TR > 64) return launch_lora_prompt<T, YT, 128>(p, tiles, st);
-  if (TR > 32) return launch_lora_prompt<T, YT, 64>(p, tiles, st);
-  return launch_lora_prompt<T, YT, 32>(p, tiles, st);
+  if constexpr (sizeof(YT) == 2) {
+    if (tile == LP_ROWS && p.targets <= LP_TARGETS) {
+      if (TR > 128) return launch_lora_prompt<T, 256>(p, tiles, st);
+      if (TR > 64) return launch_lora_prompt<T, 128>(p, tiles, st);
+      if (TR > 32) return launch_lora_prompt<T, 64>(p, tiles, st);
+      return launch_lora_prompt<T, 32>(p, tiles, st);
+    }
+  }
+  p.sub = tile / 16;                                                // (fp32 y and four targets: tiles of 16 rows of the plan's)
+  if (p.R == 16) return launch_lora_rows<T, YT, 1>(p, tiles, st);
+  if (p.R == 32) return launch_lora_rows<T, YT, 2>(p, tiles, st);
+  return launch_lora_rows<T, YT, 4>(p, tiles, st);
 }
 
 }  // namespace b200p
@@ -748,7 +773,7 @@ extern "C" int b200p_row_groups(const int32_t* index, int32_t* plan, int64_t M, 
 
 // Tiles of 64 rows read an adapter a quarter as often as tiles of 16, which spread few rows over more SMs and have less to set up.  us, tiles of 16 / 64,
 // 4096 to 5120 columns, 2 adapters: 1000 rows of rank 16 17 / 26, 2000 34 / 32, 8000 115 / 66; rank 64 33 / 57, 64 / 65, 234 / 94.
-extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1500 && M >= 16ll * groups ? 64 : 16; }
+extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1500 && M >= 16ll * groups ? LP_ROWS : 16; }
 
 extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a, const void* b, const float* scales, void* y, const int32_t* host_columns,
                                int64_t M, int adapters, int tile, int targets, int R, int64_t K, int64_t ldx, int64_t ldy, int dtype, int y_f32,
@@ -756,7 +781,7 @@ extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a
   PdlClass pdl_cls(64);
   B200P_REQUIRE(dtype == B200P_F16 || dtype == B200P_BF16, B200P_ERR_ARG, "adapters and their inputs are 16-bit");
   B200P_REQUIRE(M >= 0 && M <= RG_ROWS && adapters > 0 && adapters <= RG_GROUPS, B200P_ERR_ARG, "bad shape: %lld rows, %d adapters", (long long)M, adapters);
-  B200P_REQUIRE(tile == 16 || tile == 64, B200P_ERR_ARG, "the plan's tiles have 16 or 64 rows, not %d", tile);
+  B200P_REQUIRE(tile == 16 || tile == LP_ROWS, B200P_ERR_ARG, "the plan's tiles have 16 or 128 rows, not %d", tile);
   B200P_REQUIRE(targets > 0 && targets <= LW_TARGETS, B200P_ERR_ARG, "%d targets: 1 to %d", targets, LW_TARGETS);
   B200P_REQUIRE(R > 0 && R % 16 == 0 && R <= LW_RANK, B200P_ERR_ARG, "rank %d: a multiple of 16, %d at most", R, LW_RANK);
   B200P_REQUIRE(K > 0 && K % 8 == 0 && K < (1ll << 24) && ldx >= K, B200P_ERR_ARG, "bad K %lld: a multiple of 8, not above ldx", (long long)K);

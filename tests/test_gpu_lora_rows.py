@@ -114,7 +114,7 @@ def check(index, x, a, b, scales, columns, y, tile):
 
 
 @pytest.mark.parametrize("dtype,out", [("f16", "f32"), ("f16", "16"), ("bf16", "f32"), ("bf16", "16")])
-@pytest.mark.parametrize("tile", [16, 64])
+@pytest.mark.parametrize("tile", [16, 128])
 @pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 63, 64, 65, 130, 300])
 def test_rows(M, tile, dtype, out):
     for n in (1, 3, 40):
@@ -122,14 +122,14 @@ def test_rows(M, tile, dtype, out):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("tile", [16, 64])
+@pytest.mark.parametrize("tile", [16, 128])
 @pytest.mark.parametrize("K", [8, 16, 24, 32, 40, 64, 136, 248, 520, 4096, 8200])
 def test_inner_sizes(K, tile, dtype):
     check(index_of(37, 3), *make(37, 3, K, 16, (128, 8, 40), dtype, seed=K), tile)
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("tile", [16, 64])
+@pytest.mark.parametrize("tile", [16, 128])
 @pytest.mark.parametrize("R,targets", [(16, 1), (16, 2), (16, 3), (16, 4), (32, 1), (32, 2), (32, 4), (48, 1), (48, 2), (48, 3), (64, 1), (64, 2), (64, 3), (64, 4)])
 def test_ranks_and_targets(R, targets, tile, dtype):
     check(index_of(50, 2), *make(50, 2, 320, R, (72, 8, 16, 200)[:targets], dtype, out="16" if R % 32 else "f32", seed=R), tile)
@@ -142,7 +142,7 @@ def test_ranks_that_are_filled_up(rank):
 
 @pytest.mark.parametrize("width", [8, 16, 24, 56, 1000, 4096])
 def test_widths(width):
-    for tile in (16, 64):
+    for tile in (16, 128):
         check(index_of(33, 3), *make(33, 3, 128, 16, (width,), "f16", out="16"), tile)
 
 
@@ -163,7 +163,7 @@ def test_slices_of_wider_tensors():
     check(index_of(1, 3), wide[3:4, 16:272], a, b, s, columns, tall[:1, :y.shape[1]], 16)
 
 
-@pytest.mark.parametrize("tile", [16, 64])
+@pytest.mark.parametrize("tile", [16, 128])
 def test_rows_farther_apart_than_32_bits_reach(tile):
     x, a, b, s, columns, y = make(3, 2, 128, 16, (64, 32), "bf16", out="16")
     far = lambda n: torch.zeros((2 ** 31 + 4096,), dtype=torch.bfloat16, device="cuda").as_strided((3, n), (2 ** 30 + 64, 1))
@@ -173,8 +173,8 @@ def test_rows_farther_apart_than_32_bits_reach(tile):
 
 
 def test_many_rows():
-    check(index_of(5000, 30), *make(5000, 30, 256, 32, (128, 64), "f16", out="16"), 64)
-    check(index_of(5000, 30), *make(5000, 30, 256, 32, (128, 64), "bf16"), 64)
+    check(index_of(5000, 30), *make(5000, 30, 256, 32, (128, 64), "f16", out="16"), 128)
+    check(index_of(5000, 30), *make(5000, 30, 256, 32, (128, 64), "bf16"), 128)
     check(index_of(5000, 1024), *make(5000, 1024, 128, 16, (64,), "f16"), 16)
 
 
