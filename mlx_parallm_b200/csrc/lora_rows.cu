@@ -361,29 +361,25 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
 // 16-byte copies into tiles of 64 of K, z = x A^T grows in TMEM, meets the other CTAs' and becomes the operand of the second product, whose blocks of 64 columns
 // take b along with the old y; y grows in its place in shared memory and leaves by whole lines while the next block's product runs.
 // RK: ranks of all targets, filled up to 32, 64, 128 or 256.  8000 rows of rank 64, 4096 to 5120: LPFIG.
-constexpr int LP_ROWS = 128, LP_COLS = 64, LP_TARGETS = 3, LP_STAGES_C = 4;
+constexpr int LP_ROWS = 128, LP_COLS = 64, LP_TARGETS = 3, LP_STAGES_B = 4, LP_STAGES_Y = 5, LP_THREADS = LW_THREADS + 128;
 template <int RK>
 struct LpShape {
   static constexpr int STAGE_A = (LP_ROWS + RK) * 128, STAGES_A = RK == 256 ? 4 : 6, TMEM = RK == 256 ? 256 : 128;
-  static constexpr int B_BYTES = LP_COLS * 128, Y_PITCH = LP_COLS * 2 + 16, STAGE_C = B_BYTES + LP_ROWS * Y_PITCH;
+  static constexpr int B_BYTES = LP_COLS * 128, Y_PITCH = LP_COLS * 2 + 16, Y_BYTES = LP_ROWS * Y_PITCH;
   static constexpr int Z_TILE = LP_ROWS * 128;                    // of one part of a target's z: 64 ranks a line
   static __host__ __device__ constexpr int z_pitch(int TR) { return TR + 4; }      // floats; a row per thread without conflicts
   static __host__ __device__ constexpr int front(int TR) {
-    const int z = LP_ROWS * z_pitch(TR) * 4, c = LP_STAGES_C * STAGE_C;
+    const int z = LP_ROWS * z_pitch(TR) * 4, c = LP_STAGES_B * B_BYTES + LP_STAGES_Y * Y_BYTES;
     return ((z > c ? z : c) + 1023) / 1024 * 1024;
   }
   static __host__ __device__ constexpr int bytes(int TR, int targets) {
     const int a = STAGES_A * STAGE_A, c = front(TR) + 2 * targets * Z_TILE;
     return 1024 + (a > c ? a : c);
   }
-  static_assert(STAGE_C % 1024 == 0 && STAGE_A % 1024 == 0, "tiles at whole swizzles");
+  static_assert(B_BYTES % 1024 == 0 && STAGE_A % 1024 == 0, "tiles at whole swizzles");
 };
 
 __device__ __forceinline__ void lp_copy(uint32_t dst, const void* src, bool valid) { cp_async16(dst, src, valid); }
-__device__ __forceinline__ void lp_copy8(uint32_t dst, const void* src, bool valid) {
-  const int size = valid ? 8 : 0;                                 // zeros where there is nothing
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
-}
 __device__ __forceinline__ void lp_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n"
@@ -406,7 +402,7 @@ __device__ __forceinline__ void lp_tmem_ld32(uint32_t taddr, float* v) {
 }
 
 struct LpBarriers {
-  uint64_t step[6], block[2];                                     // a stage's products, a block's
+  uint64_t step[6], block[2], read[2];                            // a stage's products, a block's; its results are read
   uint32_t tmem;
   volatile int abort;
 };
@@ -414,7 +410,7 @@ struct LpBarriers {
 // A wait that gives up is reported and everything goes on (the other waits then give up at once): the threads keep meeting at the CTA's and the cluster's
 // barriers, and only the numbers are wrong.
 template <typename T, int RK>
-__global__ void __launch_bounds__(LW_THREADS, 1)
+__global__ void __launch_bounds__(LP_THREADS, 1)
 lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   using S = LpShape<RK>;
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -439,13 +435,12 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   if ((int)threadIdx.x < LP_ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 6; ++i) mbar_init(smem_u32(&s_bar.step[i]), 1);
-    mbar_init(smem_u32(&s_bar.block[0]), 1);
-    mbar_init(smem_u32(&s_bar.block[1]), 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&s_bar.block[i]), 1); mbar_init(smem_u32(&s_bar.read[i]), LW_WARPS); }
     s_bar.abort = 0;
     fence_barrier_init();
   }
   // (behind the wait: an older launch on this SM takes its TMEM first)
-  if (warp == 0) tmem_alloc(smem_u32(&s_bar.tmem), S::TMEM);
+  if (warp == LW_WARPS) tmem_alloc(smem_u32(&s_bar.tmem), S::TMEM);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -456,15 +451,16 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   const int steps = (int)((p.K + 63) / 64), k0 = (int)((int64_t)steps * rank / C), k1 = (int)((int64_t)steps * (rank + 1) / C);
   {
     const int c = threadIdx.x & 7, line = threadIdx.x >> 3;       // this thread's 16 bytes of a line of 64, and its first line
+    const bool copies = warp < LW_WARPS;                          // the warp behind them issues the products
     const T* xr[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = s_row[line + 32 * i];
+      const int row = copies ? s_row[line + 32 * i] : -1;
       xr[i] = row < 0 ? nullptr : reinterpret_cast<const T*>(p.x) + (int64_t)row * p.ldx + 8 * c;
     }
     const T* ar = reinterpret_cast<const T*>(p.a) + ((int64_t)tile.x * TR + line) * p.K + 8 * c;
     auto issue = [&](int s) {
-      if (s < k1) {
+      if (copies && s < k1) {
         const uint32_t at = s0 + (uint32_t)((s - k0) % S::STAGES_A) * S::STAGE_A + ((c ^ (line & 7)) << 4);
         const bool in = s * 64 + 8 * c < p.K;
 #pragma unroll
@@ -487,7 +483,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
       cp_async_wait<S::STAGES_A - 2>();
       fence_proxy_async_smem();                                   // this thread's copies, for the products
       __syncthreads();
-      if (warp == 0 && elect_one()) {
+      if (warp == LW_WARPS && elect_one()) {
         const uint32_t xs = s0 + (uint32_t)(n % S::STAGES_A) * S::STAGE_A;
         const uint64_t ad = make_desc_sw128(xs), bd = make_desc_sw128(xs + LP_ROWS * 128);
 #pragma unroll
@@ -504,7 +500,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
     __syncthreads();                                              // the stages are nobody's any more
     // a thread per row and every other 32 ranks
     const int row = 32 * (warp & 3) + lane;
-    for (int r = 32 * (warp >> 2); r < TR; r += 64) {
+    for (int r = 32 * (warp >> 2); copies && r < TR; r += 64) {
       float z[32];
       if (k1 > k0) {
         lp_tmem_ld32(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + r, z);
@@ -523,13 +519,13 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   else __syncthreads();
 
   // ---- z of all CTAs, as two 16-bit numbers: a thread per row and target ----------------------------------------------------------
-  for (int i = threadIdx.x; i < LP_ROWS * p.targets; i += LW_THREADS) {
+  for (int i = threadIdx.x; i < LP_ROWS * p.targets && warp < LW_WARPS; i += LW_THREADS) {
     const int row = i & (LP_ROWS - 1), target = i / LP_ROWS, at = row * zp + target * p.R;
     float z[LW_RANK];
 #pragma unroll
     for (int k = 0; k < LW_RANK; ++k) z[k] = 0.f;
     for (int r = 0; r < C; ++r) {                                 // in one order everywhere
-      const float* other = C > 1 ? cluster.map_shared_rank(s_z, r) + at : s_z + at;
+      const float* other = (r == rank ? s_z : cluster.map_shared_rank(s_z, r)) + at;
 #pragma unroll
       for (int k = 0; k < LW_RANK; k += 4)
         if (k < p.R) {
@@ -576,107 +572,130 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
     x.col += LP_COLS;
     if (x.col >= x.width && x.target + 1 < p.targets) ++x.target, x.col = 0, x.width = p.start[x.target + 1] - p.start[x.target];
   };
-  Place ahead{0, 0, p.start[1]};
+  Place ahead{0, 0, p.start[1]};                                  // the next block to fetch
   for (int k = 0; k < b0; ++k) step(ahead);
-  Place here = ahead, issued = ahead;                             // the next block to fetch, to store, to multiply
-  const int per = p.R / 8, pieces = LP_COLS * per;                // 16-byte pieces of a line of b, and of a block: they lie in a row
-  constexpr int BP = LP_COLS * LW_RANK / 8 / LW_THREADS, YP = LP_ROWS * 16 / LW_THREADS;
-  uint32_t b_to[BP];                                              // where this thread's pieces of b go
+  Place here = ahead;
+  if (warp >= LW_WARPS) {
+    // b, by four warps (one alone took 1500 cycles a block for its copies), and the products, by one of their threads
+    constexpr int BP = LP_COLS * LW_RANK / 8 / 128;
+    const int per = p.R / 8, pieces = LP_COLS * per;              // 16-byte pieces of a line of b, and of a block: they lie in a row
+    uint32_t to[BP];                                              // where this thread's go
 #pragma unroll
-  for (int k = 0; k < BP; ++k) {
-    const int x = threadIdx.x + k * LW_THREADS, n = x / per, c = x - n * per;
-    b_to[k] = (uint32_t)(n * 128 + ((c ^ (n & 7)) << 4));
-  }
-  const int c4 = 4 * (threadIdx.x & 15), line = threadIdx.x >> 4;  // its four columns of y, in rows `line`, `line` + 16 and so on
-  auto y_of = [&](int k) { return s_row[line + k * (LW_THREADS / 16)]; };
-  auto issue = [&](int block) {
-    if (block < b1) {
-      const uint32_t bs = s0 + (uint32_t)((block - b0) % LP_STAGES_C) * S::STAGE_C, ys = bs + S::B_BYTES;
-      const T* from = b + (int64_t)(p.start[ahead.target] + ahead.col) * p.R;
-      const int some = min(pieces, (ahead.width - ahead.col) * per);
-#pragma unroll
-      for (int k = 0; k < BP; ++k) {
-        const int x = threadIdx.x + k * LW_THREADS;
-        if (x < pieces) lp_copy(bs + b_to[k], from + (x < some ? 8 * x : 0), x < some);
-      }
-      const T* y = reinterpret_cast<const T*>(p.y) + p.col0[ahead.target] + ahead.col + c4;
-      const bool in = ahead.col + c4 < ahead.width;
-#pragma unroll
-      for (int k = 0; k < YP; ++k) {
-        const int row = y_of(k);
-        const bool ok = in && row >= 0;
-        lp_copy8(ys + (line + k * (LW_THREADS / 16)) * S::Y_PITCH + c4 * 2, ok ? y + (int64_t)row * p.ldy : reinterpret_cast<const T*>(p.y), ok);
-      }
-      step(ahead);
+    for (int k = 0; k < BP; ++k) {
+      const int x = (int)threadIdx.x - LW_THREADS + 128 * k, n = x / per, c = x - n * per;
+      to[k] = (uint32_t)(n * 128 + ((c ^ (n & 7)) << 4));
     }
-    cp_async_commit();
-  };
-  auto multiply = [&](int block) {                                // by one thread
-    const int n = block - b0;
-    const uint64_t bd = make_desc_sw128(s0 + (uint32_t)(n % LP_STAGES_C) * S::STAGE_C);
-    for (int part = 0; part < 2; ++part) {
-      const uint64_t ad = make_desc_sw128(zop + (uint32_t)(part * p.targets + issued.target) * S::Z_TILE);
+    auto issue = [&](int block) {
+      if (block < b1) {
+        const uint32_t bs = s0 + (uint32_t)((block - b0) % LP_STAGES_B) * S::B_BYTES;
+        const T* from = b + (int64_t)(p.start[ahead.target] + ahead.col) * p.R;
+        const int some = min(pieces, (ahead.width - ahead.col) * per);
 #pragma unroll
-      for (int k = 0; k < LW_RANK / 16; ++k)
-        if (16 * k < p.R) lp_mma(tmem + LP_COLS * (n & 1), ad + 2 * k, bd + 2 * k, idesc_y, part || k ? 1u : 0u);
-    }
-    umma_commit(smem_u32(&s_bar.block[n & 1]));
-  };
-  for (int s = 0; s < LP_STAGES_C - 1; ++s) issue(b0 + s);
+        for (int k = 0; k < BP; ++k) {
+          const int x = (int)threadIdx.x - LW_THREADS + 128 * k;
+          if (x < pieces) lp_copy(bs + to[k], from + (x < some ? 8 * x : 0), x < some);
+        }
+        step(ahead);
+      }
+      cp_async_commit();
+    };
+    for (int s = 0; s < LP_STAGES_B - 1; ++s) issue(b0 + s);
 #pragma unroll 1
-  for (int block = b0 - 1; block < b1; ++block) {
-    // block + 1 is here (of what is under way it is the last but one, or older); all are done with block - 1
-    cp_async_wait<LP_STAGES_C - 3>();
-    fence_proxy_async_smem();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (block + 1 < b1) {
-      if (warp == 0 && elect_one()) multiply(block + 1);
-      __syncwarp();
-      step(issued);
+    for (int block = b0; block < b1; ++block) {
+      const int n = block - b0;
+      cp_async_wait<LP_STAGES_B - 2>();
+      fence_proxy_async_smem();                                   // this thread's copies, for the products
+      named_bar_sync(3, 128);
+      if (warp == LW_WARPS) {
+        if (n >= 2) wait(s_bar.read[n & 1], (uint32_t)((n >> 1) - 1) & 1u, 9);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t bd = make_desc_sw128(s0 + (uint32_t)(n % LP_STAGES_B) * S::B_BYTES);
+          for (int part = 0; part < 2; ++part) {
+            const uint64_t ad = make_desc_sw128(zop + (uint32_t)(part * p.targets + here.target) * S::Z_TILE);
+#pragma unroll
+            for (int k = 0; k < LW_RANK / 16; ++k)
+              if (16 * k < p.R) lp_mma(tmem + LP_COLS * (n & 1), ad + 2 * k, bd + 2 * k, idesc_y, part || k ? 1u : 0u);
+          }
+          umma_commit(smem_u32(&s_bar.block[n & 1]));
+        }
+        __syncwarp();
+      }
+      step(here);
+      if (n >= 1) wait(s_bar.block[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u, 9);      // its stage is the one that is filled now
+      issue(block + LP_STAGES_B - 1);
     }
-    if (block < b0) continue;
-    issue(block + LP_STAGES_C - 1);
-    const int n = block - b0;
-    wait(s_bar.block[n & 1], (uint32_t)(n >> 1) & 1u, 9);
-    tc_fence_after();
-    uint8_t* ys = base + (size_t)(n % LP_STAGES_C) * S::STAGE_C + S::B_BYTES;
-    {
+  } else {
+    // y.  The thread that copies eight of its columns into a stage is the one that stores them, so a stage is filled again without a meeting.
+    constexpr int YP = LP_ROWS * 8 / LW_THREADS, YL = LW_THREADS / 8;
+    const uint32_t y0 = s0 + LP_STAGES_B * S::B_BYTES;
+    const int c8 = 8 * (threadIdx.x & 7), line = threadIdx.x >> 3;       // eight columns, in rows `line`, `line` + 32 and so on
+    const int at = line * S::Y_PITCH + c8 * 2;
+    T* y_row[YP];
+#pragma unroll
+    for (int k = 0; k < YP; ++k) {
+      const int row = s_row[line + k * YL];
+      y_row[k] = row < 0 ? nullptr : reinterpret_cast<T*>(p.y) + (int64_t)row * p.ldy + c8;
+    }
+    auto issue = [&](int block, int stage) {
+      if (block < b1) {
+        const int64_t col = p.col0[ahead.target] + ahead.col;
+        const bool in = ahead.col + c8 < ahead.width;
+#pragma unroll
+        for (int k = 0; k < YP; ++k) {
+          const bool ok = in && y_row[k];
+          lp_copy(y0 + stage * S::Y_BYTES + at + k * YL * S::Y_PITCH, ok ? y_row[k] + col : reinterpret_cast<const T*>(p.y), ok);
+        }
+        step(ahead);
+      }
+      cp_async_commit();
+    };
+    for (int s = 0; s < LP_STAGES_Y; ++s) issue(b0 + s, s);
+    int stage = 0;
+#pragma unroll 1
+    for (int block = b0; block < b1; ++block) {
+      const int n = block - b0;
+      cp_async_wait<LP_STAGES_Y - 1>();
+      named_bar_sync(1, LW_THREADS);
+      wait(s_bar.block[n & 1], (uint32_t)(n >> 1) & 1u, 9);
+      tc_fence_after();
+      uint8_t* ys = base + LP_STAGES_B * S::B_BYTES + (size_t)stage * S::Y_BYTES;
       const int row = 32 * (warp & 3) + lane, c0 = 32 * (warp >> 2);
       float d[32];
       lp_tmem_ld32(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + LP_COLS * (n & 1) + c0, d);
       tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s_bar.read[n & 1]));
       const float f = s_factor[here.target][row];
-      uint4* y = reinterpret_cast<uint4*>(ys + row * S::Y_PITCH + c0 * 2);
+      uint4* mine = reinterpret_cast<uint4*>(ys + row * S::Y_PITCH + c0 * 2);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        uint4 v = y[k];
+        const uint4 v = mine[k];
         const T* e = reinterpret_cast<const T*>(&v);
         const float* x = d + 8 * k;
-        v = make_uint4(pack2<T>(fmaf(f, x[0], Tr<T>::to_f(e[0])), fmaf(f, x[1], Tr<T>::to_f(e[1]))),
-                       pack2<T>(fmaf(f, x[2], Tr<T>::to_f(e[2])), fmaf(f, x[3], Tr<T>::to_f(e[3]))),
-                       pack2<T>(fmaf(f, x[4], Tr<T>::to_f(e[4])), fmaf(f, x[5], Tr<T>::to_f(e[5]))),
-                       pack2<T>(fmaf(f, x[6], Tr<T>::to_f(e[6])), fmaf(f, x[7], Tr<T>::to_f(e[7]))));
-        y[k] = v;
+        mine[k] = make_uint4(pack2<T>(fmaf(f, x[0], Tr<T>::to_f(e[0])), fmaf(f, x[1], Tr<T>::to_f(e[1]))),
+                             pack2<T>(fmaf(f, x[2], Tr<T>::to_f(e[2])), fmaf(f, x[3], Tr<T>::to_f(e[3]))),
+                             pack2<T>(fmaf(f, x[4], Tr<T>::to_f(e[4])), fmaf(f, x[5], Tr<T>::to_f(e[5]))),
+                             pack2<T>(fmaf(f, x[6], Tr<T>::to_f(e[6])), fmaf(f, x[7], Tr<T>::to_f(e[7]))));
       }
-    }
-    __syncthreads();
-    T* y = reinterpret_cast<T*>(p.y) + p.col0[here.target] + here.col + c4;
-    if (here.col + c4 < here.width) {
+      named_bar_sync(2, LW_THREADS);
+      if (here.col + c8 < here.width) {
+        const int64_t col = p.col0[here.target] + here.col;
 #pragma unroll
-      for (int k = 0; k < YP; ++k) {
-        const int row = y_of(k);
-        if (row >= 0) *reinterpret_cast<uint2*>(y + (int64_t)row * p.ldy) = *reinterpret_cast<const uint2*>(ys + (line + k * (LW_THREADS / 16)) * S::Y_PITCH + c4 * 2);
+        for (int k = 0; k < YP; ++k)
+          if (y_row[k]) *reinterpret_cast<uint4*>(y_row[k] + col) = *reinterpret_cast<const uint4*>(ys + at + k * YL * S::Y_PITCH);
       }
+      step(here);
+      issue(block + LP_STAGES_Y, stage);
+      stage = stage + 1 == LP_STAGES_Y ? 0 : stage + 1;
     }
-    step(here);
   }
   cp_async_wait<0>();
   if (s_bar.abort) wait_settle();
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == LW_WARPS) {
     tc_fence_after();
     tmem_dealloc(tmem, S::TMEM);
   }
@@ -684,7 +703,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
 
 // Clusters of up to C CTAs, as many as fit the GPU.  (us, 64 rows of 64 adapters in clusters of 1 / 2 / 4 / 8: 20.6 / 13.6 / 11.6 / 17.2; 1 row 19.8 / 12.6 / 8.7 /
 // 7.0.)
-static int launch_lora(void (*kern)(LoraRows), int most_bytes, int bytes, int C, int per_sm, std::atomic<uint64_t>& ready, const LoraRows& p, int64_t tiles,
+static int launch_lora(void (*kern)(LoraRows), int threads, int most_bytes, int bytes, int C, int per_sm, std::atomic<uint64_t>& ready, const LoraRows& p, int64_t tiles,
                        cudaStream_t st) {
   int dev = 0;
   cudaError_t ae = cudaGetDevice(&dev);
@@ -696,7 +715,7 @@ static int launch_lora(void (*kern)(LoraRows), int most_bytes, int bytes, int C,
   while (C > 1 && tiles * C > (int64_t)per_sm * sm_count()) C >>= 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C));
-  cfg.blockDim = dim3(LW_THREADS);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -715,7 +734,7 @@ template <typename T, typename YT, int KS>
 static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   const int TR = p.targets * p.R, ranks = TR > 128 ? 256 : TR > 64 ? 128 : TR > 32 ? 64 : 32;
-  return launch_lora(lora_rows_kernel<T, YT, KS>, lw_row_floats<T, YT>(LW_RANKS) * 16 * 4, lw_row_floats<T, YT>(ranks) * 16 * 4, LW_CLUSTER, 2, ready, p,
+  return launch_lora(lora_rows_kernel<T, YT, KS>, LW_THREADS, lw_row_floats<T, YT>(LW_RANKS) * 16 * 4, lw_row_floats<T, YT>(ranks) * 16 * 4, LW_CLUSTER, 2, ready, p,
                      tiles * p.sub, st);
 }
 
@@ -724,21 +743,23 @@ static int launch_lora_prompt(LoraRows p, int64_t tiles, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   if (const int rc = wait_word(WAIT_GEMM_TC, &p.wait_word)) return rc;
   const int most = RK < LW_RANK * LP_TARGETS ? RK : LW_RANK * LP_TARGETS;
-  return launch_lora(lora_prompt_kernel<T, RK>, LpShape<RK>::bytes(most, LP_TARGETS), LpShape<RK>::bytes(p.targets * p.R, p.targets), 4, 1, ready, p, tiles, st);
+  return launch_lora(lora_prompt_kernel<T, RK>, LP_THREADS, LpShape<RK>::bytes(most, LP_TARGETS), LpShape<RK>::bytes(p.targets * p.R, p.targets), 4, 1, ready, p, tiles, st);
 }
 
 template <typename T, typename YT>
 static int launch_lora_tiles(LoraRows p, int tile, int64_t tiles, cudaStream_t st) {
   const int TR = p.targets * p.R;
   if constexpr (sizeof(YT) == 2) {
-    if (tile == LP_ROWS && p.targets <= LP_TARGETS) {
+    bool whole = aligned(p.y, 16) && p.ldy % 8 == 0;                // y by 16 bytes
+    for (int k = 0; k < p.targets; ++k) whole = whole && p.col0[k] % 8 == 0;
+    if (tile == LP_ROWS && p.targets <= LP_TARGETS && whole) {
       if (TR > 128) return launch_lora_prompt<T, 256>(p, tiles, st);
       if (TR > 64) return launch_lora_prompt<T, 128>(p, tiles, st);
       if (TR > 32) return launch_lora_prompt<T, 64>(p, tiles, st);
       return launch_lora_prompt<T, 32>(p, tiles, st);
     }
   }
-  p.sub = tile / 16;                                                // (fp32 y and four targets: tiles of 16 rows of the plan's)
+  p.sub = tile / 16;                                                // (fp32 y, four targets, y by 8 bytes: tiles of 16 rows of the plan's)
   if (p.R == 16) return launch_lora_rows<T, YT, 1>(p, tiles, st);
   if (p.R == 32) return launch_lora_rows<T, YT, 2>(p, tiles, st);
   return launch_lora_rows<T, YT, 4>(p, tiles, st);
