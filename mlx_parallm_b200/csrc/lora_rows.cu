@@ -358,18 +358,19 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
 }
 
 // Tiles of 128 rows on tcgen05: prompts with 16-bit y and up to three targets.  The same steps, one CTA per SM: rows of x (wherever they lie) and of A come by
-// 16-byte copies into tiles of 64 of K, z = x A^T grows in TMEM, meets the other CTAs' and becomes the operand of the second product, whose blocks of 64 columns
-// take b along with the old y; y grows in its place in shared memory and leaves by whole lines while the next block's product runs.
-// RK: ranks of all targets, filled up to 32, 64, 128 or 256.  8000 rows of rank 64, 4096 to 5120: LPFIG.
-constexpr int LP_ROWS = 128, LP_COLS = 64, LP_TARGETS = 3, LP_STAGES_B = 4, LP_STAGES_Y = 5, LP_THREADS = LW_THREADS + 128;
-template <int RK>
+// 16-byte copies into tiles of 64 of K, z = x A^T grows in TMEM, meets the other CTAs' and becomes the operand of the second product, whose blocks of 64 or
+// 128 columns take b along with the old y; y grows in its place in shared memory and leaves by whole lines while the next block's product runs.
+// RK: ranks of all targets, filled up to 32, 64, 128 or 256.  8000 rows of rank 64, 4096 to 5120: 56 us of 31.
+constexpr int LP_ROWS = 128, LP_TARGETS = 3, LP_THREADS = LW_THREADS + 128;
+template <int RK, int COLS>
 struct LpShape {
-  static constexpr int STAGE_A = (LP_ROWS + RK) * 128, STAGES_A = RK == 256 ? 4 : 6, TMEM = RK == 256 ? 256 : 128;
-  static constexpr int B_BYTES = LP_COLS * 128, Y_PITCH = LP_COLS * 2 + 16, Y_BYTES = LP_ROWS * Y_PITCH;
+  static constexpr int STAGES_B = COLS == 128 ? 3 : 4, STAGES_Y = COLS == 128 ? 3 : 5;
+  static constexpr int STAGE_A = (LP_ROWS + RK) * 128, STAGES_A = RK == 256 ? 4 : 6, TMEM = RK == 256 || COLS == 128 ? 256 : 128;
+  static constexpr int B_BYTES = COLS * 128, Y_PITCH = COLS * 2 + 16, Y_BYTES = LP_ROWS * Y_PITCH;
   static constexpr int Z_TILE = LP_ROWS * 128;                    // of one part of a target's z: 64 ranks a line
   static __host__ __device__ constexpr int z_pitch(int TR) { return TR + 4; }      // floats; a row per thread without conflicts
   static __host__ __device__ constexpr int front(int TR) {
-    const int z = LP_ROWS * z_pitch(TR) * 4, c = LP_STAGES_B * B_BYTES + LP_STAGES_Y * Y_BYTES;
+    const int z = LP_ROWS * z_pitch(TR) * 4, c = STAGES_B * B_BYTES + STAGES_Y * Y_BYTES;
     return ((z > c ? z : c) + 1023) / 1024 * 1024;
   }
   static __host__ __device__ constexpr int bytes(int TR, int targets) {
@@ -409,13 +410,13 @@ struct LpBarriers {
 
 // A wait that gives up is reported and everything goes on (the other waits then give up at once): the threads keep meeting at the CTA's and the cluster's
 // barriers, and only the numbers are wrong.
-template <typename T, int RK>
+template <typename T, int RK, int COLS>
 __global__ void __launch_bounds__(LP_THREADS, 1)
 lora_prompt_kernel(const __grid_constant__ LoraRows p) {
-  using S = LpShape<RK>;
+  using S = LpShape<RK, COLS>;
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);      // D fp32, 128 rows, K-major operands; N below
-  constexpr uint32_t idesc_z = idesc | ((uint32_t)(RK >> 3) << 17), idesc_y = idesc | ((uint32_t)(LP_COLS >> 3) << 17);
+  constexpr uint32_t idesc_z = idesc | ((uint32_t)(RK >> 3) << 17), idesc_y = idesc | ((uint32_t)(COLS >> 3) << 17);
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int s_row[LP_ROWS];
   __shared__ float s_factor[LP_TARGETS][LP_ROWS];
@@ -518,41 +519,33 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   if (C > 1) cluster.sync();
   else __syncthreads();
 
-  // ---- z of all CTAs, as two 16-bit numbers: a thread per row and target ----------------------------------------------------------
-  for (int i = threadIdx.x; i < LP_ROWS * p.targets && warp < LW_WARPS; i += LW_THREADS) {
-    const int row = i & (LP_ROWS - 1), target = i / LP_ROWS, at = row * zp + target * p.R;
-    float z[LW_RANK];
+  // ---- z of all CTAs, as two 16-bit numbers: 16 lanes per row and target, four ranks each (a thread per row reads the other CTAs' memory by single sectors:
+  // 15 000 cycles instead of 10 900) -----------------------------------------------------------------------------------------------
+  if (warp < LW_WARPS) {
+    const int l = threadIdx.x & 15, k = 4 * l;
+#pragma unroll 4
+    for (int i = threadIdx.x >> 4; i < LP_ROWS * p.targets; i += LW_THREADS / 16) {
+      const int row = i & (LP_ROWS - 1), target = i / LP_ROWS, at = row * zp + target * p.R + k;
+      float4 z = make_float4(0.f, 0.f, 0.f, 0.f), v[4];
 #pragma unroll
-    for (int k = 0; k < LW_RANK; ++k) z[k] = 0.f;
-    for (int r = 0; r < C; ++r) {                                 // in one order everywhere
-      const float* other = (r == rank ? s_z : cluster.map_shared_rank(s_z, r)) + at;
+      for (int r = 0; r < 4; ++r)
+        v[r] = r < C && k < p.R ? *reinterpret_cast<const float4*>((r == rank ? s_z : cluster.map_shared_rank(s_z, r)) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < LW_RANK; k += 4)
-        if (k < p.R) {
-          const float4 v = *reinterpret_cast<const float4*>(other + k);
-          z[k] += v.x, z[k + 1] += v.y, z[k + 2] += v.z, z[k + 3] += v.w;
-        }
+      for (int r = 0; r < 4; ++r) z.x += v[r].x, z.y += v[r].y, z.z += v[r].z, z.w += v[r].w;      // in one order everywhere
+      float top = fmaxf(fmaxf(fabsf(z.x), fabsf(z.y)), fmaxf(fabsf(z.z), fabsf(z.w))), up, down;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+      lw_scale(top, up, down);
+      if (l == 0) s_factor[target][row] = up * p.scales[tile.x];
+      if (k >= p.R) continue;
+      z.x *= down, z.y *= down, z.z *= down, z.w *= down;
+      auto rest = [](float x) { return x - Tr<T>::to_f(Tr<T>::from_f(x)); };
+      const uint32_t to = zop + (uint32_t)target * S::Z_TILE + row * 128 + (((k >> 3) ^ (row & 7)) << 4) + (k & 4) * 2;
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(pack2<T>(z.x, z.y)), "r"(pack2<T>(z.z, z.w)) : "memory");
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + (uint32_t)p.targets * S::Z_TILE), "r"(pack2<T>(rest(z.x), rest(z.y))),
+                   "r"(pack2<T>(rest(z.z), rest(z.w)))
+                   : "memory");
     }
-    float top = 0.f, up, down;
-#pragma unroll
-    for (int k = 0; k < LW_RANK; ++k) top = fmaxf(top, fabsf(z[k]));
-    lw_scale(top, up, down);
-    s_factor[target][row] = up * p.scales[tile.x];
-#pragma unroll
-    for (int k = 0; k < LW_RANK; k += 8)
-      if (k < p.R) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = z[k + 2 * e] * down, y = z[k + 2 * e + 1] * down;
-          const T hx = Tr<T>::from_f(x), hy = Tr<T>::from_f(y);
-          hi[e] = pack2<T>(x, y);
-          lo[e] = pack2<T>(x - Tr<T>::to_f(hx), y - Tr<T>::to_f(hy));
-        }
-        const uint32_t to = zop + (uint32_t)target * S::Z_TILE + row * 128 + (((k >> 3) ^ (row & 7)) << 4);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (uint32_t)p.targets * S::Z_TILE), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
-      }
   }
   fence_proxy_async_smem();
   if (C > 1) cluster.sync();                                      // all have read: the stages may lie there again
@@ -563,13 +556,13 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   // ---- this CTA's columns -------------------------------------------------------------------------------------------------------
   const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.x * p.N * p.R;
   int blocks = 0;
-  for (int k = 0; k < p.targets; ++k) blocks += (p.start[k + 1] - p.start[k] + LP_COLS - 1) / LP_COLS;
+  for (int k = 0; k < p.targets; ++k) blocks += (p.start[k + 1] - p.start[k] + COLS - 1) / COLS;
   const int b0 = (int)((int64_t)blocks * rank / C), b1 = (int)((int64_t)blocks * (rank + 1) / C);
   struct Place {                                                  // of a block: its target and first column in it
     int target, col, width;
   };
   auto step = [&](Place& x) {
-    x.col += LP_COLS;
+    x.col += COLS;
     if (x.col >= x.width && x.target + 1 < p.targets) ++x.target, x.col = 0, x.width = p.start[x.target + 1] - p.start[x.target];
   };
   Place ahead{0, 0, p.start[1]};                                  // the next block to fetch
@@ -577,8 +570,8 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   Place here = ahead;
   if (warp >= LW_WARPS) {
     // b, by four warps (one alone took 1500 cycles a block for its copies), and the products, by one of their threads
-    constexpr int BP = LP_COLS * LW_RANK / 8 / 128;
-    const int per = p.R / 8, pieces = LP_COLS * per;              // 16-byte pieces of a line of b, and of a block: they lie in a row
+    constexpr int BP = COLS * LW_RANK / 8 / 128;
+    const int per = p.R / 8, pieces = COLS * per;              // 16-byte pieces of a line of b, and of a block: they lie in a row
     uint32_t to[BP];                                              // where this thread's go
 #pragma unroll
     for (int k = 0; k < BP; ++k) {
@@ -587,7 +580,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
     }
     auto issue = [&](int block) {
       if (block < b1) {
-        const uint32_t bs = s0 + (uint32_t)((block - b0) % LP_STAGES_B) * S::B_BYTES;
+        const uint32_t bs = s0 + (uint32_t)((block - b0) % S::STAGES_B) * S::B_BYTES;
         const T* from = b + (int64_t)(p.start[ahead.target] + ahead.col) * p.R;
         const int some = min(pieces, (ahead.width - ahead.col) * per);
 #pragma unroll
@@ -599,23 +592,23 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
       }
       cp_async_commit();
     };
-    for (int s = 0; s < LP_STAGES_B - 1; ++s) issue(b0 + s);
+    for (int s = 0; s < S::STAGES_B - 1; ++s) issue(b0 + s);
 #pragma unroll 1
     for (int block = b0; block < b1; ++block) {
       const int n = block - b0;
-      cp_async_wait<LP_STAGES_B - 2>();
+      cp_async_wait<S::STAGES_B - 2>();
       fence_proxy_async_smem();                                   // this thread's copies, for the products
       named_bar_sync(3, 128);
       if (warp == LW_WARPS) {
         if (n >= 2) wait(s_bar.read[n & 1], (uint32_t)((n >> 1) - 1) & 1u, 9);
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t bd = make_desc_sw128(s0 + (uint32_t)(n % LP_STAGES_B) * S::B_BYTES);
+          const uint64_t bd = make_desc_sw128(s0 + (uint32_t)(n % S::STAGES_B) * S::B_BYTES);
           for (int part = 0; part < 2; ++part) {
             const uint64_t ad = make_desc_sw128(zop + (uint32_t)(part * p.targets + here.target) * S::Z_TILE);
 #pragma unroll
             for (int k = 0; k < LW_RANK / 16; ++k)
-              if (16 * k < p.R) lp_mma(tmem + LP_COLS * (n & 1), ad + 2 * k, bd + 2 * k, idesc_y, part || k ? 1u : 0u);
+              if (16 * k < p.R) lp_mma(tmem + COLS * (n & 1), ad + 2 * k, bd + 2 * k, idesc_y, part || k ? 1u : 0u);
           }
           umma_commit(smem_u32(&s_bar.block[n & 1]));
         }
@@ -623,18 +616,18 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
       }
       step(here);
       if (n >= 1) wait(s_bar.block[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u, 9);      // its stage is the one that is filled now
-      issue(block + LP_STAGES_B - 1);
+      issue(block + S::STAGES_B - 1);
     }
   } else {
-    // y.  The thread that copies eight of its columns into a stage is the one that stores them, so a stage is filled again without a meeting.
-    constexpr int YP = LP_ROWS * 8 / LW_THREADS, YL = LW_THREADS / 8;
-    const uint32_t y0 = s0 + LP_STAGES_B * S::B_BYTES;
-    const int c8 = 8 * (threadIdx.x & 7), line = threadIdx.x >> 3;       // eight columns, in rows `line`, `line` + 32 and so on
-    const int at = line * S::Y_PITCH + c8 * 2;
-    T* y_row[YP];
+    // y.  A warp has 32 rows and half of a block's columns all by itself: copies, adds and stores them, and meets nobody.
+    constexpr int CL = COLS / 16, RL = 32 / CL;                   // lanes of a row (eight columns each), rows at a time
+    const uint32_t y0 = s0 + S::STAGES_B * S::B_BYTES;
+    const int r0 = 32 * (warp & 3), c0 = COLS / 2 * (warp >> 2), c8 = c0 + 8 * (lane % CL);
+    const int at = (r0 + lane / CL) * S::Y_PITCH + c8 * 2;
+    T* y_row[CL];
 #pragma unroll
-    for (int k = 0; k < YP; ++k) {
-      const int row = s_row[line + k * YL];
+    for (int k = 0; k < CL; ++k) {
+      const int row = s_row[r0 + lane / CL + RL * k];
       y_row[k] = row < 0 ? nullptr : reinterpret_cast<T*>(p.y) + (int64_t)row * p.ldy + c8;
     }
     auto issue = [&](int block, int stage) {
@@ -642,35 +635,34 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
         const int64_t col = p.col0[ahead.target] + ahead.col;
         const bool in = ahead.col + c8 < ahead.width;
 #pragma unroll
-        for (int k = 0; k < YP; ++k) {
+        for (int k = 0; k < CL; ++k) {
           const bool ok = in && y_row[k];
-          lp_copy(y0 + stage * S::Y_BYTES + at + k * YL * S::Y_PITCH, ok ? y_row[k] + col : reinterpret_cast<const T*>(p.y), ok);
+          lp_copy(y0 + stage * S::Y_BYTES + at + RL * k * S::Y_PITCH, ok ? y_row[k] + col : reinterpret_cast<const T*>(p.y), ok);
         }
         step(ahead);
       }
       cp_async_commit();
     };
-    for (int s = 0; s < LP_STAGES_Y; ++s) issue(b0 + s, s);
+    for (int s = 0; s < S::STAGES_Y; ++s) issue(b0 + s, s);
     int stage = 0;
 #pragma unroll 1
     for (int block = b0; block < b1; ++block) {
       const int n = block - b0;
-      cp_async_wait<LP_STAGES_Y - 1>();
-      named_bar_sync(1, LW_THREADS);
       wait(s_bar.block[n & 1], (uint32_t)(n >> 1) & 1u, 9);
       tc_fence_after();
-      uint8_t* ys = base + LP_STAGES_B * S::B_BYTES + (size_t)stage * S::Y_BYTES;
-      const int row = 32 * (warp & 3) + lane, c0 = 32 * (warp >> 2);
-      float d[32];
-      lp_tmem_ld32(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + LP_COLS * (n & 1) + c0, d);
+      float d[COLS / 2];
+#pragma unroll
+      for (int k = 0; k < COLS / 2; k += 32) lp_tmem_ld32(tmem + ((uint32_t)r0 << 16) + COLS * (n & 1) + c0 + k, d + k);
+      cp_async_wait<S::STAGES_Y - 1>();
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&s_bar.read[n & 1]));
-      const float f = s_factor[here.target][row];
-      uint4* mine = reinterpret_cast<uint4*>(ys + row * S::Y_PITCH + c0 * 2);
+      uint8_t* ys = base + S::STAGES_B * S::B_BYTES + (size_t)stage * S::Y_BYTES;
+      const float f = s_factor[here.target][r0 + lane];
+      uint4* mine = reinterpret_cast<uint4*>(ys + (r0 + lane) * S::Y_PITCH + c0 * 2);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < CL; ++k) {
         const uint4 v = mine[k];
         const T* e = reinterpret_cast<const T*>(&v);
         const float* x = d + 8 * k;
@@ -679,16 +671,16 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
                              pack2<T>(fmaf(f, x[4], Tr<T>::to_f(e[4])), fmaf(f, x[5], Tr<T>::to_f(e[5]))),
                              pack2<T>(fmaf(f, x[6], Tr<T>::to_f(e[6])), fmaf(f, x[7], Tr<T>::to_f(e[7]))));
       }
-      named_bar_sync(2, LW_THREADS);
+      __syncwarp();
       if (here.col + c8 < here.width) {
         const int64_t col = p.col0[here.target] + here.col;
 #pragma unroll
-        for (int k = 0; k < YP; ++k)
-          if (y_row[k]) *reinterpret_cast<uint4*>(y_row[k] + col) = *reinterpret_cast<const uint4*>(ys + at + k * YL * S::Y_PITCH);
+        for (int k = 0; k < CL; ++k)
+          if (y_row[k]) *reinterpret_cast<uint4*>(y_row[k] + col) = *reinterpret_cast<const uint4*>(ys + at + RL * k * S::Y_PITCH);
       }
       step(here);
-      issue(block + LP_STAGES_Y, stage);
-      stage = stage + 1 == LP_STAGES_Y ? 0 : stage + 1;
+      issue(block + S::STAGES_Y, stage);                          // (a lane fills what it has stored itself)
+      stage = stage + 1 == S::STAGES_Y ? 0 : stage + 1;
     }
   }
   cp_async_wait<0>();
@@ -738,12 +730,22 @@ static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
                      tiles * p.sub, st);
 }
 
+template <typename T, int RK, int COLS>
+static int launch_lora_prompt_of(LoraRows p, int64_t tiles, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
+  using S = LpShape<RK, COLS>;
+  constexpr int TARGETS = COLS == 128 ? 2 : LP_TARGETS, MOST = RK < LW_RANK * TARGETS ? RK : LW_RANK * TARGETS;
+  static_assert(S::bytes(MOST, TARGETS) <= 224 * 1024, "beside the static shared memory");
+  return launch_lora(lora_prompt_kernel<T, RK, COLS>, LP_THREADS, S::bytes(MOST, TARGETS), S::bytes(p.targets * p.R, p.targets), 4, 1, ready, p, tiles, st);
+}
+// Blocks of 128 columns, whose products take the tensor core as long as those of 64 do; of 64 where three targets' z take their room.
 template <typename T, int RK>
 static int launch_lora_prompt(LoraRows p, int64_t tiles, cudaStream_t st) {
-  static std::atomic<uint64_t> ready{0};
   if (const int rc = wait_word(WAIT_GEMM_TC, &p.wait_word)) return rc;
-  const int most = RK < LW_RANK * LP_TARGETS ? RK : LW_RANK * LP_TARGETS;
-  return launch_lora(lora_prompt_kernel<T, RK>, LP_THREADS, LpShape<RK>::bytes(most, LP_TARGETS), LpShape<RK>::bytes(p.targets * p.R, p.targets), 4, 1, ready, p, tiles, st);
+  if constexpr (RK <= 2 * LW_RANK) {
+    if (p.targets <= 2) return launch_lora_prompt_of<T, RK, 128>(p, tiles, st);
+  }
+  return launch_lora_prompt_of<T, RK, 64>(p, tiles, st);
 }
 
 template <typename T, typename YT>
@@ -792,8 +794,9 @@ extern "C" int b200p_row_groups(const int32_t* index, int32_t* plan, int64_t M, 
   return B200P_OK;
 }
 
-// Tiles of 64 rows read an adapter a quarter as often as tiles of 16, which spread few rows over more SMs and have less to set up.  us, tiles of 16 / 64,
-// 4096 to 5120 columns, 2 adapters: 1000 rows of rank 16 17 / 26, 2000 34 / 32, 8000 115 / 66; rank 64 33 / 57, 64 / 65, 234 / 94.
+// Tiles of 128 rows read an adapter an eighth as often as tiles of 16 and put it on the tensor core, and have more to set up for few rows.  us, tiles of
+// 16 / 128, 4096 to 5120 columns: 2 adapters, 1000 rows of rank 16 17 / 30, 1500 32 / 30, 8000 116 / 53; rank 64 33 / 33, 61 / 33, 234 / 55.  64 adapters,
+// 500 rows of rank 16 20 / 41, 1500 51 / 67, 8000 118 / 80; rank 64 57 / 47, 102 / 75, 226 / 90.  (A plan is laid out once for layers of every rank.)
 extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1500 && M >= 16ll * groups ? LP_ROWS : 16; }
 
 extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a, const void* b, const float* scales, void* y, const int32_t* host_columns,

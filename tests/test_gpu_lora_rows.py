@@ -259,3 +259,12 @@ def test_refusals():
             ops.row_groups(*bad)
     with pytest.raises(ValueError):
         ops.row_groups(index, 2, 16, out=ops.row_groups(index, 3, 16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("R,targets", [(32, 1), (32, 2), (32, 3), (64, 1), (64, 2), (64, 3)])
+def test_prompt_tiles_of_higher_ranks(R, targets, dtype):
+    """Blocks of columns that end inside a target, whole tiles and parts of one, at each size of the inner product's room."""
+    columns = (264, 8, 1000)[:targets]
+    check(index_of(300, 2), *make(300, 2, 4096 if R == 64 else 136, R, columns, dtype, out="16", seed=R + targets), 128)
