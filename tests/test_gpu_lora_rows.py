@@ -261,10 +261,62 @@ def test_refusals():
         ops.row_groups(index, 2, 16, out=ops.row_groups(index, 3, 16))
 
 
-@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("R,targets", [(32, 1), (32, 2), (32, 3), (64, 1), (64, 2), (64, 3)])
 def test_prompt_tiles_of_higher_ranks(R, targets, dtype):
     """Blocks of columns that end inside a target, whole tiles and parts of one, at each size of the inner product's room."""
     columns = (264, 8, 1000)[:targets]
     check(index_of(300, 2), *make(300, 2, 4096 if R == 64 else 136, R, columns, dtype, out="16", seed=R + targets), 128)
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 300.0])
+def test_prompt_tiles_of_small_and_large_inner_values(scale):
+    x, a, b, s, columns, y = make(200, 2, 512, 32, (64, 136), "f16", out="16")
+    x, a = (x.float() * scale).half(), a * (20.0 if scale > 1 else 1.0)
+    y.zero_()
+    check(index_of(200, 2, none=False), x, a, b / 64 if scale > 1 else b, s / max(scale, 1.0), columns, y, 128)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("targets", [2, 3])
+def test_prompt_tiles_keep_what_is_not_a_number_in_its_row(value, targets):
+    x, a, b, s, columns, y = make(300, 2, 1024, 32, (264, 8, 72)[:targets], "bf16", out="16")
+    plan = ops.row_groups(index_of(300, 2, none=False).cuda(), 2, 128)
+    clean = ops.lora_rows(x, plan, a, b, s, columns, y.clone())
+    x[77, 7] = value
+    got = ops.lora_rows(x, plan, a, b, s, columns, y.clone())
+    others = torch.arange(300, device="cuda") != 77
+    assert torch.equal(got[others], clean[others])
+    assert not any(got[77, c:c + w].isfinite().any() for c, w in columns)
+
+
+@pytest.mark.parametrize("targets", [1, 3])
+def test_prompt_tiles_in_graphs_on_two_streams(targets):
+    """Two calls at once, rewritten plans, the same bits every time."""
+    x, a, b, s, columns, y = make(1700, 4, 2048, 64, (512, 256, 64)[:targets], "f16", out="16")
+    index = index_of(1700, 4).cuda()
+    plan, base, out = ops.row_groups(index, 4, 128), y.clone(), y.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out.copy_(base)
+        ops.row_groups(index, 4, 128, out=plan)
+        ops.lora_rows(x, plan, a, b, s, columns, out)
+    side = torch.cuda.Stream()
+    for seed in (1, 2):
+        index.copy_(index_of(1700, 4, seed=seed))
+        other, plans = base.clone(), ops.row_groups(index, 4, 128)
+        side.wait_stream(torch.cuda.current_stream())
+        g.replay()
+        with torch.cuda.stream(side):
+            ops.lora_rows(x, plans, a, b, s, columns, other)
+        torch.cuda.synchronize()
+        assert torch.equal(out, other) and not torch.equal(out, base)
+        ops.check_waits()
+
+
+@pytest.mark.parametrize("shift,gap", [(4, 0), (0, 4), (8, 0)])
+def test_prompt_tiles_of_y_at_odd_places(shift, gap):
+    """y whose rows or columns are no multiple of 16 bytes."""
+    x, a, b, s, columns, y = make(260, 3, 256, 16, (64, 32), "bf16", gap=gap, out="16")
+    wide = torch.randn((260, y.shape[1] + 16), device="cuda").bfloat16()
+    check(index_of(260, 3), x, a, b, s, columns, wide[:, shift:shift + y.shape[1]], 128)
