@@ -8,12 +8,22 @@
 // 2^14 and small ones keep their bits.  A weight is off by half a step of its type, at random, and their sum is that of the rounded ones: with the output's own
 // rounding 1.2 (bf16) and 1.4 (f16) times that rounding alone.
 //
-// 128 rows in two groups behind 16000 and 12032 slots, 64 / 8 heads (60 GFLOP): 62 us, 3400 cycles a step of 256 rows against 2048 of the tensor core's; of
-// 64 rows behind 4000 slots a CTA has 3.5 steps, and the plan (4000 cycles), queries (5000), first copy (1500) and the part (5000) are most of its time.
+// The weights of a step's first 64 keys are multiplied while those of the last 64 are made (128 rows behind 16000 slots 109.4 -> 106.1 us).
+//
+// 128 rows in two groups behind 16000 and 12032 slots, 64 / 8 heads (60 GFLOP): CTAs end after 57 to 77 us, 68 in the median; 3450 cycles a step of 256 rows,
+// against 2048 of the tensor core's and as many of its exponentials.  Of 64 rows behind 4000 slots a CTA has 3.5 steps, and the plan (4000 cycles), queries
+// (5000), first copy (1500) and the part (5000) are most of its time.
 #pragma once
 #include "attn_tc.cuh"
 
 namespace b200p {
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+               "r"(r[15])
+               : "memory");
+}
 
 template <typename T>
 __global__ void __launch_bounds__(FT_THREADS, 1)
@@ -21,6 +31,7 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
   constexpr float SHIFT = std::is_same<T, __half>::value ? 8.f : 0.f, LAG = 6.f;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ PrefixPlan s_plan;
+  __shared__ uint64_t s_rest[2];                            // the weights of a step's last 64 keys (sh->p_full: of its first)
   __shared__ struct { PrefixCursor<FT_KEYS, false> cursor; PrefixRun run; } s_kept[8];      // the steps' loop has no registers for them
   const uint32_t raw = smem_u32(smem);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -30,7 +41,7 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&sh->q_full), 8);
     for (int s = 0; s < FT_RING; ++s) { mbar_init(smem_u32(&sh->kv_full[s]), 1); mbar_init(smem_u32(&sh->kv_empty[s]), 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&sh->s_full[i]), 1); mbar_init(smem_u32(&sh->p_full[i]), 4); mbar_init(smem_u32(&sh->o_full[i]), 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&sh->s_full[i]), 1); mbar_init(smem_u32(&sh->p_full[i]), 4); mbar_init(smem_u32(&s_rest[i]), 4); mbar_init(smem_u32(&sh->o_full[i]), 1); }
     sh->abort = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmk);
@@ -104,10 +115,10 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
           ft_mma_ss(tmem + 128 * i, ad + off, bd + off, idesc, k ? 1u : 0u);
         }
       };
-      auto pv = [&](int i, int slot, uint32_t acc) {
+      auto pv = [&](int i, int slot, int from, uint32_t acc) {
         const uint64_t bd = ft_desc_n_major(ring + slot * FT_TILE_BYTES);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)                        // 16 keys = 2048 bytes; P: 8 columns
+        for (int k = from; k < from + 4; ++k)              // 16 keys = 2048 bytes; P: 8 columns
           umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, bd + (uint64_t)(k * (2048 >> 4)), idesc_pv, (k || acc) ? 1u : 0u);
       };
       int slot = 0, round = 0;
@@ -149,10 +160,14 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
           }
           for (int i = 0; i < both; ++i) {
             if (!(ok = wait(sh->p_full[i], pph[i], 1))) break;
+            tc_fence_after();
+            if (elect_one()) pv(i, vslot, 0, j > 0 ? 1u : 0u);
+            __syncwarp();
+            if (!(ok = wait(s_rest[i], pph[i], 1))) break;
             pph[i] ^= 1u;
             tc_fence_after();
             if (elect_one()) {
-              pv(i, vslot, j > 0 ? 1u : 0u);
+              pv(i, vslot, 4, 1u);
               if (i == both - 1) umma_commit(smem_u32(&sh->kv_empty[vslot]));
               if (more) {
                 qk(i, kslot);
@@ -252,6 +267,18 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
         const bool rescale = u > first && __any_sync(~0u, mn > m);
         m = mn;
         const float2 nm2 = make_float2(-ref, -ref);
+        if (rescale) {                                     // (beside 128 scores in registers: 16 columns at a time)
+#pragma unroll 1
+          for (int c = 0; c < FT_D; c += 16) {
+            float o[16];
+            uint32_t w[16];
+            tmem_ld16(o_addr + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * f);
+            tmem_st16(o_addr + c, w);
+          }
+        }
         float2 a0 = make_float2(0.f, 0.f), a1 = a0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -264,33 +291,12 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
             if (c & 1) a1 = __fadd2_rn(a1, e); else a0 = __fadd2_rn(a0, e);
           }
           tmem_st32(s_addr + 32 * h, w);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(h ? &s_rest[i] : &sh->p_full[i]));
         }
-        if (rescale) {
-          const float2 f2 = make_float2(f, f);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float o[2][32];
-            tmem_ld32(o_addr + 64 * h, o[0]);
-            tmem_ld32(o_addr + 64 * h + 32, o[1]);
-            tmem_ld_wait();
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t w[32];
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                const float2 y = __fmul2_rn(make_float2(o[c][k], o[c][k + 1]), f2);
-                w[k] = __float_as_uint(y.x);
-                w[k + 1] = __float_as_uint(y.y);
-              }
-              tmem_st32(o_addr + 64 * h + 32 * c, w);
-            }
-          }
-        }
-        tmem_st_wait();
         sum = sum * f + ((a0.x + a0.y) + (a1.x + a1.y));
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh->p_full[i]));
       }
       if (ok) ok = wait(sh->o_full[i], oph, 2 + i);
       oph ^= 1u;
