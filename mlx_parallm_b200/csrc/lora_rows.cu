@@ -361,7 +361,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
 // 16-byte copies into tiles of 64 of K, z = x A^T grows in TMEM, meets the other CTAs' and becomes the operand of the second product, whose blocks of 64 or
 // 128 columns take b along with the old y; y grows in its place in shared memory and leaves by whole lines while the next block's product runs.
 // RK: ranks of all targets, filled up to 32, 64, 128 or 256.  8000 rows of rank 64, 4096 to 5120: 56 us of 31.
-constexpr int LP_ROWS = 128, LP_TARGETS = 3, LP_THREADS = LW_THREADS + 128;
+constexpr int LP_ROWS = 128, LP_TARGETS = 3, LP_CLUSTER = 8, LP_THREADS = LW_THREADS + 128;
 template <int RK, int COLS>
 struct LpShape {
   static constexpr int STAGES_B = COLS == 128 ? 3 : 4, STAGES_Y = COLS == 128 ? 3 : 5;
@@ -519,37 +519,47 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   if (C > 1) cluster.sync();
   else __syncthreads();
 
-  // ---- z of all CTAs, as two 16-bit numbers: 16 lanes per row and target, four ranks each (a thread per row reads the other CTAs' memory by single sectors:
-  // 15 000 cycles instead of 10 900) -----------------------------------------------------------------------------------------------
-  if (warp < LW_WARPS) {
-    const int l = threadIdx.x & 15, k = 4 * l;
-#pragma unroll 4
-    for (int i = threadIdx.x >> 4; i < LP_ROWS * p.targets; i += LW_THREADS / 16) {
-      const int row = i & (LP_ROWS - 1), target = i / LP_ROWS, at = row * zp + target * p.R + k;
-      float4 z = make_float4(0.f, 0.f, 0.f, 0.f), v[4];
+  // ---- z of all CTAs, as two 16-bit numbers: a CTA adds up and splits 1 / C of the rows for all of them, 16 lanes a row and target, four ranks each.  (Each
+  // all rows: every CTA would read the z of eight, 512 KB.) --------------------------------------------------------------------------
+  auto meet = [&](auto most) {                                    // of up to `most` CTAs
+    constexpr int CTAS = decltype(most)::value;
+    const int l = threadIdx.x & 15, k = 4 * l, rows = LP_ROWS / C;
+#pragma unroll(CTAS > 4 ? 2 : 4)
+    for (int i = threadIdx.x >> 4; i < rows * p.targets; i += LW_THREADS / 16) {
+      const int target = i / rows, row = rank * rows + i - target * rows, at = row * zp + target * p.R + k;
+      float4 z = make_float4(0.f, 0.f, 0.f, 0.f), v[CTAS];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < CTAS; ++r)
         v[r] = r < C && k < p.R ? *reinterpret_cast<const float4*>((r == rank ? s_z : cluster.map_shared_rank(s_z, r)) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) z.x += v[r].x, z.y += v[r].y, z.z += v[r].z, z.w += v[r].w;      // in one order everywhere
+      for (int r = 0; r < CTAS; ++r) z.x += v[r].x, z.y += v[r].y, z.z += v[r].z, z.w += v[r].w;      // in one order
       float top = fmaxf(fmaxf(fabsf(z.x), fabsf(z.y)), fmaxf(fabsf(z.z), fabsf(z.w))), up, down;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
       lw_scale(top, up, down);
-      if (l == 0) s_factor[target][row] = up * p.scales[tile.x];
-      if (k >= p.R) continue;
       z.x *= down, z.y *= down, z.z *= down, z.w *= down;
       auto rest = [](float x) { return x - Tr<T>::to_f(Tr<T>::from_f(x)); };
-      const uint32_t to = zop + (uint32_t)target * S::Z_TILE + row * 128 + (((k >> 3) ^ (row & 7)) << 4) + (k & 4) * 2;
-      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(pack2<T>(z.x, z.y)), "r"(pack2<T>(z.z, z.w)) : "memory");
-      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + (uint32_t)p.targets * S::Z_TILE), "r"(pack2<T>(rest(z.x), rest(z.y))),
-                   "r"(pack2<T>(rest(z.z), rest(z.w)))
-                   : "memory");
+      const uint2 high = make_uint2(pack2<T>(z.x, z.y), pack2<T>(z.z, z.w)), low = make_uint2(pack2<T>(rest(z.x), rest(z.y)), pack2<T>(rest(z.z), rest(z.w)));
+      uint8_t* to = base + S::front(TR) + (size_t)target * S::Z_TILE + row * 128 + (((k >> 3) ^ (row & 7)) << 4) + (k & 4) * 2;
+      const float factor = up * p.scales[tile.x];
+      for (int r = 0; r < C; ++r) {
+        if (l == 0) (r == rank ? s_factor : cluster.map_shared_rank(s_factor, r))[target][row] = factor;
+        if (k >= p.R) continue;
+        uint8_t* there = r == rank ? to : cluster.map_shared_rank(to, r);
+        *reinterpret_cast<uint2*>(there) = high;
+        *reinterpret_cast<uint2*>(there + (size_t)p.targets * S::Z_TILE) = low;
+      }
     }
+  };
+  if (warp < LW_WARPS) {
+    if (C == 1) meet(std::integral_constant<int, 1>());
+    else if (C <= 4) meet(std::integral_constant<int, 4>());
+    else meet(std::integral_constant<int, LP_CLUSTER>());
   }
   fence_proxy_async_smem();
-  if (C > 1) cluster.sync();                                      // all have read: the stages may lie there again
+  if (C > 1) cluster.sync();                                      // all have read and written: the stages may lie there again
   else __syncthreads();
+  fence_proxy_async_smem();                                       // (the others' writes, for the products)
   tc_fence_after();
   pdl_launch_dependents();
 
@@ -704,7 +714,9 @@ static int launch_lora(void (*kern)(LoraRows), int threads, int most_bytes, int 
     if (ae == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   if (ae != cudaSuccess) return cuda_fail(ae, "cudaFuncSetAttribute(lora kernels)");
-  while (C > 1 && tiles * C > (int64_t)per_sm * sm_count()) C >>= 1;
+  // (clusters of eight with an SM for each CTA fill three quarters of the GPU at most, as their SMs are of one GPC: 2000 rows of 2 adapters of rank 64 in 16
+  // of them 42.7, in fours 31.1)
+  while (C > 1 && tiles * C > (int64_t)per_sm * sm_count() * (C > 4 && per_sm == 1 ? 3 : 4) / 4) C >>= 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C));
   cfg.blockDim = dim3((unsigned)threads);
@@ -736,7 +748,7 @@ static int launch_lora_prompt_of(LoraRows p, int64_t tiles, cudaStream_t st) {
   using S = LpShape<RK, COLS>;
   constexpr int TARGETS = COLS == 128 ? 2 : LP_TARGETS, MOST = RK < LW_RANK * TARGETS ? RK : LW_RANK * TARGETS;
   static_assert(S::bytes(MOST, TARGETS) <= 224 * 1024, "beside the static shared memory");
-  return launch_lora(lora_prompt_kernel<T, RK, COLS>, LP_THREADS, S::bytes(MOST, TARGETS), S::bytes(p.targets * p.R, p.targets), 4, 1, ready, p, tiles, st);
+  return launch_lora(lora_prompt_kernel<T, RK, COLS>, LP_THREADS, S::bytes(MOST, TARGETS), S::bytes(p.targets * p.R, p.targets), LP_CLUSTER, 1, ready, p, tiles, st);
 }
 // Blocks of 128 columns, whose products take the tensor core as long as those of 64 do; of 64 where three targets' z take their room.
 template <typename T, int RK>
@@ -795,9 +807,10 @@ extern "C" int b200p_row_groups(const int32_t* index, int32_t* plan, int64_t M, 
 }
 
 // Tiles of 128 rows read an adapter an eighth as often as tiles of 16 and put it on the tensor core, and have more to set up for few rows.  us, tiles of
-// 16 / 128, 4096 to 5120 columns: 2 adapters, 1000 rows of rank 16 17 / 30, 1500 32 / 30, 8000 116 / 53; rank 64 33 / 33, 61 / 33, 234 / 55.  64 adapters,
-// 500 rows of rank 16 20 / 41, 1500 51 / 67, 8000 118 / 80; rank 64 57 / 47, 102 / 75, 226 / 90.  (A plan is laid out once for layers of every rank.)
-extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1500 && M >= 16ll * groups ? LP_ROWS : 16; }
+// 16 / 128, 4096 to 5120 columns, ranks 16 and 64: 2 adapters, 500 rows 13.6 / 19.4 and 23.8 / 22.0, 1000 16.4 / 19.5 and 32.6 / 22.1, 1500 32.0 / 20.1 and
+// 60.7 / 23.2, 8000 116 / 53 and 234 / 56; 16 adapters, 500 rows 13.5 / 25.8 and 25.1 / 27.7, 1000 21.8 / 26.1 and 54.3 / 28.0; 64 adapters, 500 rows
+// 19.9 / 40.9 and 56.9 / 46.7, 1500 51 / 67 and 102 / 74, 8000 118 / 80 and 226 / 88.  (A plan is laid out once for layers of every rank.)
+extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1000 && M >= 16ll * groups ? LP_ROWS : 16; }
 
 extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a, const void* b, const float* scales, void* y, const int32_t* host_columns,
                                int64_t M, int adapters, int tile, int targets, int R, int64_t K, int64_t ldx, int64_t ldy, int dtype, int y_f32,

@@ -320,3 +320,9 @@ def test_prompt_tiles_of_y_at_odd_places(shift, gap):
     x, a, b, s, columns, y = make(260, 3, 256, 16, (64, 32), "bf16", gap=gap, out="16")
     wide = torch.randn((260, y.shape[1] + 16), device="cuda").bfloat16()
     check(index_of(260, 3), x, a, b, s, columns, wide[:, shift:shift + y.shape[1]], 128)
+
+
+@pytest.mark.parametrize("M,n", [(900, 2), (2100, 6), (5000, 30), (9000, 40)])
+@pytest.mark.parametrize("R,targets", [(16, 2), (64, 3)])
+def test_prompt_tiles_of_clusters_of_every_size(M, n, R, targets):
+    check(index_of(M, n, seed=M), *make(M, n, 520, R, (136, 264, 8)[:targets], "f16", out="16", seed=n), 128)
