@@ -5,13 +5,14 @@
 // a page is fetched from behind the pages, where the copy brings zeros.  A CTA's part of the work is runs of steps of one item after the other, each of
 // which leaves a part.  Products, softmax and roles are those of the prompt kernel, but the maximum may lag by 2^6 before outputs are rescaled (a part is few
 // steps, in most of which one of a warp's rows finds a new one: 114 -> 104 thousand cycles for 30 steps), and for f16 it is held 8 lower, so that weights reach
-// 2^14 and small ones keep their bits.  A weight is off by half a step of its type, at random, and their sum is that of the rounded ones: with the output's own
-// rounding 1.2 (bf16) and 1.4 (f16) times that rounding alone.
+// 2^14 and small ones keep their bits.  A weight is two 16-bit numbers, the rounded one and what it lost, which multiply the same values one after the other, so
+// that a token's output does not depend on whether its slots are shared: it carries its own rounding only.  (As one number, with the sum of the rounded ones,
+// the error was 1.3 times that, and 128 rows behind 16000 slots took 106.0 us instead of 119.6, 64 behind 4000 44.5 instead of 46.2.)
 //
-// The weights of a step's first 64 keys are multiplied while those of the last 64 are made (128 rows behind 16000 slots 109.4 -> 106.1 us).
+// The weights of a step's first 64 keys are multiplied while those of the last 64 are made (128 rows behind 16000 slots, one number a weight, 109.4 -> 106.1 us).
 //
-// 128 rows in two groups behind 16000 and 12032 slots, 64 / 8 heads (60 GFLOP): CTAs end after 57 to 77 us, 68 in the median; 3450 cycles a step of 256 rows,
-// against 2048 of the tensor core's and as many of its exponentials.  Of 64 rows behind 4000 slots a CTA has 3.5 steps, and the plan (4000 cycles), queries
+// 128 rows in two groups behind 16000 and 12032 slots, 64 / 8 heads (60 GFLOP, 90 with the weights' second numbers): CTAs end after 72 to 91 us, 81 in the median;
+// 4250 cycles a step of 256 rows, against 3072 of the tensor core's and 2048 of its exponentials.  Of 64 rows behind 4000 slots a CTA has 3.5 steps, and the plan (4000 cycles), queries
 // (5000), first copy (1500) and the part (5000) are most of its time.
 #pragma once
 #include "attn_tc.cuh"
@@ -51,7 +52,7 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh->tmem_base;                     // S of half i at 128 i (P over its first 64), O of half i at 256 + 128 i
+  const uint32_t tmem = sh->tmem_base;                     // S of half i at 128 i (P over its first 64, what P lost over the others), O of half i at 256 + 128 i
   pdl_wait();
   pdl_launch_dependents();
   PrefixRun run;
@@ -118,8 +119,10 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
       auto pv = [&](int i, int slot, int from, uint32_t acc) {
         const uint64_t bd = ft_desc_n_major(ring + slot * FT_TILE_BYTES);
 #pragma unroll
-        for (int k = from; k < from + 4; ++k)              // 16 keys = 2048 bytes; P: 8 columns
+        for (int k = from; k < from + 4; ++k) {            // 16 keys = 2048 bytes; P: 8 columns, and what it lost 64 columns further
           umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, bd + (uint64_t)(k * (2048 >> 4)), idesc_pv, (k || acc) ? 1u : 0u);
+          umma_f16_ts(tmem + 256 + 128 * i, tmem + 128 * i + 64 + 8 * k, bd + (uint64_t)(k * (2048 >> 4)), idesc_pv, 1u);
+        }
       };
       int slot = 0, round = 0;
       uint32_t ph = 0, pph[2] = {0, 0};                    // phases of `slot` and of the probabilities' barriers
@@ -282,15 +285,21 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
         float2 a0 = make_float2(0.f, 0.f), a1 = a0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t w[32];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const float2 x = __ffma2_rn(make_float2(s[64 * h + 2 * c], s[64 * h + 2 * c + 1]), sc2, nm2);
-            w[c] = ft_pack<T>(ex2(x.x), ex2(x.y));
-            const float2 e = ft_unpack<T>(w[c]);           // the sum is that of the weights as the product uses them
-            if (c & 1) a1 = __fadd2_rn(a1, e); else a0 = __fadd2_rn(a0, e);
+          for (int part = 4 * h; part < 4 * h + 4; part += 2) {      // 32 keys at a time: what the weights lost has no registers beside all of them
+            uint32_t w[16], rest[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const int key = 16 * part + 2 * c;
+              const float2 x = __ffma2_rn(make_float2(s[key], s[key + 1]), sc2, nm2), e = make_float2(ex2(x.x), ex2(x.y));
+              w[c] = ft_pack<T>(e.x, e.y);
+              const float2 lost = __ffma2_rn(ft_unpack<T>(w[c]), make_float2(-1.f, -1.f), e);
+              rest[c] = ft_pack<T>(lost.x, lost.y);
+              if (c & 1) a1 = __fadd2_rn(a1, e); else a0 = __fadd2_rn(a0, e);
+            }
+            tmem_st16(s_addr + 8 * part, w);
+            tmem_st16(s_addr + 64 + 8 * part, rest);
           }
-          tmem_st32(s_addr + 32 * h, w);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();

@@ -294,21 +294,25 @@ paged_prefix_kernel(const __grid_constant__ PagedPrefix a) {
       }
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
-        // The weights multiply the values as 16-bit numbers, and their sum is that of the rounded ones: each is off by half a step, at random, which
-        // leaves the output's own rounding the larger error; two numbers each would cost half as many products again.
-        uint32_t pf[4] = {pack2<T>(s[2 * j][0], s[2 * j][1]), pack2<T>(s[2 * j][2], s[2 * j][3]), pack2<T>(s[2 * j + 1][0], s[2 * j + 1][1]),
-                          pack2<T>(s[2 * j + 1][2], s[2 * j + 1][3])};
+        // The weights multiply the values as two 16-bit numbers each, the rounded weight and what it lost, as in paged_attn_kernel, so that the output
+        // carries its own rounding only.  (As one number a weight is off by half a step of its type: 1.3 times the output's rounding alone in bf16.)
+        uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const T* p = reinterpret_cast<const T*>(&pf[e]);
-          l[e & 1] += Tr<T>::to_f(p[0]) + Tr<T>::to_f(p[1]);
+          const float x = s[2 * j + (e >> 1)][2 * (e & 1)], y = s[2 * j + (e >> 1)][2 * (e & 1) + 1];
+          l[e & 1] += x + y;
+          hi[e] = pack2<T>(x, y);
+          const T* p = reinterpret_cast<const T*>(&hi[e]);
+          lo[e] = pack2<T>(x - Tr<T>::to_f(p[0]), y - Tr<T>::to_f(p[1]));
         }
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           uint32_t vf[4];
           ldsm_x4_trans(vs + P::at(16 * j + r8 + 8 * (mat & 1), 2 * k + (mat >> 1)), vf);
-          mma16816<T>(o[2 * k], pf, vf[0], vf[1]);
-          mma16816<T>(o[2 * k + 1], pf, vf[2], vf[3]);
+          mma16816<T>(o[2 * k], hi, vf[0], vf[1]);
+          mma16816<T>(o[2 * k + 1], hi, vf[2], vf[3]);
+          mma16816<T>(o[2 * k], lo, vf[0], vf[1]);
+          mma16816<T>(o[2 * k + 1], lo, vf[2], vf[3]);
         }
       }
     }

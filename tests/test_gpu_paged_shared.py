@@ -338,3 +338,34 @@ def test_by_the_rule_and_by_tokens(path):
     plain = ops.paged_attn(small.q, small.k, small.v, small.table, small.row, small.slot, torch.empty_like(small.q), small.scale, workspace=ws)
     assert torch.equal(small.check(), plain)
     Case([0] * 12, [1600], [1601 + i for i in range(12)]).check()
+
+
+def fine_slack(c, out):
+    """How far outputs may be off when their own rounding is the only one to fewer than 32 bits that shows (``out`` [M, H D] the definition): a weight is two 16-bit
+    numbers, off by half a step of what the first lost, half * half, and in f16 by 2^-25 at least where the largest weight is 2^8 or more; products of 16 keys
+    are added up in fp32, a unit of 2^-23 each; a score's sums as in Case.want; 2^x and the joins."""
+    H, G, D, page, half = c.H, c.G, c.D, c.page, torch.finfo(c.q.dtype).eps / 2
+    tol = half * out.abs()
+    for t, (r, s) in enumerate(zip(c.row.tolist(), c.slot.tolist())):
+        n = s + 1
+        j = torch.arange(n, device="cuda")
+        ids = c.table[r].long()[j // page]
+        k, v = c.k[ids, :, j % page].double(), c.v[ids, :, j % page].double()
+        q = c.q[t].double().view(G, H // G, D)
+        p = torch.softmax(torch.einsum("ghd,jgd->ghj", q, k) * c.scale, -1)
+        size = torch.einsum("ghd,jgd->ghj", q.abs(), k.abs()).amax(-1, keepdim=True) * abs(c.scale)
+        spread = torch.einsum("ghj,jgd->ghd", p, v.abs())
+        lost = spread * (half * half + (n / 16 + 2 * (D / 16 + 8) * size) * 2.0 ** -23 + 2.0 ** -19) + n * 2.0 ** -33 * v.abs().amax(0)[:, None]
+        tol[t] += lost.reshape(-1)
+    return tol
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("H,G,D", [(32, 8, 128), (40, 8, 128), (4, 2, 64), (25, 5, 80), (32, 32, 96), (16, 2, 256)])
+@pytest.mark.parametrize("spread,scale", [(0.2, 1.0), (1.5, 1.0), (0.2, -1.0)])
+def test_outputs_carry_their_own_rounding_only(H, G, D, dtype, spread, scale):
+    c = Case([0, 0, 1, 0, 0, 1], [160, 640], [161, 170, 641, 165, 163, 650], H=H, G=G, D=D, dtype=dtype, spread=spread)
+    c.scale *= scale                                                # (a negative one goes through the mma.sync kernel for all sizes)
+    got, (out, _) = c.run(), c.want()
+    diff, tol = (got.double() - out).abs(), fine_slack(c, out)
+    assert diff.le(tol).all(), (float((diff - tol).max()), float((diff > tol).double().mean()))
