@@ -80,7 +80,7 @@ struct PagedAttn {
   // behind shared slots (paged_shared.cuh): a token's group, the groups' shared slots, the parts of items that lie in one share
   const int32_t *index, *prefix;
   int groups;
-  float* whole;        // [M, items, rows of a block, D + 4]
+  float* whole;        // [M, H, D + 4]
 };
 
 __device__ __forceinline__ int shared_slots(const int32_t* index, const int32_t* prefix, int groups, const PageTable& pt, int t, int seen);
@@ -742,7 +742,7 @@ paged_attn_kernel(const __grid_constant__ PagedAttn a) {
     if (lane == 0) s.part[warp] = part;
     const int head = r.head;
     const bool cut = TAIL || r.part >= 0;
-    float* rec = (TAIL && r.part < 0 ? a.whole + (int64_t)r.line * E::ROWS * (D + 4) : a.rec + (int64_t)r.part * E::ROWS * (D + 4));
+    float* rec = (TAIL && r.part < 0 ? a.whole + (int64_t)head * (D + 4) : a.rec + (int64_t)r.part * E::ROWS * (D + 4));
 #pragma unroll 1
     for (int pass = 0; pass * 8 < rows; ++pass) {
       e.publish(reinterpret_cast<float*>(smem + E::Q_BYTES + part), pass, D);
@@ -1149,14 +1149,8 @@ static bool shared_served(int64_t M, int H, int G, int D, int64_t slots, int dty
   return path == 1 || (M - 1) * slots * G * D * 4 >= 32ll << 20;
 }
 static int shared_tile(int H, int G) { return H / G < PS_ROWS ? PS_ROWS / (H / G) : 1; }
-static int64_t shared_rows(int H, int G) {                          // of a token's items with the rows that blocks are filled up to
-  const int per = H / G;
-  return (int64_t)G * (per <= 8 ? 8 : (per + 15) / 16 * 16);
-}
-static size_t whole_bytes(int64_t M, int H, int G, int D) { return round256((size_t)M * shared_rows(H, G) * (D + 4) * 4); }
-static size_t prefix_bytes(int64_t M, int H, int G, int D, int groups) {
-  return round256(((size_t)row_group_tiles(M, groups, shared_tile(H, G)) * G + sm_count()) * PS_ROWS * (D + PS_HEAD) * 4);      // (halves as items: no more)
-}
+static size_t whole_bytes(int64_t M, int H, int D) { return round256((size_t)M * H * (D + 4) * 4); }
+static size_t prefix_bytes(int64_t M, int H, int D) { return round256(((size_t)M * H + (size_t)sm_count() * PS_ROWS) * (D + PS_HEAD) * 4); }
 static size_t info_bytes(int64_t M) { return round256((size_t)M * 16 + 16); }
 
 template <typename K>
@@ -1304,7 +1298,7 @@ extern "C" int b200p_paged_attn_shared_tile(int H, int G) { return G > 0 && H >=
 
 extern "C" size_t b200p_paged_attn_shared_workspace_bytes(int64_t M, int H, int G, int D, int groups) {
   if (M <= 0 || G <= 0 || H < G || H % G || D <= 0 || groups <= 0 || groups > RG_GROUPS) return 0;
-  return workspace_bytes(M, H, D, 0, 0) + whole_bytes(M, H, G, D) + prefix_bytes(M, H, G, D, groups) + info_bytes(M);
+  return workspace_bytes(M, H, D, 0, 0) + whole_bytes(M, H, D) + prefix_bytes(M, H, D) + info_bytes(M);
 }
 
 extern "C" int b200p_paged_attn_shared(const void* q, const void* kpages, const void* vpages, const int32_t* table, const int32_t* t_row,
@@ -1342,9 +1336,9 @@ extern "C" int b200p_paged_attn_shared(const void* q, const void* kpages, const 
   PagedPrefix p{};
   p.q = q, p.k = kpages, p.v = vpages, p.pt = pt, p.t_row = t_row, p.t_slot = t_slot, p.index = index, p.prefix = prefix;
   p.plan = RowGroups{plan, (int)M}, p.M = (int)M, p.H = H, p.G = G, p.groups = groups, p.scale_log2e = a.scale_log2e;
-  p.rec = (float*)(ws += whole_bytes(M, H, G, D));
-  p.rec_rows = (int64_t)(prefix_bytes(M, H, G, D, groups) / ((D + PS_HEAD) * 4));
-  p.info = (int4*)(ws += prefix_bytes(M, H, G, D, groups));
+  p.rec = (float*)(ws += whole_bytes(M, H, D));
+  p.rec_rows = (int64_t)(prefix_bytes(M, H, D) / ((D + PS_HEAD) * 4));
+  p.info = (int4*)(ws += prefix_bytes(M, H, D));
   p.total = (unsigned*)(p.info + M);
   const int64_t tiles = row_group_tiles(M, groups, tile);
   return dtype == B200P_F16 ? launch_shared_type<__half>(a, p, tiles, (cudaStream_t)stream) : launch_shared_type<__nv_bfloat16>(a, p, tiles, (cudaStream_t)stream);

@@ -314,7 +314,7 @@ paged_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_con
         tc_fence_after();
         // A row's outputs are in a lane: 32 columns at a time go through the warp's own place among the queries, which nobody reads any more, so that
         // lines are written whole.
-        float* part = a.rec + (((int64_t)run.item + blockIdx.x) * PS_ROWS + PS_HALF * i + 32 * q) * (FT_D + PS_HEAD);
+        float* part = a.rec + (run.row0 + (int64_t)blockIdx.x * PS_ROWS + PS_HALF * i + 32 * q) * (FT_D + PS_HEAD);
         const int rows = min(32, run.rows - PS_HALF * i - 32 * q);
         if (lane < rows) *reinterpret_cast<float2*>(part + lane * (FT_D + PS_HEAD)) = make_float2(m, sum);
 #pragma unroll

@@ -24,9 +24,11 @@ struct PagedPrefix {
   float scale_log2e;
   uint64_t inv_tpp;
   int tpp;
-  float* rec;            // [items + CTAs, rows of an item, PS_HEAD + D] parts, of item i in CTA c the one at i + c
-  int4* info;            // [M] the token's tile, its place in it (and in the upper half the tile's items per key head), the tile's first unit, units of an item (0:
-                         // the token reads by itself)
+  // [M H + CTAs * rows of an item, PS_HEAD + D] parts: of a query row of an item in CTA c at the row's place among all (row0 and its place in the item)
+  // + c * rows of an item.  (Items lie on a line and every CTA has a run of it: a part begins behind the last row of the one before.)
+  float* rec;
+  int4* info;            // [M] the tile's first place in the plan's order, the token's place in it (in the upper half the tile's tokens), the tile's first unit,
+                         // units of an item (0: the token reads by itself)
   unsigned* total;       // units of all
   int* wait_word;
   int box;               // keys that one copy brings: they lie in one page
@@ -61,7 +63,8 @@ __device__ __forceinline__ int shared_slots(const int32_t* index, const int32_t*
 struct PrefixRun {
   int4 tile;
   int ti, n, common, table_row;        // the tile, units of an item, shared slots, the table row that has their pages
-  int g, half, first, last, item, rows;  // key head, half, units [first, last), number of the item, query rows of the tile
+  int g, half, first, last, rows;      // key head, half, units [first, last), query rows of the tile
+  int64_t row0;                        // the item's first query row among those of all items
 };
 
 // SPLIT: an item has half of a tile's rows (where it has more than that), else all of them.
@@ -93,7 +96,7 @@ struct PrefixCursor {
     const int at = (int)((u - base) / (unsigned)r.n), h = halves(r);
     r.g = at / h, r.half = at - r.g * h;
     r.first = (int)(u - base) - at * r.n, r.last = min(r.n, r.first + (int)(end - u));
-    r.item = SPLIT ? (ti * a.G + r.g) * 2 + r.half : ti * a.G + r.g;
+    r.row0 = (int64_t)r.tile.y * a.H + (int64_t)r.g * r.rows + PS_HALF * r.half;
     u += r.last - r.first;
     return true;
   }
@@ -102,7 +105,7 @@ struct PrefixCursor {
     if (r.g == 0 && r.half == 0 && r.first == 0 && thread < r.tile.z) {
       const int t = a.plan.order()[r.tile.y + thread];
       const bool shares = slots_seen(a.pt, a.t_slot[t]) >= r.common;
-      a.info[t] = make_int4(r.ti, thread | halves(r) << 16, (int)base, shares ? r.n : 0);
+      a.info[t] = make_int4(r.tile.y, thread | r.tile.z << 16, (int)base, shares ? r.n : 0);
     }
   }
 };
@@ -319,13 +322,14 @@ paged_prefix_kernel(const __grid_constant__ PagedPrefix a) {
     cp_async_wait<0>();
     // ---- the part ---------------------------------------------------------------------------------------------------------------
     if (works) {
-      float* rec = a.rec + ((int64_t)run.item + blockIdx.x) * PS_HALF * (D + PS_HEAD);
+      float* rec = a.rec + (run.row0 + (int64_t)blockIdx.x * PS_HALF) * (D + PS_HEAD);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float sum = l[h];
         sum += __shfl_xor_sync(~0u, sum, 1);
         sum += __shfl_xor_sync(~0u, sum, 2);
         float* row = rec + (16 * warp + 8 * h + qr) * (D + PS_HEAD);
+        if (16 * warp + 8 * h + qr >= rows) continue;               // (another item's place)
         if (qc == 0) *reinterpret_cast<float2*>(row) = make_float2(m[h], sum);
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(row + PS_HEAD + 8 * j + 2 * qc) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
@@ -354,19 +358,19 @@ paged_shared_join_kernel(const __grid_constant__ PagedAttn a, const __grid_const
   int64_t row0 = 0;                                                 // its row in the first of them
   if ((unsigned)group < (unsigned)p.groups && info.w > 0) {
     const PrefixShares sh(total, prefix_ctas, p.few);
-    const int halves = info.y >> 16, at = (info.y & 0xffff) * per + r, half = halves > 1 && at >= PS_HALF ? 1 : 0;
+    const int rows = (info.y >> 16) * per, halves = item_rows == PS_HALF && rows > PS_HALF ? 2 : 1;
+    const int at = (info.y & 0xffff) * per + r, half = halves > 1 && at >= PS_HALF ? 1 : 0;
     const unsigned u = (unsigned)info.z + (unsigned)((g * halves + half) * info.w);
     c0 = (int)sh.of(u);
     heads = (int)sh.of(u + info.w - 1) - c0 + 1;
-    row0 = (int64_t)(item_rows == PS_HALF ? (info.x * a.G + g) * 2 + half : info.x * a.G + g) + c0;
-    row0 = row0 * item_rows + at - PS_HALF * half;
+    row0 = (int64_t)info.x * a.H + (int64_t)g * rows + at + (int64_t)c0 * item_rows;
     // (a plan that is not the index's leaves what it likes here: wrong, but nothing behind the workspace is read)
-    if (heads > prefix_ctas || row0 < 0 || row0 + (int64_t)heads * item_rows > p.rec_rows) heads = 0;
+    if (heads > prefix_ctas || row0 < 0 || row0 + (int64_t)(heads - 1) * item_rows >= p.rec_rows) heads = 0;
   }
   const int all = here ? heads + (int)parts.y : 0;
   auto at = [&](int i) -> const float* {                            // its outputs; maximum and sum stand before them
     if (i < heads) return p.rec + (row0 + (int64_t)i * item_rows) * (D + PS_HEAD) + PS_HEAD;
-    if (parts.y == 1) return a.whole + (line * ROWS + r % ROWS) * (D + 4) + 4;
+    if (parts.y == 1) return a.whole + ((int64_t)t * a.H + head) * (D + 4) + 4;
     return part_at(a, parts.x, i - heads, ROWS, r % ROWS) + 4;
   };
   constexpr int AHEAD = 4;

@@ -369,3 +369,17 @@ def test_outputs_carry_their_own_rounding_only(H, G, D, dtype, spread, scale):
     got, (out, _) = c.run(), c.want()
     diff, tol = (got.double() - out).abs(), fine_slack(c, out)
     assert diff.le(tol).all(), (float((diff - tol).max()), float((diff > tol).double().mean()))
+
+
+@pytest.mark.parametrize("H,G,D,dtype", [(32, 8, 128, "bf16"), (12, 1, 64, "f16"), (9, 9, 80, "f16"), (130, 1, 64, "bf16")])
+def test_parts_stay_in_the_workspace(H, G, D, dtype):
+    """Groups of one to thirty rows, each cut over several CTAs: every part in a place of its own, and nothing behind the workspace."""
+    sizes = [1, 30, 2, 7, 1, 1, 16, 3]
+    group = [g for g, n in enumerate(sizes) for _ in range(n)] + [-1]
+    prefix = [2048 - 240 * g for g in range(len(sizes))]
+    c = Case(group, prefix, [(prefix[g] if g >= 0 else 40) + 1 + 11 * i % 50 for i, g in enumerate(group)], H=H, G=G, D=D, dtype=dtype)
+    n = ops.paged_attn_shared_workspace_bytes(len(group), H, G, D, len(sizes))
+    ws = torch.randint(0, 256, (n + (1 << 20),), dtype=torch.uint8, device="cuda")
+    behind = ws[n:].clone()
+    c.check(ws=ws[:n])
+    assert torch.equal(ws[n:], behind)

@@ -131,3 +131,12 @@ def test_pages_of_rows_that_share_a_prompt():
     with pytest.raises(PagesExhausted):
         book.adopt(side, [[0, 1, 2], [3, 4]], 40)
     assert all(not o for o in book.owned) and book.groups == [] and len(book.free) == 2
+
+
+def test_workspace_of_shared_slots_goes_by_query_rows_not_by_groups():
+    """Parts are M H query rows and 256 more per SM at most, of outputs, maximum and sum in fp32, beside one row each of the own slots."""
+    size = _lib.lib().b200p_paged_attn_shared_workspace_bytes
+    for M, H, G, D in ((1024, 32, 8, 128), (1024, 32, 32, 96), (2048, 32, 32, 128), (64, 32, 8, 128), (3, 9, 1, 256)):
+        base = ops.paged_attn_workspace_bytes(M, H, D, 0, G)
+        assert size(M, H, G, D, 1) == size(M, H, G, D, 1024)
+        assert size(M, H, G, D, 7) <= base + (2 * M * H + 256 * 160) * (D + 8) * 4 + 16 * M + 2048
