@@ -129,52 +129,69 @@ class PageBook:
 
     def adopt(self, other: "PageBook", groups: List[List[int]], tokens: int) -> None:
         """Row i of ``other``, which draws on this book's pages and holds ``tokens`` tokens, becomes all of the rows ``groups[i]``: its whole pages are theirs
-        together, of a last one that is not full everybody but the first gets a copy.  All or nothing: PagesExhausted if the pool is short."""
+        together, of a last one that is not full everybody but the first gets a copy.  All or nothing: PagesExhausted if the pool is short, or an error of the
+        device's memory, leave the book as it was."""
         whole, rest = tokens // self.page, tokens % self.page
         need = sum(len(g) - 1 for g in groups) if rest else 0
         if need > len(self.free):
             raise PagesExhausted(f"paged cache exhausted: {need} pages wanted for the rows of a shared prompt, {len(self.free)} of {self.pages} free")
-        source, copies = [], []
+        # what can fail on the device comes first: until all of it is done, only pages of nobody are written
+        new = [self.free.pop() for _ in range(need)]
+        try:
+            left, mine, copied = list(new), {}, []
+            for i, g in enumerate(groups):
+                for k, r in enumerate(g):
+                    mine[r] = list(other.owned[i][:whole + (1 if rest else 0)])
+                    if rest and k:
+                        copied.append((mine[r][-1], left[-1]))
+                        mine[r][-1] = left.pop()
+            if copied:
+                source, to = (torch.tensor(t, device=self.device) for t in zip(*copied))
+                for c in self.layers:
+                    for pages in (c.kpages, c.vpages):
+                        pages[to] = pages[source]
+            rows = torch.tensor(list(mine), device=self.device)
+            table = torch.tensor([m + [-1] * (self.width - len(m)) for m in mine.values()], dtype=torch.int32).to(self.device)
+            joined, slots = self.groups + [list(g) for g in groups], self.prefixes + [whole * self.page] * len(groups)
+            self._ready(joined, slots)
+        except BaseException:
+            self.free += reversed(new)
+            raise
+        self.groups, self.prefixes = joined, slots
+        for r, m in mine.items():
+            self.owned[r] = m
+        self.table.index_copy_(0, rows, table)
         for i, g in enumerate(groups):
-            pages = other.owned[i]
-            for k, r in enumerate(g):
-                mine = list(pages[:whole])
-                if rest:
-                    mine.append(pages[whole] if k == 0 else self.free.pop())
-                    if k:
-                        source.append(pages[whole])
-                        copies.append(mine[-1])
-                self.owned[r] = mine
-                self.table[r, :len(mine)] = torch.tensor(mine, dtype=torch.int32).to(self.device)
             if len(g) > 1:
-                for p in pages[:whole]:
+                for p in other.owned[i][:whole]:
                     self.held[p] = len(g)
             other.owned[i] = []
-            self.groups.append(list(g))
-            self.prefixes.append(whole * self.page)
-        if copies:
-            at = torch.tensor(source, device=self.device), torch.tensor(copies, device=self.device)
-            for c in self.layers:
-                for pages in (c.kpages, c.vpages):
-                    pages[at[1]] = pages[at[0]]
         for c in self.layers:
-            for g in groups:
-                for r in g:
-                    c._offsets[r] = tokens
+            for r in mine:
+                c._offsets[r] = tokens
             c.offset = max(c._offsets)
         self.layers[0]._sync_lengths()
         self._regroup()
 
-    def _regroup(self) -> None:
-        """The device's view of the groups, and whether the shared slots are worth a step's going by them.  Once it does, it does so until the cache is reset, so
-        that a captured step stays valid while rows leave."""
+    def _ready(self, groups: List[List[int]], prefixes: List[int]) -> bool:
+        """Whether a step goes by these groups; if so, what it needs on the device is there (and nothing of what the book says has changed).  Once a step
+        goes by groups it does so until the cache is reset, so that a captured one stays valid while rows leave."""
         c = self.layers[0]
-        saved = sum((len(g) - 1) * n for g, n in zip(self.groups, self.prefixes)) * 2 * c.n_kv_heads * c.head_dim * c.kpages.element_size()
+        saved = sum((len(g) - 1) * n for g, n in zip(groups, prefixes)) * 2 * c.n_kv_heads * c.head_dim * c.kpages.element_size()
         if not self.by_groups and saved < SHARED_BYTES:
+            return False
+        if self.plan is None:
+            group = torch.full((self.rows,), -1, dtype=torch.int32, device=self.device)
+            prefix = torch.zeros((self.shared_groups,), dtype=torch.int32, device=self.device)
+            plan = ops.row_groups(group, self.shared_groups, ops.paged_attn_shared_tile(c.n_heads, c.n_kv_heads))
+            self.group, self.prefix, self.plan = group, prefix, plan
+        self.shared_workspace(c.n_heads, c.n_kv_heads, c.head_dim)      # (not inside the capture of a step)
+        return True
+
+    def _regroup(self) -> None:
+        """The device's view of the groups."""
+        if not self._ready(self.groups, self.prefixes):
             return
-        if self.group is None:
-            self.group = torch.empty((self.rows,), dtype=torch.int32, device=self.device)
-            self.prefix = torch.empty((self.shared_groups,), dtype=torch.int32, device=self.device)
         index, prefix = [-1] * self.rows, [0] * self.shared_groups
         together = [(g, n) for g, n in zip(self.groups, self.prefixes) if len(g) > 1][:self.shared_groups]
         for i, (g, n) in enumerate(together):
@@ -183,9 +200,7 @@ class PageBook:
                 index[r] = i
         self.group.copy_(torch.tensor(index, dtype=torch.int32))
         self.prefix.copy_(torch.tensor(prefix, dtype=torch.int32))
-        tile = ops.paged_attn_shared_tile(c.n_heads, c.n_kv_heads)
-        self.plan = ops.row_groups(self.group, self.shared_groups, tile, out=self.plan)
-        self.shared_workspace(c.n_heads, c.n_kv_heads, c.head_dim)      # (not inside the capture of a step)
+        ops.row_groups(self.group, self.shared_groups, self.plan.tile, out=self.plan)
         self.by_groups = True
 
     @property

@@ -140,3 +140,31 @@ def test_workspace_of_shared_slots_goes_by_query_rows_not_by_groups():
         base = ops.paged_attn_workspace_bytes(M, H, D, 0, G)
         assert size(M, H, G, D, 1) == size(M, H, G, D, 1024)
         assert size(M, H, G, D, 7) <= base + (2 * M * H + 256 * 160) * (D + 8) * 4 + 16 * M + 2048
+
+
+def _state(book, layer):
+    return (list(layer._offsets), [list(o) for o in book.owned], dict(book.held), [list(g) for g in book.groups], list(book.prefixes), list(book.free),
+            book.table.tolist(), book.lengths.tolist(), book.positions.tolist(), book.by_groups)
+
+
+@pytest.mark.parametrize("fails", ["copy", "group"])
+def test_a_shared_prompt_that_finds_no_memory_leaves_the_book_as_it_was(fails, monkeypatch):
+    """What fails on the device (the copies of last pages; what a step by groups needs, here refused without a device) fails before the book changes."""
+    from mlx_parallm_b200.models import paged
+    book = paged.PageBook(4, 64, "cpu", page=16, pages=14)
+    layers = [paged.PagedLayer(book, 4, 2, 8) for _ in range(2)]
+    for layer in layers:
+        layer.kpages, layer.vpages = torch.randn((14, 2, 16, 8)), torch.randn((14, 2, 16, 8))
+    side = paged.PageBook(1, 40, "cpu", page=16, pages=14, of=book)
+    paged.PagedLayer(side, 4, 2, 8)
+    side.room_for([40])
+    if fails == "group":
+        monkeypatch.setattr(paged, "SHARED_BYTES", 0)
+    else:
+        layers[1].vpages = torch.randn((1, 2, 16, 8))               # no page to copy
+    before, theirs = _state(book, layers[0]), list(side.owned[0])
+    with pytest.raises(_lib.B200PError if fails == "group" else IndexError):
+        book.adopt(side, [[0, 1, 3]], 40)
+    assert _state(book, layers[0]) == before and side.owned[0] == theirs
+    side.shrink([0])
+    assert sorted(book.free) == list(range(14))
