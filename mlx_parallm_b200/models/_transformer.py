@@ -486,6 +486,7 @@ class DecoderModel:
             prepare_cache(cache, book.rows, 0, self.dtype, self.device)            # (the pages of every layer)
             if L + 1 > book.max_tokens:
                 raise PagesExhausted(f"a prompt of {L} tokens does not fit a paged cache of {book.max_tokens} per row")
+            book.give_back_unused(rows)
             side = PageBook(n, L, self.device, book.page, book.pages, of=book)
             layers = [PagedLayer(side, c.n_heads, c.n_kv_heads, c.head_dim) for c in cache]
             for mine, c in zip(layers, cache):

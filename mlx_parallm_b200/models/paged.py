@@ -127,12 +127,17 @@ class PageBook:
                 del self.owned[r][left:]
                 self.table[r, left:] = -1
 
+    def give_back_unused(self, rows: List[int]) -> None:
+        """Pages of rows that hold no token go back to the pool (a step that failed behind its ``room_for`` leaves its rows theirs)."""
+        self.shrink([0 if r in rows else len(o) * self.page for r, o in enumerate(self.owned)])
+
     def adopt(self, other: "PageBook", groups: List[List[int]], tokens: int) -> None:
         """Row i of ``other``, which draws on this book's pages and holds ``tokens`` tokens, becomes all of the rows ``groups[i]``: its whole pages are theirs
         together, of a last one that is not full everybody but the first gets a copy.  All or nothing: PagesExhausted if the pool is short, or an error of the
         device's memory, leave the book as it was."""
         whole, rest = tokens // self.page, tokens % self.page
         need = sum(len(g) - 1 for g in groups) if rest else 0
+        self.give_back_unused([r for g in groups for r in g])
         if need > len(self.free):
             raise PagesExhausted(f"paged cache exhausted: {need} pages wanted for the rows of a shared prompt, {len(self.free)} of {self.pages} free")
         # what can fail on the device comes first: until all of it is done, only pages of nobody are written

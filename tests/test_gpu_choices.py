@@ -313,6 +313,19 @@ def test_a_pool_that_is_too_small_for_a_shared_prompt():
     assert len(book.free) == 1
 
 
+def test_a_prompt_finds_the_pages_that_a_failed_step_left_to_its_rows():
+    cfg, om, gm = make_pair("tiny-llama", dtype="float16")
+    ids = torch.from_numpy(prompts_for(cfg, 1, 40))
+    cache = gm.make_paged_cache(2, 64, page=16, pages=4)             # the prompt's three and the copy of its last one
+    book = cache[0].book
+    book.room_for([40, 10])                                          # what a step takes before its kernels run
+    gm.share_prompt(cache, ids, [[0, 1]])
+    assert book.lengths.tolist() == [40, 40] and not book.free and len(set(book.owned[0]) | set(book.owned[1])) == 4
+    for c in cache:
+        c.reset()
+    assert sorted(book.free) == [0, 1, 2, 3]
+
+
 def test_prompts_that_cannot_be_shared():
     cfg, om, gm = make_pair("tiny-llama", dtype="float16")
     ids = torch.from_numpy(prompts_for(cfg, 2, 20))

@@ -168,3 +168,23 @@ def test_a_shared_prompt_that_finds_no_memory_leaves_the_book_as_it_was(fails, m
     assert _state(book, layers[0]) == before and side.owned[0] == theirs
     side.shrink([0])
     assert sorted(book.free) == list(range(14))
+
+
+def test_pages_that_empty_rows_have_go_back_when_they_share_a_prompt():
+    """A step that fails behind room_for leaves its rows pages; adopted rows give them back, and no page is lost or has two places."""
+    from mlx_parallm_b200.models.paged import PageBook, PagedLayer
+    book = PageBook(3, 64, "cpu", page=16, pages=10)
+    layer = PagedLayer(book, 4, 2, 8)
+    layer.kpages, layer.vpages = torch.zeros((10, 2, 16, 8)), torch.zeros((10, 2, 16, 8))
+    book.room_for([50, 10, 20])                                     # 4, 1 and 2 pages, and no token is appended
+    side = PageBook(1, 40, "cpu", page=16, pages=10, of=book)
+    PagedLayer(side, 4, 2, 8)
+    side.room_for([40])
+    book.adopt(side, [[0, 2]], 40)                                  # (the copy of the last page comes out of what rows 0 and 2 gave back)
+    assert len(book.owned[0]) == len(book.owned[2]) == 3 and len(book.owned[1]) == 1
+    used = set(book.owned[0]) | set(book.owned[1]) | set(book.owned[2])
+    assert len(used) == 5 and used.isdisjoint(book.free) and len(book.free) == len(set(book.free)) == 5
+    for r in range(3):
+        assert book.table[r].tolist() == book.owned[r] + [-1] * (4 - len(book.owned[r]))
+    layer.reset()
+    assert sorted(book.free) == list(range(10)) and (book.table == -1).all()
