@@ -952,6 +952,14 @@ def unroll_layers(n_layers: int, start: int = 0, stop: int = 0, times: int = 1) 
     return order + [(i, False) for i in range(stop, n_layers)]
 
 
+def prompt_counts(prompt_lengths, B: int, L: int) -> List[int]:
+    """Tokens of every row of packed prompts [B, L]."""
+    n = [L] * B if prompt_lengths is None else [int(v) for v in prompt_lengths]
+    if len(n) != B or any(not 0 <= v <= L for v in n):
+        raise ValueError(f"prompt_lengths are counts of 0 to {L} ids, one for each of {B} rows: got {n}")
+    return n
+
+
 class SequenceModel:
     """callable(inputs [B, L], cache=None, last_only=False, prompt_lengths=None) -> float32 logits, like the other models,
     plus ``forward_ragged`` for prompts of unequal length and arbitrary logit positions.  Subclasses build ``self.embed``,
@@ -1317,6 +1325,8 @@ class SequenceModel:
         if want is None:
             want = [[len(q) - 1] if len(q) else [] for q in seqs]
         counts = [len(q) for q in seqs]
+        if len(want) != nb or any(not 0 <= p < k for w, k in zip(want, counts) for p in w):
+            raise ValueError("a wanted position lies outside its entry's tokens")
         dev = self.device
         outs = [[None] * len(w) for w in want]
         done = [0] * nb
@@ -1361,8 +1371,6 @@ class SequenceModel:
         if sink is not None:
             return None
         flat_out = [t for o in outs for t in o]
-        if any(t is None for t in flat_out):
-            raise ValueError("a wanted position lies outside its entry's tokens")
         V = self.lm_head.out_features
         return torch.stack(flat_out, 0) if flat_out else torch.empty((0, V), dtype=torch.float32, device=dev)
 
@@ -1374,7 +1382,7 @@ class SequenceModel:
             inputs = torch.as_tensor(inputs)
         B, L = inputs.shape
         host = inputs.tolist()
-        n = [L] * B if prompt_lengths is None else [int(v) for v in prompt_lengths]
+        n = prompt_counts(prompt_lengths, B, L)
         seqs = [host[b][L - n[b]:] for b in range(B)]
         if cache is None:
             cache = self.make_cache(B, step=max(L, 1))
@@ -1394,7 +1402,7 @@ class SequenceModel:
         inputs = inputs if isinstance(inputs, torch.Tensor) else torch.as_tensor(inputs)
         B, L = inputs.shape
         host = inputs.tolist()
-        n = [L] * B if prompt_lengths is None else [int(v) for v in prompt_lengths]
+        n = prompt_counts(prompt_lengths, B, L)
         out = empty_logprobs((B, L), top, self.device)
         for t in out:
             t.zero_()

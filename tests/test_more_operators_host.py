@@ -188,3 +188,22 @@ def test_pages_that_empty_rows_have_go_back_when_they_share_a_prompt():
         assert book.table[r].tolist() == book.owned[r] + [-1] * (4 - len(book.owned[r]))
     layer.reset()
     assert sorted(book.free) == list(range(10)) and (book.table == -1).all()
+
+
+@pytest.mark.parametrize("lengths", [[5, 4], [4, -1], [4], [4, 4, 4]])
+def test_packed_prompts_that_are_no_counts_are_refused(lengths):
+    """Before anything is read: a length above L would name the last ids of another row."""
+    from mlx_parallm_b200.models._sequence import SequenceModel
+    ids = torch.zeros((2, 4), dtype=torch.int64)
+    for call in (SequenceModel.score, SequenceModel.__call__):
+        with pytest.raises(ValueError, match="prompt_lengths"):
+            call(object(), ids, prompt_lengths=lengths)
+
+
+@pytest.mark.parametrize("want", [[[2], []], [[-1], []], [[0], [0]], [[0]]])
+def test_wanted_positions_outside_their_entries_are_refused(want):
+    from types import SimpleNamespace
+    from mlx_parallm_b200.models._sequence import SequenceModel
+    for sink in (None, lambda *a: None):
+        with pytest.raises(ValueError, match="wanted position"):
+            SequenceModel._forward_ragged_locked(SimpleNamespace(device="cpu"), [[1, 2], []], [SimpleNamespace(batch_size=2)], None, want, sink)
