@@ -253,8 +253,8 @@ int b200p_sample_top_p(const float* logits, int32_t* tokens, float* probs_out, i
  *     logprob[m] = log p[tokens[m]], entropy[m] = -sum p log p, top_ids / top_logprobs [M, top] the largest logits, the lowest index first among equal ones
  * (echoed log probabilities and perplexities of the server           [server/main.py:458-659]; log probabilities of GRPO [rl_training/grpo_trainer.py:74-120]).
  * logits `dtype` [M, V] (row stride ldl); the outputs are float.  tokens[m] < 0: no token, logprob 0; tokens[m] >= V: NaN.  logprob and tokens, entropy:
- * NULL where not wanted; top <= 32 and <= V.  Logits of minus infinity have p = 0 (log p is minus infinity).  A row with a NaN, an infinite logit or nothing
- * but minus infinities gets NaN for all numbers, and its ids are those of its order with NaN as minus infinity. */
+ * NULL where not wanted; top <= 32 and <= V; temperature 1e-30 to 1e27.  Logits of minus infinity have p = 0 (log p is minus infinity).  A row with a NaN, an
+ * infinite logit or nothing but minus infinities gets NaN for all numbers, and its ids are those of its order with NaN as minus infinity. */
 int b200p_token_logprobs(const void* logits, const int32_t* tokens, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs,
                          int64_t M, int64_t V, int64_t ldl, int top, float temperature, int dtype, void* stream);
 

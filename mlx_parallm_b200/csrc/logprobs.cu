@@ -40,7 +40,8 @@ __device__ __forceinline__ float lp_max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-// Differences are held above -1e30, so that a weight of 0 times the difference of a logit of minus infinity is 0.
+// Differences are held above -1e30, so that a weight of 0 times the difference of a logit of minus infinity is 0.  (It is 0 as long as 1e30 / T is more than
+// the 88 behind which 2^x ends: temperatures up to 1e27.)
 __device__ __forceinline__ float lp_diff(float x, float m) { return lp_max_nan(x - m, -1e30f); }
 
 // an order of all floats as unsigned numbers: -0 like 0, NaN like minus infinity
@@ -411,7 +412,7 @@ extern "C" int b200p_token_logprobs(const void* logits, const int32_t* tokens, f
   B200P_REQUIRE(M >= 0 && M < (1ll << 27) && V > 0 && V < (1ll << 30) && ldl >= V, B200P_ERR_ARG, "bad shape: %lld rows of %lld logits, stride %lld",
                 (long long)M, (long long)V, (long long)ldl);
   B200P_REQUIRE(top >= 0 && top <= LP_TOP && top <= V, B200P_ERR_ARG, "%d alternatives of %lld: at most %d", top, (long long)V, LP_TOP);
-  B200P_REQUIRE(temperature >= 1e-30f && temperature <= 1e30f, B200P_ERR_ARG, "temperature must be between 1e-30 and 1e30");
+  B200P_REQUIRE(temperature >= 1e-30f && temperature <= 1e27f, B200P_ERR_ARG, "temperature must be between 1e-30 and 1e27");
   B200P_REQUIRE(dtype == B200P_F32 || dtype == B200P_F16 || dtype == B200P_BF16, B200P_ERR_ARG, "bad dtype %d", dtype);
   if (M == 0) return B200P_OK;
   B200P_REQUIRE(logits && (!logprob || tokens) && (!top || (top_ids && top_logprobs)), B200P_ERR_ARG, "null pointer");

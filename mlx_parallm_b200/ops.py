@@ -358,7 +358,7 @@ class TokenLogprobs(NamedTuple):
 
 
 def token_logprobs(logits, tokens=None, top: int = 0, temperature: float = 1.0, out: Optional[TokenLogprobs] = None) -> TokenLogprobs:
-    """Log probabilities of ``tokens`` (int32 [M]; negative: no token, 0) under softmax(logits / temperature), every row's entropy and its ``top`` <= 32 most
+    """Log probabilities of ``tokens`` (int32 [M]; negative: no token, 0) under softmax(logits / temperature), 1e-30 to 1e27, every row's entropy and its ``top`` <= 32 most
     likely tokens (b200p_token_logprobs).  ``logits`` [M, V] float32, float16 or bfloat16, a slice of columns or a row stride are fine."""
     dev = logits.get_device()
     if dev < 0 or dev != _device_index() or (tokens is not None and tokens.get_device() != dev):

@@ -215,3 +215,17 @@ def test_refusals():
     for bad in (full._replace(logprob=None), full._replace(entropy=full.entropy[:3]), full._replace(top_ids=full.top_ids.long())):
         with pytest.raises(ValueError):
             ops.token_logprobs(x, t, top=2, out=bad)
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-20, 1e20, 1e27])
+@pytest.mark.parametrize("V", [10, 1000, 4097, 32001])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_the_ends_of_the_temperatures(dtype, V, temperature):
+    """What is masked by minus infinity weighs nothing at any temperature (by the type's lowest value what that leaves it), in rows that fill a thread's loads and
+    in rows that do not."""
+    for mask in (None, -math.inf, torch.finfo(DT[dtype]).min if temperature > 1 else None):      # (a lowest value over 1e-20 is no fp32 number)
+        x, t = make(6, V, dtype, seed=V)
+        if mask is not None:
+            x[:, 3:V - 4] = mask
+            t[0] = V // 2
+        check(x, t, min(5, V), temperature)

@@ -207,3 +207,9 @@ def test_wanted_positions_outside_their_entries_are_refused(want):
     for sink in (None, lambda *a: None):
         with pytest.raises(ValueError, match="wanted position"):
             SequenceModel._forward_ragged_locked(SimpleNamespace(device="cpu"), [[1, 2], []], [SimpleNamespace(batch_size=2)], None, want, sink)
+
+
+def test_token_logprobs_refuses_temperatures_at_which_masked_logits_would_weigh_something():
+    f = _lib.lib().b200p_token_logprobs
+    for T in (1.2e27, 1e28, 1e30, 3e38, 9e-31):
+        assert f(256, 256, 256, 256, 256, 256, 4, 100, 100, 2, T, _lib.F32, 0) == -1, T
