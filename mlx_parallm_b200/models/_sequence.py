@@ -1403,6 +1403,7 @@ class SequenceModel:
         B, L = inputs.shape
         host = inputs.tolist()
         n = prompt_counts(prompt_lengths, B, L)
+        ops.check_logprobs(top, self.lm_head.out_features, temperature)
         out = empty_logprobs((B, L), top, self.device)
         for t in out:
             t.zero_()

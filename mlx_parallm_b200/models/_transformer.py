@@ -681,6 +681,7 @@ class DecoderModel:
         time, never those of all.  ``cache``: the text goes on where its rows stand; ``adapters``: every row's (bind_adapters)."""
         if self.tp_world > 1:
             raise NotImplementedError("scoring needs the whole vocabulary on one rank")
+        ops.check_logprobs(top, (self.lm_head if self.lm_head is not None else self.model.embed_tokens).out_features, temperature)
         inputs = inputs if isinstance(inputs, torch.Tensor) else torch.as_tensor(inputs)
         with self._lock:
             ids = inputs.to(self.device).to(torch.int32).contiguous()

@@ -357,6 +357,14 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor                # float32 [M, top]
 
 
+def check_logprobs(top: int, V: int, temperature: float = 1.0) -> None:
+    """What token_logprobs takes, for callers that would otherwise learn it behind a forward pass."""
+    if not 0 <= top <= min(32, V):
+        raise ValueError(f"{top} alternatives of {V}: 32 at most")
+    if not 1e-30 <= temperature <= 1e27:
+        raise ValueError(f"temperature must be between 1e-30 and 1e27: got {temperature}")
+
+
 def token_logprobs(logits, tokens=None, top: int = 0, temperature: float = 1.0, out: Optional[TokenLogprobs] = None) -> TokenLogprobs:
     """Log probabilities of ``tokens`` (int32 [M]; negative: no token, 0) under softmax(logits / temperature), 1e-30 to 1e27, every row's entropy and its ``top`` <= 32 most
     likely tokens (b200p_token_logprobs).  ``logits`` [M, V] float32, float16 or bfloat16, a slice of columns or a row stride are fine."""

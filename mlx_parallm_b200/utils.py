@@ -355,8 +355,10 @@ def generate_step(
         cache = _kv_pool.get_for(model, B)                                                           # utils.py:390-394
     elif cache and cache[0]._lengths is None:
         bind_cache_group(cache, dev)
-    if logprobs is not None and getattr(model, "tp_world", 1) > 1:
-        raise NotImplementedError("logprobs needs the whole vocabulary on one rank")
+    if logprobs is not None:
+        if getattr(model, "tp_world", 1) > 1:
+            raise NotImplementedError("logprobs needs the whole vocabulary on one rank")
+        ops.check_logprobs(logprobs, (model.lm_head if model.lm_head is not None else model.model.embed_tokens).out_features)
     if adapters is not None:
         if not hasattr(model, "bind_adapters"):
             raise NotImplementedError("this model family takes no adapters")

@@ -99,6 +99,25 @@ def test_score_of_a_model_with_packed_prompts():
         assert (s.entropy[b, at:].cpu() - torch.special.entr(lp.exp()).sum(-1)).abs().max() < 5e-3
 
 
+def test_scores_that_are_refused_leave_the_cache_as_it_was():
+    import negosun_oracle as O
+    from mlx_parallm_b200.utils import _get_classes
+    cfg, om, gm = make_pair("tiny-llama", dtype="float16")
+    ocfg = O.make_config([O.layer(4, 2, 8, 12, 0.35, v_mix=False, q_temp=(0.4, 6), mlp=O.moe_mlp(6, 2, 16, (3, 2), shared=20))])
+    Model, Args = _get_classes(ocfg)
+    packed = Model(Args.from_dict(ocfg)).load_weights(O.random_weights(ocfg, 0), device="cuda", dtype=torch.float32)
+    for model, ids in ((gm, torch.from_numpy(prompts_for(cfg, 2, 9))), (packed, torch.randint(0, ocfg["vocab"], (2, 9)))):
+        cache = model.make_cache(2)
+        for kw in (dict(top=33), dict(top=-1), dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=1e30)):
+            with pytest.raises(ValueError):
+                model.score(ids, cache=cache, **kw)
+        for k in (33, -1):
+            with pytest.raises(ValueError):
+                next(generate_step(ids, model, cache=cache, logprobs=k))
+        assert all(c.offsets == [0, 0] for c in cache)
+        assert model.score(ids, cache=cache, top=1).top_ids.shape == (2, 9, 1) and cache[-1].offsets == [9, 9]
+
+
 @pytest.mark.parametrize("paged_cache", [False, True])
 @pytest.mark.parametrize("temp", [0.0, 0.8])
 def test_log_probabilities_of_generated_tokens(temp, paged_cache):
