@@ -492,7 +492,7 @@ class DecoderModel:
             for mine, c in zip(layers, cache):
                 mine.kpages, mine.vpages = c.kpages, c.vpages
             if bound is not None:
-                self.bind_adapters(layers, [bound[g[0]] for g in groups])
+                self.bind_adapters(layers, [bound[g[0]] if bound[g[0]] < self._adapters else -1 for g in groups])      # (an adapter that is gone is none)
             try:
                 logits = self(prompts, cache=layers, last_only=True)[:, -1, :]
                 book.adopt(side, groups, L)

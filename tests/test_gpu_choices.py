@@ -314,6 +314,23 @@ def test_greedy_generation_behind_a_shared_prompt(monkeypatch, groups_always):
             assert abs(float(la.logprob[r] - lb.logprob[r])) < 0.05
 
 
+def test_a_prompt_of_rows_whose_adapter_is_gone():
+    """Rows that were bound to an adapter that is no longer held have none, and share a prompt like any others."""
+    cfg, om, gm = make_pair("tiny-llama", dtype="float16")
+    ids = torch.from_numpy(prompts_for(cfg, 2, 20))
+    gm.apply_loras([adapters_for(cfg, 8, 1), adapters_for(cfg, 8, 2)], [1.0, 1.0])
+    cache = gm.make_paged_cache(4, 64, page=16)
+    gm.bind_adapters(cache, [1, 0, 1, 0])
+    gm.apply_loras([adapters_for(cfg, 8, 1)], [1.0])
+    got = gm.share_prompt(cache, ids, [[0, 2], [1, 3]])
+    plain = gm(ids, last_only=True)[:, -1]
+    assert torch.equal(got[0], plain[0]) and not torch.equal(got[1], plain[1])
+    gm.apply_loras([], [])
+    cache = gm.make_paged_cache(4, 64, page=16)
+    cache[0].adapter_rows, cache[0].adapter_index = [1, 0, 1, 0], torch.tensor([1, 0, 1, 0], dtype=torch.int32, device="cuda")
+    assert torch.equal(gm.share_prompt(cache, ids, [[0, 2], [1, 3]]), plain)
+
+
 def test_a_pool_that_is_too_small_for_a_shared_prompt():
     cfg, om, gm = make_pair("tiny-llama", dtype="float16")
     ids = torch.from_numpy(prompts_for(cfg, 1, 40))
