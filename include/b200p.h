@@ -688,7 +688,7 @@ size_t b200p_paged_attn_workspace_bytes_of(int64_t M, int H, int G, int D, int64
  * once per token.  A token whose own slot stands before the end of its group's shared slots reads what it sees by itself.  plan: b200p_row_groups of
  * `index` in tiles of b200p_paged_attn_shared_tile(H, G) rows.  Which pages the shared slots have is looked up in the table row of a member; that the others'
  * are the same is the caller's promise.  16-bit dtypes with D 64, 80, 96, 128 or 256 and up to 256 query heads per key head go by groups where the
- * table has room for shared keys and values that are worth it (32 MiB); other calls read every token's slots by themselves.
+ * table has room for shared keys and values that are worth it (64 MiB); other calls read every token's slots by themselves.
  * b200p_paged_attn_shared_set_path: 1 by groups wherever those types allow it, 2 never, 0 by the rule.  Workspace: b200p_paged_attn_shared_workspace_bytes, aligned to 256 bytes, no initial state, one stream at a time. */
 int b200p_paged_attn_shared(const void* q, const void* kpages, const void* vpages, const int32_t* table, const int32_t* t_row, const int32_t* t_slot,
                             void* out, const int32_t* index, const int32_t* prefix, const int32_t* plan, int64_t M, int H, int G, int D, int groups,

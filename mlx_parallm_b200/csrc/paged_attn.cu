@@ -1139,14 +1139,15 @@ static int launch_paged_type(const PagedAttn& a, cudaStream_t st) {
 
 // ---- behind shared slots ------------------------------------------------------------------------------------------------------
 // Which calls go by groups: those that the matrix instructions serve (fp32 and other sizes are bound by their FMAs, of which sharing saves none), and in
-// which the tokens' rows could have keys and values of 32 MiB in common.  Below, the third launch costs more than the reading: us by token / by group, 32 / 8
-// heads of 128, 4 rows behind 900 slots 10.8 / 12.5, 8 behind 1000 (26 MiB) 13.0 / 13.3, 16 behind 512 (30 MiB) 14.0 / 13.9, 8 behind 2000 16.9 / 15.4, 64 behind
-// 1000 47.9 / 30.0, 64 behind 4000 134 / 41.
+// which the tokens' rows could have keys and values of 64 MiB in common.  Below, the third launch costs more than the reading: us by token / by group, 32 / 8
+// heads of 128, 16 rows behind 512 slots (30 MiB) 13.9 / 14.6, 32 behind 256 (31 MiB) 14.2 / 18.8, 8 behind 2000 (54 MiB) 16.9 / 16.6, 2 behind 16000 (63 MiB)
+// 23.5 / 27.6, 64 behind 256 (63 MiB) 21.1 / 24.9, 4 behind 8000 (94 MiB) 23.4 / 22.8, 16 behind 2000 (116 MiB) 24.7 / 20.4, 64 behind 1000 48.1 / 31.3, 64
+// behind 4000 134 / 43.  (Only the table's room is known here: what rows do have in common is on the device.)
 static std::atomic<int> g_shared_path{0};                           // 1: by groups wherever it is served, 2: never
 static bool shared_served(int64_t M, int H, int G, int D, int64_t slots, int dtype) {
   const int path = g_shared_path.load(std::memory_order_relaxed);
   if (path == 2 || dtype == B200P_F32 || H / G > PS_ROWS || !(D == 64 || D == 80 || D == 96 || D == 128 || D == 256)) return false;
-  return path == 1 || (M - 1) * slots * G * D * 4 >= 32ll << 20;
+  return path == 1 || (M - 1) * slots * G * D * 4 >= 64ll << 20;
 }
 static int shared_tile(int H, int G) { return H / G < PS_ROWS ? PS_ROWS / (H / G) : 1; }
 static size_t whole_bytes(int64_t M, int H, int D) { return round256((size_t)M * H * (D + 4) * 4); }

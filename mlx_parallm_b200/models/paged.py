@@ -26,8 +26,8 @@ from .base import RowState
 
 
 # Keys and values of shared pages that a layer's decode step need not read again, from which on it goes by groups (us a layer by token / by group, 32 / 8 heads of
-# 128 in 16 bits: 32 rows behind 256 tokens, 31 MiB, 14.1 / 18.3; 64 behind 256, 63 MiB, 21.2 / 24.0; 8 behind 2000, 54 MiB, 16.9 / 15.4; 4 behind 8000, 94 MiB,
-# 23.4 / 21.1; 64 behind 1000, 236 MiB, 47.9 / 30.0)
+# 128 in 16 bits: 32 rows behind 256 tokens, 31 MiB, 14.2 / 18.8; 8 behind 2000, 54 MiB, 16.9 / 16.6; 64 behind 256, 63 MiB, 21.1 / 24.9; 4 behind 8000, 94 MiB,
+# 23.4 / 22.8; 64 behind 1000, 236 MiB, 48.1 / 31.3)
 SHARED_BYTES = 64 << 20
 OBSERVED_BYTES = 256 << 20        # workspace of a call that adds up the weights of a prompt's last tokens (one token per row at least)
 

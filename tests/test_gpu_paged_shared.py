@@ -383,3 +383,15 @@ def test_parts_stay_in_the_workspace(H, G, D, dtype):
     behind = ws[n:].clone()
     c.check(ws=ws[:n])
     assert torch.equal(ws[n:], behind)
+
+
+def test_few_shared_slots_are_read_by_every_token():
+    """Where the table has no room for 64 MiB in common (here 63 and 47 MiB) a call is paged_attn's, bit by bit."""
+    _lib.lib().b200p_paged_attn_shared_set_path(0)
+    for B, prefix, tail in ((2, 16000, 40), (20, 512, 50)):
+        c = Case([0] * B, [prefix], [prefix + 1 + i * tail // B for i in range(B)], page=64, poison=False)
+        room = (B - 1) * c.table.shape[1] * 64 * 8 * 128 * 4
+        assert 32 << 20 <= room < 64 << 20
+        n = ops.paged_attn_workspace_bytes(B, 32, 128, 0, 8)
+        alone = ops.paged_attn(c.q, c.k, c.v, c.table, c.row, c.slot, torch.empty_like(c.q), c.scale, workspace=torch.empty((n,), dtype=torch.uint8, device="cuda"))
+        assert torch.equal(c.run(), alone)
