@@ -5,8 +5,9 @@
 // The rows are put in the order of their adapters once per batch (row_groups_kernel); the layers then go by tiles of 16 or 128 rows of one adapter.
 // A cluster of CTAs has a tile: every CTA takes a part of K for z = x A^T, the parts meet through distributed shared memory, and every CTA has all of
 // z for its part of the columns.  So both products are one launch, an adapter is read once for a tile, and even a single row has eight SMs.
-// z is fp32; for the second product its rows are scaled by a power of two and split into two f16 or three bf16 numbers, which carry 22 and 24 of its bits,
-// so that the update is as exact as its sums; it is added to y in fp32 and rounded once where y is 16-bit.
+// z is fp32; for the second product its rows are scaled by a power of two and split into 16-bit numbers: two of f16, which carry 22 bits of a z that is not below
+// 2^-17 of its row's largest (2^-39 of that below), or three of bf16, 24 bits of any, two and 16 where y is bf16 itself.  So the update is as exact as its sums
+// (for bf16 y as y's rounding asks for); it is added to y in fp32 and rounded once where y is 16-bit.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -112,11 +113,14 @@ __host__ __device__ constexpr int lw_row_floats(int ranks) {
   return split > LW_WARPS * 32 ? split : LW_WARPS * 32;
 }
 
-// up = 2^e, down = 2^-e with top * down in [1, 2); 1 for a row of zeros or one that is not finite
+// up = 2^e, down = 2^-e with top * down in [1, 2), for f16 in [2^14, 2^15): what is much smaller than the row's largest keeps its bits too, above the smallest
+// numbers of f16.  1 for a row of zeros or one that is not finite.
+template <typename T>
 __device__ __forceinline__ void lw_scale(float top, float& up, float& down) {
+  constexpr uint32_t LIFT = std::is_same<T, __half>::value ? 14 : 0;
   const uint32_t e = __float_as_uint(top) >> 23;
-  const bool plain = e < 1 || e > 252;
-  down = plain ? 1.f : __uint_as_float((254u - e) << 23), up = plain ? 1.f : __uint_as_float(e << 23);
+  const bool plain = e < LIFT + 1 || e > 252;
+  down = plain ? 1.f : __uint_as_float((254u + LIFT - e) << 23), up = plain ? 1.f : __uint_as_float((e - LIFT) << 23);
 }
 
 __device__ __forceinline__ void red_add4(float* p, float a, float b, float c, float d) {
@@ -273,7 +277,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
     for (int k = 0; k < NZ; ++k) top = fmaxf(top, fabsf(z[k]));
     top = warp_max(top);
     float up, down;
-    lw_scale(top, up, down);
+    lw_scale<T>(top, up, down);
     if (lane == 0) s_factor[row][target] = up * p.scales[tile.x];
 #pragma unroll
     for (int k = 0; k < NZ; ++k) {
@@ -536,7 +540,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
       float top = fmaxf(fmaxf(fabsf(z.x), fabsf(z.y)), fmaxf(fabsf(z.z), fabsf(z.w))), up, down;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-      lw_scale(top, up, down);
+      lw_scale<T>(top, up, down);
       z.x *= down, z.y *= down, z.z *= down, z.w *= down;
       auto rest = [](float x) { return x - Tr<T>::to_f(Tr<T>::from_f(x)); };
       const uint2 high = make_uint2(pack2<T>(z.x, z.y), pack2<T>(z.z, z.w)), low = make_uint2(pack2<T>(rest(z.x), rest(z.y)), pack2<T>(rest(z.z), rest(z.w)));

@@ -326,3 +326,35 @@ def test_prompt_tiles_of_y_at_odd_places(shift, gap):
 @pytest.mark.parametrize("R,targets", [(16, 2), (64, 3)])
 def test_prompt_tiles_of_clusters_of_every_size(M, n, R, targets):
     check(index_of(M, n, seed=M), *make(M, n, 520, R, (136, 264, 8)[:targets], "f16", out="16", seed=n), 128)
+
+
+@pytest.mark.parametrize("out", ["f32", "16"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("R", [16, 64])
+@pytest.mark.parametrize("tile,M", [(16, 40), (128, 200)])
+def test_a_small_z_beside_a_large_one_keeps_its_bits(tile, M, R, dtype, out):
+    """z is one exact product here, from 60 in the first rank, which b leaves out, down to 6e-6 in the others.  Two f16 numbers are off by 2^-22 of z or 2^-39 of
+    the row's largest, three bf16 ones by 2^-24, two (where y is bf16) by 2^-16; the second product adds 3 R / 16 sums in fp32, and y is rounded once."""
+    g = torch.Generator(device="cuda").manual_seed(R + M)
+    rand = lambda *s: torch.rand(s, generator=g, device="cuda")
+    K, N, dt = 64, 128, DT[dtype]
+    x = (60 * 10 ** (-7 * rand(M, K))).to(dt)
+    x[:, 0] = 60
+    a = torch.zeros((2, 1, R, K), dtype=dt, device="cuda")
+    a[:, 0, torch.arange(R), torch.arange(R)] = (1 + rand(2, R)).to(dt)
+    for keep in (1, R // 2, R - 1):                                  # ranks that b looks at: small ones by themselves
+        b = (torch.randn((2, N, R), generator=g, device="cuda")).to(dt)
+        b[:, :, :R - keep] = 0
+        index = (torch.arange(M, dtype=torch.int32) % 2).cuda()
+        scales, columns = torch.ones(2, device="cuda"), ((0, N),)
+        y = torch.zeros((M, N), dtype=torch.float32 if out == "f32" else dt, device="cuda")
+        ops.lora_rows(x, ops.row_groups(index, 2, tile), a, b, scales, columns, y)
+        z = x.double()[:, :R] * a[:, 0].double().diagonal(dim1=1, dim2=2)[index.long()]
+        B = b.double()[index.long()]
+        want = torch.einsum("mr,mnr->mn", z, B)
+        part = 2.0 ** -22 * z.abs() + 2.0 ** -39 * z.abs().amax(-1, keepdim=True) if dtype == "f16" else 2.0 ** (-24 if out == "f32" else -16) * z.abs()
+        slack = torch.einsum("mr,mnr->mn", part + (3 * R / 16 + 4) * 2.0 ** -23 * z.abs(), B.abs())
+        eps = torch.finfo(y.dtype)
+        slack += want.abs() * eps.eps / 2 + (0.0 if out == "f32" else eps.tiny * eps.eps / 2)      # (half of a smallest number)
+        diff = (y.double() - want).abs()
+        assert diff.le(slack).all(), (keep, float((diff / want.abs().clamp(min=1e-30)).max()))
