@@ -23,7 +23,7 @@ namespace b200p {
 int sm_count();
 
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
-constexpr int LP_TOP = 32;             // alternatives at most: a group of threads each, and a rank that a warp can hold
+constexpr int LP_TOP = 32;             // alternatives at most: half of the groups, so that their k-th largest maximum is a bound
 constexpr int LP_CLUSTER = 8;
 constexpr int LP_GROUPS = 64;
 static_assert(LP_WARPS * LP_CLUSTER == LP_GROUPS, "a warp is a group in the largest cluster");
@@ -116,8 +116,7 @@ struct LpSums {
 };
 
 struct LpShared {
-  float4 part[LP_WARPS > LP_CLUSTER ? LP_WARPS : LP_CLUSTER];      // m, s, t of the warps, then (in the first CTA) of the cluster's CTAs
-  float4 cta[LP_CLUSTER];
+  float4 part[LP_WARPS], cta[LP_CLUSTER];      // m, s, t of the warps, and (in the first CTA) of the cluster's CTAs
   alignas(16) float group[LP_GROUPS];
   float bound, m, log_s;
   int count;

@@ -12,9 +12,9 @@
 
 #include <atomic>
 
+#include "attn_tc.cuh"
 #include "mma_util.cuh"
 #include "rowgroups.cuh"
-#include "tc_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -151,14 +151,14 @@ __device__ __forceinline__ void lw_load(const LoraRows& p, const T* b, int run, 
       w[k][h] = n0 + 2 * h < r.width && 16 * k < p.R ? *reinterpret_cast<const uint2*>(at + 2 * h * p.R + 16 * k) : make_uint2(0, 0);
 }
 
-// Tiles of 16 rows: decode batches, bound by memory where adapters are many (64 rows of 64 adapters of rank 16, 4096 to 5120: 12.3 us for 29 MB, a floor of 4.6)
-// and by the chain of two products, the parts' meeting and two round trips where they are few (1 row 6.9 us).  Four steps of K and eight runs of 16 columns
-// are under way (two and four: 14.1 us for the 64, 6.8 for the one).  YT: y's type; KS: 16 ranks each (R or more).  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits
+// Tiles of 16 rows: decode batches, bound by memory where adapters are many (64 rows of 64 adapters of rank 16, 4096 to 5120: 12.5 us
+// for 29 MB, three sets of them in turn, 11.8 with one that stays in L2; a floor of 4.6) and by the chain of two products, the parts' meeting and two round trips
+// where they are few (1 row 7.6 us).  Four steps of K and eight runs of 16 columns are under way (two and four: 14.1 us for the 64).  YT: y's type; KS: 16 ranks each (R or more).  Eight warps: 32 ranks each (of all targets) side by side, the rest of the warps splits
 // this CTA's part of K.  Operands come straight from memory, 16 bytes a lane: the order of k within a product is free as long as both operands have the same.
 template <typename T, typename YT, int KS>
 __global__ void __launch_bounds__(LW_THREADS, 2)
 lora_rows_kernel(const __grid_constant__ LoraRows p) {
-  constexpr int MB = 1, ROWS = 16, PARTS = LwParts<T, YT>::N, NZ = (16 * KS + 31) / 32;
+  constexpr int ROWS = 16, PARTS = LwParts<T, YT>::N, NZ = (16 * KS + 31) / 32;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int s_row[ROWS];
   __shared__ float s_factor[ROWS][LW_TARGETS];
@@ -179,21 +179,17 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
   __syncthreads();
 
   // ---- this CTA's part of z ---------------------------------------------------------------------------------------------------
-  float acc[MB][4][4];
+  float acc[4][4];
 #pragma unroll
-  for (int i = 0; i < MB; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+  for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
   const int my_n = warp % wn * 32, my_k = warp / wn;
   if (my_n < TR) {
-    const T* xr[MB][2];
+    const T* xr[2];
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = s_row[16 * i + 8 * h + g];
-        xr[i][h] = row < 0 ? nullptr : reinterpret_cast<const T*>(p.x) + (int64_t)row * p.ldx + 8 * t;
-      }
+    for (int h = 0; h < 2; ++h) {
+      const int row = s_row[8 * h + g];
+      xr[h] = row < 0 ? nullptr : reinterpret_cast<const T*>(p.x) + (int64_t)row * p.ldx + 8 * t;
+    }
     const T* ar[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -205,7 +201,7 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
     constexpr int DEEP = 4;                         // steps whose loads are under way together
 #pragma unroll 1
     for (int s = s0 + my_k; s < s1; s += DEEP * wk) {
-      uint4 av[DEEP][4], xv[DEEP][MB][2];
+      uint4 av[DEEP][4], xv[DEEP][2];
 #pragma unroll
       for (int u = 0; u < DEEP; ++u) {
         const int k = (s + u * wk) * 32;
@@ -213,22 +209,18 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) av[u][j] = in && ar[j] ? *reinterpret_cast<const uint4*>(ar[j] + k) : zero;
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) xv[u][i][h] = in && xr[i][h] ? *reinterpret_cast<const uint4*>(xr[i][h] + k) : zero;
+        for (int h = 0; h < 2; ++h) xv[u][h] = in && xr[h] ? *reinterpret_cast<const uint4*>(xr[h] + k) : zero;
       }
 #pragma unroll
-      for (int u = 0; u < DEEP; ++u)
+      for (int u = 0; u < DEEP; ++u) {
+        const uint32_t lo[4] = {xv[u][0].x, xv[u][1].x, xv[u][0].y, xv[u][1].y};
+        const uint32_t hi[4] = {xv[u][0].z, xv[u][1].z, xv[u][0].w, xv[u][1].w};
 #pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          const uint32_t lo[4] = {xv[u][i][0].x, xv[u][i][1].x, xv[u][i][0].y, xv[u][i][1].y};
-          const uint32_t hi[4] = {xv[u][i][0].z, xv[u][i][1].z, xv[u][i][0].w, xv[u][i][1].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mma16816<T>(acc[i][j], lo, av[u][j].x, av[u][j].y);
-            mma16816<T>(acc[i][j], hi, av[u][j].z, av[u][j].w);
-          }
+        for (int j = 0; j < 4; ++j) {
+          mma16816<T>(acc[j], lo, av[u][j].x, av[u][j].y);
+          mma16816<T>(acc[j], hi, av[u][j].z, av[u][j].w);
         }
+      }
     }
   }
   constexpr int AHEAD = 8 / KS;                      // runs whose b is under way
@@ -238,12 +230,10 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
   {
     float* part = s_part + my_k * ROWS * ranks + my_n;
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        *reinterpret_cast<float2*>(part + (16 * i + g) * ranks + 8 * j + 2 * t) = make_float2(acc[i][j][0], acc[i][j][1]);
-        *reinterpret_cast<float2*>(part + (16 * i + 8 + g) * ranks + 8 * j + 2 * t) = make_float2(acc[i][j][2], acc[i][j][3]);
-      }
+    for (int j = 0; j < 4; ++j) {
+      *reinterpret_cast<float2*>(part + g * ranks + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+      *reinterpret_cast<float2*>(part + (8 + g) * ranks + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < tile.z * ranks; i += LW_THREADS) {
@@ -310,52 +300,44 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
       const LwRun r(p, run);
       const bool in = r.c0 + 4 * t < r.width;
       const int64_t col = p.col0[r.target] + r.c0 + 4 * t;
-      uint2 old[MB][2];                                           // 16-bit y, on its way beside the products (fp32 is added in memory)
+      uint2 old[2];                                               // 16-bit y, on its way beside the products (fp32 is added in memory)
       if constexpr (sizeof(YT) == 2) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int row = s_row[16 * i + 8 * h + g];
-            old[i][h] = row >= 0 && in ? *reinterpret_cast<const uint2*>(reinterpret_cast<const YT*>(p.y) + (int64_t)row * p.ldy + col) : make_uint2(0, 0);
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int row = s_row[8 * h + g];
+          old[h] = row >= 0 && in ? *reinterpret_cast<const uint2*>(reinterpret_cast<const YT*>(p.y) + (int64_t)row * p.ldy + col) : make_uint2(0, 0);
+        }
       }
-      float d[MB][2][4];
+      float d[2][4];
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) d[i][h][0] = d[i][h][1] = d[i][h][2] = d[i][h][3] = 0.f;
+      for (int h = 0; h < 2; ++h) d[h][0] = d[h][1] = d[h][2] = d[h][3] = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         if (16 * k >= p.R) break;
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) {
-            const T* z = s_split + (part * ROWS + 16 * i + g) * ld + r.target * p.R + 16 * k + 4 * t;
-            const uint2 lo = *reinterpret_cast<const uint2*>(z), hi = *reinterpret_cast<const uint2*>(z + 8 * ld);
-            const uint32_t f[4] = {lo.x, hi.x, lo.y, hi.y};
-            mma16816<T>(d[i][0], f, w[u][k][0].x, w[u][k][0].y);
-            mma16816<T>(d[i][1], f, w[u][k][1].x, w[u][k][1].y);
-          }
+        for (int part = 0; part < PARTS; ++part) {
+          const T* z = s_split + (part * ROWS + g) * ld + r.target * p.R + 16 * k + 4 * t;
+          const uint2 lo = *reinterpret_cast<const uint2*>(z), hi = *reinterpret_cast<const uint2*>(z + 8 * ld);
+          const uint32_t f[4] = {lo.x, hi.x, lo.y, hi.y};
+          mma16816<T>(d[0], f, w[u][k][0].x, w[u][k][0].y);
+          mma16816<T>(d[1], f, w[u][k][1].x, w[u][k][1].y);
+        }
       }
       lw_load<T, KS>(p, b, run + AHEAD * LW_WARPS, run1, w[u]);
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = 16 * i + 8 * h + g, row = s_row[at];
-          if (row < 0 || !in) continue;
-          const float f = s_factor[at][r.target];
-          YT* y = reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + col;
-          if constexpr (sizeof(YT) == 4) {
-            red_add4(y, f * d[i][0][2 * h], f * d[i][0][2 * h + 1], f * d[i][1][2 * h], f * d[i][1][2 * h + 1]);
-          } else {
-            const YT* e = reinterpret_cast<const YT*>(&old[i][h]);
-            *reinterpret_cast<uint2*>(y) = make_uint2(pack2<YT>(fmaf(f, d[i][0][2 * h], Tr<YT>::to_f(e[0])), fmaf(f, d[i][0][2 * h + 1], Tr<YT>::to_f(e[1]))),
-                                                      pack2<YT>(fmaf(f, d[i][1][2 * h], Tr<YT>::to_f(e[2])), fmaf(f, d[i][1][2 * h + 1], Tr<YT>::to_f(e[3]))));
-          }
+      for (int h = 0; h < 2; ++h) {
+        const int at = 8 * h + g, row = s_row[at];
+        if (row < 0 || !in) continue;
+        const float f = s_factor[at][r.target];
+        YT* y = reinterpret_cast<YT*>(p.y) + (int64_t)row * p.ldy + col;
+        if constexpr (sizeof(YT) == 4) {
+          red_add4(y, f * d[0][2 * h], f * d[0][2 * h + 1], f * d[1][2 * h], f * d[1][2 * h + 1]);
+        } else {
+          const YT* e = reinterpret_cast<const YT*>(&old[h]);
+          *reinterpret_cast<uint2*>(y) = make_uint2(pack2<YT>(fmaf(f, d[0][2 * h], Tr<YT>::to_f(e[0])), fmaf(f, d[0][2 * h + 1], Tr<YT>::to_f(e[1]))),
+                                                    pack2<YT>(fmaf(f, d[1][2 * h], Tr<YT>::to_f(e[2])), fmaf(f, d[1][2 * h + 1], Tr<YT>::to_f(e[3]))));
         }
+      }
     }
   }
   if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // nobody leaves before all have read
@@ -365,16 +347,16 @@ lora_rows_kernel(const __grid_constant__ LoraRows p) {
 // 16-byte copies into tiles of 64 of K, z = x A^T grows in TMEM, meets the other CTAs' and becomes the operand of the second product, whose blocks of 64 or
 // 128 columns take b along with the old y; y grows in its place in shared memory and leaves by whole lines while the next block's product runs.
 // RK: ranks of all targets, filled up to 32, 64, 128 or 256.  8000 rows of rank 64, 4096 to 5120: 56 us of 31.
-constexpr int LP_ROWS = 128, LP_TARGETS = 3, LP_CLUSTER = 8, LP_THREADS = LW_THREADS + 128;
+constexpr int LT_ROWS = 128, LT_TARGETS = 3, LT_CLUSTER = 8, LT_THREADS = LW_THREADS + 128;
 template <int RK, int COLS>
-struct LpShape {
+struct LtShape {
   static constexpr int STAGES_B = COLS == 128 ? 3 : 4, STAGES_Y = COLS == 128 ? 3 : 5;
-  static constexpr int STAGE_A = (LP_ROWS + RK) * 128, STAGES_A = RK == 256 ? 4 : 6, TMEM = RK == 256 || COLS == 128 ? 256 : 128;
-  static constexpr int B_BYTES = COLS * 128, Y_PITCH = COLS * 2 + 16, Y_BYTES = LP_ROWS * Y_PITCH;
-  static constexpr int Z_TILE = LP_ROWS * 128;                    // of one part of a target's z: 64 ranks a line
+  static constexpr int STAGE_A = (LT_ROWS + RK) * 128, STAGES_A = RK == 256 ? 4 : 6, TMEM = RK == 256 || COLS == 128 ? 256 : 128;
+  static constexpr int B_BYTES = COLS * 128, Y_PITCH = COLS * 2 + 16, Y_BYTES = LT_ROWS * Y_PITCH;
+  static constexpr int Z_TILE = LT_ROWS * 128;                    // of one part of a target's z: 64 ranks a line
   static __host__ __device__ constexpr int z_pitch(int TR) { return TR + 4; }      // floats; a row per thread without conflicts
   static __host__ __device__ constexpr int front(int TR) {
-    const int z = LP_ROWS * z_pitch(TR) * 4, c = STAGES_B * B_BYTES + STAGES_Y * Y_BYTES;
+    const int z = LT_ROWS * z_pitch(TR) * 4, c = STAGES_B * B_BYTES + STAGES_Y * Y_BYTES;
     return ((z > c ? z : c) + 1023) / 1024 * 1024;
   }
   static __host__ __device__ constexpr int bytes(int TR, int targets) {
@@ -384,29 +366,7 @@ struct LpShape {
   static_assert(B_BYTES % 1024 == 0 && STAGE_A % 1024 == 0, "tiles at whole swizzles");
 };
 
-__device__ __forceinline__ void lp_copy(uint32_t dst, const void* src, bool valid) { cp_async16(dst, src, valid); }
-__device__ __forceinline__ void lp_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-__device__ __forceinline__ void lp_tmem_ld32(uint32_t taddr, float* v) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
-      "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-
-struct LpBarriers {
+struct LtBarriers {
   uint64_t step[6], block[2], read[2];                            // a stage's products, a block's; its results are read
   uint32_t tmem;
   volatile int abort;
@@ -415,16 +375,16 @@ struct LpBarriers {
 // A wait that gives up is reported and everything goes on (the other waits then give up at once): the threads keep meeting at the CTA's and the cluster's
 // barriers, and only the numbers are wrong.
 template <typename T, int RK, int COLS>
-__global__ void __launch_bounds__(LP_THREADS, 1)
+__global__ void __launch_bounds__(LT_THREADS, 1)
 lora_prompt_kernel(const __grid_constant__ LoraRows p) {
-  using S = LpShape<RK, COLS>;
+  using S = LtShape<RK, COLS>;
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);      // D fp32, 128 rows, K-major operands; N below
   constexpr uint32_t idesc_z = idesc | ((uint32_t)(RK >> 3) << 17), idesc_y = idesc | ((uint32_t)(COLS >> 3) << 17);
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int s_row[LP_ROWS];
-  __shared__ float s_factor[LP_TARGETS][LP_ROWS];
-  __shared__ LpBarriers s_bar;
+  __shared__ int s_row[LT_ROWS];
+  __shared__ float s_factor[LT_TARGETS][LT_ROWS];
+  __shared__ LtBarriers s_bar;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), C = (int)cluster.num_blocks();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -437,7 +397,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   const int tile_index = blockIdx.x / C, tiles = p.plan.tiles();
   const int4 tile = p.plan.tile(tile_index);                      // (the plan has room for every tile of the grid)
   if (tile_index >= tiles) return;                                // (the whole cluster)
-  if ((int)threadIdx.x < LP_ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
+  if ((int)threadIdx.x < LT_ROWS) s_row[threadIdx.x] = (int)threadIdx.x < tile.z ? p.plan.order()[tile.y + threadIdx.x] : -1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 6; ++i) mbar_init(smem_u32(&s_bar.step[i]), 1);
     for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&s_bar.block[i]), 1); mbar_init(smem_u32(&s_bar.read[i]), LW_WARPS); }
@@ -471,12 +431,12 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bool ok = in && xr[i];
-          lp_copy(at + (line + 32 * i) * 128, ok ? xr[i] + s * 64 : reinterpret_cast<const T*>(p.x), ok);
+          cp_async16(at + (line + 32 * i) * 128, ok ? xr[i] + s * 64 : reinterpret_cast<const T*>(p.x), ok);
         }
 #pragma unroll
         for (int i = 0; i < RK / 32; ++i) {
           const bool ok = in && line + 32 * i < TR;
-          lp_copy(at + (LP_ROWS + line + 32 * i) * 128, ok ? ar + (int64_t)32 * i * p.K + s * 64 : reinterpret_cast<const T*>(p.a), ok);
+          cp_async16(at + (LT_ROWS + line + 32 * i) * 128, ok ? ar + (int64_t)32 * i * p.K + s * 64 : reinterpret_cast<const T*>(p.a), ok);
         }
       }
       cp_async_commit();
@@ -490,9 +450,9 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
       __syncthreads();
       if (warp == LW_WARPS && elect_one()) {
         const uint32_t xs = s0 + (uint32_t)(n % S::STAGES_A) * S::STAGE_A;
-        const uint64_t ad = make_desc_sw128(xs), bd = make_desc_sw128(xs + LP_ROWS * 128);
+        const uint64_t ad = make_desc_sw128(xs), bd = make_desc_sw128(xs + LT_ROWS * 128);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) lp_mma(tmem, ad + 2 * k, bd + 2 * k, idesc_z, n || k ? 1u : 0u);
+        for (int k = 0; k < 4; ++k) ft_mma_ss(tmem, ad + 2 * k, bd + 2 * k, idesc_z, n || k ? 1u : 0u);
         umma_commit(smem_u32(&s_bar.step[n % S::STAGES_A]));
       }
       __syncwarp();
@@ -508,7 +468,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
     for (int r = 32 * (warp >> 2); copies && r < TR; r += 64) {
       float z[32];
       if (k1 > k0) {
-        lp_tmem_ld32(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + r, z);
+        tmem_ld32(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + r, z);
         tmem_ld_wait();
       } else {
 #pragma unroll
@@ -527,7 +487,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   // all rows: every CTA would read the z of eight, 512 KB.) --------------------------------------------------------------------------
   auto meet = [&](auto most) {                                    // of up to `most` CTAs
     constexpr int CTAS = decltype(most)::value;
-    const int l = threadIdx.x & 15, k = 4 * l, rows = LP_ROWS / C;
+    const int l = threadIdx.x & 15, k = 4 * l, rows = LT_ROWS / C;
 #pragma unroll(CTAS > 4 ? 2 : 4)
     for (int i = threadIdx.x >> 4; i < rows * p.targets; i += LW_THREADS / 16) {
       const int target = i / rows, row = rank * rows + i - target * rows, at = row * zp + target * p.R + k;
@@ -558,7 +518,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   if (warp < LW_WARPS) {
     if (C == 1) meet(std::integral_constant<int, 1>());
     else if (C <= 4) meet(std::integral_constant<int, 4>());
-    else meet(std::integral_constant<int, LP_CLUSTER>());
+    else meet(std::integral_constant<int, LT_CLUSTER>());
   }
   fence_proxy_async_smem();
   if (C > 1) cluster.sync();                                      // all have read and written: the stages may lie there again
@@ -600,7 +560,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
 #pragma unroll
         for (int k = 0; k < BP; ++k) {
           const int x = (int)threadIdx.x - LW_THREADS + 128 * k;
-          if (x < pieces) lp_copy(bs + to[k], from + (x < some ? 8 * x : 0), x < some);
+          if (x < pieces) cp_async16(bs + to[k], from + (x < some ? 8 * x : 0), x < some);
         }
         step(ahead);
       }
@@ -622,7 +582,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
             const uint64_t ad = make_desc_sw128(zop + (uint32_t)(part * p.targets + here.target) * S::Z_TILE);
 #pragma unroll
             for (int k = 0; k < LW_RANK / 16; ++k)
-              if (16 * k < p.R) lp_mma(tmem + COLS * (n & 1), ad + 2 * k, bd + 2 * k, idesc_y, part || k ? 1u : 0u);
+              if (16 * k < p.R) ft_mma_ss(tmem + COLS * (n & 1), ad + 2 * k, bd + 2 * k, idesc_y, part || k ? 1u : 0u);
           }
           umma_commit(smem_u32(&s_bar.block[n & 1]));
         }
@@ -651,7 +611,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
 #pragma unroll
         for (int k = 0; k < CL; ++k) {
           const bool ok = in && y_row[k];
-          lp_copy(y0 + stage * S::Y_BYTES + at + RL * k * S::Y_PITCH, ok ? y_row[k] + col : reinterpret_cast<const T*>(p.y), ok);
+          cp_async16(y0 + stage * S::Y_BYTES + at + RL * k * S::Y_PITCH, ok ? y_row[k] + col : reinterpret_cast<const T*>(p.y), ok);
         }
         step(ahead);
       }
@@ -666,7 +626,7 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
       tc_fence_after();
       float d[COLS / 2];
 #pragma unroll
-      for (int k = 0; k < COLS / 2; k += 32) lp_tmem_ld32(tmem + ((uint32_t)r0 << 16) + COLS * (n & 1) + c0 + k, d + k);
+      for (int k = 0; k < COLS / 2; k += 32) tmem_ld32(tmem + ((uint32_t)r0 << 16) + COLS * (n & 1) + c0 + k, d + k);
       cp_async_wait<S::STAGES_Y - 1>();
       tmem_ld_wait();
       tc_fence_before();
@@ -707,8 +667,8 @@ lora_prompt_kernel(const __grid_constant__ LoraRows p) {
   }
 }
 
-// Clusters of up to C CTAs, as many as fit the GPU.  (us, 64 rows of 64 adapters in clusters of 1 / 2 / 4 / 8: 20.6 / 13.6 / 11.6 / 17.2; 1 row 19.8 / 12.6 / 8.7 /
-// 7.0.)
+// Clusters of up to C CTAs, as many as fit the GPU.  (us, 64 rows of 64 adapters in clusters of 1 / 2 / 4 / 8: 31.1 / 18.4 / 12.5 / 19.3, three sets of adapters in turn;
+// 1 row 20.9 / 13.6 / 9.3 / 7.6.)
 static int launch_lora(void (*kern)(LoraRows), int threads, int most_bytes, int bytes, int C, int per_sm, std::atomic<uint64_t>& ready, const LoraRows& p, int64_t tiles,
                        cudaStream_t st) {
   int dev = 0;
@@ -749,10 +709,10 @@ static int launch_lora_rows(const LoraRows& p, int64_t tiles, cudaStream_t st) {
 template <typename T, int RK, int COLS>
 static int launch_lora_prompt_of(LoraRows p, int64_t tiles, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
-  using S = LpShape<RK, COLS>;
-  constexpr int TARGETS = COLS == 128 ? 2 : LP_TARGETS, MOST = RK < LW_RANK * TARGETS ? RK : LW_RANK * TARGETS;
+  using S = LtShape<RK, COLS>;
+  constexpr int TARGETS = COLS == 128 ? 2 : LT_TARGETS, MOST = RK < LW_RANK * TARGETS ? RK : LW_RANK * TARGETS;
   static_assert(S::bytes(MOST, TARGETS) <= 224 * 1024, "beside the static shared memory");
-  return launch_lora(lora_prompt_kernel<T, RK, COLS>, LP_THREADS, S::bytes(MOST, TARGETS), S::bytes(p.targets * p.R, p.targets), LP_CLUSTER, 1, ready, p, tiles, st);
+  return launch_lora(lora_prompt_kernel<T, RK, COLS>, LT_THREADS, S::bytes(MOST, TARGETS), S::bytes(p.targets * p.R, p.targets), LT_CLUSTER, 1, ready, p, tiles, st);
 }
 // Blocks of 128 columns, whose products take the tensor core as long as those of 64 do; of 64 where three targets' z take their room.
 template <typename T, int RK>
@@ -770,7 +730,7 @@ static int launch_lora_tiles(LoraRows p, int tile, int64_t tiles, cudaStream_t s
   if constexpr (sizeof(YT) == 2) {
     bool whole = aligned(p.y, 16) && p.ldy % 8 == 0;                // y by 16 bytes
     for (int k = 0; k < p.targets; ++k) whole = whole && p.col0[k] % 8 == 0;
-    if (tile == LP_ROWS && p.targets <= LP_TARGETS && whole) {
+    if (tile == LT_ROWS && p.targets <= LT_TARGETS && whole) {
       if (TR > 128) return launch_lora_prompt<T, 256>(p, tiles, st);
       if (TR > 64) return launch_lora_prompt<T, 128>(p, tiles, st);
       if (TR > 32) return launch_lora_prompt<T, 64>(p, tiles, st);
@@ -814,7 +774,7 @@ extern "C" int b200p_row_groups(const int32_t* index, int32_t* plan, int64_t M, 
 // 16 / 128, 4096 to 5120 columns, ranks 16 and 64: 2 adapters, 500 rows 13.6 / 19.4 and 23.8 / 22.0, 1000 16.4 / 19.5 and 32.6 / 22.1, 1500 32.0 / 20.1 and
 // 60.7 / 23.2, 8000 116 / 53 and 234 / 56; 16 adapters, 500 rows 13.5 / 25.8 and 25.1 / 27.7, 1000 21.8 / 26.1 and 54.3 / 28.0; 64 adapters, 500 rows
 // 19.9 / 40.9 and 56.9 / 46.7, 1500 51 / 67 and 102 / 74, 8000 118 / 80 and 226 / 88.  (A plan is laid out once for layers of every rank.)
-extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1000 && M >= 16ll * groups ? LP_ROWS : 16; }
+extern "C" int b200p_lora_rows_tile(int64_t M, int groups) { return M >= 1000 && M >= 16ll * groups ? LT_ROWS : 16; }
 
 extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a, const void* b, const float* scales, void* y, const int32_t* host_columns,
                                int64_t M, int adapters, int tile, int targets, int R, int64_t K, int64_t ldx, int64_t ldy, int dtype, int y_f32,
@@ -822,7 +782,7 @@ extern "C" int b200p_lora_rows(const void* x, const int32_t* plan, const void* a
   PdlClass pdl_cls(64);
   B200P_REQUIRE(dtype == B200P_F16 || dtype == B200P_BF16, B200P_ERR_ARG, "adapters and their inputs are 16-bit");
   B200P_REQUIRE(M >= 0 && M <= RG_ROWS && adapters > 0 && adapters <= RG_GROUPS, B200P_ERR_ARG, "bad shape: %lld rows, %d adapters", (long long)M, adapters);
-  B200P_REQUIRE(tile == 16 || tile == LP_ROWS, B200P_ERR_ARG, "the plan's tiles have 16 or 128 rows, not %d", tile);
+  B200P_REQUIRE(tile == 16 || tile == LT_ROWS, B200P_ERR_ARG, "the plan's tiles have 16 or 128 rows, not %d", tile);
   B200P_REQUIRE(targets > 0 && targets <= LW_TARGETS, B200P_ERR_ARG, "%d targets: 1 to %d", targets, LW_TARGETS);
   B200P_REQUIRE(R > 0 && R % 16 == 0 && R <= LW_RANK, B200P_ERR_ARG, "rank %d: a multiple of 16, %d at most", R, LW_RANK);
   B200P_REQUIRE(K > 0 && K % 8 == 0 && K < (1ll << 24) && ldx >= K, B200P_ERR_ARG, "bad K %lld: a multiple of 8, not above ldx", (long long)K);

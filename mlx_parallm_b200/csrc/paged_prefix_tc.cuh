@@ -6,7 +6,7 @@
 // which leaves a part.  Products, softmax and roles are those of the prompt kernel, but the maximum may lag by 2^6 before outputs are rescaled (a part is few
 // steps, in most of which one of a warp's rows finds a new one: 114 -> 104 thousand cycles for 30 steps), and for f16 it is held 8 lower, so that weights reach
 // 2^14 and small ones keep their bits.  A weight is two 16-bit numbers, the rounded one and what it lost, which multiply the same values one after the other, so
-// that a token's output does not depend on whether its slots are shared: it carries its own rounding only.  (As one number, with the sum of the rounded ones,
+// that an output carries its own rounding only, as it does where nothing is shared.  (As one number, with the sum of the rounded ones,
 // the error was 1.3 times that, and 128 rows behind 16000 slots took 106.0 us instead of 119.6, 64 behind 4000 44.5 instead of 46.2.)
 //
 // The weights of a step's first 64 keys are multiplied while those of the last 64 are made (128 rows behind 16000 slots, one number a weight, 109.4 -> 106.1 us).
