@@ -345,7 +345,7 @@ def fine_slack(c, out):
     numbers, off by half a step of what the first lost, half * half, and in f16 by 2^-25 at least where the largest weight is 2^8 or more; products of 16 keys
     are added up in fp32, a unit of 2^-23 each; a score's sums as in Case.want; 2^x and the joins."""
     H, G, D, page, half = c.H, c.G, c.D, c.page, torch.finfo(c.q.dtype).eps / 2
-    tol = half * out.abs()
+    tol = half * out.abs() + torch.finfo(c.q.dtype).tiny * half      # (half a step of the type's smallest numbers)
     for t, (r, s) in enumerate(zip(c.row.tolist(), c.slot.tolist())):
         n = s + 1
         j = torch.arange(n, device="cuda")
